@@ -289,6 +289,76 @@ int nd_collective_neighborhood(const nd_graph* g, const int32_t* transits, int64
                                int32_t transits_per_sample, int32_t invalid, int32_t* sizes, int32_t* offsets,
                                int32_t* cols, float* weights, int64_t capacity, int32_t* row_offsets);
 
+/* ---- operators of models that train on samples ------------------------------------------ */
+/* No counterpart in the reference, which ends where a model begins.  Walks are sequences of
+ * different lengths over a vocabulary of |V| vertices; a training step attends over a packed batch
+ * of them, drops activations and takes the cross entropy over all vertices.  All arrays are DEVICE
+ * arrays of the current device; the work is enqueued on `stream` (a hipStream_t; NULL = the default
+ * stream) and not waited for; nothing is allocated, nothing is kept, and a call may be captured
+ * into a HIP graph.  Results do not depend on the order in which workgroups run. */
+enum { ND_F32 = 0, ND_F16 = 1, ND_BF16 = 2 };
+
+/* y_o = x_o / (1 - p) (+ residual_o) where slot o is kept, residual_o (or 0) where it is dropped; o
+ * counts the n elements of x.  Kept: nd_philox_fill_step's draw 0 of slot o at `step` (< 2^31) for
+ * step sizes over 1 is at least p.  The same call on the gradient of y gives the gradient of x.
+ * residual == NULL: none.  y may be x or residual.  p == 1 drops everything. */
+int nd_dropout(const void* d_x, const void* d_residual, void* d_y, int64_t n, int dtype, double p, uint64_t seed,
+               uint32_t step, void* stream);
+
+/* Packed sequences: sequence i is tokens starts[i] .. starts[i + 1] - 1 of n_tokens; starts[0] = 0, and tokens
+ * from starts[n_sequences] on belong to no sequence.  `starts` is the HOST array (n_sequences + 1
+ * entries), which is checked, d_starts the same on the device; the plan (nd_packed_plan_bytes(n_tokens)
+ * bytes, aligned to 16) is what every attention call over this batch reads. */
+#define ND_PACKED_MAX_TOKENS 2147483392
+#define ND_PACKED_MAX_DIM 128
+int64_t nd_packed_plan_bytes(int64_t n_tokens);
+int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
+                   void* stream);
+
+/* Causal attention within each sequence, heads / kv_heads query heads to a key head.  q, k, v and
+ * dout: [token][head][dim] with the strides given (in elements, multiples of 8, >= 0; dim elements
+ * lie side by side); out, dq: [n_tokens][heads][dim], dk, dv: [n_tokens][kv_heads][dim], lse and
+ * delta: [heads][n_tokens], all dense.  Arrays are aligned to 16 bytes, dim is a multiple of 8.
+ * Tokens of no sequence are not read; their rows of out and of the gradients are 0, their lse -inf.
+ * The backward call reads what the forward call left in out and lse; delta is working memory. */
+typedef struct nd_packed_attention {
+  int64_t n_tokens, n_covered; /* n_covered = starts[n_sequences] */
+  int32_t heads, kv_heads, dim, dtype;
+  float scale;
+  const void* plan;
+  const void *q, *k, *v, *dout;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, dout_token, dout_head;
+  void* out;
+  float *lse, *delta;
+  void *dq, *dk, *dv;
+} nd_packed_attention;
+int nd_packed_attention_forward(const nd_packed_attention* a, void* stream);
+int nd_packed_attention_backward(const nd_packed_attention* a, void* stream);
+
+/* Softmax cross entropy of `rows` vectors against `classes` class vectors, without the logits:
+ * loss_i = log sum_v exp(h_i . w_v) - h_i . w_{target_i}.  A target outside 0 .. classes - 1 (the
+ * samplers' INVALID is |V|) has loss 0 and sends nothing back.  hidden, dhidden: [rows][dim], weight,
+ * dweight: [classes][dim], dense, aligned to 16 bytes, dim a multiple of 8; lse: [rows], left by
+ * the forward call and read by the backward call; dloss: [rows], the gradient of each row's loss.
+ * workspace: nd_vocabulary_loss_workspace(...) bytes, aligned to 16, working memory of one call. */
+#define ND_VOCABULARY_MAX_ROWS 4194240
+#define ND_VOCABULARY_MAX_CLASSES 2147483392
+#define ND_VOCABULARY_MAX_DIM 65536
+typedef struct nd_vocabulary_loss {
+  int64_t rows, classes;
+  int32_t dim, dtype;
+  const void *hidden, *weight;
+  const int32_t* target;
+  float *loss, *lse;
+  const float* dloss;
+  void *dhidden, *dweight;
+  void* workspace;
+  int64_t workspace_bytes;
+} nd_vocabulary_loss;
+int64_t nd_vocabulary_loss_workspace(int64_t rows, int64_t classes, int32_t dim, int backward);
+int nd_vocabulary_loss_forward(const nd_vocabulary_loss* a, void* stream);
+int nd_vocabulary_loss_backward(const nd_vocabulary_loss* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

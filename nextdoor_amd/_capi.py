@@ -10,6 +10,25 @@ c_i32p = C.POINTER(C.c_int32)
 c_f32p = C.POINTER(C.c_float)
 c_i64p = C.POINTER(C.c_int64)
 
+
+
+class PackedAttention(C.Structure):
+    """nd_packed_attention"""
+    _fields_ = ([(n, C.c_int64) for n in ("n_tokens", "n_covered")] +
+                [(n, C.c_int32) for n in ("heads", "kv_heads", "dim", "dtype")] + [("scale", C.c_float)] +
+                [(n, C.c_void_p) for n in ("plan", "q", "k", "v", "dout")] +
+                [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "dout_token",
+                                          "dout_head")] +
+                [(n, C.c_void_p) for n in ("out", "lse", "delta", "dq", "dk", "dv")])
+
+
+class VocabularyLoss(C.Structure):
+    """nd_vocabulary_loss"""
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "classes")] + [(n, C.c_int32) for n in ("dim", "dtype")] +
+                [(n, C.c_void_p) for n in ("hidden", "weight", "target", "loss", "lse", "dloss", "dhidden", "dweight",
+                                           "workspace")] + [("workspace_bytes", C.c_int64)])
+
+
 # name -> (restype, argtypes); every symbol include/nextdoor_amd.h declares
 SIGNATURES = {
     "nd_last_error": (C.c_char_p, []),
@@ -81,6 +100,15 @@ SIGNATURES = {
                                              c_f32p, C.c_int64, c_i32p]),
     "nd_measure_gather_rate": (C.c_int, [C.c_int64, C.POINTER(C.c_double)]),
     "nd_measure_gather_rate_shaped": (C.c_int, [C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_double)]),
+    "nd_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_double, C.c_uint64, C.c_uint32,
+                             C.c_void_p]),
+    "nd_packed_plan_bytes": (C.c_int64, [C.c_int64]),
+    "nd_packed_plan": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nd_packed_attention_forward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
+    "nd_packed_attention_backward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
+    "nd_vocabulary_loss_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int]),
+    "nd_vocabulary_loss_forward": (C.c_int, [C.POINTER(VocabularyLoss), C.c_void_p]),
+    "nd_vocabulary_loss_backward": (C.c_int, [C.POINTER(VocabularyLoss), C.c_void_p]),
     "nd_unique_transits": (C.c_int, [c_i32p, C.c_int64, C.c_int32, c_i32p, c_i32p, c_i32p, c_i64p, c_i64p]),
 }
 

@@ -17,6 +17,7 @@
 #include "nd_apps_layer.hpp"
 #include "nd_apps_walks.hpp"
 #include "nd_app_registry.hpp"
+#include "nd_errors.hpp"
 #include "nd_graph.hpp"
 #include "nd_check.hpp"
 
@@ -28,27 +29,8 @@ struct nd_sampler {
 
 namespace {
 
-thread_local std::string g_error;
-
-int fail(const std::string& msg, int code = -1) {
-  g_error = msg;
-  return code;
-}
-
-// No exception leaves the library: a body that throws (host memory, a container's range
-// check) reports through the error text like any other failure.
-template <class Body>
-int guarded(Body body) {
-  try {
-    return body();
-  } catch (const std::bad_alloc&) {
-    return fail("out of host memory");
-  } catch (const std::exception& e) {
-    return fail(std::string("internal error: ") + e.what());
-  } catch (...) {
-    return fail("internal error");
-  }
-}
+using nd::fail;
+using nd::guarded;
 
 struct AppEntry {
   const char* name;
@@ -246,7 +228,7 @@ hipError_t scratch_on_current_device(uint32_t** out) {
 
 extern "C" {
 
-const char* nd_last_error(void) { return g_error.c_str(); }
+const char* nd_last_error(void) { return nd::last_error_text().c_str(); }
 
 int nd_num_apps(void) {
   std::lock_guard<std::mutex> lock(registry_mutex());
@@ -562,7 +544,7 @@ int nd_check_sampled_vertices(const nd_graph* g, int n_steps, const int32_t* ste
     shape.collective = collective != 0;
     std::string report;
     if (nd::check_sampled_vertices(*g, shape, n_samples, initial, final_samples, invalid, &report)) return 1;
-    g_error = report;
+    nd::last_error_text() = report;
     return 0;
   });
 }
@@ -592,7 +574,7 @@ int nd_sampler_check_results(nd_sampler* s, int* ok) {
       pass = nd::check_subgraph_edge_lists(*s->graph, e.num_samples(), shape.initial_size, e.initialContents.data(),
                                            e.hListStart.data(), e.hListRows.data(), e.hListCols.data(), &report);
       *ok = pass ? 1 : 0;
-      if (!pass) g_error = report;
+      if (!pass) nd::last_error_text() = report;
       return 0;
     }
     const size_t layers = shape.step_size.size(), cells = (size_t)shape.step_size[0] * shape.step_size[0];
@@ -610,7 +592,7 @@ int nd_sampler_check_results(nd_sampler* s, int* ok) {
                                         e.hFinalSamples.data(), e.invalid_vertex(), &report);
     }
     *ok = pass ? 1 : 0;
-    if (!pass) g_error = report;
+    if (!pass) nd::last_error_text() = report;
     return 0;
   });
 }
@@ -642,9 +624,9 @@ int nd_init_sampling(const char* app_name, const char* graph_path, uint64_t seed
     if (rc == 0) rc = nd_sampler_set_graph(g_module_sampler, g_module_graph);
     if (rc == 0) rc = nd_sampler_alloc(g_module_sampler, seed);
     if (rc != 0) {
-      const std::string keep = g_error;
+      const std::string keep = nd::last_error_text();
       nd_free_device_memory();
-      g_error = keep;
+      nd::last_error_text() = keep;
     }
     return rc;
   });
@@ -660,9 +642,9 @@ int nd_init_sampling_from_csr(const char* app_name, int32_t n_vertices, int64_t 
     if (rc == 0) rc = nd_sampler_set_graph(g_module_sampler, g_module_graph);
     if (rc == 0) rc = nd_sampler_alloc(g_module_sampler, seed);
     if (rc != 0) {
-      const std::string keep = g_error;
+      const std::string keep = nd::last_error_text();
       nd_free_device_memory();
-      g_error = keep;
+      nd::last_error_text() = keep;
     }
     return rc;
   });

@@ -1,0 +1,340 @@
+"""Operators of models that train on samples, on torch tensors of the GPU.
+
+Walks are sequences of different lengths whose words are the vertices of the graph.  A training step
+over a batch of them needs
+
+* :func:`packed_attention`: causal attention within each walk of a packed batch, with grouped heads;
+* :func:`dropout`: from the samplers' own random stream, the mask never stored;
+* :func:`vocabulary_loss`: softmax cross entropy over all vertices, the logits never stored.
+
+Each has a ``_forward`` and a ``_backward`` function and a differentiable form that calls both.  They
+enqueue the library's HIP kernels (include/nextdoor_amd.h) on torch's current stream of the tensors'
+device and wait for nothing; results are new tensors.  There is no other implementation: CPU tensors,
+types and shapes that the kernels do not have are errors (:class:`NextDoorError`).
+
+Import this module (or torch) before the first call into the library: torch brings its own HIP
+runtime, and streams and memory can only be shared within one.
+"""
+import math
+
+import numpy as np
+import torch
+
+from . import _capi
+from ._capi import NextDoorError, PackedAttention, VocabularyLoss, check
+
+__all__ = ["PackedSequences", "packed_attention", "packed_attention_forward", "packed_attention_backward",
+           "vocabulary_loss", "vocabulary_loss_forward", "vocabulary_loss_backward", "dropout", "dropout_forward",
+           "dropout_backward", "NextDoorError"]
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # ND_F32, ND_F16, ND_BF16
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        handle = _capi.lib()
+        with open("/proc/self/maps") as maps:
+            runtimes = {line.split()[-1] for line in maps if "libamdhip64" in line}
+        if len(runtimes) > 1:
+            raise NextDoorError("the library was loaded before torch, on a HIP runtime of its own: import torch (or "
+                                "nextdoor_amd.ops) before the first call into nextdoor_amd")
+        _lib = handle
+    return _lib
+
+
+def _need(condition, message):
+    if not condition:
+        raise NextDoorError(message)
+
+
+def _on_gpu(what, *tensors):
+    """Checks that all tensors lie on one GPU; returns its index."""
+    for t in tensors:
+        _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s: tensors on the GPU only" % what)
+    device = tensors[0].device
+    for t in tensors:
+        _need(t.device == device, "%s: tensors on different devices" % what)
+    return device.index
+
+
+class _On:
+    """Makes a device current for a call, if it is not."""
+
+    def __init__(self, index):
+        self._index = index
+        self._before = torch.cuda.current_device()
+
+    def __enter__(self):
+        if self._before != self._index:
+            torch.cuda.set_device(self._index)
+        return torch.cuda.current_stream(self._index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._before != self._index:
+            torch.cuda.set_device(self._before)
+
+
+# ---- dropout -------------------------------------------------------------------------------------
+
+
+def _dropout(x, p, seed, step, residual):
+    index = _on_gpu("dropout", x) if residual is None else _on_gpu("dropout", x, residual)
+    _need(x.dtype in _DTYPES, "dropout: no kernel for %s" % x.dtype)
+    _need(0.0 <= p <= 1.0, "dropout: p is a probability, %r given" % (p,))
+    _need(0 <= seed < 1 << 64, "dropout: a seed has 64 bits, %r given" % (seed,))
+    _need(0 <= step < 1 << 31, "dropout: step numbers are below 2^31, %r given" % (step,))
+    if residual is not None:
+        _need(residual.shape == x.shape and residual.dtype == x.dtype,
+              "dropout: the residual is of another shape or type")
+        residual = residual.contiguous()
+    x = x.contiguous()
+    out = torch.empty_like(x)
+    with _On(index) as stream:
+        check(_library().nd_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
+                                    x.numel(), _DTYPES[x.dtype], p, seed, step, stream))
+    return out
+
+
+def dropout_forward(x, p, seed, step, residual=None):
+    """x / (1 - p) where an element is kept, 0 where it is dropped (whatever it holds), plus the residual.  Element o
+    (in row-major order) is kept if ``philox_fill_uniform(seed, step, o, 1, step_size=2) >= p``: give each
+    dropout of a training step its own ``step``.  Sums are rounded once."""
+    return _dropout(x, p, seed, step, residual)
+
+
+def dropout_backward(dout, p, seed, step):
+    """The gradient of x; the residual's is ``dout`` itself."""
+    return _dropout(dout, p, seed, step, None)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, step):
+        ctx.how = p, seed, step
+        ctx.has_residual = residual is not None
+        return _dropout(x, p, seed, step, residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        dx = dropout_backward(dout, *ctx.how) if ctx.needs_input_grad[0] else None
+        return dx, dout if ctx.has_residual and ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x, p, seed, step, residual=None):
+    """:func:`dropout_forward`, differentiable in x and the residual."""
+    return _Dropout.apply(x, residual, p, seed, step)
+
+
+# ---- packed attention ------------------------------------------------------------------------------
+
+
+class PackedSequences:
+    """Where the sequences of a packed batch lie: sequence i is tokens ``starts[i] .. starts[i + 1] - 1``.
+
+    ``starts`` (a list, a numpy array or a tensor; integers) begins with 0 and does not fall; a tensor on the GPU is
+    read back to be checked, which waits for it.  ``n_tokens`` (default: ``starts[-1]``) may be larger: tokens after
+    the last sequence belong to none.  Make one per batch; every layer and both directions use it."""
+
+    def __init__(self, starts, n_tokens=None, device=None):
+        if isinstance(starts, torch.Tensor):
+            _need(not starts.is_floating_point(), "packed sequences: starts are integers")
+            device = device if device is not None or not starts.is_cuda else starts.device
+            starts = starts.cpu().numpy()
+        starts = np.asarray(starts)
+        _need(starts.ndim == 1 and len(starts) >= 1 and starts.dtype.kind in "iu",
+              "packed sequences: starts is a list of integers, one more than there are sequences")
+        _need(starts.min() >= 0 and starts.max() <= 2147483392, "packed sequences: starts out of range")
+        starts = np.ascontiguousarray(starts, dtype=np.int32)
+        self.device = torch.device("cuda" if device is None else device)
+        _need(self.device.type == "cuda", "packed sequences: on a GPU only")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.n_sequences, self.n_covered = len(starts) - 1, int(starts[-1])
+        self.n_tokens = self.n_covered if n_tokens is None else int(n_tokens)
+        lib = _library()
+        size = lib.nd_packed_plan_bytes(self.n_tokens)
+        _need(size >= 0, "packed sequences: no plan for %d tokens" % self.n_tokens)
+        on_device = torch.from_numpy(starts).to(self.device)
+        self.plan = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
+        with _On(self.device.index) as stream:
+            check(lib.nd_packed_plan(starts.ctypes.data, self.n_sequences, self.n_tokens, on_device.data_ptr(),
+                                     self.plan.data_ptr(), stream))
+
+
+def _heads(what, x, tokens, dim=None):
+    """A [token, head, dim] tensor as the kernels read it: dim side by side, the rest strided by multiples of 16 bytes.
+    Anything else is copied."""
+    _need(x.dim() == 3 and x.shape[0] == tokens, "packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
+    _need(dim is None or x.shape[2] == dim, "packed attention: %s has another head size" % what)
+    a, b, c = x.stride()
+    if (c != 1 and x.shape[2] > 1) or a % 8 or b % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+def _attention(sequences, q, k, v, scale):
+    index = _on_gpu("packed attention", q, k, v, sequences.plan)
+    _need(q.dtype in (torch.float16, torch.bfloat16), "packed attention: 16-bit types only, %s given" % q.dtype)
+    _need(k.dtype == q.dtype and v.dtype == q.dtype, "packed attention: q, k and v are of different types")
+    tokens = sequences.n_tokens
+    q = _heads("q", q, tokens)
+    dim = q.shape[2]
+    k, v = _heads("k", k, tokens, dim), _heads("v", v, tokens, dim)
+    _need(k.shape == v.shape, "packed attention: k and v are of different shapes")
+    a = PackedAttention()
+    a.n_tokens, a.n_covered = tokens, sequences.n_covered
+    a.heads, a.kv_heads, a.dim, a.dtype = q.shape[1], k.shape[1], dim, _DTYPES[q.dtype]
+    a.scale = 1 / math.sqrt(dim) if scale is None else scale
+    a.plan = sequences.plan.data_ptr()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_token, a.q_head = q.stride()[:2]
+    a.k_token, a.k_head = k.stride()[:2]
+    a.v_token, a.v_head = v.stride()[:2]
+    return index, a, (q, k, v)
+
+
+def packed_attention_forward(q, k, v, sequences, scale=None):
+    """Causal attention within each sequence: (out, lse).
+
+    q, out: [tokens, heads, dim]; k, v: [tokens, kv_heads, dim], ``heads / kv_heads`` query heads to each; dim a
+    multiple of 8 up to 128; float16 or bfloat16.  Slices of one projection are read in place.  lse:
+    [heads, tokens], float32, for the backward pass.  ``scale`` is 1 / sqrt(dim) unless given.  Rows of tokens that
+    belong to no sequence are 0 (lse -inf) and their inputs are not read."""
+    index, a, keep = _attention(sequences, q, k, v, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((a.heads, a.n_tokens), dtype=torch.float32, device=q.device)
+    a.out, a.lse = out.data_ptr(), lse.data_ptr()
+    with _On(index) as stream:
+        check(_library().nd_packed_attention_forward(a, stream))
+    del keep
+    return out, lse
+
+
+def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
+    """(dq, dk, dv) for the gradient ``dout`` of ``out``, which with ``lse`` is the forward pass's."""
+    index, a, keep = _attention(sequences, q, k, v, scale)
+    _on_gpu("packed attention", q, dout, out, lse)
+    _need(dout.shape == q.shape and dout.dtype == q.dtype, "packed attention: dout is of another shape or type than q")
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and lse.is_contiguous() and
+          lse.dtype == torch.float32 and tuple(lse.shape) == (a.heads, a.n_tokens),
+          "packed attention: out and lse are not a forward pass's")
+    dout = _heads("dout", dout, a.n_tokens)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+    delta = torch.empty_like(lse)
+    a.dout, a.out, a.lse, a.delta = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), delta.data_ptr()
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    a.dout_token, a.dout_head = dout.stride()[:2]
+    with _On(index) as stream:
+        check(_library().nd_packed_attention_backward(a, stream))
+    del keep
+    return dq, dk, dv
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sequences, scale):
+        out, lse = packed_attention_forward(q, k, v, sequences, scale)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.how = sequences, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        return (*packed_attention_backward(dout, q, k, v, out, lse, *ctx.how), None, None)
+
+
+def packed_attention(q, k, v, sequences, scale=None):
+    """The ``out`` of :func:`packed_attention_forward`, differentiable in q, k and v."""
+    return _PackedAttention.apply(q, k, v, sequences, scale)
+
+
+# ---- cross entropy over the vocabulary -----------------------------------------------------------------
+
+
+def _vectors(x):
+    if x.shape[1] % 8:  # the kernels read 16 bytes at a time
+        x = torch.nn.functional.pad(x, (0, 8 - x.shape[1] % 8))
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
+def _loss(hidden, weight, target, backward):
+    index = _on_gpu("vocabulary loss", hidden, weight, target)
+    _need(hidden.dtype in (torch.float16, torch.bfloat16), "vocabulary loss: 16-bit types only, %s given" % hidden.dtype)
+    _need(weight.dtype == hidden.dtype, "vocabulary loss: hidden and weight are of different types")
+    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1],
+          "vocabulary loss: hidden and weight are not matrices of equally long rows")
+    hidden, weight = _vectors(hidden), _vectors(weight)
+    _need(target.dim() == 1 and target.shape[0] == hidden.shape[0], "vocabulary loss: one target for each row of hidden")
+    _need(target.dtype in (torch.int32, torch.int64), "vocabulary loss: targets are int32 or int64")
+    if target.dtype == torch.int64:  # (what is no class stays none: 2^31 - 1 is above every class)
+        target = torch.where((target < 0) | (target > 2147483647), 2147483647, target).to(torch.int32)
+    target = target.contiguous()
+    a = VocabularyLoss()
+    a.rows, a.dim = hidden.shape
+    a.classes, a.dtype = weight.shape[0], _DTYPES[hidden.dtype]
+    a.hidden, a.weight, a.target = hidden.data_ptr(), weight.data_ptr(), target.data_ptr()
+    size = _library().nd_vocabulary_loss_workspace(a.rows, a.classes, a.dim, backward)
+    _need(size >= 0, "vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (a.rows, a.classes, a.dim))
+    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hidden.device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    return index, a, (hidden, weight, target, workspace)
+
+
+def vocabulary_loss_forward(hidden, weight, target):
+    """(loss, lse) of each row, float32: ``lse_i = log sum_v exp(hidden_i . weight_v)``, ``loss_i = lse_i - hidden_i .
+    weight_{target_i}``.  hidden: [rows, dim], weight: [classes, dim], float16 or bfloat16 (a dim that is no
+    multiple of 8 costs a copy); target: int32 or int64.  A row whose target is no class - the samplers' INVALID is
+    |V| - has loss 0."""
+    index, a, keep = _loss(hidden, weight, target, 0)
+    loss, lse = (torch.empty(a.rows, dtype=torch.float32, device=hidden.device) for _ in range(2))
+    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
+    with _On(index) as stream:
+        check(_library().nd_vocabulary_loss_forward(a, stream))
+    del keep
+    return loss, lse
+
+
+def vocabulary_loss_backward(dloss, hidden, weight, target, lse):
+    """(dhidden, dweight) for the gradient ``dloss`` of each row's loss; lse is the forward pass's.  Rows without a
+    target send nothing back, whatever their ``dloss``."""
+    size = hidden.shape
+    index, a, keep = _loss(hidden, weight, target, 1)
+    _on_gpu("vocabulary loss", hidden, dloss, lse)
+    _need(tuple(dloss.shape) == (a.rows,) and tuple(lse.shape) == (a.rows,) and lse.dtype == torch.float32,
+          "vocabulary loss: dloss and lse have one value for each row")
+    dloss, lse = dloss.to(torch.float32).contiguous(), lse.contiguous()
+    dhidden, dweight = torch.empty_like(keep[0]), torch.empty_like(keep[1])
+    a.dloss, a.lse, a.dhidden, a.dweight = dloss.data_ptr(), lse.data_ptr(), dhidden.data_ptr(), dweight.data_ptr()
+    with _On(index) as stream:
+        check(_library().nd_vocabulary_loss_backward(a, stream))
+    del keep
+    if size[1] != a.dim:
+        dhidden, dweight = dhidden[:, :size[1]].contiguous(), dweight[:, :size[1]].contiguous()
+    return dhidden, dweight
+
+
+class _VocabularyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target):
+        loss, lse = vocabulary_loss_forward(hidden, weight, target)
+        ctx.save_for_backward(hidden, weight, target, lse)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        return (*vocabulary_loss_backward(dloss, *ctx.saved_tensors), None)
+
+
+def vocabulary_loss(hidden, weight, target):
+    """The loss of each row (:func:`vocabulary_loss_forward`), differentiable in hidden and weight."""
+    return _VocabularyLoss.apply(hidden, weight, target)

@@ -1,0 +1,435 @@
+"""The training operators on the GPU, against their definitions in 64 bits (operators_reference.py)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from nextdoor_amd import NextDoorError, ops
+from tests import operators_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def normal(seed, *shape, dtype=BF16, std=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=gen) * std).to(dtype)
+
+
+def starts_of(lengths):
+    return np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+
+
+def check_all(got, want, off, what):
+    for name in got:
+        assert ref.close(got[name], want[name], off[name]), (what, name)
+
+
+# ---- packed attention --------------------------------------------------------------------------
+
+LENGTHS = {
+    "one_token": [1],
+    "two": [2],
+    "ones": [1] * 70,
+    "empty_between": [0, 3, 0, 0, 40, 0],
+    "tile": [128],
+    "tile_and_one": [129],
+    "one_less": [127, 1],
+    "across_tiles": [5, 120, 64, 63, 65, 1, 300, 7],
+    "long": [901],
+    "walks": list(np.random.default_rng(3).integers(1, 102, 40)),
+}
+
+
+def run_attention(q, k, v, starts, dout, scale=None, tokens=None):
+    seq = ops.PackedSequences(starts, q.shape[0] if tokens is None else tokens)
+    out, lse = ops.packed_attention_forward(q, k, v, seq, scale)
+    dq, dk, dv = ops.packed_attention_backward(dout, q, k, v, out, lse, seq, scale)
+    torch.cuda.synchronize()
+    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+@pytest.mark.parametrize("lengths", sorted(LENGTHS))
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (3, 1, 128, F16), (2, 2, 32, BF16)])
+def test_attention_over_lengths(lengths, heads, kv_heads, dim, dtype):
+    starts = starts_of(LENGTHS[lengths])
+    t = int(starts[-1])
+    q, dout = normal(1, t, heads, dim, dtype=dtype), normal(2, t, heads, dim, dtype=dtype)
+    k, v = normal(3, t, kv_heads, dim, dtype=dtype), normal(4, t, kv_heads, dim, dtype=dtype)
+    print("attention", lengths, heads, kv_heads, dim, dtype, flush=True)
+    want, off = ref.attention(q, k, v, starts, 1 / math.sqrt(dim), dout)
+    check_all(run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda()), want, off, lengths)
+
+
+@pytest.mark.parametrize("dim", [8, 16, 24, 40, 72, 80, 96, 104, 120])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_head_sizes(dim, dtype):
+    starts = starts_of([17, 150, 33])
+    t = int(starts[-1])
+    q, dout = normal(1, t, 2, dim, dtype=dtype), normal(2, t, 2, dim, dtype=dtype)
+    k, v = normal(3, t, 1, dim, dtype=dtype), normal(4, t, 1, dim, dtype=dtype)
+    want, off = ref.attention(q, k, v, starts, 1 / math.sqrt(dim), dout)
+    check_all(run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda()), want, off, dim)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
+def test_attention_scales_and_large_logits(scale):
+    starts = starts_of([90, 45])
+    q, k, v, dout = (normal(i, 135, 2, 64, std=2.0) for i in range(4))
+    want, off = ref.attention(q, k, v, starts, scale, dout)
+    check_all(run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda(), scale), want, off, scale)
+
+
+def test_attention_reads_slices_of_a_projection_in_place_and_copies_other_orders():
+    starts = starts_of([70, 1, 99])
+    t, heads, kv_heads, dim = 170, 4, 2, 64
+    qkv = normal(5, t, heads + 2 * kv_heads, dim)
+    q, k, v = qkv.split([heads, kv_heads, kv_heads], 1)
+    dout = normal(6, t, heads, dim)
+    want, off = ref.attention(q, k, v, starts, 1 / 8, dout)
+    a = qkv.cuda()
+    split = a.split([heads, kv_heads, kv_heads], 1)
+    assert ops._heads("q", split[0], t) is split[0]
+    check_all(run_attention(*split, starts, dout.cuda()), want, off, "slices")
+    # heads first; dim not side by side; rows that do not begin at multiples of 16 bytes; a broadcast gradient
+    others = [x.cuda().transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    check_all(run_attention(*others, starts, dout.cuda()), want, off, "heads first")
+    others = [x.cuda().transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    check_all(run_attention(*others, starts, dout.cuda()), want, off, "dim first")
+    wide = torch.zeros(t, heads, dim + 3, dtype=BF16, device="cuda")
+    wide[:, :, 3:] = dout.cuda()
+    check_all(run_attention(*split, starts, wide[:, :, 3:]), want, off, "odd rows")
+    one = normal(7, 1, 1, dim).expand(t, heads, dim)
+    want, off = ref.attention(q, k, v, starts, 1 / 8, one)
+    check_all(run_attention(*split, starts, one.cuda().expand(t, heads, dim)), want, off, "broadcast gradient")
+
+
+def test_attention_leaves_tokens_of_no_sequence_alone():
+    """The rest of a buffer: not read (it holds NaN here), its rows of every result 0."""
+    starts, t = starts_of([100, 55]), 155 + 210
+    q, k, v, dout = (normal(i, t, 2, 64) for i in range(4))
+    want, off = ref.attention(q, k, v, starts, 1 / 8, dout)
+    gpu = []
+    for x in (q, k, v, dout):
+        x = x.cuda()
+        x[155:] = math.nan
+        gpu.append(x)
+    got = run_attention(*gpu[:3], starts, gpu[3])
+    check_all(got, want, off, "rest")
+    assert not got["out"][155:].any() and torch.isinf(got["lse"][:, 155:]).all()
+    assert not got["dq"][155:].any() and not got["dk"][155:].any() and not got["dv"][155:].any()
+
+
+def test_attention_without_any_sequence():
+    for starts, t in (([0], 0), ([0], 5), ([0, 0, 0], 5)):
+        x = normal(1, t, 2, 32).cuda()
+        got = run_attention(x, x, x, starts, x, tokens=t)
+        assert got["out"].shape == (t, 2, 32) and not got["out"].any() and not got["dk"].any()
+
+
+def test_attention_gradients_against_differences():
+    """Directional derivatives of a fixed combination of the outputs, from the kernel's own outputs in the steps."""
+    starts, t, dim = starts_of([40, 21]), 61, 32
+    q, k, v, dout = (normal(i, t, 2, dim, dtype=F16) for i in range(4))
+    seq = ops.PackedSequences(starts)
+    args = [x.cuda().requires_grad_() for x in (q, k, v)]
+    (ops.packed_attention(*args, seq) * dout.cuda()).sum().backward()
+    step = 2.0 ** -4
+    for i, x in enumerate((q, k, v)):
+        direction = torch.sign(normal(9 + i, *x.shape, dtype=F16))
+        value = []
+        for sign in (1, -1):
+            moved = [y.double() for y in (q, k, v)]
+            moved[i] = moved[i] + sign * step * direction.double()
+            # the moved inputs are exact in float16 only by chance: the definition is moved, the kernel's slope compared
+            want, _ = ref.attention(*[_Double(y) for y in moved], starts, 1 / math.sqrt(dim))
+            value.append(float((want["out"] * dout.double()).sum()))
+        slope = (value[0] - value[1]) / (2 * step)
+        mine = float((args[i].grad.cpu().double() * direction.double()).sum())
+        # the third derivative's share of a central difference, and t * 2 * dim roundings of 2^-11 of values near 1
+        assert abs(mine - slope) <= 0.02 * abs(slope) + 2.0, (i, mine, slope)
+
+
+class _Double:
+    """A 64-bit tensor that the reference treats as float16 inputs (it only asks for a type's unit)."""
+
+    def __init__(self, x):
+        self._x, self.dtype = x, F16
+
+    def double(self):
+        return self._x
+
+
+def test_attention_is_the_same_on_another_stream_and_in_a_graph():
+    starts = starts_of([200, 77, 3])
+    q, k, v, dout = (normal(i, 280, 4, 64).cuda() for i in range(4))
+    seq = ops.PackedSequences(starts)
+
+    def step():
+        out, lse = ops.packed_attention_forward(q, k, v, seq)
+        return (out, *ops.packed_attention_backward(dout, q, k, v, out, lse, seq))
+
+    want = [x.clone() for x in step()]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = step()
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        for x in got:
+            x.zero_()
+        q.copy_(q.roll(1, 0) if i == 1 else q)
+        want = [x.clone() for x in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_attention_refuses():
+    x = normal(1, 10, 4, 64).cuda()
+    seq = ops.PackedSequences([0, 10])
+    out, lse = ops.packed_attention_forward(x, x, x, seq)
+
+    def refused(match, fn, *args, **kw):
+        with pytest.raises(NextDoorError, match=match):
+            fn(*args, **kw)
+
+    forward, backward = ops.packed_attention_forward, ops.packed_attention_backward
+    refused("16-bit", forward, x.float(), x.float(), x.float(), seq)
+    refused("different types", forward, x, x.half(), x, seq)
+    refused("GPU only", forward, x.cpu(), x, x, seq)
+    refused("10 tokens", forward, x[:9], x, x, seq)
+    refused("another head size", forward, x, x[..., :32], x[..., :32], seq)
+    refused("different shapes", forward, x, x[:, :2], x, seq)
+    refused("evenly", forward, x, x[:, :3], x[:, :3], seq)
+    refused("multiple of 8", forward, x[..., :12], x[..., :12], x[..., :12], seq)
+    wide = normal(1, 10, 1, 136).cuda()
+    refused("multiple of 8 up to 128", forward, wide, wide, wide, seq)
+    refused("not finite", forward, x, x, x, seq, math.inf)
+    refused("dout", backward, x[:, :2], x, x, x, out, lse, seq)
+    refused("forward pass's", backward, x, x, x, x, out, lse[:2], seq)
+    refused("not 0", ops.PackedSequences, [1, 10])
+    refused("before it starts", ops.PackedSequences, [0, 5, 4, 10])
+    refused("10 tokens in sequences, 9", ops.PackedSequences, [0, 10], 9)
+    refused("list of integers", ops.PackedSequences, [0.0, 10.0])
+    refused("integers", ops.PackedSequences, torch.tensor([0.0, 10.0]))
+
+
+# ---- vocabulary loss -----------------------------------------------------------------------------
+
+
+def run_loss(hidden, weight, target, dloss):
+    loss, lse = ops.vocabulary_loss_forward(hidden, weight, target)
+    dhidden, dweight = ops.vocabulary_loss_backward(dloss, hidden, weight, target, lse)
+    torch.cuda.synchronize()
+    return {"loss": loss, "lse": lse, "dhidden": dhidden, "dweight": dweight}
+
+
+def targets(seed, rows, classes):
+    """A fifth of them no class: -1, |V|, far out."""
+    rng = np.random.default_rng(seed)
+    t = rng.integers(0, classes, rows)
+    none = rng.random(rows) < 0.2
+    t[none] = rng.choice([-1, classes, 2 ** 31 - 1, -2 ** 31], int(none.sum()))
+    return torch.from_numpy(t)
+
+
+@pytest.mark.parametrize("rows,classes,dim,dtype", [
+    (1, 1, 8, BF16), (1, 2711, 64, F16), (61, 2711, 64, BF16), (128, 128, 64, BF16), (129, 257, 72, F16),
+    (127, 1, 16, BF16), (300, 1000, 128, BF16), (33, 5003, 200, F16), (257, 4099, 520, BF16), (1000, 31, 40, F16),
+    (2, 70001, 32, BF16), (700, 3001, 256, BF16), (513, 2049, 264, F16)])
+def test_loss_and_gradients(rows, classes, dim, dtype):
+    print("loss", rows, classes, dim, dtype, flush=True)
+    h, w = normal(1, rows, dim, dtype=dtype), normal(2, classes, dim, dtype=dtype, std=2 / math.sqrt(dim))
+    t = targets(3, rows, classes)
+    dloss = (0.5 + torch.rand(rows, generator=torch.Generator().manual_seed(4))) / rows
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    check_all(run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda()), want, off, (rows, classes, dim))
+    got = run_loss(h.cuda(), w.cuda(), t.to(torch.int32).cuda(), dloss.cuda())
+    check_all(got, want, off, "32-bit targets")
+
+
+def test_loss_goes_through_several_pieces_of_the_vocabulary():
+    """More rows than one piece's workspace holds for all classes; checked against products in 32 bits on the GPU, which
+    agree with 64 bits to SMALL of the sums of magnitudes."""
+    rows, classes, dim = 20000, 9001, 64
+    h, w = normal(1, rows, dim).cuda(), normal(2, classes, dim, std=0.25).cuda()
+    t = targets(3, rows, classes).cuda()
+    dloss = (0.5 + torch.rand(rows, device="cuda")) / rows
+    got = run_loss(h, w, t, dloss)
+    z = h.double() @ w.double().T
+    lse = torch.logsumexp(z, 1)
+    g = torch.exp(z - lse[:, None])
+    has = (t >= 0) & (t < classes)
+    g[has.nonzero()[:, 0], t[has]] -= 1
+    g *= torch.where(has, dloss, torch.zeros_like(dloss)).double()[:, None]
+    assert torch.allclose(got["lse"].double(), lse, rtol=0, atol=2.0 ** -13)
+    for name, value, spread in (("dhidden", g @ w.double(), g.abs() @ w.double().abs()),
+                                ("dweight", g.T @ h.double(), g.abs().T @ h.double().abs())):
+        off = 2.0 ** -8 * (value.abs() + spread) + ref.SMALL * 4 * spread
+        assert ((got[name].double() - value).abs() <= off).all(), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_loss_of_peaked_and_of_tiny_gradients(dtype):
+    """Rows whose target has nearly all the weight, logits in the hundreds, and the tiny gradients of a large mean."""
+    rows, classes, dim = 200, 700, 64
+    h, w = normal(1, rows, dim, dtype=dtype, std=3.0), normal(2, classes, dim, dtype=dtype, std=3.0)
+    t = (h.double() @ w.double().T).argmax(1)
+    for size in (1.0, 1e-7):
+        dloss = torch.rand(rows, generator=torch.Generator().manual_seed(4)) * size
+        want, off = ref.vocabulary_loss(h, w, t, dloss)
+        check_all(run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda()), want, off, size)
+
+
+def test_loss_rows_without_a_target_send_nothing_back():
+    h, w = normal(1, 50, 32).cuda(), normal(2, 100, 32).cuda()
+    h[7] = math.nan
+    t = torch.full((50,), 100, device="cuda")
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    dh, dw = ops.vocabulary_loss_backward(torch.full((50,), math.inf, device="cuda"), h, w, t, lse)
+    assert not loss.any() and not dh.any()
+
+
+def test_loss_without_rows():
+    h, w = normal(1, 0, 32).cuda(), normal(2, 100, 32).cuda()
+    t = torch.zeros(0, dtype=torch.int64, device="cuda")
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    dh, dw = ops.vocabulary_loss_backward(loss, h, w, t, lse)
+    assert loss.shape == (0,) and dh.shape == (0, 32) and dw.shape == (100, 32) and not dw.any()
+
+
+@pytest.mark.parametrize("dim", [1, 7, 50])
+def test_loss_of_odd_vectors_and_orders(dim):
+    h, w, t = normal(1, 40, dim), normal(2, 90, dim), targets(3, 40, 90)
+    dloss = torch.ones(1).expand(40)
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    got = run_loss(h.cuda(), w.T.contiguous().T.cuda(), t.cuda(), dloss.cuda().expand(40))
+    assert got["dhidden"].shape == h.shape and got["dweight"].shape == w.shape
+    check_all(got, want, off, dim)
+
+
+def test_loss_gradients_against_differences():
+    rows, classes, dim = 30, 400, 64
+    h, w, t = normal(1, rows, dim, dtype=F16), normal(2, classes, dim, dtype=F16, std=0.2), targets(3, rows, classes)
+    a, b = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    ops.vocabulary_loss(a, b, t.cuda()).sum().backward()
+    step = 2.0 ** -8
+    for i, grad in enumerate((a.grad, b.grad)):
+        direction = torch.sign(normal(9 + i, *(h, w)[i].shape, dtype=F32)).double()
+        value = []
+        for sign in (1, -1):
+            moved = [h.double(), w.double()]
+            moved[i] = moved[i] + sign * step * direction
+            z = moved[0] @ moved[1].T
+            has = (t >= 0) & (t < classes)
+            value.append(float((torch.logsumexp(z, 1)[has] - z[has, t[has]]).sum()))
+        slope = (value[0] - value[1]) / (2 * step)
+        mine = float((grad.cpu().double() * direction).sum())
+        # roundings of 2^-11 of each entry, of random sign here, and the third derivative's share
+        off = 2.0 ** -11 * float(grad.cpu().double().abs().sum()) + 2e-3 * abs(slope) + 0.05
+        assert abs(mine - slope) <= off, (i, mine, slope)
+
+
+def test_loss_is_the_same_in_a_graph():
+    h, w = normal(1, 300, 64).cuda(), normal(2, 5000, 64, std=0.2).cuda()
+    t = targets(3, 300, 5000).to(torch.int32).cuda()
+    dloss = torch.full((300,), 1 / 300, device="cuda")
+
+    def step():
+        loss, lse = ops.vocabulary_loss_forward(h, w, t)
+        return (loss, *ops.vocabulary_loss_backward(dloss, h, w, t, lse))
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        for x in got:
+            x.zero_()
+        h.copy_(h.roll(1, 0))
+        want = [x.clone() for x in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_loss_refuses():
+    h, w = normal(1, 10, 64).cuda(), normal(2, 30, 64).cuda()
+    t = torch.zeros(10, dtype=torch.int64, device="cuda")
+    _, lse = ops.vocabulary_loss_forward(h, w, t)
+
+    def refused(match, fn, *args):
+        with pytest.raises(NextDoorError, match=match):
+            fn(*args)
+
+    forward, backward = ops.vocabulary_loss_forward, ops.vocabulary_loss_backward
+    refused("16-bit", forward, h.float(), w.float(), t)
+    refused("different types", forward, h, w.half(), t)
+    refused("equally long", forward, h, w[:, :32], t)
+    refused("one target", forward, h, w, t[:9])
+    refused("int32 or int64", forward, h, w, t.float())
+    refused("GPU only", forward, h, w, t.cpu())
+    refused("classes", forward, h, w[:0], t)
+    refused("one value for each row", backward, lse[:9], h, w, t, lse)
+
+
+# ---- dropout ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("shape", [(1,), (3,), (4,), (7,), (8,), (9,), (101, 64), (33, 31), (5000, 21), (2, 3, 5)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(shape, dtype, p):
+    x, r = normal(1, *shape, dtype=dtype), normal(2, *shape, dtype=dtype)
+    seed, step = 0xFEDCBA9876543210, 17
+    want, off = ref.dropout(x, p, seed, step)
+    got = ops.dropout_forward(x.cuda(), p, seed, step)
+    assert ref.close(got, want, off)
+    assert torch.equal(got, ops.dropout_backward(x.cuda(), p, seed, step))
+    want, off = ref.dropout(x, p, seed, step, r)
+    assert ref.close(ops.dropout_forward(x.cuda(), p, seed, step, residual=r.cuda()), want, off)
+
+
+def test_dropout_uses_the_samplers_stream():
+    import nextdoor_amd as nd
+    n, seed, step = 10007, 42, 3
+    kept = nd.philox_fill_uniform(seed, step, 0, n, 1, step_size=2)[:, 0] >= np.float32(0.3)
+    got = ops.dropout_forward(torch.ones(n, device="cuda"), 0.3, seed, step).cpu().numpy()
+    assert np.array_equal(got != 0, kept)
+
+
+def test_dropout_drops_whatever_is_there_and_reads_odd_places():
+    x = normal(1, 4001, dtype=F32).cuda()
+    kept = ops.dropout_forward(torch.ones_like(x), 0.5, 1, 1) != 0
+    bad = torch.where(kept, x, torch.full_like(x, math.nan))
+    assert torch.equal(ops.dropout_forward(bad, 0.5, 1, 1), ops.dropout_forward(x, 0.5, 1, 1))
+    for dtype in (F32, BF16):
+        y = x.to(dtype)
+        assert torch.equal(ops.dropout_forward(y[1:], 0.5, 1, 1), ops.dropout_forward(y[1:].clone(), 0.5, 1, 1))
+        m = y[:4000].view(50, 80)
+        assert torch.equal(ops.dropout_forward(m.T, 0.5, 1, 1), ops.dropout_forward(m.T.contiguous(), 0.5, 1, 1))
+
+
+def test_dropout_gradients():
+    x = normal(1, 77, 33, dtype=F32).cuda().requires_grad_()
+    r = normal(2, 77, 33, dtype=F32).cuda().requires_grad_()
+    d = normal(3, 77, 33, dtype=F32).cuda()
+    ops.dropout(x, 0.2, 9, 5, r).backward(d)
+    want, off = ref.dropout(d.cpu(), 0.2, 9, 5)
+    assert ref.close(x.grad, want, off) and torch.equal(r.grad, d)
+
+
+def test_dropout_refuses():
+    x = torch.ones(8, device="cuda")
+    for args in ((x, -0.1, 1, 1), (x, 1.5, 1, 1), (x, math.nan, 1, 1), (x, 0.5, -1, 1), (x, 0.5, 1 << 64, 1), (x, 0.5, 1, 1 << 31),
+                 (x.double(), 0.5, 1, 1), (x.cpu(), 0.5, 1, 1), (x, 0.5, 1, 1, x[:7]), (x, 0.5, 1, 1, x.half())):
+        with pytest.raises(NextDoorError):
+            ops.dropout_forward(*args)
+    assert ops.dropout_forward(x[:0], 0.5, 1, 1).shape == (0,)
