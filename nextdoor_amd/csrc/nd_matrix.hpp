@@ -76,12 +76,12 @@ __device__ __forceinline__ u32x4 pack_operand(const f32x16& c, int s) {
 }
 
 // ---- LDS tiles ----------------------------------------------------------------------------------
-// A tile is rows of CHUNKS 16-byte chunks (4, 8 or 16: 64, 128 or 256 bytes).  Chunk c of row r is kept at
+// A tile is rows of CHUNKS 16-byte chunks (4, 8, 16 or 32: 64 to 512 bytes).  Chunk c of row r is kept at
 // place c ^ tile_swizzle(r): sixteen consecutive rows read at one chunk (an operand by rows) and the 64 bytes of
 // four consecutive rows (an operand by columns) then both lie in different banks.
 template <int CHUNKS>
 __device__ __forceinline__ constexpr int tile_swizzle(int r) {
-  return CHUNKS == 16  ? ((r & 3) << 2) | ((r >> 2) & 3)
+  return CHUNKS >= 16  ? ((r & 3) << 2) | ((r >> 2) & 3)
          : CHUNKS == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3)
                        : (r >> 2) & 3;
 }
@@ -118,6 +118,37 @@ __device__ __forceinline__ u32x4 read_operand_by_columns(const u32x4* tile, int 
 template <int CHUNKS>
 __device__ __forceinline__ u32x4 read_operand_by_rows(const u32x4* tile, int row, int s, int lane) {
   return tile[tile_place<CHUNKS>(row + (lane & 31), 2 * s + (lane >> 5))];
+}
+
+// ---- loads straight to LDS --------------------------------------------------------------------------
+// Each lane's 16 bytes at base + offset go to `lds` + 16 * lane (an LDS address, the same for the wave).  Written as a
+// statement of its own and not with the builtin: the compiler makes every read of LDS wait for all loads to LDS that it
+// knows of, also those of the other half of a double buffer, which are to stay in flight.  Nothing is returned in
+// registers; wait_for_loads() and a barrier stand between the load and whoever reads the tile.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is reserved; it is set and used in here only)
+__device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// A value that is the same for the whole wave, in a scalar register (what divisions leave is not).
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  typedef __attribute__((address_space(3))) const void lds_void;
+  return (uint32_t)(uintptr_t)(lds_void*)p;
+}
+// Loads and LDS writes of this wave have arrived; then all waves'.
+__device__ __forceinline__ void wait_for_loads_and_others() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The block's index such that blocks with neighbouring results run on one of the eight dies, whose L2 they share:
+// consecutive workgroups go to the dies in turn.
+__device__ __forceinline__ uint32_t block_by_die() {
+  const uint32_t n = gridDim.x, die = blockIdx.x % 8, turn = blockIdx.x / 8;
+  return die * (n / 8) + min(die, n % 8) + turn;
 }
 
 // Over the two lanes 32 apart.

@@ -21,9 +21,8 @@ namespace nd {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kTile = 128;             // rows and columns of a workgroup's product: four waves of 64 x 64
-constexpr int kDepth = 64;             // places of the sum per round
 constexpr float kGradientOne = 32768.f;  // what |g| = max |dloss| is held as (below the largest 16-bit float)
+constexpr int kClassPad = 256;           // a piece of the vocabulary is filled up to a multiple of it
 
 struct LossParams {
   const void *hidden, *weight;
@@ -33,13 +32,15 @@ struct LossParams {
   void *dhidden, *dweight;
   int32_t rows, classes, dim;
   // workspace
-  float2* partials;   // forward: (maximum, sum) of a row over 64 classes, in powers of two; [part][row]
-  u32x4* gradient;    // backward: g of one piece of the vocabulary, see gradient_place
-  float* dhidden_sum; // [rows][dim], if there is more than one piece
-  float* largest;     // max |dloss|
-  void* hidden_known; // hidden, the rows without a target zero
-  int32_t row_blocks; // of 32 rows, a multiple of 4
+  float2* partials;    // forward: (maximum, sum) of a row over one wave's classes, in powers of two; [part][row]
+  u32x4* gradient;     // backward: g of one piece of the vocabulary, see gradient_place
+  float* dhidden_sums; // [split][rows][dim]
+  float* dweight_sums; // [split][classes of the piece][dim]
+  float* largest;      // max |dloss|
+  void* hidden_known;  // hidden, filled up to padded_rows; rows without a target are zero
+  int32_t padded_rows;
   int32_t class0, class_end;  // the piece
+  int32_t dhidden_split, dweight_split;
 };
 
 // g of 32 rows x 32 classes is kept as it leaves the product that made it, ready to be an operand (PAIRED order over the
@@ -47,90 +48,149 @@ struct LossParams {
 // 16 bytes.  The rows are permuted so that reads by columns meet different banks.
 __device__ __forceinline__ int gradient_place(int r, int s, int h) { return s * 64 + h * 32 + (r ^ ((h | 2 * s) << 2)); }
 constexpr int kGradientBlock = 128;  // 16-byte chunks of 32 rows x 32 classes
+constexpr int kGradientBlockBytes = kGradientBlock * 16;
 
-// ---- operands of a round of 64 places, 128 rows ----------------------------------------------------
+// ---- the shape of a workgroup's product -------------------------------------------------------------
+// kWavesM x kWavesN waves, each with kM x kN results of 32 x 32, kDepth places of the sum per round.
+template <int WAVES_M, int WAVES_N, int M, int N, int DEPTH>
+struct Shape {
+  static constexpr int kWavesM = WAVES_M, kWavesN = WAVES_N, kM = M, kN = N, kDepth = DEPTH;
+  static constexpr int kThreads = 64 * WAVES_M * WAVES_N;
+  static constexpr int kTileM = 32 * WAVES_M * M, kTileN = 32 * WAVES_N * N;
+};
+
+// ---- operands: ROWS rows, DEPTH places of the sum a round, brought to LDS by THREADS threads --------------
+// issue() asks for the tile of a round, operand() reads 32 rows x 16 places of it.  What lies past the last place is 0 in
+// one of the two operands and some value of the same array in the other; what lies past the last row is some row.
 
 // A matrix whose rows are the operand's rows: [row][place].
+template <int ROWS, int DEPTH, int THREADS>
 struct ByRows {
+  static constexpr int kRowChunks = DEPTH / 8, kChunks = ROWS * kRowChunks, kTurns = kChunks / THREADS;
+  static_assert(kChunks % THREADS == 0, "");
   const char* base;
-  int64_t row_bytes;
-  int row0, row_end, places;
-  static constexpr int kChunks = kTile * kDepth / 8;
-  __device__ __forceinline__ void load(u32x4* tile, int place0) const {
+  uint32_t offset[kTurns];
+  int places, chunk;
+  __device__ __forceinline__ ByRows(const void* matrix, int64_t row_bytes, int row0, int row_end, int places_)
+      : base((const char*)matrix + row0 * row_bytes), places(places_) {
 #pragma unroll
-    for (int i = 0; i < kChunks / 256; ++i) {
-      const int at = threadIdx.x + 256 * i, r = at / 8, c = at % 8;
-      u32x4 v = {0, 0, 0, 0};
-      if (row0 + r < row_end && place0 + c * 8 < places)
-        v = *(const u32x4*)(base + (int64_t)(row0 + r) * row_bytes + (int64_t)(place0 + c * 8) * 2);
-      tile[tile_place<8>(r, c)] = v;
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = threadIdx.x + THREADS * i, r = at / kRowChunks, c = (at % kRowChunks) ^ tile_swizzle<kRowChunks>(r);
+      offset[i] = (uint32_t)(min(r, row_end - 1 - row0) * row_bytes + c * 16);
+      chunk = c;  // (the same in every turn: THREADS / kRowChunks is a multiple of 16 rows)
+    }
+  }
+  __device__ __forceinline__ void issue(u32x4* tile, uint32_t wave_lds, int place0) const {
+    const char* at = base + (int64_t)place0 * 2;
+    if (place0 + DEPTH <= places) {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) load_to_lds(at, offset[i], wave_lds + THREADS * 16 * i);
+    } else {
+      const bool there = place0 + chunk * 8 < places;
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        if (there) load_to_lds(at, offset[i], wave_lds + THREADS * 16 * i);
+        else tile[threadIdx.x + THREADS * i] = u32x4{0, 0, 0, 0};
+      }
     }
   }
   template <bool PAIRED>
   __device__ __forceinline__ static u32x4 operand(const u32x4* tile, int row, int s, int lane) {
     static_assert(!PAIRED, "read by rows only in the plain order");
-    return read_operand_by_rows<8>(tile, row, s, lane);
+    return read_operand_by_rows<kRowChunks>(tile, row, s, lane);
   }
 };
 
 // A matrix whose rows are the places: [place][row].
+template <int ROWS, int DEPTH, int THREADS>
 struct ByColumns {
+  static constexpr int kRowChunks = ROWS / 8, kChunks = DEPTH * kRowChunks, kTurns = kChunks / THREADS;
+  static_assert(kChunks % THREADS == 0, "");
   const char* base;
   int64_t row_bytes;
-  int row0, row_end, places;
-  static constexpr int kChunks = kTile * kDepth / 8;
-  __device__ __forceinline__ void load(u32x4* tile, int place0) const {
+  uint32_t offset[kTurns];
+  int places;
+  __device__ __forceinline__ ByColumns(const void* matrix, int64_t row_bytes_, int row0, int row_end, int places_)
+      : base((const char*)matrix + (int64_t)row0 * 2), row_bytes(row_bytes_), places(places_) {
 #pragma unroll
-    for (int i = 0; i < kChunks / 256; ++i) {
-      const int at = threadIdx.x + 256 * i, r = at / 16, c = at % 16;
-      u32x4 v = {0, 0, 0, 0};
-      if (place0 + r < places && row0 + c * 8 < row_end)
-        v = *(const u32x4*)(base + (int64_t)(place0 + r) * row_bytes + (int64_t)(row0 + c * 8) * 2);
-      tile[tile_place<16>(r, c)] = v;
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = threadIdx.x + THREADS * i, r = at / kRowChunks, c = (at % kRowChunks) ^ tile_swizzle<kRowChunks>(r);
+      offset[i] = (uint32_t)(r * row_bytes) + (row0 + c * 8 < row_end ? c * 16 : 0);
+    }
+  }
+  __device__ __forceinline__ void issue(u32x4*, uint32_t wave_lds, int place0) const {
+    const char* at = base + place0 * row_bytes;
+    if (place0 + DEPTH <= places) {
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) load_to_lds(at, offset[i], wave_lds + THREADS * 16 * i);
+    } else {  // rows past the last place: the last one (the other operand is 0 there)
+#pragma unroll
+      for (int i = 0; i < kTurns; ++i) {
+        const int r = (threadIdx.x + THREADS * i) / kRowChunks, past = max(place0 + r - (places - 1), 0);
+        load_to_lds(at, offset[i] - (uint32_t)(past * row_bytes), wave_lds + THREADS * 16 * i);
+      }
     }
   }
   template <bool PAIRED>
   __device__ __forceinline__ static u32x4 operand(const u32x4* tile, int row, int s, int lane) {
-    return read_operand_by_columns<16, PAIRED>(tile, 16 * s, row, lane);
+    return read_operand_by_columns<kRowChunks, PAIRED>(tile, 16 * s, row, lane);
   }
 };
 
 // g with the rows of the loss as rows, places = classes of the piece.
+template <int ROWS, int DEPTH, int THREADS>
 struct GradientByRows {
-  const u32x4* base;
-  int row_blocks, row0;
-  static constexpr int kChunks = kTile * kDepth / 8;
-  __device__ __forceinline__ void load(u32x4* tile, int place0) const {
+  static constexpr int kChunks = ROWS * DEPTH / 8, kTurns = kChunks / THREADS, kBlocks = ROWS / 32;
+  static_assert(kChunks % THREADS == 0, "");
+  const char* base;
+  int64_t step;
+  uint32_t offset[kTurns];
+  __device__ __forceinline__ GradientByRows(const u32x4* gradient, int padded_rows, int row0)
+      : base((const char*)gradient + (int64_t)(row0 / 32) * kGradientBlockBytes), step((int64_t)(padded_rows / 32) * kGradientBlockBytes) {
 #pragma unroll
-    for (int i = 0; i < kChunks / 256; ++i) {
-      const int at = threadIdx.x + 256 * i, vb = at / (4 * kGradientBlock);
-      tile[at] = base[((int64_t)(place0 / 32 + vb) * row_blocks + row0 / 32) * kGradientBlock + at % (4 * kGradientBlock)];
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = threadIdx.x + THREADS * i;
+      offset[i] = (uint32_t)(at / (kBlocks * kGradientBlock) * step) + at % (kBlocks * kGradientBlock) * 16;
     }
+  }
+  __device__ __forceinline__ void issue(u32x4*, uint32_t wave_lds, int place0) const {
+    const char* at = base + place0 / 32 * step;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) load_to_lds(at, offset[i], wave_lds + THREADS * 16 * i);
   }
   template <bool PAIRED>
   __device__ __forceinline__ static u32x4 operand(const u32x4* tile, int row, int s, int lane) {
     static_assert(PAIRED, "kept in the paired order");
-    return tile[((s >> 1) * 4 + row / 32) * kGradientBlock + gradient_place(lane & 31, s & 1, lane >> 5)];
+    return tile[((s >> 1) * kBlocks + row / 32) * kGradientBlock + gradient_place(lane & 31, s & 1, lane >> 5)];
   }
 };
 
 // g with the classes of the piece as rows, places = rows of the loss.
+template <int ROWS, int DEPTH, int THREADS>
 struct GradientByColumns {
-  const u32x4* base;
-  int row_blocks, row0;
-  static constexpr int kChunks = kTile * kDepth / 8;
-  __device__ __forceinline__ void load(u32x4* tile, int place0) const {
+  static constexpr int kChunks = ROWS * DEPTH / 8, kTurns = kChunks / THREADS, kBlocks = DEPTH / 32;
+  static_assert(kChunks % THREADS == 0, "");
+  const char* base;
+  uint32_t offset[kTurns];
+  __device__ __forceinline__ GradientByColumns(const u32x4* gradient, int padded_rows, int class0) {
+    const int64_t step = (int64_t)(padded_rows / 32) * kGradientBlockBytes;
+    base = (const char*)gradient + class0 / 32 * step;
 #pragma unroll
-    for (int i = 0; i < kChunks / 256; ++i) {
-      const int at = threadIdx.x + 256 * i, vb = at / (2 * kGradientBlock);
-      tile[at] = base[((int64_t)(row0 / 32 + vb) * row_blocks + place0 / 32) * kGradientBlock + at % (2 * kGradientBlock)];
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = threadIdx.x + THREADS * i;
+      offset[i] = (uint32_t)(at / (kBlocks * kGradientBlock) * step) + at % (kBlocks * kGradientBlock) * 16;
     }
+  }
+  __device__ __forceinline__ void issue(u32x4*, uint32_t wave_lds, int place0) const {
+    const char* at = base + (int64_t)(place0 / 32) * kGradientBlockBytes;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) load_to_lds(at, offset[i], wave_lds + THREADS * 16 * i);
   }
   template <bool PAIRED>
   __device__ __forceinline__ static u32x4 operand(const u32x4* tile, int row, int s, int lane) {
     static_assert(!PAIRED, "read in the plain order");
     const int h = lane >> 5, at = (lane & 15) >> 2, slice = (lane >> 4) & 1, hh = lane & 1, upper = (lane >> 1) & 1;
-    const u32x4* block = tile + ((row / 32) * 2 + (s >> 1)) * kGradientBlock;
+    const u32x4* block = tile + ((row / 32) * kBlocks + (s >> 1)) * kGradientBlock;
     const int r = 16 * (s & 1) + 8 * h + at;
     const u32x2 a = read_columns((const char*)(block + gradient_place(r, slice, hh)) + upper * 8);
     const u32x2 b = read_columns((const char*)(block + gradient_place(r + 4, slice, hh)) + upper * 8);
@@ -143,69 +203,92 @@ struct GradientByColumns {
   }
 };
 
-// acc += A B^T over all places; a wave has rows 64 * (wave / 2) of A and 64 * (wave % 2) of B.
-template <class T, bool PAIRED, class A, class B>
-__device__ __forceinline__ void multiply(f32x16 (&acc)[2][2], const A& a, const B& b, int places, u32x4* tile_a, u32x4* tile_b) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int k = 0; k < places; k += kDepth) {
-    __syncthreads();
-    a.load(tile_a, k);
-    b.load(tile_b, k);
-    __syncthreads();
+// acc += A B^T over the places place0 .. place_end - 1: while the matrix cores work on one tile the next is on its way to
+// the other half of LDS.  One barrier a round: at it, this round's tile has arrived for all and the last one's is free.
+// tiles: twice a round's tiles of LDS, which the caller may use again after a barrier.
+template <class A, class B>
+constexpr int kTileChunks = 2 * (A::kChunks + B::kChunks);
+template <class T, class S, bool PAIRED, class A, class B>
+__device__ __forceinline__ void multiply(f32x16 (&acc)[S::kM][S::kN], const A& a, const B& b, int place0, int place_end, u32x4* tiles) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = wave / S::kWavesN * 32 * S::kM, n0 = wave % S::kWavesN * 32 * S::kN;
 #pragma unroll
-    for (int s = 0; s < kDepth / 16; ++s) {
-      u32x4 fa[2], fb[2];
+  for (int i = 0; i < S::kM; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = A::template operand<PAIRED>(tile_a, 64 * (wave >> 1) + 32 * i, s, lane);
-        fb[i] = B::template operand<PAIRED>(tile_b, 64 * (wave & 1) + 32 * i, s, lane);
-      }
+    for (int j = 0; j < S::kN; ++j) acc[i][j] = f32x16{};
+  const uint32_t lds = lds_address(tiles) + wave * 1024;
+  constexpr int kHalf = A::kChunks + B::kChunks;
+  int half = 0;
+  auto issue = [&](int into, int place) {
+    a.issue(tiles + into * kHalf, lds + into * kHalf * 16, place);
+    b.issue(tiles + into * kHalf + A::kChunks, lds + (into * kHalf + A::kChunks) * 16, place);
+  };
+  if (place0 < place_end) issue(0, place0);
+  for (int place = place0; place < place_end; place += S::kDepth) {
+    wait_for_loads_and_others();
+    if (place + S::kDepth < place_end) issue(half ^ 1, place + S::kDepth);
+    const u32x4 *tile_a = tiles + half * kHalf, *tile_b = tile_a + A::kChunks;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+    for (int s = 0; s < S::kDepth / 16; ++s) {
+      u32x4 fa[S::kM], fb[S::kN];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = product_32x32x16<T>(fa[i], fb[j], acc[i][j]);
+      for (int j = 0; j < S::kN; ++j) fb[j] = B::template operand<PAIRED>(tile_b, n0 + 32 * j, s, lane);
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i) fa[i] = A::template operand<PAIRED>(tile_a, m0 + 32 * i, s, lane);
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kN; ++j) acc[i][j] = product_32x32x16<T>(fa[i], fb[j], acc[i][j]);
     }
+    half ^= 1;
   }
 }
 
 // ---- Z^T = W H^T ----------------------------------------------------------------------------------
 // Rows of the result are classes and lie in a lane's registers, its column is the lane's row of the loss: the softmax over
 // classes is mostly a lane's own.  BACKWARD: g instead of the maxima and sums.
-template <class T, bool BACKWARD>
-__global__ __launch_bounds__(256) void logits_kernel(LossParams p) {
-  __shared__ u32x4 tile_a[ByRows::kChunks], tile_b[ByRows::kChunks];
+template <class T, class S, bool BACKWARD>
+__global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, int row_tiles) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int class0 = p.class0 + blockIdx.x * kTile, row0 = blockIdx.y * kTile;
+  const uint32_t block = block_by_die();
+  const int class_tile = uniform(block / row_tiles), class0 = p.class0 + class_tile * S::kTileM;
+  const int row0 = uniform(block % row_tiles) * S::kTileN;
   const int64_t row_bytes = (int64_t)p.dim * 2;
-  f32x16 z[2][2];
+  using Classes = ByRows<S::kTileM, S::kDepth, S::kThreads>;
+  using Rows = ByRows<S::kTileN, S::kDepth, S::kThreads>;
+  __shared__ u32x4 tiles[kTileChunks<Classes, Rows>];
+  f32x16 z[S::kM][S::kN];
+  // (a tile of nothing but the piece's filling has no class to read: it reads the last one, and g is 0)
+  multiply<T, S, false>(z, Classes(p.weight, row_bytes, min(class0, p.class_end - 1), p.class_end, p.dim),
+                        Rows(p.hidden, row_bytes, row0, p.rows, p.dim), 0, p.dim, tiles);
+  const int wave_class0 = class0 + wave / S::kWavesN * 32 * S::kM;
+  const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN;
+  const bool whole = wave_class0 + 32 * S::kM <= p.class_end;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) z[i][j] = f32x16{};
-  multiply<T, false>(z, ByRows{(const char*)p.weight, row_bytes, class0, p.class_end, p.dim},
-                     ByRows{(const char*)p.hidden, row_bytes, row0, p.rows, p.dim}, p.dim, tile_a, tile_b);
-  const int wave_class0 = class0 + 64 * (wave >> 1);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int row = row0 + 64 * (wave & 1) + 32 * j + (lane & 31);
+  for (int j = 0; j < S::kN; ++j) {
+    const int row = wave_row0 + 32 * j + (lane & 31);
     if (!BACKWARD) {
       float m = -INFINITY;
+      if (!whole) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < S::kM; ++i)
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          const int c = wave_class0 + 32 * i + 8 * (n / 4) + 4 * h + n % 4;
-          z[i][j][n] = c < p.class_end ? z[i][j][n] : -INFINITY;
-          m = fmaxf(m, z[i][j][n]);
-        }
+          for (int n = 0; n < 16; ++n)
+            if (wave_class0 + 32 * i + 8 * (n / 4) + 4 * h + n % 4 >= p.class_end) z[i][j][n] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) m = fmaxf(m, z[i][j][n]);
       const float m2 = pair_max(m) * kLog2e, base = m2 == -INFINITY ? 0.f : m2;
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::kM; ++i)
 #pragma unroll
         for (int n = 0; n < 16; ++n) sum += exp2_fast(__builtin_fmaf(z[i][j][n], kLog2e, -base));
       sum = pair_sum(sum);
-      if (h == 0 && row < p.rows) p.partials[((int64_t)blockIdx.x * 2 + (wave >> 1)) * p.rows + row] = make_float2(m2, sum);
+      if (h == 0 && row < p.rows)
+        p.partials[((int64_t)class_tile * S::kWavesM + wave / S::kWavesN) * p.rows + row] = make_float2(m2, sum);
     } else {
       const bool there = row < p.rows;
       const int target = there ? p.target[row] : -1;
@@ -214,215 +297,354 @@ __global__ __launch_bounds__(256) void logits_kernel(LossParams p) {
       const float each = has && largest > 0.f ? p.dloss[row] / largest * kGradientOne : 0.f;
       const float lse2 = there ? p.lse[row] * kLog2e : 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < S::kM; ++i) {
+        const int c0 = wave_class0 + 32 * i + 4 * h;
         f32x16 g;
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
-          const int c = wave_class0 + 32 * i + 8 * (n / 4) + 4 * h + n % 4;
+          const int c = c0 + 8 * (n / 4) + n % 4;
           float v = exp2_fast(__builtin_fmaf(z[i][j][n], kLog2e, -lse2));
           if (c == target) v -= 1.f;
           g[n] = has && c < p.class_end ? v * each : 0.f;
         }
-        const int64_t block = (int64_t)((wave_class0 - p.class0) / 32 + i) * p.row_blocks + (row - (lane & 31)) / 32;
+        const int64_t at = (int64_t)((wave_class0 - p.class0) / 32 + i) * (p.padded_rows / 32) + (row - (lane & 31)) / 32;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-          p.gradient[block * kGradientBlock + gradient_place(lane & 31, s, h)] = pack_operand<T>(g, s);
+        for (int s = 0; s < 2; ++s) p.gradient[at * kGradientBlock + gradient_place(lane & 31, s, h)] = pack_operand<T>(g, s);
       }
     }
   }
 }
 
-// Joins the maxima and sums of 64 rows; loss = lse - z of the target, its logit from the vectors themselves.
+// Joins two (maximum, sum) pairs, in powers of two.
+__device__ __forceinline__ void join(float2& a, float2 b) {
+  const float top = fmaxf(a.x, b.x), base = top == -INFINITY ? 0.f : top;
+  a.y = a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base);
+  a.x = top;
+}
+
+// Joins the maxima and sums of 8 rows; loss = lse - z of the target, its logit from the vectors themselves.  A row's parts
+// are shared out among 128 lanes: there may be very many (a row of a vocabulary of millions) and few rows.
 template <class T>
-__global__ __launch_bounds__(256) void join_kernel(LossParams p, int parts) {
-  __shared__ float2 partial[4][64];
-  __shared__ float lses[64];
+__global__ __launch_bounds__(1024) void join_kernel(LossParams p, int parts) {
+  __shared__ float2 partial[16][8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row0 = blockIdx.x * 64, row = row0 + lane;
-  float m = -INFINITY, sum = 0.f;
-  if (row < p.rows)
-    for (int i = wave; i < parts; i += 4) {
-      const float2 one = p.partials[(int64_t)i * p.rows + row];
-      const float top = fmaxf(m, one.x), base = top == -INFINITY ? 0.f : top;
-      sum = sum * exp2_fast(m - base) + one.y * exp2_fast(one.x - base);
-      m = top;
-    }
-  partial[wave][lane] = make_float2(m, sum);
-  __syncthreads();
-  if (wave == 0) {
-    for (int i = 1; i < 4; ++i) {
-      const float2 one = partial[i][lane];
-      const float top = fmaxf(m, one.x), base = top == -INFINITY ? 0.f : top;
-      sum = sum * exp2_fast(m - base) + one.y * exp2_fast(one.x - base);
-      m = top;
-    }
-    lses[lane] = (m + log2f(sum)) * kLn2;
-    if (row < p.rows) p.lse[row] = lses[lane];
-  }
-  __syncthreads();
-  for (int i = wave; i < 64 && row0 + i < p.rows; i += 4) {
-    const int target = p.target[row0 + i];
-    const bool has = target >= 0 && target < p.classes;
-    float z = 0.f;
-    if (has) {
-      const u32x4* a = (const u32x4*)((const char*)p.hidden + (int64_t)(row0 + i) * p.dim * 2);
-      const u32x4* b = (const u32x4*)((const char*)p.weight + (int64_t)target * p.dim * 2);
-      for (int c = lane; c < p.dim / 8; c += 64) {
-        const u32x4 x = a[c], y = b[c];
+  const int row0 = blockIdx.x * 8, mine = row0 + (lane & 7);
+  float2 all = make_float2(-INFINITY, 0.f);
+  if (mine < p.rows) {
+    const float2* from = p.partials + mine;
+    int i = threadIdx.x >> 3;
+    for (; i + 3 * 128 < parts; i += 4 * 128) {
+      float2 four[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          z = __builtin_fmaf(unpack_low<T>(x[n]), unpack_low<T>(y[n]), z);
-          z = __builtin_fmaf(unpack_high<T>(x[n]), unpack_high<T>(y[n]), z);
-        }
+      for (int j = 0; j < 4; ++j) four[j] = from[(int64_t)(i + 128 * j) * p.rows];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) join(all, four[j]);
+    }
+    for (; i < parts; i += 128) join(all, from[(int64_t)i * p.rows]);
+  }
+#pragma unroll
+  for (int d = 8; d < 64; d *= 2) join(all, make_float2(__shfl_xor(all.x, d), __shfl_xor(all.y, d)));
+  if (lane < 8) partial[wave][lane] = all;
+  __syncthreads();
+  const int row = row0 + wave;
+  if (wave >= 8 || row >= p.rows) return;
+  all = partial[0][wave];
+  for (int i = 1; i < 16; ++i) join(all, partial[i][wave]);
+  const float lse = (all.x + log2f(all.y)) * kLn2;
+  const int target = p.target[row];
+  const bool has = target >= 0 && target < p.classes;
+  float z = 0.f;
+  if (has) {
+    const u32x4* a = (const u32x4*)((const char*)p.hidden + (int64_t)row * p.dim * 2);
+    const u32x4* b = (const u32x4*)((const char*)p.weight + (int64_t)target * p.dim * 2);
+    for (int c = lane; c < p.dim / 8; c += 64) {
+      const u32x4 x = a[c], y = b[c];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        z = __builtin_fmaf(unpack_low<T>(x[n]), unpack_low<T>(y[n]), z);
+        z = __builtin_fmaf(unpack_high<T>(x[n]), unpack_high<T>(y[n]), z);
       }
     }
+  }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) z += __shfl_xor(z, d);
-    if (lane == 0) p.loss[row0 + i] = has ? lses[i] - z : 0.f;
+  for (int d = 1; d < 64; d *= 2) z += __shfl_xor(z, d);
+  if (lane == 0) {
+    p.lse[row] = lse;
+    p.loss[row] = has ? lse - z : 0.f;
   }
 }
 
-// max |dloss|: g is held relative to it, so that 16-bit floats hold the gradient of a mean over any number of rows.
-__global__ __launch_bounds__(1024) void largest_kernel(LossParams p) {
-  __shared__ float tops[16];
-  float m = 0.f;
-  for (int i = threadIdx.x; i < p.rows; i += 1024) if (p.target[i] >= 0 && p.target[i] < p.classes) m = fmaxf(m, fabsf(p.dloss[i]));
+// Before the backward products.  First workgroup: max |dloss|; g is held relative to it, so that 16-bit floats hold the
+// gradient of a mean over any number of rows.  The others: hidden, filled up with rows of zeros and with zeros for the
+// rows without a target: such a row sends nothing to dw, whatever it holds (0 x NaN would be NaN).
+__global__ __launch_bounds__(1024) void prepare_kernel(LossParams p) {
+  if (blockIdx.x == 0) {
+    __shared__ float tops[16];
+    float m = 0.f;
+    for (int i = threadIdx.x; i < p.rows; i += 1024)
+      if (p.target[i] >= 0 && p.target[i] < p.classes) {
+        const float d = fabsf(p.dloss[i]);
+        m = d > m || d != d ? d : m;
+      }
 #pragma unroll
-  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
-    *p.largest = m;
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
+      *p.largest = m;
+    }
+    return;
   }
-}
-
-// A row without a target sends nothing to dw, whatever it holds: 0 x NaN would be NaN.
-__global__ __launch_bounds__(256) void known_rows_kernel(LossParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x;
   const int chunks = p.dim / 8;
-  if (i >= (int64_t)p.rows * chunks) return;
-  const int target = p.target[i / chunks];
+  if (i >= (int64_t)p.padded_rows * chunks) return;
+  const int row = (int)(i / chunks), target = row < p.rows ? p.target[row] : -1;
   u32x4 v = {0, 0, 0, 0};
   if (target >= 0 && target < p.classes) v = ((const u32x4*)p.hidden)[i];
   ((u32x4*)p.hidden_known)[i] = v;
 }
 
-// dh of the piece: a row of the result is a row of the loss, its column (the lane's) a column of the vectors.
-template <class T>
-__global__ __launch_bounds__(256) void dhidden_kernel(LossParams p) {
-  __shared__ u32x4 tile_a[GradientByRows::kChunks], tile_b[ByColumns::kChunks];
+// What a workgroup of the two products below leaves.  Result rows are columns of the vectors and lie in a lane's
+// registers, four next to each other at a time; the result's column is the lane's row of the output.
+// A sum of its own among several, in 32 bits:
+template <class S>
+__device__ __forceinline__ void store_sums(const f32x16 (&acc)[S::kM][S::kN], float factor, float* sums, bool add, int row0, int row_end,
+                                           int column0, int columns) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int column0 = blockIdx.x * kTile, row0 = blockIdx.y * kTile, classes = p.class_end - p.class0;
-  f32x16 acc[2][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < S::kN; ++j) {
+    const int row = row0 + 32 * (wave % S::kWavesN * S::kN + j) + (lane & 31);
+    if (row >= row_end) continue;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-  multiply<T, true>(acc, GradientByRows{p.gradient, p.row_blocks, row0},
-                    ByColumns{(const char*)p.weight + (int64_t)p.class0 * p.dim * 2, (int64_t)p.dim * 2, column0, p.dim, classes},
-                    classes, tile_a, tile_b);
-  const float factor = *p.largest / kGradientOne;
-  const bool first = p.class0 == 0, last = p.class_end == p.classes;
+    for (int i = 0; i < S::kM; ++i)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+      for (int g = 0; g < 4; ++g) {
+        const int column = column0 + 32 * (wave / S::kWavesN * S::kM + i) + 8 * g + 4 * h;
+        if (column >= columns) continue;
+        f32x4* at = (f32x4*)(sums + (int64_t)row * columns + column);
+        f32x4 v;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int column = column0 + 64 * (wave & 1) + 32 * j + (lane & 31);
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        const int row = row0 + 64 * (wave >> 1) + 32 * i + 8 * (n / 4) + 4 * h + n % 4;
-        if (row >= p.rows || column >= p.dim) continue;
-        const int64_t at = (int64_t)row * p.dim + column;
-        const float sum = acc[i][j][n] * factor + (first ? 0.f : p.dhidden_sum[at]);
-        if (last) ((T*)p.dhidden)[at] = (T)sum;
-        else p.dhidden_sum[at] = sum;
+        for (int n = 0; n < 4; ++n) v[n] = acc[i][j][4 * g + n] * factor;
+        *at = add ? v + *at : v;
       }
+  }
+}
+// The result itself: rounded, turned through the wave's own part of LDS and stored 16 bytes a lane, whole rows of
+// 32 * kM columns side by side (stored from the registers as they are, 64 bytes side by side, this took twice as long).
+template <class T, class S>
+__device__ __forceinline__ void store_result(const f32x16 (&acc)[S::kM][S::kN], float factor, T* out, int row0, int row_end, int column0,
+                                             int columns, u32x4* tiles) {
+  constexpr int kRowChunks = 4 * S::kM;  // of a row in the wave's part
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  u32x4* part = tiles + wave * 32 * kRowChunks;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < S::kN; ++j) {
+    const int r = lane & 31, first = row0 + 32 * (wave % S::kWavesN * S::kN + j);
+#pragma unroll
+    for (int i = 0; i < S::kM; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        u32x2 v;
+        v[0] = pack_pair<T>(acc[i][j][4 * g] * factor, acc[i][j][4 * g + 1] * factor);
+        v[1] = pack_pair<T>(acc[i][j][4 * g + 2] * factor, acc[i][j][4 * g + 3] * factor);
+        ((u32x2*)(part + r * kRowChunks + ((4 * i + g) ^ (r & (kRowChunks - 1)))))[h] = v;
+      }
+    // (one wave's LDS operations are done in order: no barrier between its own writes and reads)
+#pragma unroll
+    for (int n = 0; n < kRowChunks / 2; ++n) {
+      const int at = lane + 64 * n, rr = at / kRowChunks, c = at % kRowChunks;
+      const u32x4 v = part[rr * kRowChunks + (c ^ (rr & (kRowChunks - 1)))];
+      const int row = first + rr, column = column0 + 32 * (wave / S::kWavesN * S::kM) + 8 * c;
+      if (row < row_end && column < columns) *(u32x4*)(out + (int64_t)row * columns + column) = v;
     }
+  }
 }
 
-// dw of the piece's classes, whole at once.
-template <class T>
-__global__ __launch_bounds__(256) void dweight_kernel(LossParams p) {
-  __shared__ u32x4 tile_a[GradientByColumns::kChunks], tile_b[ByColumns::kChunks];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int column0 = blockIdx.x * kTile, class0 = blockIdx.y * kTile;  // in the piece
-  f32x16 acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
-  multiply<T, false>(acc, GradientByColumns{p.gradient, p.row_blocks, class0},
-                     ByColumns{(const char*)p.hidden_known, (int64_t)p.dim * 2, column0, p.dim, p.rows}, p.rows, tile_a, tile_b);
+// The share `i` of `n` in a sum over `places`, in whole rounds.
+__device__ __forceinline__ void share_of(int places, int depth, int i, int n, int& begin, int& end) {
+  const int rounds = (places + depth - 1) / depth, each = (rounds + n - 1) / n;
+  begin = uniform(min(i * each * depth, places));
+  end = uniform(min(begin + each * depth, places));
+}
+
+// dh of the piece.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void dhidden_kernel(LossParams p, int row_tiles, int column_tiles, bool alone) {
+  using Columns = ByColumns<S::kTileM, S::kDepth, S::kThreads>;
+  using Rows = GradientByRows<S::kTileN, S::kDepth, S::kThreads>;
+  __shared__ u32x4 tiles[kTileChunks<Columns, Rows>];
+  const uint32_t block = block_by_die();
+  const int of = row_tiles * column_tiles, split = uniform(block / of), tile = uniform(block % of);
+  const int row0 = uniform(tile / column_tiles) * S::kTileN, column0 = uniform(tile % column_tiles) * S::kTileM;
+  const int classes = p.class_end - p.class0;
+  int begin, end;
+  share_of(classes, S::kDepth, split, p.dhidden_split, begin, end);
+  f32x16 acc[S::kM][S::kN];
+  multiply<T, S, true>(acc, Columns((const char*)p.weight + (int64_t)p.class0 * p.dim * 2, (int64_t)p.dim * 2, column0, p.dim, classes),
+                       Rows(p.gradient, p.padded_rows, row0), begin, end, tiles);
   const float factor = *p.largest / kGradientOne;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int column = column0 + 64 * (wave & 1) + 32 * j + (lane & 31);
-#pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        const int c = p.class0 + class0 + 64 * (wave >> 1) + 32 * i + 8 * (n / 4) + 4 * h + n % 4;
-        if (c < p.class_end && column < p.dim) ((T*)p.dweight)[(int64_t)c * p.dim + column] = (T)(acc[i][j][n] * factor);
-      }
-    }
+  if (alone) store_result<T, S>(acc, factor, (T*)p.dhidden, row0, p.rows, column0, p.dim, tiles);
+  else store_sums<S>(acc, factor, p.dhidden_sums + (int64_t)split * p.rows * p.dim, p.class0 > 0, row0, p.rows, column0, p.dim);
+}
+
+// dw of the piece's classes.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void dweight_kernel(LossParams p, int class_tiles, int column_tiles) {
+  using Columns = ByColumns<S::kTileM, S::kDepth, S::kThreads>;
+  using Classes = GradientByColumns<S::kTileN, S::kDepth, S::kThreads>;
+  __shared__ u32x4 tiles[kTileChunks<Columns, Classes>];
+  const uint32_t block = block_by_die();
+  const int of = class_tiles * column_tiles, split = uniform(block / of), tile = uniform(block % of);
+  const int class0 = uniform(tile / column_tiles) * S::kTileN, column0 = uniform(tile % column_tiles) * S::kTileM;
+  const int classes = p.class_end - p.class0;
+  int begin, end;
+  share_of(p.padded_rows, S::kDepth, split, p.dweight_split, begin, end);
+  f32x16 acc[S::kM][S::kN];
+  multiply<T, S, false>(acc, Columns(p.hidden_known, (int64_t)p.dim * 2, column0, p.dim, p.padded_rows),
+                        Classes(p.gradient, p.padded_rows, class0), begin, end, tiles);
+  const float factor = *p.largest / kGradientOne;
+  if (p.dweight_split == 1)
+    store_result<T, S>(acc, factor, (T*)p.dweight + (int64_t)p.class0 * p.dim, class0, classes, column0, p.dim, tiles);
+  else store_sums<S>(acc, factor, p.dweight_sums + (int64_t)split * classes * p.dim, false, class0, classes, column0, p.dim);
+}
+
+// out = the sum of `split` arrays of n values, n a multiple of 8: sixteen lanes share out the arrays, four values at a time.
+template <class T>
+__global__ __launch_bounds__(256) void add_sums_kernel(const float* sums, T* out, int64_t n, int split) {
+  __shared__ f32x4 partial[16][17];
+  const int at = threadIdx.x & 15, share = threadIdx.x >> 4;
+  const int64_t i = ((int64_t)blockIdx.x * 16 + at) * 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (i < n)
+    for (int s = share; s < split; s += 16) v += *(const f32x4*)(sums + s * n + i);
+  partial[share][at] = v;
+  __syncthreads();
+  if (share != 0 || i >= n) return;
+  for (int s = 1; s < min(split, 16); ++s) v += partial[s][at];
+  u32x2 o;
+  o[0] = pack_pair<T>(v[0], v[1]);
+  o[1] = pack_pair<T>(v[2], v[3]);
+  *(u32x2*)(out + i) = o;
 }
 
 // ---- host -----------------------------------------------------------------------------------------
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// Classes of a piece: g of all rows stays within 256 MiB (the last-level cache), but at least 2048 classes.
-int64_t piece_classes(int64_t rows, int64_t classes) {
-  const int64_t fit = ((int64_t)256 << 20) / (2 * round_up(std::max<int64_t>(rows, 1), kTile)) / kTile * kTile;
-  return std::min(round_up(classes, kTile), std::max<int64_t>(fit, 2048));
-}
+constexpr int kFewRows = 128;  // up to here tiles of 64 rows of the loss, beyond it tiles of 256
+constexpr int64_t kWorkgroups = 256;  // what fills the GPU, one to a compute unit
 
-struct LossWorkspace {
-  int64_t partials, gradient, dhidden_sum, largest, hidden_known, bytes;
+// How the work is cut; the workspace's parts as offsets.
+struct LossPlan {
+  int64_t padded_rows, piece, column_tiles, dhidden_split, dweight_split;
+  bool alone;  // the only sum of dh
+  int64_t partials, gradient, dhidden_sums, dweight_sums, largest, hidden_known, bytes;
 };
-LossWorkspace workspace_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
-  LossWorkspace w = {};
+
+LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
+  LossPlan w = {};
   auto take = [&](int64_t bytes) {
     const int64_t at = w.bytes;
     w.bytes += round_up(bytes, 256);
     return at;
   };
   if (!backward) {
-    w.partials = take(round_up(classes, kTile) / 64 * rows * (int64_t)sizeof(float2));
-  } else {
-    const int64_t piece = piece_classes(rows, classes);
-    w.largest = take(sizeof(float));
-    w.hidden_known = take(rows * dim * 2);
-    w.gradient = take(round_up(rows, kTile) * piece * 2);
-    if (piece < classes) w.dhidden_sum = take(rows * dim * (int64_t)sizeof(float));
+    w.partials = take(round_up(classes, kClassPad) / 64 * rows * (int64_t)sizeof(float2));
+    return w;
   }
+  const int64_t tile_rows = rows > kFewRows ? 256 : 64;
+  w.padded_rows = round_up(std::max<int64_t>(rows, 1), tile_rows);
+  const int64_t tile_columns = dim > 128 ? 256 : dim > 64 ? 128 : 64;
+  w.column_tiles = (dim + tile_columns - 1) / tile_columns;
+  // g of a piece is written once and read twice: 256 MiB (what the last-level cache holds), unless that
+  // leaves compute units without a tile of dw
+  const int64_t fit = ((int64_t)256 << 20) / (2 * w.padded_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
+  w.piece = std::min(round_up(classes, kClassPad), round_up(std::max(fit, fill), kClassPad));
+  const int64_t row_tiles = w.padded_rows / tile_rows, class_tiles = w.piece / kClassPad;
+  auto split = [](int64_t tiles, int64_t places) {  // at least four rounds to a share
+    return std::max<int64_t>(1, std::min(kWorkgroups / tiles, places / 256));
+  };
+  w.dhidden_split = split(row_tiles * w.column_tiles, w.piece);
+  w.dweight_split = split(class_tiles * w.column_tiles, w.padded_rows);
+  w.alone = w.dhidden_split == 1 && w.piece >= classes;
+  w.largest = take(sizeof(float));
+  w.hidden_known = take(w.padded_rows * dim * 2);
+  w.gradient = take(w.padded_rows * w.piece * 2);
+  if (!w.alone) w.dhidden_sums = take(w.dhidden_split * rows * dim * (int64_t)sizeof(float));
+  if (w.dweight_split > 1) w.dweight_sums = take(w.dweight_split * std::min(w.piece, classes) * dim * (int64_t)sizeof(float));
   return w;
+}
+
+template <class T, class S, bool BACKWARD>
+int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_classes, hipStream_t stream) {
+  const int64_t row_tiles = (covered_rows + S::kTileN - 1) / S::kTileN, class_tiles = (covered_classes + S::kTileM - 1) / S::kTileM;
+  logits_kernel<T, S, BACKWARD><<<(uint32_t)(row_tiles * class_tiles), S::kThreads, 0, stream>>>(p, (int)row_tiles);
+  return (int)class_tiles * S::kWavesM;
+}
+// Shapes (classes x rows): few rows leave the products bound by the reading of the class vectors; short sums (up to 256)
+// do better with two workgroups to a compute unit, one of which may be in its exponentials while the other multiplies.
+template <class T, bool BACKWARD>
+int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_classes, hipStream_t stream) {
+  if (p.rows <= kFewRows) return launch_logits<T, Shape<4, 1, 2, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
+  if (p.dim <= 256) return launch_logits<T, Shape<2, 2, 2, 4, 32>, BACKWARD>(p, covered_rows, covered_classes, stream);
+  return launch_logits<T, Shape<2, 4, 4, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
 }
 
 template <class T>
 void launch_forward(LossParams p, hipStream_t stream) {
-  const dim3 grid((p.classes + kTile - 1) / kTile, (p.rows + kTile - 1) / kTile);
-  logits_kernel<T, false><<<grid, 256, 0, stream>>>(p);
-  join_kernel<T><<<(p.rows + 63) / 64, 256, 0, stream>>>(p, (int)grid.x * 2);
+  const int parts = launch_logits<T, false>(p, p.rows, p.classes, stream);
+  join_kernel<T><<<(p.rows + 7) / 8, 1024, 0, stream>>>(p, parts);
+}
+
+template <class T, class S>
+void launch_dhidden(const LossParams& p, const LossPlan& w, hipStream_t stream) {
+  const int row_tiles = p.padded_rows / S::kTileN;
+  dhidden_kernel<T, S><<<(uint32_t)(row_tiles * w.column_tiles * w.dhidden_split), S::kThreads, 0, stream>>>(p, row_tiles, (int)w.column_tiles, w.alone);
+}
+template <class T, class S>
+void launch_dweight(const LossParams& p, const LossPlan& w, hipStream_t stream) {
+  const int class_tiles = (p.class_end - p.class0 + S::kTileN - 1) / S::kTileN;
+  dweight_kernel<T, S><<<(uint32_t)(class_tiles * w.column_tiles * w.dweight_split), S::kThreads, 0, stream>>>(p, class_tiles, (int)w.column_tiles);
 }
 
 template <class T>
-void launch_backward(LossParams p, hipStream_t stream) {
-  largest_kernel<<<1, 1024, 0, stream>>>(p);
-  if (p.rows > 0)
-    known_rows_kernel<<<(uint32_t)(((int64_t)p.rows * (p.dim / 8) + 255) / 256), 256, 0, stream>>>(p);
-  const int64_t piece = piece_classes(p.rows, p.classes);
-  const uint32_t row_tiles = (p.rows + kTile - 1) / kTile, column_tiles = (p.dim + kTile - 1) / kTile;
-  for (int64_t at = 0; at < p.classes; at += piece) {
+void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
+  if (p.rows == 0) {  // no sum at all
+    const int64_t n = (int64_t)p.classes * p.dim;
+    add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(nullptr, (T*)p.dweight, n, 0);
+    return;
+  }
+  prepare_kernel<<<(uint32_t)((w.padded_rows * (p.dim / 8) + 1023) / 1024 + 1), 1024, 0, stream>>>(p);
+  for (int64_t at = 0; at < p.classes; at += w.piece) {
     p.class0 = (int32_t)at;
-    p.class_end = (int32_t)std::min<int64_t>(at + piece, p.classes);
-    const uint32_t class_tiles = (p.class_end - p.class0 + kTile - 1) / kTile;
-    if (p.rows > 0) {
-      logits_kernel<T, true><<<dim3(class_tiles, row_tiles), 256, 0, stream>>>(p);
-      dhidden_kernel<T><<<dim3(column_tiles, row_tiles), 256, 0, stream>>>(p);
+    p.class_end = (int32_t)std::min<int64_t>(at + w.piece, p.classes);
+    const int64_t classes = p.class_end - p.class0;
+    launch_logits<T, true>(p, p.padded_rows, round_up(classes, kClassPad), stream);
+    const bool few = p.rows <= kFewRows;
+    // shapes of the two products: columns of the vectors x rows of the output
+    if (p.dim > 128) {
+      if (few) launch_dhidden<T, Shape<4, 2, 2, 1, 64>>(p, w, stream);
+      else launch_dhidden<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
+      launch_dweight<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
+    } else if (p.dim > 64) {
+      if (few) launch_dhidden<T, Shape<4, 2, 1, 1, 64>>(p, w, stream);
+      else launch_dhidden<T, Shape<2, 4, 2, 2, 64>>(p, w, stream);
+      launch_dweight<T, Shape<2, 4, 2, 2, 64>>(p, w, stream);
+    } else {
+      if (few) launch_dhidden<T, Shape<2, 2, 1, 1, 64>>(p, w, stream);
+      else launch_dhidden<T, Shape<1, 8, 2, 1, 64>>(p, w, stream);
+      launch_dweight<T, Shape<1, 8, 2, 1, 64>>(p, w, stream);
     }
-    dweight_kernel<T><<<dim3(column_tiles, class_tiles), 256, 0, stream>>>(p);
+    if (w.dweight_split > 1) {
+      const int64_t n = classes * p.dim;
+      add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dweight_sums, (T*)p.dweight + at * p.dim, n, p.dweight_split);
+    }
+  }
+  if (!w.alone) {
+    const int64_t n = (int64_t)p.rows * p.dim;
+    add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dhidden_sums, (T*)p.dhidden, n, p.dhidden_split);
   }
 }
 
@@ -438,7 +660,7 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
     return fail("vocabulary loss: the vectors' size is a multiple of 8 up to " + std::to_string(ND_VOCABULARY_MAX_DIM) + ", " +
                 std::to_string(a->dim) + " given");
   if (a->rows == 0 && !backward) return 0;
-  const LossWorkspace w = workspace_of(a->rows, a->classes, a->dim, backward);
+  const LossPlan w = plan_of(a->rows, a->classes, a->dim, backward);
   if (a->workspace_bytes < w.bytes)
     return fail("vocabulary loss: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(w.bytes) + " needed");
   const void* in[] = {a->weight, a->workspace, a->dweight, a->hidden, a->dhidden};
@@ -461,14 +683,17 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
   char* work = (char*)a->workspace;
   p.partials = (float2*)(work + w.partials);
   p.gradient = (u32x4*)(work + w.gradient);
-  p.dhidden_sum = (float*)(work + w.dhidden_sum);
+  p.dhidden_sums = (float*)(work + w.dhidden_sums);
+  p.dweight_sums = (float*)(work + w.dweight_sums);
   p.largest = (float*)(work + w.largest);
   p.hidden_known = work + w.hidden_known;
-  p.row_blocks = (int32_t)(round_up(a->rows, kTile) / 32);
+  p.padded_rows = (int32_t)w.padded_rows;
+  p.dhidden_split = (int32_t)w.dhidden_split;
+  p.dweight_split = (int32_t)w.dweight_split;
   p.class_end = p.classes;
   if (backward) {
-    if (a->dtype == ND_BF16) launch_backward<__bf16>(p, (hipStream_t)stream);
-    else launch_backward<_Float16>(p, (hipStream_t)stream);
+    if (a->dtype == ND_BF16) launch_backward<__bf16>(p, w, (hipStream_t)stream);
+    else launch_backward<_Float16>(p, w, (hipStream_t)stream);
   } else {
     if (a->dtype == ND_BF16) launch_forward<__bf16>(p, (hipStream_t)stream);
     else launch_forward<_Float16>(p, (hipStream_t)stream);
@@ -487,7 +712,7 @@ int64_t nd_vocabulary_loss_workspace(int64_t rows, int64_t classes, int32_t dim,
   if (rows < 0 || rows > ND_VOCABULARY_MAX_ROWS || classes < 1 || classes > ND_VOCABULARY_MAX_CLASSES || dim < 1 ||
       dim > ND_VOCABULARY_MAX_DIM)
     return -1;
-  return nd::workspace_of(rows, classes, dim, backward != 0).bytes;
+  return nd::plan_of(rows, classes, dim, backward != 0).bytes;
 }
 
 int nd_vocabulary_loss_forward(const nd_vocabulary_loss* a, void* stream) {
