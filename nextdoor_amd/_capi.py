@@ -19,7 +19,7 @@ class PackedAttention(C.Structure):
                 [(n, C.c_void_p) for n in ("plan", "q", "k", "v", "dout")] +
                 [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "dout_token",
                                           "dout_head")] +
-                [(n, C.c_void_p) for n in ("out", "lse", "delta", "dq", "dk", "dv")])
+                [(n, C.c_void_p) for n in ("out", "lse", "dq", "dk", "dv", "workspace")] + [("workspace_bytes", C.c_int64)])
 
 
 class VocabularyLoss(C.Structure):
@@ -104,6 +104,7 @@ SIGNATURES = {
                              C.c_void_p]),
     "nd_packed_plan_bytes": (C.c_int64, [C.c_int64]),
     "nd_packed_plan": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "nd_packed_attention_workspace": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
     "nd_packed_attention_forward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
     "nd_packed_attention_backward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
     "nd_vocabulary_loss_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int]),

@@ -20,24 +20,33 @@ namespace nd {
 namespace {
 
 constexpr int kPlanThreads = 256;
-constexpr int kQueryTile = 128;  // rows of a workgroup: four waves of 32
-constexpr int kKeyTile = 64;
+constexpr int kOrderThreads = 1024;
+constexpr int kRows = 128;    // rows of a workgroup: four waves of 32
+constexpr int kColumns = 64;  // of a round, on the other side
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// A row's sums are kept relative to a maximum that is taken anew only when it has grown by this much (in powers of two):
+// weights stay below 2^8, which costs 32-bit sums and 16-bit floats nothing, and the sums are rarely scaled again.
+constexpr float kTopSlack = 8.f;
 
 struct PackedPlan {
   const int32_t* first;  // of the sequence a token belongs to; tokens from `covered` on belong to none
   const int32_t* last;   // one past it
-  int32_t tokens, covered;
+  const int32_t* query_order;  // tiles of kRows tokens, those with most keys first
+  const int32_t* key_order;    // those with most queries first
+  int32_t tokens, covered, tiles;
 };
 
 struct AttentionParams {
   PackedPlan plan;
   const void *q, *k, *v, *out, *dout;
   void *out_w, *dq, *dk, *dv;
-  float *lse, *delta;  // [heads][tokens]
-  int64_t q_token, q_head, k_token, k_head, v_token, v_head, dout_token, dout_head;  // in elements
+  float *lse, *lse2, *delta;  // [heads][tokens]; lse2: in powers of two, for the backward pass
+  float *dk_sums, *dv_sums;   // [split][tokens][kv_heads][dim], if a group's heads are shared out
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, dout_token, dout_head;  // in bytes
   int32_t heads, kv_heads, group, dim;
-  float scale, scale_log2;
+  int32_t head_split;     // shares of a group's heads
+  float scale, scale_log2;  // scale_log2 > 0
+  uint32_t flip;          // sign bits of a pair: q is taken negative for a negative scale
 };
 
 __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int32_t* starts, int32_t sequences,
@@ -57,21 +66,74 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int32_t
   last[t] = in ? max(min(starts[lo + 1], tokens), (int32_t)t + 1) : (int32_t)t;
 }
 
-// Rows row0 .. row0 + ROWS - 1 (those below `end`) of a matrix of `dim` columns into a tile; the rest is zero.
-template <int ROWS, int CHUNKS>
-__device__ __forceinline__ void load_tile(u32x4* tile, const char* base, int64_t row_bytes, int row0, int end, int dim) {
-  for (int i = threadIdx.x; i < ROWS * CHUNKS; i += 256) {
-    const int r = i / CHUNKS, c = i % CHUNKS;
-    u32x4 v = {0, 0, 0, 0};
-    if (row0 + r < end && c * 8 < dim) v = *(const u32x4*)(base + (int64_t)(row0 + r) * row_bytes + c * 16);
-    tile[tile_place<CHUNKS>(r, c)] = v;
+// Tiles by falling work, so that the last workgroups to start are short ones: a counting sort.  Workgroup 0: the keys a tile of
+// queries reads; workgroup 1: the queries a tile of keys is read by.  (The order of equal ones is left open: it decides when
+// a tile runs and nothing else.)
+__global__ __launch_bounds__(kOrderThreads) void packed_order_kernel(const int32_t* first, const int32_t* last, int32_t tokens,
+                                                                     int32_t covered, int32_t tiles, int32_t* query_order,
+                                                                     int32_t* key_order) {
+  __shared__ int32_t count[kOrderThreads];
+  const bool keys = blockIdx.x == 1;
+  int shift = 0;
+  while ((tokens / kColumns >> shift) >= kOrderThreads - 2) ++shift;
+  auto bucket = [&](int64_t tile) {
+    const int64_t t0 = tile * kRows;
+    if (t0 >= covered) return kOrderThreads - 1;
+    const int32_t t1 = (int32_t)min(t0 + kRows, (int64_t)covered);
+    const int32_t work = keys ? last[t1 - 1] - (int32_t)t0 : t1 - first[t0];
+    return kOrderThreads - 2 - min(work / kColumns >> shift, kOrderThreads - 2);
+  };
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < tiles; i += kOrderThreads) atomicAdd(&count[bucket(i)], 1);
+  __syncthreads();
+  for (int d = 1; d < kOrderThreads; d *= 2) {
+    const int v = threadIdx.x >= d ? count[threadIdx.x - d] : 0;
+    __syncthreads();
+    count[threadIdx.x] += v;
+    __syncthreads();
   }
+  // count: one past the last place of a bucket
+  for (int64_t i = threadIdx.x; i < tiles; i += kOrderThreads)
+    (keys ? key_order : query_order)[atomicSub(&count[bucket(i)], 1) - 1] = (int32_t)i;
 }
 
-template <class T, int NB>
+template <int NB>
 struct HeadTile {
-  static constexpr int kChunks = NB == 1 ? 4 : NB == 2 ? 8 : 16;
-  static constexpr int kSlices = 2 * NB;  // of 16 columns
+  static constexpr int kChunks = NB == 1 ? 4 : NB == 2 ? 8 : 16;  // of a row in LDS
+  static constexpr int kTurns = kColumns * kChunks / 256;
+  static constexpr int kSize = kColumns * kChunks;  // of a tile
+};
+
+// Brings tiles of 64 rows of one matrix of heads to LDS.  Columns past `dim` are the row's first ones again (the other operand
+// is 0 there, or the result's column is not stored), rows past the last one that one again (they are masked).
+template <int NB>
+struct TileLoader {
+  const char* base;
+  uint32_t row_bytes;
+  uint32_t offset[HeadTile<NB>::kTurns];
+  __device__ __forceinline__ TileLoader(const void* matrix, int64_t token_bytes, int64_t head_bytes, int head, int dim)
+      : base((const char*)matrix + head * head_bytes), row_bytes((uint32_t)token_bytes) {
+    constexpr int kChunks = HeadTile<NB>::kChunks;
+#pragma unroll
+    for (int i = 0; i < HeadTile<NB>::kTurns; ++i) {
+      const int at = threadIdx.x + 256 * i, r = at / kChunks, c = (at % kChunks) ^ tile_swizzle<kChunks>(r);
+      offset[i] = r * row_bytes + (c * 8 < dim ? c * 16 : 0);
+    }
+  }
+  __device__ __forceinline__ void issue(uint32_t wave_lds, int64_t token_bytes, int row0, int end) const {
+    const char* at = base + row0 * token_bytes;
+    if (row0 + kColumns <= end) {
+#pragma unroll
+      for (int i = 0; i < HeadTile<NB>::kTurns; ++i) load_to_lds(at, offset[i], wave_lds + 4096 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < HeadTile<NB>::kTurns; ++i) {
+        const int r = (threadIdx.x + 256 * i) / HeadTile<NB>::kChunks;
+        load_to_lds(at, offset[i] - max(r - (end - 1 - row0), 0) * row_bytes, wave_lds + 4096 * i);
+      }
+    }
+  }
 };
 
 // A wave's 32 rows as operands: lane's row, columns 16 s + 8 h .. + 7.
@@ -85,51 +147,85 @@ __device__ __forceinline__ void load_rows(u32x4 (&frag)[2 * NB], const char* row
   }
 }
 
-// Result rows = columns of a head, result column = token: four consecutive columns of the lane's token at a time.
+// A wave's 32 rows x NB * 32 columns: result rows = columns of a head, result column = the lane's token.  Rounded, turned
+// through the wave's part of LDS (16 x HeadTile::kChunks x 32 bytes) and stored 16 bytes a lane.
 template <class T, int NB>
-__device__ __forceinline__ void store_rows(T* row, const f32x16 (&acc)[NB], float factor, int dim, int h) {
+__device__ __forceinline__ void store_rows(T* first_row, int64_t row_elements, int rows, const f32x16 (&acc)[NB], float factor, int dim,
+                                           u32x4* part) {
+  constexpr int kChunks = HeadTile<NB>::kChunks;
+  const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int c = 32 * b + 8 * g + 4 * h;
       u32x2 v;
       v[0] = pack_pair<T>(acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor);
       v[1] = pack_pair<T>(acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor);
-      if (c < dim) *(u32x2*)(row + c) = v;
+      ((u32x2*)(part + tile_place<kChunks>(r, 4 * b + g)))[h] = v;
     }
+  // (one wave's LDS operations are done in order)
+#pragma unroll
+  for (int i = 0; i < kChunks / 2; ++i) {
+    const int at = lane + 64 * i, rr = at / kChunks, c = at % kChunks;
+    if (c >= 4 * NB) continue;
+    const u32x4 v = part[tile_place<kChunks>(rr, c)];
+    if (rr < rows && c * 8 < dim) *(u32x4*)(first_row + rr * row_elements + c * 8) = v;
+  }
+}
+
+// Which tile and head a workgroup has: heads side by side (their tiles share keys), and, where they fill the eight dies
+// evenly, a die's heads next to each other.
+__device__ __forceinline__ void tile_and_head(uint32_t block, int heads, int& rank, int& head) {
+  rank = uniform(block / heads);
+  head = uniform(block % heads);
+  if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
 }
 
 // ---- forward ------------------------------------------------------------------------------------
 // One workgroup: 128 query tokens of one head; one wave: 32 of them, lane's token is column l & 31 of S^T = K Q^T, so
-// the softmax of a row runs over a lane's own registers and its partner's, 32 lanes away.
+// the softmax of a row runs over a lane's own registers and its partner's, 32 lanes away, and P^T is the second operand of
+// O^T = V^T P^T as it is.  The next tile of keys and values is on its way to LDS while this one is worked on.
 template <class T, int NB>
-__global__ __launch_bounds__(256) void attention_forward_kernel(AttentionParams p) {
-  constexpr int kChunks = HeadTile<T, NB>::kChunks;
-  __shared__ u32x4 keys[kKeyTile * kChunks], values[kKeyTile * kChunks];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile0 = (int)(gridDim.x - 1 - blockIdx.x) * kQueryTile;
-  const int head = blockIdx.y, kv_head = head / p.group;
+__global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionParams p) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
+  __shared__ u32x4 tiles[2][2][kSize];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  int rank, head;
+  tile_and_head(blockIdx.x, p.heads, rank, head);
+  const int tile0 = uniform(p.plan.query_order[rank]) * kRows, kv_head = uniform(head / p.group);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
   const bool there = row < p.plan.covered;
-  const int first = there ? p.plan.first[row] : row + 1;
-  u32x4 qf[2 * NB];
-  load_rows<NB>(qf, (const char*)p.q + ((int64_t)row * p.q_token + (int64_t)head * p.q_head) * 2, there, p.dim, h);
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
-  float top = -INFINITY, sum = 0.f;
+  float top = -INFINITY, sum = 0.f;  // sum: over the lane's own keys
 
   if (tile0 < p.plan.covered) {
-    const int end = min(tile0 + kQueryTile, p.plan.covered);
-    const char* kbase = (const char*)p.k + (int64_t)kv_head * p.k_head * 2;
-    const char* vbase = (const char*)p.v + (int64_t)kv_head * p.v_head * 2;
-    for (int n0 = p.plan.first[tile0]; n0 < end; n0 += kKeyTile) {
-      __syncthreads();
-      load_tile<kKeyTile, kChunks>(keys, kbase, p.k_token * 2, n0, end, p.dim);
-      load_tile<kKeyTile, kChunks>(values, vbase, p.v_token * 2, n0, end, p.dim);
-      __syncthreads();
-      if (n0 > row0 + 31) continue;  // (wave-uniform) every key is later than the wave's rows
+    const int end = min(tile0 + kRows, p.plan.covered), begin = uniform(p.plan.first[tile0]);
+    const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
+    const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
+    auto issue = [&](int half, int n0) {
+      k.issue(lds + (2 * half) * kSize * 16, p.k_token, n0, end);
+      v.issue(lds + (2 * half + 1) * kSize * 16, p.v_token, n0, end);
+    };
+    issue(0, begin);
+    const int first = there ? p.plan.first[row] : row + 1;
+    // of the wave's rows: the smallest and the largest `first`
+    const int first_min = row0 < p.plan.covered ? uniform(first) : 0x7fffffff - kColumns;
+    const int first_max = uniform(p.plan.first[min(row0 + 31, p.plan.covered - 1)]);
+    u32x4 qf[2 * NB];
+    load_rows<NB>(qf, (const char*)p.q + (int64_t)row * p.q_token + (int64_t)head * p.q_head, there, p.dim, h);
+    if (p.flip) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) qf[i] ^= p.flip;
+    }
+    int half = 0;
+    for (int n0 = begin; n0 < end; n0 += kColumns, half ^= 1) {
+      wait_for_loads_and_others();
+      if (n0 + kColumns < end) issue(half ^ 1, n0 + kColumns);
+      // (wave-uniform) every key is later than the wave's rows, or before their sequences
+      if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
+      const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
       f32x16 s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -138,35 +234,41 @@ __global__ __launch_bounds__(256) void attention_forward_kernel(AttentionParams 
         for (int i = 0; i < 2 * NB; ++i)
           s[t] = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s[t]);
       }
-      float m = -INFINITY;
+      if (n0 + kColumns - 1 > row0 || n0 < first_max) {
+        const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = 32 * t + 8 * (i / 4) + i % 4;
+            s[t][i] = key >= from && key <= to ? s[t][i] : -INFINITY;
+          }
+      }
+      float m = s[0][0];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[t][i]);
+      m = pair_max(m) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(m > top + kTopSlack)) {  // (top: -inf before a row's first key)
+        const float higher = fmaxf(m, top);
+        const float shrink = higher == -INFINITY ? 0.f : exp2_fast(top - higher);
+        top = higher;
+        sum *= shrink;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[b][i] *= shrink;
+      }
+      // a row that has seen no key yet: exp2(-inf - 0) = 0 throughout
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int key = n0 + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-          s[t][i] = key >= first && key <= row ? s[t][i] * p.scale_log2 : -INFINITY;
-          m = fmaxf(m, s[t][i]);
+          s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], p.scale_log2, -base));
+          sum += s[t][i];
         }
-      m = fmaxf(pair_max(m), top);
-      // a row that has seen no key yet: its top stays -inf, and exp2(-inf - 0) = 0 throughout
-      const float base = m == -INFINITY ? 0.f : m;
-      const float shrink = exp2_fast(top - base);
-      top = m;
-      float part = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[t][i] = exp2_fast(s[t][i] - base);
-          part += s[t][i];
-        }
-      sum = sum * shrink + part;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[b][i] *= shrink;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const u32x4 pf = pack_operand<T>(s[t], j);
@@ -175,61 +277,89 @@ __global__ __launch_bounds__(256) void attention_forward_kernel(AttentionParams 
             acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(values, 32 * t + 16 * j, 32 * b, lane), pf,
                                          acc[b]);
         }
+      }
     }
+    __syncthreads();
   }
-  if (row >= p.plan.tokens) return;
+  if (row0 >= p.plan.tokens) return;
+  if (row0 + 31 >= p.plan.covered && !there) {  // (tiles that all of the wave's sequences see are not masked)
+    top = -INFINITY;
+    sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  }
   sum = pair_sum(sum);
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
-  store_rows<T, NB>((T*)p.out_w + ((int64_t)row * p.heads + head) * p.dim, acc, inverse, p.dim, h);
-  if (h == 0) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
+  if (h == 0 && row < p.plan.tokens) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
+  store_rows<T, NB>((T*)p.out_w + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, inverse,
+                    p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
 }
 
 // ---- backward -----------------------------------------------------------------------------------
-// dq: as the forward pass, with S^T and dP^T = V dO^T; dS^T is the second operand of dQ^T = K^T dS^T.  Leaves delta.
+// dq: as the forward pass, with S^T and dP^T = V dO^T; dS^T is the second operand of dQ^T = K^T dS^T.  Leaves delta and lse
+// in powers of two for the other kernel.
 template <class T, int NB>
-__global__ __launch_bounds__(256) void attention_backward_query_kernel(AttentionParams p) {
-  constexpr int kChunks = HeadTile<T, NB>::kChunks;
-  __shared__ u32x4 keys[kKeyTile * kChunks], values[kKeyTile * kChunks];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile0 = (int)(gridDim.x - 1 - blockIdx.x) * kQueryTile;
-  const int head = blockIdx.y, kv_head = head / p.group;
+__global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(AttentionParams p) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
+  __shared__ u32x4 tiles[2][2][kSize];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  int rank, head;
+  tile_and_head(blockIdx.x, p.heads, rank, head);
+  const int tile0 = uniform(p.plan.query_order[rank]) * kRows, kv_head = uniform(head / p.group);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
   const bool there = row < p.plan.covered;
-  const int first = there ? p.plan.first[row] : row + 1;
-  u32x4 qf[2 * NB], dof[2 * NB];
-  load_rows<NB>(qf, (const char*)p.q + ((int64_t)row * p.q_token + (int64_t)head * p.q_head) * 2, there, p.dim, h);
-  load_rows<NB>(dof, (const char*)p.dout + ((int64_t)row * p.dout_token + (int64_t)head * p.dout_head) * 2, there, p.dim, h);
-  float delta = 0.f, lse2 = 0.f;
-  {
-    u32x4 of[2 * NB];
-    load_rows<NB>(of, (const char*)p.out + ((int64_t)row * p.heads + head) * p.dim * 2, there, p.dim, h);
-#pragma unroll
-    for (int s = 0; s < 2 * NB; ++s)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        delta += unpack_low<T>(of[s][j]) * unpack_low<T>(dof[s][j]);
-        delta += unpack_high<T>(of[s][j]) * unpack_high<T>(dof[s][j]);
-      }
-    delta = pair_sum(delta);
-    if (there) {
-      lse2 = p.lse[(int64_t)head * p.plan.tokens + row] * kLog2e;
-      if (h == 0) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
-    }
-  }
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
 
   if (tile0 < p.plan.covered) {
-    const int end = min(tile0 + kQueryTile, p.plan.covered);
-    const char* kbase = (const char*)p.k + (int64_t)kv_head * p.k_head * 2;
-    const char* vbase = (const char*)p.v + (int64_t)kv_head * p.v_head * 2;
-    for (int n0 = p.plan.first[tile0]; n0 < end; n0 += kKeyTile) {
-      __syncthreads();
-      load_tile<kKeyTile, kChunks>(keys, kbase, p.k_token * 2, n0, end, p.dim);
-      load_tile<kKeyTile, kChunks>(values, vbase, p.v_token * 2, n0, end, p.dim);
-      __syncthreads();
-      if (n0 > row0 + 31) continue;
+    const int end = min(tile0 + kRows, p.plan.covered), begin = uniform(p.plan.first[tile0]);
+    const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
+    const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
+    auto issue = [&](int half, int n0) {
+      k.issue(lds + (2 * half) * kSize * 16, p.k_token, n0, end);
+      v.issue(lds + (2 * half + 1) * kSize * 16, p.v_token, n0, end);
+    };
+    issue(0, begin);
+    const int first = there ? p.plan.first[row] : row + 1;
+    const int first_min = row0 < p.plan.covered ? uniform(first) : 0x7fffffff - kColumns;
+    const int first_max = uniform(p.plan.first[min(row0 + 31, p.plan.covered - 1)]);
+    u32x4 qf[2 * NB], dof[2 * NB];
+    load_rows<NB>(qf, (const char*)p.q + (int64_t)row * p.q_token + (int64_t)head * p.q_head, there, p.dim, h);
+    load_rows<NB>(dof, (const char*)p.dout + (int64_t)row * p.dout_token + (int64_t)head * p.dout_head, there, p.dim, h);
+    float delta = 0.f, lse2 = 0.f;
+    {
+      u32x4 of[2 * NB];
+      load_rows<NB>(of, (const char*)p.out + ((int64_t)row * p.heads + head) * p.dim * 2, there, p.dim, h);
+#pragma unroll
+      for (int s = 0; s < 2 * NB; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          delta = __builtin_fmaf(unpack_low<T>(of[s][j]), unpack_low<T>(dof[s][j]), delta);
+          delta = __builtin_fmaf(unpack_high<T>(of[s][j]), unpack_high<T>(dof[s][j]), delta);
+        }
+      delta = pair_sum(delta);
+      if (there) {
+        const int64_t at = (int64_t)head * p.plan.tokens + row;
+        lse2 = p.lse[at] * kLog2e;
+        if (h == 0) {
+          p.delta[at] = delta;
+          p.lse2[at] = lse2;
+        }
+      }
+    }
+    if (p.flip) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) qf[i] ^= p.flip;
+    }
+    int half = 0;
+    for (int n0 = begin; n0 < end; n0 += kColumns, half ^= 1) {
+      wait_for_loads_and_others();
+      if (n0 + kColumns < end) issue(half ^ 1, n0 + kColumns);
+      if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
+      const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
+      const bool masked = n0 + kColumns - 1 > row0 || n0 < first_max;
+      const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f32x16 s = {}, dp = {};
@@ -239,10 +369,13 @@ __global__ __launch_bounds__(256) void attention_backward_query_kernel(Attention
           dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = n0 + 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-          const float weight = exp2_fast(s[i] * p.scale_log2 - lse2);
-          s[i] = key >= first && key <= row ? weight * (dp[i] - delta) : 0.f;
+        for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = 32 * t + 8 * (i / 4) + i % 4;
+            s[i] = key >= from && key <= to ? s[i] : 0.f;
+          }
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -254,26 +387,32 @@ __global__ __launch_bounds__(256) void attention_backward_query_kernel(Attention
         }
       }
     }
+    __syncthreads();
   }
-  if (row < p.plan.tokens)
-    store_rows<T, NB>((T*)p.dq + ((int64_t)row * p.heads + head) * p.dim, acc, p.scale, p.dim, h);
+  if (row0 + 31 >= p.plan.covered && !there) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  }
+  if (row0 < p.plan.tokens)
+    store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, p.scale,
+                      p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
 }
 
 // dk, dv: one workgroup has 128 keys of one key head, a wave 32 of them (lane's key is a column of S = Q K^T), and goes
-// over the query tiles that see them, for each head of the group in turn: no sum is shared between workgroups.
+// over the query tiles that see them, for each head of its share of the group in turn: no sum is shared between
+// workgroups.  Where keys and key heads are few for the GPU, a group's heads are shared out and the sums, in 32 bits, added
+// by another kernel.
 template <class T, int NB>
-__global__ __launch_bounds__(256) void attention_backward_key_kernel(AttentionParams p) {
-  constexpr int kChunks = HeadTile<T, NB>::kChunks;
-  __shared__ u32x4 queries[kKeyTile * kChunks], douts[kKeyTile * kChunks];
-  __shared__ float lse2[kKeyTile], deltas[kKeyTile];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int tile0 = (int)blockIdx.x * kQueryTile, kv_head = blockIdx.y;
+__global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(AttentionParams p) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
+  __shared__ u32x4 tiles[2][2][kSize];
+  __shared__ float rows_of[2][2][kColumns];  // lse2 and delta of a tile's queries
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  int rank, part;
+  tile_and_head(blockIdx.x, p.kv_heads * p.head_split, rank, part);
+  const int tile0 = uniform(p.plan.key_order[rank]) * kRows, kv_head = uniform(part / p.head_split), share = part % p.head_split;
   const int key0 = tile0 + wave * 32, key = key0 + (lane & 31);
   const bool there = key < p.plan.covered;
-  const int last = there ? p.plan.last[key] : key;
-  u32x4 kf[2 * NB], vf[2 * NB];
-  load_rows<NB>(kf, (const char*)p.k + ((int64_t)key * p.k_token + (int64_t)kv_head * p.k_head) * 2, there, p.dim, h);
-  load_rows<NB>(vf, (const char*)p.v + ((int64_t)key * p.v_token + (int64_t)kv_head * p.v_head) * 2, there, p.dim, h);
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -281,22 +420,45 @@ __global__ __launch_bounds__(256) void attention_backward_key_kernel(AttentionPa
     dv[b] = f32x16{};
   }
   if (tile0 < p.plan.covered) {
-    const int end = p.plan.last[min(tile0 + kQueryTile, p.plan.covered) - 1];
-    for (int head = kv_head * p.group; head < (kv_head + 1) * p.group; ++head) {
-      const char* qbase = (const char*)p.q + (int64_t)head * p.q_head * 2;
-      const char* dobase = (const char*)p.dout + (int64_t)head * p.dout_head * 2;
-      for (int m0 = tile0; m0 < end; m0 += kKeyTile) {
-        __syncthreads();
-        load_tile<kKeyTile, kChunks>(queries, qbase, p.q_token * 2, m0, end, p.dim);
-        load_tile<kKeyTile, kChunks>(douts, dobase, p.dout_token * 2, m0, end, p.dim);
-        if (threadIdx.x < kKeyTile) {
-          const int64_t at = (int64_t)head * p.plan.tokens + m0 + threadIdx.x;
-          const bool in = m0 + (int)threadIdx.x < end;
-          lse2[threadIdx.x] = in ? p.lse[at] * kLog2e : 0.f;
-          deltas[threadIdx.x] = in ? p.delta[at] : 0.f;
-        }
-        __syncthreads();
-        if (m0 + kKeyTile <= key0) continue;  // every query is earlier than the wave's keys
+    const int end = uniform(p.plan.last[min(tile0 + kRows, p.plan.covered) - 1]);
+    const int heads = p.group / p.head_split, head0 = kv_head * p.group + share * heads;
+    const TileLoader<NB> q(p.q, p.q_token, p.q_head, head0, p.dim), d(p.dout, p.dout_token, p.dout_head, head0, p.dim);
+    const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024, rows_lds = lds_address(&rows_of[0][0][0]);
+    auto issue = [&](int half, int head, int m0) {  // head: of the share
+      TileLoader<NB> qh = q, dh = d;
+      qh.base += head * p.q_head;
+      dh.base += head * p.dout_head;
+      qh.issue(lds + (2 * half) * kSize * 16, p.q_token, m0, end);
+      dh.issue(lds + (2 * half + 1) * kSize * 16, p.dout_token, m0, end);
+      if (wave < 2)
+        load_words_to_lds((const char*)((wave == 0 ? p.lse2 : p.delta) + (int64_t)(head0 + head) * p.plan.tokens + m0),
+                          min(lane, end - 1 - m0) * 4, rows_lds + (2 * half + wave) * kColumns * 4);
+    };
+    issue(0, 0, tile0);
+    const int last = there ? p.plan.last[key] : key;
+    // of the wave's keys: the smallest and the largest `last`
+    const int last_min = key0 < p.plan.covered ? uniform(last) : 0;
+    const int last_max = key0 < p.plan.covered ? uniform(p.plan.last[min(key0 + 31, p.plan.covered - 1)]) : 0;
+    u32x4 kf[2 * NB], vf[2 * NB];
+    load_rows<NB>(kf, (const char*)p.k + (int64_t)key * p.k_token + (int64_t)kv_head * p.k_head, there, p.dim, h);
+    load_rows<NB>(vf, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, there, p.dim, h);
+    if (p.flip) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) kf[i] ^= p.flip;
+    }
+    int half = 0, head = 0, m0 = tile0;
+    while (head < heads) {
+      int next_head = head, next = m0 + kColumns;
+      if (next >= end) {
+        next = tile0;
+        ++next_head;
+      }
+      wait_for_loads_and_others();
+      if (next_head < heads) issue(half ^ 1, next_head, next);
+      if (m0 + kColumns > key0 && m0 < last_max) {  // (else no query of the tile sees a key of the wave)
+        const u32x4 *queries = tiles[half][0], *douts = tiles[half][1];
+        const bool masked = m0 < key0 + 31 || m0 + kColumns > last_min;
+        const int from = key - m0 - 4 * h, to = last - m0 - 4 * h;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x16 s = {}, dp = {};
@@ -306,12 +468,24 @@ __global__ __launch_bounds__(256) void attention_backward_key_kernel(AttentionPa
             dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(douts, 32 * t, i, lane), vf[i], dp);
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * t + 8 * (i / 4) + 4 * h + i % 4, query = m0 + at;
-            const bool sees = query >= key && query < last;
-            const float weight = sees ? exp2_fast(s[i] * p.scale_log2 - lse2[at]) : 0.f;
-            dp[i] = sees ? weight * (dp[i] - deltas[at]) : 0.f;
-            s[i] = weight;
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 lse2 = *(const f32x4*)&rows_of[half][0][32 * t + 8 * g + 4 * h];
+            const f32x4 delta = *(const f32x4*)&rows_of[half][1][32 * t + 8 * g + 4 * h];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int i = 4 * g + n;
+              s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2[n]));
+              dp[i] = s[i] * (dp[i] - delta[n]);
+            }
+          }
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int query = 32 * t + 8 * (i / 4) + i % 4;
+              const bool sees = query >= from && query < to;
+              s[i] = sees ? s[i] : 0.f;
+              dp[i] = sees ? dp[i] : 0.f;
+            }
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -326,27 +500,106 @@ __global__ __launch_bounds__(256) void attention_backward_key_kernel(AttentionPa
           }
         }
       }
+      head = next_head;
+      m0 = next;
+      half ^= 1;
     }
+    __syncthreads();
   }
-  if (key < p.plan.tokens) {
-    const int64_t at = ((int64_t)key * p.kv_heads + kv_head) * p.dim;
-    store_rows<T, NB>((T*)p.dk + at, dk, p.scale, p.dim, h);
-    store_rows<T, NB>((T*)p.dv + at, dv, 1.f, p.dim, h);
+  if (key0 >= p.plan.tokens) return;
+  const int64_t row_elements = (int64_t)p.kv_heads * p.dim;
+  if (p.head_split == 1) {
+    u32x4* part_lds = &tiles[0][0][0] + wave * 32 * kChunks;
+    const int64_t at = ((int64_t)key0 * p.kv_heads + kv_head) * p.dim;
+    store_rows<T, NB>((T*)p.dk + at, row_elements, p.plan.tokens - key0, dk, p.scale, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dv + at, row_elements, p.plan.tokens - key0, dv, 1.f, p.dim, part_lds);
+  } else if (key < p.plan.tokens) {
+    const int64_t at = (((int64_t)share * p.plan.tokens + key) * p.kv_heads + kv_head) * p.dim;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * b + 8 * g + 4 * h;
+        if (c >= p.dim) continue;
+        f32x4 a, e;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          a[n] = dk[b][4 * g + n] * p.scale;
+          e[n] = dv[b][4 * g + n];
+        }
+        *(f32x4*)(p.dk_sums + at + c) = a;
+        *(f32x4*)(p.dv_sums + at + c) = e;
+      }
   }
+}
+
+// dk and dv from the shares' sums: n values each, a multiple of 8.
+template <class T>
+__global__ __launch_bounds__(256) void add_shares_kernel(AttentionParams p, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float* sums = blockIdx.y ? p.dv_sums : p.dk_sums;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.head_split; ++s) v += *(const f32x4*)(sums + s * n + i);
+  u32x2 o;
+  o[0] = pack_pair<T>(v[0], v[1]);
+  o[1] = pack_pair<T>(v[2], v[3]);
+  *(u32x2*)((T*)(blockIdx.y ? p.dv : p.dk) + i) = o;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t tiles_of(int64_t tokens) { return (tokens + kRows - 1) / kRows; }
+
+// The plan's parts, in words: first, last, query_order, key_order.
+struct PlanParts {
+  int64_t last, query_order, key_order, words;
+};
+PlanParts plan_parts(int64_t tokens) {
+  PlanParts w;
+  w.last = round_up(tokens, 4);
+  w.query_order = 2 * w.last;
+  w.key_order = w.query_order + round_up(tiles_of(tokens), 4);
+  w.words = w.key_order + round_up(tiles_of(tokens), 4);
+  return w;
+}
+
+// Shares of a group's heads in the dk, dv kernel: as many as it takes for four workgroups to a compute unit.
+int head_split_of(int64_t tokens, int kv_heads, int group) {
+  const int64_t tiles = tiles_of(tokens) * kv_heads;
+  for (int split = 1; split < group; ++split)
+    if (group % split == 0 && tiles * split >= 1024) return split;
+  return group;
+}
+
+// The backward pass's working memory, in bytes: lse2, delta, and the shares' sums.
+struct WorkParts {
+  int64_t delta, dk_sums, dv_sums, bytes;
+};
+WorkParts work_parts(int64_t tokens, int heads, int kv_heads, int dim) {
+  WorkParts w;
+  const int split = head_split_of(tokens, kv_heads, heads / kv_heads);
+  const int64_t sums = split > 1 ? round_up(split * tokens * kv_heads * dim * 4, 256) : 0;
+  w.delta = round_up(tokens * heads * 4, 256);
+  w.dk_sums = 2 * w.delta;
+  w.dv_sums = w.dk_sums + sums;
+  w.bytes = w.dv_sums + sums;
+  return w;
+}
+
 template <class T, int NB>
 void launch_forward(const AttentionParams& p, hipStream_t stream) {
-  const dim3 grid((p.plan.tokens + kQueryTile - 1) / kQueryTile, p.heads);
-  attention_forward_kernel<T, NB><<<grid, 256, 0, stream>>>(p);
+  attention_forward_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads, 256, 0, stream>>>(p);
 }
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
-  const int tiles = (p.plan.tokens + kQueryTile - 1) / kQueryTile;
-  attention_backward_query_kernel<T, NB><<<dim3(tiles, p.heads), 256, 0, stream>>>(p);
-  attention_backward_key_kernel<T, NB><<<dim3(tiles, p.kv_heads), 256, 0, stream>>>(p);
+  attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads, 256, 0, stream>>>(p);
+  attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split, 256, 0, stream>>>(p);
+  if (p.head_split > 1) {
+    const int64_t n = (int64_t)p.plan.tokens * p.kv_heads * p.dim;
+    add_shares_kernel<T><<<dim3((uint32_t)((n / 4 + 255) / 256), 2), 256, 0, stream>>>(p, n);
+  }
 }
 
 template <class T>
@@ -374,25 +627,38 @@ int check_attention(const nd_packed_attention* a, bool backward) {
                 std::to_string(a->dim) + " given");
   if (!isfinite(a->scale)) return fail("packed attention: the scale is not finite");
   if (a->n_tokens == 0) return 0;
-  const void* in[] = {a->q, a->k, a->v, a->out, a->lse, a->plan, a->dout, a->dq, a->dk, a->dv, a->delta};
+  if (tiles_of(a->n_tokens) * a->heads > 0x7fffffff) return fail("packed attention: more tokens and heads than one launch holds");
+  const void* in[] = {a->q, a->k, a->v, a->out, a->lse, a->plan, a->dout, a->dq, a->dk, a->dv, a->workspace};
   for (int i = 0; i < (backward ? 11 : 6); ++i) {
     if (!in[i]) return fail("packed attention: null array");
     if ((uintptr_t)in[i] & 15) return fail("packed attention: arrays are aligned to 16 bytes");
   }
   const int64_t strides[] = {a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->dout_token, a->dout_head};
   for (int i = 0; i < (backward ? 8 : 6); ++i)
-    if (strides[i] < 0 || strides[i] % 8 != 0) return fail("packed attention: strides are multiples of 8 elements");
+    if (strides[i] < 0 || strides[i] % 8 != 0 || (i % 2 == 0 && strides[i] > ND_PACKED_MAX_TOKEN_STRIDE))
+      return fail("packed attention: strides are multiples of 8 elements, a token's at most " +
+                  std::to_string(ND_PACKED_MAX_TOKEN_STRIDE));
+  if (backward) {
+    const int64_t bytes = work_parts(a->n_tokens, a->heads, a->kv_heads, a->dim).bytes;
+    if (a->workspace_bytes < bytes)
+      return fail("packed attention: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(bytes) +
+                  " needed");
+  }
   return 0;
 }
 
 int run_attention(const nd_packed_attention* a, bool backward, void* stream) {
   const int rc = check_attention(a, backward);
   if (rc != 0 || a->n_tokens == 0) return rc;
-  AttentionParams p;
+  AttentionParams p = {};
+  const PlanParts parts = plan_parts(a->n_tokens);
   p.plan.first = (const int32_t*)a->plan;
-  p.plan.last = p.plan.first + (a->n_tokens + 3) / 4 * 4;
+  p.plan.last = p.plan.first + parts.last;
+  p.plan.query_order = p.plan.first + parts.query_order;
+  p.plan.key_order = p.plan.first + parts.key_order;
   p.plan.tokens = (int32_t)a->n_tokens;
   p.plan.covered = (int32_t)a->n_covered;
+  p.plan.tiles = (int32_t)tiles_of(a->n_tokens);
   p.q = a->q;
   p.k = a->k;
   p.v = a->v;
@@ -402,21 +668,31 @@ int run_attention(const nd_packed_attention* a, bool backward, void* stream) {
   p.dk = a->dk;
   p.dv = a->dv;
   p.lse = a->lse;
-  p.delta = a->delta;
-  p.q_token = a->q_token;
-  p.q_head = a->q_head;
-  p.k_token = a->k_token;
-  p.k_head = a->k_head;
-  p.v_token = a->v_token;
-  p.v_head = a->v_head;
-  p.dout_token = a->dout_token;
-  p.dout_head = a->dout_head;
+  p.head_split = 1;
+  if (backward) {
+    const WorkParts w = work_parts(a->n_tokens, a->heads, a->kv_heads, a->dim);
+    p.lse2 = (float*)a->workspace;
+    p.delta = (float*)((char*)a->workspace + w.delta);
+    p.dk_sums = (float*)((char*)a->workspace + w.dk_sums);
+    p.dv_sums = (float*)((char*)a->workspace + w.dv_sums);
+    p.head_split = head_split_of(a->n_tokens, a->kv_heads, a->heads / a->kv_heads);
+  }
+  p.q_token = a->q_token * 2;
+  p.q_head = a->q_head * 2;
+  p.k_token = a->k_token * 2;
+  p.k_head = a->k_head * 2;
+  p.v_token = a->v_token * 2;
+  p.v_head = a->v_head * 2;
+  p.dout_token = a->dout_token * 2;
+  p.dout_head = a->dout_head * 2;
   p.heads = a->heads;
   p.kv_heads = a->kv_heads;
   p.group = a->heads / a->kv_heads;
   p.dim = a->dim;
   p.scale = a->scale;
-  p.scale_log2 = a->scale * kLog2e;
+  // (a scale of 0 as the smallest one: -inf x 0 would be NaN where a key is masked)
+  p.scale_log2 = fmaxf(fabsf(a->scale) * kLog2e, 1e-37f);
+  p.flip = a->scale < 0.f ? 0x80008000u : 0u;
   if (a->dtype == ND_BF16) launch<__bf16>(p, backward, (hipStream_t)stream);
   else launch<_Float16>(p, backward, (hipStream_t)stream);
   const hipError_t e = hipGetLastError();
@@ -431,7 +707,7 @@ extern "C" {
 
 int64_t nd_packed_plan_bytes(int64_t n_tokens) {
   if (n_tokens < 0 || n_tokens > ND_PACKED_MAX_TOKENS) return -1;
-  return 2 * ((n_tokens + 3) / 4 * 4) * (int64_t)sizeof(int32_t);
+  return nd::plan_parts(n_tokens).words * (int64_t)sizeof(int32_t);
 }
 
 int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
@@ -450,13 +726,23 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
     if (n_tokens == 0) return 0;
     if (!d_starts || !d_plan || ((uintptr_t)d_plan & 15)) return nd::fail("packed sequences: null or misaligned device array");
     int32_t* first = (int32_t*)d_plan;
+    const nd::PlanParts parts = nd::plan_parts(n_tokens);
     nd::packed_plan_kernel<<<(uint32_t)((n_tokens + nd::kPlanThreads - 1) / nd::kPlanThreads), nd::kPlanThreads, 0,
-                             (hipStream_t)stream>>>(d_starts, (int32_t)n_sequences, (int32_t)n_tokens, first,
-                                                    first + (n_tokens + 3) / 4 * 4);
+                             (hipStream_t)stream>>>(d_starts, (int32_t)n_sequences, (int32_t)n_tokens, first, first + parts.last);
+    nd::packed_order_kernel<<<2, nd::kOrderThreads, 0, (hipStream_t)stream>>>(
+        first, first + parts.last, (int32_t)n_tokens, starts[n_sequences], (int32_t)nd::tiles_of(n_tokens), first + parts.query_order,
+        first + parts.key_order);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return nd::fail(std::string("packed sequences: ") + hipGetErrorString(e));
     return 0;
   });
+}
+
+int64_t nd_packed_attention_workspace(int64_t n_tokens, int32_t heads, int32_t kv_heads, int32_t dim) {
+  if (n_tokens < 0 || n_tokens > ND_PACKED_MAX_TOKENS || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || dim < 1 ||
+      dim > ND_PACKED_MAX_DIM)
+    return -1;
+  return nd::work_parts(n_tokens, heads, kv_heads, dim).bytes;
 }
 
 int nd_packed_attention_forward(const nd_packed_attention* a, void* stream) {

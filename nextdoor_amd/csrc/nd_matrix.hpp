@@ -130,6 +130,10 @@ __device__ __forceinline__ u32x4 read_operand_by_rows(const u32x4* tile, int row
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void load_words_to_lds(const char* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // A value that is the same for the whole wave, in a scalar register (what divisions leave is not).
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -170,7 +170,7 @@ def _heads(what, x, tokens, dim=None):
     _need(x.dim() == 3 and x.shape[0] == tokens, "packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
     _need(dim is None or x.shape[2] == dim, "packed attention: %s has another head size" % what)
     a, b, c = x.stride()
-    if (c != 1 and x.shape[2] > 1) or a % 8 or b % 8 or x.data_ptr() % 16:
+    if (c != 1 and x.shape[2] > 1) or a % 8 or b % 8 or a > 16777216 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
@@ -226,8 +226,11 @@ def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
     dout = _heads("dout", dout, a.n_tokens)
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    delta = torch.empty_like(lse)
-    a.dout, a.out, a.lse, a.delta = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), delta.data_ptr()
+    size = _library().nd_packed_attention_workspace(a.n_tokens, a.heads, a.kv_heads, a.dim)
+    _need(size >= 0, "packed attention: %d heads do not share %d key heads evenly" % (a.heads, a.kv_heads))
+    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
+    a.dout, a.out, a.lse = dout.data_ptr(), out.data_ptr(), lse.data_ptr()
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     a.dout_token, a.dout_head = dout.stride()[:2]
     with _On(index) as stream:
