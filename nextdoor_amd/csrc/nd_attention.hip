@@ -101,34 +101,35 @@ __global__ __launch_bounds__(kOrderThreads) void packed_order_kernel(const int32
 template <int NB>
 struct HeadTile {
   static constexpr int kChunks = NB == 1 ? 4 : NB == 2 ? 8 : 16;  // of a row in LDS
-  static constexpr int kTurns = kColumns * kChunks / 256;
-  static constexpr int kSize = kColumns * kChunks;  // of a tile
+  static constexpr int kSize = kColumns * kChunks;                // of a tile
 };
 
-// Brings tiles of 64 rows of one matrix of heads to LDS.  Columns past `dim` are the row's first ones again (the other operand
+// Brings tiles of ROWS rows of one matrix of heads to LDS.  Columns past `dim` are the row's first ones again (the other operand
 // is 0 there, or the result's column is not stored), rows past the last one that one again (they are masked).
-template <int NB>
+template <int NB, int ROWS = kColumns>
 struct TileLoader {
+  static constexpr int kTurns = ROWS * HeadTile<NB>::kChunks / 256;
+  static_assert(kTurns >= 1, "");
   const char* base;
   uint32_t row_bytes;
-  uint32_t offset[HeadTile<NB>::kTurns];
+  uint32_t offset[kTurns];
   __device__ __forceinline__ TileLoader(const void* matrix, int64_t token_bytes, int64_t head_bytes, int head, int dim)
       : base((const char*)matrix + head * head_bytes), row_bytes((uint32_t)token_bytes) {
     constexpr int kChunks = HeadTile<NB>::kChunks;
 #pragma unroll
-    for (int i = 0; i < HeadTile<NB>::kTurns; ++i) {
+    for (int i = 0; i < kTurns; ++i) {
       const int at = threadIdx.x + 256 * i, r = at / kChunks, c = (at % kChunks) ^ tile_swizzle<kChunks>(r);
       offset[i] = r * row_bytes + (c * 8 < dim ? c * 16 : 0);
     }
   }
   __device__ __forceinline__ void issue(uint32_t wave_lds, int64_t token_bytes, int row0, int end) const {
     const char* at = base + row0 * token_bytes;
-    if (row0 + kColumns <= end) {
+    if (row0 + ROWS <= end) {
 #pragma unroll
-      for (int i = 0; i < HeadTile<NB>::kTurns; ++i) load_to_lds(at, offset[i], wave_lds + 4096 * i);
+      for (int i = 0; i < kTurns; ++i) load_to_lds(at, offset[i], wave_lds + 4096 * i);
     } else {
 #pragma unroll
-      for (int i = 0; i < HeadTile<NB>::kTurns; ++i) {
+      for (int i = 0; i < kTurns; ++i) {
         const int r = (threadIdx.x + 256 * i) / HeadTile<NB>::kChunks;
         load_to_lds(at, offset[i] - max(r - (end - 1 - row0), 0) * row_bytes, wave_lds + 4096 * i);
       }
@@ -402,11 +403,18 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
 // over the query tiles that see them, for each head of its share of the group in turn: no sum is shared between
 // workgroups.  Where keys and key heads are few for the GPU, a group's heads are shared out and the sums, in 32 bits, added
 // by another kernel.
+//
+// Heads of up to 128: dk and dv of 32 keys take 128 registers and the keys 32; with the values in registers too a wave has
+// to do without half of its 256 or run alone on its SIMD (long sequences of 4 x 128: 821 us with 43 registers spilled, 569
+// alone).  They are read from LDS instead, and a round takes 32 queries, so that two workgroups fit a compute unit.
 template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(AttentionParams p) {
-  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
+  constexpr int kChunks = HeadTile<NB>::kChunks;
+  constexpr bool kValuesInLds = NB == 4;
+  constexpr int kRound = kValuesInLds ? 32 : 64, kSize = kRound * kChunks;
   __shared__ u32x4 tiles[2][2][kSize];
-  __shared__ float rows_of[2][2][kColumns];  // lse2 and delta of a tile's queries
+  __shared__ u32x4 values[kValuesInLds ? kRows * kChunks : 1];
+  __shared__ float rows_of[2][2][64];  // lse2 and delta of a round's queries
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
   int rank, part;
   tile_and_head(blockIdx.x, p.kv_heads * p.head_split, rank, part);
@@ -422,50 +430,61 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
   if (tile0 < p.plan.covered) {
     const int end = uniform(p.plan.last[min(tile0 + kRows, p.plan.covered) - 1]);
     const int heads = p.group / p.head_split, head0 = kv_head * p.group + share * heads;
-    const TileLoader<NB> q(p.q, p.q_token, p.q_head, head0, p.dim), d(p.dout, p.dout_token, p.dout_head, head0, p.dim);
+    const TileLoader<NB, kRound> q(p.q, p.q_token, p.q_head, head0, p.dim), d(p.dout, p.dout_token, p.dout_head, head0, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024, rows_lds = lds_address(&rows_of[0][0][0]);
     auto issue = [&](int half, int head, int m0) {  // head: of the share
-      TileLoader<NB> qh = q, dh = d;
+      TileLoader<NB, kRound> qh = q, dh = d;
       qh.base += head * p.q_head;
       dh.base += head * p.dout_head;
       qh.issue(lds + (2 * half) * kSize * 16, p.q_token, m0, end);
       dh.issue(lds + (2 * half + 1) * kSize * 16, p.dout_token, m0, end);
       if (wave < 2)
         load_words_to_lds((const char*)((wave == 0 ? p.lse2 : p.delta) + (int64_t)(head0 + head) * p.plan.tokens + m0),
-                          min(lane, end - 1 - m0) * 4, rows_lds + (2 * half + wave) * kColumns * 4);
+                          min(lane, end - 1 - m0) * 4, rows_lds + (2 * half + wave) * 256);
     };
+    if (kValuesInLds) {
+      const TileLoader<NB, kRows> v(p.v, p.v_token, p.v_head, kv_head, p.dim);
+      v.issue(lds_address(values) + wave * 1024, p.v_token, tile0, min(tile0 + kRows, p.plan.covered));
+      if (p.dim < 8 * kChunks) {  // the other operand has a row's first columns past `dim`: 0 here
+        wait_for_loads_and_others();
+        for (int at = threadIdx.x; at < kRows * kChunks; at += 256)
+          if (at % kChunks * 8 >= p.dim) values[tile_place<kChunks>(at / kChunks, at % kChunks)] = u32x4{0, 0, 0, 0};
+      }
+    }
     issue(0, 0, tile0);
     const int last = there ? p.plan.last[key] : key;
     // of the wave's keys: the smallest and the largest `last`
     const int last_min = key0 < p.plan.covered ? uniform(last) : 0;
     const int last_max = key0 < p.plan.covered ? uniform(p.plan.last[min(key0 + 31, p.plan.covered - 1)]) : 0;
-    u32x4 kf[2 * NB], vf[2 * NB];
+    u32x4 kf[2 * NB], vf[kValuesInLds ? 1 : 2 * NB];
     load_rows<NB>(kf, (const char*)p.k + (int64_t)key * p.k_token + (int64_t)kv_head * p.k_head, there, p.dim, h);
-    load_rows<NB>(vf, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, there, p.dim, h);
+    if constexpr (!kValuesInLds)
+      load_rows<NB>(vf, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, there, p.dim, h);
     if (p.flip) {
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) kf[i] ^= p.flip;
     }
     int half = 0, head = 0, m0 = tile0;
     while (head < heads) {
-      int next_head = head, next = m0 + kColumns;
+      int next_head = head, next = m0 + kRound;
       if (next >= end) {
         next = tile0;
         ++next_head;
       }
       wait_for_loads_and_others();
       if (next_head < heads) issue(half ^ 1, next_head, next);
-      if (m0 + kColumns > key0 && m0 < last_max) {  // (else no query of the tile sees a key of the wave)
+      if (m0 + kRound > key0 && m0 < last_max) {  // (else no query of the tile sees a key of the wave)
         const u32x4 *queries = tiles[half][0], *douts = tiles[half][1];
-        const bool masked = m0 < key0 + 31 || m0 + kColumns > last_min;
+        const bool masked = m0 < key0 + 31 || m0 + kRound > last_min;
         const int from = key - m0 - 4 * h, to = last - m0 - 4 * h;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kRound / 32; ++t) {
           f32x16 s = {}, dp = {};
 #pragma unroll
           for (int i = 0; i < 2 * NB; ++i) {
             s = product_32x32x16<T>(read_operand_by_rows<kChunks>(queries, 32 * t, i, lane), kf[i], s);
-            dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(douts, 32 * t, i, lane), vf[i], dp);
+            dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(douts, 32 * t, i, lane),
+                                     kValuesInLds ? read_operand_by_rows<kChunks>(values, 32 * wave, i, lane) : vf[kValuesInLds ? 0 : i], dp);
           }
 #pragma unroll
           for (int g = 0; g < 4; ++g) {

@@ -49,31 +49,33 @@ def _need(condition, message):
         raise NextDoorError(message)
 
 
-def _on_gpu(what, *tensors):
-    """Checks that all tensors lie on one GPU; returns its index."""
-    for t in tensors:
-        _need(isinstance(t, torch.Tensor) and t.is_cuda, "%s: tensors on the GPU only" % what)
-    device = tensors[0].device
-    for t in tensors:
-        _need(t.device == device, "%s: tensors on different devices" % what)
-    return device.index
+def _on_gpu(what, first, *others):
+    """Checks that all are tensors on one GPU; returns its index."""
+    try:
+        index = first.get_device()
+        for t in others:
+            if t.get_device() != index:
+                index = -1
+    except AttributeError:
+        index = -1
+    if index < 0:
+        _need(all(isinstance(t, torch.Tensor) and t.is_cuda for t in (first, *others)), "%s: tensors on the GPU only" % what)
+        raise NextDoorError("%s: tensors on different devices" % what)
+    return index
 
 
-class _On:
-    """Makes a device current for a call, if it is not."""
+_raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream wraps in an object
 
-    def __init__(self, index):
-        self._index = index
-        self._before = torch.cuda.current_device()
 
-    def __enter__(self):
-        if self._before != self._index:
-            torch.cuda.set_device(self._index)
-        return torch.cuda.current_stream(self._index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self._before != self._index:
-            torch.cuda.set_device(self._before)
+def _run(index, fn, *args):
+    """Calls an entry point that takes a stream last, on torch's current one, with the device current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc)
 
 
 # ---- dropout -------------------------------------------------------------------------------------
@@ -91,9 +93,8 @@ def _dropout(x, p, seed, step, residual):
         residual = residual.contiguous()
     x = x.contiguous()
     out = torch.empty_like(x)
-    with _On(index) as stream:
-        check(_library().nd_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
-                                    x.numel(), _DTYPES[x.dtype], p, seed, step, stream))
+    _run(index, _library().nd_dropout, x.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
+         x.numel(), _DTYPES[x.dtype], p, seed, step)
     return out
 
 
@@ -159,43 +160,46 @@ class PackedSequences:
         _need(size >= 0, "packed sequences: no plan for %d tokens" % self.n_tokens)
         on_device = torch.from_numpy(starts).to(self.device)
         self.plan = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
-        with _On(self.device.index) as stream:
-            check(lib.nd_packed_plan(starts.ctypes.data, self.n_sequences, self.n_tokens, on_device.data_ptr(),
-                                     self.plan.data_ptr(), stream))
+        _run(self.device.index, lib.nd_packed_plan, starts.ctypes.data, self.n_sequences, self.n_tokens,
+             on_device.data_ptr(), self.plan.data_ptr())
 
 
-def _heads(what, x, tokens, dim=None):
-    """A [token, head, dim] tensor as the kernels read it: dim side by side, the rest strided by multiples of 16 bytes.
-    Anything else is copied."""
-    _need(x.dim() == 3 and x.shape[0] == tokens, "packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
-    _need(dim is None or x.shape[2] == dim, "packed attention: %s has another head size" % what)
+def _heads(what, x, tokens, dim):
+    """A [token, head, dim] tensor as the kernels read it - dim side by side, the rest strided by multiples of 16 bytes -
+    and its strides.  Anything else is copied."""
+    shape = x.shape
+    _need(len(shape) == 3 and shape[0] == tokens, "packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
+    _need(shape[2] == dim, "packed attention: %s has another head size" % what)
     a, b, c = x.stride()
-    if (c != 1 and x.shape[2] > 1) or a % 8 or b % 8 or a > 16777216 or x.data_ptr() % 16:
+    if (c != 1 and dim > 1) or a % 8 or b % 8 or a > 16777216 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x
+        a, b, c = x.stride()
+    return x, a, b
 
 
-def _attention(sequences, q, k, v, scale):
+def _attention(sequences, q, k, v, scale, dout=None):
+    """Checked arguments: (device index, the tensors read, the struct's first fields, shape of lse)."""
     index = _on_gpu("packed attention", q, k, v, sequences.plan)
-    _need(q.dtype in (torch.float16, torch.bfloat16), "packed attention: 16-bit types only, %s given" % q.dtype)
-    _need(k.dtype == q.dtype and v.dtype == q.dtype, "packed attention: q, k and v are of different types")
-    tokens = sequences.n_tokens
-    q = _heads("q", q, tokens)
-    dim = q.shape[2]
-    k, v = _heads("k", k, tokens, dim), _heads("v", v, tokens, dim)
+    dtype = q.dtype
+    _need(dtype is torch.bfloat16 or dtype is torch.float16, "packed attention: 16-bit types only, %s given" % dtype)
+    _need(k.dtype is dtype and v.dtype is dtype, "packed attention: q, k and v are of different types")
+    tokens, dim = sequences.n_tokens, q.shape[-1]
+    q, q_token, q_head = _heads("q", q, tokens, dim)
+    k, k_token, k_head = _heads("k", k, tokens, dim)
+    v, v_token, v_head = _heads("v", v, tokens, dim)
     _need(k.shape == v.shape, "packed attention: k and v are of different shapes")
-    a = PackedAttention()
-    a.n_tokens, a.n_covered = tokens, sequences.n_covered
-    a.heads, a.kv_heads, a.dim, a.dtype = q.shape[1], k.shape[1], dim, _DTYPES[q.dtype]
-    a.scale = 1 / math.sqrt(dim) if scale is None else scale
-    a.plan = sequences.plan.data_ptr()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_token, a.q_head = q.stride()[:2]
-    a.k_token, a.k_head = k.stride()[:2]
-    a.v_token, a.v_head = v.stride()[:2]
-    return index, a, (q, k, v)
+    heads = q.shape[1]
+    d_at, d_token, d_head = None, 0, 0
+    if dout is not None:
+        _need(dout.shape == q.shape and dout.dtype is dtype, "packed attention: dout is of another shape or type than q")
+        dout, d_token, d_head = _heads("dout", dout, tokens, dim)
+        d_at = dout.data_ptr()
+    fields = (tokens, sequences.n_covered, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
+              sequences.plan.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), d_at,
+              q_token, q_head, k_token, k_head, v_token, v_head, d_token, d_head)
+    return index, (q, k, v, dout), fields, (heads, tokens)
 
 
 def packed_attention_forward(q, k, v, sequences, scale=None):
@@ -205,36 +209,28 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
     multiple of 8 up to 128; float16 or bfloat16.  Slices of one projection are read in place.  lse:
     [heads, tokens], float32, for the backward pass.  ``scale`` is 1 / sqrt(dim) unless given.  Rows of tokens that
     belong to no sequence are 0 (lse -inf) and their inputs are not read."""
-    index, a, keep = _attention(sequences, q, k, v, scale)
+    index, keep, fields, rows = _attention(sequences, q, k, v, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((a.heads, a.n_tokens), dtype=torch.float32, device=q.device)
-    a.out, a.lse = out.data_ptr(), lse.data_ptr()
-    with _On(index) as stream:
-        check(_library().nd_packed_attention_forward(a, stream))
+    lse = torch.empty(rows, dtype=torch.float32, device=q.device)
+    _run(index, _library().nd_packed_attention_forward, PackedAttention(*fields, out.data_ptr(), lse.data_ptr()))
     del keep
     return out, lse
 
 
 def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
     """(dq, dk, dv) for the gradient ``dout`` of ``out``, which with ``lse`` is the forward pass's."""
-    index, a, keep = _attention(sequences, q, k, v, scale)
     _on_gpu("packed attention", q, dout, out, lse)
-    _need(dout.shape == q.shape and dout.dtype == q.dtype, "packed attention: dout is of another shape or type than q")
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and lse.is_contiguous() and
-          lse.dtype == torch.float32 and tuple(lse.shape) == (a.heads, a.n_tokens),
-          "packed attention: out and lse are not a forward pass's")
-    dout = _heads("dout", dout, a.n_tokens)
+    index, keep, fields, rows = _attention(sequences, q, k, v, scale, dout)
+    _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and lse.is_contiguous() and
+          lse.dtype is torch.float32 and lse.shape == rows, "packed attention: out and lse are not a forward pass's")
+    size = _library().nd_packed_attention_workspace(rows[1], rows[0], k.shape[1], q.shape[2])
+    _need(size >= 0, "packed attention: no kernel for %d heads of %d over %d key heads" % (rows[0], q.shape[2], k.shape[1]))
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    size = _library().nd_packed_attention_workspace(a.n_tokens, a.heads, a.kv_heads, a.dim)
-    _need(size >= 0, "packed attention: %d heads do not share %d key heads evenly" % (a.heads, a.kv_heads))
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
-    a.dout, a.out, a.lse = dout.data_ptr(), out.data_ptr(), lse.data_ptr()
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.dout_token, a.dout_head = dout.stride()[:2]
-    with _On(index) as stream:
-        check(_library().nd_packed_attention_backward(a, stream))
+    _run(index, _library().nd_packed_attention_backward,
+         PackedAttention(*fields, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                         workspace.data_ptr(), size))
     del keep
     return dq, dk, dv
 
@@ -270,26 +266,26 @@ def _vectors(x):
 
 
 def _loss(hidden, weight, target, backward):
+    """Checked arguments: (device index, the tensors read, the struct's first fields, workspace, its size)."""
     index = _on_gpu("vocabulary loss", hidden, weight, target)
-    _need(hidden.dtype in (torch.float16, torch.bfloat16), "vocabulary loss: 16-bit types only, %s given" % hidden.dtype)
-    _need(weight.dtype == hidden.dtype, "vocabulary loss: hidden and weight are of different types")
+    dtype = hidden.dtype
+    _need(dtype is torch.bfloat16 or dtype is torch.float16, "vocabulary loss: 16-bit types only, %s given" % dtype)
+    _need(weight.dtype is dtype, "vocabulary loss: hidden and weight are of different types")
     _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1],
           "vocabulary loss: hidden and weight are not matrices of equally long rows")
     hidden, weight = _vectors(hidden), _vectors(weight)
-    _need(target.dim() == 1 and target.shape[0] == hidden.shape[0], "vocabulary loss: one target for each row of hidden")
+    rows, dim = hidden.shape
+    classes = weight.shape[0]
+    _need(target.dim() == 1 and target.shape[0] == rows, "vocabulary loss: one target for each row of hidden")
     _need(target.dtype in (torch.int32, torch.int64), "vocabulary loss: targets are int32 or int64")
-    if target.dtype == torch.int64:  # (what is no class stays none: 2^31 - 1 is above every class)
+    if target.dtype is torch.int64:  # (what is no class stays none: 2^31 - 1 is above every class)
         target = torch.where((target < 0) | (target > 2147483647), 2147483647, target).to(torch.int32)
     target = target.contiguous()
-    a = VocabularyLoss()
-    a.rows, a.dim = hidden.shape
-    a.classes, a.dtype = weight.shape[0], _DTYPES[hidden.dtype]
-    a.hidden, a.weight, a.target = hidden.data_ptr(), weight.data_ptr(), target.data_ptr()
-    size = _library().nd_vocabulary_loss_workspace(a.rows, a.classes, a.dim, backward)
-    _need(size >= 0, "vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (a.rows, a.classes, a.dim))
+    size = _library().nd_vocabulary_loss_workspace(rows, classes, dim, backward)
+    _need(size >= 0, "vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (rows, classes, dim))
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hidden.device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
-    return index, a, (hidden, weight, target, workspace)
+    fields = (rows, classes, dim, _DTYPES[dtype], hidden.data_ptr(), weight.data_ptr(), target.data_ptr())
+    return index, (hidden, weight, target), fields, workspace, size
 
 
 def vocabulary_loss_forward(hidden, weight, target):
@@ -297,11 +293,10 @@ def vocabulary_loss_forward(hidden, weight, target):
     weight_{target_i}``.  hidden: [rows, dim], weight: [classes, dim], float16 or bfloat16 (a dim that is no
     multiple of 8 costs a copy); target: int32 or int64.  A row whose target is no class - the samplers' INVALID is
     |V| - has loss 0."""
-    index, a, keep = _loss(hidden, weight, target, 0)
-    loss, lse = (torch.empty(a.rows, dtype=torch.float32, device=hidden.device) for _ in range(2))
-    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-    with _On(index) as stream:
-        check(_library().nd_vocabulary_loss_forward(a, stream))
+    index, keep, fields, workspace, size = _loss(hidden, weight, target, 0)
+    loss, lse = (torch.empty(fields[0], dtype=torch.float32, device=hidden.device) for _ in range(2))
+    _run(index, _library().nd_vocabulary_loss_forward,
+         VocabularyLoss(*fields, loss.data_ptr(), lse.data_ptr(), None, None, None, workspace.data_ptr(), size))
     del keep
     return loss, lse
 
@@ -309,19 +304,19 @@ def vocabulary_loss_forward(hidden, weight, target):
 def vocabulary_loss_backward(dloss, hidden, weight, target, lse):
     """(dhidden, dweight) for the gradient ``dloss`` of each row's loss; lse is the forward pass's.  Rows without a
     target send nothing back, whatever their ``dloss``."""
-    size = hidden.shape
-    index, a, keep = _loss(hidden, weight, target, 1)
     _on_gpu("vocabulary loss", hidden, dloss, lse)
-    _need(tuple(dloss.shape) == (a.rows,) and tuple(lse.shape) == (a.rows,) and lse.dtype == torch.float32,
+    width = hidden.shape[-1]
+    index, keep, fields, workspace, size = _loss(hidden, weight, target, 1)
+    _need(tuple(dloss.shape) == fields[:1] and tuple(lse.shape) == fields[:1] and lse.dtype is torch.float32,
           "vocabulary loss: dloss and lse have one value for each row")
     dloss, lse = dloss.to(torch.float32).contiguous(), lse.contiguous()
     dhidden, dweight = torch.empty_like(keep[0]), torch.empty_like(keep[1])
-    a.dloss, a.lse, a.dhidden, a.dweight = dloss.data_ptr(), lse.data_ptr(), dhidden.data_ptr(), dweight.data_ptr()
-    with _On(index) as stream:
-        check(_library().nd_vocabulary_loss_backward(a, stream))
+    _run(index, _library().nd_vocabulary_loss_backward,
+         VocabularyLoss(*fields, None, lse.data_ptr(), dloss.data_ptr(), dhidden.data_ptr(), dweight.data_ptr(),
+                        workspace.data_ptr(), size))
     del keep
-    if size[1] != a.dim:
-        dhidden, dweight = dhidden[:, :size[1]].contiguous(), dweight[:, :size[1]].contiguous()
+    if width != fields[2]:
+        dhidden, dweight = dhidden[:, :width].contiguous(), dweight[:, :width].contiguous()
     return dhidden, dweight
 
 

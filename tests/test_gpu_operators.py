@@ -91,7 +91,7 @@ def test_attention_reads_slices_of_a_projection_in_place_and_copies_other_orders
     want, off = ref.attention(q, k, v, starts, 1 / 8, dout)
     a = qkv.cuda()
     split = a.split([heads, kv_heads, kv_heads], 1)
-    assert ops._heads("q", split[0], t) is split[0]
+    assert ops._heads("q", split[0], t, dim)[0] is split[0]
     check_all(run_attention(*split, starts, dout.cuda()), want, off, "slices")
     # heads first; dim not side by side; rows that do not begin at multiples of 16 bytes; a broadcast gradient
     others = [x.cuda().transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
