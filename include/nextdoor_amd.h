@@ -308,23 +308,26 @@ int nd_dropout(const void* d_x, const void* d_residual, void* d_y, int64_t n, in
 /* Packed sequences: sequence i is tokens starts[i] .. starts[i + 1] - 1 of n_tokens; starts[0] = 0, and tokens
  * from starts[n_sequences] on belong to no sequence.  `starts` is the HOST array (n_sequences + 1
  * entries), which is checked, d_starts the same on the device; the plan (nd_packed_plan_bytes(n_tokens)
- * bytes, aligned to 16) is what every attention call over this batch reads. */
+ * bytes, aligned to 16) is what every attention call over this batch reads.  rounds (on the host): how
+ * much work there is in all and in the largest tile, by which attention calls cut it. */
 #define ND_PACKED_MAX_TOKENS 2147483392
 #define ND_PACKED_MAX_DIM 128
 #define ND_PACKED_MAX_TOKEN_STRIDE 16777216
 int64_t nd_packed_plan_bytes(int64_t n_tokens);
 int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
-                   void* stream);
+                   int64_t rounds[2], void* stream);
 
 /* Causal attention within each sequence, heads / kv_heads query heads to a key head.  q, k, v and
  * dout: [token][head][dim] with the strides given (in elements, multiples of 8, >= 0; dim elements
  * lie side by side); out, dq: [n_tokens][heads][dim], dk, dv: [n_tokens][kv_heads][dim], lse:
  * [heads][n_tokens], all dense.  Arrays are aligned to 16 bytes, dim is a multiple of 8.
  * Tokens of no sequence are not read; their rows of out and of the gradients are 0, their lse -inf.
- * The backward call reads what the forward call left in out and lse; its workspace
- * (nd_packed_attention_workspace(...) bytes) is working memory of one call. */
+ * The backward call reads what the forward call left in out and lse.  The workspace
+ * (nd_packed_attention_workspace(...) bytes, which reads the struct's numbers only; may be 0) is
+ * working memory of one call. */
 typedef struct nd_packed_attention {
   int64_t n_tokens, n_covered; /* n_covered = starts[n_sequences] */
+  int64_t rounds, most_rounds; /* nd_packed_plan's */
   int32_t heads, kv_heads, dim, dtype;
   float scale;
   const void* plan;
@@ -336,7 +339,7 @@ typedef struct nd_packed_attention {
   void* workspace;
   int64_t workspace_bytes;
 } nd_packed_attention;
-int64_t nd_packed_attention_workspace(int64_t n_tokens, int32_t heads, int32_t kv_heads, int32_t dim);
+int64_t nd_packed_attention_workspace(const nd_packed_attention* a, int backward);
 int nd_packed_attention_forward(const nd_packed_attention* a, void* stream);
 int nd_packed_attention_backward(const nd_packed_attention* a, void* stream);
 

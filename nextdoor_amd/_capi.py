@@ -14,7 +14,7 @@ c_i64p = C.POINTER(C.c_int64)
 
 class PackedAttention(C.Structure):
     """nd_packed_attention"""
-    _fields_ = ([(n, C.c_int64) for n in ("n_tokens", "n_covered")] +
+    _fields_ = ([(n, C.c_int64) for n in ("n_tokens", "n_covered", "rounds", "most_rounds")] +
                 [(n, C.c_int32) for n in ("heads", "kv_heads", "dim", "dtype")] + [("scale", C.c_float)] +
                 [(n, C.c_void_p) for n in ("plan", "q", "k", "v", "dout")] +
                 [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "dout_token",
@@ -103,8 +103,8 @@ SIGNATURES = {
     "nd_dropout": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int, C.c_double, C.c_uint64, C.c_uint32,
                              C.c_void_p]),
     "nd_packed_plan_bytes": (C.c_int64, [C.c_int64]),
-    "nd_packed_plan": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "nd_packed_attention_workspace": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "nd_packed_plan": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, c_i64p, C.c_void_p]),
+    "nd_packed_attention_workspace": (C.c_int64, [C.POINTER(PackedAttention), C.c_int]),
     "nd_packed_attention_forward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
     "nd_packed_attention_backward": (C.c_int, [C.POINTER(PackedAttention), C.c_void_p]),
     "nd_vocabulary_loss_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int]),

@@ -13,6 +13,9 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "nd_errors.hpp"
 #include "nd_matrix.hpp"
 
@@ -27,6 +30,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // A row's sums are kept relative to a maximum that is taken anew only when it has grown by this much (in powers of two):
 // weights stay below 2^8, which costs 32-bit sums and 16-bit floats nothing, and the sums are rarely scaled again.
 constexpr float kTopSlack = 8.f;
+constexpr int kExactDeltaRounds = 4;
 
 struct PackedPlan {
   const int32_t* first;  // of the sequence a token belongs to; tokens from `covered` on belong to none
@@ -41,10 +45,15 @@ struct AttentionParams {
   const void *q, *k, *v, *out, *dout;
   void *out_w, *dq, *dk, *dv;
   float *lse, *lse2, *delta;  // [heads][tokens]; lse2: in powers of two, for the backward pass
-  float *dk_sums, *dv_sums;   // [split][tokens][kv_heads][dim], if a group's heads are shared out
+  // what the chunks of a tile whose work is cut leave: [chunk][token][head][dim] of out or dq, [chunk][head][token] of
+  // maxima and sums, [chunk][token][kv_head][dim] of dk and dv
+  float *row_sums, *dk_sums, *dv_sums;
+  float2* row_tops;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, dout_token, dout_head;  // in bytes
   int32_t heads, kv_heads, group, dim;
-  int32_t head_split;     // shares of a group's heads
+  int32_t chunk, max_chunks;          // rounds that a workgroup of the query kernels takes, chunks of a tile at most
+  int32_t key_chunk, max_key_chunks;  // of the key kernel
+  int32_t head_split;                 // shares of a group's heads in the key kernel
   float scale, scale_log2;  // scale_log2 > 0
   uint32_t flip;          // sign bits of a pair: q is taken negative for a negative scale
 };
@@ -174,9 +183,35 @@ __device__ __forceinline__ void store_rows(T* first_row, int64_t row_elements, i
   }
 }
 
-// Which tile and head a workgroup has: heads side by side (their tiles share keys), and, where they fill the eight dies
-// evenly, a die's heads next to each other.
-__device__ __forceinline__ void tile_and_head(uint32_t block, int heads, int& rank, int& head) {
+// The same of the lane's token as they are, in 32 bits.
+template <int NB>
+__device__ __forceinline__ void store_sums(float* row, const f32x16 (&acc)[NB], float factor, int dim, int h) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * b + 8 * g + 4 * h;
+      f32x4 v;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v[n] = acc[b][4 * g + n] * factor;
+      if (c < dim) *(f32x4*)(row + c) = v;
+    }
+}
+
+// A tile's rounds are cut into chunks of about `chunk` where that shortens what the GPU would wait for at the end: a long
+// row among short ones, or few rows.  Chunks leave sums in 32 bits that another kernel joins.
+__host__ __device__ __forceinline__ int64_t chunks_of(int64_t rounds, int64_t chunk, int64_t most) {
+  const int64_t n = rounds <= 2 * chunk ? 1 : (rounds + chunk - 1) / chunk;
+  return n < most ? n : most;
+}
+
+// What a workgroup has: heads side by side (their tiles share keys), and, where they fill the eight dies evenly, a die's
+// heads next to each other; then the tiles by falling work; then the chunks, the first ones last.  A chunk that a tile does
+// not have ends at once, but workgroups go to the parts of a die in turn: the empty ones stay together, or half of the GPU
+// would get nothing else (chunks next to each other: 264 us where this takes 177).
+__device__ __forceinline__ void chunk_tile_and_head(int max_chunks, int heads, int& chunk, int& rank, int& head) {
+  const uint32_t each = gridDim.x / max_chunks, block = blockIdx.x % each;
+  chunk = max_chunks - 1 - uniform(blockIdx.x / each);
   rank = uniform(block / heads);
   head = uniform(block % heads);
   if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
@@ -191,8 +226,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
   __shared__ u32x4 tiles[2][2][kSize];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  int rank, head;
-  tile_and_head(blockIdx.x, p.heads, rank, head);
+  int chunk, rank, head;
+  chunk_tile_and_head(p.max_chunks, p.heads, chunk, rank, head);
   const int tile0 = uniform(p.plan.query_order[rank]) * kRows, kv_head = uniform(head / p.group);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
   const bool there = row < p.plan.covered;
@@ -200,9 +235,15 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   float top = -INFINITY, sum = 0.f;  // sum: over the lane's own keys
+  int chunks = 1;
 
   if (tile0 < p.plan.covered) {
-    const int end = min(tile0 + kRows, p.plan.covered), begin = uniform(p.plan.first[tile0]);
+    const int end = min(tile0 + kRows, p.plan.covered), first_key = uniform(p.plan.first[tile0]);
+    const int rounds = (end - first_key + kColumns - 1) / kColumns;
+    chunks = uniform((int)chunks_of(rounds, p.chunk, p.max_chunks));
+    if (chunk >= chunks) return;
+    const int begin = first_key + uniform(rounds * chunk / chunks) * kColumns;
+    const int stop = chunk + 1 < chunks ? first_key + uniform(rounds * (chunk + 1) / chunks) * kColumns : end;
     const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
     auto issue = [&](int half, int n0) {
@@ -221,9 +262,9 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
       for (int i = 0; i < 2 * NB; ++i) qf[i] ^= p.flip;
     }
     int half = 0;
-    for (int n0 = begin; n0 < end; n0 += kColumns, half ^= 1) {
+    for (int n0 = begin; n0 < stop; n0 += kColumns, half ^= 1) {
       wait_for_loads_and_others();
-      if (n0 + kColumns < end) issue(half ^ 1, n0 + kColumns);
+      if (n0 + kColumns < stop) issue(half ^ 1, n0 + kColumns);
       // (wave-uniform) every key is later than the wave's rows, or before their sequences
       if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
       const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
@@ -281,6 +322,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
       }
     }
     __syncthreads();
+  } else if (chunk > 0) {
+    return;
   }
   if (row0 >= p.plan.tokens) return;
   if (row0 + 31 >= p.plan.covered && !there) {  // (tiles that all of the wave's sequences see are not masked)
@@ -290,31 +333,78 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
   sum = pair_sum(sum);
+  if (chunks > 1) {
+    if (row >= p.plan.tokens) return;
+    if (h == 0) p.row_tops[((int64_t)chunk * p.heads + head) * p.plan.tokens + row] = make_float2(top, sum);
+    store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, 1.f, p.dim, h);
+    return;
+  }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
   if (h == 0 && row < p.plan.tokens) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
   store_rows<T, NB>((T*)p.out_w + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, inverse,
                     p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
 }
 
+// Joins the chunks of the rows of cut tiles: a lane has four columns of a row.
+template <class T>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionParams p, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int column = (int)(i % p.dim), head = (int)(i / p.dim % p.heads), row = (int)(i / p.dim / p.heads);
+  const int tile0 = row / kRows * kRows;
+  if (tile0 >= p.plan.covered) return;
+  const int rounds = (min(tile0 + kRows, p.plan.covered) - p.plan.first[tile0] + kColumns - 1) / kColumns;
+  const int chunks = (int)chunks_of(rounds, p.chunk, p.max_chunks);
+  if (chunks == 1) return;
+  const int64_t at = (int64_t)head * p.plan.tokens + row, step = (int64_t)p.heads * p.plan.tokens;
+  float top = -INFINITY;
+  for (int c = 0; c < chunks; ++c) top = fmaxf(top, p.row_tops[c * step + at].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < chunks; ++c) {
+    const float2 one = p.row_tops[c * step + at];
+    const float weight = exp2_fast(one.x - base);
+    sum = __builtin_fmaf(one.y, weight, sum);
+    const f32x4 part = *(const f32x4*)(p.row_sums + c * n + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = weight == 0.f ? v[j] : __builtin_fmaf(part[j], weight, v[j]);
+  }
+  const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  u32x2 o;
+  o[0] = pack_pair<T>(v[0] * inverse, v[1] * inverse);
+  o[1] = pack_pair<T>(v[2] * inverse, v[3] * inverse);
+  *(u32x2*)((T*)p.out_w + i) = o;
+  if (column == 0) p.lse[at] = (top + log2f(sum)) * kLn2;
+}
+
 // ---- backward -----------------------------------------------------------------------------------
 // dq: as the forward pass, with S^T and dP^T = V dO^T; dS^T is the second operand of dQ^T = K^T dS^T.  Leaves delta and lse
 // in powers of two for the other kernel.
+//
+// delta_i = do_i . o_i comes from an o that is rounded to 16 bits, which shifts all of a row's ds by the same amount; the fewer
+// keys a row has, the more that weighs.  Tiles of few keys go over them twice and take delta_i = sum_j p_ij (do_i . v_j), the
+// same sum, in 32 bits.
 template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(AttentionParams p) {
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
   __shared__ u32x4 tiles[2][2][kSize];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  int rank, head;
-  tile_and_head(blockIdx.x, p.heads, rank, head);
+  int chunk, rank, head;
+  chunk_tile_and_head(p.max_chunks, p.heads, chunk, rank, head);
   const int tile0 = uniform(p.plan.query_order[rank]) * kRows, kv_head = uniform(head / p.group);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
   const bool there = row < p.plan.covered;
   f32x16 acc[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
-
+  int chunks = 1;
   if (tile0 < p.plan.covered) {
-    const int end = min(tile0 + kRows, p.plan.covered), begin = uniform(p.plan.first[tile0]);
+    const int end = min(tile0 + kRows, p.plan.covered), first_key = uniform(p.plan.first[tile0]);
+    const int rounds = (end - first_key + kColumns - 1) / kColumns;
+    chunks = uniform((int)chunks_of(rounds, p.chunk, p.max_chunks));
+    if (chunk >= chunks) return;
+    const int begin = first_key + uniform(rounds * chunk / chunks) * kColumns;
+    const int stop = chunk + 1 < chunks ? first_key + uniform(rounds * (chunk + 1) / chunks) * kColumns : end;
+    const bool exact = chunks == 1 && rounds <= kExactDeltaRounds;
     const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
     auto issue = [&](int half, int n0) {
@@ -343,56 +433,86 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
       if (there) {
         const int64_t at = (int64_t)head * p.plan.tokens + row;
         lse2 = p.lse[at] * kLog2e;
-        if (h == 0) {
+        if (h == 0 && chunk == 0) {
           p.delta[at] = delta;
           p.lse2[at] = lse2;
         }
       }
+      if (exact) delta = 0.f;
     }
     if (p.flip) {
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) qf[i] ^= p.flip;
     }
     int half = 0;
-    for (int n0 = begin; n0 < end; n0 += kColumns, half ^= 1) {
-      wait_for_loads_and_others();
-      if (n0 + kColumns < end) issue(half ^ 1, n0 + kColumns);
-      if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
-      const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
-      const bool masked = n0 + kColumns - 1 > row0 || n0 < first_max;
-      const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
+    // one sweep over the keys; DELTA: the first of two, for delta (then the first tile is asked for again at its end)
+    auto sweep = [&](auto delta_only) {
+      constexpr bool DELTA = decltype(delta_only)::value;
+      float sum = 0.f;
+      for (int n0 = begin; n0 < stop; n0 += kColumns, half ^= 1) {
+        wait_for_loads_and_others();
+        if (n0 + kColumns < stop) issue(half ^ 1, n0 + kColumns);
+        else if (DELTA) issue(half ^ 1, begin);
+        if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
+        const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
+        const bool masked = n0 + kColumns - 1 > row0 || n0 < first_max;
+        const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x16 s = {}, dp = {};
+        for (int t = 0; t < 2; ++t) {
+          f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) {
-          s = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s);
-          dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
-        }
+          for (int i = 0; i < 2 * NB; ++i) {
+            s = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s);
+            dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
+          }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
-        if (masked) {
+          for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = 32 * t + 8 * (i / 4) + i % 4;
-            s[i] = key >= from && key <= to ? s[i] : 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const int key = 32 * t + 8 * (i / 4) + i % 4;
+              s[i] = key >= from && key <= to ? s[i] : 0.f;
+            }
+          }
+          if constexpr (DELTA) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += s[i];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const u32x4 dsf = pack_operand<T>(s, j);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(keys, 32 * t + 16 * j, 32 * b, lane), dsf,
+                                             acc[b]);
+            }
           }
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const u32x4 dsf = pack_operand<T>(s, j);
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(keys, 32 * t + 16 * j, 32 * b, lane), dsf,
-                                         acc[b]);
-        }
       }
-    }
+      if constexpr (DELTA) {
+        delta = pair_sum(sum);
+        if (h == 0 && there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
+      }
+    };
+    if (exact) sweep(std::true_type());
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+    sweep(std::false_type());
     __syncthreads();
+  } else if (chunk > 0) {
+    return;
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
   if (row0 + 31 >= p.plan.covered && !there) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  }
+  if (chunks > 1) {
+    if (row < p.plan.tokens)
+      store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, p.scale, p.dim, h);
+    return;
   }
   if (row0 < p.plan.tokens)
     store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, p.scale,
@@ -401,8 +521,8 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
 
 // dk, dv: one workgroup has 128 keys of one key head, a wave 32 of them (lane's key is a column of S = Q K^T), and goes
 // over the query tiles that see them, for each head of its share of the group in turn: no sum is shared between
-// workgroups.  Where keys and key heads are few for the GPU, a group's heads are shared out and the sums, in 32 bits, added
-// by another kernel.
+// workgroups.  Where keys and key heads are few for the GPU a group's heads are shared out; shares and chunks leave sums in
+// 32 bits, which another kernel adds.
 //
 // Heads of up to 128: dk and dv of 32 keys take 128 registers and the keys 32; with the values in registers too a wave has
 // to do without half of its 256 or run alone on its SIMD (long sequences of 4 x 128: 821 us with 43 registers spilled, 569
@@ -416,9 +536,10 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
   __shared__ u32x4 values[kValuesInLds ? kRows * kChunks : 1];
   __shared__ float rows_of[2][2][64];  // lse2 and delta of a round's queries
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  int rank, part;
-  tile_and_head(blockIdx.x, p.kv_heads * p.head_split, rank, part);
-  const int tile0 = uniform(p.plan.key_order[rank]) * kRows, kv_head = uniform(part / p.head_split), share = part % p.head_split;
+  int chunk, rank, unit;
+  chunk_tile_and_head(p.max_key_chunks, p.kv_heads * p.head_split, chunk, rank, unit);
+  const int kv_head = uniform(unit / p.head_split), share = unit - kv_head * p.head_split, heads = uniform(p.group / p.head_split);
+  const int tile0 = uniform(p.plan.key_order[rank]) * kRows;
   const int key0 = tile0 + wave * 32, key = key0 + (lane & 31);
   const bool there = key < p.plan.covered;
   f32x16 dk[NB], dv[NB];
@@ -427,9 +548,14 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     dk[b] = f32x16{};
     dv[b] = f32x16{};
   }
+  int chunks = 1;
   if (tile0 < p.plan.covered) {
     const int end = uniform(p.plan.last[min(tile0 + kRows, p.plan.covered) - 1]);
-    const int heads = p.group / p.head_split, head0 = kv_head * p.group + share * heads;
+    const int head0 = kv_head * p.group + share * heads, head_rounds = (end - tile0 + kRound - 1) / kRound, rounds = head_rounds * heads;
+    chunks = uniform((int)chunks_of(rounds, p.key_chunk, p.max_key_chunks));
+    if (chunk >= chunks) return;
+    // round i: head i / head_rounds of the share, queries from tile0 + i % head_rounds * kRound on
+    const int begin = uniform((int)((int64_t)rounds * chunk / chunks)), stop = uniform((int)((int64_t)rounds * (chunk + 1) / chunks));
     const TileLoader<NB, kRound> q(p.q, p.q_token, p.q_head, head0, p.dim), d(p.dout, p.dout_token, p.dout_head, head0, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024, rows_lds = lds_address(&rows_of[0][0][0]);
     auto issue = [&](int half, int head, int m0) {  // head: of the share
@@ -451,7 +577,8 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
           if (at % kChunks * 8 >= p.dim) values[tile_place<kChunks>(at / kChunks, at % kChunks)] = u32x4{0, 0, 0, 0};
       }
     }
-    issue(0, 0, tile0);
+    int head = uniform(begin / head_rounds), m0 = tile0 + uniform(begin % head_rounds) * kRound;
+    issue(0, head, m0);
     const int last = there ? p.plan.last[key] : key;
     // of the wave's keys: the smallest and the largest `last`
     const int last_min = key0 < p.plan.covered ? uniform(last) : 0;
@@ -464,15 +591,15 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) kf[i] ^= p.flip;
     }
-    int half = 0, head = 0, m0 = tile0;
-    while (head < heads) {
+    int half = 0;
+    for (int round = begin; round < stop; ++round) {
       int next_head = head, next = m0 + kRound;
       if (next >= end) {
         next = tile0;
         ++next_head;
       }
       wait_for_loads_and_others();
-      if (next_head < heads) issue(half ^ 1, next_head, next);
+      if (round + 1 < stop) issue(half ^ 1, next_head, next);
       if (m0 + kRound > key0 && m0 < last_max) {  // (else no query of the tile sees a key of the wave)
         const u32x4 *queries = tiles[half][0], *douts = tiles[half][1];
         const bool masked = m0 < key0 + 31 || m0 + kRound > last_min;
@@ -524,46 +651,45 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
       half ^= 1;
     }
     __syncthreads();
+  } else if (chunk > 0) {
+    return;
   }
   if (key0 >= p.plan.tokens) return;
   const int64_t row_elements = (int64_t)p.kv_heads * p.dim;
-  if (p.head_split == 1) {
+  if (chunks * p.head_split == 1) {
     u32x4* part_lds = &tiles[0][0][0] + wave * 32 * kChunks;
     const int64_t at = ((int64_t)key0 * p.kv_heads + kv_head) * p.dim;
     store_rows<T, NB>((T*)p.dk + at, row_elements, p.plan.tokens - key0, dk, p.scale, p.dim, part_lds);
     store_rows<T, NB>((T*)p.dv + at, row_elements, p.plan.tokens - key0, dv, 1.f, p.dim, part_lds);
   } else if (key < p.plan.tokens) {
-    const int64_t at = (((int64_t)share * p.plan.tokens + key) * p.kv_heads + kv_head) * p.dim;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int c = 32 * b + 8 * g + 4 * h;
-        if (c >= p.dim) continue;
-        f32x4 a, e;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          a[n] = dk[b][4 * g + n] * p.scale;
-          e[n] = dv[b][4 * g + n];
-        }
-        *(f32x4*)(p.dk_sums + at + c) = a;
-        *(f32x4*)(p.dv_sums + at + c) = e;
-      }
+    const int64_t at = (((int64_t)(chunk * p.head_split + share) * p.plan.tokens + key) * p.kv_heads + kv_head) * p.dim;
+    store_sums<NB>(p.dk_sums + at, dk, p.scale, p.dim, h);
+    store_sums<NB>(p.dv_sums + at, dv, 1.f, p.dim, h);
   }
 }
 
-// dk and dv from the shares' sums: n values each, a multiple of 8.
+// Adds the chunks of cut tiles: dq (WHICH 0), dk (1), dv (2); n values each, a lane has four.
 template <class T>
-__global__ __launch_bounds__(256) void add_shares_kernel(AttentionParams p, int64_t n) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  const float* sums = blockIdx.y ? p.dv_sums : p.dk_sums;
+__global__ __launch_bounds__(256) void attention_add_kernel(AttentionParams p, int64_t n_rows, int64_t n_keys, int key_round) {
+  const int which = blockIdx.y;
+  const int64_t n = which == 0 ? n_rows : n_keys, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n || (which == 0 ? p.max_chunks : p.max_key_chunks * p.head_split) == 1) return;
+  const int token = (int)(i / p.dim / (which == 0 ? p.heads : p.kv_heads)), tile0 = token / kRows * kRows;
+  if (tile0 >= p.plan.covered) return;
+  const int tile_end = min(tile0 + kRows, p.plan.covered);
+  int chunks;
+  if (which == 0) chunks = (int)chunks_of((tile_end - p.plan.first[tile0] + kColumns - 1) / kColumns, p.chunk, p.max_chunks);
+  else
+    chunks = (int)chunks_of((p.plan.last[tile_end - 1] - tile0 + key_round - 1) / key_round * (p.group / p.head_split), p.key_chunk, p.max_key_chunks);
+  if (which > 0) chunks *= p.head_split;
+  if (chunks == 1) return;
+  const float* sums = which == 0 ? p.row_sums : which == 1 ? p.dk_sums : p.dv_sums;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.head_split; ++s) v += *(const f32x4*)(sums + s * n + i);
+  for (int c = 0; c < chunks; ++c) v += *(const f32x4*)(sums + c * n + i);
   u32x2 o;
   o[0] = pack_pair<T>(v[0], v[1]);
   o[1] = pack_pair<T>(v[2], v[3]);
-  *(u32x2*)((T*)(blockIdx.y ? p.dv : p.dk) + i) = o;
+  *(u32x2*)((T*)(which == 0 ? p.dq : which == 1 ? p.dk : p.dv) + i) = o;
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -584,40 +710,67 @@ PlanParts plan_parts(int64_t tokens) {
   return w;
 }
 
-// Shares of a group's heads in the dk, dv kernel: as many as it takes for four workgroups to a compute unit.
-int head_split_of(int64_t tokens, int kv_heads, int group) {
-  const int64_t tiles = tiles_of(tokens) * kv_heads;
-  for (int split = 1; split < group; ++split)
-    if (group % split == 0 && tiles * split >= 1024) return split;
-  return group;
-}
-
-// The backward pass's working memory, in bytes: lse2, delta, and the shares' sums.
-struct WorkParts {
-  int64_t delta, dk_sums, dv_sums, bytes;
+// How the work is cut into chunks, and the parts of the workspace in bytes.  About kItems equal pieces of work fill the GPU
+// (512 workgroups at a time) twice over; a tile with much more than its share of them is cut (one sequence of 8192 tokens and
+// two heads: 128 tiles of up to 128 rounds).
+constexpr int64_t kItems = 1024;
+constexpr int64_t kMostChunkBytes = (int64_t)1 << 30;
+struct Cuts {
+  int64_t chunk, max_chunks, key_chunk, max_key_chunks, head_split;
+  int64_t delta, row_sums, row_tops, dk_sums, dv_sums, bytes;
 };
-WorkParts work_parts(int64_t tokens, int heads, int kv_heads, int dim) {
-  WorkParts w;
-  const int split = head_split_of(tokens, kv_heads, heads / kv_heads);
-  const int64_t sums = split > 1 ? round_up(split * tokens * kv_heads * dim * 4, 256) : 0;
-  w.delta = round_up(tokens * heads * 4, 256);
-  w.dk_sums = 2 * w.delta;
-  w.dv_sums = w.dk_sums + sums;
-  w.bytes = w.dv_sums + sums;
+int64_t key_round_of(int dim) { return dim > 96 ? 32 : 64; }
+Cuts cuts_of(const nd_packed_attention& a, bool backward) {
+  Cuts w = {};
+  auto most = [](int64_t largest, int64_t chunk, int64_t bytes_each) {
+    return chunks_of(largest, chunk, std::max<int64_t>(1, kMostChunkBytes / std::max<int64_t>(bytes_each, 1)));
+  };
+  auto take = [&](int64_t bytes) {
+    const int64_t at = w.bytes;
+    w.bytes += round_up(bytes, 256);
+    return at;
+  };
+  const int64_t row_bytes = a.n_tokens * a.heads * a.dim * 4, key_bytes = a.n_tokens * a.kv_heads * a.dim * 4;
+  w.chunk = std::max<int64_t>(8, (a.rounds * a.heads + kItems - 1) / kItems);
+  w.max_chunks = most(a.most_rounds, w.chunk, row_bytes);
+  w.max_key_chunks = w.key_chunk = w.head_split = 1;
+  if (backward) {
+    const int64_t finer = kColumns / key_round_of(a.dim), group = a.heads / a.kv_heads;
+    while (w.head_split < group && (group % w.head_split != 0 || tiles_of(a.n_tokens) * a.kv_heads * w.head_split < kItems))
+      ++w.head_split;
+    w.key_chunk = std::min<int64_t>(w.chunk * finer, 0x3fffffff);
+    w.max_key_chunks = most(a.most_rounds * finer * (group / w.head_split), w.key_chunk, key_bytes * w.head_split);
+    take(a.n_tokens * a.heads * 4);  // lse2
+    w.delta = take(a.n_tokens * a.heads * 4);
+  }
+  w.chunk = std::min<int64_t>(w.chunk, 0x3fffffff);
+  if (w.max_chunks > 1) w.row_sums = take(w.max_chunks * row_bytes);
+  if (w.max_chunks > 1 && !backward) w.row_tops = take(w.max_chunks * a.n_tokens * a.heads * (int64_t)sizeof(float2));
+  if (w.max_key_chunks * w.head_split > 1) {
+    w.dk_sums = take(w.max_key_chunks * w.head_split * key_bytes);
+    w.dv_sums = take(w.max_key_chunks * w.head_split * key_bytes);
+  }
   return w;
 }
 
 template <class T, int NB>
 void launch_forward(const AttentionParams& p, hipStream_t stream) {
-  attention_forward_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads, 256, 0, stream>>>(p);
+  attention_forward_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
+  if (p.max_chunks > 1) {
+    const int64_t n = (int64_t)p.plan.tokens * p.heads * p.dim;
+    attention_join_kernel<T><<<(uint32_t)((n / 4 + 255) / 256), 256, 0, stream>>>(p, n);
+  }
 }
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
-  attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads, 256, 0, stream>>>(p);
-  attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split, 256, 0, stream>>>(p);
-  if (p.head_split > 1) {
-    const int64_t n = (int64_t)p.plan.tokens * p.kv_heads * p.dim;
-    add_shares_kernel<T><<<dim3((uint32_t)((n / 4 + 255) / 256), 2), 256, 0, stream>>>(p, n);
+  attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
+  attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split * p.max_key_chunks, 256, 0, stream>>>(p);
+  const bool add_keys = p.max_key_chunks * p.head_split > 1;
+  if (p.max_chunks > 1 || add_keys) {
+    const int64_t n_rows = (int64_t)p.plan.tokens * p.heads * p.dim, n_keys = (int64_t)p.plan.tokens * p.kv_heads * p.dim;
+    const int64_t n = p.max_chunks > 1 ? n_rows : n_keys;
+    attention_add_kernel<T><<<dim3((uint32_t)((n / 4 + 255) / 256), add_keys ? 3 : 1), 256, 0, stream>>>(
+        p, n_rows, n_keys, (int)key_round_of(p.dim));
   }
 }
 
@@ -646,9 +799,10 @@ int check_attention(const nd_packed_attention* a, bool backward) {
                 std::to_string(a->dim) + " given");
   if (!isfinite(a->scale)) return fail("packed attention: the scale is not finite");
   if (a->n_tokens == 0) return 0;
-  if (tiles_of(a->n_tokens) * a->heads > 0x7fffffff) return fail("packed attention: more tokens and heads than one launch holds");
-  const void* in[] = {a->q, a->k, a->v, a->out, a->lse, a->plan, a->dout, a->dq, a->dk, a->dv, a->workspace};
-  for (int i = 0; i < (backward ? 11 : 6); ++i) {
+  if (a->rounds < 0 || a->most_rounds < 0 || a->most_rounds > a->n_tokens / kColumns + 2)
+    return fail("packed attention: rounds that no plan of these tokens has");
+  const void* in[] = {a->q, a->k, a->v, a->out, a->lse, a->plan, a->dout, a->dq, a->dk, a->dv};
+  for (int i = 0; i < (backward ? 10 : 6); ++i) {
     if (!in[i]) return fail("packed attention: null array");
     if ((uintptr_t)in[i] & 15) return fail("packed attention: arrays are aligned to 16 bytes");
   }
@@ -657,12 +811,14 @@ int check_attention(const nd_packed_attention* a, bool backward) {
     if (strides[i] < 0 || strides[i] % 8 != 0 || (i % 2 == 0 && strides[i] > ND_PACKED_MAX_TOKEN_STRIDE))
       return fail("packed attention: strides are multiples of 8 elements, a token's at most " +
                   std::to_string(ND_PACKED_MAX_TOKEN_STRIDE));
-  if (backward) {
-    const int64_t bytes = work_parts(a->n_tokens, a->heads, a->kv_heads, a->dim).bytes;
-    if (a->workspace_bytes < bytes)
-      return fail("packed attention: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(bytes) +
-                  " needed");
-  }
+  const Cuts cuts = cuts_of(*a, backward);
+  if (tiles_of(a->n_tokens) * a->heads * std::max(cuts.max_chunks, cuts.max_key_chunks) > 0x7fffffff)
+    return fail("packed attention: more tokens and heads than one launch holds");
+  if (a->workspace_bytes < cuts.bytes)
+    return fail("packed attention: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(cuts.bytes) +
+                " needed");
+  if (cuts.bytes > 0 && (!a->workspace || ((uintptr_t)a->workspace & 15)))
+    return fail("packed attention: null workspace, or one not aligned to 16 bytes");
   return 0;
 }
 
@@ -687,15 +843,19 @@ int run_attention(const nd_packed_attention* a, bool backward, void* stream) {
   p.dk = a->dk;
   p.dv = a->dv;
   p.lse = a->lse;
-  p.head_split = 1;
-  if (backward) {
-    const WorkParts w = work_parts(a->n_tokens, a->heads, a->kv_heads, a->dim);
-    p.lse2 = (float*)a->workspace;
-    p.delta = (float*)((char*)a->workspace + w.delta);
-    p.dk_sums = (float*)((char*)a->workspace + w.dk_sums);
-    p.dv_sums = (float*)((char*)a->workspace + w.dv_sums);
-    p.head_split = head_split_of(a->n_tokens, a->kv_heads, a->heads / a->kv_heads);
-  }
+  const Cuts w = cuts_of(*a, backward);
+  char* work = (char*)a->workspace;
+  p.lse2 = (float*)work;
+  p.delta = (float*)(work + w.delta);
+  p.row_sums = (float*)(work + w.row_sums);
+  p.row_tops = (float2*)(work + w.row_tops);
+  p.dk_sums = (float*)(work + w.dk_sums);
+  p.dv_sums = (float*)(work + w.dv_sums);
+  p.chunk = (int32_t)w.chunk;
+  p.max_chunks = (int32_t)w.max_chunks;
+  p.key_chunk = (int32_t)w.key_chunk;
+  p.max_key_chunks = (int32_t)w.max_key_chunks;
+  p.head_split = (int32_t)w.head_split;
   p.q_token = a->q_token * 2;
   p.q_head = a->q_head * 2;
   p.k_token = a->k_token * 2;
@@ -730,7 +890,7 @@ int64_t nd_packed_plan_bytes(int64_t n_tokens) {
 }
 
 int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
-                   void* stream) {
+                   int64_t rounds[2], void* stream) {
   return nd::guarded([&]() -> int {
     if (n_tokens < 0 || n_tokens > ND_PACKED_MAX_TOKENS || n_sequences < 0 || n_sequences > ND_PACKED_MAX_TOKENS)
       return nd::fail("packed sequences: between 0 and " + std::to_string((int64_t)ND_PACKED_MAX_TOKENS) + " tokens and sequences");
@@ -742,6 +902,18 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
     if (starts[n_sequences] > n_tokens)
       return nd::fail("packed sequences: " + std::to_string(starts[n_sequences]) + " tokens in sequences, " +
                       std::to_string(n_tokens) + " tokens");
+    if (!rounds) return nd::fail("packed sequences: null array");
+    rounds[0] = rounds[1] = 0;
+    int64_t of = 0;  // the sequence that a tile's first token is in
+    for (int64_t t = 0; t < starts[n_sequences]; t += nd::kRows) {
+      while (starts[of + 1] <= t) ++of;
+      const int64_t end = std::min<int64_t>(t + nd::kRows, starts[n_sequences]);
+      const int64_t one = (end - starts[of] + nd::kColumns - 1) / nd::kColumns;
+      rounds[0] += one;
+      // as a tile of queries, and as one of keys (whose last token's sequence may end after it)
+      const int32_t* after = std::upper_bound(starts + of + 1, starts + n_sequences + 1, (int32_t)(end - 1));
+      rounds[1] = std::max(rounds[1], std::max(one, (*after - t + nd::kColumns - 1) / nd::kColumns));
+    }
     if (n_tokens == 0) return 0;
     if (!d_starts || !d_plan || ((uintptr_t)d_plan & 15)) return nd::fail("packed sequences: null or misaligned device array");
     int32_t* first = (int32_t*)d_plan;
@@ -757,11 +929,11 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
   });
 }
 
-int64_t nd_packed_attention_workspace(int64_t n_tokens, int32_t heads, int32_t kv_heads, int32_t dim) {
-  if (n_tokens < 0 || n_tokens > ND_PACKED_MAX_TOKENS || kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || dim < 1 ||
-      dim > ND_PACKED_MAX_DIM)
+int64_t nd_packed_attention_workspace(const nd_packed_attention* a, int backward) {
+  if (!a || a->n_tokens < 0 || a->n_tokens > ND_PACKED_MAX_TOKENS || a->rounds < 0 || a->most_rounds < 0 || a->kv_heads < 1 ||
+      a->heads < a->kv_heads || a->heads % a->kv_heads != 0 || a->dim < 1 || a->dim > ND_PACKED_MAX_DIM)
     return -1;
-  return nd::work_parts(n_tokens, heads, kv_heads, dim).bytes;
+  return nd::cuts_of(*a, backward != 0).bytes;
 }
 
 int nd_packed_attention_forward(const nd_packed_attention* a, void* stream) {

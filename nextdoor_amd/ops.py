@@ -15,6 +15,7 @@ types and shapes that the kernels do not have are errors (:class:`NextDoorError`
 Import this module (or torch) before the first call into the library: torch brings its own HIP
 runtime, and streams and memory can only be shared within one.
 """
+import ctypes as C
 import math
 
 import numpy as np
@@ -160,8 +161,10 @@ class PackedSequences:
         _need(size >= 0, "packed sequences: no plan for %d tokens" % self.n_tokens)
         on_device = torch.from_numpy(starts).to(self.device)
         self.plan = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
+        rounds = (C.c_int64 * 2)()
         _run(self.device.index, lib.nd_packed_plan, starts.ctypes.data, self.n_sequences, self.n_tokens,
-             on_device.data_ptr(), self.plan.data_ptr())
+             on_device.data_ptr(), self.plan.data_ptr(), rounds)
+        self.rounds = rounds[0], rounds[1]
 
 
 def _heads(what, x, tokens, dim):
@@ -196,10 +199,20 @@ def _attention(sequences, q, k, v, scale, dout=None):
         _need(dout.shape == q.shape and dout.dtype is dtype, "packed attention: dout is of another shape or type than q")
         dout, d_token, d_head = _heads("dout", dout, tokens, dim)
         d_at = dout.data_ptr()
-    fields = (tokens, sequences.n_covered, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
+    fields = (tokens, sequences.n_covered, *sequences.rounds, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
               sequences.plan.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), d_at,
               q_token, q_head, k_token, k_head, v_token, v_head, d_token, d_head)
     return index, (q, k, v, dout), fields, (heads, tokens)
+
+
+def _workspace(a, backward, device):
+    """The workspace of a call, if it needs one (a call that no kernel can do has none: the call says why)."""
+    size = _library().nd_packed_attention_workspace(a, backward)
+    if size <= 0:
+        return None
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    return workspace
 
 
 def packed_attention_forward(q, k, v, sequences, scale=None):
@@ -212,8 +225,10 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
     index, keep, fields, rows = _attention(sequences, q, k, v, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(rows, dtype=torch.float32, device=q.device)
-    _run(index, _library().nd_packed_attention_forward, PackedAttention(*fields, out.data_ptr(), lse.data_ptr()))
-    del keep
+    a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr())
+    workspace = _workspace(a, 0, q.device)
+    _run(index, _library().nd_packed_attention_forward, a)
+    del keep, workspace
     return out, lse
 
 
@@ -223,15 +238,12 @@ def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
     index, keep, fields, rows = _attention(sequences, q, k, v, scale, dout)
     _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and lse.is_contiguous() and
           lse.dtype is torch.float32 and lse.shape == rows, "packed attention: out and lse are not a forward pass's")
-    size = _library().nd_packed_attention_workspace(rows[1], rows[0], k.shape[1], q.shape[2])
-    _need(size >= 0, "packed attention: no kernel for %d heads of %d over %d key heads" % (rows[0], q.shape[2], k.shape[1]))
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=q.device)
-    _run(index, _library().nd_packed_attention_backward,
-         PackedAttention(*fields, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                         workspace.data_ptr(), size))
-    del keep
+    a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    workspace = _workspace(a, 1, q.device)
+    _run(index, _library().nd_packed_attention_backward, a)
+    del keep, workspace
     return dq, dk, dv
 
 
