@@ -5,23 +5,28 @@
 // A row whose target is no class (the engine's "no vertex" is |V|) has loss 0 and no gradient.
 //
 // The logits are never kept.  Forward: a workgroup makes a tile of Z^T = W H^T and keeps one maximum and one sum of a row
-// for it; a second kernel joins them.  Backward: for one piece of the vocabulary after another the tiles are made again,
-// turned into g (16 bits, in a workspace of one piece) and multiplied by w and by h.
+// for it; a second kernel joins them.  Backward, vectors of up to 128: dh and dw each make the logits once more and turn them
+// into g in registers, where it is the operand of their second product.  Longer vectors: the logits are made once more for one
+// piece of the vocabulary after another, and g (16 bits, in a workspace of one piece) is multiplied by w and by h.
 #include "../../include/nextdoor_amd.h"
 
 #include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nd_errors.hpp"
 #include "nd_matrix.hpp"
+#include "nd_row_tiles.hpp"
 
 namespace nd {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kGradientOne = 32768.f;  // what |g| = max |dloss| is held as (below the largest 16-bit float)
+// What g is held times: in 16-bit floats such that max |dloss| becomes this (below their largest); bfloat16 has the exponents of
+// 32 bits, and a constant keeps the smallest weights of a mean over millions of rows among the normal numbers.
+constexpr float kGradientOne = 32768.f, kGradientScale = 4294967296.f;
 constexpr int kClassPad = 256;           // a piece of the vocabulary is filled up to a multiple of it
 
 struct LossParams {
@@ -36,8 +41,11 @@ struct LossParams {
   u32x4* gradient;     // backward: g of one piece of the vocabulary, see gradient_place
   float* dhidden_sums; // [split][rows][dim]
   float* dweight_sums; // [split][classes of the piece][dim]
-  float* largest;      // max |dloss|
+  float* scale;        // what g is held times, and one over it
   void* hidden_known;  // hidden, filled up to padded_rows; rows without a target are zero
+  // of a row: g = +-exp2(z log2(e) + shift) - [class = target] each; no target: each 0, shift -inf, target -1
+  float *row_each, *row_shift;
+  int32_t* row_target;
   int32_t padded_rows;
   int32_t class0, class_end;  // the piece
   int32_t dhidden_split, dweight_split;
@@ -260,7 +268,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, in
   f32x16 z[S::kM][S::kN];
   // (a tile of nothing but the piece's filling has no class to read: it reads the last one, and g is 0)
   multiply<T, S, false>(z, Classes(p.weight, row_bytes, min(class0, p.class_end - 1), p.class_end, p.dim),
-                        Rows(p.hidden, row_bytes, row0, p.rows, p.dim), 0, p.dim, tiles);
+                        Rows(BACKWARD ? p.hidden_known : p.hidden, row_bytes, row0, BACKWARD ? p.padded_rows : p.rows, p.dim), 0, p.dim, tiles);
   const int wave_class0 = class0 + wave / S::kWavesN * 32 * S::kM;
   const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN;
   const bool whole = wave_class0 + 32 * S::kM <= p.class_end;
@@ -290,28 +298,117 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, in
       if (h == 0 && row < p.rows)
         p.partials[((int64_t)class_tile * S::kWavesM + wave / S::kWavesN) * p.rows + row] = make_float2(m2, sum);
     } else {
-      const bool there = row < p.rows;
-      const int target = there ? p.target[row] : -1;
-      const bool has = target >= 0 && target < p.classes;
-      const float largest = *p.largest;
-      const float each = has && largest > 0.f ? p.dloss[row] / largest * kGradientOne : 0.f;
-      const float lse2 = there ? p.lse[row] * kLog2e : 0.f;
+      const int target = p.row_target[row];
+      const float each = p.row_each[row], shift = p.row_shift[row];
+      const uint32_t negative = each < 0.f ? 0x80000000u : 0u;
+      const bool targets_here = __builtin_amdgcn_ballot_w64(target >= wave_class0 && target < wave_class0 + 32 * S::kM) != 0;
+      const bool negatives = __builtin_amdgcn_ballot_w64(negative) != 0;
 #pragma unroll
       for (int i = 0; i < S::kM; ++i) {
-        const int c0 = wave_class0 + 32 * i + 4 * h;
         f32x16 g;
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          const int c = c0 + 8 * (n / 4) + n % 4;
-          float v = exp2_fast(__builtin_fmaf(z[i][j][n], kLog2e, -lse2));
-          if (c == target) v -= 1.f;
-          g[n] = has && c < p.class_end ? v * each : 0.f;
+        for (int n = 0; n < 16; ++n) g[n] = exp2_fast(__builtin_fmaf(z[i][j][n], kLog2e, shift));
+        if (negatives) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n) g[n] = __uint_as_float(__float_as_uint(g[n]) ^ negative);
+        }
+        if (targets_here || !whole) {
+          const int c0 = wave_class0 + 32 * i + 4 * h;
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const int c = c0 + 8 * (n / 4) + n % 4;
+            if (c == target) g[n] -= each;
+            if (c >= p.class_end) g[n] = 0.f;
+          }
         }
         const int64_t at = (int64_t)((wave_class0 - p.class0) / 32 + i) * (p.padded_rows / 32) + (row - (lane & 31)) / 32;
 #pragma unroll
         for (int s = 0; s < 2; ++s) p.gradient[at * kGradientBlock + gradient_place(lane & 31, s, h)] = pack_operand<T>(g, s);
       }
     }
+  }
+}
+
+constexpr int kRound = 64;  // rows of the other side in a round of the kernels for short vectors
+
+// Rounds of a share of n: whole ones, spread evenly.
+__device__ __forceinline__ void rounds_of(int rounds, int i, int n, int& begin, int& end) {
+  begin = uniform((int)((int64_t)rounds * i / n));
+  end = uniform((int)((int64_t)rounds * (i + 1) / n));
+}
+
+// The same for vectors of up to 128: a workgroup has 256 rows, a wave 64 of them (two columns of Z^T a lane) in registers, and
+// goes over its share of the classes with a running maximum and sum.  Each read of the classes serves two products.
+template <class T, int NB>
+__global__ __launch_bounds__(256, 2) void logits_short_kernel(LossParams p, int row_tiles, int splits) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
+  __shared__ u32x4 tiles[2][kSize];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t block = block_by_die();
+  const int split = uniform(block / row_tiles), row0 = uniform(block % row_tiles) * 256 + wave * 64;
+  int begin, end;
+  rounds_of((p.classes + kRound - 1) / kRound, split, splits, begin, end);
+  const int64_t row_bytes = (int64_t)p.dim * 2;
+  const TileLoader<NB, kRound> w(p.weight, row_bytes, 0, 0, p.dim);
+  const uint32_t lds = lds_address(&tiles[0][0]) + wave * 1024;
+  if (begin < end) w.issue(lds, row_bytes, begin * kRound, p.classes);
+  u32x4 hf[2][2 * NB];
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = row0 + 32 * j + (lane & 31);
+    load_rows<NB>(hf[j], (const char*)p.hidden + row * row_bytes, row < p.rows, p.dim, h);
+  }
+  int half = 0;
+  for (int i = begin; i < end; ++i, half ^= 1) {
+    wait_for_loads_and_others();
+    if (i + 1 < end) w.issue(lds + (half ^ 1) * kSize * 16, row_bytes, (i + 1) * kRound, p.classes);
+    if (row0 >= p.rows) continue;
+    const u32x4* tile = tiles[half];
+    f32x16 z[2][kRound / 32];
+#pragma unroll
+    for (int t = 0; t < kRound / 32; ++t) {
+      z[0][t] = z[1][t] = f32x16{};
+#pragma unroll
+      for (int s = 0; s < 2 * NB; ++s) {
+        const u32x4 wf = read_operand_by_rows<kChunks>(tile, 32 * t, s, lane);
+        z[0][t] = product_32x32x16<T>(wf, hf[0][s], z[0][t]);
+        z[1][t] = product_32x32x16<T>(wf, hf[1][s], z[1][t]);
+      }
+    }
+    if ((i + 1) * kRound > p.classes) {
+#pragma unroll
+      for (int t = 0; t < kRound / 32; ++t)
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          if (i * kRound + 32 * t + 8 * (n / 4) + 4 * h + n % 4 >= p.classes) z[0][t][n] = z[1][t][n] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float m = z[j][0][0];
+#pragma unroll
+      for (int t = 0; t < kRound / 32; ++t)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) m = fmaxf(m, z[j][t][n]);
+      m = pair_max(m) * kLog2e;
+      // the sums are taken relative to a maximum that may be up to 2^8 too small, and are rarely scaled again
+      if (__builtin_amdgcn_ballot_w64(m > top[j] + 8.f)) {
+        const float higher = fmaxf(m, top[j]);
+        sum[j] *= higher == -INFINITY ? 0.f : exp2_fast(top[j] - higher);
+        top[j] = higher;
+      }
+      const float base = top[j] == -INFINITY ? 0.f : top[j];
+#pragma unroll
+      for (int t = 0; t < kRound / 32; ++t)
+#pragma unroll
+        for (int n = 0; n < 16; ++n) sum[j] += exp2_fast(__builtin_fmaf(z[j][t][n], kLog2e, -base));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int row = row0 + 32 * j + (lane & 31);
+    const float all = pair_sum(sum[j]);
+    if (h == 0 && row < p.rows) p.partials[(int64_t)split * p.rows + row] = make_float2(top[j], all);
   }
 }
 
@@ -374,42 +471,210 @@ __global__ __launch_bounds__(1024) void join_kernel(LossParams p, int parts) {
   }
 }
 
-// Before the backward products.  First workgroup: max |dloss|; g is held relative to it, so that 16-bit floats hold the
-// gradient of a mean over any number of rows.  The others: hidden, filled up with rows of zeros and with zeros for the
-// rows without a target: such a row sends nothing to dw, whatever it holds (0 x NaN would be NaN).
-__global__ __launch_bounds__(1024) void prepare_kernel(LossParams p) {
-  if (blockIdx.x == 0) {
-    __shared__ float tops[16];
-    float m = 0.f;
-    for (int i = threadIdx.x; i < p.rows; i += 1024)
-      if (p.target[i] >= 0 && p.target[i] < p.classes) {
-        const float d = fabsf(p.dloss[i]);
-        m = d > m || d != d ? d : m;
-      }
+// g in 16-bit floats is held relative to max |dloss|, so that they hold the gradient of a mean over any number of rows.
+__global__ __launch_bounds__(1024) void largest_kernel(LossParams p) {
+  __shared__ float tops[16];
+  float m = 0.f;
+  for (int i = threadIdx.x; i < p.rows; i += 1024)
+    if (p.target[i] >= 0 && p.target[i] < p.classes) m = fmaxf(m, fabsf(p.dloss[i]));
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
-      *p.largest = m;
-    }
-    return;
+  for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
+    const bool scaled = m > 0.f && m < INFINITY;
+    p.scale[0] = scaled ? kGradientOne / m : 1.f;
+    p.scale[1] = scaled ? m / kGradientOne : 1.f;
   }
-  const int64_t i = (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x;
+}
+
+// Before the backward products: hidden, filled up with rows of zeros and with zeros for the rows without a target (such a
+// row sends nothing to dw, whatever it holds: 0 x NaN would be NaN), and what g takes of each row.
+template <bool SCALED>
+__global__ __launch_bounds__(256) void prepare_kernel(LossParams p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int chunks = p.dim / 8;
   if (i >= (int64_t)p.padded_rows * chunks) return;
   const int row = (int)(i / chunks), target = row < p.rows ? p.target[row] : -1;
+  const bool has = target >= 0 && target < p.classes;
   u32x4 v = {0, 0, 0, 0};
-  if (target >= 0 && target < p.classes) v = ((const u32x4*)p.hidden)[i];
+  if (has) v = ((const u32x4*)p.hidden)[i];
   ((u32x4*)p.hidden_known)[i] = v;
+  if (i % chunks == 0) {
+    const float each = has ? p.dloss[row] * (SCALED ? p.scale[0] : kGradientScale) : 0.f;
+    p.row_each[row] = each;
+    p.row_shift[row] = has ? log2f(fabsf(each)) - p.lse[row] * kLog2e : -INFINITY;
+    p.row_target[row] = has ? target : -1;
+  }
+  if (!SCALED && i == 0) p.scale[1] = 1.f / kGradientScale;
 }
 
+// ---- backward, vectors of up to 128 --------------------------------------------------------------------
+// dh: one workgroup has 128 rows, a wave 32 of them (lane's row is a column of Z^T = W H^T) in registers, and goes over its
+// share of the classes; G^T is the second operand of dH^T = W^T G^T as it leaves the exponentials.
+template <class T, int NB>
+__global__ __launch_bounds__(256, 2) void dhidden_short_kernel(LossParams p, int row_tiles, bool alone) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
+  __shared__ u32x4 tiles[2][kSize];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t block = block_by_die();
+  const int split = uniform(block / row_tiles), row0 = uniform(block % row_tiles) * 128 + wave * 32, row = row0 + (lane & 31);
+  const bool work = row0 < p.padded_rows;  // (wave-uniform: padded_rows is a multiple of 32)
+  int begin, end;
+  rounds_of((p.classes + kRound - 1) / kRound, split, p.dhidden_split, begin, end);
+  const int64_t row_bytes = (int64_t)p.dim * 2;
+  const TileLoader<NB, kRound> w(p.weight, row_bytes, 0, 0, p.dim);
+  const uint32_t lds = lds_address(&tiles[0][0]) + wave * 1024;
+  if (begin < end) w.issue(lds, row_bytes, begin * kRound, p.classes);
+  u32x4 hf[2 * NB];
+  load_rows<NB>(hf, (const char*)p.hidden_known + row * row_bytes, work, p.dim, h);
+  const int target = work ? p.row_target[row] : -1;
+  const float each = work ? p.row_each[row] : 0.f, shift = work ? p.row_shift[row] : -INFINITY;
+  const uint32_t negative = each < 0.f ? 0x80000000u : 0u;
+  const bool negatives = __builtin_amdgcn_ballot_w64(negative) != 0;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  int half = 0;
+  for (int i = begin; i < end; ++i, half ^= 1) {
+    wait_for_loads_and_others();
+    if (i + 1 < end) w.issue(lds + (half ^ 1) * kSize * 16, row_bytes, (i + 1) * kRound, p.classes);
+    if (!work) continue;
+    const int class0 = i * kRound;
+    const u32x4* tile = tiles[half];
+    const bool edge = class0 + kRound > p.classes ||
+                      __builtin_amdgcn_ballot_w64(target >= class0 && target < class0 + kRound) != 0;
+#pragma unroll
+    for (int t = 0; t < kRound / 32; ++t) {
+      f32x16 g = {};
+#pragma unroll
+      for (int s = 0; s < 2 * NB; ++s) g = product_32x32x16<T>(read_operand_by_rows<kChunks>(tile, 32 * t, s, lane), hf[s], g);
+#pragma unroll
+      for (int n = 0; n < 16; ++n) g[n] = exp2_fast(__builtin_fmaf(g[n], kLog2e, shift));
+      // (branches inside the round: with a body of its own for rounds without an edge the compiler runs out of registers,
+      // 276 us where this takes 232)
+      if (negatives) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) g[n] = __uint_as_float(__float_as_uint(g[n]) ^ negative);
+      }
+      if (edge) {
+        const int c0 = class0 + 32 * t + 4 * h;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const int c = c0 + 8 * (n / 4) + n % 4;
+          if (c == target) g[n] -= each;
+          if (c >= p.classes) g[n] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x4 gf = pack_operand<T>(g, j);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(tile, 32 * t + 16 * j, 32 * b, lane), gf, acc[b]);
+      }
+    }
+  }
+  __syncthreads();
+  if (row0 >= p.rows) return;
+  const float factor = p.scale[1];
+  if (alone)
+    store_rows<T, NB>((T*)p.dhidden + (int64_t)row0 * p.dim, p.dim, p.rows - row0, acc, factor, p.dim,
+                      &tiles[0][0] + wave * 32 * kChunks);
+  else if (row < p.rows)
+    store_sums<NB>(p.dhidden_sums + ((int64_t)split * p.rows + row) * p.dim, acc, factor, p.dim, h);
+}
+
+// dw: one workgroup has 128 classes, a wave 32 of them (lane's class is a column of Z = H W^T), and goes over its share of the
+// rows, whose shifts are read from LDS.
+template <class T, int NB>
+__global__ __launch_bounds__(256, 2) void dweight_short_kernel(LossParams p, int class_tiles) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
+  __shared__ u32x4 tiles[2][kSize];
+  __shared__ float shifts[2][kRound], eaches[2][kRound];
+  __shared__ int32_t targets[2][kRound];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const uint32_t block = block_by_die();
+  const int split = uniform(block / class_tiles), class0 = uniform(block % class_tiles) * 128 + wave * 32, mine = class0 + (lane & 31);
+  int begin, end;
+  rounds_of(p.padded_rows / kRound, split, p.dweight_split, begin, end);
+  const int64_t row_bytes = (int64_t)p.dim * 2;
+  const TileLoader<NB, kRound> rows(p.hidden_known, row_bytes, 0, 0, p.dim);
+  const uint32_t lds = lds_address(&tiles[0][0]) + wave * 1024;
+  auto issue = [&](int half, int i) {
+    rows.issue(lds + half * kSize * 16, row_bytes, i * kRound, p.padded_rows);
+#pragma unroll
+    for (int j = 0; j < kRound; j += 64) {
+      if (wave == 0) load_words_to_lds((const char*)(p.row_shift + i * kRound + j), lane * 4, lds_address(shifts[half] + j));
+      if (wave == 1) load_words_to_lds((const char*)(p.row_target + i * kRound + j), lane * 4, lds_address(targets[half] + j));
+      if (wave == 2) load_words_to_lds((const char*)(p.row_each + i * kRound + j), lane * 4, lds_address(eaches[half] + j));
+    }
+  };
+  if (begin < end) issue(0, begin);
+  const bool work = class0 < p.classes;
+  u32x4 wf[2 * NB];
+  load_rows<NB>(wf, (const char*)p.weight + mine * row_bytes, mine < p.classes, p.dim, h);
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  int half = 0;
+  for (int i = begin; i < end; ++i, half ^= 1) {
+    wait_for_loads_and_others();
+    if (i + 1 < end) issue(half ^ 1, i + 1);
+    if (!work) continue;
+    const u32x4* tile = tiles[half];
+    // a row of the round whose target is a class of the wave, or whose gradient is negative
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < kRound; j += 64)
+      odd = odd || (targets[half][j + lane] >= class0 && targets[half][j + lane] < class0 + 32) || eaches[half][j + lane] < 0.f;
+    const bool edge = __builtin_amdgcn_ballot_w64(odd) != 0;
+#pragma unroll
+    for (int t = 0; t < kRound / 32; ++t) {
+      f32x16 g = {};
+#pragma unroll
+      for (int s = 0; s < 2 * NB; ++s) g = product_32x32x16<T>(read_operand_by_rows<kChunks>(tile, 32 * t, s, lane), wf[s], g);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 shift = *(const f32x4*)&shifts[half][32 * t + 8 * q + 4 * h];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) g[4 * q + n] = exp2_fast(__builtin_fmaf(g[4 * q + n], kLog2e, shift[n]));
+      }
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          const int at = 32 * t + 8 * (n / 4) + 4 * h + n % 4;
+          const float each = eaches[half][at];
+          if (each < 0.f) g[n] = -g[n];
+          if (targets[half][at] == mine) g[n] -= each;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const u32x4 gf = pack_operand<T>(g, j);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(tile, 32 * t + 16 * j, 32 * b, lane), gf, acc[b]);
+      }
+    }
+  }
+  __syncthreads();
+  if (!work) return;
+  const float factor = p.scale[1];
+  if (p.dweight_split == 1)
+    store_rows<T, NB>((T*)p.dweight + (int64_t)class0 * p.dim, p.dim, p.classes - class0, acc, factor, p.dim,
+                      &tiles[0][0] + wave * 32 * kChunks);
+  else if (mine < p.classes)
+    store_sums<NB>(p.dweight_sums + ((int64_t)split * p.classes + mine) * p.dim, acc, factor, p.dim, h);
+}
+
+// ---- backward, longer vectors ------------------------------------------------------------------------------
 // What a workgroup of the two products below leaves.  Result rows are columns of the vectors and lie in a lane's
 // registers, four next to each other at a time; the result's column is the lane's row of the output.
 // A sum of its own among several, in 32 bits:
 template <class S>
-__device__ __forceinline__ void store_sums(const f32x16 (&acc)[S::kM][S::kN], float factor, float* sums, bool add, int row0, int row_end,
+__device__ __forceinline__ void store_tile_sums(const f32x16 (&acc)[S::kM][S::kN], float factor, float* sums, bool add, int row0, int row_end,
                                            int column0, int columns) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
 #pragma unroll
@@ -484,9 +749,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void dhidden_kernel(LossParams p, i
   f32x16 acc[S::kM][S::kN];
   multiply<T, S, true>(acc, Columns((const char*)p.weight + (int64_t)p.class0 * p.dim * 2, (int64_t)p.dim * 2, column0, p.dim, classes),
                        Rows(p.gradient, p.padded_rows, row0), begin, end, tiles);
-  const float factor = *p.largest / kGradientOne;
+  const float factor = p.scale[1];
   if (alone) store_result<T, S>(acc, factor, (T*)p.dhidden, row0, p.rows, column0, p.dim, tiles);
-  else store_sums<S>(acc, factor, p.dhidden_sums + (int64_t)split * p.rows * p.dim, p.class0 > 0, row0, p.rows, column0, p.dim);
+  else store_tile_sums<S>(acc, factor, p.dhidden_sums + (int64_t)split * p.rows * p.dim, p.class0 > 0, row0, p.rows, column0, p.dim);
 }
 
 // dw of the piece's classes.
@@ -504,10 +769,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void dweight_kernel(LossParams p, i
   f32x16 acc[S::kM][S::kN];
   multiply<T, S, false>(acc, Columns(p.hidden_known, (int64_t)p.dim * 2, column0, p.dim, p.padded_rows),
                         Classes(p.gradient, p.padded_rows, class0), begin, end, tiles);
-  const float factor = *p.largest / kGradientOne;
+  const float factor = p.scale[1];
   if (p.dweight_split == 1)
     store_result<T, S>(acc, factor, (T*)p.dweight + (int64_t)p.class0 * p.dim, class0, classes, column0, p.dim, tiles);
-  else store_sums<S>(acc, factor, p.dweight_sums + (int64_t)split * classes * p.dim, false, class0, classes, column0, p.dim);
+  else store_tile_sums<S>(acc, factor, p.dweight_sums + (int64_t)split * classes * p.dim, false, class0, classes, column0, p.dim);
 }
 
 // out = the sum of `split` arrays of n values, n a multiple of 8: sixteen lanes share out the arrays, four values at a time.
@@ -535,12 +800,15 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 constexpr int kFewRows = 128;  // up to here tiles of 64 rows of the loss, beyond it tiles of 256
 constexpr int64_t kWorkgroups = 256;  // what fills the GPU, one to a compute unit
+// Vectors whose g stays in registers.  At 128 and 8192 rows x 56944 classes dh and dw take 495 us so, and 757 us over a g in
+// memory, most of it the 933 MB of g; the third making of the logits costs as much as that saves at 256.
+constexpr int64_t kShortVector = 128;
 
 // How the work is cut; the workspace's parts as offsets.
 struct LossPlan {
-  int64_t padded_rows, piece, column_tiles, dhidden_split, dweight_split;
+  int64_t padded_rows, piece, column_tiles, logits_split, dhidden_split, dweight_split;
   bool alone;  // the only sum of dh
-  int64_t partials, gradient, dhidden_sums, dweight_sums, largest, hidden_known, bytes;
+  int64_t partials, gradient, dhidden_sums, dweight_sums, scale, row_each, row_shift, row_target, hidden_known, bytes;
 };
 
 LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
@@ -550,28 +818,38 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
     w.bytes += round_up(bytes, 256);
     return at;
   };
+  auto split = [](int64_t workgroups, int64_t tiles, int64_t rounds, int64_t least) {  // at least so many rounds to a share
+    return std::max<int64_t>(1, std::min(workgroups / std::max<int64_t>(tiles, 1), rounds / least));
+  };
+  const bool is_short = dim <= kShortVector;
   if (!backward) {
-    w.partials = take(round_up(classes, kClassPad) / 64 * rows * (int64_t)sizeof(float2));
+    w.logits_split = is_short ? split(4 * kWorkgroups, (rows + 255) / 256, (classes + kRound - 1) / kRound, 2) : 1;
+    w.partials = take((is_short ? w.logits_split : round_up(classes, kClassPad) / 64) * rows * (int64_t)sizeof(float2));
     return w;
   }
-  const int64_t tile_rows = rows > kFewRows ? 256 : 64;
-  w.padded_rows = round_up(std::max<int64_t>(rows, 1), tile_rows);
-  const int64_t tile_columns = dim > 128 ? 256 : dim > 64 ? 128 : 64;
-  w.column_tiles = (dim + tile_columns - 1) / tile_columns;
-  // g of a piece is written once and read twice: 256 MiB (what the last-level cache holds), unless that
-  // leaves compute units without a tile of dw
-  const int64_t fit = ((int64_t)256 << 20) / (2 * w.padded_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
-  w.piece = std::min(round_up(classes, kClassPad), round_up(std::max(fit, fill), kClassPad));
-  const int64_t row_tiles = w.padded_rows / tile_rows, class_tiles = w.piece / kClassPad;
-  auto split = [](int64_t tiles, int64_t places) {  // at least four rounds to a share
-    return std::max<int64_t>(1, std::min(kWorkgroups / tiles, places / 256));
-  };
-  w.dhidden_split = split(row_tiles * w.column_tiles, w.piece);
-  w.dweight_split = split(class_tiles * w.column_tiles, w.padded_rows);
-  w.alone = w.dhidden_split == 1 && w.piece >= classes;
-  w.largest = take(sizeof(float));
+  const int64_t tile_rows = rows <= kFewRows ? 64 : 256;
+  w.padded_rows = round_up(std::max<int64_t>(rows, 1), is_short ? kRound : tile_rows);
+  if (is_short) {
+    w.dhidden_split = split(2 * kWorkgroups, (w.padded_rows + 127) / 128, (classes + kRound - 1) / kRound, 2);
+    w.dweight_split = split(2 * kWorkgroups, (classes + 127) / 128, w.padded_rows / kRound, 4);
+    w.alone = w.dhidden_split == 1;
+    w.piece = classes;
+  } else {
+    w.column_tiles = (dim + 255) / 256;
+    // g of a piece is written once and read twice: 256 MiB (what the last-level cache holds), unless that
+    // leaves compute units without a tile of dw
+    const int64_t fit = ((int64_t)256 << 20) / (2 * w.padded_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
+    w.piece = std::min(round_up(classes, kClassPad), round_up(std::max(fit, fill), kClassPad));
+    w.dhidden_split = split(kWorkgroups, w.padded_rows / tile_rows * w.column_tiles, w.piece / 64, 4);
+    w.dweight_split = split(kWorkgroups, w.piece / kClassPad * w.column_tiles, w.padded_rows / 64, 4);
+    w.alone = w.dhidden_split == 1 && w.piece >= classes;
+    w.gradient = take(w.padded_rows * w.piece * 2);
+  }
+  w.scale = take(2 * sizeof(float));
+  w.row_each = take(w.padded_rows * 4);
+  w.row_shift = take(w.padded_rows * 4);
+  w.row_target = take(w.padded_rows * 4);
   w.hidden_known = take(w.padded_rows * dim * 2);
-  w.gradient = take(w.padded_rows * w.piece * 2);
   if (!w.alone) w.dhidden_sums = take(w.dhidden_split * rows * dim * (int64_t)sizeof(float));
   if (w.dweight_split > 1) w.dweight_sums = take(w.dweight_split * std::min(w.piece, classes) * dim * (int64_t)sizeof(float));
   return w;
@@ -592,9 +870,21 @@ int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_cla
   return launch_logits<T, Shape<2, 4, 4, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
 }
 
+template <class T, int NB>
+int launch_logits_short(const LossParams& p, int splits, hipStream_t stream) {
+  const int row_tiles = (p.rows + 255) / 256;
+  logits_short_kernel<T, NB><<<(uint32_t)(row_tiles * splits), 256, 0, stream>>>(p, row_tiles, splits);
+  return splits;
+}
+
 template <class T>
-void launch_forward(LossParams p, hipStream_t stream) {
-  const int parts = launch_logits<T, false>(p, p.rows, p.classes, stream);
+void launch_forward(LossParams p, const LossPlan& w, hipStream_t stream) {
+  int parts;
+  if (p.dim > kShortVector) parts = launch_logits<T, false>(p, p.rows, p.classes, stream);
+  else if (p.dim > 96) parts = launch_logits_short<T, 4>(p, (int)w.logits_split, stream);
+  else if (p.dim > 64) parts = launch_logits_short<T, 3>(p, (int)w.logits_split, stream);
+  else if (p.dim > 32) parts = launch_logits_short<T, 2>(p, (int)w.logits_split, stream);
+  else parts = launch_logits_short<T, 1>(p, (int)w.logits_split, stream);
   join_kernel<T><<<(p.rows + 7) / 8, 1024, 0, stream>>>(p, parts);
 }
 
@@ -609,6 +899,13 @@ void launch_dweight(const LossParams& p, const LossPlan& w, hipStream_t stream) 
   dweight_kernel<T, S><<<(uint32_t)(class_tiles * w.column_tiles * w.dweight_split), S::kThreads, 0, stream>>>(p, class_tiles, (int)w.column_tiles);
 }
 
+template <class T, int NB>
+void launch_short(const LossParams& p, const LossPlan& w, hipStream_t stream) {
+  const int row_tiles = (p.padded_rows + 127) / 128, class_tiles = (p.classes + 127) / 128;
+  dhidden_short_kernel<T, NB><<<(uint32_t)(row_tiles * w.dhidden_split), 256, 0, stream>>>(p, row_tiles, w.alone);
+  dweight_short_kernel<T, NB><<<(uint32_t)(class_tiles * w.dweight_split), 256, 0, stream>>>(p, class_tiles);
+}
+
 template <class T>
 void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
   if (p.rows == 0) {  // no sum at all
@@ -616,7 +913,27 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
     add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(nullptr, (T*)p.dweight, n, 0);
     return;
   }
-  prepare_kernel<<<(uint32_t)((w.padded_rows * (p.dim / 8) + 1023) / 1024 + 1), 1024, 0, stream>>>(p);
+  const uint32_t prepare_blocks = (uint32_t)((w.padded_rows * (p.dim / 8) + 255) / 256);
+  if (std::is_same<T, _Float16>::value) {
+    largest_kernel<<<1, 1024, 0, stream>>>(p);
+    prepare_kernel<true><<<prepare_blocks, 256, 0, stream>>>(p);
+  } else {
+    prepare_kernel<false><<<prepare_blocks, 256, 0, stream>>>(p);
+  }
+  auto add_dweight = [&](int64_t class0, int64_t classes) {
+    const int64_t n = classes * p.dim;
+    if (w.dweight_split > 1)
+      add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dweight_sums, (T*)p.dweight + class0 * p.dim, n, p.dweight_split);
+  };
+  if (p.dim <= kShortVector) {
+    switch ((p.dim + 31) / 32) {
+      case 1: launch_short<T, 1>(p, w, stream); break;
+      case 2: launch_short<T, 2>(p, w, stream); break;
+      case 3: launch_short<T, 3>(p, w, stream); break;
+      default: launch_short<T, 4>(p, w, stream); break;
+    }
+    add_dweight(0, p.classes);
+  } else
   for (int64_t at = 0; at < p.classes; at += w.piece) {
     p.class0 = (int32_t)at;
     p.class_end = (int32_t)std::min<int64_t>(at + w.piece, p.classes);
@@ -624,23 +941,10 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
     launch_logits<T, true>(p, p.padded_rows, round_up(classes, kClassPad), stream);
     const bool few = p.rows <= kFewRows;
     // shapes of the two products: columns of the vectors x rows of the output
-    if (p.dim > 128) {
-      if (few) launch_dhidden<T, Shape<4, 2, 2, 1, 64>>(p, w, stream);
-      else launch_dhidden<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
-      launch_dweight<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
-    } else if (p.dim > 64) {
-      if (few) launch_dhidden<T, Shape<4, 2, 1, 1, 64>>(p, w, stream);
-      else launch_dhidden<T, Shape<2, 4, 2, 2, 64>>(p, w, stream);
-      launch_dweight<T, Shape<2, 4, 2, 2, 64>>(p, w, stream);
-    } else {
-      if (few) launch_dhidden<T, Shape<2, 2, 1, 1, 64>>(p, w, stream);
-      else launch_dhidden<T, Shape<1, 8, 2, 1, 64>>(p, w, stream);
-      launch_dweight<T, Shape<1, 8, 2, 1, 64>>(p, w, stream);
-    }
-    if (w.dweight_split > 1) {
-      const int64_t n = classes * p.dim;
-      add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dweight_sums, (T*)p.dweight + at * p.dim, n, p.dweight_split);
-    }
+    if (few) launch_dhidden<T, Shape<4, 2, 2, 1, 64>>(p, w, stream);
+    else launch_dhidden<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
+    launch_dweight<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
+    add_dweight(at, classes);
   }
   if (!w.alone) {
     const int64_t n = (int64_t)p.rows * p.dim;
@@ -685,7 +989,10 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
   p.gradient = (u32x4*)(work + w.gradient);
   p.dhidden_sums = (float*)(work + w.dhidden_sums);
   p.dweight_sums = (float*)(work + w.dweight_sums);
-  p.largest = (float*)(work + w.largest);
+  p.scale = (float*)(work + w.scale);
+  p.row_each = (float*)(work + w.row_each);
+  p.row_shift = (float*)(work + w.row_shift);
+  p.row_target = (int32_t*)(work + w.row_target);
   p.hidden_known = work + w.hidden_known;
   p.padded_rows = (int32_t)w.padded_rows;
   p.dhidden_split = (int32_t)w.dhidden_split;
@@ -695,8 +1002,8 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
     if (a->dtype == ND_BF16) launch_backward<__bf16>(p, w, (hipStream_t)stream);
     else launch_backward<_Float16>(p, w, (hipStream_t)stream);
   } else {
-    if (a->dtype == ND_BF16) launch_forward<__bf16>(p, (hipStream_t)stream);
-    else launch_forward<_Float16>(p, (hipStream_t)stream);
+    if (a->dtype == ND_BF16) launch_forward<__bf16>(p, w, (hipStream_t)stream);
+    else launch_forward<_Float16>(p, w, (hipStream_t)stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(std::string("vocabulary loss: ") + hipGetErrorString(e));
