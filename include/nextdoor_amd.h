@@ -308,14 +308,15 @@ int nd_dropout(const void* d_x, const void* d_residual, void* d_y, int64_t n, in
 /* Packed sequences: sequence i is tokens starts[i] .. starts[i + 1] - 1 of n_tokens; starts[0] = 0, and tokens
  * from starts[n_sequences] on belong to no sequence.  `starts` is the HOST array (n_sequences + 1
  * entries), which is checked, d_starts the same on the device; the plan (nd_packed_plan_bytes(n_tokens)
- * bytes, aligned to 16) is what every attention call over this batch reads.  rounds (on the host): how
- * much work there is in all and in the largest tile, by which attention calls cut it. */
+ * bytes, aligned to 16) is what every attention call over this batch reads.  sizes (on the host): how
+ * much work there is in all and in the largest tile, and the tiles of whole sequences (0 if some are too
+ * long), by which attention calls choose their kernels.  Not for graph capture. */
 #define ND_PACKED_MAX_TOKENS 2147483392
 #define ND_PACKED_MAX_DIM 128
 #define ND_PACKED_MAX_TOKEN_STRIDE 16777216
 int64_t nd_packed_plan_bytes(int64_t n_tokens);
 int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
-                   int64_t rounds[2], void* stream);
+                   int64_t sizes[3], void* stream);
 
 /* Causal attention within each sequence, heads / kv_heads query heads to a key head.  q, k, v and
  * dout: [token][head][dim] with the strides given (in elements, multiples of 8, >= 0; dim elements
@@ -327,7 +328,7 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
  * working memory of one call. */
 typedef struct nd_packed_attention {
   int64_t n_tokens, n_covered; /* n_covered = starts[n_sequences] */
-  int64_t rounds, most_rounds; /* nd_packed_plan's */
+  int64_t rounds, most_rounds, short_tiles; /* nd_packed_plan's sizes */
   int32_t heads, kv_heads, dim, dtype;
   float scale;
   const void* plan;

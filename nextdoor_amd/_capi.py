@@ -14,7 +14,7 @@ c_i64p = C.POINTER(C.c_int64)
 
 class PackedAttention(C.Structure):
     """nd_packed_attention"""
-    _fields_ = ([(n, C.c_int64) for n in ("n_tokens", "n_covered", "rounds", "most_rounds")] +
+    _fields_ = ([(n, C.c_int64) for n in ("n_tokens", "n_covered", "rounds", "most_rounds", "short_tiles")] +
                 [(n, C.c_int32) for n in ("heads", "kv_heads", "dim", "dtype")] + [("scale", C.c_float)] +
                 [(n, C.c_void_p) for n in ("plan", "q", "k", "v", "dout")] +
                 [(n, C.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "dout_token",

@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <vector>
 
 #include "nd_errors.hpp"
 #include "nd_matrix.hpp"
@@ -37,7 +38,10 @@ struct PackedPlan {
   const int32_t* last;   // one past it
   const int32_t* query_order;  // tiles of kRows tokens, those with most keys first
   const int32_t* key_order;    // those with most queries first
-  int32_t tokens, covered, tiles;
+  // No sequence is longer than a tile: tile i is the whole sequences in tokens short_starts[i] .. short_starts[i + 1] - 1
+  // (short_tiles of them; 0: there are longer sequences).
+  const int32_t* short_starts;
+  int32_t tokens, covered, tiles, short_tiles;
 };
 
 struct AttentionParams {
@@ -137,9 +141,18 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
   int chunk, rank, head;
   chunk_tile_and_head(p.max_chunks, p.heads, chunk, rank, head);
-  const int tile0 = uniform(p.plan.query_order[rank]) * kRows, kv_head = uniform(head / p.group);
+  const int kv_head = uniform(head / p.group);
+  int tile0, tile_end;
+  if (p.plan.short_tiles > 0) {
+    tile0 = uniform(p.plan.short_starts[rank]);
+    tile_end = uniform(p.plan.short_starts[rank + 1]);
+  } else {
+    tile0 = uniform(p.plan.query_order[rank]) * kRows;
+    tile_end = min(tile0 + kRows, p.plan.tokens);
+  }
+  const int end = min(tile_end, p.plan.covered);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
-  const bool there = row < p.plan.covered;
+  const bool there = row < end;
   f32x16 acc[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
@@ -147,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
   int chunks = 1;
 
   if (tile0 < p.plan.covered) {
-    const int end = min(tile0 + kRows, p.plan.covered), first_key = uniform(p.plan.first[tile0]);
+    const int first_key = uniform(p.plan.first[tile0]);
     const int rounds = (end - first_key + kColumns - 1) / kColumns;
     chunks = uniform((int)chunks_of(rounds, p.chunk, p.max_chunks));
     if (chunk >= chunks) return;
@@ -162,8 +175,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     issue(0, begin);
     const int first = there ? p.plan.first[row] : row + 1;
     // of the wave's rows: the smallest and the largest `first`
-    const int first_min = row0 < p.plan.covered ? uniform(first) : 0x7fffffff - kColumns;
-    const int first_max = uniform(p.plan.first[min(row0 + 31, p.plan.covered - 1)]);
+    const int first_min = row0 < end ? uniform(first) : 0x7fffffff - kColumns;
+    const int first_max = uniform(p.plan.first[min(row0 + 31, end - 1)]);
     u32x4 qf[2 * NB];
     load_rows<NB>(qf, (const char*)p.q + (int64_t)row * p.q_token + (int64_t)head * p.q_head, there, p.dim, h);
     if (p.flip) {
@@ -234,8 +247,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
   } else if (chunk > 0) {
     return;
   }
-  if (row0 >= p.plan.tokens) return;
-  if (row0 + 31 >= p.plan.covered && !there) {  // (tiles that all of the wave's sequences see are not masked)
+  if (row0 >= tile_end) return;
+  if (row0 + 31 >= end && !there) {  // (tiles that all of the wave's sequences see are not masked)
     top = -INFINITY;
     sum = 0.f;
 #pragma unroll
@@ -243,14 +256,14 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
   }
   sum = pair_sum(sum);
   if (chunks > 1) {
-    if (row >= p.plan.tokens) return;
+    if (row >= tile_end) return;
     if (h == 0) p.row_tops[((int64_t)chunk * p.heads + head) * p.plan.tokens + row] = make_float2(top, sum);
     store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, 1.f, p.dim, h);
     return;
   }
   const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
-  if (h == 0 && row < p.plan.tokens) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
-  store_rows<T, NB>((T*)p.out_w + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, inverse,
+  if (h == 0 && row < tile_end) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
+  store_rows<T, NB>((T*)p.out_w + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, tile_end - row0, acc, inverse,
                     p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
 }
 
@@ -577,6 +590,147 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
   }
 }
 
+// Sequences of at most a tile: one workgroup has the whole sequences of a tile and one key head, so that it reads queries, keys,
+// values and output gradients once and has all of dq, dk and dv (batch of walks, 8 heads of 64: 59 us; 91 for the two kernels
+// above, which are bound by what they read).  Per head of the group each wave first has 32 queries, as in the dq kernel, then
+// 32 keys, as in the other one; delta always comes from the weights themselves.
+template <class T, int NB>
+__global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short_kernel(AttentionParams p) {
+  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRows * kChunks;
+  __shared__ u32x4 keys[kSize], values[kSize], queries[kSize], douts[kSize];
+  __shared__ float lse2s[kRows], deltas[kRows];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  const int kv_head = uniform(blockIdx.x % p.kv_heads), tile = uniform(blockIdx.x / p.kv_heads);
+  const int tile0 = uniform(p.plan.short_starts[tile]), tile_end = uniform(p.plan.short_starts[tile + 1]);
+  const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);  // as queries and as keys
+  u32x4* const part_lds = queries + wave * 32 * kChunks;
+  const int64_t q_elements = (int64_t)p.heads * p.dim, k_elements = (int64_t)p.kv_heads * p.dim;
+  f32x16 dk[NB], dv[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
+
+  if (tile0 < p.plan.covered) {
+    // (such a tile ends at `covered` or before it)
+    const bool there = row < tile_end, work = row0 < tile_end;
+    const int first = there ? p.plan.first[row] : row + 1, last = there ? p.plan.last[row] : row;
+    const int first_tile = work ? (uniform(first) - tile0) / 32 : 0;                                    // of the wave's keys
+    const int last_tile = work ? (uniform(p.plan.last[min(row0 + 31, tile_end - 1)]) - 1 - tile0) / 32 : 0;  // of its queries
+    const uint32_t part = wave * 1024;
+    const TileLoader<NB, kRows> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
+    k.issue(lds_address(keys) + part, p.k_token, tile0, tile_end);
+    v.issue(lds_address(values) + part, p.v_token, tile0, tile_end);
+    for (int g = 0; g < p.group; ++g) {
+      const int head = kv_head * p.group + g;
+      if (g > 0) __syncthreads();  // (the last head's dq has left through `queries`)
+      const TileLoader<NB, kRows> q(p.q, p.q_token, p.q_head, head, p.dim), d(p.dout, p.dout_token, p.dout_head, head, p.dim);
+      q.issue(lds_address(queries) + part, p.q_token, tile0, tile_end);
+      d.issue(lds_address(douts) + part, p.dout_token, tile0, tile_end);
+      const float lse2 = there ? p.lse[(int64_t)head * p.plan.tokens + row] * kLog2e : 0.f;
+      if (h == 0) lse2s[wave * 32 + (lane & 31)] = lse2;
+      wait_for_loads_and_others();
+      if (g == 0 && p.dim < 8 * kChunks) {  // the other operands have a row's first columns past `dim`: 0 here
+        for (int at = threadIdx.x; at < kSize; at += 256)
+          if (at % kChunks * 8 >= p.dim) {
+            const int place = tile_place<kChunks>(at / kChunks, at % kChunks);
+            keys[place] = values[place] = u32x4{0, 0, 0, 0};
+          }
+        __syncthreads();
+      }
+      f32x16 dq[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) dq[b] = f32x16{};
+      if (work) {
+        u32x4 qf[2 * NB], dof[2 * NB];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+          qf[i] = read_operand_by_rows<kChunks>(queries, 32 * wave, i, lane) ^ p.flip;
+          dof[i] = read_operand_by_rows<kChunks>(douts, 32 * wave, i, lane);
+        }
+        float delta = 0.f;
+        for (int sweep = 0; sweep < 2; ++sweep) {  // for delta, then for dq
+          float sum = 0.f;
+          for (int t = first_tile; t <= wave; ++t) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i) {
+              s = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s);
+              dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
+            }
+            const int from = first - tile0 - 32 * t - 4 * h, to = row - tile0 - 32 * t - 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = 8 * (i / 4) + i % 4;
+              const float ds = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+              s[i] = key >= from && key <= to ? ds : 0.f;
+              sum += s[i];
+            }
+            if (sweep == 0) continue;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const u32x4 dsf = pack_operand<T>(s, j);
+#pragma unroll
+              for (int b = 0; b < NB; ++b)
+                dq[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(keys, 32 * t + 16 * j, 32 * b, lane), dsf, dq[b]);
+            }
+          }
+          if (sweep == 0) delta = pair_sum(sum);
+        }
+        if (h == 0) deltas[wave * 32 + (lane & 31)] = delta;
+      }
+      __syncthreads();
+      if (work) {
+        u32x4 kf[2 * NB], vf[2 * NB];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) {
+          kf[i] = read_operand_by_rows<kChunks>(keys, 32 * wave, i, lane) ^ p.flip;
+          vf[i] = read_operand_by_rows<kChunks>(values, 32 * wave, i, lane);
+        }
+        for (int t = wave; t <= last_tile; ++t) {
+          f32x16 s = {}, dp = {};
+#pragma unroll
+          for (int i = 0; i < 2 * NB; ++i) {
+            s = product_32x32x16<T>(read_operand_by_rows<kChunks>(queries, 32 * t, i, lane), kf[i], s);
+            dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(douts, 32 * t, i, lane), vf[i], dp);
+          }
+          const int from = row - tile0 - 32 * t - 4 * h, to = last - tile0 - 32 * t - 4 * h;
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const f32x4 lses = *(const f32x4*)&lse2s[32 * t + 8 * q4 + 4 * h], delta = *(const f32x4*)&deltas[32 * t + 8 * q4 + 4 * h];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int i = 4 * q4 + n, query = 8 * q4 + n;
+              const bool sees = query >= from && query < to;
+              const float weight = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lses[n]));
+              s[i] = sees ? weight : 0.f;
+              dp[i] = sees ? weight * (dp[i] - delta[n]) : 0.f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const u32x4 pf = pack_operand<T>(s, j), dsf = pack_operand<T>(dp, j);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+              dv[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(douts, 32 * t + 16 * j, 32 * b, lane), pf, dv[b]);
+              dk[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(queries, 32 * t + 16 * j, 32 * b, lane), dsf, dk[b]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+      if (work)
+        store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, p.scale, p.dim, part_lds);
+    }
+  } else if (row0 < tile_end) {  // tokens of no sequence
+    for (int g = 0; g < p.group; ++g)
+      store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + kv_head * p.group + g) * p.dim, q_elements, tile_end - row0, dk, 0.f, p.dim,
+                        part_lds);
+  }
+  if (row0 >= tile_end) return;
+  const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
+  store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, p.scale, p.dim, part_lds);
+  store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, 1.f, p.dim, part_lds);
+}
+
 // Adds the chunks of cut tiles: dq (WHICH 0), dk (1), dv (2); n values each, a lane has four.
 template <class T>
 __global__ __launch_bounds__(256) void attention_add_kernel(AttentionParams p, int64_t n_rows, int64_t n_keys, int key_round) {
@@ -606,16 +760,18 @@ __global__ __launch_bounds__(256) void attention_add_kernel(AttentionParams p, i
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 int64_t tiles_of(int64_t tokens) { return (tokens + kRows - 1) / kRows; }
 
-// The plan's parts, in words: first, last, query_order, key_order.
+// The plan's parts, in words: first, last, query_order, key_order, short_starts (two tiles next to each other have more than kRows
+// tokens).
 struct PlanParts {
-  int64_t last, query_order, key_order, words;
+  int64_t last, query_order, key_order, short_starts, words;
 };
 PlanParts plan_parts(int64_t tokens) {
   PlanParts w;
   w.last = round_up(tokens, 4);
   w.query_order = 2 * w.last;
   w.key_order = w.query_order + round_up(tiles_of(tokens), 4);
-  w.words = w.key_order + round_up(tiles_of(tokens), 4);
+  w.short_starts = w.key_order + round_up(tiles_of(tokens), 4);
+  w.words = w.short_starts + round_up(2 * tiles_of(tokens) + 4, 4);
   return w;
 }
 
@@ -640,6 +796,11 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     return at;
   };
   const int64_t row_bytes = a.n_tokens * a.heads * a.dim * 4, key_bytes = a.n_tokens * a.kv_heads * a.dim * 4;
+  if (a.short_tiles > 0) {  // nothing to cut, nothing to keep
+    w.chunk = w.max_chunks = w.key_chunk = w.max_key_chunks = w.head_split = 1 << 20;
+    w.max_chunks = w.max_key_chunks = w.head_split = 1;
+    return w;
+  }
   w.chunk = std::max<int64_t>(8, (a.rounds * a.heads + kItems - 1) / kItems);
   w.max_chunks = most(a.most_rounds, w.chunk, row_bytes);
   w.max_key_chunks = w.key_chunk = w.head_split = 1;
@@ -664,7 +825,8 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
 
 template <class T, int NB>
 void launch_forward(const AttentionParams& p, hipStream_t stream) {
-  attention_forward_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
+  const uint32_t tiles = p.plan.short_tiles > 0 ? p.plan.short_tiles : p.plan.tiles;
+  attention_forward_kernel<T, NB><<<tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
   if (p.max_chunks > 1) {
     const int64_t n = (int64_t)p.plan.tokens * p.heads * p.dim;
     attention_join_kernel<T><<<(uint32_t)((n / 4 + 255) / 256), 256, 0, stream>>>(p, n);
@@ -672,6 +834,10 @@ void launch_forward(const AttentionParams& p, hipStream_t stream) {
 }
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
+  if (p.plan.short_tiles > 0) {
+    attention_backward_short_kernel<T, NB><<<(uint32_t)p.plan.short_tiles * p.kv_heads, 256, 0, stream>>>(p);
+    return;
+  }
   attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
   attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split * p.max_key_chunks, 256, 0, stream>>>(p);
   const bool add_keys = p.max_key_chunks * p.head_split > 1;
@@ -708,8 +874,9 @@ int check_attention(const nd_packed_attention* a, bool backward) {
                 std::to_string(a->dim) + " given");
   if (!isfinite(a->scale)) return fail("packed attention: the scale is not finite");
   if (a->n_tokens == 0) return 0;
-  if (a->rounds < 0 || a->most_rounds < 0 || a->most_rounds > a->n_tokens / kColumns + 2)
-    return fail("packed attention: rounds that no plan of these tokens has");
+  if (a->rounds < 0 || a->most_rounds < 0 || a->most_rounds > a->n_tokens / kColumns + 2 || a->short_tiles < 0 ||
+      a->short_tiles > 2 * tiles_of(a->n_tokens) + 3)
+    return fail("packed attention: a size that no plan of these tokens has");
   const void* in[] = {a->q, a->k, a->v, a->out, a->lse, a->plan, a->dout, a->dq, a->dk, a->dv};
   for (int i = 0; i < (backward ? 10 : 6); ++i) {
     if (!in[i]) return fail("packed attention: null array");
@@ -721,7 +888,7 @@ int check_attention(const nd_packed_attention* a, bool backward) {
       return fail("packed attention: strides are multiples of 8 elements, a token's at most " +
                   std::to_string(ND_PACKED_MAX_TOKEN_STRIDE));
   const Cuts cuts = cuts_of(*a, backward);
-  if (tiles_of(a->n_tokens) * a->heads * std::max(cuts.max_chunks, cuts.max_key_chunks) > 0x7fffffff)
+  if ((2 * tiles_of(a->n_tokens) + 3) * a->heads * std::max(cuts.max_chunks, cuts.max_key_chunks) > 0x7fffffff)
     return fail("packed attention: more tokens and heads than one launch holds");
   if (a->workspace_bytes < cuts.bytes)
     return fail("packed attention: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(cuts.bytes) +
@@ -740,6 +907,8 @@ int run_attention(const nd_packed_attention* a, bool backward, void* stream) {
   p.plan.last = p.plan.first + parts.last;
   p.plan.query_order = p.plan.first + parts.query_order;
   p.plan.key_order = p.plan.first + parts.key_order;
+  p.plan.short_starts = p.plan.first + parts.short_starts;
+  p.plan.short_tiles = (int32_t)a->short_tiles;
   p.plan.tokens = (int32_t)a->n_tokens;
   p.plan.covered = (int32_t)a->n_covered;
   p.plan.tiles = (int32_t)tiles_of(a->n_tokens);
@@ -799,7 +968,7 @@ int64_t nd_packed_plan_bytes(int64_t n_tokens) {
 }
 
 int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens, const int32_t* d_starts, void* d_plan,
-                   int64_t rounds[2], void* stream) {
+                   int64_t sizes[3], void* stream) {
   return nd::guarded([&]() -> int {
     if (n_tokens < 0 || n_tokens > ND_PACKED_MAX_TOKENS || n_sequences < 0 || n_sequences > ND_PACKED_MAX_TOKENS)
       return nd::fail("packed sequences: between 0 and " + std::to_string((int64_t)ND_PACKED_MAX_TOKENS) + " tokens and sequences");
@@ -811,17 +980,29 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
     if (starts[n_sequences] > n_tokens)
       return nd::fail("packed sequences: " + std::to_string(starts[n_sequences]) + " tokens in sequences, " +
                       std::to_string(n_tokens) + " tokens");
-    if (!rounds) return nd::fail("packed sequences: null array");
-    rounds[0] = rounds[1] = 0;
+    if (!sizes) return nd::fail("packed sequences: null array");
+    sizes[0] = sizes[1] = sizes[2] = 0;
     int64_t of = 0;  // the sequence that a tile's first token is in
     for (int64_t t = 0; t < starts[n_sequences]; t += nd::kRows) {
       while (starts[of + 1] <= t) ++of;
       const int64_t end = std::min<int64_t>(t + nd::kRows, starts[n_sequences]);
       const int64_t one = (end - starts[of] + nd::kColumns - 1) / nd::kColumns;
-      rounds[0] += one;
+      sizes[0] += one;
       // as a tile of queries, and as one of keys (whose last token's sequence may end after it)
       const int32_t* after = std::upper_bound(starts + of + 1, starts + n_sequences + 1, (int32_t)(end - 1));
-      rounds[1] = std::max(rounds[1], std::max(one, (*after - t + nd::kColumns - 1) / nd::kColumns));
+      sizes[1] = std::max(sizes[1], std::max(one, (*after - t + nd::kColumns - 1) / nd::kColumns));
+    }
+    // whole sequences to a tile, if none is longer
+    std::vector<int32_t> cuts;
+    int64_t longest = 0;
+    for (int64_t i = 0; i < n_sequences; ++i) longest = std::max<int64_t>(longest, starts[i + 1] - starts[i]);
+    if (longest <= nd::kRows) {
+      cuts.push_back(0);
+      for (int64_t i = 1; i <= n_sequences; ++i)
+        if (starts[i] - cuts.back() > nd::kRows) cuts.push_back(starts[i - 1]);
+      if (starts[n_sequences] > cuts.back()) cuts.push_back(starts[n_sequences]);
+      while (cuts.back() < n_tokens) cuts.push_back((int32_t)std::min<int64_t>((int64_t)cuts.back() + nd::kRows, n_tokens));
+      sizes[2] = (int64_t)cuts.size() - 1;
     }
     if (n_tokens == 0) return 0;
     if (!d_starts || !d_plan || ((uintptr_t)d_plan & 15)) return nd::fail("packed sequences: null or misaligned device array");
@@ -832,7 +1013,10 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
     nd::packed_order_kernel<<<2, nd::kOrderThreads, 0, (hipStream_t)stream>>>(
         first, first + parts.last, (int32_t)n_tokens, starts[n_sequences], (int32_t)nd::tiles_of(n_tokens), first + parts.query_order,
         first + parts.key_order);
-    const hipError_t e = hipGetLastError();
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && sizes[2] > 0)  // (from pageable memory: done with it when the call returns)
+      e = hipMemcpyAsync(first + parts.short_starts, cuts.data(), cuts.size() * sizeof(int32_t), hipMemcpyHostToDevice,
+                         (hipStream_t)stream);
     if (e != hipSuccess) return nd::fail(std::string("packed sequences: ") + hipGetErrorString(e));
     return 0;
   });

@@ -161,10 +161,10 @@ class PackedSequences:
         _need(size >= 0, "packed sequences: no plan for %d tokens" % self.n_tokens)
         on_device = torch.from_numpy(starts).to(self.device)
         self.plan = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
-        rounds = (C.c_int64 * 2)()
+        sizes = (C.c_int64 * 3)()
         _run(self.device.index, lib.nd_packed_plan, starts.ctypes.data, self.n_sequences, self.n_tokens,
-             on_device.data_ptr(), self.plan.data_ptr(), rounds)
-        self.rounds = rounds[0], rounds[1]
+             on_device.data_ptr(), self.plan.data_ptr(), sizes)
+        self.sizes = tuple(sizes)
 
 
 def _heads(what, x, tokens, dim):
@@ -199,7 +199,7 @@ def _attention(sequences, q, k, v, scale, dout=None):
         _need(dout.shape == q.shape and dout.dtype is dtype, "packed attention: dout is of another shape or type than q")
         dout, d_token, d_head = _heads("dout", dout, tokens, dim)
         d_at = dout.data_ptr()
-    fields = (tokens, sequences.n_covered, *sequences.rounds, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
+    fields = (tokens, sequences.n_covered, *sequences.sizes, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
               sequences.plan.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), d_at,
               q_token, q_head, k_token, k_head, v_token, v_head, d_token, d_head)
     return index, (q, k, v, dout), fields, (heads, tokens)
