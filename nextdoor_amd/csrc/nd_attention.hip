@@ -186,9 +186,12 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     int half = 0;
     for (int n0 = begin; n0 < stop; n0 += kColumns, half ^= 1) {
       wait_for_loads_and_others();
-      if (n0 + kColumns < stop) issue(half ^ 1, n0 + kColumns);
+      const bool more = n0 + kColumns < stop;
       // (wave-uniform) every key is later than the wave's rows, or before their sequences
-      if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
+      if (n0 > row0 + 31 || n0 + kColumns <= first_min) {
+        if (more) issue(half ^ 1, n0 + kColumns);
+        continue;
+      }
       const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
       f32x16 s[2];
 #pragma unroll
@@ -198,6 +201,9 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
         for (int i = 0; i < 2 * NB; ++i)
           s[t] = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s[t]);
       }
+      // (asked for behind the first products and not before them, where the wave would wait for its loads to be taken: 38 for
+      // 44 us with few workgroups, 2 % with many)
+      if (more) issue(half ^ 1, n0 + kColumns);
       if (n0 + kColumns - 1 > row0 || n0 < first_max) {
         const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
 #pragma unroll
@@ -373,9 +379,11 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
       float sum = 0.f;
       for (int n0 = begin; n0 < stop; n0 += kColumns, half ^= 1) {
         wait_for_loads_and_others();
-        if (n0 + kColumns < stop) issue(half ^ 1, n0 + kColumns);
-        else if (DELTA) issue(half ^ 1, begin);
-        if (n0 > row0 + 31 || n0 + kColumns <= first_min) continue;
+        const int next = n0 + kColumns < stop ? n0 + kColumns : DELTA ? begin : -1;
+        if (n0 > row0 + 31 || n0 + kColumns <= first_min) {
+          if (next >= 0) issue(half ^ 1, next);
+          continue;
+        }
         const u32x4 *keys = tiles[half][0], *values = tiles[half][1];
         const bool masked = n0 + kColumns - 1 > row0 || n0 < first_max;
         const int from = first - n0 - 4 * h, to = row - n0 - 4 * h;
@@ -387,6 +395,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
             s = product_32x32x16<T>(read_operand_by_rows<kChunks>(keys, 32 * t, i, lane), qf[i], s);
             dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
           }
+          if (t == 0 && next >= 0) issue(half ^ 1, next);
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
           if (masked) {
