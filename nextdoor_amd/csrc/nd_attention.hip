@@ -130,6 +130,168 @@ __device__ __forceinline__ void chunk_tile_and_head(int max_chunks, int heads, i
   if (heads % 8 == 0) head = (head % 8) * (heads / 8) + head / 8;
 }
 
+// ---- values that are not finite ---------------------------------------------------------------------
+// A key that a row does not see has weight 0 in the matrix products, and 0 x NaN is NaN: an infinity or NaN of one sequence, or
+// of a later token, would reach every row whose tile holds it.  A wave whose sums have turned out not finite (one instruction
+// for each at its end) takes them again here, pair by pair, leaving out the pairs that the mask leaves out; what a row
+// does see comes out as it should, finite or not.  Lane: a row and half of its columns, 16 s + 8 h .. + 7; 32-bit arithmetic on
+// the vector units, so that a wave takes some 0.5 us for each key.
+template <int NB>
+__device__ __forceinline__ bool all_finite(const f32x16 (&acc)[NB]) {
+  float zero = 0.f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(acc[b][i], 0.f, zero);
+  return zero == 0.f;
+}
+// Rows are read again for every pair: few registers, and none that the sums above would have to leave.
+template <class T>
+__device__ __forceinline__ float dot_rows(const char* a, const char* b, int dim, int h) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 16 * h; c < 2 * dim; c += 32) {
+    const u32x4 x = *(const u32x4*)(a + c), y = *(const u32x4*)(b + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sum = __builtin_fmaf(unpack_low<T>(x[j]), unpack_low<T>(y[j]), sum);
+      sum = __builtin_fmaf(unpack_high<T>(x[j]), unpack_high<T>(y[j]), sum);
+    }
+  }
+  return pair_sum(sum);
+}
+template <int NB>
+struct HalfRow {
+  float v[16 * NB];
+};
+// acc = acc shrink + weight row
+template <class T, int NB>
+__device__ __forceinline__ void add_row(HalfRow<NB>& acc, float shrink, float weight, const char* row, int dim, int h) {
+#pragma unroll
+  for (int s = 0; s < 2 * NB; ++s) {
+    if (16 * s + 8 * h >= dim) continue;
+    const u32x4 v = *(const u32x4*)(row + 32 * s + 16 * h);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc.v[8 * s + 2 * j] = __builtin_fmaf(weight, unpack_low<T>(v[j]), acc.v[8 * s + 2 * j] * shrink);
+      acc.v[8 * s + 2 * j + 1] = __builtin_fmaf(weight, unpack_high<T>(v[j]), acc.v[8 * s + 2 * j + 1] * shrink);
+    }
+  }
+}
+// A lane's half of a result row: `row` as the final values, or, if it is null, `sums` in 32 bits.
+template <class T, int NB>
+__device__ __forceinline__ void store_half(T* row, float* sums, const HalfRow<NB>& acc, float factor, int dim, int h) {
+#pragma unroll
+  for (int s = 0; s < 2 * NB; ++s) {
+    const int column = 16 * s + 8 * h;
+    if (column >= dim) continue;
+    if (row) {
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = pack_pair<T>(acc.v[8 * s + 2 * j] * factor, acc.v[8 * s + 2 * j + 1] * factor);
+      *(u32x4*)(row + column) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[column + j] = acc.v[8 * s + j] * factor;
+    }
+  }
+}
+
+// (there: first <= row.  The rows of lanes that are not there are read all the same: a row that is.)
+template <class T, int NB>
+__device__ __forceinline__ void forward_carefully(const AttentionParams& p, int head, int kv_head, int row, int first, int begin, int stop,
+                                                  int row_end, int chunk, int chunks) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const bool there = first <= row;
+  const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
+  const char* q = (const char*)p.q + (int64_t)(there ? row : begin) * p.q_token + (int64_t)head * p.q_head;
+  HalfRow<NB> acc = {};
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+  for (int key = begin; key < stop; ++key) {
+    const bool sees = there && key >= first && key <= row;
+    if (__builtin_amdgcn_ballot_w64(sees) == 0) continue;
+    const float s = dot_rows<T>(q, (const char*)p.k + (int64_t)key * p.k_token + (int64_t)kv_head * p.k_head, p.dim, h) * scale;
+    if (!sees) continue;
+    const float higher = fmaxf(top, s), base = higher == -INFINITY ? 0.f : higher;
+    const float shrink = exp2_fast(top - base), weight = exp2_fast(s - base);
+    top = higher;
+    sum = sum * shrink + weight;
+    add_row<T, NB>(acc, shrink, weight, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, p.dim, h);
+  }
+  if (row >= row_end) return;
+  const int64_t at = (int64_t)head * p.plan.tokens + row;
+  if (chunks > 1) {
+    if (h == 0) p.row_tops[(int64_t)chunk * p.heads * p.plan.tokens + at] = make_float2(top, sum);
+    store_half<T, NB>(nullptr, p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, 1.f, p.dim, h);
+    return;
+  }
+  if (h == 0) p.lse[at] = (top + log2f(sum)) * kLn2;
+  store_half<T, NB>((T*)p.out_w + ((int64_t)row * p.heads + head) * p.dim, nullptr, acc, sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum,
+                    p.dim, h);
+}
+
+template <class T, int NB>
+__device__ __forceinline__ void dq_carefully(const AttentionParams& p, int head, int kv_head, int row, int first, int begin, int stop,
+                                             int row_end, float delta, int chunk, int chunks) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const bool there = first <= row;
+  const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
+  const float lse2 = there ? p.lse[(int64_t)head * p.plan.tokens + row] * kLog2e : 0.f;
+  const char* q = (const char*)p.q + (int64_t)(there ? row : begin) * p.q_token + (int64_t)head * p.q_head;
+  const char* d = (const char*)p.dout + (int64_t)(there ? row : begin) * p.dout_token + (int64_t)head * p.dout_head;
+  HalfRow<NB> acc = {};
+#pragma unroll 1
+  for (int key = begin; key < stop; ++key) {
+    const bool sees = there && key >= first && key <= row;
+    if (__builtin_amdgcn_ballot_w64(sees) == 0) continue;
+    const char* k = (const char*)p.k + (int64_t)key * p.k_token + (int64_t)kv_head * p.k_head;
+    const float dp = dot_rows<T>(d, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, p.dim, h);
+    const float ds = exp2_fast(__builtin_fmaf(dot_rows<T>(q, k, p.dim, h), scale, -lse2)) * (dp - delta);
+    if (sees) add_row<T, NB>(acc, 1.f, ds, k, p.dim, h);
+  }
+  if (row >= row_end) return;
+  const int64_t at = (int64_t)row * p.heads + head;
+  store_half<T, NB>(chunks > 1 ? nullptr : (T*)p.dq + at * p.dim,
+                    chunks > 1 ? p.row_sums + ((int64_t)chunk * p.plan.tokens * p.heads + at) * p.dim : nullptr, acc, p.scale, p.dim, h);
+}
+
+// Rounds begin .. stop - 1 of `round` queries each, as the dk, dv kernel counts them; part: of the sums, or -1.
+template <class T, int NB>
+__device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv_head, int head0, int key, int last, int tile0, int end,
+                                                int round, int head_rounds, int begin, int stop, int key_end, int part) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const bool there = last > key;
+  const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
+  const char* k = (const char*)p.k + (int64_t)(there ? key : tile0) * p.k_token + (int64_t)kv_head * p.k_head;
+  const char* v = (const char*)p.v + (int64_t)(there ? key : tile0) * p.v_token + (int64_t)kv_head * p.v_head;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {  // dv, dk
+    HalfRow<NB> acc = {};
+#pragma unroll 1
+    for (int n = begin; n < stop; ++n) {
+      const int head = head0 + n / head_rounds, m0 = tile0 + n % head_rounds * round;
+#pragma unroll 1
+      for (int query = m0; query < min(m0 + round, end); ++query) {
+        const bool sees = there && query >= key && query < last;
+        if (__builtin_amdgcn_ballot_w64(sees) == 0) continue;
+        const int64_t at = (int64_t)head * p.plan.tokens + query;
+        const char* q = (const char*)p.q + (int64_t)query * p.q_token + (int64_t)head * p.q_head;
+        const char* d = (const char*)p.dout + (int64_t)query * p.dout_token + (int64_t)head * p.dout_head;
+        float weight = exp2_fast(__builtin_fmaf(dot_rows<T>(k, q, p.dim, h), scale, -p.lse[at] * kLog2e));
+        if (which == 1) weight *= dot_rows<T>(v, d, p.dim, h) - p.delta[at];
+        if (sees) add_row<T, NB>(acc, 1.f, weight, which == 0 ? d : q, p.dim, h);
+      }
+    }
+    if (key >= key_end) continue;
+    const int64_t at = (int64_t)key * p.kv_heads + kv_head;
+    float* const sums = which == 0 ? p.dv_sums : p.dk_sums;
+    store_half<T, NB>(part >= 0 ? nullptr : (T*)(which == 0 ? p.dv : p.dk) + at * p.dim,
+                      part >= 0 ? sums + ((int64_t)part * p.plan.tokens * p.kv_heads + at) * p.dim : nullptr, acc,
+                      which == 0 ? 1.f : p.scale, p.dim, h);
+  }
+}
+
 // ---- forward ------------------------------------------------------------------------------------
 // One workgroup: 128 query tokens of one head; one wave: 32 of them, lane's token is column l & 31 of S^T = K Q^T, so
 // the softmax of a row runs over a lane's own registers and its partner's, 32 lanes away, and P^T is the second operand of
@@ -157,7 +319,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
 #pragma unroll
   for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   float top = -INFINITY, sum = 0.f;  // sum: over the lane's own keys
-  int chunks = 1;
+  int chunks = 1, careful_begin = 0, careful_stop = 0;
 
   if (tile0 < p.plan.covered) {
     const int first_key = uniform(p.plan.first[tile0]);
@@ -166,6 +328,8 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     if (chunk >= chunks) return;
     const int begin = first_key + uniform(rounds * chunk / chunks) * kColumns;
     const int stop = chunk + 1 < chunks ? first_key + uniform(rounds * (chunk + 1) / chunks) * kColumns : end;
+    careful_begin = begin;
+    careful_stop = stop;
     const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
     auto issue = [&](int half, int n0) {
@@ -261,6 +425,10 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
   sum = pair_sum(sum);
+  if (__builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0) {
+    forward_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, tile_end, chunk, chunks);
+    return;
+  }
   if (chunks > 1) {
     if (row >= tile_end) return;
     if (h == 0) p.row_tops[((int64_t)chunk * p.heads + head) * p.plan.tokens + row] = make_float2(top, sum);
@@ -324,7 +492,8 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);
   const bool there = row < p.plan.covered;
   f32x16 acc[NB];
-  int chunks = 1;
+  int chunks = 1, careful_begin = 0, careful_stop = 0;
+  float delta = 0.f;
   if (tile0 < p.plan.covered) {
     const int end = min(tile0 + kRows, p.plan.covered), first_key = uniform(p.plan.first[tile0]);
     const int rounds = (end - first_key + kColumns - 1) / kColumns;
@@ -332,6 +501,8 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
     if (chunk >= chunks) return;
     const int begin = first_key + uniform(rounds * chunk / chunks) * kColumns;
     const int stop = chunk + 1 < chunks ? first_key + uniform(rounds * (chunk + 1) / chunks) * kColumns : end;
+    careful_begin = begin;
+    careful_stop = stop;
     const bool exact = chunks == 1 && rounds <= kExactDeltaRounds;
     const TileLoader<NB> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024;
@@ -346,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
     u32x4 qf[2 * NB], dof[2 * NB];
     load_rows<NB>(qf, (const char*)p.q + (int64_t)row * p.q_token + (int64_t)head * p.q_head, there, p.dim, h);
     load_rows<NB>(dof, (const char*)p.dout + (int64_t)row * p.dout_token + (int64_t)head * p.dout_head, there, p.dim, h);
-    float delta = 0.f, lse2 = 0.f;
+    float lse2 = 0.f;
     {
       u32x4 of[2 * NB];
       load_rows<NB>(of, (const char*)p.out + ((int64_t)row * p.heads + head) * p.dim * 2, there, p.dim, h);
@@ -440,6 +611,11 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
+  if (row0 < p.plan.tokens && __builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0) {
+    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, p.plan.tokens, delta, chunk,
+                        chunks);
+    return;
+  }
   if (chunks > 1) {
     if (row < p.plan.tokens)
       store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, p.scale, p.dim, h);
@@ -479,7 +655,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     dk[b] = f32x16{};
     dv[b] = f32x16{};
   }
-  int chunks = 1;
+  int chunks = 1, careful_begin = 0, careful_stop = 0, careful_rounds = 1, careful_end = 0;
   if (tile0 < p.plan.covered) {
     const int end = uniform(p.plan.last[min(tile0 + kRows, p.plan.covered) - 1]);
     const int head0 = kv_head * p.group + share * heads, head_rounds = (end - tile0 + kRound - 1) / kRound, rounds = head_rounds * heads;
@@ -487,6 +663,10 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     if (chunk >= chunks) return;
     // round i: head i / head_rounds of the share, queries from tile0 + i % head_rounds * kRound on
     const int begin = uniform((int)((int64_t)rounds * chunk / chunks)), stop = uniform((int)((int64_t)rounds * (chunk + 1) / chunks));
+    careful_begin = begin;
+    careful_stop = stop;
+    careful_rounds = head_rounds;
+    careful_end = end;
     const TileLoader<NB, kRound> q(p.q, p.q_token, p.q_head, head0, p.dim), d(p.dout, p.dout_token, p.dout_head, head0, p.dim);
     const uint32_t lds = lds_address(&tiles[0][0][0]) + wave * 1024, rows_lds = lds_address(&rows_of[0][0][0]);
     auto issue = [&](int half, int head, int m0) {  // head: of the share
@@ -586,6 +766,12 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     return;
   }
   if (key0 >= p.plan.tokens) return;
+  if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) != 0) {
+    dk_dv_carefully<T, NB>(p, kv_head, kv_head * p.group + share * heads, key, there ? p.plan.last[key] : key, tile0, careful_end, kRound,
+                           careful_rounds, careful_begin, careful_stop, p.plan.tokens,
+                           chunks * p.head_split == 1 ? -1 : chunk * p.head_split + share);
+    return;
+  }
   const int64_t row_elements = (int64_t)p.kv_heads * p.dim;
   if (chunks * p.head_split == 1) {
     u32x4* part_lds = &tiles[0][0][0] + wave * 32 * kChunks;
@@ -617,6 +803,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
+  bool again = false;  // some head's dq is not finite: taken carefully at the end, where no sums are in registers
 
   if (tile0 < p.plan.covered) {
     // (such a tile ends at `covered` or before it)
@@ -684,7 +871,10 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
           }
           if (sweep == 0) delta = pair_sum(sum);
         }
-        if (h == 0) deltas[wave * 32 + (lane & 31)] = delta;
+        if (h == 0) {
+          deltas[wave * 32 + (lane & 31)] = delta;
+          if (there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
+        }
       }
       __syncthreads();
       if (work) {
@@ -726,6 +916,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
         }
       }
       __syncthreads();
+      again = again || __builtin_amdgcn_ballot_w64(!all_finite(dq)) != 0;
       if (work)
         store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, p.scale, p.dim, part_lds);
     }
@@ -735,9 +926,22 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
                         part_lds);
   }
   if (row0 >= tile_end) return;
-  const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
-  store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, p.scale, p.dim, part_lds);
-  store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, 1.f, p.dim, part_lds);
+  if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) == 0) {
+    const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
+    store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, p.scale, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, 1.f, p.dim, part_lds);
+  } else {
+    dk_dv_carefully<T, NB>(p, kv_head, kv_head * p.group, row, row < tile_end ? p.plan.last[row] : row, tile0, tile_end, kRows, 1, 0, p.group,
+                           tile_end, -1);
+  }
+  if (!again) return;
+#pragma unroll 1
+  for (int g = 0; g < p.group; ++g) {
+    const int head = kv_head * p.group + g;
+    const bool there = row < tile_end;
+    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, tile0, tile_end, tile_end,
+                        there ? p.delta[(int64_t)head * p.plan.tokens + row] : 0.f, 0, 1);
+  }
 }
 
 // Adds the chunks of cut tiles: dq (WHICH 0), dk (1), dv (2); n values each, a lane has four.
@@ -805,9 +1009,10 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     return at;
   };
   const int64_t row_bytes = a.n_tokens * a.heads * a.dim * 4, key_bytes = a.n_tokens * a.kv_heads * a.dim * 4;
-  if (a.short_tiles > 0) {  // nothing to cut, nothing to keep
-    w.chunk = w.max_chunks = w.key_chunk = w.max_key_chunks = w.head_split = 1 << 20;
+  if (a.short_tiles > 0) {  // nothing to cut
+    w.chunk = w.key_chunk = 1 << 20;
     w.max_chunks = w.max_key_chunks = w.head_split = 1;
+    if (backward) w.delta = take(a.n_tokens * a.heads * 4);
     return w;
   }
   w.chunk = std::max<int64_t>(8, (a.rounds * a.heads + kItems - 1) / kItems);

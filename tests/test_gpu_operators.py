@@ -65,8 +65,9 @@ def test_attention_over_lengths(lengths, heads, kv_heads, dim, dtype):
 
 @pytest.mark.parametrize("dim", [8, 16, 24, 40, 72, 80, 96, 104, 120])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_attention_head_sizes(dim, dtype):
-    starts = starts_of([17, 150, 33])
+@pytest.mark.parametrize("longest", [150, 77])
+def test_attention_head_sizes(dim, dtype, longest):
+    starts = starts_of([17, longest, 33])
     t = int(starts[-1])
     q, dout = normal(1, t, 2, dim, dtype=dtype), normal(2, t, 2, dim, dtype=dtype)
     k, v = normal(3, t, 1, dim, dtype=dtype), normal(4, t, 1, dim, dtype=dtype)
@@ -120,6 +121,44 @@ def test_attention_leaves_tokens_of_no_sequence_alone():
     check_all(got, want, off, "rest")
     assert not got["out"][155:].any() and torch.isinf(got["lse"][:, 155:]).all()
     assert not got["dq"][155:].any() and not got["dk"][155:].any() and not got["dv"][155:].any()
+
+
+@pytest.mark.parametrize("lengths,dim,kv_heads", [
+    ([40, 50, 30], 64, 2), ([3, 17, 100, 8], 128, 1), ([1, 1, 5, 60], 32, 2), ([100, 28, 128], 96, 4),  # whole sequences to a tile
+    ([200, 90, 300], 64, 2), ([129, 5, 140], 128, 4), ([70, 350, 9], 80, 1), ([20, 1500, 30], 128, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_what_is_not_seen_does_not_matter(lengths, dim, kv_heads, dtype):
+    """A NaN or infinity in one token reaches the rows whose formulas hold it and no other: not the sequences next to it
+    in a tile, not the earlier rows of its own."""
+    starts = starts_of(lengths)
+    t, heads = int(starts[-1]), 4
+    q, dout = normal(1, t, heads, dim, dtype=dtype), normal(2, t, heads, dim, dtype=dtype)
+    k, v = normal(3, t, kv_heads, dim, dtype=dtype), normal(4, t, kv_heads, dim, dtype=dtype)
+    want, off = ref.attention(q, k, v, starts, 1 / math.sqrt(dim), dout)
+    seq = int(np.argmax(lengths))
+    begin, end = int(starts[seq]), int(starts[seq + 1])
+    bad = begin + (end - begin) * 2 // 3
+    rows = torch.arange(t)
+    for value in (math.nan, math.inf):
+        # v of one token: out and dq of the rows from it on; through their delta, dk of the whole sequence; never dv
+        x = v.clone()
+        x[bad] = value
+        got = run_attention(q.cuda(), k.cuda(), x.cuda(), starts, dout.cuda())
+        hit = (rows >= bad) & (rows < end)
+        whole = (rows >= begin) & (rows < end)
+        for name, these in (("out", hit), ("dq", hit), ("dk", whole), ("dv", rows < 0)):
+            assert not torch.isfinite(got[name].cpu()[these]).any(), (name, value)
+            assert ref.close(got[name].cpu()[~these], want[name][~these], off[name][~these]), (name, value)
+        assert ref.close(got["lse"], want["lse"], off["lse"])
+        # the gradient of one row: its own dq, dk and dv of the keys up to it
+        x = dout.clone()
+        x[bad] = value
+        got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, x.cuda())
+        upto = (rows >= begin) & (rows <= bad)
+        for name, these in (("out", rows < 0), ("dq", rows == bad), ("dk", upto), ("dv", upto)):
+            finite = torch.isfinite(got[name].cpu()[these]).float().mean() if these.any() else 0
+            assert finite < 0.5, (name, value, finite)  # (a weight that has become 0 in 16 bits times infinity is NaN too)
+            assert ref.close(got[name].cpu()[~these], want[name][~these], off[name][~these]), (name, value)
 
 
 def test_attention_without_any_sequence():
