@@ -472,3 +472,69 @@ def test_dropout_refuses():
         with pytest.raises(NextDoorError):
             ops.dropout_forward(*args)
     assert ops.dropout_forward(x[:0], 0.5, 1, 1).shape == (0,)
+
+
+# ---- together --------------------------------------------------------------------------------------
+
+
+def test_a_walk_model_learns():
+    """Walks from the engine, packed, through all three operators, forward and backward: the loss falls from that of a guess,
+    and the same seeds give the same losses."""
+    from nextdoor_amd import Graph, walk_model
+    graph = Graph.chung_lu(500, 6000, 2.2, seed=3)
+    losses = [walk_model.train(graph, steps=30, walks=400, seed=5, log=None, dropout=0.1)[1] for _ in range(2)]
+    assert abs(losses[0][0] - math.log(500)) < 1.0
+    assert losses[0][-1] < losses[0][0] - 0.5
+    assert losses[0][0] == losses[1][0]
+
+
+def test_walk_model_gradients_are_those_of_plain_operations():
+    """One step of the model in 16 bits against the same model with the definitions in 64 bits."""
+    from nextdoor_amd import walk_model
+    torch.manual_seed(1)
+    n, width = 97, 64
+    rng = np.random.default_rng(2)
+    samples = rng.integers(0, n, (20, 30)).astype(np.int32)
+    for walk in samples[::2]:
+        walk[rng.integers(0, 30):] = n
+    tokens, targets, starts = walk_model.pack_walks(rng.integers(0, n, 20), samples, n)
+    model = walk_model.WalkModel(n, width=width, heads=2, kv_heads=1, layers=1, dropout=0.2).to("cuda", BF16)
+    batch = walk_model.batch_of(tokens, targets, starts)
+    each = model(*batch[:3], batch[3], 11)
+    each.sum().backward()
+
+    exact = walk_model.WalkModel(n, width=width, heads=2, kv_heads=1, layers=1, dropout=0.2).double()
+    exact.load_state_dict({k: v.double().cpu() for k, v in model.state_dict().items()})
+
+    def attention(q, k, v, sequences, scale=None):
+        of = torch.from_numpy(np.repeat(np.arange(len(starts) - 1), np.diff(starts)))
+        at = torch.arange(len(of))
+        sees = (of[:, None] == of) & (at[:, None] >= at)
+        out = []
+        for h in range(q.shape[1]):
+            s = (q[:, h] @ k[:, h // (q.shape[1] // k.shape[1])].T / math.sqrt(q.shape[2])).masked_fill(~sees, -math.inf)
+            out.append(torch.softmax(s, 1) @ v[:, h // (q.shape[1] // k.shape[1])])
+        return torch.stack(out, 1)
+
+    def drop(x, p, seed, step, residual=None):
+        kept = torch.from_numpy(ref.uniforms(x.numel(), seed, step) >= np.float32(p)).view(x.shape)
+        y = x * kept / (1 - p)
+        return y if residual is None else y + residual
+
+    def loss(h, w, t):
+        has = (t >= 0) & (t < n)
+        z = h @ w.T
+        return torch.where(has, torch.logsumexp(z, 1) - z.gather(1, torch.where(has, t, 0).long()[:, None])[:, 0], 0.0)
+
+    kept = ops.packed_attention, ops.dropout, ops.vocabulary_loss
+    try:
+        ops.packed_attention, ops.dropout, ops.vocabulary_loss = attention, drop, loss
+        want = exact(batch[0].cpu(), batch[1].cpu(), batch[2].cpu(), None, 11)
+        want.sum().backward()
+    finally:
+        ops.packed_attention, ops.dropout, ops.vocabulary_loss = kept
+    # the model itself works in bfloat16 throughout: a dozen roundings of 2^-9 each on a path, of random sign
+    assert abs(float(each.detach().sum()) / float(want.detach().sum()) - 1) < 0.02
+    for (name, a), (_, b) in zip(model.named_parameters(), exact.named_parameters()):
+        off = float((a.grad.double().cpu() - b.grad).norm() / b.grad.norm())
+        assert off < 0.05, (name, off)
