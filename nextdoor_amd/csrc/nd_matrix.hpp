@@ -150,10 +150,11 @@ __device__ __forceinline__ void wait_for_loads_and_others() {
 
 // The block's index such that blocks with neighbouring results run on one of the eight dies, whose L2 they share:
 // consecutive workgroups go to the dies in turn.
-__device__ __forceinline__ uint32_t block_by_die() {
-  const uint32_t n = gridDim.x, die = blockIdx.x % 8, turn = blockIdx.x / 8;
+__device__ __forceinline__ uint32_t block_by_die(uint32_t block, uint32_t n) {
+  const uint32_t die = block % 8, turn = block / 8;
   return die * (n / 8) + min(die, n % 8) + turn;
 }
+__device__ __forceinline__ uint32_t block_by_die() { return block_by_die(blockIdx.x, gridDim.x); }
 
 // Over the two lanes 32 apart.
 __device__ __forceinline__ float pair_max(float v) {
