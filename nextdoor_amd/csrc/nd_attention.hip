@@ -787,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
 
 // Sequences of at most a tile: one workgroup has the whole sequences of a tile and one key head, so that it reads queries, keys,
 // values and output gradients once and has all of dq, dk and dv (batch of walks, 8 heads of 64: 59 us; 91 for the two kernels
-// above, which are bound by what they read).  Per head of the group each wave first has 32 queries, as in the dq kernel, then
+// above, which are bound by what they read).  Where tiles are few a group's heads are shared out, as in the dk, dv kernel.  Per head of the group each wave first has 32 queries, as in the dq kernel, then
 // 32 keys, as in the other one; delta always comes from the weights themselves.
 template <class T, int NB>
 __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short_kernel(AttentionParams p) {
@@ -795,7 +795,9 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   __shared__ u32x4 keys[kSize], values[kSize], queries[kSize], douts[kSize];
   __shared__ float lse2s[kRows], deltas[kRows];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
-  const int kv_head = uniform(blockIdx.x % p.kv_heads), tile = uniform(blockIdx.x / p.kv_heads);
+  const int units = p.kv_heads * p.head_split, unit = uniform(blockIdx.x % units), tile = uniform(blockIdx.x / units);
+  const int kv_head = uniform(unit / p.head_split), share = unit - kv_head * p.head_split, heads = uniform(p.group / p.head_split);
+  const int head0 = kv_head * p.group + share * heads;
   const int tile0 = uniform(p.plan.short_starts[tile]), tile_end = uniform(p.plan.short_starts[tile + 1]);
   const int row0 = tile0 + wave * 32, row = row0 + (lane & 31);  // as queries and as keys
   u32x4* const part_lds = queries + wave * 32 * kChunks;
@@ -815,8 +817,8 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
     const TileLoader<NB, kRows> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     k.issue(lds_address(keys) + part, p.k_token, tile0, tile_end);
     v.issue(lds_address(values) + part, p.v_token, tile0, tile_end);
-    for (int g = 0; g < p.group; ++g) {
-      const int head = kv_head * p.group + g;
+    for (int g = 0; g < heads; ++g) {
+      const int head = head0 + g;
       if (g > 0) __syncthreads();  // (the last head's dq has left through `queries`)
       const TileLoader<NB, kRows> q(p.q, p.q_token, p.q_head, head, p.dim), d(p.dout, p.dout_token, p.dout_head, head, p.dim);
       q.issue(lds_address(queries) + part, p.q_token, tile0, tile_end);
@@ -921,23 +923,27 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
         store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, p.scale, p.dim, part_lds);
     }
   } else if (row0 < tile_end) {  // tokens of no sequence
-    for (int g = 0; g < p.group; ++g)
-      store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + kv_head * p.group + g) * p.dim, q_elements, tile_end - row0, dk, 0.f, p.dim,
+    for (int g = 0; g < heads; ++g)
+      store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head0 + g) * p.dim, q_elements, tile_end - row0, dk, 0.f, p.dim,
                         part_lds);
   }
   if (row0 >= tile_end) return;
-  if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) == 0) {
+  if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) != 0) {
+    dk_dv_carefully<T, NB>(p, kv_head, head0, row, row < tile_end ? p.plan.last[row] : row, tile0, tile_end, kRows, 1, 0, heads, tile_end,
+                           p.head_split == 1 ? -1 : share);
+  } else if (p.head_split == 1) {
     const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
     store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, p.scale, p.dim, part_lds);
     store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, 1.f, p.dim, part_lds);
-  } else {
-    dk_dv_carefully<T, NB>(p, kv_head, kv_head * p.group, row, row < tile_end ? p.plan.last[row] : row, tile0, tile_end, kRows, 1, 0, p.group,
-                           tile_end, -1);
+  } else if (row < tile_end) {
+    const int64_t at = (((int64_t)share * p.plan.tokens + row) * p.kv_heads + kv_head) * p.dim;
+    store_sums<NB>(p.dk_sums + at, dk, p.scale, p.dim, h);
+    store_sums<NB>(p.dv_sums + at, dv, 1.f, p.dim, h);
   }
   if (!again) return;
 #pragma unroll 1
-  for (int g = 0; g < p.group; ++g) {
-    const int head = kv_head * p.group + g;
+  for (int g = 0; g < heads; ++g) {
+    const int head = head0 + g;
     const bool there = row < tile_end;
     dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, tile0, tile_end, tile_end,
                         there ? p.delta[(int64_t)head * p.plan.tokens + row] : 0.f, 0, 1);
@@ -951,10 +957,10 @@ __global__ __launch_bounds__(256) void attention_add_kernel(AttentionParams p, i
   const int64_t n = which == 0 ? n_rows : n_keys, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n || (which == 0 ? p.max_chunks : p.max_key_chunks * p.head_split) == 1) return;
   const int token = (int)(i / p.dim / (which == 0 ? p.heads : p.kv_heads)), tile0 = token / kRows * kRows;
-  if (tile0 >= p.plan.covered) return;
   const int tile_end = min(tile0 + kRows, p.plan.covered);
   int chunks;
-  if (which == 0) chunks = (int)chunks_of((tile_end - p.plan.first[tile0] + kColumns - 1) / kColumns, p.chunk, p.max_chunks);
+  if (tile0 >= p.plan.covered) chunks = 1;  // (of the zeros there each share has left its own)
+  else if (which == 0) chunks = (int)chunks_of((tile_end - p.plan.first[tile0] + kColumns - 1) / kColumns, p.chunk, p.max_chunks);
   else
     chunks = (int)chunks_of((p.plan.last[tile_end - 1] - tile0 + key_round - 1) / key_round * (p.group / p.head_split), p.key_chunk, p.max_key_chunks);
   if (which > 0) chunks *= p.head_split;
@@ -1009,20 +1015,14 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     return at;
   };
   const int64_t row_bytes = a.n_tokens * a.heads * a.dim * 4, key_bytes = a.n_tokens * a.kv_heads * a.dim * 4;
-  if (a.short_tiles > 0) {  // nothing to cut
-    w.chunk = w.key_chunk = 1 << 20;
-    w.max_chunks = w.max_key_chunks = w.head_split = 1;
-    if (backward) w.delta = take(a.n_tokens * a.heads * 4);
-    return w;
-  }
   w.chunk = std::max<int64_t>(8, (a.rounds * a.heads + kItems - 1) / kItems);
   w.max_chunks = most(a.most_rounds, w.chunk, row_bytes);
   w.max_key_chunks = w.key_chunk = w.head_split = 1;
   if (backward) {
     const int64_t finer = kColumns / key_round_of(a.dim), group = a.heads / a.kv_heads;
-    while (w.head_split < group && (group % w.head_split != 0 || tiles_of(a.n_tokens) * a.kv_heads * w.head_split < kItems))
-      ++w.head_split;
-    w.key_chunk = std::min<int64_t>(w.chunk * finer, 0x3fffffff);
+    const int64_t tiles = a.short_tiles > 0 ? 2 * a.short_tiles : tiles_of(a.n_tokens);  // (half the work to be worth a share)
+    while (w.head_split < group && (group % w.head_split != 0 || tiles * a.kv_heads * w.head_split < kItems)) ++w.head_split;
+    w.key_chunk = a.short_tiles > 0 ? 0x3fffffff : std::min<int64_t>(w.chunk * finer, 0x3fffffff);  // (whole tiles are not cut)
     w.max_key_chunks = most(a.most_rounds * finer * (group / w.head_split), w.key_chunk, key_bytes * w.head_split);
     take(a.n_tokens * a.heads * 4);  // lse2
     w.delta = take(a.n_tokens * a.heads * 4);
@@ -1049,11 +1049,11 @@ void launch_forward(const AttentionParams& p, hipStream_t stream) {
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
   if (p.plan.short_tiles > 0) {
-    attention_backward_short_kernel<T, NB><<<(uint32_t)p.plan.short_tiles * p.kv_heads, 256, 0, stream>>>(p);
-    return;
+    attention_backward_short_kernel<T, NB><<<(uint32_t)p.plan.short_tiles * p.kv_heads * p.head_split, 256, 0, stream>>>(p);
+  } else {
+    attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
+    attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split * p.max_key_chunks, 256, 0, stream>>>(p);
   }
-  attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
-  attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split * p.max_key_chunks, 256, 0, stream>>>(p);
   const bool add_keys = p.max_key_chunks * p.head_split > 1;
   if (p.max_chunks > 1 || add_keys) {
     const int64_t n_rows = (int64_t)p.plan.tokens * p.heads * p.dim, n_keys = (int64_t)p.plan.tokens * p.kv_heads * p.dim;

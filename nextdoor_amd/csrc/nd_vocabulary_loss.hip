@@ -789,19 +789,35 @@ __global__ __launch_bounds__(S::kThreads, 2) void dweight_kernel(LossParams p, i
   else store_tile_sums<S>(acc, factor, p.dweight_sums + (int64_t)split * classes * p.dim, false, class0, classes, column0, p.dim);
 }
 
-// out = the sum of `split` arrays of n values, n a multiple of 8: sixteen lanes share out the arrays, four values at a time.
-template <class T>
+// out = the sum of `split` arrays of n values, n a multiple of 8, four values a lane.  SHARES lanes share out the arrays: one
+// where there are few (18726 x 256 values, 3 arrays: 27 us with sixteen lanes, most of them idle), sixteen where there are
+// many and the result is small.
+template <class T, int SHARES>
 __global__ __launch_bounds__(256) void add_sums_kernel(const float* sums, T* out, int64_t n, int split) {
-  __shared__ f32x4 partial[16][17];
-  const int at = threadIdx.x & 15, share = threadIdx.x >> 4;
-  const int64_t i = ((int64_t)blockIdx.x * 16 + at) * 4;
+  constexpr int kLanes = 256 / SHARES;
+  __shared__ f32x4 partial[SHARES][kLanes + 1];
+  const int at = threadIdx.x % kLanes, share = threadIdx.x / kLanes;
+  const int64_t i = ((int64_t)blockIdx.x * kLanes + at) * 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (i < n)
-    for (int s = share; s < split; s += 16) v += *(const f32x4*)(sums + s * n + i);
-  partial[share][at] = v;
-  __syncthreads();
-  if (share != 0 || i >= n) return;
-  for (int s = 1; s < min(split, 16); ++s) v += partial[s][at];
+  if (i < n) {
+    const float* from = sums + i;
+    int s = share;
+    for (; s + 3 * SHARES < split; s += 4 * SHARES) {
+      f32x4 four[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) four[j] = *(const f32x4*)(from + (s + j * SHARES) * n);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v += four[j];
+    }
+    for (; s < split; s += SHARES) v += *(const f32x4*)(from + s * n);
+  }
+  if constexpr (SHARES > 1) {
+    partial[share][at] = v;
+    __syncthreads();
+    if (share != 0) return;
+    for (int s = 1; s < min(split, SHARES); ++s) v += partial[s][at];
+  }
+  if (i >= n) return;
   u32x2 o;
   o[0] = pack_pair<T>(v[0], v[1]);
   o[1] = pack_pair<T>(v[2], v[3]);
@@ -913,6 +929,12 @@ void launch_dweight(const LossParams& p, const LossPlan& w, hipStream_t stream) 
   dweight_kernel<T, S><<<(uint32_t)(class_tiles * w.column_tiles * w.dweight_split), S::kThreads, 0, stream>>>(p, class_tiles, (int)w.column_tiles);
 }
 
+template <class T>
+void launch_add_sums(const float* sums, void* out, int64_t n, int64_t split, hipStream_t stream) {
+  if (split <= 16) add_sums_kernel<T, 1><<<(uint32_t)((n / 4 + 255) / 256), 256, 0, stream>>>(sums, (T*)out, n, (int)split);
+  else add_sums_kernel<T, 16><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(sums, (T*)out, n, (int)split);
+}
+
 template <class T, int NB>
 void launch_short(const LossParams& p, const LossPlan& w, hipStream_t stream) {
   const int row_tiles = (p.padded_rows + 127) / 128, class_tiles = (p.classes + 127) / 128;
@@ -925,7 +947,7 @@ template <class T>
 void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
   if (p.rows == 0) {  // no sum at all
     const int64_t n = (int64_t)p.classes * p.dim;
-    add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(nullptr, (T*)p.dweight, n, 0);
+    launch_add_sums<T>(nullptr, p.dweight, n, 0, stream);
     return;
   }
   const uint32_t prepare_blocks = (uint32_t)((w.padded_rows * (p.dim / 8) + 255) / 256);
@@ -938,7 +960,7 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
   auto add_dweight = [&](int64_t class0, int64_t classes) {
     const int64_t n = classes * p.dim;
     if (w.dweight_split > 1)
-      add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dweight_sums, (T*)p.dweight + class0 * p.dim, n, p.dweight_split);
+      launch_add_sums<T>(p.dweight_sums, (T*)p.dweight + class0 * p.dim, n, p.dweight_split, stream);
   };
   if (p.dim <= kShortVector) {
     switch ((p.dim + 31) / 32) {
@@ -963,7 +985,7 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
   }
   if (!w.alone) {
     const int64_t n = (int64_t)p.rows * p.dim;
-    add_sums_kernel<T><<<(uint32_t)((n / 4 + 15) / 16), 256, 0, stream>>>(p.dhidden_sums, (T*)p.dhidden, n, p.dhidden_split);
+    launch_add_sums<T>(p.dhidden_sums, p.dhidden, n, p.dhidden_split, stream);
   }
 }
 

@@ -52,7 +52,7 @@ def run_attention(q, k, v, starts, dout, scale=None, tokens=None):
 
 
 @pytest.mark.parametrize("lengths", sorted(LENGTHS))
-@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (3, 1, 128, F16), (2, 2, 32, BF16)])
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 2, 64, BF16), (3, 1, 128, F16), (2, 2, 32, BF16), (12, 2, 40, F16)])
 def test_attention_over_lengths(lengths, heads, kv_heads, dim, dtype):
     starts = starts_of(LENGTHS[lengths])
     t = int(starts[-1])
@@ -107,10 +107,12 @@ def test_attention_reads_slices_of_a_projection_in_place_and_copies_other_orders
     check_all(run_attention(*split, starts, one.cuda().expand(t, heads, dim)), want, off, "broadcast gradient")
 
 
-def test_attention_leaves_tokens_of_no_sequence_alone():
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([100, 55], 2, 2), ([140, 15], 2, 2), ([100, 55], 8, 1), ([140, 15], 6, 2)])
+def test_attention_leaves_tokens_of_no_sequence_alone(lengths, heads, kv_heads):
     """The rest of a buffer: not read (it holds NaN here), its rows of every result 0."""
-    starts, t = starts_of([100, 55]), 155 + 210
-    q, k, v, dout = (normal(i, t, 2, 64) for i in range(4))
+    starts, t = starts_of(lengths), 155 + 210
+    q, dout = normal(0, t, heads, 64), normal(3, t, heads, 64)
+    k, v = normal(1, t, kv_heads, 64), normal(2, t, kv_heads, 64)
     want, off = ref.attention(q, k, v, starts, 1 / 8, dout)
     gpu = []
     for x in (q, k, v, dout):
