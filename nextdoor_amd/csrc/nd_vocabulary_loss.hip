@@ -42,11 +42,13 @@ struct LossParams {
   float* dhidden_sums; // [split][rows][dim]
   float* dweight_sums; // [split][classes of the piece][dim]
   float* scale;        // what g is held times, and one over it
-  void* hidden_known;  // hidden, filled up to padded_rows; rows without a target are zero
+  void* hidden_known;  // hidden, filled up to padded_rows; rows without a target are zero; twice, if g_rows says so
   // of a row: g = +-exp2(z log2(e) + shift) - [class = target] each; no target: each 0, shift -inf, target -1
   float *row_each, *row_shift;
   int32_t* row_target;
   int32_t padded_rows;
+  // longer vectors: rows that g is kept for.  Few rows: twice padded_rows, g rounded and what the rounding left, for dw
+  int32_t g_rows;
   int32_t class0, class_end;  // the piece
   int32_t dhidden_split, dweight_split;
 };
@@ -55,6 +57,15 @@ struct LossParams {
 // classes): slice s has classes 16 s .. + 15, half h of it (row r, classes 16 s + 4 h .. + 3 and 16 s + 8 + 4 h .. + 3) in
 // 16 bytes.  The rows are permuted so that reads by columns meet different banks.
 __device__ __forceinline__ int gradient_place(int r, int s, int h) { return s * 64 + h * 32 + (r ^ ((h | 2 * s) << 2)); }
+// The gradient of a row is -each at its target and small elsewhere: that one rounding of g would show in every column of dh.
+// So g is formed with `each` rounded to 16 bits, where the target's is exact but for its own weight, and the rows of dh, in 32
+// bits, are multiplied by each / (each rounded); dw takes g in two parts, rounded and rest.  Longer vectors do so where rows are
+// few; over many such roundings are as good as any.
+template <class T>
+__device__ __forceinline__ float row_ratio(float each) {
+  const float rounded = unpack_low<T>(pack_pair<T>(each, 0.f)), ratio = each / rounded;
+  return rounded != 0.f && fabsf(ratio - 1.f) < 0.01f ? ratio : 1.f;
+}
 constexpr int kGradientBlock = 128;  // 16-byte chunks of 32 rows x 32 classes
 constexpr int kGradientBlockBytes = kGradientBlock * 16;
 
@@ -299,7 +310,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, in
         p.partials[((int64_t)class_tile * S::kWavesM + wave / S::kWavesN) * p.rows + row] = make_float2(m2, sum);
     } else {
       const int target = p.row_target[row];
-      const float each = p.row_each[row], shift = p.row_shift[row];
+      const bool in_parts = p.g_rows > p.padded_rows;
+      const float exact = p.row_each[row], ratio = in_parts ? row_ratio<T>(exact) : 1.f, each = exact / ratio;
+      const float shift = p.row_shift[row] - log2f(ratio);
       const uint32_t negative = each < 0.f ? 0x80000000u : 0u;
       const bool targets_here = __builtin_amdgcn_ballot_w64(target >= wave_class0 && target < wave_class0 + 32 * S::kM) != 0;
       const bool negatives = __builtin_amdgcn_ballot_w64(negative) != 0;
@@ -321,9 +334,20 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, in
             if (c >= p.class_end) g[n] = 0.f;
           }
         }
-        const int64_t at = (int64_t)((wave_class0 - p.class0) / 32 + i) * (p.padded_rows / 32) + (row - (lane & 31)) / 32;
+        const int64_t at = (int64_t)((wave_class0 - p.class0) / 32 + i) * (p.g_rows / 32) + (row - (lane & 31)) / 32;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) p.gradient[at * kGradientBlock + gradient_place(lane & 31, s, h)] = pack_operand<T>(g, s);
+        for (int s = 0; s < 2; ++s) {
+          const u32x4 gf = pack_operand<T>(g, s);
+          p.gradient[at * kGradientBlock + gradient_place(lane & 31, s, h)] = gf;
+          if (in_parts) {
+            // (dh has `each` rounded, so has this: what is left over of both, of g with `each` itself)
+            u32x4 rest;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              rest[n] = pack_pair<T>(g[8 * s + 2 * n] * ratio - unpack_low<T>(gf[n]), g[8 * s + 2 * n + 1] * ratio - unpack_high<T>(gf[n]));
+            p.gradient[(at + p.padded_rows / 32) * kGradientBlock + gradient_place(lane & 31, s, h)] = rest;
+          }
+        }
       }
     }
   }
@@ -491,7 +515,7 @@ __global__ __launch_bounds__(1024) void largest_kernel(LossParams p) {
 
 // Before the backward products: hidden, filled up with rows of zeros and with zeros for the rows without a target (such a
 // row sends nothing to dw, whatever it holds: 0 x NaN would be NaN), and what g takes of each row.
-template <bool SCALED>
+template <class T, bool SCALED>
 __global__ __launch_bounds__(256) void prepare_kernel(LossParams p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int chunks = p.dim / 8;
@@ -501,8 +525,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(LossParams p) {
   u32x4 v = {0, 0, 0, 0};
   if (has) v = ((const u32x4*)p.hidden)[i];
   ((u32x4*)p.hidden_known)[i] = v;
+  const float each = has ? p.dloss[row] * (SCALED ? p.scale[0] : kGradientScale) : 0.f;
+  if (p.g_rows > p.padded_rows) ((u32x4*)p.hidden_known)[i + (int64_t)p.padded_rows * chunks] = v;
   if (i % chunks == 0) {
-    const float each = has ? p.dloss[row] * (SCALED ? p.scale[0] : kGradientScale) : 0.f;
     p.row_each[row] = each;
     p.row_shift[row] = has ? log2f(fabsf(each)) - p.lse[row] * kLog2e : -INFINITY;
     p.row_target[row] = has ? target : -1;
@@ -536,7 +561,8 @@ __device__ __forceinline__ void dhidden_short(const LossParams& p, uint32_t bloc
   u32x4 hf[2 * NB];
   load_rows<NB>(hf, (const char*)p.hidden_known + row * row_bytes, work, p.dim, h);
   const int target = work ? p.row_target[row] : -1;
-  const float each = work ? p.row_each[row] : 0.f, shift = work ? p.row_shift[row] : -INFINITY;
+  const float exact = work ? p.row_each[row] : 0.f, ratio = row_ratio<T>(exact), each = exact / ratio;
+  const float shift = work ? p.row_shift[row] - log2f(ratio) : -INFINITY;
   const uint32_t negative = each < 0.f ? 0x80000000u : 0u;
   const bool negatives = __builtin_amdgcn_ballot_w64(negative) != 0;
   f32x16 acc[NB];
@@ -584,7 +610,7 @@ __device__ __forceinline__ void dhidden_short(const LossParams& p, uint32_t bloc
   }
   __syncthreads();
   if (row0 >= p.rows) return;
-  const float factor = p.scale[1];
+  const float factor = p.scale[1] * ratio;
   if (alone)
     store_rows<T, NB>((T*)p.dhidden + (int64_t)row0 * p.dim, p.dim, p.rows - row0, acc, factor, p.dim,
                       &tiles[0][0] + wave * 32 * kChunks);
@@ -593,7 +619,8 @@ __device__ __forceinline__ void dhidden_short(const LossParams& p, uint32_t bloc
 }
 
 // dw: one workgroup has 128 classes, a wave 32 of them (lane's class is a column of Z = H W^T), and goes over its share of the
-// rows, whose shifts are read from LDS.
+// rows, whose shifts are read from LDS.  In rounds in which a target is one of the classes g is multiplied in two parts,
+// rounded and rest (see row_ratio: here a row is no lane's own, and the rows of h have their logits to make).
 template <class T, int NB>
 __device__ __forceinline__ void dweight_short(const LossParams& p, uint32_t block, int class_tiles, ShortTiles<NB>& lds_tiles) {
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
@@ -662,6 +689,15 @@ __device__ __forceinline__ void dweight_short(const LossParams& p, uint32_t bloc
 #pragma unroll
         for (int b = 0; b < NB; ++b)
           acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(tile, 32 * t + 16 * j, 32 * b, lane), gf, acc[b]);
+        if (edge) {
+          u32x4 rest;
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            rest[n] = pack_pair<T>(g[8 * j + 2 * n] - unpack_low<T>(gf[n]), g[8 * j + 2 * n + 1] - unpack_high<T>(gf[n]));
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            acc[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(tile, 32 * t + 16 * j, 32 * b, lane), rest, acc[b]);
+        }
       }
     }
   }
@@ -762,7 +798,17 @@ __global__ __launch_bounds__(S::kThreads, 2) void dhidden_kernel(LossParams p, i
   share_of(classes, S::kDepth, split, p.dhidden_split, begin, end);
   f32x16 acc[S::kM][S::kN];
   multiply<T, S, true>(acc, Columns((const char*)p.weight + (int64_t)p.class0 * p.dim * 2, (int64_t)p.dim * 2, column0, p.dim, classes),
-                       Rows(p.gradient, p.padded_rows, row0), begin, end, tiles);
+                       Rows(p.gradient, p.g_rows, row0), begin, end, tiles);
+  // the lane's rows are columns of the result
+  const int wave = threadIdx.x >> 6, mine = row0 + 32 * (wave % S::kWavesN * S::kN) + (threadIdx.x & 31);
+#pragma unroll
+  for (int j = 0; j < S::kN; ++j) {
+    const float ratio = p.g_rows > p.padded_rows && mine + 32 * j < p.rows ? row_ratio<T>(p.row_each[mine + 32 * j]) : 1.f;
+#pragma unroll
+    for (int i = 0; i < S::kM; ++i)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) acc[i][j][n] *= ratio;
+  }
   const float factor = p.scale[1];
   if (alone) store_result<T, S>(acc, factor, (T*)p.dhidden, row0, p.rows, column0, p.dim, tiles);
   else store_tile_sums<S>(acc, factor, p.dhidden_sums + (int64_t)split * p.rows * p.dim, p.class0 > 0, row0, p.rows, column0, p.dim);
@@ -779,10 +825,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void dweight_kernel(LossParams p, i
   const int class0 = uniform(tile / column_tiles) * S::kTileN, column0 = uniform(tile % column_tiles) * S::kTileM;
   const int classes = p.class_end - p.class0;
   int begin, end;
-  share_of(p.padded_rows, S::kDepth, split, p.dweight_split, begin, end);
+  share_of(p.g_rows, S::kDepth, split, p.dweight_split, begin, end);
   f32x16 acc[S::kM][S::kN];
-  multiply<T, S, false>(acc, Columns(p.hidden_known, (int64_t)p.dim * 2, column0, p.dim, p.padded_rows),
-                        Classes(p.gradient, p.padded_rows, class0), begin, end, tiles);
+  multiply<T, S, false>(acc, Columns(p.hidden_known, (int64_t)p.dim * 2, column0, p.dim, p.g_rows),
+                        Classes(p.gradient, p.g_rows, class0), begin, end, tiles);
   const float factor = p.scale[1];
   if (p.dweight_split == 1)
     store_result<T, S>(acc, factor, (T*)p.dweight + (int64_t)p.class0 * p.dim, class0, classes, column0, p.dim, tiles);
@@ -836,7 +882,7 @@ constexpr int64_t kShortVector = 128;
 
 // How the work is cut; the workspace's parts as offsets.
 struct LossPlan {
-  int64_t padded_rows, piece, column_tiles, logits_split, dhidden_split, dweight_split;
+  int64_t padded_rows, g_rows, piece, column_tiles, logits_split, dhidden_split, dweight_split;
   bool alone;  // the only sum of dh
   int64_t partials, gradient, dhidden_sums, dweight_sums, scale, row_each, row_shift, row_target, hidden_known, bytes;
 };
@@ -859,6 +905,7 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   }
   const int64_t tile_rows = rows <= kFewRows ? 64 : 256;
   w.padded_rows = round_up(std::max<int64_t>(rows, 1), is_short ? kRound : tile_rows);
+  w.g_rows = !is_short && rows <= kFewRows ? 2 * w.padded_rows : w.padded_rows;
   if (is_short) {
     w.dhidden_split = split(2 * kWorkgroups, (w.padded_rows + 127) / 128, (classes + kRound - 1) / kRound, 2);
     w.dweight_split = split(2 * kWorkgroups, (classes + 127) / 128, w.padded_rows / kRound, 4);
@@ -868,18 +915,18 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
     w.column_tiles = (dim + 255) / 256;
     // g of a piece: 256 MiB (4096 rows x 131072 classes x 1024: 4.23 ms with pieces of 128 to 512 MiB, 4.14 with one of 1024,
     // 5.1 of 64), or more if that would leave compute units without a tile of dw
-    const int64_t fit = ((int64_t)256 << 20) / (2 * w.padded_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
+    const int64_t fit = ((int64_t)256 << 20) / (2 * w.g_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
     w.piece = std::min(round_up(classes, kClassPad), round_up(std::max(fit, fill), kClassPad));
     w.dhidden_split = split(kWorkgroups, w.padded_rows / tile_rows * w.column_tiles, w.piece / 64, 4);
-    w.dweight_split = split(kWorkgroups, w.piece / kClassPad * w.column_tiles, w.padded_rows / 64, 4);
+    w.dweight_split = split(kWorkgroups, w.piece / kClassPad * w.column_tiles, w.g_rows / 64, 4);
     w.alone = w.dhidden_split == 1 && w.piece >= classes;
-    w.gradient = take(w.padded_rows * w.piece * 2);
+    w.gradient = take(w.g_rows * w.piece * 2);
   }
   w.scale = take(2 * sizeof(float));
   w.row_each = take(w.padded_rows * 4);
   w.row_shift = take(w.padded_rows * 4);
   w.row_target = take(w.padded_rows * 4);
-  w.hidden_known = take(w.padded_rows * dim * 2);
+  w.hidden_known = take(w.g_rows * dim * 2);
   if (!w.alone) w.dhidden_sums = take(w.dhidden_split * rows * dim * (int64_t)sizeof(float));
   if (w.dweight_split > 1) w.dweight_sums = take(w.dweight_split * std::min(w.piece, classes) * dim * (int64_t)sizeof(float));
   return w;
@@ -953,9 +1000,9 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
   const uint32_t prepare_blocks = (uint32_t)((w.padded_rows * (p.dim / 8) + 255) / 256);
   if (std::is_same<T, _Float16>::value) {
     largest_kernel<<<1, 1024, 0, stream>>>(p);
-    prepare_kernel<true><<<prepare_blocks, 256, 0, stream>>>(p);
+    prepare_kernel<T, true><<<prepare_blocks, 256, 0, stream>>>(p);
   } else {
-    prepare_kernel<false><<<prepare_blocks, 256, 0, stream>>>(p);
+    prepare_kernel<T, false><<<prepare_blocks, 256, 0, stream>>>(p);
   }
   auto add_dweight = [&](int64_t class0, int64_t classes) {
     const int64_t n = classes * p.dim;
@@ -1031,6 +1078,7 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
   p.row_shift = (float*)(work + w.row_shift);
   p.row_target = (int32_t*)(work + w.row_target);
   p.hidden_known = work + w.hidden_known;
+  p.g_rows = (int32_t)w.g_rows;
   p.padded_rows = (int32_t)w.padded_rows;
   p.dhidden_split = (int32_t)w.dhidden_split;
   p.dweight_split = (int32_t)w.dweight_split;
