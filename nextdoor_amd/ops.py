@@ -45,11 +45,6 @@ def _library():
     return _lib
 
 
-def _need(condition, message):
-    if not condition:
-        raise NextDoorError(message)
-
-
 def _on_gpu(what, first, *others):
     """Checks that all are tensors on one GPU; returns its index."""
     try:
@@ -60,7 +55,8 @@ def _on_gpu(what, first, *others):
     except AttributeError:
         index = -1
     if index < 0:
-        _need(all(isinstance(t, torch.Tensor) and t.is_cuda for t in (first, *others)), "%s: tensors on the GPU only" % what)
+        if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (first, *others)):
+            raise NextDoorError("%s: tensors on the GPU only" % what)
         raise NextDoorError("%s: tensors on different devices" % what)
     return index
 
@@ -84,13 +80,17 @@ def _run(index, fn, *args):
 
 def _dropout(x, p, seed, step, residual):
     index = _on_gpu("dropout", x) if residual is None else _on_gpu("dropout", x, residual)
-    _need(x.dtype in _DTYPES, "dropout: no kernel for %s" % x.dtype)
-    _need(0.0 <= p <= 1.0, "dropout: p is a probability, %r given" % (p,))
-    _need(0 <= seed < 1 << 64, "dropout: a seed has 64 bits, %r given" % (seed,))
-    _need(0 <= step < 1 << 31, "dropout: step numbers are below 2^31, %r given" % (step,))
+    if x.dtype not in _DTYPES:
+        raise NextDoorError("dropout: no kernel for %s" % x.dtype)
+    if not 0.0 <= p <= 1.0:
+        raise NextDoorError("dropout: p is a probability, %r given" % (p,))
+    if not 0 <= seed < 1 << 64:
+        raise NextDoorError("dropout: a seed has 64 bits, %r given" % (seed,))
+    if not 0 <= step < 1 << 31:
+        raise NextDoorError("dropout: step numbers are below 2^31, %r given" % (step,))
     if residual is not None:
-        _need(residual.shape == x.shape and residual.dtype == x.dtype,
-              "dropout: the residual is of another shape or type")
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise NextDoorError("dropout: the residual is of another shape or type")
         residual = residual.contiguous()
     x = x.contiguous()
     out = torch.empty_like(x)
@@ -142,37 +142,44 @@ class PackedSequences:
 
     def __init__(self, starts, n_tokens=None, device=None):
         if isinstance(starts, torch.Tensor):
-            _need(not starts.is_floating_point(), "packed sequences: starts are integers")
+            if starts.is_floating_point():
+                raise NextDoorError("packed sequences: starts are integers")
             device = device if device is not None or not starts.is_cuda else starts.device
             starts = starts.cpu().numpy()
         starts = np.asarray(starts)
-        _need(starts.ndim == 1 and len(starts) >= 1 and starts.dtype.kind in "iu",
-              "packed sequences: starts is a list of integers, one more than there are sequences")
-        _need(starts.min() >= 0 and starts.max() <= 2147483392, "packed sequences: starts out of range")
+        if not (starts.ndim == 1 and len(starts) >= 1 and starts.dtype.kind in "iu"):
+            raise NextDoorError("packed sequences: starts is a list of integers, one more than there are sequences")
+        if not (starts.min() >= 0 and starts.max() <= 2147483392):
+            raise NextDoorError("packed sequences: starts out of range")
         starts = np.ascontiguousarray(starts, dtype=np.int32)
         self.device = torch.device("cuda" if device is None else device)
-        _need(self.device.type == "cuda", "packed sequences: on a GPU only")
+        if self.device.type != "cuda":
+            raise NextDoorError("packed sequences: on a GPU only")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.n_sequences, self.n_covered = len(starts) - 1, int(starts[-1])
         self.n_tokens = self.n_covered if n_tokens is None else int(n_tokens)
         lib = _library()
         size = lib.nd_packed_plan_bytes(self.n_tokens)
-        _need(size >= 0, "packed sequences: no plan for %d tokens" % self.n_tokens)
+        if size < 0:
+            raise NextDoorError("packed sequences: no plan for %d tokens" % self.n_tokens)
         on_device = torch.from_numpy(starts).to(self.device)
         self.plan = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
         sizes = (C.c_int64 * 3)()
         _run(self.device.index, lib.nd_packed_plan, starts.ctypes.data, self.n_sequences, self.n_tokens,
              on_device.data_ptr(), self.plan.data_ptr(), sizes)
         self.sizes = tuple(sizes)
+        self.workspace_sizes = {}  # of attention calls over this batch
 
 
 def _heads(what, x, tokens, dim):
     """A [token, head, dim] tensor as the kernels read it - dim side by side, the rest strided by multiples of 16 bytes -
     and its strides.  Anything else is copied."""
     shape = x.shape
-    _need(len(shape) == 3 and shape[0] == tokens, "packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
-    _need(shape[2] == dim, "packed attention: %s has another head size" % what)
+    if not (len(shape) == 3 and shape[0] == tokens):
+        raise NextDoorError("packed attention: %s is not [%d tokens, heads, dim]" % (what, tokens))
+    if shape[2] != dim:
+        raise NextDoorError("packed attention: %s has another head size" % what)
     a, b, c = x.stride()
     if (c != 1 and dim > 1) or a % 8 or b % 8 or a > 16777216 or x.data_ptr() % 16:
         x = x.contiguous()
@@ -186,28 +193,36 @@ def _attention(sequences, q, k, v, scale, dout=None):
     """Checked arguments: (device index, the tensors read, the struct's first fields, shape of lse)."""
     index = _on_gpu("packed attention", q, k, v, sequences.plan)
     dtype = q.dtype
-    _need(dtype is torch.bfloat16 or dtype is torch.float16, "packed attention: 16-bit types only, %s given" % dtype)
-    _need(k.dtype is dtype and v.dtype is dtype, "packed attention: q, k and v are of different types")
+    if not (dtype is torch.bfloat16 or dtype is torch.float16):
+        raise NextDoorError("packed attention: 16-bit types only, %s given" % dtype)
+    if not (k.dtype is dtype and v.dtype is dtype):
+        raise NextDoorError("packed attention: q, k and v are of different types")
     tokens, dim = sequences.n_tokens, q.shape[-1]
     q, q_token, q_head = _heads("q", q, tokens, dim)
     k, k_token, k_head = _heads("k", k, tokens, dim)
     v, v_token, v_head = _heads("v", v, tokens, dim)
-    _need(k.shape == v.shape, "packed attention: k and v are of different shapes")
+    if k.shape != v.shape:
+        raise NextDoorError("packed attention: k and v are of different shapes")
     heads = q.shape[1]
     d_at, d_token, d_head = None, 0, 0
     if dout is not None:
-        _need(dout.shape == q.shape and dout.dtype is dtype, "packed attention: dout is of another shape or type than q")
+        if not (dout.shape == q.shape and dout.dtype is dtype):
+            raise NextDoorError("packed attention: dout is of another shape or type than q")
         dout, d_token, d_head = _heads("dout", dout, tokens, dim)
         d_at = dout.data_ptr()
-    fields = (tokens, sequences.n_covered, *sequences.sizes, heads, k.shape[1], dim, _DTYPES[dtype], 1 / math.sqrt(dim) if scale is None else scale,
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    fields = (tokens, sequences.n_covered, *sequences.sizes, heads, k.shape[1], dim, _DTYPES[dtype], scale,
               sequences.plan.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), d_at,
               q_token, q_head, k_token, k_head, v_token, v_head, d_token, d_head)
     return index, (q, k, v, dout), fields, (heads, tokens)
 
 
-def _workspace(a, backward, device):
+def _workspace(sequences, a, shape, backward, device):
     """The workspace of a call, if it needs one (a call that no kernel can do has none: the call says why)."""
-    size = _library().nd_packed_attention_workspace(a, backward)
+    key = shape, backward
+    size = sequences.workspace_sizes.get(key)
+    if size is None:
+        size = sequences.workspace_sizes[key] = _library().nd_packed_attention_workspace(a, backward)
     if size <= 0:
         return None
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
@@ -226,7 +241,7 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(rows, dtype=torch.float32, device=q.device)
     a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr())
-    workspace = _workspace(a, 0, q.device)
+    workspace = _workspace(sequences, a, (q.shape, k.shape), 0, q.device)
     _run(index, _library().nd_packed_attention_forward, a)
     del keep, workspace
     return out, lse
@@ -236,12 +251,13 @@ def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
     """(dq, dk, dv) for the gradient ``dout`` of ``out``, which with ``lse`` is the forward pass's."""
     _on_gpu("packed attention", q, dout, out, lse)
     index, keep, fields, rows = _attention(sequences, q, k, v, scale, dout)
-    _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and lse.is_contiguous() and
-          lse.dtype is torch.float32 and lse.shape == rows, "packed attention: out and lse are not a forward pass's")
+    if not (out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and lse.is_contiguous() and
+            lse.dtype is torch.float32 and lse.shape == rows):
+        raise NextDoorError("packed attention: out and lse are not a forward pass's")
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
     a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
-    workspace = _workspace(a, 1, q.device)
+    workspace = _workspace(sequences, a, (q.shape, k.shape), 1, q.device)
     _run(index, _library().nd_packed_attention_backward, a)
     del keep, workspace
     return dq, dk, dv
@@ -281,20 +297,25 @@ def _loss(hidden, weight, target, backward):
     """Checked arguments: (device index, the tensors read, the struct's first fields, workspace, its size)."""
     index = _on_gpu("vocabulary loss", hidden, weight, target)
     dtype = hidden.dtype
-    _need(dtype is torch.bfloat16 or dtype is torch.float16, "vocabulary loss: 16-bit types only, %s given" % dtype)
-    _need(weight.dtype is dtype, "vocabulary loss: hidden and weight are of different types")
-    _need(hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1],
-          "vocabulary loss: hidden and weight are not matrices of equally long rows")
+    if not (dtype is torch.bfloat16 or dtype is torch.float16):
+        raise NextDoorError("vocabulary loss: 16-bit types only, %s given" % dtype)
+    if weight.dtype is not dtype:
+        raise NextDoorError("vocabulary loss: hidden and weight are of different types")
+    if not (hidden.dim() == 2 and weight.dim() == 2 and hidden.shape[1] == weight.shape[1]):
+        raise NextDoorError("vocabulary loss: hidden and weight are not matrices of equally long rows")
     hidden, weight = _vectors(hidden), _vectors(weight)
     rows, dim = hidden.shape
     classes = weight.shape[0]
-    _need(target.dim() == 1 and target.shape[0] == rows, "vocabulary loss: one target for each row of hidden")
-    _need(target.dtype in (torch.int32, torch.int64), "vocabulary loss: targets are int32 or int64")
+    if not (target.dim() == 1 and target.shape[0] == rows):
+        raise NextDoorError("vocabulary loss: one target for each row of hidden")
+    if target.dtype not in (torch.int32, torch.int64):
+        raise NextDoorError("vocabulary loss: targets are int32 or int64")
     if target.dtype is torch.int64:  # (what is no class stays none: 2^31 - 1 is above every class)
         target = torch.where((target < 0) | (target > 2147483647), 2147483647, target).to(torch.int32)
     target = target.contiguous()
     size = _library().nd_vocabulary_loss_workspace(rows, classes, dim, backward)
-    _need(size >= 0, "vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (rows, classes, dim))
+    if size < 0:
+        raise NextDoorError("vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (rows, classes, dim))
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hidden.device)
     fields = (rows, classes, dim, _DTYPES[dtype], hidden.data_ptr(), weight.data_ptr(), target.data_ptr())
     return index, (hidden, weight, target), fields, workspace, size
@@ -319,8 +340,8 @@ def vocabulary_loss_backward(dloss, hidden, weight, target, lse):
     _on_gpu("vocabulary loss", hidden, dloss, lse)
     width = hidden.shape[-1]
     index, keep, fields, workspace, size = _loss(hidden, weight, target, 1)
-    _need(tuple(dloss.shape) == fields[:1] and tuple(lse.shape) == fields[:1] and lse.dtype is torch.float32,
-          "vocabulary loss: dloss and lse have one value for each row")
+    if tuple(dloss.shape) != fields[:1] or tuple(lse.shape) != fields[:1] or lse.dtype is not torch.float32:
+        raise NextDoorError("vocabulary loss: dloss and lse have one value for each row")
     dloss, lse = dloss.to(torch.float32).contiguous(), lse.contiguous()
     dhidden, dweight = torch.empty_like(keep[0]), torch.empty_like(keep[1])
     _run(index, _library().nd_vocabulary_loss_backward,
