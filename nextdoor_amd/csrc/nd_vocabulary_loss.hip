@@ -899,7 +899,7 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   };
   const bool is_short = dim <= kShortVector;
   if (!backward) {
-    w.logits_split = is_short ? split(4 * kWorkgroups, (rows + 255) / 256, (classes + kRound - 1) / kRound, 2) : 1;
+    w.logits_split = is_short ? split(4 * kWorkgroups, (rows + 255) / 256, (classes + kRound - 1) / kRound, 1) : 1;
     w.partials = take((is_short ? w.logits_split : round_up(classes, kClassPad) / 64) * rows * (int64_t)sizeof(float2));
     return w;
   }
@@ -907,7 +907,7 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   w.padded_rows = round_up(std::max<int64_t>(rows, 1), is_short ? kRound : tile_rows);
   w.g_rows = !is_short && rows <= kFewRows ? 2 * w.padded_rows : w.padded_rows;
   if (is_short) {
-    w.dhidden_split = split(2 * kWorkgroups, (w.padded_rows + 127) / 128, (classes + kRound - 1) / kRound, 2);
+    w.dhidden_split = split(2 * kWorkgroups, (w.padded_rows + 127) / 128, (classes + kRound - 1) / kRound, 1);
     w.dweight_split = split(2 * kWorkgroups, (classes + 127) / 128, w.padded_rows / kRound, 4);
     w.alone = w.dhidden_split == 1;
     w.piece = classes;
