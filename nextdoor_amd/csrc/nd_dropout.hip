@@ -10,6 +10,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "nd_errors.hpp"
 #include "nd_matrix.hpp"
 #include "nd_philox.hpp"
@@ -39,7 +41,7 @@ struct alignas(sizeof(T) * kDropoutSlots <= 16 ? 16 : 32) DropoutRun {
 // VECTOR: every array is aligned to 16 bytes, whole runs of eight move as vectors.
 template <class T, bool RESIDUAL, bool VECTOR>
 __global__ __launch_bounds__(kDropoutThreads) void dropout_kernel(DropoutParams p) {
-  const int64_t base = ((int64_t)blockIdx.x * kDropoutThreads + threadIdx.x) * kDropoutSlots;
+  const int64_t base = (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kDropoutThreads + threadIdx.x) * kDropoutSlots;
   if (base >= p.n) return;
   const T* x = (const T*)p.x + base;
   const T* r = (const T*)p.residual + base;
@@ -79,7 +81,8 @@ __global__ __launch_bounds__(kDropoutThreads) void dropout_kernel(DropoutParams 
 template <class T>
 hipError_t launch_dropout(const DropoutParams& p, hipStream_t stream) {
   const int64_t lanes = (p.n + kDropoutSlots - 1) / kDropoutSlots;
-  const dim3 grid((uint32_t)((lanes + kDropoutThreads - 1) / kDropoutThreads));
+  const int64_t blocks = (lanes + kDropoutThreads - 1) / kDropoutThreads, most = 1 << 22;  // (a row of a grid has fewer than 2^32 threads)
+  const dim3 grid((uint32_t)std::min(blocks, most), (uint32_t)((blocks + most - 1) / most));
   const bool vector = (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.residual) & 15) == 0;
   if (p.residual) {
     if (vector) dropout_kernel<T, true, true><<<grid, kDropoutThreads, 0, stream>>>(p);
