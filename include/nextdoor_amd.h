@@ -347,7 +347,7 @@ int nd_packed_attention_backward(const nd_packed_attention* a, void* stream);
 /* Softmax cross entropy of `rows` vectors against `classes` class vectors, without the logits:
  * loss_i = log sum_v exp(h_i . w_v) - h_i . w_{target_i}.  A target outside 0 .. classes - 1 (the
  * samplers' INVALID is |V|) has loss 0 and sends nothing back.  hidden, dhidden: [rows][dim], weight,
- * dweight: [classes][dim], dense, aligned to 16 bytes, dim a multiple of 8; lse: [rows], left by
+ * dweight: [classes][dim], dense, aligned to 16 bytes, dim a multiple of 8, fewer than 2^34 elements; lse: [rows], left by
  * the forward call and read by the backward call; dloss: [rows], the gradient of each row's loss.
  * workspace: nd_vocabulary_loss_workspace(...) bytes, aligned to 16, working memory of one call. */
 #define ND_VOCABULARY_MAX_ROWS 4194240

@@ -1102,7 +1102,7 @@ int check_attention(const nd_packed_attention* a, bool backward) {
       return fail("packed attention: strides are multiples of 8 elements, a token's at most " +
                   std::to_string(ND_PACKED_MAX_TOKEN_STRIDE));
   const Cuts cuts = cuts_of(*a, backward);
-  if ((2 * tiles_of(a->n_tokens) + 3) * a->heads * std::max(cuts.max_chunks, cuts.max_key_chunks) > 0x7fffffff)
+  if (std::max(a->short_tiles, tiles_of(a->n_tokens)) * a->heads * std::max(cuts.max_chunks, cuts.max_key_chunks) > 0xffffff)  // (of 256 threads)
     return fail("packed attention: more tokens and heads than one launch holds");
   if (a->workspace_bytes < cuts.bytes)
     return fail("packed attention: the workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(cuts.bytes) +

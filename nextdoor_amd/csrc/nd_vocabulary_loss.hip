@@ -879,10 +879,12 @@ constexpr int64_t kWorkgroups = 256;  // what fills the GPU, one to a compute un
 // Vectors whose g stays in registers.  At 128 and 8192 rows x 56944 classes dh and dw take 495 us so, and 757 us over a g in
 // memory, most of it the 933 MB of g; the third making of the logits costs as much as that saves at 256.
 constexpr int64_t kShortVector = 128;
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // of what is kept for one piece of the work
+constexpr int64_t kMostElements = ((int64_t)1 << 34) - 1024;  // of a matrix: one launch has fewer than 2^32 threads, of four each
 
 // How the work is cut; the workspace's parts as offsets.
 struct LossPlan {
-  int64_t padded_rows, g_rows, piece, column_tiles, logits_split, dhidden_split, dweight_split;
+  int64_t forward_rows, padded_rows, g_rows, piece, column_tiles, logits_split, dhidden_split, dweight_split;
   bool alone;  // the only sum of dh
   int64_t partials, gradient, dhidden_sums, dweight_sums, scale, row_each, row_shift, row_target, hidden_known, bytes;
 };
@@ -900,7 +902,11 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   const bool is_short = dim <= kShortVector;
   if (!backward) {
     w.logits_split = is_short ? split(4 * kWorkgroups, (rows + 255) / 256, (classes + kRound - 1) / kRound, 1) : 1;
-    w.partials = take((is_short ? w.logits_split : round_up(classes, kClassPad) / 64) * rows * (int64_t)sizeof(float2));
+    // Longer vectors leave a pair for each row and 64 classes, a sixteenth of the logits: rows are taken as many at a time as
+    // have 256 MiB of them, at least a tile.
+    const int64_t row_bytes = (is_short ? w.logits_split : round_up(classes, kClassPad) / 64) * (int64_t)sizeof(float2);
+    w.forward_rows = is_short ? rows : std::min(rows, std::max<int64_t>(kPieceBytes / row_bytes / 256, 1) * 256);
+    w.partials = take(w.forward_rows * row_bytes);
     return w;
   }
   const int64_t tile_rows = rows <= kFewRows ? 64 : 256;
@@ -914,9 +920,10 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   } else {
     w.column_tiles = (dim + 255) / 256;
     // g of a piece: 256 MiB (4096 rows x 131072 classes x 1024: 4.23 ms with pieces of 128 to 512 MiB, 4.14 with one of 1024,
-    // 5.1 of 64), or more if that would leave compute units without a tile of dw
-    const int64_t fit = ((int64_t)256 << 20) / (2 * w.g_rows), fill = kWorkgroups / w.column_tiles * kClassPad;
-    w.piece = std::min(round_up(classes, kClassPad), round_up(std::max(fit, fill), kClassPad));
+    // 5.1 of 64), up to four times that where it would leave compute units without a tile of dw, and no less than eight
+    // times the rows' vectors, whose sums each piece reads and writes
+    const int64_t fit = kPieceBytes / (2 * w.g_rows), fill = std::min(kWorkgroups / w.column_tiles * kClassPad, 4 * fit);
+    w.piece = std::min(round_up(classes, kClassPad), round_up(std::max({fit, fill, 8 * dim}), kClassPad));
     w.dhidden_split = split(kWorkgroups, w.padded_rows / tile_rows * w.column_tiles, w.piece / 64, 4);
     w.dweight_split = split(kWorkgroups, w.piece / kClassPad * w.column_tiles, w.g_rows / 64, 4);
     w.alone = w.dhidden_split == 1 && w.piece >= classes;
@@ -955,10 +962,23 @@ int launch_logits_short(const LossParams& p, int splits, hipStream_t stream) {
 }
 
 template <class T>
-void launch_forward(LossParams p, const LossPlan& w, hipStream_t stream) {
+void launch_forward(const LossParams& p, const LossPlan& w, hipStream_t stream) {
   int parts;
-  if (p.dim > kShortVector) parts = launch_logits<T, false>(p, p.rows, p.classes, stream);
-  else if (p.dim > 96) parts = launch_logits_short<T, 4>(p, (int)w.logits_split, stream);
+  if (p.dim > kShortVector) {
+    const int64_t rows = p.rows;
+    for (int64_t at = 0; at < rows; at += w.forward_rows) {
+      LossParams q = p;
+      q.rows = (int32_t)std::min(w.forward_rows, rows - at);
+      q.hidden = (const char*)p.hidden + at * p.dim * 2;
+      q.target += at;
+      q.loss += at;
+      q.lse += at;
+      parts = launch_logits<T, false>(q, q.rows, q.classes, stream);
+      join_kernel<T><<<(q.rows + 7) / 8, 1024, 0, stream>>>(q, parts);
+    }
+    return;
+  }
+  if (p.dim > 96) parts = launch_logits_short<T, 4>(p, (int)w.logits_split, stream);
   else if (p.dim > 64) parts = launch_logits_short<T, 3>(p, (int)w.logits_split, stream);
   else if (p.dim > 32) parts = launch_logits_short<T, 2>(p, (int)w.logits_split, stream);
   else parts = launch_logits_short<T, 1>(p, (int)w.logits_split, stream);
@@ -1047,6 +1067,8 @@ int run_loss(const nd_vocabulary_loss* a, bool backward, void* stream) {
   if (a->dim < 8 || a->dim > ND_VOCABULARY_MAX_DIM || a->dim % 8 != 0)
     return fail("vocabulary loss: the vectors' size is a multiple of 8 up to " + std::to_string(ND_VOCABULARY_MAX_DIM) + ", " +
                 std::to_string(a->dim) + " given");
+  if (a->rows * a->dim > kMostElements || a->classes * a->dim > kMostElements)
+    return fail("vocabulary loss: at most " + std::to_string(kMostElements) + " elements to a matrix");
   if (a->rows == 0 && !backward) return 0;
   const LossPlan w = plan_of(a->rows, a->classes, a->dim, backward);
   if (a->workspace_bytes < w.bytes)

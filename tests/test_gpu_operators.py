@@ -317,6 +317,54 @@ def test_loss_goes_through_several_pieces_of_the_vocabulary():
         assert ((got[name].double() - value).abs() <= off).all(), name
 
 
+def test_loss_of_more_rows_than_are_taken_at_a_time():
+    """A few rows and classes of many, in 64 bits on the GPU.  Forward: rows in pieces of 8192 for so many classes;
+    backward: vectors too long to keep gradients in registers, the classes in two pieces."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    def some(rows, classes, dim):
+        h = torch.randn(rows, dim, device="cuda", generator=gen).to(BF16)
+        w = (torch.randn(classes, dim, device="cuda", generator=gen) * (2 / math.sqrt(dim))).to(BF16)
+        return h, w, targets(rows, rows, classes).cuda()
+
+    def logits(h, w):
+        """and how far they may be off: dim products summed in 32 bits"""
+        z = h.double() @ w.double().T
+        off = (h.shape[1] + 8) * 2.0 ** -24 * (h.double().abs() @ w.double().abs().T).amax(1) + 2.0 ** -21 * z.abs().amax(1)
+        return z, off
+
+    h, w, t = some(8503, 262100, 136)
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    at = torch.tensor([0, 1, 4095, 8190, 8191, 8192, 8193, 8447, 8448, 8502], device="cuda")
+    z, z_off = logits(h[at], w)
+    want = torch.logsumexp(z, 1)
+    assert ((lse[at].double() - want).abs() <= z_off + 2.0 ** -13).all()
+    has = (t[at] >= 0) & (t[at] < len(w))
+    mine = z.gather(1, torch.where(has, t[at], torch.zeros_like(t[at]))[:, None])[:, 0]
+    assert ((loss[at].double() - torch.where(has, want - mine, torch.zeros_like(mine))).abs() <= 2 * z_off + 2.0 ** -13).all()
+
+    h, w, t = some(16700, 40001, 136)
+    dloss = (0.5 + torch.rand(len(h), device="cuda", generator=gen)) / len(h)
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    dhidden, dweight = ops.vocabulary_loss_backward(dloss, h, w, t, lse)
+    each = torch.where((t >= 0) & (t < len(w)), dloss, torch.zeros_like(dloss)).double()
+    for row0 in (0, 8256, 16636):  # all classes
+        rows = slice(row0, row0 + 64)
+        z, z_off = logits(h[rows], w)
+        p = torch.exp(z - torch.logsumexp(z, 1, keepdim=True)) * each[rows, None]
+        g = p - each[rows, None] * (t[rows, None] == torch.arange(len(w), device="cuda"))
+        value = g @ w.double()
+        g_off = (2.0 ** -8 + ref.SMALL) * g.abs() + (2 * z_off[:, None] + ref.SMALL) * p
+        assert ((dhidden[rows].double() - value).abs() <= 2.0 ** -8 * value.abs() + g_off @ w.double().abs()).all()
+    for class0 in (0, 32192, 32256, 39937):  # all rows
+        classes = slice(class0, class0 + 64)
+        z, z_off = logits(h, w[classes])
+        p = torch.exp(z - lse.double()[:, None]) * each[:, None]
+        g = p - each[:, None] * (t[:, None] == torch.arange(class0, class0 + 64, device="cuda"))
+        value = g.T @ h.double()
+        g_off = (2.0 ** -8 + ref.SMALL) * g.abs() + (2 * (z_off[:, None] + 2.0 ** -13) + ref.SMALL) * p
+        assert ((dweight[classes].double() - value).abs() <= 2.0 ** -8 * value.abs() + g_off.T @ h.double().abs()).all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 def test_loss_of_peaked_and_of_tiny_gradients(dtype):
     """Rows whose target has nearly all the weight, logits in the hundreds, and the tiny gradients of a large mean."""
@@ -444,6 +492,21 @@ def test_dropout_uses_the_samplers_stream():
     kept = nd.philox_fill_uniform(seed, step, 0, n, 1, step_size=2)[:, 0] >= np.float32(0.3)
     got = ops.dropout_forward(torch.ones(n, device="cuda"), 0.3, seed, step).cpu().numpy()
     assert np.array_equal(got != 0, kept)
+
+
+def test_dropout_of_more_elements_than_one_row_of_workgroups_has():
+    import nextdoor_amd as nd
+    n, seed, step = 2 ** 33 + 1003, 42, 3
+    x = torch.empty(n, dtype=BF16, device="cuda")
+    places = [0, 2 ** 32 - 500, 2 ** 33 - 500, n - 1000]
+    for at in places:
+        x[at:at + 1000] = 1
+    y = ops.dropout_forward(x, 0.3, seed, step)
+    for at in places:
+        kept = nd.philox_fill_uniform(seed, step, at, 1000, 1, step_size=2)[:, 0] >= np.float32(0.3)
+        assert np.array_equal((y[at:at + 1000] != 0).cpu().numpy(), kept), at
+    del x, y
+    torch.cuda.empty_cache()
 
 
 def test_dropout_drops_whatever_is_there_and_reads_odd_places():

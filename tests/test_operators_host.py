@@ -172,3 +172,17 @@ def test_reference_attention_gradient_is_the_derivative():
             moved = [y + sign * 1e-5 * direction if y is x else y for y in (q, k, v)]
             value.append(float((ref.attention(*map(Double, moved), starts, 0.3)[0]["out"] * d).sum()))
         assert abs((value[0] - value[1]) / 2e-5 - float((got[name] * direction).sum())) < 1e-6
+
+
+def test_calls_that_one_launch_does_not_hold_are_refused():
+    lib = _capi.lib()
+    a = attention_call(n_tokens=1 << 26, n_covered=1 << 26, heads=65535, kv_heads=1, dim=8)
+    assert lib.nd_packed_attention_forward(a, None) != 0
+    assert "one launch" in lib.nd_last_error().decode()
+    base = 1 << 40
+    for rows, classes, dim in ((1 << 20, 100, 65536), (100, 1 << 30, 64)):
+        a = _capi.VocabularyLoss(rows=rows, classes=classes, dim=dim, dtype=2, hidden=base, weight=base, target=base, loss=base, lse=base,
+                                 dloss=base, dhidden=base, dweight=base, workspace=base, workspace_bytes=1 << 60)
+        for fn in (lib.nd_vocabulary_loss_forward, lib.nd_vocabulary_loss_backward):
+            assert fn(a, None) != 0
+            assert "elements to a matrix" in lib.nd_last_error().decode()
