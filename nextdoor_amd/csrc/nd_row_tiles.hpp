@@ -11,7 +11,7 @@ constexpr int kColumns = 64;  // rows of a tile (columns of the product that rea
 // Rows of up to 32 * NB columns.
 template <int NB>
 struct HeadTile {
-  static constexpr int kChunks = NB == 1 ? 4 : NB == 2 ? 8 : 16;  // of a row in LDS
+  static constexpr int kChunks = NB == 1 ? 4 : NB == 2 ? 8 : NB <= 4 ? 16 : 32;  // of a row in LDS
   static constexpr int kSize = kColumns * kChunks;                // of a tile
 };
 

@@ -5,7 +5,7 @@
 // A row whose target is no class (the engine's "no vertex" is |V|) has loss 0 and no gradient.
 //
 // The logits are never kept.  Forward: a workgroup makes a tile of Z^T = W H^T and keeps one maximum and one sum of a row
-// for it; a second kernel joins them.  Backward, vectors of up to 128: dh and dw each make the logits once more and turn them
+// for it; a second kernel joins them.  Backward, vectors of up to 224: dh and dw each make the logits once more and turn them
 // into g in registers, where it is the operand of their second product.  Longer vectors: the logits are made once more for one
 // piece of the vocabulary after another, and g (16 bits, in a workspace of one piece) is multiplied by w and by h.
 #include "../../include/nextdoor_amd.h"
@@ -353,7 +353,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, in
   }
 }
 
-constexpr int kRound = 64;  // rows of the other side in a round of the kernels for short vectors
+constexpr int kRound = 64;  // classes in a round of the kernel for short vectors
 
 // Rounds of a share of n: whole ones, spread evenly.
 __device__ __forceinline__ void rounds_of(int rounds, int i, int n, int& begin, int& end) {
@@ -361,7 +361,7 @@ __device__ __forceinline__ void rounds_of(int rounds, int i, int n, int& begin, 
   end = uniform((int)((int64_t)rounds * (i + 1) / n));
 }
 
-// The same for vectors of up to 128: a workgroup has 256 rows, a wave 64 of them (two columns of Z^T a lane) in registers, and
+// The same for vectors of up to 256: a workgroup has 256 rows, a wave 64 of them (two columns of Z^T a lane) in registers, and
 // goes over its share of the classes with a running maximum and sum.  Each read of the classes serves two products.
 template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void logits_short_kernel(LossParams p, int row_tiles, int splits) {
@@ -535,19 +535,23 @@ __global__ __launch_bounds__(256) void prepare_kernel(LossParams p) {
   if (!SCALED && i == 0) p.scale[1] = 1.f / kGradientScale;
 }
 
-// ---- backward, vectors of up to 128 --------------------------------------------------------------------
+// ---- backward, vectors of up to 224 --------------------------------------------------------------------
 template <int NB>
 struct ShortTiles {
-  u32x4 tiles[2][kRound * HeadTile<NB>::kChunks];
-  float shifts[2][kRound], eaches[2][kRound];
-  int32_t targets[2][kRound];
+  // Rows of the other side in a round.  Vectors above 160 leave registers for one product of 32 x 32 at a time only (192: 792 us
+  // with 34 registers spilled, 712; 8192 rows x 56944 classes).
+  static constexpr int kRound = NB > 5 ? 32 : 64;
+  static constexpr int kSize = 64 * HeadTile<NB>::kChunks;  // (results leave through both halves: 32 rows of each of four waves)
+  u32x4 tiles[2][kSize];
+  float shifts[2][64], eaches[2][64];
+  int32_t targets[2][64];
 };
 
 // dh: one workgroup has 128 rows, a wave 32 of them (lane's row is a column of Z^T = W H^T) in registers, and goes over its
 // share of the classes; G^T is the second operand of dH^T = W^T G^T as it leaves the exponentials.
 template <class T, int NB>
 __device__ __forceinline__ void dhidden_short(const LossParams& p, uint32_t block, int row_tiles, bool alone, ShortTiles<NB>& lds_tiles) {
-  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
+  constexpr int kRound = ShortTiles<NB>::kRound, kChunks = HeadTile<NB>::kChunks, kSize = ShortTiles<NB>::kSize;
   auto& tiles = lds_tiles.tiles;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
   const int split = uniform(block / row_tiles), row0 = uniform(block % row_tiles) * 128 + wave * 32, row = row0 + (lane & 31);
@@ -623,7 +627,7 @@ __device__ __forceinline__ void dhidden_short(const LossParams& p, uint32_t bloc
 // rounded and rest (see row_ratio: here a row is no lane's own, and the rows of h have their logits to make).
 template <class T, int NB>
 __device__ __forceinline__ void dweight_short(const LossParams& p, uint32_t block, int class_tiles, ShortTiles<NB>& lds_tiles) {
-  constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRound * kChunks;
+  constexpr int kRound = ShortTiles<NB>::kRound, kChunks = HeadTile<NB>::kChunks, kSize = ShortTiles<NB>::kSize;
   auto& tiles = lds_tiles.tiles;
   auto& shifts = lds_tiles.shifts;
   auto& eaches = lds_tiles.eaches;
@@ -639,9 +643,9 @@ __device__ __forceinline__ void dweight_short(const LossParams& p, uint32_t bloc
     rows.issue(lds + half * kSize * 16, row_bytes, i * kRound, p.padded_rows);
 #pragma unroll
     for (int j = 0; j < kRound; j += 64) {
-      if (wave == 0) load_words_to_lds((const char*)(p.row_shift + i * kRound + j), lane * 4, lds_address(shifts[half] + j));
-      if (wave == 1) load_words_to_lds((const char*)(p.row_target + i * kRound + j), lane * 4, lds_address(targets[half] + j));
-      if (wave == 2) load_words_to_lds((const char*)(p.row_each + i * kRound + j), lane * 4, lds_address(eaches[half] + j));
+      if (wave == 0) load_words_to_lds((const char*)(p.row_shift + i * kRound + j), min(lane, kRound - 1) * 4, lds_address(shifts[half] + j));
+      if (wave == 1) load_words_to_lds((const char*)(p.row_target + i * kRound + j), min(lane, kRound - 1) * 4, lds_address(targets[half] + j));
+      if (wave == 2) load_words_to_lds((const char*)(p.row_each + i * kRound + j), min(lane, kRound - 1) * 4, lds_address(eaches[half] + j));
     }
   };
   if (begin < end) issue(0, begin);
@@ -876,9 +880,10 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 constexpr int kFewRows = 128;  // up to here tiles of 64 rows of the loss, beyond it tiles of 256
 constexpr int64_t kWorkgroups = 256;  // what fills the GPU, one to a compute unit
-// Vectors whose g stays in registers.  At 128 and 8192 rows x 56944 classes dh and dw take 495 us so, and 757 us over a g in
-// memory, most of it the 933 MB of g; the third making of the logits costs as much as that saves at 256.
-constexpr int64_t kShortVector = 128;
+// Vectors whose g stays in registers, and whose rows do in the forward pass.  8192 rows x 56944 classes, dh and dw in us so and
+// over a g in memory (933 MB): 495 and 757 at 128, 600 and 835 at 160, 712 and 864 at 192, 801 and 968 at 224; at 256 the sums
+// leave too few registers (1576 and 935).  Forward, and by tiles: 185 and 264 at 136, 235 and 324 at 256.
+constexpr int64_t kShortVector = 224, kShortForward = 256;
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // of what is kept for one piece of the work
 constexpr int64_t kMostElements = ((int64_t)1 << 34) - 1024;  // of a matrix: one launch has fewer than 2^32 threads, of four each
 
@@ -899,7 +904,7 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   auto split = [](int64_t workgroups, int64_t tiles, int64_t rounds, int64_t least) {  // at least so many rounds to a share
     return std::max<int64_t>(1, std::min(workgroups / std::max<int64_t>(tiles, 1), rounds / least));
   };
-  const bool is_short = dim <= kShortVector;
+  const bool is_short = dim <= (backward ? kShortVector : kShortForward);
   if (!backward) {
     w.logits_split = is_short ? split(4 * kWorkgroups, (rows + 255) / 256, (classes + kRound - 1) / kRound, 1) : 1;
     // Longer vectors leave a pair for each row and 64 classes, a sixteenth of the logits: rows are taken as many at a time as
@@ -945,12 +950,10 @@ int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_cla
   logits_kernel<T, S, BACKWARD><<<(uint32_t)(row_tiles * class_tiles), S::kThreads, 0, stream>>>(p, (int)row_tiles);
   return (int)class_tiles * S::kWavesM;
 }
-// Shapes (classes x rows): few rows leave the products bound by the reading of the class vectors; short sums (up to 256)
-// do better with two workgroups to a compute unit, one of which may be in its exponentials while the other multiplies.
+// Shapes (classes x rows): few rows leave the products bound by the reading of the class vectors.
 template <class T, bool BACKWARD>
 int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_classes, hipStream_t stream) {
   if (p.rows <= kFewRows) return launch_logits<T, Shape<4, 1, 2, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
-  if (p.dim <= 256) return launch_logits<T, Shape<2, 2, 2, 4, 32>, BACKWARD>(p, covered_rows, covered_classes, stream);
   return launch_logits<T, Shape<2, 4, 4, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
 }
 
@@ -964,7 +967,7 @@ int launch_logits_short(const LossParams& p, int splits, hipStream_t stream) {
 template <class T>
 void launch_forward(const LossParams& p, const LossPlan& w, hipStream_t stream) {
   int parts;
-  if (p.dim > kShortVector) {
+  if (p.dim > kShortForward) {
     const int64_t rows = p.rows;
     for (int64_t at = 0; at < rows; at += w.forward_rows) {
       LossParams q = p;
@@ -978,7 +981,11 @@ void launch_forward(const LossParams& p, const LossPlan& w, hipStream_t stream) 
     }
     return;
   }
-  if (p.dim > 96) parts = launch_logits_short<T, 4>(p, (int)w.logits_split, stream);
+  if (p.dim > 224) parts = launch_logits_short<T, 8>(p, (int)w.logits_split, stream);
+  else if (p.dim > 192) parts = launch_logits_short<T, 7>(p, (int)w.logits_split, stream);
+  else if (p.dim > 160) parts = launch_logits_short<T, 6>(p, (int)w.logits_split, stream);
+  else if (p.dim > 128) parts = launch_logits_short<T, 5>(p, (int)w.logits_split, stream);
+  else if (p.dim > 96) parts = launch_logits_short<T, 4>(p, (int)w.logits_split, stream);
   else if (p.dim > 64) parts = launch_logits_short<T, 3>(p, (int)w.logits_split, stream);
   else if (p.dim > 32) parts = launch_logits_short<T, 2>(p, (int)w.logits_split, stream);
   else parts = launch_logits_short<T, 1>(p, (int)w.logits_split, stream);
@@ -1034,7 +1041,10 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
       case 1: launch_short<T, 1>(p, w, stream); break;
       case 2: launch_short<T, 2>(p, w, stream); break;
       case 3: launch_short<T, 3>(p, w, stream); break;
-      default: launch_short<T, 4>(p, w, stream); break;
+      case 4: launch_short<T, 4>(p, w, stream); break;
+      case 5: launch_short<T, 5>(p, w, stream); break;
+      case 6: launch_short<T, 6>(p, w, stream); break;
+      default: launch_short<T, 7>(p, w, stream); break;
     }
     add_dweight(0, p.classes);
   } else
