@@ -794,7 +794,10 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRows * kChunks;
   __shared__ u32x4 keys[kSize], values[kSize], queries[kSize], douts[kSize];
   __shared__ float lse2s[kRows], deltas[kRows];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), h = lane >> 5;
+  // (what is computed from `lane` is computed anew after each empty asm: addresses kept from one part to the next cost 14 to 47
+  // spilled registers, 66 and 397 us for 60 and 342 at heads of 64 and 128)
+  int lane = threadIdx.x & 63;
+  const int wave = uniform(threadIdx.x >> 6), h = lane >> 5;
   const int units = p.kv_heads * p.head_split, unit = uniform(blockIdx.x % units), tile = uniform(blockIdx.x / units);
   const int kv_head = uniform(unit / p.head_split), share = unit - kv_head * p.head_split, heads = uniform(p.group / p.head_split);
   const int head0 = kv_head * p.group + share * heads;
@@ -847,7 +850,9 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
         float delta = 0.f;
         for (int sweep = 0; sweep < 2; ++sweep) {  // for delta, then for dq
           float sum = 0.f;
-          for (int t = first_tile; t <= wave; ++t) {
+          for (int at = first_tile; at <= wave; ++at) {
+            int t = at;
+            asm volatile("" : "+s"(t));
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int i = 0; i < 2 * NB; ++i) {
@@ -871,8 +876,10 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
                 dq[b] = product_32x32x16<T>(read_operand_by_columns<kChunks, true>(keys, 32 * t + 16 * j, 32 * b, lane), dsf, dq[b]);
             }
           }
+          asm volatile("" : "+v"(lane));
           if (sweep == 0) delta = pair_sum(sum);
         }
+        asm volatile("" : "+v"(lane));
         if (h == 0) {
           deltas[wave * 32 + (lane & 31)] = delta;
           if (there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
@@ -886,7 +893,9 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
           kf[i] = read_operand_by_rows<kChunks>(keys, 32 * wave, i, lane) ^ p.flip;
           vf[i] = read_operand_by_rows<kChunks>(values, 32 * wave, i, lane);
         }
-        for (int t = wave; t <= last_tile; ++t) {
+        for (int at = wave; at <= last_tile; ++at) {
+          int t = at;
+          asm volatile("" : "+s"(t));
           f32x16 s = {}, dp = {};
 #pragma unroll
           for (int i = 0; i < 2 * NB; ++i) {
