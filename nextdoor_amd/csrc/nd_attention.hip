@@ -300,7 +300,7 @@ __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv
 //
 // 16384 tokens, 16 heads of 128 on 2: 1.04 ms, 1.06 PFLOP/s, the matrix cores busy 57 % of the cycles; what is left is the
 // exponentials between a wave's two products, which the other wave of its SIMD fills as far as it can.  1024 walks of up to
-// 101 tokens, 8 heads of 64: 24 us, 57 MB moved (2.4 TB/s): two or three rounds a workgroup, bound by the latency of their loads.
+// 101 tokens, 8 heads of 64: 24 us, 89 MB (3.7 TB/s): two or three rounds a workgroup, bound by the latency of their loads.
 template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionParams p) {
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = HeadTile<NB>::kSize;
@@ -804,7 +804,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
 // dk, dv kernel.  Per head of the group each wave first has 32 queries, as in the dq kernel, then 32 keys, as in the other one;
 // delta always comes from the weights themselves.
 //
-// 1024 walks of up to 101 tokens, 8 heads of 64: 57 us where the two kernels above take 97, 113 MB moved (2.0 TB/s), bound by the
+// 1024 walks of up to 101 tokens, 8 heads of 64: 57 us where the two kernels above take 97, 155 MB (2.7 TB/s), bound by the
 // latency of one load of a tile and three sweeps over it.  8 heads of 128, walks of 20 to 101: 342 us for 370; of 101 throughout,
 // which leave a fifth of each tile empty, 791 for 733.
 template <class T, int NB>
@@ -977,8 +977,8 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   }
 }
 
-// Adds the chunks of cut tiles: dq (`which` 0), dk (1), dv (2); n values each, a lane has four.  Bound by the sums: 119 MB in 36
-// us (3.3 TB/s).
+// Adds the chunks of cut tiles: dq (`which` 0), dk (1), dv (2); n values each, a lane has four.  Bound by the sums, which the
+// last cache holds: 214 MB in 36 us (5.9 TB/s).
 template <class T>
 __global__ __launch_bounds__(256) void attention_add_kernel(AttentionParams p, int64_t n_rows, int64_t n_keys, int key_round) {
   const int which = blockIdx.y;

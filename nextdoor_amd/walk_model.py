@@ -94,7 +94,7 @@ def train(graph, steps=20, walks=1024, seed=42, log=print, **model_args):
         some = order.choice(len(roots), min(walks, len(roots)), replace=False)
         tokens, places, targets, sequences = batch_of(*pack_walks(roots[some], samples[some], graph.n_vertices))
         begin = time.perf_counter()
-        each = model(tokens, places, targets, sequences, seed * 1000003 + step)
+        each = model(tokens, places, targets, sequences, (seed * 1000003 + step) % (1 << 64))
         loss = each.sum() / (targets < graph.n_vertices).sum()
         optimizer.zero_grad()
         loss.backward()
