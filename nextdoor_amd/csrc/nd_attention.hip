@@ -401,12 +401,13 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
       }
       // a row that has seen no key yet: exp2(-inf - 0) = 0 throughout
       const float base = top == -INFINITY ? 0.f : top;
+      float part = 0.f;  // (a round's weights among themselves first: thousands of equal ones added to one sum are rounded alike)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           s[t][i] = exp2_fast(__builtin_fmaf(s[t][i], p.scale_log2, -base));
-          sum += s[t][i];
+          part += s[t][i];
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -417,6 +418,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
                                          acc[b]);
         }
       }
+      sum += part;
     }
     __syncthreads();
   } else if (chunk > 0) {

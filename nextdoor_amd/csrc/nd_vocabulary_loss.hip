@@ -428,11 +428,15 @@ __global__ __launch_bounds__(256, 2) void logits_short_kernel(LossParams p, int 
         sum[j] *= higher == -INFINITY ? 0.f : exp2_fast(top[j] - higher);
         top[j] = higher;
       }
+      // (a round's weights among themselves first: a share may have a hundred thousand classes, and that many equal weights
+      // added to one sum would all be rounded alike)
       const float base = top[j] == -INFINITY ? 0.f : top[j];
+      float part = 0.f;
 #pragma unroll
       for (int t = 0; t < kRound / 32; ++t)
 #pragma unroll
-        for (int n = 0; n < 16; ++n) sum[j] += exp2_fast(__builtin_fmaf(z[j][t][n], kLog2e, -base));
+        for (int n = 0; n < 16; ++n) part += exp2_fast(__builtin_fmaf(z[j][t][n], kLog2e, -base));
+      sum[j] += part;
     }
   }
 #pragma unroll

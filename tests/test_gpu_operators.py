@@ -163,6 +163,47 @@ def test_attention_what_is_not_seen_does_not_matter(lengths, dim, kv_heads, dtyp
             assert ref.close(got[name].cpu()[~these], want[name][~these], off[name][~these]), (name, value)
 
 
+def test_attention_of_tokens_that_lie_far_apart():
+    """Strides of up to 32 MiB a token: the last ones lie 8 GB behind the first, and 128 rows of a tile span 4 GiB."""
+    lengths = [200, 31, 20]
+    starts, tokens = starts_of(lengths), sum(lengths)
+    room = torch.empty(tokens << 24, dtype=BF16, device="cuda")
+    wide = [room.as_strided((tokens, heads, 64), (1 << 24, 64, 1), at) for heads, at in ((4, 0), (2, 4096), (2, 8192), (4, 16384))]
+    for i, x in enumerate(wide):
+        x.copy_(normal(i, *x.shape))
+    for length in (lengths, [120, 111, 20]):
+        starts = starts_of(length)
+        got = run_attention(*wide[:3], starts, wide[3])
+        want = run_attention(*(x.contiguous() for x in wide[:3]), starts, wide[3].contiguous())
+        for name in got:
+            assert torch.equal(got[name], want[name]), name
+    del room, wide
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("length", [96, 160])
+def test_attention_of_more_elements_than_32_bits_count(length):
+    """The last sequences of a batch of 2^32 elements and more give what they give alone."""
+    heads, kv_heads, dim = 64, 2, 128
+    tokens = (2 ** 32 // (heads * dim) // length + 20) * length
+    starts = np.arange(0, tokens + 1, length, dtype=np.int32)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = [torch.zeros(tokens, n, dim, dtype=BF16, device="cuda") for n in (heads, kv_heads, kv_heads, heads)]
+    last = slice(tokens - 10 * length, tokens)
+    for t in x:
+        t[last].normal_(generator=gen)
+        t[:length].normal_(generator=gen)
+    got = run_attention(*x[:3], starts, x[3])
+    assert x[0].numel() > 2 ** 32
+    for part, n in ((last, 10), (slice(0, length), 1)):
+        q, k, v, dout = (t[part].contiguous().cpu() for t in x)
+        want, off = ref.attention(q, k, v, starts[:n + 1], 1 / math.sqrt(dim), dout)
+        for name in got:
+            assert ref.close(got[name][:, part] if name == "lse" else got[name][part], want[name], off[name]), name
+    del x, got
+    torch.cuda.empty_cache()
+
+
 def test_attention_without_any_sequence():
     for starts, t in (([0], 0), ([0], 5), ([0, 0, 0], 5)):
         x = normal(1, t, 2, 32).cuda()
@@ -373,6 +414,38 @@ def test_loss_of_more_rows_than_are_taken_at_a_time():
         value = g.T @ h.double()
         g_off = (2.0 ** -8 + ref.SMALL) * g.abs() + (2 * (z_off[:, None] + 2.0 ** -13) + ref.SMALL) * p
         assert ((dweight[classes].double() - value).abs() <= 2.0 ** -8 * value.abs() + g_off.T @ h.double().abs()).all()
+
+
+@pytest.mark.parametrize("dim", [64, 512])
+def test_loss_of_more_elements_than_32_bits_count(dim):
+    """A vocabulary of over 2^32 elements: three rows' loss, and the gradients of its first and last classes."""
+    rows, classes = 3, 2 ** 32 // dim + 1001
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    h = torch.randn(rows, dim, device="cuda", generator=gen).to(BF16)
+    w = torch.zeros(classes, dim, dtype=BF16, device="cuda")
+    ends = torch.cat([torch.arange(500, device="cuda"), torch.arange(classes - 500, classes, device="cuda")])
+    w[ends] = (torch.randn(1000, dim, device="cuda", generator=gen) * (8 / math.sqrt(dim))).to(BF16)
+    t = torch.tensor([classes - 7, 3, classes], device="cuda")
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    dloss = torch.full((rows,), 1000.0, device="cuda")
+    dhidden, dweight = ops.vocabulary_loss_backward(dloss, h, w, t, lse)
+    # all other logits are 0
+    z = h.double() @ w[ends].double().T
+    z_off = (dim + 8) * 2.0 ** -24 * (h.double().abs() @ w[ends].double().abs().T).amax(1) + 2.0 ** -21 * z.abs().amax(1) + 2.0 ** -21 * 20
+    want = torch.logsumexp(torch.cat([z, torch.full((rows, 1), math.log(classes - 1000), dtype=torch.float64, device="cuda")], 1), 1)
+    assert ((lse.double() - want).abs() <= z_off + 2.0 ** -13).all()
+    target = torch.tensor([[993], [3]], device="cuda")
+    assert ((loss[:2].double() - (want[:2] - z[:2].gather(1, target)[:, 0])).abs() <= 2 * z_off[:2] + 2.0 ** -13).all() and loss[2] == 0
+    p = torch.exp(z - want[:, None]) * 1000
+    p[2] = 0
+    g = p.clone()
+    g[[0, 1], target[:, 0]] -= 1000
+    g_off = (2.0 ** -8 + ref.SMALL) * g.abs() + (2 * (z_off[:, None] + 2.0 ** -13) + ref.SMALL) * p
+    for got, value, off in ((dhidden, g @ w[ends].double(), g_off @ w[ends].double().abs()),
+                            (dweight[ends], g.T @ h.double(), g_off.T @ h.double().abs())):
+        assert ((got.double() - value).abs() <= 2.0 ** -8 * value.abs() + off).all()
+    del w, dweight
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
