@@ -1027,7 +1027,9 @@ PlanParts plan_parts(int64_t tokens) {
 // How the work is cut into chunks, and the parts of the workspace in bytes.  About kItems equal pieces of work fill the GPU
 // (512 workgroups at a time) twice over; a tile with much more than its share of them is cut (one sequence of 8192 tokens and
 // two heads: 128 tiles of up to 128 rounds).
-constexpr int64_t kItems = 1024;
+// Chunks have no fewer than 8 rounds, or than 4 if even so they do not fill it once (both directions in us: 4 heads of 64, 2048
+// tokens, 1088 rounds in all: 79 with 4, 92 with 8; 2 heads, 4096 tokens, 2112 rounds: 109 and 96).
+constexpr int64_t kItems = 1024, kFewRounds = 1536;
 constexpr int64_t kMostChunkBytes = (int64_t)1 << 30;
 struct Cuts {
   int64_t chunk, max_chunks, key_chunk, max_key_chunks, head_split;
@@ -1045,7 +1047,8 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     return at;
   };
   const int64_t row_bytes = a.n_tokens * a.heads * a.dim * 4, key_bytes = a.n_tokens * a.kv_heads * a.dim * 4;
-  w.chunk = std::max<int64_t>(8, (a.rounds * a.heads + kItems - 1) / kItems);
+  const int64_t work = a.rounds * a.heads;
+  w.chunk = std::max<int64_t>(work <= kFewRounds ? 4 : 8, (work + kItems - 1) / kItems);
   w.max_chunks = most(a.most_rounds, w.chunk, row_bytes);
   w.max_key_chunks = w.key_chunk = w.head_split = 1;
   if (backward) {

@@ -16,6 +16,7 @@ Import this module (or torch) before the first call into the library: torch brin
 runtime, and streams and memory can only be shared within one.
 """
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -293,6 +294,11 @@ def _vectors(x):
     return x.clone() if x.data_ptr() % 16 else x
 
 
+@functools.lru_cache(maxsize=256)
+def _loss_workspace(rows, classes, dim, backward):
+    return _library().nd_vocabulary_loss_workspace(rows, classes, dim, backward)
+
+
 def _loss(hidden, weight, target, backward):
     """Checked arguments: (device index, the tensors read, the struct's first fields, workspace, its size)."""
     index = _on_gpu("vocabulary loss", hidden, weight, target)
@@ -313,7 +319,7 @@ def _loss(hidden, weight, target, backward):
     if target.dtype is torch.int64:  # (what is no class stays none: 2^31 - 1 is above every class)
         target = torch.where((target < 0) | (target > 2147483647), 2147483647, target).to(torch.int32)
     target = target.contiguous()
-    size = _library().nd_vocabulary_loss_workspace(rows, classes, dim, backward)
+    size = _loss_workspace(rows, classes, dim, backward)
     if size < 0:
         raise NextDoorError("vocabulary loss: no kernel for %d rows, %d classes, vectors of %d" % (rows, classes, dim))
     workspace = torch.empty(max(size, 16), dtype=torch.uint8, device=hidden.device)
