@@ -76,6 +76,7 @@ struct Shape {
   static constexpr int kWavesM = WAVES_M, kWavesN = WAVES_N, kM = M, kN = N, kDepth = DEPTH;
   static constexpr int kThreads = 64 * WAVES_M * WAVES_N;
   static constexpr int kTileM = 32 * WAVES_M * M, kTileN = 32 * WAVES_N * N;
+  static constexpr int kWavesPerSimd = DEPTH > 64 ? 1 : 2;  // (at least; what LDS has room for)
 };
 
 // ---- operands: ROWS rows, DEPTH places of the sum a round, brought to LDS by THREADS threads --------------
@@ -273,7 +274,7 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[S::kM][S::kN], const A& a
 // ms; a quarter of the classes with g, 268 MB written: 286 us, 0.96 PFLOP/s.  1021 x 100003 x 520: 140 us, 0.76 PFLOP/s: 1564 tiles
 // are 6.1 to a compute unit, and the last 8 of 520 places take a round of 64.
 template <class T, class S, bool BACKWARD>
-__global__ __launch_bounds__(S::kThreads, 2) void logits_kernel(LossParams p, int row_tiles) {
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void logits_kernel(LossParams p, int row_tiles) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const uint32_t block = block_by_die();
   const int class_tile = uniform(block / row_tiles), class0 = p.class0 + class_tile * S::kTileM;
@@ -894,6 +895,10 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 constexpr int kFewRows = 128;  // up to here tiles of 64 rows of the loss, beyond it tiles of 256
 constexpr int64_t kWorkgroups = 256;  // what fills the GPU, one to a compute unit
+// More rows, but tiles of 256 x 256 for less than half of the compute units: smaller ones throughout (both directions in us: 24
+// tiles, 268 rows x 2864 x 784, 118 -> 75; 114 tiles, 266 x 14352 x 696, 122 -> 109; 192 tiles, 2000 x 6000 x 1024, 185 -> 213, so not
+// there).
+bool few_tiles(int64_t rows, int64_t classes) { return rows > kFewRows && ((rows + 255) / 256) * ((classes + 255) / 256) <= kWorkgroups / 2; }
 // Vectors whose g stays in registers, and whose rows do in the forward pass.  8192 rows x 56944 classes, dh and dw in us so and
 // over a g in memory (933 MB): 495 and 757 at 128, 600 and 835 at 160, 712 and 864 at 192, 801 and 968 at 224; at 256 the sums
 // leave too few registers (1576 and 935).  Forward, and by tiles: 185 and 264 at 136, 235 and 324 at 256.
@@ -928,7 +933,8 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
     w.partials = take(w.forward_rows * row_bytes);
     return w;
   }
-  const int64_t tile_rows = rows <= kFewRows ? 64 : 256;
+  const bool small = few_tiles(rows, classes);
+  const int64_t tile_rows = rows <= kFewRows || small ? 64 : 256;
   w.padded_rows = round_up(std::max<int64_t>(rows, 1), is_short ? kRound : tile_rows);
   w.g_rows = !is_short && rows <= kFewRows ? 2 * w.padded_rows : w.padded_rows;
   if (is_short) {
@@ -944,7 +950,7 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
     const int64_t fit = kPieceBytes / (2 * w.g_rows), fill = std::min(kWorkgroups / w.column_tiles * kClassPad, 4 * fit);
     w.piece = std::min(round_up(classes, kClassPad), round_up(std::max({fit, fill, 8 * dim}), kClassPad));
     w.dhidden_split = split(kWorkgroups, w.padded_rows / tile_rows * w.column_tiles, w.piece / 64, 4);
-    w.dweight_split = split(kWorkgroups, w.piece / kClassPad * w.column_tiles, w.g_rows / 64, 4);
+    w.dweight_split = split(kWorkgroups, w.piece / (small ? 64 : kClassPad) * w.column_tiles, w.g_rows / 64, 4);
     w.alone = w.dhidden_split == 1 && w.piece >= classes;
     w.gradient = take(w.g_rows * w.piece * 2);
   }
@@ -964,9 +970,11 @@ int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_cla
   logits_kernel<T, S, BACKWARD><<<(uint32_t)(row_tiles * class_tiles), S::kThreads, 0, stream>>>(p, (int)row_tiles);
   return (int)class_tiles * S::kWavesM;
 }
-// Shapes (classes x rows): few rows leave the products bound by the reading of the class vectors.
+// Shapes (classes x rows): few rows leave the products bound by the reading of the class vectors; few tiles, by the rounds of a
+// lone workgroup, of which these have a quarter of the work and half as many (268 rows x 2864 x 784: 41 -> 27 us forward, 74 -> 48 backward).
 template <class T, bool BACKWARD>
 int launch_logits(const LossParams& p, int64_t covered_rows, int64_t covered_classes, hipStream_t stream) {
+  if (few_tiles(p.rows, p.classes)) return launch_logits<T, Shape<2, 2, 2, 1, 128>, BACKWARD>(p, covered_rows, covered_classes, stream);
   if (p.rows <= kFewRows) return launch_logits<T, Shape<4, 1, 2, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
   return launch_logits<T, Shape<2, 4, 4, 2, 64>, BACKWARD>(p, covered_rows, covered_classes, stream);
 }
@@ -1067,11 +1075,12 @@ void launch_backward(LossParams p, const LossPlan& w, hipStream_t stream) {
     p.class_end = (int32_t)std::min<int64_t>(at + w.piece, p.classes);
     const int64_t classes = p.class_end - p.class0;
     launch_logits<T, true>(p, p.padded_rows, round_up(classes, kClassPad), stream);
-    const bool few = p.rows <= kFewRows;
+    const bool small = few_tiles(p.rows, p.classes), few = p.rows <= kFewRows || small;
     // shapes of the two products: columns of the vectors x rows of the output
     if (few) launch_dhidden<T, Shape<4, 2, 2, 1, 64>>(p, w, stream);
     else launch_dhidden<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
-    launch_dweight<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
+    if (small) launch_dweight<T, Shape<4, 2, 2, 1, 64>>(p, w, stream);
+    else launch_dweight<T, Shape<2, 4, 4, 2, 64>>(p, w, stream);
     add_dweight(at, classes);
   }
   if (!w.alone) {

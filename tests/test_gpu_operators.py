@@ -347,6 +347,16 @@ def test_loss_of_vectors_around_those_that_stay_in_registers(rows, classes, dtyp
     check_all(run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda()), want, off, (rows, classes, dim))
 
 
+@pytest.mark.parametrize("dim", [264, 392, 1000])
+@pytest.mark.parametrize("rows,classes,dtype", [(129, 50, BF16), (500, 3001, F16), (1090, 6399, BF16), (1090, 6401, BF16)])
+def test_loss_of_longer_vectors_in_few_and_in_many_tiles(rows, classes, dtype, dim):
+    h, w = normal(1, rows, dim, dtype=dtype), normal(2, classes, dim, dtype=dtype, std=2 / math.sqrt(dim))
+    t = targets(3, rows, classes)
+    dloss = (0.5 + torch.rand(rows, generator=torch.Generator().manual_seed(4))) / rows
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    check_all(run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda()), want, off, (rows, classes, dim))
+
+
 def test_loss_goes_through_several_pieces_of_the_vocabulary():
     """More rows than one piece's workspace holds for all classes; checked against products in 32 bits on the GPU, which
     agree with 64 bits to SMALL of the sums of magnitudes."""
