@@ -232,6 +232,38 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
                     p.dim, h);
 }
 
+// ---- rows with one key ----------------------------------------------------------------------------------
+// The first token of a sequence has itself as its only key: its weight is 1 and ds = p (dp - delta) = 0 whatever it holds.  Weights
+// made again from lse are 1 +- some 2^-24 |s|, which would leave noise where nothing belongs (and an optimizer that normalises makes
+// full steps of it).  So the backward kernels take its lse as infinite, which makes the weight 0 and with it ds (NaN, where the
+// row is not finite), and put the weight of the pair back to 1 for dv.
+__device__ __forceinline__ float one_key_lse2(float lse) { return INFINITY + (lse - lse); }
+// A result's 32 x 32 weights, rows = queries, where the lane's key is query `at` + 4 h of them and its own query's only key (at = -32: it is not).
+__device__ __forceinline__ void one_key_weight(f32x16& weights, int at) {
+  asm volatile("" : "+v"(at));  // (else the sixteen comparisons are kept over the whole loop: 21 to 82 scalar registers spilled)
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (8 * (i / 4) + i % 4 == at && weights[i] == weights[i]) weights[i] = 1.f;
+}
+// The same at once, where the queries' output gradients are in LDS (in the loop above the comparisons would take registers that are
+// not there: 9 spilled at heads of 64): dv of the lane's key, which is row `r` of them, += that row.
+template <class T, int NB>
+__device__ __forceinline__ void one_key_dv(f32x16 (&dv)[NB], const u32x4* douts, int r, bool one, int h) {
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 v = ((const u32x2*)(douts + tile_place<HeadTile<NB>::kChunks>(r, 4 * b + g)))[h];
+      dv[b][4 * g] += one ? unpack_low<T>(v[0]) : 0.f;
+      dv[b][4 * g + 1] += one ? unpack_high<T>(v[0]) : 0.f;
+      dv[b][4 * g + 2] += one ? unpack_low<T>(v[1]) : 0.f;
+      dv[b][4 * g + 3] += one ? unpack_high<T>(v[1]) : 0.f;
+    }
+}
+// For the same reason: delta = sum p dp, and the weights' own sum, by which the errors that they share go out of it, so that a row's ds add up
+// to 0.  (Logits so large that 32 bits hold no weight have no sum to go by.)
+__device__ __forceinline__ float delta_of(float sum, float weights) { return weights > 0.5f && weights < 2.f ? sum / weights : sum; }
+
 template <class T, int NB>
 __device__ __forceinline__ void dq_carefully(const AttentionParams& p, int head, int kv_head, int row, int first, int begin, int stop,
                                              int row_end, float delta, int chunk, int chunks) {
@@ -248,7 +280,8 @@ __device__ __forceinline__ void dq_carefully(const AttentionParams& p, int head,
     if (__builtin_amdgcn_ballot_w64(sees) == 0) continue;
     const char* k = (const char*)p.k + (int64_t)key * p.k_token + (int64_t)kv_head * p.k_head;
     const float dp = dot_rows<T>(d, (const char*)p.v + (int64_t)key * p.v_token + (int64_t)kv_head * p.v_head, p.dim, h);
-    const float ds = exp2_fast(__builtin_fmaf(dot_rows<T>(q, k, p.dim, h), scale, -lse2)) * (dp - delta);
+    const float ds = first == row ? (dp - dp) + (lse2 - lse2)  // (see one_key_lse2)
+                                  : exp2_fast(__builtin_fmaf(dot_rows<T>(q, k, p.dim, h), scale, -lse2)) * (dp - delta);
     if (sees) add_row<T, NB>(acc, 1.f, ds, k, p.dim, h);
   }
   if (row >= row_end) return;
@@ -266,6 +299,7 @@ __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv
   const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
   const char* k = (const char*)p.k + (int64_t)(there ? key : tile0) * p.k_token + (int64_t)kv_head * p.k_head;
   const char* v = (const char*)p.v + (int64_t)(there ? key : tile0) * p.v_token + (int64_t)kv_head * p.v_head;
+  const bool begins = there && p.plan.first[key] == key;  // (query `key` has this key only: see one_key_lse2)
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {  // dv, dk
     HalfRow<NB> acc = {};
@@ -279,8 +313,13 @@ __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv
         const int64_t at = (int64_t)head * p.plan.tokens + query;
         const char* q = (const char*)p.q + (int64_t)query * p.q_token + (int64_t)head * p.q_head;
         const char* d = (const char*)p.dout + (int64_t)query * p.dout_token + (int64_t)head * p.dout_head;
+        const bool one = begins && query == key;
         float weight = exp2_fast(__builtin_fmaf(dot_rows<T>(k, q, p.dim, h), scale, -p.lse[at] * kLog2e));
-        if (which == 1) weight *= dot_rows<T>(v, d, p.dim, h) - p.delta[at];
+        if (one) weight = 1.f + (p.lse[at] - p.lse[at]);
+        if (which == 1) {
+          const float dp = dot_rows<T>(v, d, p.dim, h);
+          weight *= dp - (one ? dp : p.delta[at]);
+        }
         if (sees) add_row<T, NB>(acc, 1.f, weight, which == 0 ? d : q, p.dim, h);
       }
     }
@@ -543,13 +582,13 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
       delta = pair_sum(delta);
       if (there) {
         const int64_t at = (int64_t)head * p.plan.tokens + row;
-        lse2 = p.lse[at] * kLog2e;
+        const float lse = p.lse[at];
+        lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e;
         if (h == 0 && chunk == 0) {
           p.delta[at] = delta;
           p.lse2[at] = lse2;
         }
       }
-      if (exact) delta = 0.f;
     }
     if (p.flip) {
 #pragma unroll
@@ -559,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
     // one sweep over the keys; DELTA: the first of two, for delta (then the first tile is asked for again at its end)
     auto sweep = [&](auto delta_only) {
       constexpr bool DELTA = decltype(delta_only)::value;
-      float sum = 0.f;
+      float sum = 0.f, weights = 0.f;
       for (int n0 = begin; n0 < stop; n0 += kColumns, half ^= 1) {
         wait_for_loads_and_others();
         const int next = n0 + kColumns < stop ? n0 + kColumns : DELTA ? begin : -1;
@@ -579,19 +618,25 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
             dp = product_32x32x16<T>(read_operand_by_rows<kChunks>(values, 32 * t, i, lane), dof[i], dp);
           }
           if (t == 0 && next >= 0) issue(half ^ 1, next);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
-          if (masked) {
+          if constexpr (DELTA) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = 32 * t + 8 * (i / 4) + i % 4;
-              s[i] = key >= from && key <= to ? s[i] : 0.f;
+              const bool sees = !masked || (key >= from && key <= to);
+              const float weight = sees ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
+              sum += sees ? weight * dp[i] : 0.f;
+              weights += weight;
             }
-          }
-          if constexpr (DELTA) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += s[i];
           } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int key = 32 * t + 8 * (i / 4) + i % 4;
+                s[i] = key >= from && key <= to ? s[i] : 0.f;
+              }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const u32x4 dsf = pack_operand<T>(s, j);
@@ -604,7 +649,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
         }
       }
       if constexpr (DELTA) {
-        delta = pair_sum(sum);
+        delta = delta_of(pair_sum(sum), pair_sum(weights));
         if (h == 0 && there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
       }
     };
@@ -707,6 +752,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     int head = uniform(begin / head_rounds), m0 = tile0 + uniform(begin % head_rounds) * kRound;
     issue(0, head, m0);
     const int last = there ? p.plan.last[key] : key;
+    const int one_at = there && p.plan.first[key] == key ? (lane & 31) - 4 * h : -32;
     // of the wave's keys: the smallest and the largest `last`
     const int last_min = key0 < p.plan.covered ? uniform(last) : 0;
     const int last_max = key0 < p.plan.covered ? uniform(p.plan.last[min(key0 + 31, p.plan.covered - 1)]) : 0;
@@ -760,6 +806,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
               dp[i] = sees ? dp[i] : 0.f;
             }
           }
+          if (m0 + 32 * t == key0) one_key_weight(s, one_at);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const u32x4 pf = pack_operand<T>(s, j), dsf = pack_operand<T>(dp, j);
@@ -846,7 +893,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
       const TileLoader<NB, kRows> q(p.q, p.q_token, p.q_head, head, p.dim), d(p.dout, p.dout_token, p.dout_head, head, p.dim);
       q.issue(lds_address(queries) + part, p.q_token, tile0, tile_end);
       d.issue(lds_address(douts) + part, p.dout_token, tile0, tile_end);
-      const float lse2 = there ? p.lse[(int64_t)head * p.plan.tokens + row] * kLog2e : 0.f;
+      const float lse = there ? p.lse[(int64_t)head * p.plan.tokens + row] : 0.f, lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e;
       if (h == 0) lse2s[wave * 32 + (lane & 31)] = lse2;
       wait_for_loads_and_others();
       if (g == 0 && p.dim < 8 * kChunks) {  // the other operands have a row's first columns past `dim`: 0 here
@@ -869,7 +916,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
         }
         float delta = 0.f;
         for (int sweep = 0; sweep < 2; ++sweep) {  // for delta, then for dq
-          float sum = 0.f;
+          float sum = 0.f, weights = 0.f;
           for (int at = first_tile; at <= wave; ++at) {
             int t = at;
             asm volatile("" : "+s"(t));
@@ -883,8 +930,10 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = 8 * (i / 4) + i % 4;
-              const float ds = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
-              s[i] = key >= from && key <= to ? ds : 0.f;
+              s[i] = key >= from && key <= to ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
+              weights += s[i];
+              dp[i] = key >= from && key <= to ? dp[i] : 0.f;
+              s[i] *= dp[i] - delta;
               sum += s[i];
             }
             if (sweep == 0) continue;
@@ -897,7 +946,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
             }
           }
           asm volatile("" : "+v"(lane));
-          if (sweep == 0) delta = pair_sum(sum);
+          if (sweep == 0) delta = delta_of(pair_sum(sum), pair_sum(weights));
         }
         asm volatile("" : "+v"(lane));
         if (h == 0) {
@@ -945,6 +994,9 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
             }
           }
         }
+        asm volatile("" : "+v"(lane));
+        const bool one = lse2s[32 * wave + (lane & 31)] == INFINITY;
+        if (__builtin_amdgcn_ballot_w64(one) != 0) one_key_dv<T, NB>(dv, douts, 32 * wave + (lane & 31), one, h);
       }
       __syncthreads();
       again = again || __builtin_amdgcn_ballot_w64(!all_finite(dq)) != 0;

@@ -1,0 +1,68 @@
+"""Training operators on the GPU where a definition leaves no room: results that are exactly 0, and gradients so small or so
+large that a 16-bit operand could lose them."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from nextdoor_amd import ops
+from tests import operators_reference as ref
+from tests.test_gpu_operators import BF16, F16, normal, run_attention, starts_of
+
+pytestmark = pytest.mark.gpu
+
+# whole sequences to a tile; longer ones; ones that are cut into chunks
+ONE_KEY = {"ones": [1] * 70, "one": [1], "short": [1, 5, 1, 100, 1, 28, 1], "long": [129, 901, 1, 40, 1], "cut": [1, 1500, 1, 1, 700, 129, 1]}
+
+
+@pytest.mark.parametrize("lengths", sorted(ONE_KEY))
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (4, 1, 128), (6, 2, 40)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("std", [1.0, 10.0])
+def test_attention_rows_with_one_key_send_nothing_to_queries_and_keys(lengths, heads, kv_heads, dim, dtype, std):
+    """Such a row's weight is 1 whatever its logit is: dq = 0, and dk = 0 of a sequence of one token, exactly; dv is the
+    output's gradient."""
+    starts = starts_of(ONE_KEY[lengths])
+    t, first = int(starts[-1]), torch.from_numpy(starts[:-1].astype(np.int64))
+    q, dout = normal(1, t, heads, dim, dtype=dtype, std=std), normal(2, t, heads, dim, dtype=dtype, std=std)
+    k, v = normal(3, t, kv_heads, dim, dtype=dtype, std=std), normal(4, t, kv_heads, dim, dtype=dtype, std=std)
+    got = {n: x.cpu() for n, x in run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda()).items()}
+    assert not got["dq"][first].any()
+    alone = first[torch.from_numpy(np.diff(starts) == 1)]
+    assert not got["dk"][alone].any()
+    # the group's heads added up in 32 bits and rounded once
+    want = dout[alone].double().view(len(alone), kv_heads, -1, dim)
+    off = (ref.UNIT[dtype] + heads * 2.0 ** -23) * want.abs().sum(2) if heads > kv_heads else torch.zeros(1, dtype=torch.float64)
+    assert ref.close(got["dv"][alone], want.sum(2), off.expand(len(alone), kv_heads, dim))
+    assert torch.equal(got["out"][alone], v[alone].repeat_interleave(heads // kv_heads, 1))
+
+
+@pytest.mark.parametrize("lengths", [[40, 3, 70, 2], [100, 28], [200, 56, 130]])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 2)])
+def test_attention_equal_values_send_nothing_to_queries_and_keys(lengths, dtype, heads, kv_heads):
+    """Where all values of a sequence are equal, do . v is too, whatever the weights are: ds is 0 but for the roundings of
+    delta = sum p dp / sum p, sums of n weights in 32 bits.  Logits in the thousands: weights that are made again from a rounded
+    lse have a sum of 1 +- some 1e-4."""
+    starts, dim, scale = starts_of(lengths), 64, 1.0
+    t = int(starts[-1])
+    q, dout = normal(1, t, heads, dim, dtype=dtype, std=10.0), normal(2, t, heads, dim, dtype=dtype)
+    k, v = normal(3, t, kv_heads, dim, dtype=dtype, std=10.0), normal(4, len(lengths), kv_heads, dim, dtype=dtype)
+    v = v.repeat_interleave(torch.tensor(lengths), 0)
+    got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda(), scale)
+    for head in range(heads):
+        kv = head // (heads // kv_heads)
+        dp = (dout[:, head].double().abs() * v[:, kv].double().abs()).sum(1)
+        longest = torch.from_numpy(np.repeat(lengths, lengths)).double()
+        # two sums and a quotient; and do . v of the two kernels, dim products in another order
+        e = dp * (2 * (longest + 4) + 2 * (dim + 8)) * 2.0 ** -24
+        for i in range(len(lengths)):
+            at = slice(int(starts[i]), int(starts[i + 1]))
+            most_k, most_q = k[at, kv].double().abs().amax(0), q[at, head].double().abs().amax(0)
+            n = lengths[i]
+            dq = got["dq"][at, head].cpu().double().abs()
+            assert (dq <= scale * e[at, None] * most_k * 1.01 + ref.LEAST[dtype] * (1 + n * most_k)).all(), (head, i, "dq")
+            if heads == kv_heads:
+                dk = got["dk"][at, kv].cpu().double().abs()
+                assert (dk <= scale * e[at].sum() * most_q * 1.01 + ref.LEAST[dtype] * (1 + n * most_q)).all(), (head, i, "dk")
