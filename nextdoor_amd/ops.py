@@ -182,11 +182,11 @@ def _heads(what, x, tokens, dim):
     if shape[2] != dim:
         raise NextDoorError("packed attention: %s has another head size" % what)
     a, b, c = x.stride()
+    # (of one token or one head the stride is never used, but torch keeps it, also in contiguous() and clone())
+    a, b = a if tokens > 1 else 0, b if shape[1] > 1 else 0
     if (c != 1 and dim > 1) or a % 8 or b % 8 or a > 16777216 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-        a, b, c = x.stride()
+        x = torch.empty(shape, dtype=x.dtype, device=x.device).copy_(x)
+        a, b = x.stride()[:2]
     return x, a, b
 
 

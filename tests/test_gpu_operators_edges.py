@@ -66,3 +66,21 @@ def test_attention_equal_values_send_nothing_to_queries_and_keys(lengths, dtype,
             if heads == kv_heads:
                 dk = got["dk"][at, kv].cpu().double().abs()
                 assert (dk <= scale * e[at].sum() * most_q * 1.01 + ref.LEAST[dtype] * (1 + n * most_q)).all(), (head, i, "dk")
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 2)])
+def test_attention_of_one_token_in_odd_places(heads, kv_heads):
+    """One token whose rows lie at odd pitches and places, which torch calls contiguous: as any other layout."""
+    dim = 64
+    gen = torch.Generator().manual_seed(1)
+
+    def odd(n, seed):
+        wide = torch.randn(3, n * dim + 3, generator=gen.manual_seed(seed)).to(BF16).cuda()
+        return wide[:1, 3:].unflatten(1, (n, dim)), wide[:1, :n * dim].unflatten(1, (n, dim))
+
+    for place in (0, 1):
+        q, k, v, dout = (odd(n, i)[place] for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+        want, off = ref.attention(q.cpu(), k.cpu(), v.cpu(), [0, 1], 1 / 8, dout.cpu())
+        got = run_attention(q, k, v, [0, 1], dout)
+        for name in got:
+            assert ref.close(got[name], want[name], off[name]), name
