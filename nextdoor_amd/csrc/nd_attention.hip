@@ -32,6 +32,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // weights stay below 2^8, which costs 32-bit sums and 16-bit floats nothing, and the sums are rarely scaled again.
 constexpr float kTopSlack = 8.f;
 constexpr int kExactDeltaRounds = 4;
+constexpr int kTopParts = 256;  // workgroups that look for the largest output gradient and value
 
 struct PackedPlan {
   const int32_t* first;  // of the sequence a token belongs to; tokens from `covered` on belong to none
@@ -48,11 +49,12 @@ struct AttentionParams {
   PackedPlan plan;
   const void *q, *k, *v, *out, *dout;
   void *out_w, *dq, *dk, *dv;
-  float *lse, *lse2, *delta;  // [heads][tokens]; lse2: in powers of two, for the backward pass
+  float *lse, *lse2, *delta;  // [heads][tokens]; the backward kernels': lse in powers of two less what p is held times, delta times k
   // what the chunks of a tile whose work is cut leave: [chunk][token][head][dim] of out or dq, [chunk][head][token] of
   // maxima and sums, [chunk][token][kv_head][dim] of dk and dv
   float *row_sums, *dk_sums, *dv_sums;
   float2* row_tops;
+  uint32_t* gradient_tops;  // 16-bit floats, backward: [kTopParts], see attention_top_kernel
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, dout_token, dout_head;  // in bytes
   int32_t heads, kv_heads, group, dim;
   int32_t chunk, max_chunks;          // rounds that a workgroup of the query kernels takes, chunks of a tile at most
@@ -232,6 +234,68 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
                     p.dim, h);
 }
 
+// ---- what 16-bit floats hold ------------------------------------------------------------------------------
+// The backward pass rounds p and ds to 16 bits as operands.  The smallest 16-bit floats are steps of 2^-24, and p of a row of
+// thousands of keys and the ds of a mean's gradient are near that or below, while dq and dk are not (8000 keys, output gradients of 1e-3:
+// dq and dk off by 0.003 without this and by 0.00046 with it, of which 0.0004 are the result's own rounding); above 65504 they would be infinite.  So the kernels hold 2^15 p, and k 2^15 ds with the largest
+// power of two k <= 1 / (2 B), B = dim max |do| max |v| >= |dp|: |k 2^15 ds| <= 2^15.  2^15 goes into the exponent that makes p, k
+// into the subtraction of delta, which is kept times k: not one instruction more.  bfloat16 has the exponents of 32 bits: both are 1.
+template <class T>
+struct Held {
+  static constexpr float kShift = 0.f, kWeight = 1.f;
+};
+template <>
+struct Held<_Float16> {
+  static constexpr float kShift = 15.f, kWeight = 32768.f;
+};
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_of_halves(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// The largest |x| of a part of the tokens, as 16-bit floats: low half of `out`, high half of v.  What is not finite does not count: its rows are
+// taken carefully.  A launch and its latency where there is little to read (8.3 thousand tokens, 6 heads of 80 and 3: 12 MB in 4.6 us).
+__device__ __forceinline__ uint32_t top_of(const char* x, int64_t token_bytes, int64_t head_bytes, uint32_t heads, uint32_t chunks, int64_t begin,
+                                           int64_t end) {
+  const uint32_t n = (uint32_t)(end - begin) * heads * chunks;  // (a launch holds 2^31 rows of up to 16 chunks at most, a part a 256th)
+  uint32_t top = 0;
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < n; i += 1024) {
+    const uint32_t c = i % chunks, row = i / chunks;
+    const u32x4 v = *(const u32x4*)(x + (begin + row / heads) * token_bytes + row % heads * head_bytes + c * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t low = v[j] & 0x7fff, high = v[j] >> 16 & 0x7fff;
+      top = max(top, max(low < 0x7c00 ? low : 0, high < 0x7c00 ? high : 0));
+    }
+  }
+  return top;
+}
+__global__ __launch_bounds__(1024) void attention_top_kernel(AttentionParams p) {
+  __shared__ uint32_t tops[16];
+  const int64_t begin = (int64_t)p.plan.covered * blockIdx.x / kTopParts, end = (int64_t)p.plan.covered * (blockIdx.x + 1) / kTopParts;
+  uint32_t top = top_of((const char*)p.dout, p.dout_token, p.dout_head, p.heads, p.dim / 8, begin, end) |
+                 top_of((const char*)p.v, p.v_token, p.v_head, p.kv_heads, p.dim / 8, begin, end) << 16;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = max_of_halves(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < 16; ++i) top = max_of_halves(top, tops[i]);
+  p.gradient_tops[blockIdx.x] = top;
+}
+// k, by every wave for itself.
+template <class T>
+__device__ __forceinline__ float gradient_scale(const AttentionParams& p) {
+  if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kTopParts; i += 64) top = max_of_halves(top, p.gradient_tops[i + (threadIdx.x & 63)]);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = max_of_halves(top, __shfl_xor(top, d));
+  const float most = unpack_low<_Float16>(top) * unpack_high<_Float16>(top) * (float)p.dim;  // B, between 2^-46 and 2^39, or 0
+  return __uint_as_float((uint32_t)uniform(most > 0.f ? 252 - (__float_as_uint(most) >> 23) : 127) << 23);  // (its exponent e: 2^(-2 - e))
+}
+
 // ---- rows with one key ----------------------------------------------------------------------------------
 // The first token of a sequence has itself as its only key: its weight is 1 and ds = p (dp - delta) = 0 whatever it holds.  Weights
 // made again from lse are 1 +- some 2^-24 |s|, which would leave noise where nothing belongs (and an optimizer that normalises makes
@@ -239,11 +303,12 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
 // row is not finite), and put the weight of the pair back to 1 for dv.
 __device__ __forceinline__ float one_key_lse2(float lse) { return INFINITY + (lse - lse); }
 // A result's 32 x 32 weights, rows = queries, where the lane's key is query `at` + 4 h of them and its own query's only key (at = -32: it is not).
+template <class T>
 __device__ __forceinline__ void one_key_weight(f32x16& weights, int at) {
   asm volatile("" : "+v"(at));  // (else the sixteen comparisons are kept over the whole loop: 21 to 82 scalar registers spilled)
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (8 * (i / 4) + i % 4 == at && weights[i] == weights[i]) weights[i] = 1.f;
+    if (8 * (i / 4) + i % 4 == at && weights[i] == weights[i]) weights[i] = Held<T>::kWeight;
 }
 // The same at once, where the queries' output gradients are in LDS (in the loop above the comparisons would take registers that are
 // not there: 9 spilled at heads of 64): dv of the lane's key, which is row `r` of them, += that row.
@@ -254,15 +319,19 @@ __device__ __forceinline__ void one_key_dv(f32x16 (&dv)[NB], const u32x4* douts,
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const u32x2 v = ((const u32x2*)(douts + tile_place<HeadTile<NB>::kChunks>(r, 4 * b + g)))[h];
-      dv[b][4 * g] += one ? unpack_low<T>(v[0]) : 0.f;
-      dv[b][4 * g + 1] += one ? unpack_high<T>(v[0]) : 0.f;
-      dv[b][4 * g + 2] += one ? unpack_low<T>(v[1]) : 0.f;
-      dv[b][4 * g + 3] += one ? unpack_high<T>(v[1]) : 0.f;
+      dv[b][4 * g] += one ? unpack_low<T>(v[0]) * Held<T>::kWeight : 0.f;
+      dv[b][4 * g + 1] += one ? unpack_high<T>(v[0]) * Held<T>::kWeight : 0.f;
+      dv[b][4 * g + 2] += one ? unpack_low<T>(v[1]) * Held<T>::kWeight : 0.f;
+      dv[b][4 * g + 3] += one ? unpack_high<T>(v[1]) * Held<T>::kWeight : 0.f;
     }
 }
 // For the same reason: delta = sum p dp, and the weights' own sum, by which the errors that they share go out of it, so that a row's ds add up
 // to 0.  (Logits so large that 32 bits hold no weight have no sum to go by.)
-__device__ __forceinline__ float delta_of(float sum, float weights) { return weights > 0.5f && weights < 2.f ? sum / weights : sum; }
+template <class T>
+__device__ __forceinline__ float delta_of(float sum, float weights) {
+  constexpr float kOne = Held<T>::kWeight;
+  return weights > 0.5f * kOne && weights < 2.f * kOne ? sum / weights : sum * (1.f / kOne);
+}
 
 template <class T, int NB>
 __device__ __forceinline__ void dq_carefully(const AttentionParams& p, int head, int kv_head, int row, int first, int begin, int stop,
@@ -293,7 +362,7 @@ __device__ __forceinline__ void dq_carefully(const AttentionParams& p, int head,
 // Rounds begin .. stop - 1 of `round` queries each, as the dk, dv kernel counts them; part: of the sums, or -1.
 template <class T, int NB>
 __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv_head, int head0, int key, int last, int tile0, int end,
-                                                int round, int head_rounds, int begin, int stop, int key_end, int part) {
+                                                int round, int head_rounds, int begin, int stop, int key_end, int part, float k_scale) {
   const int h = (threadIdx.x & 63) >> 5;
   const bool there = last > key;
   const float scale = p.flip ? -p.scale_log2 : p.scale_log2;
@@ -318,7 +387,7 @@ __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv
         if (one) weight = 1.f + (p.lse[at] - p.lse[at]);
         if (which == 1) {
           const float dp = dot_rows<T>(v, d, p.dim, h);
-          weight *= dp - (one ? dp : p.delta[at]);
+          weight *= dp - (one ? dp : p.delta[at] / k_scale);
         }
         if (sees) add_row<T, NB>(acc, 1.f, weight, which == 0 ? d : q, p.dim, h);
       }
@@ -544,7 +613,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
   const bool there = row < p.plan.covered;
   f32x16 acc[NB];
   int chunks = 1, careful_begin = 0, careful_stop = 0;
-  float delta = 0.f;
+  float delta = 0.f, k_scale = 1.f;  // delta: times k_scale
   if (tile0 < p.plan.covered) {
     const int end = min(tile0 + kRows, p.plan.covered), first_key = uniform(p.plan.first[tile0]);
     const int rounds = (end - first_key + kColumns - 1) / kColumns;
@@ -579,11 +648,12 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
           delta = __builtin_fmaf(unpack_low<T>(of[s][j]), unpack_low<T>(dof[s][j]), delta);
           delta = __builtin_fmaf(unpack_high<T>(of[s][j]), unpack_high<T>(dof[s][j]), delta);
         }
-      delta = pair_sum(delta);
+      k_scale = gradient_scale<T>(p);
+      delta = pair_sum(delta) * k_scale;
       if (there) {
         const int64_t at = (int64_t)head * p.plan.tokens + row;
         const float lse = p.lse[at];
-        lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e;
+        lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e - Held<T>::kShift;
         if (h == 0 && chunk == 0) {
           p.delta[at] = delta;
           p.lse2[at] = lse2;
@@ -629,7 +699,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i) s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) * __builtin_fmaf(dp[i], k_scale, -delta);
             if (masked) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
@@ -649,7 +719,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
         }
       }
       if constexpr (DELTA) {
-        delta = delta_of(pair_sum(sum), pair_sum(weights));
+        delta = delta_of<T>(pair_sum(sum), pair_sum(weights)) * k_scale;
         if (h == 0 && there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
       }
     };
@@ -669,17 +739,18 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
   if (row0 < p.plan.tokens && __builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0) {
-    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, p.plan.tokens, delta, chunk,
-                        chunks);
+    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, p.plan.tokens, delta / k_scale,
+                        chunk, chunks);
     return;
   }
+  const float factor = p.scale / (Held<T>::kWeight * k_scale);
   if (chunks > 1) {
     if (row < p.plan.tokens)
-      store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, p.scale, p.dim, h);
+      store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, factor, p.dim, h);
     return;
   }
   if (row0 < p.plan.tokens)
-    store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, p.scale,
+    store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, p.plan.tokens - row0, acc, factor,
                       p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
 }
 
@@ -717,6 +788,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     dv[b] = f32x16{};
   }
   int chunks = 1, careful_begin = 0, careful_stop = 0, careful_rounds = 1, careful_end = 0;
+  float k_scale = 1.f;
   if (tile0 < p.plan.covered) {
     const int end = uniform(p.plan.last[min(tile0 + kRows, p.plan.covered) - 1]);
     const int head0 = kv_head * p.group + share * heads, head_rounds = (end - tile0 + kRound - 1) / kRound, rounds = head_rounds * heads;
@@ -751,6 +823,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     }
     int head = uniform(begin / head_rounds), m0 = tile0 + uniform(begin % head_rounds) * kRound;
     issue(0, head, m0);
+    k_scale = gradient_scale<T>(p);
     const int last = there ? p.plan.last[key] : key;
     const int one_at = there && p.plan.first[key] == key ? (lane & 31) - 4 * h : -32;
     // of the wave's keys: the smallest and the largest `last`
@@ -794,7 +867,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
             for (int n = 0; n < 4; ++n) {
               const int i = 4 * g + n;
               s[i] = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2[n]));
-              dp[i] = s[i] * (dp[i] - delta[n]);
+              dp[i] = s[i] * __builtin_fmaf(dp[i], k_scale, -delta[n]);
             }
           }
           if (masked) {
@@ -806,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
               dp[i] = sees ? dp[i] : 0.f;
             }
           }
-          if (m0 + 32 * t == key0) one_key_weight(s, one_at);
+          if (m0 + 32 * t == key0) one_key_weight<T>(s, one_at);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const u32x4 pf = pack_operand<T>(s, j), dsf = pack_operand<T>(dp, j);
@@ -832,19 +905,20 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
   if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) != 0) {
     dk_dv_carefully<T, NB>(p, kv_head, kv_head * p.group + share * heads, key, there ? p.plan.last[key] : key, tile0, careful_end, kRound,
                            careful_rounds, careful_begin, careful_stop, p.plan.tokens,
-                           chunks * p.head_split == 1 ? -1 : chunk * p.head_split + share);
+                           chunks * p.head_split == 1 ? -1 : chunk * p.head_split + share, k_scale);
     return;
   }
   const int64_t row_elements = (int64_t)p.kv_heads * p.dim;
+  const float dk_factor = p.scale / (Held<T>::kWeight * k_scale), dv_factor = 1.f / Held<T>::kWeight;
   if (chunks * p.head_split == 1) {
     u32x4* part_lds = &tiles[0][0][0] + wave * 32 * kChunks;
     const int64_t at = ((int64_t)key0 * p.kv_heads + kv_head) * p.dim;
-    store_rows<T, NB>((T*)p.dk + at, row_elements, p.plan.tokens - key0, dk, p.scale, p.dim, part_lds);
-    store_rows<T, NB>((T*)p.dv + at, row_elements, p.plan.tokens - key0, dv, 1.f, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dk + at, row_elements, p.plan.tokens - key0, dk, dk_factor, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dv + at, row_elements, p.plan.tokens - key0, dv, dv_factor, p.dim, part_lds);
   } else if (key < p.plan.tokens) {
     const int64_t at = (((int64_t)(chunk * p.head_split + share) * p.plan.tokens + key) * p.kv_heads + kv_head) * p.dim;
-    store_sums<NB>(p.dk_sums + at, dk, p.scale, p.dim, h);
-    store_sums<NB>(p.dv_sums + at, dv, 1.f, p.dim, h);
+    store_sums<NB>(p.dk_sums + at, dk, dk_factor, p.dim, h);
+    store_sums<NB>(p.dv_sums + at, dv, dv_factor, p.dim, h);
   }
 }
 
@@ -875,6 +949,8 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   f32x16 dk[NB], dv[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
+  const float dv_factor = 1.f / Held<T>::kWeight;
+  float k_scale = 1.f, dk_factor = 0.f;
   bool again = false;  // some head's dq is not finite: taken carefully at the end, where no sums are in registers
 
   if (tile0 < p.plan.covered) {
@@ -887,13 +963,15 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
     const TileLoader<NB, kRows> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     k.issue(lds_address(keys) + part, p.k_token, tile0, tile_end);
     v.issue(lds_address(values) + part, p.v_token, tile0, tile_end);
+    k_scale = gradient_scale<T>(p);
+    dk_factor = p.scale / (Held<T>::kWeight * k_scale);  // (of dq too)
     for (int g = 0; g < heads; ++g) {
       const int head = head0 + g;
       if (g > 0) __syncthreads();  // (the last head's dq has left through `queries`)
       const TileLoader<NB, kRows> q(p.q, p.q_token, p.q_head, head, p.dim), d(p.dout, p.dout_token, p.dout_head, head, p.dim);
       q.issue(lds_address(queries) + part, p.q_token, tile0, tile_end);
       d.issue(lds_address(douts) + part, p.dout_token, tile0, tile_end);
-      const float lse = there ? p.lse[(int64_t)head * p.plan.tokens + row] : 0.f, lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e;
+      const float lse = there ? p.lse[(int64_t)head * p.plan.tokens + row] : 0.f, lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e - Held<T>::kShift;
       if (h == 0) lse2s[wave * 32 + (lane & 31)] = lse2;
       wait_for_loads_and_others();
       if (g == 0 && p.dim < 8 * kChunks) {  // the other operands have a row's first columns past `dim`: 0 here
@@ -933,7 +1011,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
               s[i] = key >= from && key <= to ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
               weights += s[i];
               dp[i] = key >= from && key <= to ? dp[i] : 0.f;
-              s[i] *= dp[i] - delta;
+              s[i] *= __builtin_fmaf(dp[i], k_scale, -delta);
               sum += s[i];
             }
             if (sweep == 0) continue;
@@ -946,7 +1024,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
             }
           }
           asm volatile("" : "+v"(lane));
-          if (sweep == 0) delta = delta_of(pair_sum(sum), pair_sum(weights));
+          if (sweep == 0) delta = delta_of<T>(pair_sum(sum), pair_sum(weights));
         }
         asm volatile("" : "+v"(lane));
         if (h == 0) {
@@ -981,7 +1059,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
               const bool sees = query >= from && query < to;
               const float weight = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lses[n]));
               s[i] = sees ? weight : 0.f;
-              dp[i] = sees ? weight * (dp[i] - delta[n]) : 0.f;
+              dp[i] = sees ? weight * __builtin_fmaf(dp[i], k_scale, -delta[n]) : 0.f;
             }
           }
 #pragma unroll
@@ -1001,7 +1079,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
       __syncthreads();
       again = again || __builtin_amdgcn_ballot_w64(!all_finite(dq)) != 0;
       if (work)
-        store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, p.scale, p.dim, part_lds);
+        store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, dk_factor, p.dim, part_lds);
     }
   } else if (row0 < tile_end) {  // tokens of no sequence
     for (int g = 0; g < heads; ++g)
@@ -1011,15 +1089,15 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
   if (row0 >= tile_end) return;
   if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) != 0) {
     dk_dv_carefully<T, NB>(p, kv_head, head0, row, row < tile_end ? p.plan.last[row] : row, tile0, tile_end, kRows, 1, 0, heads, tile_end,
-                           p.head_split == 1 ? -1 : share);
+                           p.head_split == 1 ? -1 : share, k_scale);
   } else if (p.head_split == 1) {
     const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
-    store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, p.scale, p.dim, part_lds);
-    store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, 1.f, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, dk_factor, p.dim, part_lds);
+    store_rows<T, NB>((T*)p.dv + at, k_elements, tile_end - row0, dv, dv_factor, p.dim, part_lds);
   } else if (row < tile_end) {
     const int64_t at = (((int64_t)share * p.plan.tokens + row) * p.kv_heads + kv_head) * p.dim;
-    store_sums<NB>(p.dk_sums + at, dk, p.scale, p.dim, h);
-    store_sums<NB>(p.dv_sums + at, dv, 1.f, p.dim, h);
+    store_sums<NB>(p.dk_sums + at, dk, dk_factor, p.dim, h);
+    store_sums<NB>(p.dv_sums + at, dv, dv_factor, p.dim, h);
   }
   if (!again) return;
 #pragma unroll 1
@@ -1027,7 +1105,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
     const int head = head0 + g;
     const bool there = row < tile_end;
     dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, tile0, tile_end, tile_end,
-                        there ? p.delta[(int64_t)head * p.plan.tokens + row] : 0.f, 0, 1);
+                        there ? p.delta[(int64_t)head * p.plan.tokens + row] / k_scale : 0.f, 0, 1);
   }
 }
 
@@ -1085,7 +1163,7 @@ constexpr int64_t kItems = 1024, kFewRounds = 1536;
 constexpr int64_t kMostChunkBytes = (int64_t)1 << 30;
 struct Cuts {
   int64_t chunk, max_chunks, key_chunk, max_key_chunks, head_split;
-  int64_t delta, row_sums, row_tops, dk_sums, dv_sums, bytes;
+  int64_t delta, row_sums, row_tops, gradient_tops, dk_sums, dv_sums, bytes;
 };
 int64_t key_round_of(int dim) { return dim > 96 ? 32 : 64; }
 Cuts cuts_of(const nd_packed_attention& a, bool backward) {
@@ -1111,6 +1189,7 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     w.max_key_chunks = most(a.most_rounds * finer * (group / w.head_split), w.key_chunk, key_bytes * w.head_split);
     take(a.n_tokens * a.heads * 4);  // lse2
     w.delta = take(a.n_tokens * a.heads * 4);
+    if (a.dtype == ND_F16) w.gradient_tops = take(kTopParts * 4);
   }
   w.chunk = std::min<int64_t>(w.chunk, 0x3fffffff);
   if (w.max_chunks > 1) w.row_sums = take(w.max_chunks * row_bytes);
@@ -1133,6 +1212,7 @@ void launch_forward(const AttentionParams& p, hipStream_t stream) {
 }
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
+  if (std::is_same<T, _Float16>::value) attention_top_kernel<<<kTopParts, 1024, 0, stream>>>(p);
   if (p.plan.short_tiles > 0) {
     attention_backward_short_kernel<T, NB><<<(uint32_t)p.plan.short_tiles * p.kv_heads * p.head_split, 256, 0, stream>>>(p);
   } else {
@@ -1226,6 +1306,7 @@ int run_attention(const nd_packed_attention* a, bool backward, void* stream) {
   p.delta = (float*)(work + w.delta);
   p.row_sums = (float*)(work + w.row_sums);
   p.row_tops = (float2*)(work + w.row_tops);
+  p.gradient_tops = (uint32_t*)(work + w.gradient_tops);
   p.dk_sums = (float*)(work + w.dk_sums);
   p.dv_sums = (float*)(work + w.dv_sums);
   p.chunk = (int32_t)w.chunk;

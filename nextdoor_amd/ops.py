@@ -218,9 +218,9 @@ def _attention(sequences, q, k, v, scale, dout=None):
     return index, (q, k, v, dout), fields, (heads, tokens)
 
 
-def _workspace(sequences, a, shape, backward, device):
+def _workspace(sequences, a, sizes, backward, device):
     """The workspace of a call, if it needs one (a call that no kernel can do has none: the call says why)."""
-    key = shape, backward
+    key = sizes, backward
     size = sequences.workspace_sizes.get(key)
     if size is None:
         size = sequences.workspace_sizes[key] = _library().nd_packed_attention_workspace(a, backward)
@@ -242,7 +242,7 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(rows, dtype=torch.float32, device=q.device)
     a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr())
-    workspace = _workspace(sequences, a, (q.shape, k.shape), 0, q.device)
+    workspace = _workspace(sequences, a, (q.shape, k.shape, q.dtype), 0, q.device)
     _run(index, _library().nd_packed_attention_forward, a)
     del keep, workspace
     return out, lse
@@ -258,7 +258,7 @@ def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
     a = PackedAttention(*fields, out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
-    workspace = _workspace(sequences, a, (q.shape, k.shape), 1, q.device)
+    workspace = _workspace(sequences, a, (q.shape, k.shape, q.dtype), 1, q.device)
     _run(index, _library().nd_packed_attention_backward, a)
     del keep, workspace
     return dq, dk, dv

@@ -84,3 +84,86 @@ def test_attention_of_one_token_in_odd_places(heads, kv_heads):
         got = run_attention(q, k, v, [0, 1], dout)
         for name in got:
             assert ref.close(got[name], want[name], off[name]), name
+
+
+def gradients(q, k, v, starts, scale, dout):
+    """dq, dk, dv in 64 bits, and what the roundings of the backward pass can do to them where 16-bit floats hold 2^15 p and
+    2^15 k ds, k at least 1 / (4 B) with B = dim max |dout| max |v|: half their smallest step is 2^-40 of p and 2^-38 B of
+    ds, however small the gradient is."""
+    unit, step = ref.UNIT[q.dtype], 2.0 ** -24 if q.dtype == F16 else 2.0 ** -126
+    want, off = {n: torch.zeros_like(x).double() for n, x in zip(("dq", "dk", "dv"), (q, k, v))}, {}
+    off = {n: torch.zeros_like(x) for n, x in want.items()}
+    group, dim = q.shape[1] // k.shape[1], q.shape[2]
+    most = dim * float(dout.abs().max()) * float(v.abs().max())
+    for begin, end in zip(starts[:-1].tolist(), starts[1:].tolist()):
+        at, n = slice(begin, end), end - begin
+        later = torch.ones(n, n, dtype=torch.bool).triu(1)
+        for h in range(q.shape[1]):
+            a, b, c, d = (x[at, i].double() for x, i in ((q, h), (k, h // group), (v, h // group), (dout, h)))
+            p = torch.softmax((a @ b.T * scale).masked_fill_(later, -math.inf), 1)
+            dp, out = d @ c.T, p @ c
+            ds = p * (dp - (d * out).sum(1)[:, None])
+            spread = p @ c.abs()
+            delta_off = (d.abs() * (unit * (out.abs() + spread) + ref.SMALL * spread + step * (1 + spread))).sum(1)
+            delta_off += ref.SMALL * (d.abs() @ c.abs().T).amax(1)
+            ds_off = unit * ds.abs() + p * delta_off[:, None] + ref.SMALL * ds.abs() + 2.0 ** -14 * step * most * (p > 0)
+            p_off = (unit + ref.SMALL) * p + 2.0 ** -16 * step * (p > 0)
+            kv = h // group
+            for name, to, value, bound in (("dq", h, ds @ b * scale, ds_off @ b.abs() * scale), ("dk", kv, ds.T @ a * scale, ds_off.T @ a.abs() * scale),
+                                           ("dv", kv, p.T @ d, p_off.T @ d.abs())):
+                want[name][at, to] += value
+                off[name][at, to] += bound
+    for n in want:
+        off[n] += unit * want[n].abs() + step / 2
+    return want, off
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([100, 1, 31, 77] * 8, 4, 2, 64), ([5000], 2, 1, 64), ([300, 900, 40], 3, 3, 128)])
+def test_attention_small_gradients_of_16_bit_floats_are_not_lost(lengths, heads, kv_heads, dim, size):
+    starts = starts_of(lengths)
+    t = int(starts[-1])
+    q, dout = normal(1, t, heads, dim, dtype=F16), normal(2, t, heads, dim, dtype=F16, std=size)
+    k, v = normal(3, t, kv_heads, dim, dtype=F16), normal(4, t, kv_heads, dim, dtype=F16)
+    want, off = gradients(q, k, v, starts, 1 / math.sqrt(dim), dout)
+    got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda())
+    for name in want:
+        assert ref.close(got[name], want[name], off[name]), name
+        # roundings of random sign: of the operand, of delta and of the result, each under 2^-11 of what it rounds; and half a step of
+        # the smallest result
+        error = float((got[name].cpu().double() - want[name]).norm())
+        assert error <= 4 * 2.0 ** -11 * float(want[name].norm()) + 2.0 ** -25 * math.sqrt(want[name].numel()), (name, error)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([100, 1, 31, 77], 4, 2), ([1500, 200], 2, 1)])
+def test_attention_large_gradients_of_16_bit_floats(lengths, heads, kv_heads):
+    """ds far above the largest 16-bit float, dq and dk below it (as the scale is small)."""
+    starts, dim, scale = starts_of(lengths), 64, 2.0 ** -9
+    t = int(starts[-1])
+    q, dout = normal(1, t, heads, dim, dtype=F16), normal(2, t, heads, dim, dtype=F16, std=2000.0)
+    k, v = normal(3, t, kv_heads, dim, dtype=F16), normal(4, t, kv_heads, dim, dtype=F16, std=8.0)
+    want, off = gradients(q, k, v, starts, scale, dout)
+    got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda(), scale)
+    for name in ("dq", "dk"):
+        assert float(want[name].abs().max()) < 65504
+        assert ref.close(got[name], want[name], off[name]), name
+
+
+def test_attention_rows_that_are_not_finite_do_not_decide_what_16_bit_floats_hold():
+    """An infinite output gradient or value in one sequence leaves the small gradients of the others as they are."""
+    heads, kv_heads, dim = 2, 1, 64
+    for lengths in ([90, 60, 100, 40], [90, 600, 2000, 40]):
+        starts = starts_of(lengths)
+        t = int(starts[-1])
+        q, dout = normal(1, t, heads, dim, dtype=F16), normal(2, t, heads, dim, dtype=F16, std=1e-4)
+        k, v = normal(3, t, kv_heads, dim, dtype=F16), normal(4, t, kv_heads, dim, dtype=F16)
+        want, off = gradients(q, k, v, starts, 1 / 8, dout)
+        bad, others = int(starts[1]) + 30, torch.ones(t, dtype=torch.bool)
+        others[starts[1]:starts[2]] = False
+        for value in (math.inf, math.nan):
+            for which in (0, 1):
+                x, y = dout.clone(), v.clone()
+                (x, y)[which][bad] = value
+                got = run_attention(q.cuda(), k.cuda(), y.cuda(), starts, x.cuda())
+                for name in want:
+                    assert ref.close(got[name].cpu()[others], want[name][others], off[name][others]), (lengths, value, which, name)
