@@ -905,6 +905,7 @@ bool few_tiles(int64_t rows, int64_t classes) { return rows > kFewRows && ((rows
 constexpr int64_t kShortVector = 224, kShortForward = 256;
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;  // of what is kept for one piece of the work
 constexpr int64_t kMostElements = ((int64_t)1 << 34) - 1024;  // of a matrix: one launch has fewer than 2^32 threads, of four each
+constexpr int64_t kMostWorkgroups = 0xffffff;                 // of 256 threads, for the same reason
 
 // How the work is cut; the workspace's parts as offsets.
 struct LossPlan {
@@ -1034,9 +1035,16 @@ void launch_add_sums(const float* sums, void* out, int64_t n, int64_t split, hip
 template <class T, int NB>
 void launch_short(const LossParams& p, const LossPlan& w, hipStream_t stream) {
   const int row_tiles = (p.padded_rows + 127) / 128, class_tiles = (p.classes + 127) / 128;
-  const int dhidden_blocks = (int)(row_tiles * w.dhidden_split);
-  gradients_short_kernel<T, NB><<<(uint32_t)(dhidden_blocks + class_tiles * w.dweight_split), 256, 0, stream>>>(
-      p, dhidden_blocks, row_tiles, w.alone, class_tiles);
+  const int64_t dhidden_blocks = row_tiles * w.dhidden_split, dweight_blocks = class_tiles * w.dweight_split;
+  auto launch = [&](int64_t blocks, int64_t of_dhidden) {
+    gradients_short_kernel<T, NB><<<(uint32_t)blocks, 256, 0, stream>>>(p, (int)of_dhidden, row_tiles, w.alone, class_tiles);
+  };
+  if (dhidden_blocks + dweight_blocks <= kMostWorkgroups) {
+    launch(dhidden_blocks + dweight_blocks, dhidden_blocks);
+  } else {  // (over two billion classes)
+    launch(dhidden_blocks, dhidden_blocks);
+    launch(dweight_blocks, 0);
+  }
 }
 
 template <class T>

@@ -167,3 +167,33 @@ def test_attention_rows_that_are_not_finite_do_not_decide_what_16_bit_floats_hol
                 got = run_attention(q.cuda(), k.cuda(), y.cuda(), starts, x.cuda())
                 for name in want:
                     assert ref.close(got[name].cpu()[others], want[name][others], off[name][others]), (lengths, value, which, name)
+
+
+def test_loss_of_the_most_classes():
+    """The largest vocabulary that is accepted: three rows' loss, and the gradients of its first and last classes."""
+    rows, classes, dim = 3, 2147483392, 8
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    h = torch.randn(rows, dim, device="cuda", generator=gen).to(BF16)
+    w = torch.zeros(classes, dim, dtype=BF16, device="cuda")
+    ends = torch.cat([torch.arange(500, device="cuda"), torch.arange(classes - 500, classes, device="cuda")])
+    w[ends] = (torch.randn(1000, dim, device="cuda", generator=gen) * 4).to(BF16)
+    t = torch.tensor([classes - 7, 3, classes], device="cuda")
+    loss, lse = ops.vocabulary_loss_forward(h, w, t)
+    dhidden, dweight = ops.vocabulary_loss_backward(torch.full((rows,), 1e6, device="cuda"), h, w, t, lse)
+    # all other logits are 0
+    z = h.double() @ w[ends].double().T
+    z_off = (dim + 8) * 2.0 ** -24 * (h.double().abs() @ w[ends].double().abs().T).amax(1) + 2.0 ** -21 * z.abs().amax(1) + 2.0 ** -21 * 22
+    want = torch.logsumexp(torch.cat([z, torch.full((rows, 1), math.log(classes - 1000), dtype=torch.float64, device="cuda")], 1), 1)
+    assert ((lse.double() - want).abs() <= z_off + 2.0 ** -13).all()
+    target = torch.tensor([[993], [3]], device="cuda")
+    assert ((loss[:2].double() - (want[:2] - z[:2].gather(1, target)[:, 0])).abs() <= 2 * z_off[:2] + 2.0 ** -13).all() and loss[2] == 0
+    p = torch.exp(z - want[:, None]) * 1e6
+    p[2] = 0
+    g = p.clone()
+    g[[0, 1], target[:, 0]] -= 1e6
+    g_off = (2.0 ** -8 + ref.SMALL) * g.abs() + (2 * (z_off[:, None] + 2.0 ** -13) + ref.SMALL) * p
+    for got, value, off in ((dhidden, g @ w[ends].double(), g_off @ w[ends].double().abs()),
+                            (dweight[ends], g.T @ h.double(), g_off.T @ h.double().abs())):
+        assert ((got.double() - value).abs() <= 2.0 ** -8 * value.abs() + off).all()
+    del w, dweight
+    torch.cuda.empty_cache()
