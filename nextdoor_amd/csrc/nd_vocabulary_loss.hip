@@ -946,10 +946,13 @@ LossPlan plan_of(int64_t rows, int64_t classes, int64_t dim, bool backward) {
   } else {
     w.column_tiles = (dim + 255) / 256;
     // g of a piece: 256 MiB (4096 rows x 131072 classes x 1024: 4.23 ms with pieces of 128 to 512 MiB, 4.14 with one of 1024,
-    // 5.1 of 64), up to four times that where it would leave compute units without a tile of dw, and no less than eight
-    // times the rows' vectors, whose sums each piece reads and writes
+    // 5.1 of 64), up to four times that where it would leave compute units without a tile of dw.  Each piece reads and writes the
+    // sums of dh, 8 bytes for 6 operations a class: 300 / classes of its time.  So no fewer classes than eight times the vectors,
+    // or than 4 GiB hold; and no fewer than 1024, which are more than that for over two million rows (131072 rows x 40000 x 4096: 118 ms
+    // with 4 GiB, 121 with 8; 2097152 x 10000 x 264: 81 ms with 4, 74 with 9; 4194240 rows of it: 163 with 8, 150 with 18)
     const int64_t fit = kPieceBytes / (2 * w.g_rows), fill = std::min(kWorkgroups / w.column_tiles * kClassPad, 4 * fit);
-    w.piece = std::min(round_up(classes, kClassPad), round_up(std::max({fit, fill, 8 * dim}), kClassPad));
+    const int64_t sums = std::min(8 * dim, std::max<int64_t>(16 * fit, 1024));
+    w.piece = std::min(round_up(classes, kClassPad), round_up(std::max({fit, fill, sums}), kClassPad));
     w.dhidden_split = split(kWorkgroups, w.padded_rows / tile_rows * w.column_tiles, w.piece / 64, 4);
     w.dweight_split = split(kWorkgroups, w.piece / (small ? 64 : kClassPad) * w.column_tiles, w.g_rows / 64, 4);
     w.alone = w.dhidden_split == 1 && w.piece >= classes;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from nextdoor_amd import ops
+from nextdoor_amd import _capi, ops
 
 BF16 = torch.bfloat16
 
@@ -35,3 +35,18 @@ def test_slices_that_can_be_read_in_place_are_not_copied():
     qkv = filled(5, 6, 64)
     for x in qkv.split([4, 1, 1], 1):
         assert ops._heads("q", x, 5, 64)[0] is x
+
+
+@pytest.mark.parametrize("rows,classes,dim", [
+    (4096, 131072, 1024), (16700, 40001, 232), (65536, 131072, 4096), (131072, 131072, 4096), (32768, 131072, 8192), (262144, 50000, 65536),
+    (1 << 20, 20000, 300), (1 << 21, 20000, 8192), (4194240, 3000, 4096), (4194240, 131072, 264)])
+def test_the_loss_keeps_a_few_gib_of_gradients_however_many_rows_there_are(rows, classes, dim):
+    """What the backward call asks for beyond the rows themselves in 16 bits (once) and the sums of their gradients: g of one piece of the
+    classes, up to 4 GiB, or 1024 classes where that is more, filled up to a multiple of 256."""
+    dim = -(-dim // 8) * 8
+    size = _capi.lib().nd_vocabulary_loss_workspace(rows, classes, dim, 1)
+    padded = -(-rows // 256) * 256
+    g = max(4 << 30, 2 * padded * 1024) + 2 * padded * 256
+    # (rows that do not fill the GPU leave several sums of dh, and dw's of one piece)
+    shares = max(1, 256 // (padded // 256 * -(-dim // 256)))
+    assert 0 < size <= g + padded * dim * 2 + shares * rows * dim * 4 + 12 * padded + 4096, (size - g) / 2 ** 30
