@@ -27,6 +27,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // What g is held times: in 16-bit floats such that max |dloss| becomes this (below their largest); bfloat16 has the exponents of
 // 32 bits, and a constant keeps the smallest weights of a mean over millions of rows among the normal numbers.
 constexpr float kGradientOne = 32768.f, kGradientScale = 4294967296.f;
+constexpr float kLeastLargest = 0x1p-100f;  // max |dloss| that this is done for: one over it is still finite, and less is 0 in 16 bits
 constexpr int kClassPad = 256;           // a piece of the vocabulary is filled up to a multiple of it
 
 struct LossParams {
@@ -521,9 +522,9 @@ __global__ __launch_bounds__(1024) void largest_kernel(LossParams p) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
-    const bool scaled = m > 0.f && m < INFINITY;
-    p.scale[0] = scaled ? kGradientOne / m : 1.f;
-    p.scale[1] = scaled ? m / kGradientOne : 1.f;
+    m = m < INFINITY ? fmaxf(m, kLeastLargest) : kGradientOne;  // (also where there is none)
+    p.scale[0] = kGradientOne / m;
+    p.scale[1] = m / kGradientOne;
   }
 }
 

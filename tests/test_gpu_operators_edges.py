@@ -8,7 +8,7 @@ import torch
 
 from nextdoor_amd import ops
 from tests import operators_reference as ref
-from tests.test_gpu_operators import BF16, F16, normal, run_attention, starts_of
+from tests.test_gpu_operators import BF16, F16, normal, run_attention, run_loss, starts_of, targets
 
 pytestmark = pytest.mark.gpu
 
@@ -197,3 +197,11 @@ def test_loss_of_the_most_classes():
         assert ((got.double() - value).abs() <= 2.0 ** -8 * value.abs() + off).all()
     del w, dweight
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,classes,dim", [(60, 500, 64), (60, 500, 264), (300, 500, 264)])
+@pytest.mark.parametrize("size", [1e-36, 1e-41])
+def test_loss_gradients_far_below_16_bit_floats_are_zero(rows, classes, dim, size):
+    h, w = normal(1, rows, dim, dtype=F16), normal(2, classes, dim, dtype=F16, std=2 / math.sqrt(dim))
+    got = run_loss(h.cuda(), w.cuda(), targets(3, rows, classes).cuda(), torch.full((rows,), size, device="cuda"))
+    assert not got["dhidden"].any() and not got["dweight"].any()
