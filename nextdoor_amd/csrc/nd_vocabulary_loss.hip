@@ -509,20 +509,20 @@ __global__ __launch_bounds__(1024) void join_kernel(LossParams p, int parts) {
   }
 }
 
-// g in 16-bit floats is held relative to max |dloss|, so that they hold the gradient of a mean over any number of rows.  One
-// workgroup, no atomics: 4 bytes a row are little next to the products that follow.
+// g in 16-bit floats is held relative to max |dloss|, so that they hold the gradient of a mean over any number of rows.  What is
+// not finite does not count: the other rows' dh are as they would be without it.  One workgroup, no atomics: 4 bytes a row are little next to the products that follow.
 __global__ __launch_bounds__(1024) void largest_kernel(LossParams p) {
   __shared__ float tops[16];
   float m = 0.f;
   for (int i = threadIdx.x; i < p.rows; i += 1024)
-    if (p.target[i] >= 0 && p.target[i] < p.classes) m = fmaxf(m, fabsf(p.dloss[i]));
+    if (p.target[i] >= 0 && p.target[i] < p.classes && fabsf(p.dloss[i]) < INFINITY) m = fmaxf(m, fabsf(p.dloss[i]));
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 16; ++i) m = fmaxf(m, tops[i]);
-    m = m < INFINITY ? fmaxf(m, kLeastLargest) : kGradientOne;  // (also where there is none)
+    m = fmaxf(m, kLeastLargest);  // (also where there is none)
     p.scale[0] = kGradientOne / m;
     p.scale[1] = m / kGradientOne;
   }

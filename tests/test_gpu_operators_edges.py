@@ -205,3 +205,18 @@ def test_loss_gradients_far_below_16_bit_floats_are_zero(rows, classes, dim, siz
     h, w = normal(1, rows, dim, dtype=F16), normal(2, classes, dim, dtype=F16, std=2 / math.sqrt(dim))
     got = run_loss(h.cuda(), w.cuda(), targets(3, rows, classes).cuda(), torch.full((rows,), size, device="cuda"))
     assert not got["dhidden"].any() and not got["dweight"].any()
+
+
+@pytest.mark.parametrize("rows,classes,dim", [(60, 500, 64), (60, 500, 264), (300, 500, 264)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_loss_one_row_that_is_not_finite_leaves_the_others_gradients(rows, classes, dim, value, dtype):
+    h, w = normal(1, rows, dim, dtype=dtype), normal(2, classes, dim, dtype=dtype, std=2 / math.sqrt(dim))
+    t = torch.arange(rows) % classes
+    dloss = torch.full((rows,), 1e-4)
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    dloss[7] = value
+    got = run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda())
+    others = torch.arange(rows) != 7
+    assert ref.close(got["dhidden"].cpu()[others], want["dhidden"][others], off["dhidden"][others])
+    assert not torch.isfinite(got["dhidden"][7]).any() and not torch.isfinite(got["dweight"]).all()
