@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kPlanThreads) void packed_plan_kernel(const int32_t
   // the last sequence that starts at or before t (empty ones start where the next does)
   int32_t lo = 0, hi = sequences;
   while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) >> 1;
+    const int32_t mid = lo + (hi - lo) / 2;  // (there may be more than 2^30 of them, most of them empty)
     if (starts[mid] <= t) lo = mid;
     else hi = mid;
   }

@@ -220,3 +220,17 @@ def test_loss_one_row_that_is_not_finite_leaves_the_others_gradients(rows, class
     others = torch.arange(rows) != 7
     assert ref.close(got["dhidden"].cpu()[others], want["dhidden"][others], off["dhidden"][others])
     assert not torch.isfinite(got["dhidden"][7]).any() and not torch.isfinite(got["dweight"]).all()
+
+
+def test_plan_of_more_sequences_than_half_of_32_bits_count():
+    """Over 2^30 sequences, all but the last ones empty: a batch is what its tokens are."""
+    lengths = [3, 0, 40, 1, 0, 2]
+    starts = np.zeros(2 ** 30 + 6, np.int32)
+    starts[-6:] = np.cumsum(lengths)
+    t = int(starts[-1])
+    q, k, v = (normal(i, t, 2, 64).cuda() for i in range(3))
+    got = ops.packed_attention_forward(q, k, v, ops.PackedSequences(starts))
+    want = ops.packed_attention_forward(q, k, v, ops.PackedSequences(starts_of(lengths)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del starts, got
+    torch.cuda.empty_cache()
