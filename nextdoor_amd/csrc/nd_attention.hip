@@ -230,8 +230,7 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
     return;
   }
   if (h == 0) p.lse[at] = (top + log2f(sum)) * kLn2;
-  store_half<T, NB>((T*)p.out_w + ((int64_t)row * p.heads + head) * p.dim, nullptr, acc, sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum,
-                    p.dim, h);
+  store_half<T, NB>((T*)p.out_w + ((int64_t)row * p.heads + head) * p.dim, nullptr, acc, there ? 1.f / sum : 0.f, p.dim, h);
 }
 
 // ---- what 16-bit floats hold ------------------------------------------------------------------------------
@@ -550,7 +549,7 @@ __global__ __launch_bounds__(256, 2) void attention_forward_kernel(AttentionPara
     store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, 1.f, p.dim, h);
     return;
   }
-  const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // (NaN stays NaN)
+  const float inverse = there ? 1.f / sum : 0.f;  // (a row of nothing but logits of -inf: 0 / 0, NaN as the formulas say)
   if (h == 0 && row < tile_end) p.lse[(int64_t)head * p.plan.tokens + row] = (top + log2f(sum)) * kLn2;
   store_rows<T, NB>((T*)p.out_w + ((int64_t)row0 * p.heads + head) * p.dim, (int64_t)p.heads * p.dim, tile_end - row0, acc, inverse,
                     p.dim, &tiles[0][0][0] + wave * 32 * kChunks);
@@ -582,7 +581,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionParams p, 
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = weight == 0.f ? v[j] : __builtin_fmaf(part[j], weight, v[j]);
   }
-  const float inverse = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const float inverse = row < p.plan.covered ? 1.f / sum : 0.f;
   u32x2 o;
   o[0] = pack_pair<T>(v[0] * inverse, v[1] * inverse);
   o[1] = pack_pair<T>(v[2] * inverse, v[3] * inverse);

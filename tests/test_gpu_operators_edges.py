@@ -234,3 +234,21 @@ def test_plan_of_more_sequences_than_half_of_32_bits_count():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     del starts, got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("lengths", [[5, 1, 30], [70, 200, 9], [40, 1500, 3]])
+@pytest.mark.parametrize("dim", [64, 40])
+def test_attention_rows_of_logits_that_are_all_minus_infinity_are_not_a_number(lengths, dim):
+    """exp(s - lse) is NaN there; lse is -inf, and the rows of other sequences are as ever."""
+    starts, heads = starts_of(lengths), 2
+    t = int(starts[-1])
+    q, k, v, dout = (normal(i, t, heads, dim) for i in range(4))
+    hit = torch.zeros(t, dtype=torch.bool)
+    hit[starts[1]:starts[2]] = True
+    want, off = ref.attention(q, k, v, starts, 1 / math.sqrt(dim), dout)
+    q[hit], k[hit] = 1e25, -1e25
+    got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda())
+    assert torch.isinf(got["lse"].cpu()[:, hit]).all() and (got["lse"].cpu()[:, hit] < 0).all()
+    for name in ("out", "dq", "dk", "dv"):
+        assert torch.isnan(got[name].cpu()[hit]).all(), name
+        assert ref.close(got[name].cpu()[~hit], want[name][~hit], off[name][~hit]), name
