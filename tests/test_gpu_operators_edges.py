@@ -252,3 +252,40 @@ def test_attention_rows_of_logits_that_are_all_minus_infinity_are_not_a_number(l
     for name in ("out", "dq", "dk", "dv"):
         assert torch.isnan(got[name].cpu()[hit]).all(), name
         assert ref.close(got[name].cpu()[~hit], want[name][~hit], off[name][~hit]), name
+
+
+@pytest.mark.parametrize("rows,classes,dim,dtype", [(20000, 40001, 232, BF16), (20000, 40001, 232, F16), (20011, 30011, 520, F16), (20000, 25000, 776, BF16)])
+def test_loss_of_longer_vectors_goes_through_several_pieces_of_the_vocabulary(rows, classes, dim, dtype):
+    """More rows than one piece's workspace holds for all classes: every value of both gradients, in 64 bits on the GPU."""
+    h, w = normal(1, rows, dim, dtype=dtype).cuda(), normal(2, classes, dim, dtype=dtype, std=2 / math.sqrt(dim)).cuda()
+    t = targets(3, rows, classes).cuda()
+    dloss = ((0.5 + torch.rand(rows, generator=torch.Generator().manual_seed(4))) / rows).cuda()
+    one = ops._loss_workspace(rows, classes, dim, 1) - ops._loss_workspace(rows, 256, dim, 1)
+    assert one < 2 * rows * classes  # (g of all classes is not kept)
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    got = run_loss(h, w, t, dloss)
+    for name in want:
+        assert ref.close(got[name], want[name].cpu(), off[name].cpu()), name
+    del want, off
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows,classes,dim", [(50, 100, 32), (300, 500, 64), (60, 500, 264), (300, 500, 264), (300, 9000, 264)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("known", [0.0, 0.7])
+def test_loss_rows_without_a_target_send_nothing_to_the_classes(rows, classes, dim, dtype, known):
+    """Whatever they and their dloss hold, among rows that have one."""
+    h, w = normal(1, rows, dim, dtype=dtype), normal(2, classes, dim, dtype=dtype, std=2 / math.sqrt(dim))
+    rng = np.random.default_rng(1)
+    none = torch.from_numpy(rng.random(rows) >= known)
+    t = torch.where(none, classes, torch.from_numpy(rng.integers(0, classes, rows)))
+    dloss = torch.full((rows,), 1 / rows)
+    want, off = ref.vocabulary_loss(h, w, t, dloss)
+    at = none.nonzero()[:, 0]
+    h[at[::2]], h[at[1::2]], dloss[at] = math.nan, math.inf, math.inf
+    got = run_loss(h.cuda(), w.cuda(), t.cuda(), dloss.cuda())
+    for name in ("loss", "dhidden", "dweight"):
+        assert ref.close(got[name], want[name], off[name]), name
+    assert not got["dhidden"].cpu()[none].any() and not got["loss"].cpu()[none].any()
+    if known == 0.0:
+        assert not got["dweight"].any()
