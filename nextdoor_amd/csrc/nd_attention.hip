@@ -1007,13 +1007,20 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = 8 * (i / 4) + i % 4;
-              s[i] = key >= from && key <= to ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
-              weights += s[i];
-              dp[i] = key >= from && key <= to ? dp[i] : 0.f;
-              s[i] *= __builtin_fmaf(dp[i], k_scale, -delta);
-              sum += s[i];
+              const bool sees = key >= from && key <= to;
+              s[i] = sees ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
+              dp[i] = sees ? __builtin_fmaf(dp[i], k_scale, -delta) : 0.f;
             }
-            if (sweep == 0) continue;
+            if (sweep == 0) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                weights += s[i];
+                sum = __builtin_fmaf(s[i], dp[i], sum);
+              }
+              continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= dp[i];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const u32x4 dsf = pack_operand<T>(s, j);
