@@ -198,7 +198,7 @@ def _attention(sequences, q, k, v, scale, dout=None):
         raise NextDoorError("packed attention: 16-bit types only, %s given" % dtype)
     if not (k.dtype is dtype and v.dtype is dtype):
         raise NextDoorError("packed attention: q, k and v are of different types")
-    tokens, dim = sequences.n_tokens, q.shape[-1]
+    tokens, dim = sequences.n_tokens, q.shape[-1] if q.dim() else 0
     q, q_token, q_head = _heads("q", q, tokens, dim)
     k, k_token, k_head = _heads("k", k, tokens, dim)
     v, v_token, v_head = _heads("v", v, tokens, dim)
@@ -211,7 +211,7 @@ def _attention(sequences, q, k, v, scale, dout=None):
             raise NextDoorError("packed attention: dout is of another shape or type than q")
         dout, d_token, d_head = _heads("dout", dout, tokens, dim)
         d_at = dout.data_ptr()
-    scale = 1 / math.sqrt(dim) if scale is None else scale
+    scale = 1 / math.sqrt(max(dim, 1)) if scale is None else scale
     fields = (tokens, sequences.n_covered, *sequences.sizes, heads, k.shape[1], dim, _DTYPES[dtype], scale,
               sequences.plan.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), d_at,
               q_token, q_head, k_token, k_head, v_token, v_head, d_token, d_head)
@@ -344,8 +344,8 @@ def vocabulary_loss_backward(dloss, hidden, weight, target, lse):
     """(dhidden, dweight) for the gradient ``dloss`` of each row's loss; lse is the forward pass's.  Rows without a
     target send nothing back, whatever their ``dloss``."""
     _on_gpu("vocabulary loss", hidden, dloss, lse)
-    width = hidden.shape[-1]
     index, keep, fields, workspace, size = _loss(hidden, weight, target, 1)
+    width = hidden.shape[1]
     if tuple(dloss.shape) != fields[:1] or tuple(lse.shape) != fields[:1] or lse.dtype is not torch.float32:
         raise NextDoorError("vocabulary loss: dloss and lse have one value for each row")
     dloss, lse = dloss.to(torch.float32).contiguous(), lse.contiguous()

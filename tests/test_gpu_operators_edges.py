@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from nextdoor_amd import ops
+from nextdoor_amd import NextDoorError, ops
 from tests import operators_reference as ref
 from tests.test_gpu_operators import BF16, F16, normal, run_attention, run_loss, starts_of, targets
 
@@ -289,3 +289,16 @@ def test_loss_rows_without_a_target_send_nothing_to_the_classes(rows, classes, d
     assert not got["dhidden"].cpu()[none].any() and not got["loss"].cpu()[none].any()
     if known == 0.0:
         assert not got["dweight"].any()
+
+
+def test_tensors_of_other_shapes_are_refused_as_the_rest_is():
+    x, seq = normal(1, 10, 4, 64).cuda(), ops.PackedSequences([0, 10])
+    out, lse = ops.packed_attention_forward(x, x, x, seq)
+    one, none = x[0, 0, 0], x[..., :0]
+    h, t = x[:, 0].contiguous(), torch.zeros(10, dtype=torch.int64, device="cuda")
+    for fn, args in ((ops.packed_attention_forward, (one, one, one, seq)), (ops.packed_attention_forward, (none, none, none, seq)),
+                     (ops.packed_attention_backward, (one, one, one, one, out, lse, seq)),
+                     (ops.vocabulary_loss_forward, (one, one, t)), (ops.vocabulary_loss_backward, (lse[0], one, one, t, lse[0])),
+                     (ops.vocabulary_loss_forward, (h[:, :0], h[:, :0], t)), (ops.vocabulary_loss_backward, (lse[0], h, h, t, one.float()))):
+        with pytest.raises(NextDoorError):
+            fn(*args)
