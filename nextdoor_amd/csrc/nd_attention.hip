@@ -49,7 +49,7 @@ struct AttentionParams {
   PackedPlan plan;
   const void *q, *k, *v, *out, *dout;
   void *out_w, *dq, *dk, *dv;
-  float *lse, *lse2, *delta;  // [heads][tokens]; the backward kernels': lse in powers of two less what p is held times, delta times k
+  float *lse, *lse2, *delta;  // [heads][tokens]; the backward kernels': lse in powers of two less what p is held times, delta times k (whole sequences to a tile: as it is)
   // what the chunks of a tile whose work is cut leave: [chunk][token][head][dim] of out or dq, [chunk][head][token] of
   // maxima and sums, [chunk][token][kv_head][dim] of dk and dv
   float *row_sums, *dk_sums, *dv_sums;
@@ -236,9 +236,11 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
 // ---- what 16-bit floats hold ------------------------------------------------------------------------------
 // The backward pass rounds p and ds to 16 bits as operands.  The smallest 16-bit floats are steps of 2^-24, and p of a row of
 // thousands of keys and the ds of a mean's gradient are near that or below, while dq and dk are not (8000 keys, output gradients of 1e-3:
-// dq and dk off by 0.003 without this and by 0.00046 with it, of which 0.0004 are the result's own rounding); above 65504 they would be infinite.  So the kernels hold 2^15 p, and k 2^15 ds with the largest
-// power of two k <= 1 / (2 B), B = dim max |do| max |v| >= |dp|: |k 2^15 ds| <= 2^15.  2^15 goes into the exponent that makes p, k
-// into the subtraction of delta, which is kept times k: not one instruction more.  bfloat16 has the exponents of 32 bits: both are 1.
+// dq and dk off by 0.003 without this and by 0.00046 with it, of which 0.0004 are the result's own rounding); above 65504 they would
+// be infinite.  So the kernels hold 2^15 p, and k 2^15 ds with a power of two k, more than 1 / (4 B) and at most 1 / (2 B), B = dim
+// max |do| max |v| >= |dp|: |k 2^15 ds| <= 2^15.  2^15 goes into the exponent that makes p, k into the subtraction of delta, which is
+// kept times k: not one instruction more.  The maxima are those of the batch, from a launch before, or, where a workgroup has whole
+// sequences in LDS, its own.  bfloat16 has the exponents of 32 bits: both are 1.
 template <class T>
 struct Held {
   static constexpr float kShift = 0.f, kWeight = 1.f;
@@ -251,6 +253,28 @@ typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max_of_halves(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
+__device__ __forceinline__ uint32_t top_of(u32x4 v) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t low = v[j] & 0x7fff, high = v[j] >> 16 & 0x7fff;
+    top = max(top, max(low < 0x7c00 ? low : 0, high < 0x7c00 ? high : 0));
+  }
+  return top;
+}
+template <int CONTROL>
+__device__ __forceinline__ uint32_t turned(uint32_t v) { return __builtin_amdgcn_update_dpp(0, v, CONTROL, 0xf, 0xf, true); }
+__device__ __forceinline__ uint32_t top_of_wave(uint32_t top) {
+  // sixteen lanes by turning them by 1, 2, 4 and 8, then the four sixteens
+  top = max_of_halves(top, turned<0x121>(top));
+  top = max_of_halves(top, turned<0x122>(top));
+  top = max_of_halves(top, turned<0x124>(top));
+  top = max_of_halves(top, turned<0x128>(top));
+  const auto rows = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+  top = max_of_halves(rows[0], rows[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+  return max_of_halves(halves[0], halves[1]);
+}
 // The largest |x| of a part of the tokens, as 16-bit floats: low half of `out`, high half of v.  What is not finite does not count: its rows are
 // taken carefully.  A launch and its latency where there is little to read (8.3 thousand tokens, 6 heads of 80 and 3: 12 MB in 4.6 us).
 __device__ __forceinline__ uint32_t top_of(const char* x, int64_t token_bytes, int64_t head_bytes, uint32_t heads, uint32_t chunks, int64_t begin,
@@ -260,12 +284,7 @@ __device__ __forceinline__ uint32_t top_of(const char* x, int64_t token_bytes, i
 #pragma unroll 4
   for (uint32_t i = threadIdx.x; i < n; i += 1024) {
     const uint32_t c = i % chunks, row = i / chunks;
-    const u32x4 v = *(const u32x4*)(x + (begin + row / heads) * token_bytes + row % heads * head_bytes + c * 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t low = v[j] & 0x7fff, high = v[j] >> 16 & 0x7fff;
-      top = max(top, max(low < 0x7c00 ? low : 0, high < 0x7c00 ? high : 0));
-    }
+    top = max(top, top_of(*(const u32x4*)(x + (begin + row / heads) * token_bytes + row % heads * head_bytes + c * 16)));
   }
   return top;
 }
@@ -274,32 +293,37 @@ __global__ __launch_bounds__(1024) void attention_top_kernel(AttentionParams p) 
   const int64_t begin = (int64_t)p.plan.covered * blockIdx.x / kTopParts, end = (int64_t)p.plan.covered * (blockIdx.x + 1) / kTopParts;
   uint32_t top = top_of((const char*)p.dout, p.dout_token, p.dout_head, p.heads, p.dim / 8, begin, end) |
                  top_of((const char*)p.v, p.v_token, p.v_head, p.kv_heads, p.dim / 8, begin, end) << 16;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = max_of_halves(top, __shfl_xor(top, d));
+  top = top_of_wave(top);
   if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
   __syncthreads();
   if (threadIdx.x != 0) return;
   for (int i = 1; i < 16; ++i) top = max_of_halves(top, tops[i]);
   p.gradient_tops[blockIdx.x] = top;
 }
-// k, by every wave for itself.
+// k for a pair of them.
+__device__ __forceinline__ float scale_of_tops(uint32_t top, int dim) {
+  const float most = unpack_low<_Float16>(top) * unpack_high<_Float16>(top) * (float)dim;  // B, between 2^-46 and 2^39, or 0
+  return __uint_as_float((uint32_t)uniform(most > 0.f ? 252 - (__float_as_uint(most) >> 23) : 127) << 23);  // (its exponent e: 2^(-2 - e))
+}
+// 1 / k, of a power of two.
+__device__ __forceinline__ float one_over(float k) { return __uint_as_float(0x7f000000 - __float_as_uint(k)); }
+// k of the whole batch, by every wave for itself.
 template <class T>
 __device__ __forceinline__ float gradient_scale(const AttentionParams& p) {
   if constexpr (!std::is_same<T, _Float16>::value) return 1.f;
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kTopParts; i += 64) top = max_of_halves(top, p.gradient_tops[i + (threadIdx.x & 63)]);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = max_of_halves(top, __shfl_xor(top, d));
-  const float most = unpack_low<_Float16>(top) * unpack_high<_Float16>(top) * (float)p.dim;  // B, between 2^-46 and 2^39, or 0
-  return __uint_as_float((uint32_t)uniform(most > 0.f ? 252 - (__float_as_uint(most) >> 23) : 127) << 23);  // (its exponent e: 2^(-2 - e))
+  return scale_of_tops(top_of_wave(top), p.dim);
 }
 
 // ---- rows with one key ----------------------------------------------------------------------------------
 // The first token of a sequence has itself as its only key: its weight is 1 and ds = p (dp - delta) = 0 whatever it holds.  Weights
 // made again from lse are 1 +- some 2^-24 |s|, which would leave noise where nothing belongs (and an optimizer that normalises makes
-// full steps of it).  So the backward kernels take its lse as infinite, which makes the weight 0 and with it ds (NaN, where the
-// row is not finite), and put the weight of the pair back to 1 for dv.
+// full steps of it).  The kernels for long sequences take its lse as infinite, which makes the weight 0 and with it ds (NaN, where the
+// row is not finite), and put the weight of the pair back to 1 for dv.  The kernel for short ones has a factor of each row in LDS
+// anyway, which is 0 for it: p (0 dp - 0); its dv has the weight as it is, 1 once rounded to 16 bits (up to logits of a thousand).
+// (There the weight of the pair by comparisons took 440 us where this takes 436 at heads of 128, and 424 with neither.)
 __device__ __forceinline__ float one_key_lse2(float lse) { return INFINITY + (lse - lse); }
 // A result's 32 x 32 weights, rows = queries, where the lane's key is query `at` + 4 h of them and its own query's only key (at = -32: it is not).
 template <class T>
@@ -308,21 +332,6 @@ __device__ __forceinline__ void one_key_weight(f32x16& weights, int at) {
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     if (8 * (i / 4) + i % 4 == at && weights[i] == weights[i]) weights[i] = Held<T>::kWeight;
-}
-// The same at once, where the queries' output gradients are in LDS (in the loop above the comparisons would take registers that are
-// not there: 9 spilled at heads of 64): dv of the lane's key, which is row `r` of them, += that row.
-template <class T, int NB>
-__device__ __forceinline__ void one_key_dv(f32x16 (&dv)[NB], const u32x4* douts, int r, bool one, int h) {
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const u32x2 v = ((const u32x2*)(douts + tile_place<HeadTile<NB>::kChunks>(r, 4 * b + g)))[h];
-      dv[b][4 * g] += one ? unpack_low<T>(v[0]) * Held<T>::kWeight : 0.f;
-      dv[b][4 * g + 1] += one ? unpack_high<T>(v[0]) * Held<T>::kWeight : 0.f;
-      dv[b][4 * g + 2] += one ? unpack_low<T>(v[1]) * Held<T>::kWeight : 0.f;
-      dv[b][4 * g + 3] += one ? unpack_high<T>(v[1]) * Held<T>::kWeight : 0.f;
-    }
 }
 // For the same reason: delta = sum p dp, and the weights' own sum, by which the errors that they share go out of it, so that a row's ds add up
 // to 0.  (Logits so large that 32 bits hold no weight have no sum to go by.)
@@ -386,7 +395,7 @@ __device__ __forceinline__ void dk_dv_carefully(const AttentionParams& p, int kv
         if (one) weight = 1.f + (p.lse[at] - p.lse[at]);
         if (which == 1) {
           const float dp = dot_rows<T>(v, d, p.dim, h);
-          weight *= dp - (one ? dp : p.delta[at] / k_scale);
+          weight *= dp - (one ? dp : p.delta[at] * one_over(k_scale));
         }
         if (sees) add_row<T, NB>(acc, 1.f, weight, which == 0 ? d : q, p.dim, h);
       }
@@ -738,11 +747,11 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
   }
   if (row0 < p.plan.tokens && __builtin_amdgcn_ballot_w64(!all_finite(acc)) != 0) {
-    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, p.plan.tokens, delta / k_scale,
+    dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, careful_begin, careful_stop, p.plan.tokens, delta * one_over(k_scale),
                         chunk, chunks);
     return;
   }
-  const float factor = p.scale / (Held<T>::kWeight * k_scale);
+  const float factor = p.scale * (1.f / Held<T>::kWeight) * one_over(k_scale);
   if (chunks > 1) {
     if (row < p.plan.tokens)
       store_sums<NB>(p.row_sums + (((int64_t)chunk * p.plan.tokens + row) * p.heads + head) * p.dim, acc, factor, p.dim, h);
@@ -908,7 +917,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
     return;
   }
   const int64_t row_elements = (int64_t)p.kv_heads * p.dim;
-  const float dk_factor = p.scale / (Held<T>::kWeight * k_scale), dv_factor = 1.f / Held<T>::kWeight;
+  const float dk_factor = p.scale * (1.f / Held<T>::kWeight) * one_over(k_scale), dv_factor = 1.f / Held<T>::kWeight;
   if (chunks * p.head_split == 1) {
     u32x4* part_lds = &tiles[0][0][0] + wave * 32 * kChunks;
     const int64_t at = ((int64_t)key0 * p.kv_heads + kv_head) * p.dim;
@@ -933,7 +942,8 @@ template <class T, int NB>
 __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short_kernel(AttentionParams p) {
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRows * kChunks;
   __shared__ u32x4 keys[kSize], values[kSize], queries[kSize], douts[kSize];
-  __shared__ float lse2s[kRows], deltas[kRows];
+  __shared__ float lse2s[kRows], deltas[kRows], factors[kRows];
+  __shared__ uint32_t tops[4];
   // (what is computed from `lane` is computed anew after each empty asm: addresses kept from one part to the next cost 14 to 47
   // spilled registers, 66 and 397 us for 60 and 342 at heads of 64 and 128)
   int lane = threadIdx.x & 63;
@@ -949,7 +959,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
 #pragma unroll
   for (int b = 0; b < NB; ++b) dk[b] = dv[b] = f32x16{};
   const float dv_factor = 1.f / Held<T>::kWeight;
-  float k_scale = 1.f, dk_factor = 0.f;
+  float k_scale = 1.f;
   bool again = false;  // some head's dq is not finite: taken carefully at the end, where no sums are in registers
 
   if (tile0 < p.plan.covered) {
@@ -962,15 +972,13 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
     const TileLoader<NB, kRows> k(p.k, p.k_token, p.k_head, kv_head, p.dim), v(p.v, p.v_token, p.v_head, kv_head, p.dim);
     k.issue(lds_address(keys) + part, p.k_token, tile0, tile_end);
     v.issue(lds_address(values) + part, p.v_token, tile0, tile_end);
-    k_scale = gradient_scale<T>(p);
-    dk_factor = p.scale / (Held<T>::kWeight * k_scale);  // (of dq too)
     for (int g = 0; g < heads; ++g) {
       const int head = head0 + g;
       if (g > 0) __syncthreads();  // (the last head's dq has left through `queries`)
       const TileLoader<NB, kRows> q(p.q, p.q_token, p.q_head, head, p.dim), d(p.dout, p.dout_token, p.dout_head, head, p.dim);
       q.issue(lds_address(queries) + part, p.q_token, tile0, tile_end);
       d.issue(lds_address(douts) + part, p.dout_token, tile0, tile_end);
-      const float lse = there ? p.lse[(int64_t)head * p.plan.tokens + row] : 0.f, lse2 = first == row ? one_key_lse2(lse) : lse * kLog2e - Held<T>::kShift;
+      const float lse = there ? p.lse[(int64_t)head * p.plan.tokens + row] : 0.f, lse2 = lse * kLog2e - Held<T>::kShift;
       if (h == 0) lse2s[wave * 32 + (lane & 31)] = lse2;
       wait_for_loads_and_others();
       if (g == 0 && p.dim < 8 * kChunks) {  // the other operands have a row's first columns past `dim`: 0 here
@@ -980,6 +988,39 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
             keys[place] = values[place] = u32x4{0, 0, 0, 0};
           }
         __syncthreads();
+      }
+      if constexpr (std::is_same<T, _Float16>::value) {
+        // k of what is in LDS and of the heads before (walks of up to 101, 8 heads of 64 and of 128: 57 and 464 us, 67 and 552 with the
+        // launch before that reads all output gradients and values; 54 and 436 with neither)
+        uint32_t top = 0, others = 0;
+#pragma unroll
+        for (int i = 0; i < kSize; i += 256) {
+          const u32x4 a = douts[i + 64 * wave + lane], b = values[i + 64 * wave + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            top = max_of_halves(top, a[j] & 0x7fff7fff);
+            others = max_of_halves(others, b[j] & 0x7fff7fff);
+          }
+        }
+        top = max(top & 0xffff, top >> 16) | max(others & 0xffff, others >> 16) << 16;
+        if (__builtin_amdgcn_ballot_w64((top & 0xffff) >= 0x7c00 || top >= 0x7c000000) != 0) {  // (what is not finite does not count)
+          top = 0;
+#pragma unroll 1
+          for (int at = 64 * wave + lane; at < kSize; at += 256) top = max_of_halves(top, top_of(douts[at]) | top_of(values[at]) << 16);
+        }
+        top = top_of_wave(top);
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        const float k = scale_of_tops(max_of_halves(max_of_halves(tops[0], tops[1]), max_of_halves(tops[2], tops[3])), p.dim);
+        asm volatile("" : "+v"(lane));
+        if (g == 0 || k < k_scale) {
+          const float ratio = g == 0 ? 1.f : k * one_over(k_scale);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[b][i] *= ratio;
+          k_scale = k;
+        }
       }
       f32x16 dq[NB];
 #pragma unroll
@@ -992,6 +1033,8 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
           dof[i] = read_operand_by_rows<kChunks>(douts, 32 * wave, i, lane);
         }
         float delta = 0.f;
+        const float factor = first == row ? 0.f : k_scale;
+        if (h == 0) factors[wave * 32 + (lane & 31)] = factor;
         for (int sweep = 0; sweep < 2; ++sweep) {  // for delta, then for dq
           float sum = 0.f, weights = 0.f;
           for (int at = first_tile; at <= wave; ++at) {
@@ -1009,7 +1052,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
               const int key = 8 * (i / 4) + i % 4;
               const bool sees = key >= from && key <= to;
               s[i] = sees ? exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lse2)) : 0.f;
-              dp[i] = sees ? __builtin_fmaf(dp[i], k_scale, -delta) : 0.f;
+              dp[i] = sees ? __builtin_fmaf(dp[i], factor, -delta) : 0.f;
             }
             if (sweep == 0) {
 #pragma unroll
@@ -1035,7 +1078,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
         asm volatile("" : "+v"(lane));
         if (h == 0) {
           deltas[wave * 32 + (lane & 31)] = delta;
-          if (there) p.delta[(int64_t)head * p.plan.tokens + row] = delta;
+          if (there) p.delta[(int64_t)head * p.plan.tokens + row] = delta * one_over(k_scale);
         }
       }
       __syncthreads();
@@ -1059,13 +1102,14 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             const f32x4 lses = *(const f32x4*)&lse2s[32 * t + 8 * q4 + 4 * h], delta = *(const f32x4*)&deltas[32 * t + 8 * q4 + 4 * h];
+            const f32x4 factor = *(const f32x4*)&factors[32 * t + 8 * q4 + 4 * h];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
               const int i = 4 * q4 + n, query = 8 * q4 + n;
               const bool sees = query >= from && query < to;
               const float weight = exp2_fast(__builtin_fmaf(s[i], p.scale_log2, -lses[n]));
               s[i] = sees ? weight : 0.f;
-              dp[i] = sees ? weight * __builtin_fmaf(dp[i], k_scale, -delta[n]) : 0.f;
+              dp[i] = sees ? weight * __builtin_fmaf(dp[i], factor[n], -delta[n]) : 0.f;
             }
           }
 #pragma unroll
@@ -1078,14 +1122,12 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
             }
           }
         }
-        asm volatile("" : "+v"(lane));
-        const bool one = lse2s[32 * wave + (lane & 31)] == INFINITY;
-        if (__builtin_amdgcn_ballot_w64(one) != 0) one_key_dv<T, NB>(dv, douts, 32 * wave + (lane & 31), one, h);
       }
       __syncthreads();
       again = again || __builtin_amdgcn_ballot_w64(!all_finite(dq)) != 0;
       if (work)
-        store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq, dk_factor, p.dim, part_lds);
+        store_rows<T, NB>((T*)p.dq + ((int64_t)row0 * p.heads + head) * p.dim, q_elements, tile_end - row0, dq,
+                          p.scale * (1.f / Held<T>::kWeight) * one_over(k_scale), p.dim, part_lds);
     }
   } else if (row0 < tile_end) {  // tokens of no sequence
     for (int g = 0; g < heads; ++g)
@@ -1093,9 +1135,10 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
                         part_lds);
   }
   if (row0 >= tile_end) return;
+  const float dk_factor = p.scale * (1.f / Held<T>::kWeight) * one_over(k_scale);
   if (__builtin_amdgcn_ballot_w64(!(all_finite(dk) && all_finite(dv))) != 0) {
     dk_dv_carefully<T, NB>(p, kv_head, head0, row, row < tile_end ? p.plan.last[row] : row, tile0, tile_end, kRows, 1, 0, heads, tile_end,
-                           p.head_split == 1 ? -1 : share, k_scale);
+                           p.head_split == 1 ? -1 : share, 1.f);
   } else if (p.head_split == 1) {
     const int64_t at = ((int64_t)row0 * p.kv_heads + kv_head) * p.dim;
     store_rows<T, NB>((T*)p.dk + at, k_elements, tile_end - row0, dk, dk_factor, p.dim, part_lds);
@@ -1111,7 +1154,7 @@ __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short
     const int head = head0 + g;
     const bool there = row < tile_end;
     dq_carefully<T, NB>(p, head, kv_head, row, there ? p.plan.first[row] : row + 1, tile0, tile_end, tile_end,
-                        there ? p.delta[(int64_t)head * p.plan.tokens + row] / k_scale : 0.f, 0, 1);
+                        there ? p.delta[(int64_t)head * p.plan.tokens + row] : 0.f, 0, 1);
   }
 }
 
@@ -1195,7 +1238,7 @@ Cuts cuts_of(const nd_packed_attention& a, bool backward) {
     w.max_key_chunks = most(a.most_rounds * finer * (group / w.head_split), w.key_chunk, key_bytes * w.head_split);
     take(a.n_tokens * a.heads * 4);  // lse2
     w.delta = take(a.n_tokens * a.heads * 4);
-    if (a.dtype == ND_F16) w.gradient_tops = take(kTopParts * 4);
+    if (a.dtype == ND_F16 && a.short_tiles == 0) w.gradient_tops = take(kTopParts * 4);
   }
   w.chunk = std::min<int64_t>(w.chunk, 0x3fffffff);
   if (w.max_chunks > 1) w.row_sums = take(w.max_chunks * row_bytes);
@@ -1218,10 +1261,10 @@ void launch_forward(const AttentionParams& p, hipStream_t stream) {
 }
 template <class T, int NB>
 void launch_backward(const AttentionParams& p, hipStream_t stream) {
-  if (std::is_same<T, _Float16>::value) attention_top_kernel<<<kTopParts, 1024, 0, stream>>>(p);
   if (p.plan.short_tiles > 0) {
     attention_backward_short_kernel<T, NB><<<(uint32_t)p.plan.short_tiles * p.kv_heads * p.head_split, 256, 0, stream>>>(p);
   } else {
+    if (std::is_same<T, _Float16>::value) attention_top_kernel<<<kTopParts, 1024, 0, stream>>>(p);
     attention_backward_query_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.heads * p.max_chunks, 256, 0, stream>>>(p);
     attention_backward_key_kernel<T, NB><<<(uint32_t)p.plan.tiles * p.kv_heads * p.head_split * p.max_key_chunks, 256, 0, stream>>>(p);
   }

@@ -302,3 +302,17 @@ def test_tensors_of_other_shapes_are_refused_as_the_rest_is():
                      (ops.vocabulary_loss_forward, (h[:, :0], h[:, :0], t)), (ops.vocabulary_loss_backward, (lse[0], h, h, t, one.float()))):
         with pytest.raises(NextDoorError):
             fn(*args)
+
+
+@pytest.mark.parametrize("lengths", [[100, 1, 31, 77, 120] * 60, [100, 28, 5], [300, 70]])
+def test_attention_heads_of_a_group_with_gradients_of_different_sizes(lengths):
+    """Small, then large, then small ones again, in 16-bit floats: the sums of a key are those of all of them."""
+    starts, heads, kv_heads, dim = starts_of(lengths), 8, 2, 64
+    t = int(starts[-1])
+    q, k, v = (normal(i, t, n, dim, dtype=F16) for i, n in enumerate((heads, kv_heads, kv_heads)))
+    sizes = torch.tensor([1e-4, 1.0, 1e-5, 30.0, 30.0, 1e-5, 1.0, 0.0])
+    dout = (normal(5, t, heads, dim, dtype=torch.float32) * sizes[:, None]).to(F16)
+    want, off = gradients(q, k, v, starts, 1 / 8, dout)
+    got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda())
+    for name in want:
+        assert ref.close(got[name], want[name], off[name]), name
