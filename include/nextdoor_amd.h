@@ -310,7 +310,7 @@ int nd_dropout(const void* d_x, const void* d_residual, void* d_y, int64_t n, in
  * entries), which is checked, d_starts the same on the device; the plan (nd_packed_plan_bytes(n_tokens)
  * bytes, aligned to 16) is what every attention call over this batch reads.  sizes (on the host): how
  * much work there is in all and in the largest tile, and the tiles of whole sequences (0 if some are too
- * long), by which attention calls choose their kernels.  Not for graph capture. */
+ * long), by which attention calls choose their kernels.  Not for graph capture; calls on other streams come after it. */
 #define ND_PACKED_MAX_TOKENS 2147483392
 #define ND_PACKED_MAX_DIM 128
 #define ND_PACKED_MAX_TOKEN_STRIDE 16777216
@@ -323,6 +323,7 @@ int nd_packed_plan(const int32_t* starts, int64_t n_sequences, int64_t n_tokens,
  * lie side by side); out, dq: [n_tokens][heads][dim], dk, dv: [n_tokens][kv_heads][dim], lse:
  * [heads][n_tokens], all dense.  Arrays are aligned to 16 bytes, dim is a multiple of 8.
  * Tokens of no sequence are not read; their rows of out and of the gradients are 0, their lse -inf.
+ * The first token of a sequence sees itself only: dq = 0 exactly, and dk = 0 of a sequence of one.
  * The backward call reads what the forward call left in out and lse.  The workspace
  * (nd_packed_attention_workspace(...) bytes, which reads the struct's numbers only; may be 0) is
  * working memory of one call. */
@@ -348,7 +349,8 @@ int nd_packed_attention_backward(const nd_packed_attention* a, void* stream);
  * loss_i = log sum_v exp(h_i . w_v) - h_i . w_{target_i}.  A target outside 0 .. classes - 1 (the
  * samplers' INVALID is |V|) has loss 0 and sends nothing back.  hidden, dhidden: [rows][dim], weight,
  * dweight: [classes][dim], dense, aligned to 16 bytes, dim a multiple of 8, fewer than 2^34 elements; lse: [rows], left by
- * the forward call and read by the backward call; dloss: [rows], the gradient of each row's loss.
+ * the forward call and read by the backward call; dloss: [rows], the gradient of each row's loss (ND_BF16: below 2^95,
+ * it is held times 2^32).
  * workspace: nd_vocabulary_loss_workspace(...) bytes, aligned to 16, working memory of one call. */
 #define ND_VOCABULARY_MAX_ROWS 4194240
 #define ND_VOCABULARY_MAX_CLASSES 2147483392

@@ -772,7 +772,7 @@ __global__ __launch_bounds__(256, 2) void attention_backward_query_kernel(Attent
 // alone).  They are read from LDS instead, and a round takes 32 queries, so that two workgroups fit a compute unit.
 //
 // Four products, two of them those of the dq kernel once more (taking dq here too would need atomics, or its sums for every tile
-// of keys in memory).  The long sequences above, 4 key heads: 318 us, 0.88 PFLOP/s, matrix cores busy 46 %, 191 MB of sums and
+// of keys in memory).  The long sequences above, 4 key heads: 325 us, 0.86 PFLOP/s, matrix cores busy 44 %, 190 MB of sums and
 // results written.
 template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(AttentionParams p) {
@@ -936,8 +936,8 @@ __global__ __launch_bounds__(256, 2) void attention_backward_key_kernel(Attentio
 // delta always comes from the weights themselves.
 //
 // 1024 walks of up to 101 tokens, 8 heads of 64: 57 us where the two kernels above take 97, 155 MB (2.7 TB/s), bound by the
-// latency of one load of a tile and three sweeps over it.  8 heads of 128, walks of 20 to 101: 342 us for 370; of 101 throughout,
-// which leave a fifth of each tile empty, 791 for 733.
+// latency of one load of a tile and three sweeps over it.  8 heads of 128, walks of 20 to 101 spread over the logarithm: 349 us for
+// 360; spread evenly 435 for 423; of 101 throughout, which leave a fifth of each tile empty, 798 for 716.
 template <class T, int NB>
 __global__ __launch_bounds__(256, NB <= 2 ? 2 : 1) void attention_backward_short_kernel(AttentionParams p) {
   constexpr int kChunks = HeadTile<NB>::kChunks, kSize = kRows * kChunks;

@@ -139,7 +139,9 @@ class PackedSequences:
 
     ``starts`` (a list, a numpy array or a tensor; integers) begins with 0 and does not fall; a tensor on the GPU is
     read back to be checked, which waits for it.  ``n_tokens`` (default: ``starts[-1]``) may be larger: tokens after
-    the last sequence belong to none.  Make one per batch; every layer and both directions use it."""
+    the last sequence belong to none.  Make one per batch; every layer and both directions use it (30 to 50 us on the host).
+    Like any tensor it is filled on the stream that is current here: a call on another stream has to come after that
+    (``stream.wait_stream``), and it has to live until such a call is done.  Not while a graph is recorded."""
 
     def __init__(self, starts, n_tokens=None, device=None):
         if isinstance(starts, torch.Tensor):
@@ -237,7 +239,8 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
     q, out: [tokens, heads, dim]; k, v: [tokens, kv_heads, dim], ``heads / kv_heads`` query heads to each; dim a
     multiple of 8 up to 128; float16 or bfloat16.  Slices of one projection are read in place.  lse:
     [heads, tokens], float32, for the backward pass.  ``scale`` is 1 / sqrt(dim) unless given.  Rows of tokens that
-    belong to no sequence are 0 (lse -inf) and their inputs are not read."""
+    belong to no sequence are 0 (lse -inf) and their inputs are not read.  Weights are rounded to the type of q before they
+    meet v, results once."""
     index, keep, fields, rows = _attention(sequences, q, k, v, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(rows, dtype=torch.float32, device=q.device)
@@ -249,7 +252,9 @@ def packed_attention_forward(q, k, v, sequences, scale=None):
 
 
 def packed_attention_backward(dout, q, k, v, out, lse, sequences, scale=None):
-    """(dq, dk, dv) for the gradient ``dout`` of ``out``, which with ``lse`` is the forward pass's."""
+    """(dq, dk, dv) for the gradient ``dout`` of ``out``, which with ``lse`` is the forward pass's.  Weights and their gradients
+    are rounded to the type of q before their second product (float16: times a power of two, so that small ones are not
+    lost).  The first token of a sequence, which sees itself only, has dq = 0 exactly."""
     _on_gpu("packed attention", q, dout, out, lse)
     index, keep, fields, rows = _attention(sequences, q, k, v, scale, dout)
     if not (out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and lse.is_contiguous() and
@@ -342,7 +347,7 @@ def vocabulary_loss_forward(hidden, weight, target):
 
 def vocabulary_loss_backward(dloss, hidden, weight, target, lse):
     """(dhidden, dweight) for the gradient ``dloss`` of each row's loss; lse is the forward pass's.  Rows without a
-    target send nothing back, whatever their ``dloss``."""
+    target send nothing back, whatever their ``dloss``.  bfloat16: ``dloss`` below 2^95."""
     _on_gpu("vocabulary loss", hidden, dloss, lse)
     index, keep, fields, workspace, size = _loss(hidden, weight, target, 1)
     width = hidden.shape[1]

@@ -1,8 +1,8 @@
 """A language model over sampled walks: ``python -m nextdoor_amd.walk_model``.
 
-Walks are its sentences, vertices its words.  A step samples one walk per vertex with the engine, packs them one after
-another (a walk ends where a vertex has no edges), and trains a small transformer to predict each next vertex: embeddings
-with dropout, causal attention within each walk, softmax cross entropy over all vertices
+Walks are its sentences, vertices its words.  The engine samples one walk from every vertex, once; a step takes some of them,
+packs them one after another (a walk ends where a vertex has no edges), and trains a small transformer to predict each next
+vertex: embeddings with dropout, causal attention within each walk, softmax cross entropy over all vertices
 (nextdoor_amd/ops.py).  It shows the operators as a training program uses them; nothing is tuned for accuracy.
 """
 import argparse

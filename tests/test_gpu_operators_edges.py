@@ -316,3 +316,28 @@ def test_attention_heads_of_a_group_with_gradients_of_different_sizes(lengths):
     got = run_attention(q.cuda(), k.cuda(), v.cuda(), starts, dout.cuda())
     for name in want:
         assert ref.close(got[name], want[name], off[name]), name
+
+
+@pytest.mark.parametrize("lengths", [[100, 28, 5, 77], [300, 1, 170]])
+def test_attention_of_16_bit_floats_is_the_same_in_a_graph(lengths):
+    """What they are held times is found anew at every replay."""
+    starts = starts_of(lengths)
+    q, k, v, dout = (normal(i, int(starts[-1]), 4, 64, dtype=F16).cuda() for i in range(4))
+    seq = ops.PackedSequences(starts)
+
+    def step():
+        out, lse = ops.packed_attention_forward(q, k, v, seq)
+        return (out, *ops.packed_attention_backward(dout, q, k, v, out, lse, seq))
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        for x in got:
+            x.zero_()
+        dout.mul_(0.01 if i < 2 else 3000.0)
+        want = [x.clone() for x in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
