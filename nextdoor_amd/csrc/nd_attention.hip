@@ -237,7 +237,7 @@ __device__ __forceinline__ void forward_carefully(const AttentionParams& p, int 
 // The backward pass rounds p and ds to 16 bits as operands.  The smallest 16-bit floats are steps of 2^-24, and p of a row of
 // thousands of keys and the ds of a mean's gradient are near that or below, while dq and dk are not (8000 keys, output gradients of 1e-3:
 // dq and dk off by 0.003 without this and by 0.00046 with it, of which 0.0004 are the result's own rounding); above 65504 they would
-// be infinite.  So the kernels hold 2^15 p, and k 2^15 ds with a power of two k, more than 1 / (4 B) and at most 1 / (2 B), B = dim
+// be infinite.  So the kernels hold 2^15 p, and k 2^15 ds with a power of two k, at least 1 / (4 B) and below 1 / (2 B), B = dim
 // max |do| max |v| >= |dp|: |k 2^15 ds| <= 2^15.  2^15 goes into the exponent that makes p, k into the subtraction of delta, which is
 // kept times k: not one instruction more.  The maxima are those of the batch, from a launch before, or, where a workgroup has whole
 // sequences in LDS, its own.  bfloat16 has the exponents of 32 bits: both are 1.
@@ -275,7 +275,7 @@ __device__ __forceinline__ uint32_t top_of_wave(uint32_t top) {
   const auto halves = __builtin_amdgcn_permlane32_swap(top, top, false, false);
   return max_of_halves(halves[0], halves[1]);
 }
-// The largest |x| of a part of the tokens, as 16-bit floats: low half of `out`, high half of v.  What is not finite does not count: its rows are
+// The largest |x| of a part of the tokens, as 16-bit floats: low half of dout, high half of v.  What is not finite does not count: its rows are
 // taken carefully.  A launch and its latency where there is little to read (8.3 thousand tokens, 6 heads of 80 and 3: 12 MB in 4.6 us).
 __device__ __forceinline__ uint32_t top_of(const char* x, int64_t token_bytes, int64_t head_bytes, uint32_t heads, uint32_t chunks, int64_t begin,
                                            int64_t end) {
