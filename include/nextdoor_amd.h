@@ -370,6 +370,79 @@ int64_t nd_vocabulary_loss_workspace(int64_t rows, int64_t classes, int32_t dim,
 int nd_vocabulary_loss_forward(const nd_vocabulary_loss* a, void* stream);
 int nd_vocabulary_loss_backward(const nd_vocabulary_loss* a, void* stream);
 
+/* Layer norm of `rows` vectors of `dim` values: mean_i and rstd_i = 1 / sqrt(variance_i + eps) (over dim, not dim - 1), out =
+ * (x - mean_i) rstd_i weight + bias.  Gradients: with e = dout weight and n = (x - mean_i) rstd_i, dx = rstd_i (e - mean(e)
+ * - n mean(e n)), dweight = sum over the rows of dout n, dbias that of dout.  x and dout: rows x_row and dout_row elements
+ * apart (any number >= 0; dim elements lie side by side); out and dx: dense; weight, bias, dweight, dbias: [dim], of
+ * weight_dtype, which is dtype or ND_F32; weight NULL: 1, bias NULL: 0; mean, rstd: [rows], left by the forward call and read by the
+ * backward call.  dx, dweight or dbias NULL: not computed.  Arrays are aligned as their elements are.  Sums are in 32 bits.
+ * workspace: nd_layer_norm_workspace(...) bytes (backward only), aligned to 16, working memory of one call. */
+#define ND_LAYER_NORM_MAX_DIM 16384
+typedef struct nd_layer_norm {
+  int64_t rows;
+  int32_t dim, dtype, weight_dtype;
+  float eps;
+  int64_t x_row, dout_row;
+  const void *x, *weight, *bias;
+  void* out;
+  float *mean, *rstd;
+  const void* dout;
+  void *dx, *dweight, *dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+} nd_layer_norm;
+int64_t nd_layer_norm_workspace(const nd_layer_norm* a);
+int nd_layer_norm_forward(const nd_layer_norm* a, void* stream);
+int nd_layer_norm_backward(const nd_layer_norm* a, void* stream);
+
+/* Linear maps of `rows` vectors of `dim` places to `out_dim`: z = x weight^T + bias, out = activation(z) + residual.
+ * weight: [out_dim][dim]; bias: [out_dim] or NULL; residual: like out, or NULL.  z NULL: not kept; the backward call of a map
+ * with an activation reads it.  Gradients of dout: dz = dout activation'(z), dx = dz weight, dweight = dz^T x, dbias = sum of
+ * the rows of dz; the residual's is dout itself.  dx, dweight or dbias NULL: not computed.
+ * ND_GELU is x times the normal distribution's integral up to x, ND_GELU_TANH its approximation by tanh, ND_SILU x / (1 +
+ * exp(-x)).  ND_F16 and ND_BF16; dim and out_dim are multiples of 8; arrays are aligned to 16 bytes; rows of x, residual and dout
+ * lie x_row, residual_row and dout_row elements apart (multiples of 8, >= 0; rows may overlap or be the same), everything else is
+ * dense.  Sums are in 32 bits; out, z, dz and the gradients are rounded to 16 bits once.
+ * workspace: nd_linear_workspace(...) bytes, which reads the struct's numbers and which arrays are NULL (may be 0), aligned to
+ * 16, working memory of one call. */
+enum { ND_NO_ACTIVATION = 0, ND_RELU = 1, ND_GELU = 2, ND_GELU_TANH = 3, ND_SILU = 4 };
+#define ND_LINEAR_MAX_ROWS 2147483392
+#define ND_LINEAR_MAX_DIM 1048576
+#define ND_LINEAR_MAX_ROW_STRIDE 4194304
+typedef struct nd_linear {
+  int64_t rows;
+  int32_t dim, out_dim, dtype, activation;
+  int64_t x_row, residual_row, dout_row;
+  const void *x, *weight, *bias, *residual;
+  void *out, *z;
+  const void* dout;
+  void *dx, *dweight, *dbias;
+  void* workspace;
+  int64_t workspace_bytes;
+} nd_linear;
+int64_t nd_linear_workspace(const nd_linear* a, int backward);
+int nd_linear_forward(const nd_linear* a, void* stream);
+int nd_linear_backward(const nd_linear* a, void* stream);
+
+/* A feed-forward part: z = x up^T + up_bias, h = activation(z) (gated == 0) or, of z = [g, u], activation(g) u (gated != 0), out = h
+ * down^T + down_bias + residual.  up: [inner][dim], gated [2 inner][dim] (the rows of g, then those of u); down: [out_dim][inner].
+ * h: [rows][inner], always written, and z, [rows][inner or 2 inner], unless it is NULL, are what the backward call reads (z is
+ * not needed without an activation and a gate).  Everything else as for linear maps. */
+typedef struct nd_mlp {
+  int64_t rows;
+  int32_t dim, inner, out_dim, dtype, activation, gated;
+  int64_t x_row, residual_row, dout_row;
+  const void *x, *up, *up_bias, *down, *down_bias, *residual;
+  void *out, *z, *h;
+  const void* dout;
+  void *dx, *dup, *dup_bias, *ddown, *ddown_bias;
+  void* workspace;
+  int64_t workspace_bytes;
+} nd_mlp;
+int64_t nd_mlp_workspace(const nd_mlp* a, int backward);
+int nd_mlp_forward(const nd_mlp* a, void* stream);
+int nd_mlp_backward(const nd_mlp* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,31 @@ class VocabularyLoss(C.Structure):
                                            "workspace")] + [("workspace_bytes", C.c_int64)])
 
 
+class LayerNorm(C.Structure):
+    """nd_layer_norm"""
+    _fields_ = ([("rows", C.c_int64)] + [(n, C.c_int32) for n in ("dim", "dtype", "weight_dtype")] + [("eps", C.c_float)] +
+                [(n, C.c_int64) for n in ("x_row", "dout_row")] +
+                [(n, C.c_void_p) for n in ("x", "weight", "bias", "out", "mean", "rstd", "dout", "dx", "dweight", "dbias",
+                                           "workspace")] + [("workspace_bytes", C.c_int64)])
+
+
+class Linear(C.Structure):
+    """nd_linear"""
+    _fields_ = ([("rows", C.c_int64)] + [(n, C.c_int32) for n in ("dim", "out_dim", "dtype", "activation")] +
+                [(n, C.c_int64) for n in ("x_row", "residual_row", "dout_row")] +
+                [(n, C.c_void_p) for n in ("x", "weight", "bias", "residual", "out", "z", "dout", "dx", "dweight", "dbias",
+                                           "workspace")] + [("workspace_bytes", C.c_int64)])
+
+
+class Mlp(C.Structure):
+    """nd_mlp"""
+    _fields_ = ([("rows", C.c_int64)] + [(n, C.c_int32) for n in ("dim", "inner", "out_dim", "dtype", "activation", "gated")] +
+                [(n, C.c_int64) for n in ("x_row", "residual_row", "dout_row")] +
+                [(n, C.c_void_p) for n in ("x", "up", "up_bias", "down", "down_bias", "residual", "out", "z", "h", "dout", "dx",
+                                           "dup", "dup_bias", "ddown", "ddown_bias", "workspace")] +
+                [("workspace_bytes", C.c_int64)])
+
+
 # name -> (restype, argtypes); every symbol include/nextdoor_amd.h declares
 SIGNATURES = {
     "nd_last_error": (C.c_char_p, []),
@@ -110,6 +135,15 @@ SIGNATURES = {
     "nd_vocabulary_loss_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32, C.c_int]),
     "nd_vocabulary_loss_forward": (C.c_int, [C.POINTER(VocabularyLoss), C.c_void_p]),
     "nd_vocabulary_loss_backward": (C.c_int, [C.POINTER(VocabularyLoss), C.c_void_p]),
+    "nd_layer_norm_workspace": (C.c_int64, [C.POINTER(LayerNorm)]),
+    "nd_layer_norm_forward": (C.c_int, [C.POINTER(LayerNorm), C.c_void_p]),
+    "nd_layer_norm_backward": (C.c_int, [C.POINTER(LayerNorm), C.c_void_p]),
+    "nd_linear_workspace": (C.c_int64, [C.POINTER(Linear), C.c_int]),
+    "nd_linear_forward": (C.c_int, [C.POINTER(Linear), C.c_void_p]),
+    "nd_linear_backward": (C.c_int, [C.POINTER(Linear), C.c_void_p]),
+    "nd_mlp_workspace": (C.c_int64, [C.POINTER(Mlp), C.c_int]),
+    "nd_mlp_forward": (C.c_int, [C.POINTER(Mlp), C.c_void_p]),
+    "nd_mlp_backward": (C.c_int, [C.POINTER(Mlp), C.c_void_p]),
     "nd_unique_transits": (C.c_int, [c_i32p, C.c_int64, C.c_int32, c_i32p, c_i32p, c_i32p, c_i64p, c_i64p]),
 }
 

@@ -10,7 +10,7 @@ OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libnextdoor_amd.so")
 
 SOURCES = ["nd_capi.hip", "nd_graph.cpp", "nd_check.cpp", "nd_dropout.hip", "nd_attention.hip",
-           "nd_vocabulary_loss.hip"]
+           "nd_vocabulary_loss.hip", "nd_layer_norm.hip", "nd_linear.hip", "nd_linear_bf16.hip", "nd_linear_f16.hip"]
 
 # -ffp-contract=off: the samplers compare single IEEE float operations bit for bit with
 # the CPU checker.  The target-feature pair switches packed-fp32 code generation off.

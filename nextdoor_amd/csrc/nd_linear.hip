@@ -1,0 +1,455 @@
+// C entries of linear maps and feed-forward parts: checks, workspaces, and which kernels run (nd_linear.hpp).
+#include "../../include/nextdoor_amd.h"
+
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "nd_errors.hpp"
+#include "nd_linear.hpp"
+
+namespace nd {
+
+// ---- float16: what dz is held times ----------------------------------------------------------------------------
+
+// The largest finite |dout| of a share of the rows.
+__global__ __launch_bounds__(256) void largest_kernel(const char* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* parts) {
+  __shared__ float wave[4];
+  float most = 0.f;
+  const int groups = columns / 8;
+  const int64_t n = rows * groups;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const u32x4 w = *(const u32x4*)(dout + i / groups * row_bytes + i % groups * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = fabsf(unpack_low<_Float16>(w[j])), hi = fabsf(unpack_high<_Float16>(w[j]));
+      most = fmaxf(most, fmaxf(lo < INFINITY ? lo : 0.f, hi < INFINITY ? hi : 0.f));
+    }
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(wave[0], wave[1]), fmaxf(wave[2], wave[3]));
+}
+// scale[0] = the power of two that takes the largest of all to between 1/2 and 1 (1, if that is 0), scale[1] = one over it.
+__global__ __launch_bounds__(64) void scale_kernel(const float* parts, int n, float* scale) {
+  float most = 0.f;
+  for (int i = threadIdx.x; i < n; i += 64) most = fmaxf(most, parts[i]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  if (threadIdx.x == 0) {
+    int power = 0;
+    if (most > 0.f) frexpf(most, &power);
+    scale[0] = ldexpf(1.f, -power);
+    scale[1] = ldexpf(1.f, power);
+  }
+}
+hipError_t launch_scale(const void* dout, int64_t dout_bytes, int64_t rows, int32_t columns, float* parts, float* scale, hipStream_t stream) {
+  const int64_t turns = (rows * (columns / 8) + 1023) / 1024;
+  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kLargestParts, turns));
+  largest_kernel<<<blocks, 256, 0, stream>>>((const char*)dout, dout_bytes, rows, columns, parts);
+  scale_kernel<<<1, 64, 0, stream>>>(parts, blocks, scale);
+  return hipGetLastError();
+}
+
+namespace {
+
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// ---- which tiles, and how many shares of a sum -------------------------------------------------------------------
+
+// An estimate of a product's time in us from its rounds of 64 places: what a workgroup takes for one, and beside them, with the
+// compute units full.
+struct ShapeCost {
+  int m, n, at_once;         // rows of C, columns of C, workgroups that the GPU holds at a time
+  double round, alone, once; // us: a round with all of them, a round where a compute unit has one only, everything else
+};
+constexpr ShapeCost kShapes[3] = {{256, 256, 256, 1.5, 1.5, 8.0}, {128, 128, 512, 0.95, 0.6, 4.0}, {64, 64, 768, 0.6, 0.35, 3.0}};
+constexpr int kMostShares = 128;
+
+LinearPlan plan_of(int64_t m, int64_t n, int64_t k, bool gated) {
+  const int64_t rounds = std::max<int64_t>(1, (k + 63) / 64), columns = gated ? 2 * n : n;
+  LinearPlan best = {0, 1, (int)(rounds * 64)};
+  double least = INFINITY;
+  for (int shape = 0; shape < 3; ++shape) {
+    const ShapeCost& c = kShapes[shape];
+    const int64_t tiles = ((m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
+    for (int64_t want = 1; want <= kMostShares; want = want < 4 ? want + 1 : want * 3 / 2) {
+      const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
+      if (shares != want && want > 1) continue;
+      const int64_t groups = tiles * shares;
+      const double turns = groups <= 256 ? 1 : ceil((double)groups / c.at_once);
+      double time = turns * (each * (groups <= 256 ? c.alone : c.round) + c.once);
+      if (shares > 1) time += 3.0 + (double)shares * m * columns * 8 / 4e6;
+      if (time < least) {
+        least = time;
+        best = {shape, (int)shares, (int)(each * 64)};
+      }
+    }
+  }
+  return best;
+}
+
+int64_t sums_bytes(const LinearPlan& p, int64_t m, int64_t columns) { return p.shares > 1 ? round_up(m * columns * 4 * p.shares, 256) : 0; }
+
+// Shares of the rows for the sums over them: workgroups of 64 columns, at least 64 rows to each, some thousand in all.
+int64_t row_shares(int64_t rows, int64_t columns) {
+  const int64_t across = (columns + 63) / 64;
+  return std::max<int64_t>(1, std::min<int64_t>({(rows + 63) / 64, std::max<int64_t>(1, 2048 / across), (int64_t)65535}));
+}
+
+// ---- calls --------------------------------------------------------------------------------------------------------
+
+struct Call {
+  const char* what;
+  bool bf16;
+  hipStream_t stream;
+  hipError_t error;
+  Call(const char* what_, int dtype, void* stream_) : what(what_), bf16(dtype == ND_BF16), stream((hipStream_t)stream_), error(hipSuccess) {}
+  void note(hipError_t e) {
+    if (error == hipSuccess) error = e;
+  }
+  void product(const LinearParams& a, Layout layout, After after, const LinearPlan& plan) {
+    if (a.m == 0 || a.n == 0) return;
+    note(bf16 ? launch_linear<__bf16>(a, layout, after, plan, stream) : launch_linear<_Float16>(a, layout, after, plan, stream));
+  }
+  // out rows of a matrix by rows
+  void forward(const LinearParams& a, After after, float* sums) {
+    if (a.m == 0) return;
+    if (a.m <= kFewRows) {
+      note(bf16 ? launch_few_rows<__bf16>(a, after, stream) : launch_few_rows<_Float16>(a, after, stream));
+      return;
+    }
+    LinearParams p = a;
+    p.sums = sums;
+    product(p, Layout::kRows, after, plan_of(a.m, a.n, a.k, after == After::kGated));
+  }
+  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums) {
+    const int64_t shares = row_shares(a.m, a.n);
+    note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, stream) : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, stream));
+  }
+  void column_join(const float* sums, int64_t rows, int64_t columns, const float* scale, void* out) {
+    const int64_t shares = row_shares(rows, columns);
+    note(bf16 ? launch_column_join<__bf16>(sums, shares, columns, scale, out, stream) : launch_column_join<_Float16>(sums, shares, columns, scale, out, stream));
+  }
+  // The sums of the rows of a matrix [rows][columns].
+  void column_sums(const void* matrix, int64_t row_bytes, int64_t rows, int32_t columns, const float* scale, float* sums, void* out) {
+    LinearParams p = {};
+    p.m = (int32_t)rows;
+    p.n = columns;
+    slope(p, matrix, row_bytes, sums);
+    column_join(sums, rows, columns, scale, out);
+  }
+  // dx [rows][dim] = dz weight;  dweight [out][dim] = dz^T x
+  void gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, const float* scale, void* dx, float* sums) {
+    LinearParams p = {};
+    p.p = weight;
+    p.p_bytes = (int64_t)dim * 2;
+    p.q = dz;
+    p.q_bytes = dz_bytes;
+    p.m = (int32_t)rows;
+    p.n = dim;
+    p.k = out;
+    p.scale = scale;
+    p.out = dx;
+    p.sums = sums;
+    product(p, Layout::kWeightColumns, After::kPlain, plan_of(rows, dim, out, false));
+  }
+  void gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, const float* scale,
+                          void* dweight, float* sums) {
+    LinearParams p = {};
+    p.p = x;
+    p.p_bytes = x_bytes;
+    p.q = dz;
+    p.q_bytes = dz_bytes;
+    p.m = out;
+    p.n = dim;
+    p.k = (int32_t)rows;
+    p.scale = scale;
+    p.out = dweight;
+    p.sums = sums;
+    product(p, Layout::kColumns, After::kPlain, plan_of(out, dim, rows, false));
+  }
+  int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
+};
+
+std::string number(int64_t v) { return std::to_string(v); }
+
+// Checks that both kinds of call share; an empty text if all is well.
+std::string refuse(int64_t rows, std::initializer_list<int64_t> dims, int dtype, int activation, std::initializer_list<int64_t> strides) {
+  if (dtype != ND_F16 && dtype != ND_BF16) return "16-bit types only (ND_F16, ND_BF16)";
+  if (rows < 0 || rows > ND_LINEAR_MAX_ROWS) return "between 0 and " + number(ND_LINEAR_MAX_ROWS) + " rows, " + number(rows) + " given";
+  for (const int64_t d : dims)
+    if (d < 8 || d > ND_LINEAR_MAX_DIM || d % 8 != 0)
+      return "sizes of vectors are multiples of 8 up to " + number(ND_LINEAR_MAX_DIM) + ", " + number(d) + " given";
+  if (activation < ND_NO_ACTIVATION || activation > ND_SILU) return "unknown activation " + number(activation);
+  for (const int64_t s : strides)
+    if (s < 0 || s > ND_LINEAR_MAX_ROW_STRIDE || s % 8 != 0)
+      return "rows lie a multiple of 8 elements apart, at most " + number(ND_LINEAR_MAX_ROW_STRIDE) + ", " + number(s) + " given";
+  return "";
+}
+
+struct Array {
+  const void* at;
+  bool needed;
+};
+std::string refuse(std::initializer_list<Array> arrays) {
+  for (const Array& a : arrays) {
+    if (a.needed && !a.at) return "null array";
+    if ((uintptr_t)a.at & 15) return "arrays are aligned to 16 bytes";
+  }
+  return "";
+}
+
+// Where the parts of a workspace lie.
+struct Layouter {
+  int64_t bytes = 0;
+  int64_t take(int64_t n) {
+    const int64_t at = bytes;
+    bytes += round_up(n, 256);
+    return at;
+  }
+};
+
+int64_t forward_sums(int64_t m, int64_t n, int64_t k, bool gated) {
+  return m <= kFewRows ? 0 : sums_bytes(plan_of(m, n, k, gated), m, gated ? 2 * n : n);
+}
+
+// ---- linear ---------------------------------------------------------------------------------------------------------
+
+struct LinearWork {
+  int64_t dz, products, rows, parts, scale, bytes;
+};
+LinearWork work_of(const nd_linear* a, bool backward) {
+  LinearWork w = {};
+  Layouter l;
+  if (!backward) {
+    w.products = l.take(forward_sums(a->rows, a->out_dim, a->dim, false));
+  } else {
+    const bool active = a->activation != ND_NO_ACTIVATION;
+    w.dz = l.take(active ? a->rows * a->out_dim * 2 : 0);
+    w.products = l.take(std::max(a->dx ? sums_bytes(plan_of(a->rows, a->dim, a->out_dim, false), a->rows, a->dim) : 0,
+                                 a->dweight ? sums_bytes(plan_of(a->out_dim, a->dim, a->rows, false), a->out_dim, a->dim) : 0));
+    w.rows = l.take(a->dbias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
+    const bool scaled = active && a->dtype == ND_F16;
+    w.parts = l.take(scaled ? kLargestParts * 4 : 0);
+    w.scale = l.take(scaled ? 8 : 0);
+  }
+  w.bytes = l.bytes;
+  return w;
+}
+
+std::string refuse(const nd_linear* a) {
+  if (!a) return "null argument";
+  return refuse(a->rows, {a->dim, a->out_dim}, a->dtype, a->activation, {a->x_row, a->residual_row, a->dout_row});
+}
+
+int run_linear(const nd_linear* a, bool backward, void* stream) {
+  std::string why = refuse(a);
+  if (!why.empty()) return fail("linear: " + why);
+  const bool some = a->rows > 0, active = a->activation != ND_NO_ACTIVATION;
+  if (!backward)
+    why = refuse({{a->x, some}, {a->weight, some}, {a->bias, false}, {a->residual, false}, {a->out, some}, {a->z, false}});
+  else
+    why = refuse({{a->x, some && a->dweight}, {a->weight, some && a->dx}, {a->dout, some}, {a->z, some && active}, {a->dx, false}, {a->dweight, false}, {a->dbias, false}});
+  if (!why.empty()) return fail("linear: " + why);
+  const LinearWork w = work_of(a, backward);
+  if (w.bytes > 0 && (a->workspace_bytes < w.bytes || !a->workspace || ((uintptr_t)a->workspace & 15)))
+    return fail("linear: the workspace has " + number(a->workspace ? a->workspace_bytes : 0) + " bytes, " + number(w.bytes) + " needed, aligned to 16");
+  char* work = (char*)a->workspace;
+  float* sums = (float*)(work + w.products);
+  Call call("linear", a->dtype, stream);
+  if (!backward) {
+    LinearParams p = {};
+    p.p = a->weight;
+    p.p_bytes = (int64_t)a->dim * 2;
+    p.q = a->x;
+    p.q_bytes = a->x_row * 2;
+    p.m = (int32_t)a->rows;
+    p.n = a->out_dim;
+    p.k = a->dim;
+    p.activation = a->activation;
+    p.bias = a->bias;
+    p.residual = a->residual;
+    p.residual_bytes = a->residual_row * 2;
+    p.out = a->out;
+    p.z = a->z;
+    call.forward(p, After::kForward, sums);
+    return call.done();
+  }
+  const void* dz = a->dout;
+  int64_t dz_bytes = a->dout_row * 2;
+  const float* scale = nullptr;
+  float* rows = (float*)(work + w.rows);
+  if (active && (a->dx || a->dweight || a->dbias)) {
+    if (!call.bf16) {
+      scale = (const float*)(work + w.scale);
+      call.note(launch_scale(a->dout, dz_bytes, a->rows, a->out_dim, (float*)(work + w.parts), (float*)(work + w.scale), call.stream));
+    }
+    LinearParams p = {};
+    p.m = (int32_t)a->rows;
+    p.n = a->out_dim;
+    p.activation = a->activation;
+    p.z = a->z;
+    p.scale = scale;
+    p.out = work + w.dz;
+    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr);
+    if (a->dbias) call.column_join(rows, a->rows, a->out_dim, nullptr, a->dbias);
+    dz = work + w.dz;
+    dz_bytes = (int64_t)a->out_dim * 2;
+  } else if (a->dbias) {
+    call.column_sums(a->dout, dz_bytes, a->rows, a->out_dim, nullptr, rows, a->dbias);
+  }
+  if (a->dx) call.gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, scale, a->dx, sums);
+  if (a->dweight) call.gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, scale, a->dweight, sums);
+  return call.done();
+}
+
+// ---- mlp --------------------------------------------------------------------------------------------------------------
+
+struct MlpWork {
+  int64_t dz, products, rows, parts, scale, bytes;
+};
+MlpWork work_of(const nd_mlp* a, bool backward) {
+  MlpWork w = {};
+  Layouter l;
+  const int64_t wide = (int64_t)a->inner * (a->gated ? 2 : 1);
+  if (!backward) {
+    w.products = l.take(std::max(forward_sums(a->rows, a->inner, a->dim, a->gated), forward_sums(a->rows, a->out_dim, a->inner, false)));
+  } else {
+    const bool first = a->dx || a->dup || a->dup_bias;
+    w.dz = l.take(first ? a->rows * wide * 2 : 0);
+    int64_t most = 0;
+    auto product = [&](bool wanted, int64_t m, int64_t n, int64_t k) {
+      if (wanted) most = std::max(most, sums_bytes(plan_of(m, n, k, false), m, n));
+    };
+    product(first, a->rows, a->inner, a->out_dim);
+    product(a->dx, a->rows, a->dim, wide);
+    product(a->dup, wide, a->dim, a->rows);
+    product(a->ddown, a->out_dim, a->inner, a->rows);
+    w.products = l.take(most);
+    w.rows = l.take(std::max(a->dup_bias ? row_shares(a->rows, wide) * wide * 4 : 0, a->ddown_bias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0));
+    const bool scaled = first && a->dtype == ND_F16;
+    w.parts = l.take(scaled ? kLargestParts * 4 : 0);
+    w.scale = l.take(scaled ? 8 : 0);
+  }
+  w.bytes = l.bytes;
+  return w;
+}
+
+std::string refuse(const nd_mlp* a) {
+  if (!a) return "null argument";
+  std::string why = refuse(a->rows, {a->dim, a->inner, a->out_dim}, a->dtype, a->activation, {a->x_row, a->residual_row, a->dout_row});
+  if (why.empty() && a->gated && a->inner > ND_LINEAR_MAX_DIM / 2) why = "gated: at most " + number(ND_LINEAR_MAX_DIM / 2) + " inner places";
+  return why;
+}
+
+int run_mlp(const nd_mlp* a, bool backward, void* stream) {
+  std::string why = refuse(a);
+  if (!why.empty()) return fail("mlp: " + why);
+  const bool some = a->rows > 0, first = a->dx || a->dup || a->dup_bias, slope = a->gated || a->activation != ND_NO_ACTIVATION;
+  if (!backward)
+    why = refuse({{a->x, some}, {a->up, some}, {a->down, some}, {a->up_bias, false}, {a->down_bias, false}, {a->residual, false}, {a->out, some}, {a->z, false}, {a->h, some}});
+  else
+    why = refuse({{a->x, some && a->dup}, {a->up, some && a->dx}, {a->down, some && first}, {a->z, some && first && slope}, {a->h, some && a->ddown},
+                  {a->dout, some}, {a->dx, false}, {a->dup, false}, {a->dup_bias, false}, {a->ddown, false}, {a->ddown_bias, false}});
+  if (!why.empty()) return fail("mlp: " + why);
+  const MlpWork w = work_of(a, backward);
+  if (w.bytes > 0 && (a->workspace_bytes < w.bytes || !a->workspace || ((uintptr_t)a->workspace & 15)))
+    return fail("mlp: the workspace has " + number(a->workspace ? a->workspace_bytes : 0) + " bytes, " + number(w.bytes) + " needed, aligned to 16");
+  char* work = (char*)a->workspace;
+  float* sums = (float*)(work + w.products);
+  Call call("mlp", a->dtype, stream);
+  const int32_t wide = a->inner * (a->gated ? 2 : 1);
+  const int64_t inner_bytes = (int64_t)a->inner * 2, wide_bytes = (int64_t)wide * 2;
+  if (!backward) {
+    LinearParams p = {};
+    p.p = a->up;
+    p.p_bytes = (int64_t)a->dim * 2;
+    p.q = a->x;
+    p.q_bytes = a->x_row * 2;
+    p.m = (int32_t)a->rows;
+    p.n = a->inner;
+    p.k = a->dim;
+    p.activation = a->activation;
+    p.bias = a->up_bias;
+    p.out = a->h;
+    p.z = a->z;
+    call.forward(p, a->gated ? After::kGated : After::kForward, sums);
+    LinearParams r = {};
+    r.p = a->down;
+    r.p_bytes = inner_bytes;
+    r.q = a->h;
+    r.q_bytes = inner_bytes;
+    r.m = (int32_t)a->rows;
+    r.n = a->out_dim;
+    r.k = a->inner;
+    r.bias = a->down_bias;
+    r.residual = a->residual;
+    r.residual_bytes = a->residual_row * 2;
+    r.out = a->out;
+    call.forward(r, After::kForward, sums);
+    return call.done();
+  }
+  float* rows = (float*)(work + w.rows);
+  const int64_t dout_bytes = a->dout_row * 2;
+  if (a->ddown_bias) call.column_sums(a->dout, dout_bytes, a->rows, a->out_dim, nullptr, rows, a->ddown_bias);
+  if (a->ddown) call.gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, sums);
+  if (!first) return call.done();
+  const float* scale = nullptr;
+  if (!call.bf16) {
+    scale = (const float*)(work + w.scale);
+    call.note(launch_scale(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.parts), (float*)(work + w.scale), call.stream));
+  }
+  LinearParams p = {};
+  p.p = a->down;
+  p.p_bytes = inner_bytes;
+  p.q = a->dout;
+  p.q_bytes = dout_bytes;
+  p.m = (int32_t)a->rows;
+  p.n = a->inner;
+  p.k = a->out_dim;
+  p.activation = a->activation;
+  p.gated = a->gated;
+  p.z = slope ? a->z : nullptr;
+  p.out = work + w.dz;
+  p.sums = sums;
+  p.scale = scale;
+  call.product(p, Layout::kWeightColumns, After::kSlope, plan_of(a->rows, a->inner, a->out_dim, false));
+  const char* dz = work + w.dz;
+  if (a->dup_bias) call.column_sums(dz, wide_bytes, a->rows, wide, scale, rows, a->dup_bias);
+  if (a->dx) call.gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, scale, a->dx, sums);
+  if (a->dup) call.gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, scale, a->dup, sums);
+  return call.done();
+}
+
+}  // namespace
+}  // namespace nd
+
+extern "C" {
+
+int64_t nd_linear_workspace(const nd_linear* a, int backward) {
+  if (!nd::refuse(a).empty()) return -1;
+  return nd::work_of(a, backward != 0).bytes;
+}
+int nd_linear_forward(const nd_linear* a, void* stream) {
+  return nd::guarded([&]() -> int { return nd::run_linear(a, false, stream); });
+}
+int nd_linear_backward(const nd_linear* a, void* stream) {
+  return nd::guarded([&]() -> int { return nd::run_linear(a, true, stream); });
+}
+
+int64_t nd_mlp_workspace(const nd_mlp* a, int backward) {
+  if (!nd::refuse(a).empty()) return -1;
+  return nd::work_of(a, backward != 0).bytes;
+}
+int nd_mlp_forward(const nd_mlp* a, void* stream) {
+  return nd::guarded([&]() -> int { return nd::run_mlp(a, false, stream); });
+}
+int nd_mlp_backward(const nd_mlp* a, void* stream) {
+  return nd::guarded([&]() -> int { return nd::run_mlp(a, true, stream); });
+}
+
+}  // extern "C"

@@ -1,0 +1,363 @@
+// Linear maps with what follows them (C entries: nd_linear_*, nd_mlp_*): what their kernels share.
+//
+//   linear:  z = x W^T + b,  y = a(z) + r;     dz = dy a'(z),  dx = dz W,  dW = dz^T x,  db = sum of the rows of dz
+//   mlp:     [g, u] = x U^T + b,  h = a(g) u (gated) or a(g),  y = h D^T + d + r
+//            dh = dy D,  dg = dh u a'(g),  du = dh a(g),  then as above with dz = [dg, du]
+//
+// Three products of the same tiles (nd_product.hpp): both operands by rows (forward), the weights by columns (gradient of x),
+// both by columns (gradient of the weights).  What follows a product is done to its results before they leave the registers.
+// Sums are held in 32 bits; z, h and dz, which the next product or the backward pass reads, are rounded to 16 bits once, as
+// the results are.  float16: dz is held times a power of two that takes max |dy| to between 1/2 and 1, so that the small
+// gradients of a mean over many rows are not lost below 2^-14; what is made of it is divided by that in 32 bits.
+#pragma once
+
+#include "nd_activation.hpp"
+#include "nd_product.hpp"
+
+namespace nd {
+
+enum class After { kSums, kForward, kGated, kPlain, kSlope };
+
+struct LinearParams {
+  // C [m][n], sums over k; gated: n counts pairs, and P has 2 n rows
+  const void *p, *q;
+  int64_t p_bytes, q_bytes;  // of a row
+  int32_t m, n, k;
+  int32_t activation, gated;
+  const void *bias, *residual;
+  int64_t residual_bytes;  // of a row
+  void* out;
+  void* z;  // forward: written unless null; backward: read.  [m][n], gated [m][2 n]
+  const float* scale;  // null: 1; kSlope: the sums are multiplied with scale[0]; kPlain: with scale[1], one over it
+  // shares of the sum: share s has places s * share .. and leaves [m][width] values in 32 bits
+  float* sums;
+  int32_t shares, share, width;
+};
+
+// What follows the sums v (gated: and u) of columns c .. c + 7 of a row.
+template <class T, After AFTER>
+__device__ __forceinline__ void finish(const LinearParams& a, int row, int c, float (&v)[8], float (&u)[8]) {
+  auto unpack = [](const u32x4& w, float(&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = unpack_low<T>(w[i]);
+      x[2 * i + 1] = unpack_high<T>(w[i]);
+    }
+  };
+  auto pack = [](const float(&x)[8]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(x[2 * i], x[2 * i + 1]);
+    return w;
+  };
+  auto at = [&](const void* matrix, int64_t row_bytes, int column) { return (u32x4*)((char*)matrix + row * row_bytes + (int64_t)column * 2); };
+  constexpr bool kForward = AFTER == After::kForward || AFTER == After::kGated;
+  const int64_t n_bytes = (int64_t)a.n * 2;
+  float x[8];
+  if (!kForward && a.scale) {
+    const float factor = a.scale[AFTER == After::kPlain];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= factor;
+  }
+  if (kForward && a.bias) {
+    unpack(*at(a.bias, 0, c), x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += x[i];
+    if (AFTER == After::kGated) {
+      unpack(*at(a.bias, 0, a.n + c), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] += x[i];
+    }
+  }
+  if (AFTER == After::kForward) {
+    if (a.z) *at(a.z, n_bytes, c) = pack(v);
+    activate(a.activation, v);
+    if (a.residual) {
+      unpack(*at(a.residual, a.residual_bytes, c), x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += x[i];
+    }
+  } else if (AFTER == After::kGated) {
+    if (a.z) {
+      *at(a.z, 2 * n_bytes, c) = pack(v);
+      *at(a.z, 2 * n_bytes, a.n + c) = pack(u);
+    }
+    activate(a.activation, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= u[i];
+  } else if (AFTER == After::kSlope && a.z) {
+    float slope[8];
+    unpack(*at(a.z, a.gated ? 2 * n_bytes : n_bytes, c), x);
+    activate_with_slope(a.activation, x, slope);
+    if (a.gated) {
+      unpack(*at(a.z, 2 * n_bytes, a.n + c), u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] *= v[i];
+        v[i] *= u[i] * slope[i];
+      }
+      *at(a.out, 2 * n_bytes, a.n + c) = pack(x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= slope[i];
+    }
+  }
+  *at(a.out, AFTER == After::kSlope && a.gated ? 2 * n_bytes : n_bytes, c) = pack(v);
+}
+
+// ---- a tile of C to a workgroup ---------------------------------------------------------------------------
+
+// 256 x 256, eight waves with 4 x 2 results each, alone on a compute unit; 128 x 128 and 64 x 64, two and three of which share
+// one.
+using Large = product::Shape<2, 4, 4, 2, 64, 2, 4, 16, 2>;
+using Medium = product::Shape<2, 2, 2, 2, 64, 2, 4, 8, 2>;
+using Small = product::Shape<1, 2, 2, 1, 64, 3, 2, 4, 2>;
+
+enum class Layout { kRows, kWeightColumns, kColumns };  // both operands by rows; P by columns; both by columns
+
+template <class T, class S, Layout LAYOUT, After AFTER>
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(LinearParams a, int m_tiles, int n_tiles) {
+  constexpr bool kGated = AFTER == After::kGated;
+  constexpr int kColumns = kGated ? S::kTileM / 2 : S::kTileM;  // of C to a tile
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  __shared__ u32x4 tiles[S::kTileChunks];
+  // Bands of eight tiles of rows, in a band column after column: the tiles that a die works on at a time (32 or more) share few rows
+  // of both operands.  Shares of a sum one after another.
+  uint32_t block = block_by_die();
+  const int per_share = m_tiles * n_tiles, share = uniform(block / per_share);
+  block -= share * per_share;
+  const int band = uniform(block / (8 * n_tiles)), in_band = block - band * 8 * n_tiles, width = min(8, m_tiles - band * 8);
+  const int column0 = uniform(in_band / width) * kColumns, row0 = (band * 8 + uniform(in_band % width)) * S::kTileN;
+  const int place0 = share * a.share, place_end = AFTER == After::kSums && share + 1 < a.shares ? place0 + a.share : a.k;
+  f32x16 acc[S::kM][S::kN];
+  if constexpr (LAYOUT == Layout::kRows) {
+    using P = product::ByRows<S::kTileM, S::kDepth, S::kThreads, kGated>;
+    using Q = product::ByRows<S::kTileN, S::kDepth, S::kThreads>;
+    product::multiply<T, S>(acc, P(a.p, a.p_bytes, column0, a.n, place_end, a.n), Q(a.q, a.q_bytes, row0, a.m, place_end), place0, place_end, tiles);
+  } else if constexpr (LAYOUT == Layout::kWeightColumns) {
+    using P = product::ByColumns<S::kTileM, S::kDepth, S::kThreads>;
+    using Q = product::ByRows<S::kTileN, S::kDepth, S::kThreads>;
+    product::multiply<T, S>(acc, P(a.p, a.p_bytes, column0, a.n, place_end), Q(a.q, a.q_bytes, row0, a.m, place_end), place0, place_end, tiles);
+  } else {
+    using P = product::ByColumns<S::kTileM, S::kDepth, S::kThreads>;
+    using Q = product::ByColumns<S::kTileN, S::kDepth, S::kThreads>;
+    product::multiply<T, S>(acc, P(a.p, a.p_bytes, column0, a.n, place_end), Q(a.q, a.q_bytes, row0, a.m, place_end), place0, place_end, tiles);
+  }
+  product::meet();
+  // ---- the results: wave's rows from wave_row0 on, columns from wave_column0 on
+  constexpr int kWaveChunks = S::kTileChunks / (S::kThreads / 64);
+  u32x4* mine = tiles + wave * kWaveChunks;
+  const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN, wave_column0 = column0 + wave / S::kWavesN * (kColumns / S::kWavesM);
+  const int h = lane >> 5;
+  const int64_t n_bytes = (int64_t)a.n * 2;
+  if constexpr (AFTER == After::kSums) {
+    // blocks of 32 columns, 128 bytes of a row
+    float* sums = a.sums + (int64_t)share * a.m * a.width;
+#pragma unroll
+    for (int j = 0; j < S::kN; ++j)
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = lane & 31;
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+          *(f32x4*)(mine + r * 8 + ((2 * q + h) ^ (r & 7))) = v;
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int r = t * 8 + lane / 8, c = lane % 8, row = wave_row0 + 32 * j + r, column = wave_column0 + 32 * i + 4 * c;
+          const f32x4 v = *(const f32x4*)(mine + r * 8 + (c ^ (r & 7)));
+          if (row < a.m && column < a.n) *(f32x4*)(sums + (int64_t)row * a.width + column) = v;
+        }
+        asm volatile("" ::: "memory");
+      }
+    return;
+  }
+  // four values of a result's column (a lane's row, columns 8 q + 4 h .. of block i)
+  auto four = [&](const f32x16& c, int q, float(&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = c[4 * q + e];
+  };
+  auto unpack = [](u32x2 w, float(&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[2 * e] = unpack_low<T>(w[e]);
+      v[2 * e + 1] = unpack_high<T>(w[e]);
+    }
+  };
+  auto pack = [](const float(&v)[4]) {
+    u32x2 w;
+    w[0] = pack_pair<T>(v[0], v[1]);
+    w[1] = pack_pair<T>(v[2], v[3]);
+    return w;
+  };
+  auto bias_of = [&](int column, int end, int past) {  // (columns past the end have no bias, and are not stored)
+    u32x2 w = {0, 0};
+    if (a.bias && column < end) w = *(const u32x2*)((const char*)a.bias + (int64_t)(past + column) * 2);
+    return w;
+  };
+  if constexpr (AFTER == After::kGated) {
+    using Out = product::Region<2 * S::kM>;
+    const Out gates{mine}, values{mine + Out::kSize}, products{mine + 2 * Out::kSize};
+    static_assert(3 * Out::kSize <= kWaveChunks, "");
+#pragma unroll
+    for (int j = 0; j < S::kN; ++j) {
+      const int at = wave_row0 + 32 * j;
+#pragma unroll
+      for (int i = 0; i < S::kM / 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int column = wave_column0 + 32 * i + 8 * q + 4 * h;
+          float g[4], u[4], b[4];
+          four(acc[2 * i][j], q, g);
+          four(acc[2 * i + 1][j], q, u);
+          unpack(bias_of(column, a.n, 0), b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[e] += b[e];
+          unpack(bias_of(column, a.n, a.n), b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] += b[e];
+          if (a.z) {
+            gates.piece(4 * i + q, lane) = pack(g);
+            values.piece(4 * i + q, lane) = pack(u);
+          }
+          activate(a.activation, g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) g[e] *= u[e];
+          products.piece(4 * i + q, lane) = pack(g);
+        }
+      if (a.z) {
+        gates.put(a.z, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        values.put((char*)a.z + n_bytes, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
+      }
+      products.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
+    }
+  } else {
+    using Out = product::Region<4 * S::kM>;
+    constexpr int kRegions = kWaveChunks / Out::kSize;
+    static_assert(kRegions >= 2 && kRegions >= S::kN, "");
+    const bool residual = AFTER == After::kForward && a.residual, keep = AFTER == After::kForward && a.z;
+    const bool slope = AFTER == After::kSlope && a.z, gated = slope && a.gated;  // (without a z, dz is what the product gives)
+    // Regions of rows j: what is read, and goes out again in the same place; with a second matrix one region further.  All
+    // rows are asked for at once where there are regions enough.
+    const int step = keep || gated ? 2 : 1;
+    const bool ahead = step * S::kN <= kRegions;
+    const int64_t z_bytes = gated ? 2 * n_bytes : n_bytes;
+    auto bring = [&](int j) {
+      const Out first{mine + (ahead ? step * j : 0) * Out::kSize}, second{first.at + Out::kSize};
+      const int at = wave_row0 + 32 * j;
+      if (residual) first.bring(a.residual, a.residual_bytes, at, a.m, wave_column0, a.n, lane);
+      if (slope) first.bring(a.z, z_bytes, at, a.m, wave_column0, a.n, lane);
+      if (gated) second.bring((const char*)a.z + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
+    };
+    const float factor = AFTER != After::kForward && a.scale ? a.scale[AFTER == After::kPlain] : 1.f;
+    if (ahead) {
+#pragma unroll
+      for (int j = 0; j < S::kN; ++j) bring(j);
+      if (residual || slope) product::wait_for_loads<0>();
+    }
+#pragma unroll
+    for (int j = 0; j < S::kN; ++j) {
+      const int at = wave_row0 + 32 * j;
+      if (!ahead) {
+        bring(j);
+        if (residual || slope) product::wait_for_loads<0>();
+      }
+      const Out first{mine + (ahead ? step * j : 0) * Out::kSize}, second{first.at + Out::kSize};
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int column = wave_column0 + 32 * i + 8 * q + 4 * h;
+          float v[4], x[4];
+          four(acc[i][j], q, v);
+          if (AFTER != After::kForward) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= factor;
+          }
+          if (AFTER == After::kForward) {
+            unpack(bias_of(column, a.n, 0), x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += x[e];
+            if (keep) second.piece(4 * i + q, lane) = pack(v);
+            activate(a.activation, v);
+            if (residual) {
+              unpack(first.piece(4 * i + q, lane), x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] += x[e];
+            }
+          } else if (slope) {
+            float s[4], u[4];
+            unpack(first.piece(4 * i + q, lane), x);
+            activate_with_slope(a.activation, x, s);
+            if (gated) {
+              unpack(second.piece(4 * i + q, lane), u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x[e] *= v[e];
+                s[e] *= u[e];
+              }
+              second.piece(4 * i + q, lane) = pack(x);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= s[e];
+          }
+          first.piece(4 * i + q, lane) = pack(v);
+        }
+      if (keep) second.put(a.z, n_bytes, at, a.m, wave_column0, a.n, lane);
+      if (gated) second.put((char*)a.out + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
+      first.put(a.out, z_bytes, at, a.m, wave_column0, a.n, lane);
+    }
+  }
+}
+
+// The shares' sums added up, and what follows: eight columns of a row to a lane.
+template <class T, After AFTER>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearParams a) {
+  const int64_t groups = a.n / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= groups * a.m) return;
+  const int row = (int)(at / groups), c = (int)(at % groups) * 8;
+  float v[8], u[8];
+  auto total = [&](int column, float(&x)[8]) {
+    const float* from = a.sums + (int64_t)row * a.width + column;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    for (int s = 0; s < a.shares; ++s, from += (int64_t)a.m * a.width) {
+      const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] += lo[i];
+        x[4 + i] += hi[i];
+      }
+    }
+  };
+  total(c, v);
+  if (AFTER == After::kGated) total(a.n + c, u);
+  finish<T, AFTER>(a, row, c, v, u);
+}
+
+// ---- launches (nd_linear_types.hpp, compiled for each type by itself) -----------------------------------------
+
+struct LinearPlan {
+  int shape;  // 0 large, 1 medium, 2 small
+  int shares, share;
+};
+template <class T>
+hipError_t launch_linear(const LinearParams& a, Layout layout, After after, const LinearPlan& plan, hipStream_t stream);
+template <class T>
+hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
+// dz = dout a'(z) times scale[0], if there is a z, and sums of its rows (times 1).
+template <class T>
+hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, hipStream_t stream);
+// scale: null, or as above: the sums are multiplied with scale[1].
+template <class T>
+hipError_t launch_column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out, hipStream_t stream);
+constexpr int kLargestParts = 512;
+hipError_t launch_scale(const void* dout, int64_t dout_bytes, int64_t rows, int32_t columns, float* parts, float* scale, hipStream_t stream);
+
+constexpr int kFewRows = 64;  // at most: a kernel of its own, which reads the weights once and keeps a sum in many waves
+
+}  // namespace nd

@@ -1,0 +1,220 @@
+// The kernels of nd_linear.hpp and the two that go with them, for one type of values.
+#pragma once
+
+#include <algorithm>
+
+#include "nd_column_sums.hpp"
+#include "nd_linear.hpp"
+
+namespace nd {
+
+// ---- few rows: the weights are what there is to read -----------------------------------------------------------
+
+__device__ __forceinline__ f32x4 product_16x16x32(u32x4 a, u32x4 b, f32x4 c, __bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 product_16x16x32(u32x4 a, u32x4 b, f32x4 c, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// A workgroup makes 16 columns of C (gated: 16 pairs) for up to 16 ROW_BLOCKS rows.  Its waves share out the sum, 64 places at a
+// time, and read the weights straight to registers: lane l has row l & 15, places 8 (l >> 4) .. + 7 of 32, so two products use
+// whole lines of 128 bytes.  x is the same for all workgroups and comes from the caches.
+template <class T, int ROW_BLOCKS, After AFTER, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinearParams a) {
+  constexpr int kSides = AFTER == After::kGated ? 2 : 1, kAhead = 4;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), column0 = blockIdx.x * 16;
+  __shared__ float part[WAVES][kSides * ROW_BLOCKS][16][17];
+  f32x4 sum[kSides][ROW_BLOCKS];
+#pragma unroll
+  for (int s = 0; s < kSides; ++s)
+#pragma unroll
+    for (int b = 0; b < ROW_BLOCKS; ++b) sum[s][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const char *weight[kSides], *row[ROW_BLOCKS];
+  const int own = (lane >> 4) * 16;  // bytes into 64 of a row
+#pragma unroll
+  for (int s = 0; s < kSides; ++s) weight[s] = (const char*)a.p + (int64_t)(s * a.n + min(column0 + (lane & 15), a.n - 1)) * a.p_bytes + own;
+#pragma unroll
+  for (int b = 0; b < ROW_BLOCKS; ++b) row[b] = (const char*)a.q + (int64_t)min(16 * b + (lane & 15), a.m - 1) * a.q_bytes + own;
+  const int bytes = a.k * 2;
+  // slices of 32 places: wave w has pairs of them w, w + WAVES, ...
+  auto get = [&](const char* from, int at) {
+    u32x4 v = {0, 0, 0, 0};
+    if (at + own < bytes) v = *(const u32x4*)(from + at);
+    return v;
+  };
+  for (int base = wave * 128; base < bytes; base += 128 * WAVES * (kAhead / 2)) {
+    u32x4 w[kAhead][kSides], x[kAhead][ROW_BLOCKS];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) {
+      const int at = base + (t / 2) * 128 * WAVES + (t & 1) * 64;
+#pragma unroll
+      for (int s = 0; s < kSides; ++s) w[t][s] = get(weight[s], at);
+#pragma unroll
+      for (int b = 0; b < ROW_BLOCKS; ++b) x[t][b] = get(row[b], at);
+    }
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t)
+#pragma unroll
+      for (int s = 0; s < kSides; ++s)
+#pragma unroll
+        for (int b = 0; b < ROW_BLOCKS; ++b) sum[s][b] = product_16x16x32(w[t][s], x[t][b], sum[s][b], T());
+  }
+  // lane: row l & 15, columns 4 (l >> 4) .. + 3
+#pragma unroll
+  for (int s = 0; s < kSides; ++s)
+#pragma unroll
+    for (int b = 0; b < ROW_BLOCKS; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave][s * ROW_BLOCKS + b][lane & 15][4 * (lane >> 4) + e] = sum[s][b][e];
+  __syncthreads();
+  for (int t = threadIdx.x; t < 32 * ROW_BLOCKS; t += 64 * WAVES) {
+    const int r = t >> 1, c = (t & 1) * 8;
+    if (r >= a.m || column0 + c >= a.n) continue;
+    float v[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = 0.f;
+      for (int w = 0; w < WAVES; ++w) v[e] += part[w][r >> 4][r & 15][c + e];
+      if (kSides == 2) {
+        u[e] = 0.f;
+        for (int w = 0; w < WAVES; ++w) u[e] += part[w][ROW_BLOCKS * (kSides - 1) + (r >> 4)][r & 15][c + e];
+      }
+    }
+    finish<T, AFTER>(a, r, column0 + c, v, u);
+  }
+}
+
+template <class T, After AFTER>
+hipError_t launch_few_rows_of(const LinearParams& a, hipStream_t stream) {
+  const dim3 grid((a.n + 15) / 16);
+  if (a.m <= 16) few_rows_kernel<T, 1, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  else if (a.m <= 32) few_rows_kernel<T, 2, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  else few_rows_kernel<T, 4, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  return hipGetLastError();
+}
+template <class T>
+hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream) {
+  return after == After::kGated ? launch_few_rows_of<T, After::kGated>(a, stream) : launch_few_rows_of<T, After::kForward>(a, stream);
+}
+
+// ---- dz = dy a'(z) of a linear map, and the sums of the rows of dz ------------------------------------------------
+
+constexpr int kSlopeColumns = 64;  // to a workgroup: 8 lanes of 8 values, 32 rows at a time
+
+// a.z null: dz is dy, and only its sums are wanted.  Bound by memory.
+template <class T>
+__global__ __launch_bounds__(256) void slope_kernel(LinearParams a, const void* dout, int64_t dout_bytes, float* sums, int64_t rows_per_share) {
+  __shared__ float part[32][kSlopeColumns + 4];
+  const int c = blockIdx.x * kSlopeColumns + (threadIdx.x & 7) * 8, r0 = threadIdx.x >> 3;
+  float total[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total[i] = 0.f;
+  const float factor = a.scale ? a.scale[0] : 1.f;
+  if (c < a.n) {
+    const int64_t begin = blockIdx.y * rows_per_share, end = min(begin + rows_per_share, (int64_t)a.m);
+    for (int64_t row = begin + r0; row < end; row += 32) {
+      u32x4 w = *(const u32x4*)((const char*)dout + row * dout_bytes + (int64_t)c * 2);
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d[2 * i] = unpack_low<T>(w[i]);
+        d[2 * i + 1] = unpack_high<T>(w[i]);
+      }
+      if (a.z) {
+        // (the sums are of dz as it is, not as it is held)
+        const u32x4 wz = *(const u32x4*)((const char*)a.z + (row * a.n + c) * 2);
+        float z[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          z[2 * i] = unpack_low<T>(wz[i]);
+          z[2 * i + 1] = unpack_high<T>(wz[i]);
+        }
+        activate_with_slope(a.activation, z, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= s[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(d[2 * i] * factor, d[2 * i + 1] * factor);
+        *(u32x4*)((char*)a.out + (row * a.n + c) * 2) = w;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) total[i] += d[i];
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[r0][(threadIdx.x & 7) * 8 + i] = total[i];
+  __syncthreads();
+  const int column = blockIdx.x * kSlopeColumns + threadIdx.x;
+  if (threadIdx.x < kSlopeColumns && column < a.n) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) sum += part[r][threadIdx.x];
+    sums[(int64_t)blockIdx.y * a.n + column] = sum;
+  }
+}
+
+template <class T>
+hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, hipStream_t stream) {
+  const int64_t rows_per_share = (a.m + shares - 1) / shares;
+  slope_kernel<T><<<dim3((a.n + kSlopeColumns - 1) / kSlopeColumns, (uint32_t)shares), 256, 0, stream>>>(a, dout, dout_bytes, sums, rows_per_share);
+  return hipGetLastError();
+}
+template <class T>
+hipError_t launch_column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out, hipStream_t stream) {
+  return column_join<T>(sums, shares, columns, scale ? scale + 1 : nullptr, out, columns, nullptr, stream);
+}
+
+// ---- tiles ----------------------------------------------------------------------------------------------------
+
+template <class T, class S, Layout LAYOUT, After AFTER>
+hipError_t launch_tiles(const LinearParams& a, int shares, hipStream_t stream) {
+  const int columns = AFTER == After::kGated ? S::kTileM / 2 : S::kTileM;
+  const int m_tiles = (a.m + S::kTileN - 1) / S::kTileN, n_tiles = (a.n + columns - 1) / columns;
+  if ((int64_t)m_tiles * n_tiles * shares * S::kThreads >> 32) return hipErrorInvalidConfiguration;  // (more than one launch holds)
+  linear_kernel<T, S, LAYOUT, AFTER><<<dim3((uint32_t)m_tiles * n_tiles * shares), S::kThreads, 0, stream>>>(a, m_tiles, n_tiles);
+  return hipGetLastError();
+}
+template <class T, Layout LAYOUT, After AFTER>
+hipError_t launch_shape(const LinearParams& a, int shape, int shares, hipStream_t stream) {
+  if (shape == 0) return launch_tiles<T, Large, LAYOUT, AFTER>(a, shares, stream);
+  if (shape == 1) return launch_tiles<T, Medium, LAYOUT, AFTER>(a, shares, stream);
+  return launch_tiles<T, Small, LAYOUT, AFTER>(a, shares, stream);
+}
+template <class T, After AFTER>
+hipError_t launch_join(const LinearParams& a, hipStream_t stream) {
+  const int64_t lanes = (int64_t)a.m * (a.n / 8);
+  linear_join_kernel<T, AFTER><<<(uint32_t)((lanes + 255) / 256), 256, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_linear(const LinearParams& a, Layout layout, After after, const LinearPlan& plan, hipStream_t stream) {
+  LinearParams p = a;
+  p.shares = plan.shares;
+  p.share = plan.share;
+  if (plan.shares > 1) {
+    p.n = p.width = after == After::kGated ? 2 * a.n : a.n;
+    hipError_t e = layout == Layout::kRows            ? launch_shape<T, Layout::kRows, After::kSums>(p, plan.shape, plan.shares, stream)
+                   : layout == Layout::kWeightColumns ? launch_shape<T, Layout::kWeightColumns, After::kSums>(p, plan.shape, plan.shares, stream)
+                                                      : launch_shape<T, Layout::kColumns, After::kSums>(p, plan.shape, plan.shares, stream);
+    if (e != hipSuccess) return e;
+    p.n = a.n;
+    switch (after) {
+      case After::kForward: return launch_join<T, After::kForward>(p, stream);
+      case After::kGated: return launch_join<T, After::kGated>(p, stream);
+      case After::kSlope: return launch_join<T, After::kSlope>(p, stream);
+      default: return launch_join<T, After::kPlain>(p, stream);
+    }
+  }
+  switch (after) {
+    case After::kForward: return launch_shape<T, Layout::kRows, After::kForward>(p, plan.shape, 1, stream);
+    case After::kGated: return launch_shape<T, Layout::kRows, After::kGated>(p, plan.shape, 1, stream);
+    case After::kSlope: return launch_shape<T, Layout::kWeightColumns, After::kSlope>(p, plan.shape, 1, stream);
+    default:
+      return layout == Layout::kWeightColumns ? launch_shape<T, Layout::kWeightColumns, After::kPlain>(p, plan.shape, 1, stream)
+                                              : launch_shape<T, Layout::kColumns, After::kPlain>(p, plan.shape, 1, stream);
+  }
+}
+
+}  // namespace nd

@@ -5,7 +5,10 @@ over a batch of them needs
 
 * :func:`packed_attention`: causal attention within each walk of a packed batch, with grouped heads;
 * :func:`dropout`: from the samplers' own random stream, the mask never stored;
-* :func:`vocabulary_loss`: softmax cross entropy over all vertices, the logits never stored.
+* :func:`vocabulary_loss`: softmax cross entropy over all vertices, the logits never stored;
+* :func:`layer_norm`: of each row, with the gradients of its weight and bias;
+* :func:`linear`: a matrix product with bias, activation and residual in one kernel;
+* :func:`mlp`: the feed-forward part of a block, gated or not.
 
 Each has a ``_forward`` and a ``_backward`` function and a differentiable form that calls both.  They
 enqueue the library's HIP kernels (include/nextdoor_amd.h) on torch's current stream of the tensors'
@@ -23,11 +26,12 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._capi import NextDoorError, PackedAttention, VocabularyLoss, check
+from ._capi import LayerNorm, Linear, Mlp, NextDoorError, PackedAttention, VocabularyLoss, check
 
 __all__ = ["PackedSequences", "packed_attention", "packed_attention_forward", "packed_attention_backward",
            "vocabulary_loss", "vocabulary_loss_forward", "vocabulary_loss_backward", "dropout", "dropout_forward",
-           "dropout_backward", "NextDoorError"]
+           "dropout_backward", "layer_norm", "layer_norm_forward", "layer_norm_backward", "linear", "linear_forward",
+           "linear_backward", "mlp", "mlp_forward", "mlp_backward", "NextDoorError"]
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # ND_F32, ND_F16, ND_BF16
 _lib = None
@@ -380,3 +384,391 @@ class _VocabularyLoss(torch.autograd.Function):
 def vocabulary_loss(hidden, weight, target):
     """The loss of each row (:func:`vocabulary_loss_forward`), differentiable in hidden and weight."""
     return _VocabularyLoss.apply(hidden, weight, target)
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------
+
+
+def _rows_in_place(x, dim, multiple):
+    """x as [rows, dim] and the elements between its rows, a multiple of ``multiple``.  What cannot be read so is copied."""
+    x = x.reshape(-1, dim) if x.dim() != 2 else x
+    rows, step = x.shape[0], x.stride(0)
+    if rows <= 1 or dim == 0:
+        step = dim + -dim % multiple  # (never used, but torch keeps one)
+    if (x.stride(1) != 1 and dim > 1) or step % multiple or step > 4194304 or (multiple > 1 and x.data_ptr() % 16):
+        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+        step = dim
+    return x, step
+
+
+def _norm(x, weight, bias, eps, others=()):
+    """Checked arguments: (device index, x as rows, the struct's first fields, weight, bias)."""
+    index = _on_gpu("layer norm", x, *(t for t in (weight, bias, *others) if t is not None))
+    dtype = x.dtype
+    if dtype not in _DTYPES:
+        raise NextDoorError("layer norm: no kernel for %s" % dtype)
+    if x.dim() == 0:
+        raise NextDoorError("layer norm: x has no rows")
+    dim = x.shape[-1]
+    weight_dtype = dtype
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != (dim,):
+            raise NextDoorError("layer norm: %s is not [%d]" % (name, dim))
+        if t.dtype is not dtype and t.dtype is not torch.float32:
+            raise NextDoorError("layer norm: %s is neither of the type of x nor float32" % name)
+        weight_dtype = t.dtype
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
+        raise NextDoorError("layer norm: weight and bias are of different types")
+    if not 0.0 <= eps < math.inf:
+        raise NextDoorError("layer norm: eps is a number of at least 0, %r given" % (eps,))
+    if not 1 <= dim <= 16384:
+        raise NextDoorError("layer norm: rows of 1 to 16384 values, %d given" % dim)
+    x, x_row = _rows_in_place(x, dim, 1)
+    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+    return index, x, (x.shape[0], dim, _DTYPES[dtype], _DTYPES[weight_dtype], eps), x_row, weight, bias
+
+
+def _pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
+    """(out, mean, rstd): each row of x (its last dimension, up to 16384 values) less its mean, over its standard deviation
+    (``rstd = 1 / sqrt(variance + eps)``), times weight (1 unless given), plus bias (0).  float32, float16 or bfloat16; weight and bias
+    of that type or float32.  mean and rstd: [rows], float32, for the backward pass.  Sums are in 32 bits, results rounded
+    once."""
+    index, rows, fields, x_row, weight, bias = _norm(x, weight, bias, eps)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = (torch.empty(fields[0], dtype=torch.float32, device=x.device) for _ in range(2))
+    _run(index, _library().nd_layer_norm_forward,
+         LayerNorm(*fields, x_row, 0, rows.data_ptr(), _pointer(weight), _pointer(bias), out.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
+    return out, mean, rstd
+
+
+def layer_norm_backward(dout, x, weight, mean, rstd, needs=(True, True, True)):
+    """(dx, dweight, dbias) for the gradient ``dout`` of ``out``; mean and rstd are the forward pass's, ``weight`` None if there was
+    none (the gradients of weight and bias then have the type of x).  ``needs``: which to compute; the others are None."""
+    index, rows, fields, x_row, weight, _ = _norm(x, weight, None, 0.0, (dout, mean, rstd))
+    if dout.shape != x.shape or dout.dtype is not x.dtype:
+        raise NextDoorError("layer norm: dout is of another shape or type than x")
+    for t in (mean, rstd):
+        if not (t.shape == (fields[0],) and t.dtype is torch.float32 and t.is_contiguous()):
+            raise NextDoorError("layer norm: mean and rstd are not a forward pass's")
+    dout, dout_row = _rows_in_place(dout, fields[1], 1)
+    kind = x.dtype if weight is None else weight.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
+    dweight, dbias = (torch.empty(fields[1], dtype=kind, device=x.device) if need else None for need in needs[1:])
+    a = LayerNorm(*fields, x_row, dout_row, rows.data_ptr(), _pointer(weight), None, None, mean.data_ptr(), rstd.data_ptr(),
+                  dout.data_ptr(), _pointer(dx), _pointer(dweight), _pointer(dbias))
+    workspace = _room(a, _library().nd_layer_norm_workspace(a), x.device)
+    _run(index, _library().nd_layer_norm_backward, a)
+    del workspace
+    return dx, dweight, dbias
+
+
+def _room(a, size, device):
+    """A workspace of the size that a call needs, if any (a call that no kernel can do has none: the call says why)."""
+    if size <= 0:
+        return None
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    return workspace
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        out, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dweight, dbias = layer_norm_backward(dout, x, weight, mean, rstd, ctx.needs_input_grad[:3])
+        return dx, dweight, dbias if dbias is None else dbias.to(ctx.bias_dtype), None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """The ``out`` of :func:`layer_norm_forward`, differentiable in x, weight and bias."""
+    return _LayerNorm.apply(x, weight, bias, eps)
+
+
+# ---- linear maps -------------------------------------------------------------------------------------------
+
+_ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # ND_NO_ACTIVATION ...
+
+
+def _activation(what, name):
+    try:
+        return _ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise NextDoorError("%s: no activation %r; there are None, %s" % (what, name, ", ".join(sorted(filter(None, _ACTIVATIONS))))) from None
+
+
+def _types(what, first, *others):
+    dtype = first.dtype
+    if not (dtype is torch.bfloat16 or dtype is torch.float16):
+        raise NextDoorError("%s: 16-bit types only, %s given" % (what, dtype))
+    for t in others:
+        if t is not None and t.dtype is not dtype:
+            raise NextDoorError("%s: tensors of different types" % what)
+
+
+def _matrix(t):
+    """A weight or a bias as the kernels read it; a last dimension that is no multiple of 8, or a matrix's first, is
+    filled up with zeros, which costs a copy."""
+    if t is None:
+        return None
+    fill = [n for size in reversed(t.shape) for n in (0, -size % 8)]
+    if any(fill):
+        t = torch.nn.functional.pad(t, fill)
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _vectors_in_place(x, dim):
+    """x as [rows, a multiple of 8], filled up with zeros if need be, and the elements between its rows."""
+    if dim % 8:
+        x = torch.nn.functional.pad(x.reshape(-1, dim), (0, -dim % 8))
+    return _rows_in_place(x, dim + -dim % 8, 8)
+
+
+def _check_rows(what, name, t, shape, dtype):
+    if t.shape != shape or t.dtype is not dtype:
+        raise NextDoorError("%s: %s is of another shape or type than the result" % (what, name))
+
+
+def _cut(t, *shape):
+    """The part of a filled-up result that was asked for."""
+    if t is None or t.shape == shape:
+        return t
+    for i, n in enumerate(shape):
+        t = t.narrow(i, 0, n)
+    return t.contiguous()
+
+
+def _linear_arguments(what, x, weight, bias):
+    if not (x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1]):
+        raise NextDoorError("%s: x and weight are not vectors and a matrix of equally long rows" % what)
+    out_dim, dim = weight.shape
+    if bias is not None and bias.shape != (out_dim,):
+        raise NextDoorError("%s: a bias is not [%d]" % (what, out_dim))
+    if not (1 <= dim <= 1048576 and 1 <= out_dim <= 1048576):
+        raise NextDoorError("%s: vectors of 1 to 1048576 places, %d and %d given" % (what, dim, out_dim))
+    return out_dim, dim
+
+
+def linear_forward(x, weight, bias=None, activation=None, residual=None, keep=False):
+    """``activation(x weight^T + bias) + residual``, or with ``keep`` (out, z), z being what the backward pass reads (None without an
+    activation).
+
+    x: [..., dim], weight: [out_dim, dim], bias: [out_dim], residual: [..., out_dim], float16 or bfloat16; activation: None,
+    "relu", "gelu", "gelu_tanh" or "silu".  Slices whose rows begin at multiples of 16 bytes are read in place; dims that are no
+    multiples of 8 cost copies.  Sums are in 32 bits; the result, and z, are rounded once."""
+    index = _on_gpu("linear", x, weight, *(t for t in (bias, residual) if t is not None))
+    _types("linear", x, weight, bias, residual)
+    code = _activation("linear", activation)
+    out_dim, dim = _linear_arguments("linear", x, weight, bias)
+    shape = (*x.shape[:-1], out_dim)
+    wide = out_dim + -out_dim % 8
+    rows, x_row = _vectors_in_place(x, dim)
+    residual_row = 0
+    if residual is not None:
+        _check_rows("linear", "the residual", residual, shape, x.dtype)
+        residual, residual_row = _vectors_in_place(residual, out_dim)
+    weight, bias = _matrix(weight), _matrix(bias)
+    n = rows.shape[0]
+    out = torch.empty((n, wide), dtype=x.dtype, device=x.device)
+    z = torch.empty((n, wide), dtype=x.dtype, device=x.device) if keep and code else None
+    a = Linear(n, weight.shape[1], wide, _DTYPES[x.dtype], code, x_row, residual_row, 0, rows.data_ptr(), weight.data_ptr(), _pointer(bias),
+               _pointer(residual), out.data_ptr(), _pointer(z))
+    workspace = _room(a, _library().nd_linear_workspace(a, 0), x.device)
+    _run(index, _library().nd_linear_forward, a)
+    del workspace
+    out = _cut(out, n, out_dim).view(shape)
+    return (out, z) if keep else out
+
+
+def linear_backward(dout, x, weight, z=None, activation=None, with_bias=True, needs=(True, True)):
+    """(dx, dweight, dbias) for the gradient ``dout`` of ``out``; z is what the forward pass kept.  The residual's gradient is
+    ``dout`` itself.  ``needs``: whether dx and dweight are wanted; what is not is None.  With an activation the gradient of z is
+    rounded to 16 bits before its products (float16: relative to max |dout|, so that small ones are not lost)."""
+    index = _on_gpu("linear", x, dout, weight, *(() if z is None else (z,)))
+    _types("linear", x, dout, weight, z)
+    code = _activation("linear", activation)
+    out_dim, dim = _linear_arguments("linear", x, weight, None)
+    _check_rows("linear", "dout", dout, (*x.shape[:-1], out_dim), x.dtype)
+    rows, x_row = _vectors_in_place(x, dim)
+    dout, dout_row = _vectors_in_place(dout, out_dim)
+    weight = _matrix(weight)
+    n, wide, high = rows.shape[0], out_dim + -out_dim % 8, dim + -dim % 8
+    if code and not (z is not None and z.shape == (n, wide) and z.is_contiguous()):
+        raise NextDoorError("linear: z is not what a forward pass kept")
+    dx = torch.empty((n, high), dtype=x.dtype, device=x.device) if needs[0] else None
+    dweight = torch.empty((wide, high), dtype=x.dtype, device=x.device) if needs[1] else None
+    dbias = torch.empty(wide, dtype=x.dtype, device=x.device) if with_bias else None
+    a = Linear(n, high, wide, _DTYPES[x.dtype], code, x_row, 0, dout_row, rows.data_ptr(), weight.data_ptr(), None, None, None,
+               _pointer(z) if code else None, dout.data_ptr(), _pointer(dx), _pointer(dweight), _pointer(dbias))
+    workspace = _room(a, _library().nd_linear_workspace(a, 1), x.device)
+    _run(index, _library().nd_linear_backward, a)
+    del workspace
+    dx = dx if dx is None else _cut(dx, n, dim).view(x.shape)
+    return dx, _cut(dweight, out_dim, dim), _cut(dbias, out_dim)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        keep = activation is not None and any(ctx.needs_input_grad[:3])
+        out = linear_forward(x, weight, bias, activation, residual, keep)
+        out, z = out if keep else (out, None)
+        ctx.save_for_backward(x, weight, z)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, weight, z = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        got = (None, None, None)
+        if any(needs[:3]):
+            got = linear_backward(dout, x, weight, z, ctx.activation, needs[2], needs[:2])
+        return (*got, dout if needs[3] else None, None)
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """:func:`linear_forward`, differentiable in x, weight, bias and the residual."""
+    return _Linear.apply(x, weight, bias, residual, activation)
+
+
+# ---- feed-forward parts ------------------------------------------------------------------------------------
+
+
+def _mlp_arguments(x, up, down, up_bias, down_bias, activation, gated):
+    if not (down.dim() == 2 and up.dim() == 2):
+        raise NextDoorError("mlp: up and down are matrices")
+    inner = down.shape[1]
+    if up.shape[0] != (2 * inner if gated else inner):
+        raise NextDoorError("mlp: up has %d rows, down has rows of %d: %s" %
+                            (up.shape[0], inner, "a gated part has twice as many" if gated else "they are as many"))
+    wide, dim = _linear_arguments("mlp", x, up, up_bias)
+    if down_bias is not None and down_bias.shape != (down.shape[0],):
+        raise NextDoorError("mlp: a bias is not [%d]" % down.shape[0])
+    if not 1 <= down.shape[0] <= 1048576:
+        raise NextDoorError("mlp: vectors of 1 to 1048576 places, %d given" % down.shape[0])
+    return dim, inner, down.shape[0], _activation("mlp", activation)
+
+
+def _up(t, inner, gated):
+    """The rows of both projections, each filled up to a multiple of 8."""
+    if t is None or not gated or inner % 8 == 0:
+        return _matrix(t)
+    halves = [torch.nn.functional.pad(half, (0, 0) * (t.dim() - 1) + (0, -inner % 8)) for half in t.split(inner)]
+    return _matrix(torch.cat(halves))
+
+
+def _up_cut(t, inner, gated, *rest):
+    """The gradient of up or its bias without what was filled up."""
+    if t is None or not gated or inner % 8 == 0:
+        return _cut(t, inner * (2 if gated else 1), *rest)
+    return torch.cat([_cut(half, inner, *rest) for half in t.split(t.shape[0] // 2)])
+
+
+def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None, keep=False):
+    """The feed-forward part of a block: ``h down^T + down_bias + residual``, or with ``keep`` (out, z, h), which the backward
+    pass reads.
+
+    z = x up^T + up_bias; gated: ``h = activation(g) u`` with ``g, u = z.chunk(2, -1)``, else ``h = activation(z)``.  x: [..., dim];
+    up: [2 inner or inner, dim]; down: [out_dim, inner]; activations, types and sizes as in :func:`linear_forward`.  Both
+    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second."""
+    index = _on_gpu("mlp", x, up, down, *(t for t in (up_bias, down_bias, residual) if t is not None))
+    _types("mlp", x, up, down, up_bias, down_bias, residual)
+    gated = bool(gated)
+    dim, inner, out_dim, code = _mlp_arguments(x, up, down, up_bias, down_bias, activation, gated)
+    shape = (*x.shape[:-1], out_dim)
+    rows, x_row = _vectors_in_place(x, dim)
+    residual_row = 0
+    if residual is not None:
+        _check_rows("mlp", "the residual", residual, shape, x.dtype)
+        residual, residual_row = _vectors_in_place(residual, out_dim)
+    up, up_bias, down, down_bias = _up(up, inner, gated), _up(up_bias, inner, gated), _matrix(down), _matrix(down_bias)
+    n, wide = rows.shape[0], down.shape[0]
+
+    def empty(columns):
+        return torch.empty((n, columns), dtype=x.dtype, device=x.device)
+
+    out, h = empty(wide), empty(down.shape[1])
+    z = empty(up.shape[0]) if keep and (gated or code) else None
+    a = Mlp(n, up.shape[1], down.shape[1], wide, _DTYPES[x.dtype], code, gated, x_row, residual_row, 0, rows.data_ptr(), up.data_ptr(),
+            _pointer(up_bias), down.data_ptr(), _pointer(down_bias), _pointer(residual), out.data_ptr(), _pointer(z), h.data_ptr())
+    workspace = _room(a, _library().nd_mlp_workspace(a, 0), x.device)
+    _run(index, _library().nd_mlp_forward, a)
+    del workspace
+    out = _cut(out, n, out_dim).view(shape)
+    return (out, z, h) if keep else out
+
+
+def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up_bias=True, with_down_bias=True,
+                 needs=(True, True, True)):
+    """(dx, dup, ddown, dup_bias, ddown_bias) for the gradient ``dout`` of ``out``; z and h are what the forward pass kept.  The
+    residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None.  The gradient of z
+    is rounded to 16 bits before its products (float16: relative to max |dout|, and must stay below 65504 times that)."""
+    index = _on_gpu("mlp", x, dout, up, down, h, *(() if z is None else (z,)))
+    _types("mlp", x, dout, up, down, z, h)
+    gated = bool(gated)
+    dim, inner, out_dim, code = _mlp_arguments(x, up, down, None, None, activation, gated)
+    _check_rows("mlp", "dout", dout, (*x.shape[:-1], out_dim), x.dtype)
+    rows, x_row = _vectors_in_place(x, dim)
+    dout, dout_row = _vectors_in_place(dout, out_dim)
+    up, down = _up(up, inner, gated), _matrix(down)
+    n = rows.shape[0]
+    if not (h.shape == (n, down.shape[1]) and h.is_contiguous()):
+        raise NextDoorError("mlp: h is not what a forward pass kept")
+    if (gated or code) and not (z is not None and z.shape == (n, up.shape[0]) and z.is_contiguous()):
+        raise NextDoorError("mlp: z is not what a forward pass kept")
+
+    def empty(need, *size):
+        return torch.empty(size, dtype=x.dtype, device=x.device) if need else None
+
+    dx, dup, ddown = empty(needs[0], n, up.shape[1]), empty(needs[1], *up.shape), empty(needs[2], *down.shape)
+    dup_bias, ddown_bias = empty(with_up_bias, up.shape[0]), empty(with_down_bias, down.shape[0])
+    a = Mlp(n, up.shape[1], down.shape[1], down.shape[0], _DTYPES[x.dtype], code, gated, x_row, 0, dout_row, rows.data_ptr(), up.data_ptr(),
+            None, down.data_ptr(), None, None, None, _pointer(z), h.data_ptr(), dout.data_ptr(), _pointer(dx), _pointer(dup),
+            _pointer(dup_bias), _pointer(ddown), _pointer(ddown_bias))
+    workspace = _room(a, _library().nd_mlp_workspace(a, 1), x.device)
+    _run(index, _library().nd_mlp_backward, a)
+    del workspace
+    dx = dx if dx is None else _cut(dx, n, dim).view(x.shape)
+    return (dx, _up_cut(dup, inner, gated, dim), _cut(ddown, out_dim, inner), _up_cut(dup_bias, inner, gated), _cut(ddown_bias, out_dim))
+
+
+class _Mlp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, up, down, up_bias, down_bias, activation, gated, residual):
+        keep = any(ctx.needs_input_grad[:5])
+        got = mlp_forward(x, up, down, up_bias, down_bias, activation, gated, residual, keep)
+        out, z, h = got if keep else (got, None, None)
+        ctx.save_for_backward(x, up, down, z, h)
+        ctx.how = activation, gated
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        x, up, down, z, h = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        got = (None,) * 5
+        if any(needs[:5]):
+            got = mlp_backward(dout, x, up, down, z, h, *ctx.how, needs[3], needs[4], needs[:3])
+        return (*got, None, None, dout if needs[7] else None)
+
+
+def mlp(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None):
+    """:func:`mlp_forward`, differentiable in x, the weights, the biases and the residual."""
+    return _Mlp.apply(x, up, down, up_bias, down_bias, activation, gated, residual)
