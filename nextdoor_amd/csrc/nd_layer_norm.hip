@@ -84,10 +84,19 @@ struct Places {
   }
   // Weights: of this type or in 32 bits; a null array is `otherwise` everywhere.
   __device__ __forceinline__ static void load_weights(const void* w, bool in_32, float otherwise, int dim, int lane, float (&x)[VALUES]) {
+    if (!w) {
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {
-      const int c = column(i, lane);
-      x[i] = !w ? otherwise : c >= dim ? 0.f : in_32 ? ((const float*)w)[c] : (float)((const T*)w)[c];
+      for (int i = 0; i < VALUES; ++i) x[i] = otherwise;
+    } else if (in_32) {
+      Places<float, LANES, VALUES, VECTOR> all;
+      all.load((const char*)w, dim, lane);
+#pragma unroll
+      for (int i = 0; i < VALUES; ++i) x[i] = all.v[i];
+    } else {
+      Places all;
+      all.load((const char*)w, dim, lane);
+#pragma unroll
+      for (int i = 0; i < VALUES; ++i) x[i] = (float)all.v[i];
     }
   }
 };
@@ -106,7 +115,7 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 (*scratch)[THREADS /
     if ((threadIdx.x & 63) == 0) scratch[turn & 1][wave] = v;
     __syncthreads();  // (two arrays in turn: this one is written again only after the barrier of the next call)
     v = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 4
     for (int w = 0; w < kWaves; ++w) {
       v.x += scratch[turn & 1][first + w].x;
       v.y += scratch[turn & 1][first + w].y;
@@ -115,96 +124,107 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 (*scratch)[THREADS /
   return v;
 }
 
-template <class T, int LANES, int VALUES, int THREADS, bool VECTOR>
+template <class T, int LANES, int VALUES, int THREADS, int AHEAD, bool VECTOR>
 __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormParams p) {
   using Row = Places<T, LANES, VALUES, VECTOR>;
   constexpr int kGroups = THREADS / LANES;
   __shared__ float2 scratch[2][THREADS / 64];
   const int lane = threadIdx.x % LANES;
   const int64_t stride = (int64_t)gridDim.x * kGroups;
+  Row next[AHEAD];
+  int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / LANES;
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a)
+    if (row + a * stride < p.rows) next[a].load(p.x + (row + a * stride) * p.x_bytes, p.dim, lane);
   float w[VALUES], b[VALUES];
   Row::load_weights(p.weight, p.weight_32, 1.f, p.dim, lane, w);
   Row::load_weights(p.bias, p.weight_32, 0.f, p.dim, lane, b);
-  Row next;
-  int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / LANES;
-  if (row < p.rows) next.load(p.x + row * p.x_bytes, p.dim, lane);
   int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < p.rows; base += stride, row += stride) {
-    const bool there = row < p.rows;
-    float x[VALUES], sum = 0.f;
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < p.rows; base += AHEAD * stride) {
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {
-      x[i] = there ? (float)next.v[i] : 0.f;
-      sum += x[i];
-    }
-    if (row + stride < p.rows) next.load(p.x + (row + stride) * p.x_bytes, p.dim, lane);
-    const float mean = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
-    sum = 0.f;
+    for (int a = 0; a < AHEAD; ++a, row += stride) {
+      const bool there = row < p.rows;
+      float x[VALUES], sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {
-      x[i] = Row::column(i, lane) < p.dim ? x[i] - mean : 0.f;
-      sum = __builtin_fmaf(x[i], x[i], sum);
-    }
-    const float variance = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
-    const float rstd = 1.f / sqrtf(variance + p.eps);
+      for (int i = 0; i < VALUES; ++i) {
+        x[i] = there ? (float)next[a].v[i] : 0.f;
+        sum += x[i];
+      }
+      if (row + AHEAD * stride < p.rows) next[a].load(p.x + (row + AHEAD * stride) * p.x_bytes, p.dim, lane);
+      const float mean = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
+      sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) x[i] = __builtin_fmaf(x[i] * rstd, w[i], b[i]);
-    if (there) {
-      Row::store((char*)p.out + row * p.dim * (int64_t)sizeof(T), p.dim, lane, x);
-      if (lane == 0) {
-        p.mean[row] = mean;
-        p.rstd[row] = rstd;
+      for (int i = 0; i < VALUES; ++i) {
+        x[i] = Row::column(i, lane) < p.dim ? x[i] - mean : 0.f;
+        sum = __builtin_fmaf(x[i], x[i], sum);
+      }
+      const float variance = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
+      const float rstd = 1.f / sqrtf(variance + p.eps);
+#pragma unroll
+      for (int i = 0; i < VALUES; ++i) x[i] = __builtin_fmaf(x[i] * rstd, w[i], b[i]);
+      if (there) {
+        Row::store((char*)p.out + row * p.dim * (int64_t)sizeof(T), p.dim, lane, x);
+        if (lane == 0) {
+          p.mean[row] = mean;
+          p.rstd[row] = rstd;
+        }
       }
     }
   }
 }
 
-template <class T, int LANES, int VALUES, int THREADS, bool VECTOR>
+template <class T, int LANES, int VALUES, int THREADS, int AHEAD, bool VECTOR>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
   using Row = Places<T, LANES, VALUES, VECTOR>;
   constexpr int kGroups = THREADS / LANES;
   __shared__ float2 scratch[2][THREADS / 64];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int64_t stride = (int64_t)gridDim.x * kGroups;
-  float w[VALUES], dw[VALUES], db[VALUES];
-  Row::load_weights(p.weight, p.weight_32, 1.f, p.dim, lane, w);
-#pragma unroll
-  for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = 0.f;
-  Row next, next_dout;
-  float next_mean = 0.f, next_rstd = 0.f;
-  auto ask = [&](int64_t row) {
+  Row next[AHEAD], next_dout[AHEAD];
+  float next_mean[AHEAD], next_rstd[AHEAD];
+  auto ask = [&](int a, int64_t row) {
     if (row >= p.rows) return;
-    next.load(p.x + row * p.x_bytes, p.dim, lane);
-    next_dout.load(p.dout + row * p.dout_bytes, p.dim, lane);
-    next_mean = p.mean[row];
-    next_rstd = p.rstd[row];
+    next[a].load(p.x + row * p.x_bytes, p.dim, lane);
+    next_dout[a].load(p.dout + row * p.dout_bytes, p.dim, lane);
+    next_mean[a] = p.mean[row];
+    next_rstd[a] = p.rstd[row];
   };
   int64_t row = (int64_t)blockIdx.x * kGroups + group;
-  ask(row);
+#pragma unroll
+  for (int a = 0; a < AHEAD; ++a) ask(a, row + a * stride);
+  constexpr bool kKeepWeights = VALUES <= 8;  // (the longest rows read them again each time, from the caches)
+  float w[VALUES], dw[VALUES], db[VALUES];
+  if (kKeepWeights) Row::load_weights(p.weight, p.weight_32, 1.f, p.dim, lane, w);
+#pragma unroll
+  for (int i = 0; i < VALUES; ++i) dw[i] = db[i] = 0.f;
   int turn = 0;
-  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < p.rows; base += stride, row += stride) {
-    const bool there = row < p.rows;
-    const float mean = next_mean, rstd = next_rstd;
-    float n[VALUES], e[VALUES];
-    float2 sum = make_float2(0.f, 0.f);
+  for (int64_t base = (int64_t)blockIdx.x * kGroups; base < p.rows; base += AHEAD * stride) {
 #pragma unroll
-    for (int i = 0; i < VALUES; ++i) {
-      const bool inside = there && Row::column(i, lane) < p.dim;
-      const float d = inside ? (float)next_dout.v[i] : 0.f;
-      n[i] = inside ? ((float)next.v[i] - mean) * rstd : 0.f;
-      dw[i] = __builtin_fmaf(d, n[i], dw[i]);
-      db[i] += d;
-      e[i] = d * w[i];
-      sum.x += e[i];
-      sum.y = __builtin_fmaf(e[i], n[i], sum.y);
-    }
-    ask(row + stride);
-    if (p.out) {
-      sum = row_sums<LANES, THREADS>(sum, scratch, turn++);
-      const float mean_e = sum.x / p.dim, mean_en = sum.y / p.dim;
+    for (int a = 0; a < AHEAD; ++a, row += stride) {
+      const bool there = row < p.rows;
+      const float mean = next_mean[a], rstd = next_rstd[a];
+      if (!kKeepWeights) Row::load_weights(p.weight, p.weight_32, 1.f, p.dim, lane, w);
+      float n[VALUES], e[VALUES];
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < VALUES; ++i) e[i] = (e[i] - __builtin_fmaf(n[i], mean_en, mean_e)) * rstd;
-      if (there) Row::store((char*)p.out + row * p.dim * (int64_t)sizeof(T), p.dim, lane, e);
+      for (int i = 0; i < VALUES; ++i) {
+        const bool inside = there && Row::column(i, lane) < p.dim;
+        const float d = inside ? (float)next_dout[a].v[i] : 0.f;
+        n[i] = inside ? ((float)next[a].v[i] - mean) * rstd : 0.f;
+        dw[i] = __builtin_fmaf(d, n[i], dw[i]);
+        db[i] += d;
+        e[i] = d * w[i];
+        sum.x += e[i];
+        sum.y = __builtin_fmaf(e[i], n[i], sum.y);
+      }
+      ask(a, row + AHEAD * stride);
+      if (p.out) {
+        sum = row_sums<LANES, THREADS>(sum, scratch, turn++);
+        const float mean_e = sum.x / p.dim, mean_en = sum.y / p.dim;
+#pragma unroll
+        for (int i = 0; i < VALUES; ++i) e[i] = (e[i] - __builtin_fmaf(n[i], mean_en, mean_e)) * rstd;
+        if (there) Row::store((char*)p.out + row * p.dim * (int64_t)sizeof(T), p.dim, lane, e);
+      }
     }
   }
   if (!p.sums) return;
@@ -241,50 +261,55 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
   }
 }
 
-// Rows by size: sixteen lanes to a short one, a wave, four waves or sixteen to longer ones, eight or sixteen places to a lane.
+// Rows by size: eight places to a lane, sixteen for the longest, and as many lanes as that takes; `rows` of a workgroup at a time in
+// the backward pass, which has one workgroup of 1024 lanes to a compute unit, so that few sums are left to add.  The forward pass
+// has workgroups of 256 or what a row takes.
 struct NormShape {
-  int most, groups;  // places of a row; rows of a workgroup at a time
+  int most, lanes, rows;
 };
-constexpr NormShape kNormShapes[] = {{128, 64}, {512, 16}, {1024, 16}, {2048, 4}, {4096, 4}, {8192, 1}, {16384, 1}};
+constexpr NormShape kNormShapes[] = {{128, 16, 64}, {512, 64, 16}, {1024, 128, 8}, {2048, 256, 4}, {4096, 512, 2}, {8192, 1024, 1}, {16384, 1024, 1}};
+constexpr int kForwardLanes = 1 << 19, kBackwardBlocks = 256;
 int shape_of(int32_t dim) {
   int i = 0;
   while (dim > kNormShapes[i].most) ++i;
   return i;
 }
-constexpr int kForwardBlocks = 2048, kBackwardBlocks = 512;
-int64_t blocks_of(int64_t rows, int32_t dim, int most) {
-  const int groups = kNormShapes[shape_of(dim)].groups;
-  return std::max<int64_t>(1, std::min<int64_t>(most, (rows + groups - 1) / groups));
+int64_t backward_blocks(int64_t rows, int32_t dim) {
+  const int at_once = kNormShapes[shape_of(dim)].rows;
+  return std::max<int64_t>(1, std::min<int64_t>(kBackwardBlocks, (rows + at_once - 1) / at_once));
 }
 
-template <class T, int LANES, int VALUES, int THREADS>
-void launch_norm_of(const NormParams& p, bool backward, bool vector, uint32_t blocks, hipStream_t stream) {
+template <class T, int LANES, int VALUES>
+void launch_norm_of(const NormParams& p, bool backward, bool vector, hipStream_t stream) {
   if (backward) {
-    if (vector) norm_backward_kernel<T, LANES, VALUES, THREADS, true><<<blocks, THREADS, 0, stream>>>(p);
-    else norm_backward_kernel<T, LANES, VALUES, THREADS, false><<<blocks, THREADS, 0, stream>>>(p);
+    const uint32_t blocks = (uint32_t)backward_blocks(p.rows, p.dim);
+    if (vector) norm_backward_kernel<T, LANES, VALUES, 1024, VALUES == 8 && sizeof(T) == 2 ? 2 : 1, true><<<blocks, 1024, 0, stream>>>(p);
+    else norm_backward_kernel<T, LANES, VALUES, 1024, 1, false><<<blocks, 1024, 0, stream>>>(p);
   } else {
-    if (vector) norm_forward_kernel<T, LANES, VALUES, THREADS, true><<<blocks, THREADS, 0, stream>>>(p);
-    else norm_forward_kernel<T, LANES, VALUES, THREADS, false><<<blocks, THREADS, 0, stream>>>(p);
+    constexpr int kThreads = LANES < 256 ? 256 : LANES, kGroups = kThreads / LANES;
+    const uint32_t blocks = (uint32_t)std::min<int64_t>((p.rows + kGroups - 1) / kGroups, kForwardLanes / kThreads);
+    if (vector) norm_forward_kernel<T, LANES, VALUES, kThreads, 1, true><<<blocks, kThreads, 0, stream>>>(p);
+    else norm_forward_kernel<T, LANES, VALUES, kThreads, 1, false><<<blocks, kThreads, 0, stream>>>(p);
   }
 }
 template <class T>
 void launch_norm(const NormParams& p, bool backward, hipStream_t stream) {
-  const uint32_t blocks = (uint32_t)blocks_of(p.rows, p.dim, backward ? kBackwardBlocks : kForwardBlocks);
-  const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.out | (uintptr_t)p.x_bytes | (backward ? (uintptr_t)p.dout | (uintptr_t)p.dout_bytes : 0);
+  const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.out | (uintptr_t)p.weight | (uintptr_t)p.bias | (uintptr_t)p.x_bytes |
+                       (backward ? (uintptr_t)p.dout | (uintptr_t)p.dout_bytes : 0);
   const bool vector = p.dim % 8 == 0 && (at & 15) == 0;
   switch (shape_of(p.dim)) {
-    case 0: return launch_norm_of<T, 16, 8, 1024>(p, backward, vector, blocks, stream);
-    case 1: return launch_norm_of<T, 64, 8, 1024>(p, backward, vector, blocks, stream);
-    case 2: return launch_norm_of<T, 64, 16, 1024>(p, backward, vector, blocks, stream);
-    case 3: return launch_norm_of<T, 256, 8, 1024>(p, backward, vector, blocks, stream);
-    case 4: return launch_norm_of<T, 256, 16, 1024>(p, backward, vector, blocks, stream);
-    case 5: return launch_norm_of<T, 1024, 8, 1024>(p, backward, vector, blocks, stream);
-    default: return launch_norm_of<T, 1024, 16, 1024>(p, backward, vector, blocks, stream);
+    case 0: return launch_norm_of<T, 16, 8>(p, backward, vector, stream);
+    case 1: return launch_norm_of<T, 64, 8>(p, backward, vector, stream);
+    case 2: return launch_norm_of<T, 128, 8>(p, backward, vector, stream);
+    case 3: return launch_norm_of<T, 256, 8>(p, backward, vector, stream);
+    case 4: return launch_norm_of<T, 512, 8>(p, backward, vector, stream);
+    case 5: return launch_norm_of<T, 1024, 8>(p, backward, vector, stream);
+    default: return launch_norm_of<T, 1024, 16>(p, backward, vector, stream);
   }
 }
 
 int64_t norm_workspace(const nd_layer_norm* a) {
-  return a->dweight || a->dbias ? blocks_of(a->rows, a->dim, kBackwardBlocks) * 2 * a->dim * 4 : 0;
+  return a->dweight || a->dbias ? backward_blocks(a->rows, a->dim) * 2 * a->dim * 4 : 0;
 }
 
 std::string refuse(const nd_layer_norm* a) {
@@ -347,7 +372,7 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
   else launch_norm<__bf16>(p, backward, (hipStream_t)stream);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && sums) {
-    const int64_t blocks = blocks_of(a->rows, a->dim, kBackwardBlocks), columns = 2 * a->dim;
+    const int64_t blocks = backward_blocks(a->rows, a->dim), columns = 2 * a->dim;
     const hipStream_t s = (hipStream_t)stream;
     if (a->weight_dtype == ND_F32) e = column_join<float>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);
     else if (a->weight_dtype == ND_F16) e = column_join<_Float16>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);

@@ -60,29 +60,38 @@ int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
 // ---- which tiles, and how many shares of a sum -------------------------------------------------------------------
 
-// An estimate of a product's time in us from its rounds of 64 places: what a workgroup takes for one, and beside them, with the
-// compute units full.
+// An estimate of a product's time in us, from what its workgroups take for a round of 64 places where a compute unit here and there
+// has one, where each has one, and where each has as many as it holds; and beside the rounds.
 struct ShapeCost {
-  int m, n, at_once;         // rows of C, columns of C, workgroups that the GPU holds at a time
-  double round, alone, once; // us: a round with all of them, a round where a compute unit has one only, everything else
+  int m, n, at_once;  // rows of C, columns of C, workgroups that the GPU holds at a time
+  double lone, one, full, once;
 };
-constexpr ShapeCost kShapes[3] = {{256, 256, 256, 1.5, 1.5, 8.0}, {128, 128, 512, 0.95, 0.6, 4.0}, {64, 64, 768, 0.6, 0.35, 3.0}};
+constexpr ShapeCost kShapes[4] = {{256, 256, 256, 1.05, 1.5, 1.5, 10.0},
+                                  {128, 128, 512, 0.56, 0.6, 0.87, 4.0},
+                                  {64, 64, 768, 0.32, 0.4, 0.5, 3.0},
+                                  {256, 192, 256, 0.9, 1.2, 1.2, 9.0}};
 constexpr int kMostShares = 128;
+constexpr double kJoin = 4.0, kJoinRate = 8e6;  // us of one more kernel; bytes a us of sums, written and read again
+
+double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
+  const int64_t full = groups / c.at_once, rest = groups % c.at_once;
+  const double last = rest <= 256 ? c.lone + (c.one - c.lone) * rest / 256 : c.one + (c.full - c.one) * (rest - 256) / (c.at_once - 256);
+  return full * (rounds * c.full + c.once) + (rest ? rounds * last + c.once : 0);
+}
 
 LinearPlan plan_of(int64_t m, int64_t n, int64_t k, bool gated) {
   const int64_t rounds = std::max<int64_t>(1, (k + 63) / 64), columns = gated ? 2 * n : n;
   LinearPlan best = {0, 1, (int)(rounds * 64)};
   double least = INFINITY;
-  for (int shape = 0; shape < 3; ++shape) {
+  for (int shape = 0; shape < 4; ++shape) {
     const ShapeCost& c = kShapes[shape];
     const int64_t tiles = ((m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
     for (int64_t want = 1; want <= kMostShares; want = want < 4 ? want + 1 : want * 3 / 2) {
+      if (shape == 3 && gated && want == 1) continue;  // (there pairs of columns are 64 apart)
       const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
       if (shares != want && want > 1) continue;
-      const int64_t groups = tiles * shares;
-      const double turns = groups <= 256 ? 1 : ceil((double)groups / c.at_once);
-      double time = turns * (each * (groups <= 256 ? c.alone : c.round) + c.once);
-      if (shares > 1) time += 3.0 + (double)shares * m * columns * 8 / 4e6;
+      double time = time_of(c, tiles * shares, each);
+      if (shares > 1) time += kJoin + (double)shares * m * columns * 8 / kJoinRate;
       if (time < least) {
         least = time;
         best = {shape, (int)shares, (int)(each * 64)};

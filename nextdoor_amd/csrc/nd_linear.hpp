@@ -107,11 +107,12 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
 
 // ---- a tile of C to a workgroup ---------------------------------------------------------------------------
 
-// 256 x 256, eight waves with 4 x 2 results each, alone on a compute unit; 128 x 128 and 64 x 64, two and three of which share
-// one.
-using Large = product::Shape<2, 4, 4, 2, 64, 2, 4, 16, 2>;
-using Medium = product::Shape<2, 2, 2, 2, 64, 2, 4, 8, 2>;
-using Small = product::Shape<1, 2, 2, 1, 64, 3, 2, 4, 2>;
+// 256 x 256, eight waves with 4 x 2 results each, alone on a compute unit; 256 rows of C x 192 columns, which leaves fewer compute
+// units without work at the end of some sizes; 128 x 128 and 64 x 64, two and three of which share a compute unit.
+using Large = product::Shape<2, 4, 4, 2, 64, 2, 1, 4, 16, 2>;
+using Narrow = product::Shape<2, 4, 3, 2, 64, 2, 1, 4, 12, 2>;
+using Medium = product::Shape<2, 2, 2, 2, 64, 2, 2, 4, 8, 2>;
+using Small = product::Shape<1, 2, 2, 1, 64, 3, 2, 2, 4, 1>;
 
 enum class Layout { kRows, kWeightColumns, kColumns };  // both operands by rows; P by columns; both by columns
 
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   constexpr bool kGated = AFTER == After::kGated;
   constexpr int kColumns = kGated ? S::kTileM / 2 : S::kTileM;  // of C to a tile
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  __shared__ u32x4 tiles[S::kTileChunks];
+  __shared__ u32x4 tiles[S::kLdsChunks];
   // Bands of eight tiles of rows, in a band column after column: the tiles that a die works on at a time (32 or more) share few rows
   // of both operands.  Shares of a sum one after another.
   uint32_t block = block_by_die();
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   }
   product::meet();
   // ---- the results: wave's rows from wave_row0 on, columns from wave_column0 on
-  constexpr int kWaveChunks = S::kTileChunks / (S::kThreads / 64);
+  constexpr int kWaveChunks = S::kLdsChunks / (S::kThreads / 64);
   u32x4* mine = tiles + wave * kWaveChunks;
   const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN, wave_column0 = column0 + wave / S::kWavesN * (kColumns / S::kWavesM);
   const int h = lane >> 5;
@@ -176,62 +177,87 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
       }
     return;
   }
-  // four values of a result's column (a lane's row, columns 8 q + 4 h .. of block i)
-  auto four = [&](const f32x16& c, int q, float(&v)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = c[4 * q + e];
-  };
-  auto unpack = [](u32x2 w, float(&v)[4]) {
+  // A lane has 16 values of a result: its row, columns 8 q + 4 h .. + 3 of block i in registers 4 q .. 4 q + 3.
+  auto unpack = [](u32x2 w, float* v) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       v[2 * e] = unpack_low<T>(w[e]);
       v[2 * e + 1] = unpack_high<T>(w[e]);
     }
   };
-  auto pack = [](const float(&v)[4]) {
-    u32x2 w;
-    w[0] = pack_pair<T>(v[0], v[1]);
-    w[1] = pack_pair<T>(v[2], v[3]);
-    return w;
+  auto read = [&](const auto& region, int i, float(&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) unpack(region.piece(4 * i + q, lane), v + 4 * q);
   };
-  auto bias_of = [&](int column, int end, int past) {  // (columns past the end have no bias, and are not stored)
-    u32x2 w = {0, 0};
-    if (a.bias && column < end) w = *(const u32x2*)((const char*)a.bias + (int64_t)(past + column) * 2);
-    return w;
+  auto write = [&](const auto& region, int i, const float(&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      u32x2 w;
+      w[0] = pack_pair<T>(v[4 * q], v[4 * q + 1]);
+      w[1] = pack_pair<T>(v[4 * q + 2], v[4 * q + 3]);
+      region.piece(4 * i + q, lane) = w;
+    }
+  };
+  // (of a block of 32 columns of C; columns past the end have no bias, and are not stored)
+  struct Bias {
+    u32x2 w[4];
+  };
+  auto bias_of = [&](int first, int past) {
+    Bias b;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int column = first + 8 * q + 4 * h;
+      b.w[q] = u32x2{0, 0};
+      if (column < a.n) b.w[q] = *(const u32x2*)((const char*)a.bias + (int64_t)(past + column) * 2);
+    }
+    return b;
+  };
+  auto add_bias = [&](const Bias& b, float(&v)[16]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float x[4];
+      unpack(b.w[q], x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] += x[e];
+    }
+  };
+  auto values = [](const f32x16& c, float(&v)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = c[e];
   };
   if constexpr (AFTER == After::kGated) {
     using Out = product::Region<2 * S::kM>;
-    const Out gates{mine}, values{mine + Out::kSize}, products{mine + 2 * Out::kSize};
+    const Out gates{mine}, others{mine + Out::kSize}, products{mine + 2 * Out::kSize};
     static_assert(3 * Out::kSize <= kWaveChunks, "");
+    Bias bias[S::kM];
+    if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i) bias[i] = bias_of(wave_column0 + i / 2 * 32, i % 2 * a.n);
+    }
 #pragma unroll
     for (int j = 0; j < S::kN; ++j) {
       const int at = wave_row0 + 32 * j;
 #pragma unroll
-      for (int i = 0; i < S::kM / 2; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int column = wave_column0 + 32 * i + 8 * q + 4 * h;
-          float g[4], u[4], b[4];
-          four(acc[2 * i][j], q, g);
-          four(acc[2 * i + 1][j], q, u);
-          unpack(bias_of(column, a.n, 0), b);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] += b[e];
-          unpack(bias_of(column, a.n, a.n), b);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] += b[e];
-          if (a.z) {
-            gates.piece(4 * i + q, lane) = pack(g);
-            values.piece(4 * i + q, lane) = pack(u);
-          }
-          activate(a.activation, g);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] *= u[e];
-          products.piece(4 * i + q, lane) = pack(g);
+      for (int i = 0; i < S::kM / 2; ++i) {
+        float g[16], u[16];
+        values(acc[2 * i][j], g);
+        values(acc[2 * i + 1][j], u);
+        if (a.bias) {
+          add_bias(bias[2 * i], g);
+          add_bias(bias[2 * i + 1], u);
         }
+        if (a.z) {
+          write(gates, i, g);
+          write(others, i, u);
+        }
+        activate(a.activation, g);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) g[e] *= u[e];
+        write(products, i, g);
+      }
       if (a.z) {
         gates.put(a.z, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
-        values.put((char*)a.z + n_bytes, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        others.put((char*)a.z + n_bytes, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
       }
       products.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
     }
@@ -254,6 +280,11 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
       if (gated) second.bring((const char*)a.z + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
     };
     const float factor = AFTER != After::kForward && a.scale ? a.scale[AFTER == After::kPlain] : 1.f;
+    Bias bias[S::kM];
+    if (AFTER == After::kForward && a.bias) {
+#pragma unroll
+      for (int i = 0; i < S::kM; ++i) bias[i] = bias_of(wave_column0 + 32 * i, 0);
+    }
     if (ahead) {
 #pragma unroll
       for (int j = 0; j < S::kN; ++j) bring(j);
@@ -268,45 +299,40 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
       }
       const Out first{mine + (ahead ? step * j : 0) * Out::kSize}, second{first.at + Out::kSize};
 #pragma unroll
-      for (int i = 0; i < S::kM; ++i)
+      for (int i = 0; i < S::kM; ++i) {
+        float v[16], x[16];
+        values(acc[i][j], v);
+        if (AFTER == After::kForward) {
+          if (a.bias) add_bias(bias[i], v);
+          if (keep) write(second, i, v);
+          activate(a.activation, v);
+          if (residual) {
+            read(first, i, x);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int column = wave_column0 + 32 * i + 8 * q + 4 * h;
-          float v[4], x[4];
-          four(acc[i][j], q, v);
-          if (AFTER != After::kForward) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= factor;
+            for (int e = 0; e < 16; ++e) v[e] += x[e];
           }
-          if (AFTER == After::kForward) {
-            unpack(bias_of(column, a.n, 0), x);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += x[e];
-            if (keep) second.piece(4 * i + q, lane) = pack(v);
-            activate(a.activation, v);
-            if (residual) {
-              unpack(first.piece(4 * i + q, lane), x);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] += x[e];
-            }
-          } else if (slope) {
-            float s[4], u[4];
-            unpack(first.piece(4 * i + q, lane), x);
-            activate_with_slope(a.activation, x, s);
-            if (gated) {
-              unpack(second.piece(4 * i + q, lane), u);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                x[e] *= v[e];
-                s[e] *= u[e];
-              }
-              second.piece(4 * i + q, lane) = pack(x);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= s[e];
-          }
-          first.piece(4 * i + q, lane) = pack(v);
+          for (int e = 0; e < 16; ++e) v[e] *= factor;
         }
+        if (slope) {
+          float s[16], u[16];
+          read(first, i, x);
+          activate_with_slope(a.activation, x, s);
+          if (gated) {
+            read(second, i, u);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              x[e] *= v[e];
+              s[e] *= u[e];
+            }
+            write(second, i, x);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] *= s[e];
+        }
+        write(first, i, v);
+      }
       if (keep) second.put(a.z, n_bytes, at, a.m, wave_column0, a.n, lane);
       if (gated) second.put((char*)a.out + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
       first.put(a.out, z_bytes, at, a.m, wave_column0, a.n, lane);
@@ -314,35 +340,57 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   }
 }
 
-// The shares' sums added up, and what follows: eight columns of a row to a lane.
-template <class T, After AFTER>
+// The shares' sums added up, and what follows: eight columns of a row to LANES lanes, which share out the shares where there are
+// few rows and columns.
+template <class T, After AFTER, int LANES>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams a) {
-  const int64_t groups = a.n / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= groups * a.m) return;
-  const int row = (int)(at / groups), c = (int)(at % groups) * 8;
+  constexpr int kGroups = 256 / LANES, kSides = AFTER == After::kGated ? 2 : 1;
+  __shared__ float part[LANES > 1 ? LANES : 1][LANES > 1 ? kGroups : 1][8 * kSides + 1];
+  const int64_t groups = a.n / 8;
+  const int own = threadIdx.x % kGroups, lane = threadIdx.x / kGroups;
+  const int64_t at = (int64_t)blockIdx.x * kGroups + own;
+  const bool there = at < groups * a.m;
+  const int row = there ? (int)(at / groups) : 0, c = there ? (int)(at % groups) * 8 : 0;
   float v[8], u[8];
-  auto total = [&](int column, float(&x)[8]) {
-    const float* from = a.sums + (int64_t)row * a.width + column;
+  auto total = [&](int column, float(&x)[8], int side) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    for (int s = 0; s < a.shares; ++s, from += (int64_t)a.m * a.width) {
-      const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
+    if (there) {
+      const float* from = a.sums + ((int64_t)lane * a.m + row) * a.width + column;
+#pragma unroll 4
+      for (int s = lane; s < a.shares; s += LANES, from += (int64_t)LANES * a.m * a.width) {
+        const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] += lo[i];
-        x[4 + i] += hi[i];
+        for (int i = 0; i < 4; ++i) {
+          x[i] += lo[i];
+          x[4 + i] += hi[i];
+        }
       }
     }
+    if (LANES > 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[lane][own][side * 8 + i] = x[i];
+    }
   };
-  total(c, v);
-  if (AFTER == After::kGated) total(a.n + c, u);
-  finish<T, AFTER>(a, row, c, v, u);
+  total(c, v, 0);
+  if (AFTER == After::kGated) total(a.n + c, u, kSides - 1);
+  if (LANES > 1) {
+    __syncthreads();
+    if (lane > 0) return;
+    for (int l = 1; l < LANES; ++l)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] += part[l][own][i];
+        if (kSides == 2) u[i] += part[l][own][8 * (kSides - 1) + i];
+      }
+  }
+  if (there) finish<T, AFTER>(a, row, c, v, u);
 }
 
 // ---- launches (nd_linear_types.hpp, compiled for each type by itself) -----------------------------------------
 
 struct LinearPlan {
-  int shape;  // 0 large, 1 medium, 2 small
+  int shape;  // 0 large, 1 medium, 2 small, 3 narrow
   int shares, share;
 };
 template <class T>

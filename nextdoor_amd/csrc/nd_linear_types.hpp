@@ -85,12 +85,19 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinearParams a) {
   }
 }
 
+constexpr int kLongSum = 2048;
+
 template <class T, After AFTER>
 hipError_t launch_few_rows_of(const LinearParams& a, hipStream_t stream) {
   const dim3 grid((a.n + 15) / 16);
-  if (a.m <= 16) few_rows_kernel<T, 1, AFTER, 8><<<grid, 512, 0, stream>>>(a);
-  else if (a.m <= 32) few_rows_kernel<T, 2, AFTER, 8><<<grid, 512, 0, stream>>>(a);
-  else few_rows_kernel<T, 4, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  if (a.m <= 16) {
+    if (a.k >= kLongSum) few_rows_kernel<T, 1, AFTER, 16><<<grid, 1024, 0, stream>>>(a);
+    else few_rows_kernel<T, 1, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  } else if (a.m <= 32) {
+    few_rows_kernel<T, 2, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  } else {
+    few_rows_kernel<T, 4, AFTER, 8><<<grid, 512, 0, stream>>>(a);
+  }
   return hipGetLastError();
 }
 template <class T>
@@ -179,12 +186,17 @@ template <class T, Layout LAYOUT, After AFTER>
 hipError_t launch_shape(const LinearParams& a, int shape, int shares, hipStream_t stream) {
   if (shape == 0) return launch_tiles<T, Large, LAYOUT, AFTER>(a, shares, stream);
   if (shape == 1) return launch_tiles<T, Medium, LAYOUT, AFTER>(a, shares, stream);
+  if constexpr (AFTER != After::kGated) {
+    if (shape == 3) return launch_tiles<T, Narrow, LAYOUT, AFTER>(a, shares, stream);
+  }
   return launch_tiles<T, Small, LAYOUT, AFTER>(a, shares, stream);
 }
 template <class T, After AFTER>
 hipError_t launch_join(const LinearParams& a, hipStream_t stream) {
-  const int64_t lanes = (int64_t)a.m * (a.n / 8);
-  linear_join_kernel<T, AFTER><<<(uint32_t)((lanes + 255) / 256), 256, 0, stream>>>(a);
+  const int64_t groups = (int64_t)a.m * (a.n / 8);
+  // (64 x 256 values of 16 shares: 7.5 us with a lane to eight values, for the reads of one lane follow each other; 3.3 with eight)
+  if (groups <= 1 << 14 && a.shares >= 4) linear_join_kernel<T, AFTER, 8><<<(uint32_t)((groups + 31) / 32), 256, 0, stream>>>(a);
+  else linear_join_kernel<T, AFTER, 1><<<(uint32_t)((groups + 255) / 256), 256, 0, stream>>>(a);
   return hipGetLastError();
 }
 

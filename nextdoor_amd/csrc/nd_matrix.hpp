@@ -78,10 +78,12 @@ __device__ __forceinline__ u32x4 pack_operand(const f32x16& c, int s) {
 // ---- LDS tiles ----------------------------------------------------------------------------------
 // A tile is rows of CHUNKS 16-byte chunks (4, 8, 16 or 32: 64 to 512 bytes).  Chunk c of row r is kept at
 // place c ^ tile_swizzle(r): sixteen consecutive rows read at one chunk (an operand by rows) and the 64 bytes of
-// four consecutive rows (an operand by columns) then both lie in different banks.
+// four consecutive rows (an operand by columns) then both lie in different banks.  24 chunks: by columns only (rows begin 128
+// bytes of the banks apart, so every second pair of them changes places with its neighbour).
 template <int CHUNKS>
 __device__ __forceinline__ constexpr int tile_swizzle(int r) {
-  return CHUNKS >= 16  ? ((r & 3) << 2) | ((r >> 2) & 3)
+  return CHUNKS == 24 ? ((r >> 1) & 1) << 2
+         : CHUNKS >= 16  ? ((r & 3) << 2) | ((r >> 2) & 3)
          : CHUNKS == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3)
                        : (r >> 2) & 3;
 }
