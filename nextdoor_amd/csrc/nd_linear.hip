@@ -11,47 +11,23 @@
 
 namespace nd {
 
-// ---- float16: what dz is held times ----------------------------------------------------------------------------
-
-// The largest finite |dout| of a share of the rows.
-__global__ __launch_bounds__(256) void largest_kernel(const char* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* parts) {
+// float16: what dz is held times.  scale[0] = the power of two that takes the largest of all parts to between 1/2 and 1 (1, if that is
+// 0), scale[1] = one over it.
+__global__ __launch_bounds__(256) void scale_kernel(const float* parts, int64_t n, float* scale) {
   __shared__ float wave[4];
   float most = 0.f;
-  const int groups = columns / 8;
-  const int64_t n = rows * groups;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const u32x4 w = *(const u32x4*)(dout + i / groups * row_bytes + i % groups * 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float lo = fabsf(unpack_low<_Float16>(w[j])), hi = fabsf(unpack_high<_Float16>(w[j]));
-      most = fmaxf(most, fmaxf(lo < INFINITY ? lo : 0.f, hi < INFINITY ? hi : 0.f));
-    }
-  }
+  for (int64_t i = threadIdx.x; i < n; i += 256) most = fmaxf(most, parts[i]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = most;
   __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.x] = fmaxf(fmaxf(wave[0], wave[1]), fmaxf(wave[2], wave[3]));
-}
-// scale[0] = the power of two that takes the largest of all to between 1/2 and 1 (1, if that is 0), scale[1] = one over it.
-__global__ __launch_bounds__(64) void scale_kernel(const float* parts, int n, float* scale) {
-  float most = 0.f;
-  for (int i = threadIdx.x; i < n; i += 64) most = fmaxf(most, parts[i]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   if (threadIdx.x == 0) {
+    most = fmaxf(fmaxf(wave[0], wave[1]), fmaxf(wave[2], wave[3]));
     int power = 0;
     if (most > 0.f) frexpf(most, &power);
     scale[0] = ldexpf(1.f, -power);
     scale[1] = ldexpf(1.f, power);
   }
-}
-hipError_t launch_scale(const void* dout, int64_t dout_bytes, int64_t rows, int32_t columns, float* parts, float* scale, hipStream_t stream) {
-  const int64_t turns = (rows * (columns / 8) + 1023) / 1024;
-  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(kLargestParts, turns));
-  largest_kernel<<<blocks, 256, 0, stream>>>((const char*)dout, dout_bytes, rows, columns, parts);
-  scale_kernel<<<1, 64, 0, stream>>>(parts, blocks, scale);
-  return hipGetLastError();
 }
 
 namespace {
@@ -79,15 +55,16 @@ double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
   return full * (rounds * c.full + c.once) + (rest ? rounds * last + c.once : 0);
 }
 
-LinearPlan plan_of(int64_t m, int64_t n, int64_t k, bool gated) {
+LinearPlan plan_of(int64_t m, int64_t n, int64_t k, After after) {
+  const bool gated = after == After::kGated, pairs = gated || after == After::kSlope;
   const int64_t rounds = std::max<int64_t>(1, (k + 63) / 64), columns = gated ? 2 * n : n;
   LinearPlan best = {0, 1, (int)(rounds * 64)};
   double least = INFINITY;
   for (int shape = 0; shape < 4; ++shape) {
     const ShapeCost& c = kShapes[shape];
     const int64_t tiles = ((m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
-    for (int64_t want = 1; want <= kMostShares; want = want < 4 ? want + 1 : want * 3 / 2) {
-      if (shape == 3 && gated && want == 1) continue;  // (there pairs of columns are 64 apart)
+    for (int64_t want = 1; want <= (after == After::kSlope ? 1 : kMostShares); want = want < 4 ? want + 1 : want * 3 / 2) {
+      if (shape == 3 && pairs && want == 1) continue;  // (columns in pairs of 32)
       const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
       if (shares != want && want > 1) continue;
       double time = time_of(c, tiles * shares, each);
@@ -108,6 +85,9 @@ int64_t row_shares(int64_t rows, int64_t columns) {
   const int64_t across = (columns + 63) / 64;
   return std::max<int64_t>(1, std::min<int64_t>({(rows + 63) / 64, std::max<int64_t>(1, 2048 / across), (int64_t)65535}));
 }
+
+// Workgroups of a survey of a matrix.
+int64_t survey_parts(int64_t rows, int64_t columns) { return row_shares(rows, columns) * ((columns + kSlopeColumns - 1) / kSlopeColumns); }
 
 // ---- calls --------------------------------------------------------------------------------------------------------
 
@@ -133,23 +113,27 @@ struct Call {
     }
     LinearParams p = a;
     p.sums = sums;
-    product(p, Layout::kRows, after, plan_of(a.m, a.n, a.k, after == After::kGated));
+    product(p, Layout::kRows, after, plan_of(a.m, a.n, a.k, after));
   }
-  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums) {
+  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, float* parts) {
     const int64_t shares = row_shares(a.m, a.n);
-    note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, stream) : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, stream));
+    note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, parts, stream)
+              : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, parts, stream));
   }
-  void column_join(const float* sums, int64_t rows, int64_t columns, const float* scale, void* out) {
-    const int64_t shares = row_shares(rows, columns);
+  void column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out) {
     note(bf16 ? launch_column_join<__bf16>(sums, shares, columns, scale, out, stream) : launch_column_join<_Float16>(sums, shares, columns, scale, out, stream));
   }
-  // The sums of the rows of a matrix [rows][columns].
-  void column_sums(const void* matrix, int64_t row_bytes, int64_t rows, int32_t columns, const float* scale, float* sums, void* out) {
+  // Of dout [rows][columns]: the sums of its rows, unless out is null, and what dz is held times, unless scale is.
+  void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts, float* scale) {
     LinearParams p = {};
     p.m = (int32_t)rows;
     p.n = columns;
-    slope(p, matrix, row_bytes, sums);
-    column_join(sums, rows, columns, scale, out);
+    slope(p, dout, row_bytes, out ? sums : nullptr, scale ? parts : nullptr);
+    if (out) column_join(sums, row_shares(rows, columns), columns, nullptr, out);
+    if (scale) {
+      scale_kernel<<<1, 256, 0, stream>>>(parts, survey_parts(rows, columns), scale);
+      note(hipGetLastError());
+    }
   }
   // dx [rows][dim] = dz weight;  dweight [out][dim] = dz^T x
   void gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, const float* scale, void* dx, float* sums) {
@@ -164,7 +148,7 @@ struct Call {
     p.scale = scale;
     p.out = dx;
     p.sums = sums;
-    product(p, Layout::kWeightColumns, After::kPlain, plan_of(rows, dim, out, false));
+    product(p, Layout::kWeightColumns, After::kPlain, plan_of(rows, dim, out, After::kPlain));
   }
   void gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, const float* scale,
                           void* dweight, float* sums) {
@@ -179,7 +163,7 @@ struct Call {
     p.scale = scale;
     p.out = dweight;
     p.sums = sums;
-    product(p, Layout::kColumns, After::kPlain, plan_of(out, dim, rows, false));
+    product(p, Layout::kColumns, After::kPlain, plan_of(out, dim, rows, After::kPlain));
   }
   int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
 };
@@ -223,8 +207,9 @@ struct Layouter {
 };
 
 int64_t forward_sums(int64_t m, int64_t n, int64_t k, bool gated) {
-  return m <= kFewRows ? 0 : sums_bytes(plan_of(m, n, k, gated), m, gated ? 2 * n : n);
+  return m <= kFewRows ? 0 : sums_bytes(plan_of(m, n, k, gated ? After::kGated : After::kForward), m, gated ? 2 * n : n);
 }
+int64_t plain_sums(int64_t m, int64_t n, int64_t k) { return sums_bytes(plan_of(m, n, k, After::kPlain), m, n); }
 
 // ---- linear ---------------------------------------------------------------------------------------------------------
 
@@ -239,11 +224,10 @@ LinearWork work_of(const nd_linear* a, bool backward) {
   } else {
     const bool active = a->activation != ND_NO_ACTIVATION;
     w.dz = l.take(active ? a->rows * a->out_dim * 2 : 0);
-    w.products = l.take(std::max(a->dx ? sums_bytes(plan_of(a->rows, a->dim, a->out_dim, false), a->rows, a->dim) : 0,
-                                 a->dweight ? sums_bytes(plan_of(a->out_dim, a->dim, a->rows, false), a->out_dim, a->dim) : 0));
+    w.products = l.take(std::max(a->dx ? plain_sums(a->rows, a->dim, a->out_dim) : 0, a->dweight ? plain_sums(a->out_dim, a->dim, a->rows) : 0));
     w.rows = l.take(a->dbias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
     const bool scaled = active && a->dtype == ND_F16;
-    w.parts = l.take(scaled ? kLargestParts * 4 : 0);
+    w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
     w.scale = l.take(scaled ? 8 : 0);
   }
   w.bytes = l.bytes;
@@ -295,7 +279,7 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
   if (active && (a->dx || a->dweight || a->dbias)) {
     if (!call.bf16) {
       scale = (const float*)(work + w.scale);
-      call.note(launch_scale(a->dout, dz_bytes, a->rows, a->out_dim, (float*)(work + w.parts), (float*)(work + w.scale), call.stream));
+      call.survey(a->dout, dz_bytes, a->rows, a->out_dim, nullptr, nullptr, (float*)(work + w.parts), (float*)(work + w.scale));
     }
     LinearParams p = {};
     p.m = (int32_t)a->rows;
@@ -304,12 +288,12 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
     p.z = a->z;
     p.scale = scale;
     p.out = work + w.dz;
-    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr);
-    if (a->dbias) call.column_join(rows, a->rows, a->out_dim, nullptr, a->dbias);
+    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr, nullptr);
+    if (a->dbias) call.column_join(rows, row_shares(a->rows, a->out_dim), a->out_dim, nullptr, a->dbias);
     dz = work + w.dz;
     dz_bytes = (int64_t)a->out_dim * 2;
   } else if (a->dbias) {
-    call.column_sums(a->dout, dz_bytes, a->rows, a->out_dim, nullptr, rows, a->dbias);
+    call.survey(a->dout, dz_bytes, a->rows, a->out_dim, rows, a->dbias, nullptr, nullptr);
   }
   if (a->dx) call.gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, scale, a->dx, sums);
   if (a->dweight) call.gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, scale, a->dweight, sums);
@@ -318,8 +302,15 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
 
 // ---- mlp --------------------------------------------------------------------------------------------------------------
 
+// The product that makes dz, and the shares of the rows whose sums it leaves.
+LinearPlan slope_plan(const nd_mlp* a) { return plan_of(a->rows, a->inner, a->out_dim, After::kSlope); }
+int64_t slope_shares(const nd_mlp* a) {
+  const int shape = slope_plan(a).shape, rows = kShapes[shape].m, waves = shape == 0 ? Large::kWavesN : shape == 1 ? Medium::kWavesN : Small::kWavesN;
+  return (a->rows + rows - 1) / rows * waves;
+}
+
 struct MlpWork {
-  int64_t dz, products, rows, parts, scale, bytes;
+  int64_t dz, products, rows, columns, parts, scale, bytes;
 };
 MlpWork work_of(const nd_mlp* a, bool backward) {
   MlpWork w = {};
@@ -328,20 +319,13 @@ MlpWork work_of(const nd_mlp* a, bool backward) {
   if (!backward) {
     w.products = l.take(std::max(forward_sums(a->rows, a->inner, a->dim, a->gated), forward_sums(a->rows, a->out_dim, a->inner, false)));
   } else {
-    const bool first = a->dx || a->dup || a->dup_bias;
+    const bool first = a->dx || a->dup || a->dup_bias, scaled = first && a->dtype == ND_F16;
     w.dz = l.take(first ? a->rows * wide * 2 : 0);
-    int64_t most = 0;
-    auto product = [&](bool wanted, int64_t m, int64_t n, int64_t k) {
-      if (wanted) most = std::max(most, sums_bytes(plan_of(m, n, k, false), m, n));
-    };
-    product(first, a->rows, a->inner, a->out_dim);
-    product(a->dx, a->rows, a->dim, wide);
-    product(a->dup, wide, a->dim, a->rows);
-    product(a->ddown, a->out_dim, a->inner, a->rows);
-    w.products = l.take(most);
-    w.rows = l.take(std::max(a->dup_bias ? row_shares(a->rows, wide) * wide * 4 : 0, a->ddown_bias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0));
-    const bool scaled = first && a->dtype == ND_F16;
-    w.parts = l.take(scaled ? kLargestParts * 4 : 0);
+    w.products = l.take(std::max({a->dx ? plain_sums(a->rows, a->dim, wide) : 0, a->dup ? plain_sums(wide, a->dim, a->rows) : 0,
+                                  a->ddown ? plain_sums(a->out_dim, a->inner, a->rows) : 0}));
+    w.rows = l.take(a->ddown_bias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
+    w.columns = l.take(a->dup_bias ? std::max<int64_t>(1, slope_shares(a)) * wide * 4 : 0);
+    w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
     w.scale = l.take(scaled ? 8 : 0);
   }
   w.bytes = l.bytes;
@@ -402,16 +386,13 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     call.forward(r, After::kForward, sums);
     return call.done();
   }
-  float* rows = (float*)(work + w.rows);
   const int64_t dout_bytes = a->dout_row * 2;
-  if (a->ddown_bias) call.column_sums(a->dout, dout_bytes, a->rows, a->out_dim, nullptr, rows, a->ddown_bias);
+  float* scale = first && !call.bf16 ? (float*)(work + w.scale) : nullptr;
+  if (a->ddown_bias || scale)
+    call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, (float*)(work + w.parts), scale);
   if (a->ddown) call.gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, sums);
   if (!first) return call.done();
-  const float* scale = nullptr;
-  if (!call.bf16) {
-    scale = (const float*)(work + w.scale);
-    call.note(launch_scale(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.parts), (float*)(work + w.scale), call.stream));
-  }
+  float* columns = a->dup_bias ? (float*)(work + w.columns) : nullptr;
   LinearParams p = {};
   p.p = a->down;
   p.p_bytes = inner_bytes;
@@ -424,11 +405,11 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   p.gated = a->gated;
   p.z = slope ? a->z : nullptr;
   p.out = work + w.dz;
-  p.sums = sums;
   p.scale = scale;
-  call.product(p, Layout::kWeightColumns, After::kSlope, plan_of(a->rows, a->inner, a->out_dim, false));
+  p.column_sums = columns;
+  call.product(p, Layout::kWeightColumns, After::kSlope, slope_plan(a));
   const char* dz = work + w.dz;
-  if (a->dup_bias) call.column_sums(dz, wide_bytes, a->rows, wide, scale, rows, a->dup_bias);
+  if (columns) call.column_join(columns, slope_shares(a), wide, scale, a->dup_bias);
   if (a->dx) call.gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, scale, a->dx, sums);
   if (a->dup) call.gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, scale, a->dup, sums);
   return call.done();

@@ -7,7 +7,8 @@
 // Three products of the same tiles (nd_product.hpp): both operands by rows (forward), the weights by columns (gradient of x),
 // both by columns (gradient of the weights).  What follows a product is done to its results before they leave the registers.
 // Sums are held in 32 bits; z, h and dz, which the next product or the backward pass reads, are rounded to 16 bits once, as
-// the results are.  float16: dz is held times a power of two that takes max |dy| to between 1/2 and 1, so that the small
+// the results are; but the z of a gated part, of which g and u are both factors of dz, keeps the upper 24 bits of 32: rounded to
+// bfloat16 they had brought the gradients' error from 2.4e-3 to 3.0e-3 (1.7e-3 is that of rounding them alone).  float16: dz is held times a power of two that takes max |dy| to between 1/2 and 1, so that the small
 // gradients of a mean over many rows are not lost below 2^-14; what is made of it is divided by that in 32 bits.
 #pragma once
 
@@ -27,12 +28,50 @@ struct LinearParams {
   const void *bias, *residual;
   int64_t residual_bytes;  // of a row
   void* out;
-  void* z;  // forward: written unless null; backward: read.  [m][n], gated [m][2 n]
+  void* z;  // forward: written unless null; backward: read.  [m][n]; gated: rows of 6 n bytes, see Upper24
   const float* scale;  // null: 1; kSlope: the sums are multiplied with scale[0]; kPlain: with scale[1], one over it
   // shares of the sum: share s has places s * share .. and leaves [m][width] values in 32 bits
   float* sums;
   int32_t shares, share, width;
+  float* column_sums;  // kSlope, unless null: sums of 32 kN rows of dz, [share of the rows][columns of dz]
 };
+
+// Rows of z of a gated part: the upper 16 bits of g (n of them), of u, and of every 8 places 16 bytes with the next 8 bits: four
+// of g, four of u, and of the other four places the same.
+struct Upper24 {
+  static __device__ __forceinline__ u32x2 upper(const float* v) {
+    u32x2 w;
+    w[0] = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302);
+    w[1] = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302);
+    return w;
+  }
+  static __device__ __forceinline__ uint32_t next(const float* v) {
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x0c0c0501);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100);
+  }
+  static __device__ __forceinline__ void value(u32x2 upper, uint32_t next, float* v) {
+    v[0] = __uint_as_float(__builtin_amdgcn_perm(upper[0], next, 0x0504000c));
+    v[1] = __uint_as_float(__builtin_amdgcn_perm(upper[0], next, 0x0706010c));
+    v[2] = __uint_as_float(__builtin_amdgcn_perm(upper[1], next, 0x0504020c));
+    v[3] = __uint_as_float(__builtin_amdgcn_perm(upper[1], next, 0x0706030c));
+  }
+};
+
+// The sums of 16 values over the 32 lanes of a half: lane l has that of value l & 15.  Each step sends half of the values on.
+__device__ __forceinline__ float sums_of_rows(const float (&v)[16], int lane) {
+  auto other = [](float x, auto how) { return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), decltype(how)::value, 0xf, 0xf, true)); };
+  float a[8], b[4], c[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = (lane & 8 ? v[8 + i] : v[i]) + other(lane & 8 ? v[i] : v[8 + i], std::integral_constant<int, 0x140>());  // lane 15 - l
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = (lane & 4 ? a[4 + i] : a[i]) + other(lane & 4 ? a[i] : a[4 + i], std::integral_constant<int, 0x141>());  // 7 - l
+#pragma unroll
+  for (int i = 0; i < 2; ++i) c[i] = (lane & 2 ? b[2 + i] : b[i]) + other(lane & 2 ? b[i] : b[2 + i], std::integral_constant<int, 0x4e>());  // l ^ 2
+  const float d = (lane & 1 ? c[1] : c[0]) + other(lane & 1 ? c[0] : c[1], std::integral_constant<int, 0xb1>());  // l ^ 1
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(d), __float_as_uint(d), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // What follows the sums v (gated: and u) of columns c .. c + 7 of a row.
 template <class T, After AFTER>
@@ -55,9 +94,8 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
   const int64_t n_bytes = (int64_t)a.n * 2;
   float x[8];
   if (!kForward && a.scale) {
-    const float factor = a.scale[AFTER == After::kPlain];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= factor;
+    for (int i = 0; i < 8; ++i) v[i] *= a.scale[1];
   }
   if (kForward && a.bias) {
     unpack(*at(a.bias, 0, c), x);
@@ -79,30 +117,16 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
     }
   } else if (AFTER == After::kGated) {
     if (a.z) {
-      *at(a.z, 2 * n_bytes, c) = pack(v);
-      *at(a.z, 2 * n_bytes, a.n + c) = pack(u);
+      const u32x2 g0 = Upper24::upper(v), g1 = Upper24::upper(v + 4), u0 = Upper24::upper(u), u1 = Upper24::upper(u + 4);
+      *at(a.z, 3 * n_bytes, c) = u32x4{g0[0], g0[1], g1[0], g1[1]};
+      *at(a.z, 3 * n_bytes, a.n + c) = u32x4{u0[0], u0[1], u1[0], u1[1]};
+      *at(a.z, 3 * n_bytes, 2 * a.n + c) = u32x4{Upper24::next(v), Upper24::next(u), Upper24::next(v + 4), Upper24::next(u + 4)};
     }
     activate(a.activation, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= u[i];
-  } else if (AFTER == After::kSlope && a.z) {
-    float slope[8];
-    unpack(*at(a.z, a.gated ? 2 * n_bytes : n_bytes, c), x);
-    activate_with_slope(a.activation, x, slope);
-    if (a.gated) {
-      unpack(*at(a.z, 2 * n_bytes, a.n + c), u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] *= v[i];
-        v[i] *= u[i] * slope[i];
-      }
-      *at(a.out, 2 * n_bytes, a.n + c) = pack(x);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= slope[i];
-    }
   }
-  *at(a.out, AFTER == After::kSlope && a.gated ? 2 * n_bytes : n_bytes, c) = pack(v);
+  *at(a.out, n_bytes, c) = pack(v);
 }
 
 // ---- a tile of C to a workgroup ---------------------------------------------------------------------------
@@ -121,7 +145,10 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   constexpr bool kGated = AFTER == After::kGated;
   constexpr int kColumns = kGated ? S::kTileM / 2 : S::kTileM;  // of C to a tile
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  __shared__ u32x4 tiles[S::kLdsChunks];
+  // (what follows a product wants room for its results: two regions of a wave, and five of 64 columns where a slope is read)
+  constexpr int kWaves = S::kThreads / 64, kRoom = AFTER == After::kSlope ? 5 * product::Region<8>::kSize : S::kWaveResults;
+  constexpr int kWaveChunks = S::kTileChunks / kWaves > kRoom ? S::kTileChunks / kWaves : kRoom;
+  __shared__ u32x4 tiles[kWaveChunks * kWaves];
   // Bands of eight tiles of rows, in a band column after column: the tiles that a die works on at a time (32 or more) share few rows
   // of both operands.  Shares of a sum one after another.
   uint32_t block = block_by_die();
@@ -146,7 +173,6 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   }
   product::meet();
   // ---- the results: wave's rows from wave_row0 on, columns from wave_column0 on
-  constexpr int kWaveChunks = S::kLdsChunks / (S::kThreads / 64);
   u32x4* mine = tiles + wave * kWaveChunks;
   const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN, wave_column0 = column0 + wave / S::kWavesN * (kColumns / S::kWavesM);
   const int h = lane >> 5;
@@ -227,8 +253,8 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   };
   if constexpr (AFTER == After::kGated) {
     using Out = product::Region<2 * S::kM>;
-    const Out gates{mine}, others{mine + Out::kSize}, products{mine + 2 * Out::kSize};
-    static_assert(3 * Out::kSize <= kWaveChunks, "");
+    const Out gates{mine}, others{mine + Out::kSize}, next{mine + 2 * Out::kSize}, products{mine + 3 * Out::kSize};
+    static_assert(4 * Out::kSize <= kWaveChunks, "");
     Bias bias[S::kM];
     if (a.bias) {
 #pragma unroll
@@ -247,8 +273,12 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
           add_bias(bias[2 * i + 1], u);
         }
         if (a.z) {
-          write(gates, i, g);
-          write(others, i, u);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            gates.piece(4 * i + q, lane) = Upper24::upper(g + 4 * q);
+            others.piece(4 * i + q, lane) = Upper24::upper(u + 4 * q);
+            next.piece(4 * i + q, lane) = u32x2{Upper24::next(g + 4 * q), Upper24::next(u + 4 * q)};
+          }
         }
         activate(a.activation, g);
 #pragma unroll
@@ -256,30 +286,118 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
         write(products, i, g);
       }
       if (a.z) {
-        gates.put(a.z, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
-        others.put((char*)a.z + n_bytes, 2 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        gates.put(a.z, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        others.put((char*)a.z + n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        next.put((char*)a.z + 2 * n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
       }
       products.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
+    }
+  } else if constexpr (AFTER == After::kSlope) {
+    // Parts of 32 rows x 64 columns one after another: what is read of the next is on its way while one is worked on, and dz
+    // goes out from where z was.
+    using Part = product::Region<8>;
+    constexpr int kParts = S::kM / 2 * S::kN;
+    static_assert(S::kM % 2 == 0 && 5 * Part::kSize <= kWaveChunks, "");
+    const bool slope = a.z, gated = a.gated;  // (without a z, dz is what the product gives)
+    const bool whole = wave_row0 + 32 * S::kN <= a.m && wave_column0 + 32 * S::kM <= a.n;
+    const int64_t z_bytes = gated ? 3 * n_bytes : n_bytes, out_bytes = gated ? 2 * n_bytes : n_bytes;
+    const Part next{mine + 4 * Part::kSize};
+    auto region = [&](int part, int which) { return Part{mine + ((part & 1) * 2 + which) * Part::kSize}; };
+    auto row_of = [&](int part) { return wave_row0 + 32 * (part % S::kN); };
+    auto column_of = [&](int part) { return wave_column0 + 64 * (part / S::kN); };
+    auto bring = [&](int part) {
+      if (slope) region(part, 0).bring(a.z, z_bytes, row_of(part), a.m, column_of(part), a.n, lane);
+      if (gated) region(part, 1).bring((const char*)a.z + n_bytes, z_bytes, row_of(part), a.m, column_of(part), a.n, lane);
+    };
+    auto bring_next = [&](int part) {
+      if (gated) next.bring((const char*)a.z + 2 * n_bytes, z_bytes, row_of(part), a.m, column_of(part), a.n, lane);
+    };
+    const float factor = a.scale ? a.scale[0] : 1.f;
+    bring(0);
+    bring_next(0);
+    float own_sums[2], other_sums[2];
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const int j = part % S::kN, first = part / S::kN * 2;
+      // (behind the loads only the stores of the part before this one; all of them are there if the tile is whole)
+      if (part == 0 || !whole) product::wait_for_loads<0>();
+      else if (gated) product::wait_for_loads<2 * Part::kTurns>();
+      else product::wait_for_loads<Part::kTurns>();
+      if (part + 1 < kParts) bring(part + 1);
+      const Part mine0 = region(part, 0), mine1 = region(part, 1);
+      const bool counts = row_of(part) + (lane & 31) < a.m;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float v[16], x[16], s[16], u[16];
+        values(acc[first + i][j], v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= factor;
+        if (slope) {
+          if (gated) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const u32x2 low = next.piece(4 * i + q, lane);
+              Upper24::value(mine0.piece(4 * i + q, lane), low[0], x + 4 * q);
+              Upper24::value(mine1.piece(4 * i + q, lane), low[1], u + 4 * q);
+            }
+          } else {
+            read(mine0, i, x);
+          }
+          activate_with_slope(a.activation, x, s);
+          if (gated) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              x[e] *= v[e];
+              s[e] *= u[e];
+            }
+            write(mine1, i, x);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] *= s[e];
+        }
+        write(mine0, i, v);
+        if (a.column_sums) {  // of dz before it is rounded, over the parts with these columns
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            v[e] = counts ? v[e] : 0.f;
+            x[e] = counts ? x[e] : 0.f;
+          }
+          const float own = sums_of_rows(v, lane);
+          own_sums[i] = j == 0 ? own : own_sums[i] + own;
+          if (gated) {
+            const float other = sums_of_rows(x, lane);
+            other_sums[i] = j == 0 ? other : other_sums[i] + other;
+          }
+        }
+      }
+      if (part + 1 < kParts) bring_next(part + 1);
+      mine0.put(a.out, out_bytes, row_of(part), a.m, column_of(part), a.n, lane);
+      if (gated) mine1.put((char*)a.out + n_bytes, out_bytes, row_of(part), a.m, column_of(part), a.n, lane);
+      if (a.column_sums && j == S::kN - 1) {
+        const int64_t share_of_rows = (int64_t)(row0 / S::kTileN) * S::kWavesN + wave % S::kWavesN;
+        float* sums = a.column_sums + share_of_rows * (gated ? 2 * a.n : a.n);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int column = column_of(part) + 32 * i + 8 * ((lane & 15) / 4) + 4 * h + (lane & 3);
+          if (lane & 16 || column >= a.n) continue;
+          sums[column] = own_sums[i];
+          if (gated) sums[a.n + column] = other_sums[i];
+        }
+      }
     }
   } else {
     using Out = product::Region<4 * S::kM>;
     constexpr int kRegions = kWaveChunks / Out::kSize;
     static_assert(kRegions >= 2 && kRegions >= S::kN, "");
     const bool residual = AFTER == After::kForward && a.residual, keep = AFTER == After::kForward && a.z;
-    const bool slope = AFTER == After::kSlope && a.z, gated = slope && a.gated;  // (without a z, dz is what the product gives)
-    // Regions of rows j: what is read, and goes out again in the same place; with a second matrix one region further.  All
-    // rows are asked for at once where there are regions enough.
-    const int step = keep || gated ? 2 : 1;
+    // Regions of rows j: what is read, and goes out again in the same place; with z one region further.  All rows are asked for
+    // at once where there are regions enough.
+    const int step = keep ? 2 : 1;
     const bool ahead = step * S::kN <= kRegions;
-    const int64_t z_bytes = gated ? 2 * n_bytes : n_bytes;
     auto bring = [&](int j) {
-      const Out first{mine + (ahead ? step * j : 0) * Out::kSize}, second{first.at + Out::kSize};
-      const int at = wave_row0 + 32 * j;
-      if (residual) first.bring(a.residual, a.residual_bytes, at, a.m, wave_column0, a.n, lane);
-      if (slope) first.bring(a.z, z_bytes, at, a.m, wave_column0, a.n, lane);
-      if (gated) second.bring((const char*)a.z + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
+      if (residual) Out{mine + (ahead ? step * j : 0) * Out::kSize}.bring(a.residual, a.residual_bytes, wave_row0 + 32 * j, a.m, wave_column0, a.n, lane);
     };
-    const float factor = AFTER != After::kForward && a.scale ? a.scale[AFTER == After::kPlain] : 1.f;
+    const float factor = AFTER == After::kPlain && a.scale ? a.scale[1] : 1.f;
     Bias bias[S::kM];
     if (AFTER == After::kForward && a.bias) {
 #pragma unroll
@@ -288,14 +406,14 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
     if (ahead) {
 #pragma unroll
       for (int j = 0; j < S::kN; ++j) bring(j);
-      if (residual || slope) product::wait_for_loads<0>();
+      if (residual) product::wait_for_loads<0>();
     }
 #pragma unroll
     for (int j = 0; j < S::kN; ++j) {
       const int at = wave_row0 + 32 * j;
       if (!ahead) {
         bring(j);
-        if (residual || slope) product::wait_for_loads<0>();
+        if (residual) product::wait_for_loads<0>();
       }
       const Out first{mine + (ahead ? step * j : 0) * Out::kSize}, second{first.at + Out::kSize};
 #pragma unroll
@@ -315,27 +433,10 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] *= factor;
         }
-        if (slope) {
-          float s[16], u[16];
-          read(first, i, x);
-          activate_with_slope(a.activation, x, s);
-          if (gated) {
-            read(second, i, u);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              x[e] *= v[e];
-              s[e] *= u[e];
-            }
-            write(second, i, x);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] *= s[e];
-        }
         write(first, i, v);
       }
       if (keep) second.put(a.z, n_bytes, at, a.m, wave_column0, a.n, lane);
-      if (gated) second.put((char*)a.out + n_bytes, z_bytes, at, a.m, wave_column0, a.n, lane);
-      first.put(a.out, z_bytes, at, a.m, wave_column0, a.n, lane);
+      first.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
     }
   }
 }
@@ -397,14 +498,14 @@ template <class T>
 hipError_t launch_linear(const LinearParams& a, Layout layout, After after, const LinearPlan& plan, hipStream_t stream);
 template <class T>
 hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
-// dz = dout a'(z) times scale[0], if there is a z, and sums of its rows (times 1).
+// dz = dout a'(z) times scale[0], if there is a z, and unless they are null sums of its rows (times 1), and the largest finite
+// |dout| of each workgroup.
 template <class T>
-hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, hipStream_t stream);
+hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts, hipStream_t stream);
+constexpr int kSlopeColumns = 64;  // of a workgroup there
 // scale: null, or as above: the sums are multiplied with scale[1].
 template <class T>
 hipError_t launch_column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out, hipStream_t stream);
-constexpr int kLargestParts = 512;
-hipError_t launch_scale(const void* dout, int64_t dout_bytes, int64_t rows, int32_t columns, float* parts, float* scale, hipStream_t stream);
 
 constexpr int kFewRows = 64;  // at most: a kernel of its own, which reads the weights once and keeps a sum in many waves
 

@@ -27,9 +27,7 @@ struct Shape {
   static constexpr int kThreads = 64 * WAVES_M * WAVES_N;
   static constexpr int kTileM = 32 * WAVES_M * M, kTileN = 32 * WAVES_N * N;
   static constexpr int kTileChunks = STAGES * (kTileM + kTileN) * DEPTH / 8;
-  // LDS has room for the tiles, and afterwards for two regions of results of each wave
-  static constexpr int kWaveResults = 2 * 32 * (M > 2 ? 16 : 8), kResults = kWaveResults * WAVES_M * WAVES_N;
-  static constexpr int kLdsChunks = kTileChunks > kResults ? kTileChunks : kResults;
+  static constexpr int kWaveResults = 2 * 32 * (M > 2 ? 16 : 8);  // chunks of two regions of a wave's results
   static_assert(DEPTH == 64 && AHEAD >= 1 && AHEAD <= 3 && LOAD_SPAN <= 3 * M * N && STAGES >= 2, "");
 };
 

@@ -411,14 +411,14 @@ def _norm(x, weight, bias, eps, others=()):
         raise NextDoorError("layer norm: x has no rows")
     dim = x.shape[-1]
     weight_dtype = dtype
-    for name, t in (("weight", weight), ("bias", bias)):
+    for t in (weight, bias):
         if t is None:
             continue
         if t.shape != (dim,):
-            raise NextDoorError("layer norm: %s is not [%d]" % (name, dim))
-        if t.dtype is not dtype and t.dtype is not torch.float32:
-            raise NextDoorError("layer norm: %s is neither of the type of x nor float32" % name)
+            raise NextDoorError("layer norm: weight or bias is not [%d]" % dim)
         weight_dtype = t.dtype
+        if weight_dtype is not dtype and weight_dtype is not torch.float32:
+            raise NextDoorError("layer norm: weight or bias is neither of the type of x nor float32")
     if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise NextDoorError("layer norm: weight and bias are of different types")
     if not 0.0 <= eps < math.inf:
@@ -426,7 +426,7 @@ def _norm(x, weight, bias, eps, others=()):
     if not 1 <= dim <= 16384:
         raise NextDoorError("layer norm: rows of 1 to 16384 values, %d given" % dim)
     x, x_row = _rows_in_place(x, dim, 1)
-    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+    weight, bias = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
     return index, x, (x.shape[0], dim, _DTYPES[dtype], _DTYPES[weight_dtype], eps), x_row, weight, bias
 
 
@@ -440,8 +440,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     of that type or float32.  mean and rstd: [rows], float32, for the backward pass.  Sums are in 32 bits, results rounded
     once."""
     index, rows, fields, x_row, weight, bias = _norm(x, weight, bias, eps)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = (torch.empty(fields[0], dtype=torch.float32, device=x.device) for _ in range(2))
+    device = x.device
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean, rstd = torch.empty(fields[0], dtype=torch.float32, device=device), torch.empty(fields[0], dtype=torch.float32, device=device)
     _run(index, _library().nd_layer_norm_forward,
          LayerNorm(*fields, x_row, 0, rows.data_ptr(), _pointer(weight), _pointer(bias), out.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
     return out, mean, rstd
@@ -524,9 +525,8 @@ def _matrix(t):
     filled up with zeros, which costs a copy."""
     if t is None:
         return None
-    fill = [n for size in reversed(t.shape) for n in (0, -size % 8)]
-    if any(fill):
-        t = torch.nn.functional.pad(t, fill)
+    if any([size % 8 for size in t.shape]):
+        t = torch.nn.functional.pad(t, [n for size in reversed(t.shape) for n in (0, -size % 8)])
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
@@ -543,6 +543,11 @@ def _check_rows(what, name, t, shape, dtype):
         raise NextDoorError("%s: %s is of another shape or type than the result" % (what, name))
 
 
+def _result(x, wanted, *shape):
+    """Room for a result that the kernels write as a matrix or vector of `shape`, in the shape that is wanted where both are the same."""
+    return torch.empty(wanted if wanted[-1] == shape[-1] else shape, dtype=x.dtype, device=x.device)
+
+
 def _cut(t, *shape):
     """The part of a filled-up result that was asked for."""
     if t is None or t.shape == shape:
@@ -550,6 +555,11 @@ def _cut(t, *shape):
     for i, n in enumerate(shape):
         t = t.narrow(i, 0, n)
     return t.contiguous()
+
+
+def _shaped(t, rows, dim, wanted):
+    """The rows of a result of :func:`_result` as the caller wants them."""
+    return t if t is None or t.shape == wanted else _cut(t, rows, dim).view(wanted)
 
 
 def _linear_arguments(what, x, weight, bias):
@@ -583,14 +593,14 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep=Fa
         residual, residual_row = _vectors_in_place(residual, out_dim)
     weight, bias = _matrix(weight), _matrix(bias)
     n = rows.shape[0]
-    out = torch.empty((n, wide), dtype=x.dtype, device=x.device)
+    out = _result(x, shape, n, wide)
     z = torch.empty((n, wide), dtype=x.dtype, device=x.device) if keep and code else None
     a = Linear(n, weight.shape[1], wide, _DTYPES[x.dtype], code, x_row, residual_row, 0, rows.data_ptr(), weight.data_ptr(), _pointer(bias),
                _pointer(residual), out.data_ptr(), _pointer(z))
     workspace = _room(a, _library().nd_linear_workspace(a, 0), x.device)
     _run(index, _library().nd_linear_forward, a)
     del workspace
-    out = _cut(out, n, out_dim).view(shape)
+    out = _shaped(out, n, out_dim, shape)
     return (out, z) if keep else out
 
 
@@ -609,7 +619,7 @@ def linear_backward(dout, x, weight, z=None, activation=None, with_bias=True, ne
     n, wide, high = rows.shape[0], out_dim + -out_dim % 8, dim + -dim % 8
     if code and not (z is not None and z.shape == (n, wide) and z.is_contiguous()):
         raise NextDoorError("linear: z is not what a forward pass kept")
-    dx = torch.empty((n, high), dtype=x.dtype, device=x.device) if needs[0] else None
+    dx = _result(x, x.shape, n, high) if needs[0] else None
     dweight = torch.empty((wide, high), dtype=x.dtype, device=x.device) if needs[1] else None
     dbias = torch.empty(wide, dtype=x.dtype, device=x.device) if with_bias else None
     a = Linear(n, high, wide, _DTYPES[x.dtype], code, x_row, 0, dout_row, rows.data_ptr(), weight.data_ptr(), None, None, None,
@@ -617,8 +627,7 @@ def linear_backward(dout, x, weight, z=None, activation=None, with_bias=True, ne
     workspace = _room(a, _library().nd_linear_workspace(a, 1), x.device)
     _run(index, _library().nd_linear_backward, a)
     del workspace
-    dx = dx if dx is None else _cut(dx, n, dim).view(x.shape)
-    return dx, _cut(dweight, out_dim, dim), _cut(dbias, out_dim)
+    return _shaped(dx, n, dim, x.shape), _cut(dweight, out_dim, dim), _cut(dbias, out_dim)
 
 
 class _Linear(torch.autograd.Function):
@@ -682,7 +691,7 @@ def _up_cut(t, inner, gated, *rest):
 
 def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None, keep=False):
     """The feed-forward part of a block: ``h down^T + down_bias + residual``, or with ``keep`` (out, z, h), which the backward
-    pass reads.
+    pass reads (z of a gated part holds 24 bits of each value, as bytes).
 
     z = x up^T + up_bias; gated: ``h = activation(g) u`` with ``g, u = z.chunk(2, -1)``, else ``h = activation(z)``.  x: [..., dim];
     up: [2 inner or inner, dim]; down: [out_dim, inner]; activations, types and sizes as in :func:`linear_forward`.  Both
@@ -703,14 +712,18 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
     def empty(columns):
         return torch.empty((n, columns), dtype=x.dtype, device=x.device)
 
-    out, h = empty(wide), empty(down.shape[1])
-    z = empty(up.shape[0]) if keep and (gated or code) else None
+    out, h = _result(x, shape, n, wide), empty(down.shape[1])
+    z = None
+    if keep and gated:
+        z = torch.empty((n, 3 * up.shape[0]), dtype=torch.uint8, device=x.device)
+    elif keep and code:
+        z = empty(up.shape[0])
     a = Mlp(n, up.shape[1], down.shape[1], wide, _DTYPES[x.dtype], code, gated, x_row, residual_row, 0, rows.data_ptr(), up.data_ptr(),
             _pointer(up_bias), down.data_ptr(), _pointer(down_bias), _pointer(residual), out.data_ptr(), _pointer(z), h.data_ptr())
     workspace = _room(a, _library().nd_mlp_workspace(a, 0), x.device)
     _run(index, _library().nd_mlp_forward, a)
     del workspace
-    out = _cut(out, n, out_dim).view(shape)
+    out = _shaped(out, n, out_dim, shape)
     return (out, z, h) if keep else out
 
 
@@ -720,7 +733,7 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
     residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None.  The gradient of z
     is rounded to 16 bits before its products (float16: relative to max |dout|, and must stay below 65504 times that)."""
     index = _on_gpu("mlp", x, dout, up, down, h, *(() if z is None else (z,)))
-    _types("mlp", x, dout, up, down, z, h)
+    _types("mlp", x, dout, up, down, h)
     gated = bool(gated)
     dim, inner, out_dim, code = _mlp_arguments(x, up, down, None, None, activation, gated)
     _check_rows("mlp", "dout", dout, (*x.shape[:-1], out_dim), x.dtype)
@@ -730,13 +743,16 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
     n = rows.shape[0]
     if not (h.shape == (n, down.shape[1]) and h.is_contiguous()):
         raise NextDoorError("mlp: h is not what a forward pass kept")
-    if (gated or code) and not (z is not None and z.shape == (n, up.shape[0]) and z.is_contiguous()):
-        raise NextDoorError("mlp: z is not what a forward pass kept")
+    if gated or code:
+        kept = ((n, 3 * up.shape[0]), torch.uint8) if gated else ((n, up.shape[0]), x.dtype)
+        if z is None or (z.shape, z.dtype) != kept or not z.is_contiguous():
+            raise NextDoorError("mlp: z is not what a forward pass kept")
 
     def empty(need, *size):
         return torch.empty(size, dtype=x.dtype, device=x.device) if need else None
 
-    dx, dup, ddown = empty(needs[0], n, up.shape[1]), empty(needs[1], *up.shape), empty(needs[2], *down.shape)
+    dx = _result(x, x.shape, n, up.shape[1]) if needs[0] else None
+    dup, ddown = empty(needs[1], *up.shape), empty(needs[2], *down.shape)
     dup_bias, ddown_bias = empty(with_up_bias, up.shape[0]), empty(with_down_bias, down.shape[0])
     a = Mlp(n, up.shape[1], down.shape[1], down.shape[0], _DTYPES[x.dtype], code, gated, x_row, 0, dout_row, rows.data_ptr(), up.data_ptr(),
             None, down.data_ptr(), None, None, None, _pointer(z), h.data_ptr(), dout.data_ptr(), _pointer(dx), _pointer(dup),
@@ -744,8 +760,8 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
     workspace = _room(a, _library().nd_mlp_workspace(a, 1), x.device)
     _run(index, _library().nd_mlp_backward, a)
     del workspace
-    dx = dx if dx is None else _cut(dx, n, dim).view(x.shape)
-    return (dx, _up_cut(dup, inner, gated, dim), _cut(ddown, out_dim, inner), _up_cut(dup_bias, inner, gated), _cut(ddown_bias, out_dim))
+    return (_shaped(dx, n, dim, x.shape), _up_cut(dup, inner, gated, dim), _cut(ddown, out_dim, inner), _up_cut(dup_bias, inner, gated),
+            _cut(ddown_bias, out_dim))
 
 
 class _Mlp(torch.autograd.Function):

@@ -120,17 +120,20 @@ def mlp(x, up, down, up_bias=None, down_bias=None, name="silu", gated=True, resi
     if dout is not None:
         d = dout.double()
         dh, dh_off = _product(d, torch.zeros_like(d), dn)
-        kept = _rounded(z, z_off, unit, least) if gated or name else z_off
+        kept = z_off if name is None else _rounded(z, z_off, unit, least)
+        if gated:
+            kept = _rounded(z, z_off, 2.0 ** -15, 2.0 ** -126)
         _, _, a, a_off, slope, slope_off, v, v_off = hidden(z, kept)
         factor, factor_off = v * slope, v_off * slope.abs() + v.abs() * slope_off + v_off * slope_off
         dz, dz_off = dh * factor, dh_off * (factor.abs() + factor_off) + dh.abs() * factor_off
         if gated:
             dz = torch.cat([dz, dh * a], 1)
             dz_off = torch.cat([dz_off, dh_off * (a.abs() + a_off) + dh.abs() * a_off], 1)
-        dz_off = _rounded(dz, dz_off + 2.0 ** -22 * dz.abs(), unit, _held(d, least))
+        plain_off = dz_off + 2.0 ** -22 * dz.abs()
+        dz_off = _rounded(dz, plain_off, unit, _held(d, least))
         got["dx"], dx_off = _product(dz, dz_off, u)
         got["dup"], du_off = _product(dz.T, dz_off.T, x)
-        got["dup_bias"], db_off = dz.sum(0), dz_off.sum(0) + _sum_off(len(d)) * dz.abs().sum(0)
+        got["dup_bias"], db_off = dz.sum(0), plain_off.sum(0) + _sum_off(len(d)) * dz.abs().sum(0)
         dd, dd_off = _product(h.T, h_off.T, d)
         got["ddown"], dd_off = dd.T, dd_off.T
         got["ddown_bias"], de_off = d.sum(0), _sum_off(len(d)) * d.abs().sum(0)
