@@ -47,7 +47,7 @@ constexpr ShapeCost kShapes[4] = {{256, 256, 256, 1.05, 1.5, 1.5, 10.0},
                                   {64, 64, 768, 0.32, 0.4, 0.5, 3.0},
                                   {256, 192, 256, 0.9, 1.2, 1.2, 9.0}};
 constexpr int kMostShares = 128;
-constexpr double kJoin = 4.0, kJoinRate = 8e6;  // us of one more kernel; bytes a us of sums, written and read again
+constexpr double kJoin = 4.0, kJoinRate = 8e6, kLaunch = 3.0;  // us of adding sums; bytes a us of them, written and read again; us of a launch
 
 double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
   const int64_t full = groups / c.at_once, rest = groups % c.at_once;
@@ -55,30 +55,69 @@ double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
   return full * (rounds * c.full + c.once) + (rest ? rounds * last + c.once : 0);
 }
 
-LinearPlan plan_of(int64_t m, int64_t n, int64_t k, After after) {
-  const bool gated = after == After::kGated, pairs = gated || after == After::kSlope;
-  const int64_t rounds = std::max<int64_t>(1, (k + 63) / 64), columns = gated ? 2 * n : n;
-  LinearPlan best = {0, 1, (int)(rounds * 64)};
-  double least = INFINITY;
-  for (int shape = 0; shape < 4; ++shape) {
-    const ShapeCost& c = kShapes[shape];
-    const int64_t tiles = ((m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
-    for (int64_t want = 1; want <= (after == After::kSlope ? 1 : kMostShares); want = want < 4 ? want + 1 : want * 3 / 2) {
-      if (shape == 3 && pairs && want == 1) continue;  // (columns in pairs of 32)
-      const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
-      if (shares != want && want > 1) continue;
-      double time = time_of(c, tiles * shares, each);
-      if (shares > 1) time += kJoin + (double)shares * m * columns * 8 / kJoinRate;
-      if (time < least) {
-        least = time;
-        best = {shape, (int)shares, (int)(each * 64)};
-      }
+// A product C [m][n], sums over k.
+struct Task {
+  int64_t m, n, k;
+  After after;
+};
+struct Estimate {
+  LinearPlan plan;
+  int64_t groups, rounds;    // workgroups; rounds of each
+  double time, joined;       // us in all, and how much of it is what adds the shares
+};
+// The best number of shares with tiles of one shape.
+Estimate estimate(const Task& t, int shape) {
+  const ShapeCost& c = kShapes[shape];
+  const int64_t rounds = std::max<int64_t>(1, (t.k + 63) / 64), columns = t.after == After::kGated ? 2 * t.n : t.n;
+  const int64_t tiles = ((t.m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
+  Estimate best = {};
+  best.time = INFINITY;
+  for (int64_t want = 1; want <= (t.after == After::kSlope ? 1 : kMostShares); want = want < 4 ? want + 1 : want * 3 / 2) {
+    if (shape == 3 && want == 1 && (t.after == After::kGated || t.after == After::kSlope)) continue;  // (columns in pairs of 32)
+    const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
+    if (shares != want && want > 1) continue;
+    if (want > 1 && tiles * want > 4 * c.at_once) break;
+    const double joined = shares > 1 ? kJoin + (double)shares * t.m * columns * 8 / kJoinRate : 0;
+    const double time = time_of(c, tiles * shares, each) + joined;
+    if (time < best.time) best = {{shape, (int)shares, (int)(each * 64)}, tiles * shares, each, time, joined};
+  }
+  return best;
+}
+Estimate estimate(const Task& t) {
+  Estimate best = estimate(t, 0);
+  for (int shape = 1; shape < 4; ++shape) {
+    const Estimate e = estimate(t, shape);
+    if (e.time < best.time) best = e;
+  }
+  return best;
+}
+LinearPlan plan_of(const Task& t) { return estimate(t).plan; }
+
+// Two products of which neither needs the other, of one shape in one launch where that is faster.
+struct TwoPlans {
+  LinearPlan first, second;
+  bool together;
+};
+TwoPlans plan_two(const Task* a, const Task* b) {  // null: not wanted
+  TwoPlans best = {};
+  const Estimate x = a ? estimate(*a) : Estimate{}, y = b ? estimate(*b) : Estimate{};
+  best.first = x.plan;
+  best.second = y.plan;
+  if (!a || !b) return best;
+  double least = x.time + y.time + kLaunch;
+  for (int shape = 1; shape < 3; ++shape) {
+    const Estimate p = estimate(*a, shape), q = estimate(*b, shape);
+    if (p.groups + q.groups > 2 * kShapes[shape].at_once) continue;
+    const double time = time_of(kShapes[shape], p.groups + q.groups, std::max(p.rounds, q.rounds)) + p.joined + q.joined;
+    if (time < least) {
+      least = time;
+      best = {p.plan, q.plan, true};
     }
   }
   return best;
 }
 
-int64_t sums_bytes(const LinearPlan& p, int64_t m, int64_t columns) { return p.shares > 1 ? round_up(m * columns * 4 * p.shares, 256) : 0; }
+int64_t sums_bytes(const LinearPlan& p, int64_t m, int64_t columns) { return p.shares > 1 ? m * columns * 4 * p.shares : 0; }
 
 // Shares of the rows for the sums over them: workgroups of 64 columns, at least 64 rows to each, some thousand in all.
 int64_t row_shares(int64_t rows, int64_t columns) {
@@ -96,15 +135,14 @@ struct Call {
   bool bf16;
   hipStream_t stream;
   hipError_t error;
-  Call(const char* what_, int dtype, void* stream_) : what(what_), bf16(dtype == ND_BF16), stream((hipStream_t)stream_), error(hipSuccess) {}
+  Joins joins;
+  uint32_t join_blocks;
+  Call(const char* what_, int dtype, void* stream_)
+      : what(what_), bf16(dtype == ND_BF16), stream((hipStream_t)stream_), error(hipSuccess), joins{}, join_blocks(0) {}
   void note(hipError_t e) {
     if (error == hipSuccess) error = e;
   }
-  void product(const LinearParams& a, Layout layout, After after, const LinearPlan& plan) {
-    if (a.m == 0 || a.n == 0) return;
-    note(bf16 ? launch_linear<__bf16>(a, layout, after, plan, stream) : launch_linear<_Float16>(a, layout, after, plan, stream));
-  }
-  // out rows of a matrix by rows
+  // A product of a forward pass, whose columns are rows of a matrix.
   void forward(const LinearParams& a, After after, float* sums) {
     if (a.m == 0) return;
     if (a.m <= kFewRows) {
@@ -113,15 +151,40 @@ struct Call {
     }
     LinearParams p = a;
     p.sums = sums;
-    product(p, Layout::kRows, after, plan_of(a.m, a.n, a.k, after));
+    const LinearPlan plan = plan_of({a.m, a.n, a.k, after});
+    note(bf16 ? launch_linear<__bf16>(p, Layout::kRows, after, plan, stream) : launch_linear<_Float16>(p, Layout::kRows, after, plan, stream));
+  }
+  // What is to be added up at the end of the call.
+  void join(const float* sums, int64_t shares, int64_t values, const float* factor, void* out) {
+    Join& j = joins.job[joins.n++];
+    j = {sums, out, factor, values / 8, (int32_t)shares, 1, join_blocks};
+    // (few values: the reads of one lane follow each other)
+    if (j.groups <= 1 << 14 && shares >= 4) j.lanes = shares >= 64 && j.groups <= 1 << 10 ? 32 : 8;
+    join_blocks += (uint32_t)((j.groups * j.lanes + 255) / 256);
+  }
+  void add_up() {
+    if (joins.n > 0) note(bf16 ? launch_joins<__bf16>(joins, join_blocks, stream) : launch_joins<_Float16>(joins, join_blocks, stream));
+    joins.n = 0;
+  }
+  // One or two products of a backward pass (null: not wanted): by columns of the weights, and by columns.
+  void backward(const LinearParams* a, After after, const LinearParams* b, const TwoPlans& plans) {
+    if (a && a->m == 0) a = nullptr;
+    if (plans.together && a && b) {
+      note(bf16 ? launch_pair<__bf16>(*a, after, plans.first, *b, plans.second, stream) : launch_pair<_Float16>(*a, after, plans.first, *b, plans.second, stream));
+    } else {
+      if (a) one(*a, Layout::kWeightColumns, after, plans.first);
+      if (b) one(*b, Layout::kColumns, After::kPlain, plans.second);
+    }
+    if (a && plans.first.shares > 1) join(a->sums, plans.first.shares, (int64_t)a->m * a->n, a->scale ? a->scale + 1 : nullptr, a->out);
+    if (b && plans.second.shares > 1) join(b->sums, plans.second.shares, (int64_t)b->m * b->n, b->scale ? b->scale + 1 : nullptr, b->out);
+  }
+  void one(const LinearParams& a, Layout layout, After after, const LinearPlan& plan) {
+    note(bf16 ? launch_linear<__bf16>(a, layout, after, plan, stream) : launch_linear<_Float16>(a, layout, after, plan, stream));
   }
   void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, float* parts) {
     const int64_t shares = row_shares(a.m, a.n);
     note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, parts, stream)
               : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, parts, stream));
-  }
-  void column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out) {
-    note(bf16 ? launch_column_join<__bf16>(sums, shares, columns, scale, out, stream) : launch_column_join<_Float16>(sums, shares, columns, scale, out, stream));
   }
   // Of dout [rows][columns]: the sums of its rows, unless out is null, and what dz is held times, unless scale is.
   void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts, float* scale) {
@@ -129,44 +192,45 @@ struct Call {
     p.m = (int32_t)rows;
     p.n = columns;
     slope(p, dout, row_bytes, out ? sums : nullptr, scale ? parts : nullptr);
-    if (out) column_join(sums, row_shares(rows, columns), columns, nullptr, out);
+    if (out) join(sums, row_shares(rows, columns), columns, nullptr, out);
     if (scale) {
       scale_kernel<<<1, 256, 0, stream>>>(parts, survey_parts(rows, columns), scale);
       note(hipGetLastError());
     }
   }
-  // dx [rows][dim] = dz weight;  dweight [out][dim] = dz^T x
-  void gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, const float* scale, void* dx, float* sums) {
-    LinearParams p = {};
-    p.p = weight;
-    p.p_bytes = (int64_t)dim * 2;
-    p.q = dz;
-    p.q_bytes = dz_bytes;
-    p.m = (int32_t)rows;
-    p.n = dim;
-    p.k = out;
-    p.scale = scale;
-    p.out = dx;
-    p.sums = sums;
-    product(p, Layout::kWeightColumns, After::kPlain, plan_of(rows, dim, out, After::kPlain));
-  }
-  void gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, const float* scale,
-                          void* dweight, float* sums) {
-    LinearParams p = {};
-    p.p = x;
-    p.p_bytes = x_bytes;
-    p.q = dz;
-    p.q_bytes = dz_bytes;
-    p.m = out;
-    p.n = dim;
-    p.k = (int32_t)rows;
-    p.scale = scale;
-    p.out = dweight;
-    p.sums = sums;
-    product(p, Layout::kColumns, After::kPlain, plan_of(out, dim, rows, After::kPlain));
-  }
   int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
 };
+
+// dx [rows][dim] = dz weight;  dweight [out][dim] = dz^T x
+LinearParams gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, const float* scale, void* dx, float* sums) {
+  LinearParams p = {};
+  p.p = weight;
+  p.p_bytes = (int64_t)dim * 2;
+  p.q = dz;
+  p.q_bytes = dz_bytes;
+  p.m = (int32_t)rows;
+  p.n = dim;
+  p.k = out;
+  p.scale = scale;
+  p.out = dx;
+  p.sums = sums;
+  return p;
+}
+LinearParams gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, const float* scale,
+                                void* dweight, float* sums) {
+  LinearParams p = {};
+  p.p = x;
+  p.p_bytes = x_bytes;
+  p.q = dz;
+  p.q_bytes = dz_bytes;
+  p.m = out;
+  p.n = dim;
+  p.k = (int32_t)rows;
+  p.scale = scale;
+  p.out = dweight;
+  p.sums = sums;
+  return p;
+}
 
 std::string number(int64_t v) { return std::to_string(v); }
 
@@ -207,26 +271,28 @@ struct Layouter {
 };
 
 int64_t forward_sums(int64_t m, int64_t n, int64_t k, bool gated) {
-  return m <= kFewRows ? 0 : sums_bytes(plan_of(m, n, k, gated ? After::kGated : After::kForward), m, gated ? 2 * n : n);
+  return m <= kFewRows ? 0 : sums_bytes(plan_of({m, n, k, gated ? After::kGated : After::kForward}), m, gated ? 2 * n : n);
 }
-int64_t plain_sums(int64_t m, int64_t n, int64_t k) { return sums_bytes(plan_of(m, n, k, After::kPlain), m, n); }
 
 // ---- linear ---------------------------------------------------------------------------------------------------------
 
 struct LinearWork {
-  int64_t dz, products, rows, parts, scale, bytes;
+  TwoPlans plans;  // dx, dweight
+  int64_t dz, forward, dx, dweight, rows, parts, scale, bytes;
 };
 LinearWork work_of(const nd_linear* a, bool backward) {
   LinearWork w = {};
   Layouter l;
   if (!backward) {
-    w.products = l.take(forward_sums(a->rows, a->out_dim, a->dim, false));
+    w.forward = l.take(forward_sums(a->rows, a->out_dim, a->dim, false));
   } else {
-    const bool active = a->activation != ND_NO_ACTIVATION;
+    const bool active = a->activation != ND_NO_ACTIVATION, scaled = active && a->dtype == ND_F16;
+    const Task dx = {a->rows, a->dim, a->out_dim, After::kPlain}, dweight = {a->out_dim, a->dim, a->rows, After::kPlain};
+    w.plans = plan_two(a->dx ? &dx : nullptr, a->dweight ? &dweight : nullptr);
     w.dz = l.take(active ? a->rows * a->out_dim * 2 : 0);
-    w.products = l.take(std::max(a->dx ? plain_sums(a->rows, a->dim, a->out_dim) : 0, a->dweight ? plain_sums(a->out_dim, a->dim, a->rows) : 0));
+    w.dx = l.take(a->dx ? sums_bytes(w.plans.first, dx.m, dx.n) : 0);
+    w.dweight = l.take(a->dweight ? sums_bytes(w.plans.second, dweight.m, dweight.n) : 0);
     w.rows = l.take(a->dbias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
-    const bool scaled = active && a->dtype == ND_F16;
     w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
     w.scale = l.take(scaled ? 8 : 0);
   }
@@ -252,7 +318,6 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
   if (w.bytes > 0 && (a->workspace_bytes < w.bytes || !a->workspace || ((uintptr_t)a->workspace & 15)))
     return fail("linear: the workspace has " + number(a->workspace ? a->workspace_bytes : 0) + " bytes, " + number(w.bytes) + " needed, aligned to 16");
   char* work = (char*)a->workspace;
-  float* sums = (float*)(work + w.products);
   Call call("linear", a->dtype, stream);
   if (!backward) {
     LinearParams p = {};
@@ -269,7 +334,7 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
     p.residual_bytes = a->residual_row * 2;
     p.out = a->out;
     p.z = a->z;
-    call.forward(p, After::kForward, sums);
+    call.forward(p, After::kForward, (float*)(work + w.forward));
     return call.done();
   }
   const void* dz = a->dout;
@@ -289,42 +354,47 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
     p.scale = scale;
     p.out = work + w.dz;
     call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr, nullptr);
-    if (a->dbias) call.column_join(rows, row_shares(a->rows, a->out_dim), a->out_dim, nullptr, a->dbias);
+    if (a->dbias) call.join(rows, row_shares(a->rows, a->out_dim), a->out_dim, nullptr, a->dbias);
     dz = work + w.dz;
     dz_bytes = (int64_t)a->out_dim * 2;
   } else if (a->dbias) {
     call.survey(a->dout, dz_bytes, a->rows, a->out_dim, rows, a->dbias, nullptr, nullptr);
   }
-  if (a->dx) call.gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, scale, a->dx, sums);
-  if (a->dweight) call.gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, scale, a->dweight, sums);
+  const LinearParams dx = gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, scale, a->dx, (float*)(work + w.dx));
+  const LinearParams dweight =
+      gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, scale, a->dweight, (float*)(work + w.dweight));
+  call.backward(a->dx ? &dx : nullptr, After::kPlain, a->dweight ? &dweight : nullptr, w.plans);
+  call.add_up();
   return call.done();
 }
 
 // ---- mlp --------------------------------------------------------------------------------------------------------------
 
-// The product that makes dz, and the shares of the rows whose sums it leaves.
-LinearPlan slope_plan(const nd_mlp* a) { return plan_of(a->rows, a->inner, a->out_dim, After::kSlope); }
-int64_t slope_shares(const nd_mlp* a) {
-  const int shape = slope_plan(a).shape, rows = kShapes[shape].m, waves = shape == 0 ? Large::kWavesN : shape == 1 ? Medium::kWavesN : Small::kWavesN;
-  return (a->rows + rows - 1) / rows * waves;
-}
-
 struct MlpWork {
-  int64_t dz, products, rows, columns, parts, scale, bytes;
+  TwoPlans first, second;  // dz and ddown; dx and dup
+  int64_t shares;          // of the rows, whose sums the product that makes dz leaves
+  int64_t dz, forward, dx, dup, ddown, rows, columns, parts, scale, bytes;
 };
 MlpWork work_of(const nd_mlp* a, bool backward) {
   MlpWork w = {};
   Layouter l;
   const int64_t wide = (int64_t)a->inner * (a->gated ? 2 : 1);
   if (!backward) {
-    w.products = l.take(std::max(forward_sums(a->rows, a->inner, a->dim, a->gated), forward_sums(a->rows, a->out_dim, a->inner, false)));
+    w.forward = l.take(std::max(forward_sums(a->rows, a->inner, a->dim, a->gated), forward_sums(a->rows, a->out_dim, a->inner, false)));
   } else {
-    const bool first = a->dx || a->dup || a->dup_bias, scaled = first && a->dtype == ND_F16;
-    w.dz = l.take(first ? a->rows * wide * 2 : 0);
-    w.products = l.take(std::max({a->dx ? plain_sums(a->rows, a->dim, wide) : 0, a->dup ? plain_sums(wide, a->dim, a->rows) : 0,
-                                  a->ddown ? plain_sums(a->out_dim, a->inner, a->rows) : 0}));
+    const bool some = a->dx || a->dup || a->dup_bias, scaled = some && a->dtype == ND_F16;
+    const Task dz = {a->rows, a->inner, a->out_dim, After::kSlope}, ddown = {a->out_dim, a->inner, a->rows, After::kPlain};
+    const Task dx = {a->rows, a->dim, wide, After::kPlain}, dup = {wide, a->dim, a->rows, After::kPlain};
+    w.first = plan_two(some ? &dz : nullptr, a->ddown ? &ddown : nullptr);
+    w.second = plan_two(a->dx ? &dx : nullptr, a->dup ? &dup : nullptr);
+    const int rows = kShapes[w.first.first.shape].m, waves[] = {Large::kWavesN, Medium::kWavesN, Small::kWavesN};
+    w.shares = (a->rows + rows - 1) / rows * waves[std::min(w.first.first.shape, 2)];
+    w.dz = l.take(some ? a->rows * wide * 2 : 0);
+    w.dx = l.take(a->dx ? sums_bytes(w.second.first, dx.m, dx.n) : 0);
+    w.dup = l.take(a->dup ? sums_bytes(w.second.second, dup.m, dup.n) : 0);
+    w.ddown = l.take(a->ddown ? sums_bytes(w.first.second, ddown.m, ddown.n) : 0);
     w.rows = l.take(a->ddown_bias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
-    w.columns = l.take(a->dup_bias ? std::max<int64_t>(1, slope_shares(a)) * wide * 4 : 0);
+    w.columns = l.take(a->dup_bias ? w.shares * wide * 4 : 0);
     w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
     w.scale = l.take(scaled ? 8 : 0);
   }
@@ -353,7 +423,6 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   if (w.bytes > 0 && (a->workspace_bytes < w.bytes || !a->workspace || ((uintptr_t)a->workspace & 15)))
     return fail("mlp: the workspace has " + number(a->workspace ? a->workspace_bytes : 0) + " bytes, " + number(w.bytes) + " needed, aligned to 16");
   char* work = (char*)a->workspace;
-  float* sums = (float*)(work + w.products);
   Call call("mlp", a->dtype, stream);
   const int32_t wide = a->inner * (a->gated ? 2 : 1);
   const int64_t inner_bytes = (int64_t)a->inner * 2, wide_bytes = (int64_t)wide * 2;
@@ -370,7 +439,7 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     p.bias = a->up_bias;
     p.out = a->h;
     p.z = a->z;
-    call.forward(p, a->gated ? After::kGated : After::kForward, sums);
+    call.forward(p, a->gated ? After::kGated : After::kForward, (float*)(work + w.forward));
     LinearParams r = {};
     r.p = a->down;
     r.p_bytes = inner_bytes;
@@ -383,15 +452,13 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     r.residual = a->residual;
     r.residual_bytes = a->residual_row * 2;
     r.out = a->out;
-    call.forward(r, After::kForward, sums);
+    call.forward(r, After::kForward, (float*)(work + w.forward));
     return call.done();
   }
   const int64_t dout_bytes = a->dout_row * 2;
   float* scale = first && !call.bf16 ? (float*)(work + w.scale) : nullptr;
   if (a->ddown_bias || scale)
     call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, (float*)(work + w.parts), scale);
-  if (a->ddown) call.gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, sums);
-  if (!first) return call.done();
   float* columns = a->dup_bias ? (float*)(work + w.columns) : nullptr;
   LinearParams p = {};
   p.p = a->down;
@@ -407,11 +474,15 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   p.out = work + w.dz;
   p.scale = scale;
   p.column_sums = columns;
-  call.product(p, Layout::kWeightColumns, After::kSlope, slope_plan(a));
+  const LinearParams ddown =
+      gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, (float*)(work + w.ddown));
+  call.backward(first ? &p : nullptr, After::kSlope, a->ddown ? &ddown : nullptr, w.first);
+  if (columns) call.join(columns, w.shares, wide, scale ? scale + 1 : nullptr, a->dup_bias);
   const char* dz = work + w.dz;
-  if (columns) call.column_join(columns, slope_shares(a), wide, scale, a->dup_bias);
-  if (a->dx) call.gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, scale, a->dx, sums);
-  if (a->dup) call.gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, scale, a->dup, sums);
+  const LinearParams dx = gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, scale, a->dx, (float*)(work + w.dx));
+  const LinearParams dup = gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, scale, a->dup, (float*)(work + w.dup));
+  call.backward(a->dx ? &dx : nullptr, After::kPlain, a->dup ? &dup : nullptr, w.second);
+  call.add_up();
   return call.done();
 }
 

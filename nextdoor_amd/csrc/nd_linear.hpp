@@ -12,12 +12,14 @@
 // gradients of a mean over many rows are not lost below 2^-14; what is made of it is divided by that in 32 bits.
 #pragma once
 
+#include <algorithm>
+
 #include "nd_activation.hpp"
 #include "nd_product.hpp"
 
 namespace nd {
 
-enum class After { kSums, kForward, kGated, kPlain, kSlope };
+enum class After { kSums, kForward, kGated, kPlain, kSlope };  // (kPlain: sums too, where there are shares)
 
 struct LinearParams {
   // C [m][n], sums over k; gated: n counts pairs, and P has 2 n rows
@@ -30,9 +32,9 @@ struct LinearParams {
   void* out;
   void* z;  // forward: written unless null; backward: read.  [m][n]; gated: rows of 6 n bytes, see Upper24
   const float* scale;  // null: 1; kSlope: the sums are multiplied with scale[0]; kPlain: with scale[1], one over it
-  // shares of the sum: share s has places s * share .. and leaves [m][width] values in 32 bits
+  // shares of the sum: share s has places s * share .. and leaves [m][n] values (gated: [m][2 n]) in 32 bits
   float* sums;
-  int32_t shares, share, width;
+  int32_t shares, share;
   float* column_sums;  // kSlope, unless null: sums of 32 kN rows of dz, [share of the rows][columns of dz]
 };
 
@@ -73,7 +75,7 @@ __device__ __forceinline__ float sums_of_rows(const float (&v)[16], int lane) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// What follows the sums v (gated: and u) of columns c .. c + 7 of a row.
+// What follows the sums v (gated: and u) of columns c .. c + 7 of a row of a forward pass.
 template <class T, After AFTER>
 __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, float (&v)[8], float (&u)[8]) {
   auto unpack = [](const u32x4& w, float(&x)[8]) {
@@ -90,14 +92,10 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
     return w;
   };
   auto at = [&](const void* matrix, int64_t row_bytes, int column) { return (u32x4*)((char*)matrix + row * row_bytes + (int64_t)column * 2); };
-  constexpr bool kForward = AFTER == After::kForward || AFTER == After::kGated;
+  static_assert(AFTER == After::kForward || AFTER == After::kGated, "");
   const int64_t n_bytes = (int64_t)a.n * 2;
   float x[8];
-  if (!kForward && a.scale) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= a.scale[1];
-  }
-  if (kForward && a.bias) {
+  if (a.bias) {
     unpack(*at(a.bias, 0, c), x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += x[i];
@@ -115,7 +113,7 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += x[i];
     }
-  } else if (AFTER == After::kGated) {
+  } else {
     if (a.z) {
       const u32x2 g0 = Upper24::upper(v), g1 = Upper24::upper(v + 4), u0 = Upper24::upper(u), u1 = Upper24::upper(u + 4);
       *at(a.z, 3 * n_bytes, c) = u32x4{g0[0], g0[1], g1[0], g1[1]};
@@ -140,23 +138,24 @@ using Small = product::Shape<1, 2, 2, 1, 64, 3, 2, 2, 4, 1>;
 
 enum class Layout { kRows, kWeightColumns, kColumns };  // both operands by rows; P by columns; both by columns
 
+// Chunks of LDS of a wave.  (What follows a product wants room for its results: two regions, and five of 64 columns where a slope
+// is read.)
+template <class S, After AFTER>
+constexpr int kWaveChunks = std::max(S::kTileChunks / (S::kThreads / 64), AFTER == After::kSlope ? 5 * product::Region<8>::kSize : S::kWaveResults);
+
+// Tile `block` of C, of share 0, then of share 1 and so on.  tiles: kWaveChunks for each wave.
 template <class T, class S, Layout LAYOUT, After AFTER>
-__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(LinearParams a, int m_tiles, int n_tiles) {
+__device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block, int m_tiles, int n_tiles, u32x4* tiles) {
   constexpr bool kGated = AFTER == After::kGated;
   constexpr int kColumns = kGated ? S::kTileM / 2 : S::kTileM;  // of C to a tile
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  // (what follows a product wants room for its results: two regions of a wave, and five of 64 columns where a slope is read)
-  constexpr int kWaves = S::kThreads / 64, kRoom = AFTER == After::kSlope ? 5 * product::Region<8>::kSize : S::kWaveResults;
-  constexpr int kWaveChunks = S::kTileChunks / kWaves > kRoom ? S::kTileChunks / kWaves : kRoom;
-  __shared__ u32x4 tiles[kWaveChunks * kWaves];
   // Bands of eight tiles of rows, in a band column after column: the tiles that a die works on at a time (32 or more) share few rows
-  // of both operands.  Shares of a sum one after another.
-  uint32_t block = block_by_die();
+  // of both operands.
   const int per_share = m_tiles * n_tiles, share = uniform(block / per_share);
   block -= share * per_share;
   const int band = uniform(block / (8 * n_tiles)), in_band = block - band * 8 * n_tiles, width = min(8, m_tiles - band * 8);
   const int column0 = uniform(in_band / width) * kColumns, row0 = (band * 8 + uniform(in_band % width)) * S::kTileN;
-  const int place0 = share * a.share, place_end = AFTER == After::kSums && share + 1 < a.shares ? place0 + a.share : a.k;
+  const int place0 = share * a.share, place_end = share + 1 < a.shares ? place0 + a.share : a.k;
   f32x16 acc[S::kM][S::kN];
   if constexpr (LAYOUT == Layout::kRows) {
     using P = product::ByRows<S::kTileM, S::kDepth, S::kThreads, kGated>;
@@ -173,13 +172,14 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   }
   product::meet();
   // ---- the results: wave's rows from wave_row0 on, columns from wave_column0 on
-  u32x4* mine = tiles + wave * kWaveChunks;
+  constexpr int kRoom = kWaveChunks<S, AFTER>;
+  u32x4* mine = tiles + wave * kRoom;
   const int wave_row0 = row0 + wave % S::kWavesN * 32 * S::kN, wave_column0 = column0 + wave / S::kWavesN * (kColumns / S::kWavesM);
   const int h = lane >> 5;
   const int64_t n_bytes = (int64_t)a.n * 2;
-  if constexpr (AFTER == After::kSums) {
+  if (AFTER == After::kSums || (AFTER == After::kPlain && a.shares > 1)) {
     // blocks of 32 columns, 128 bytes of a row
-    float* sums = a.sums + (int64_t)share * a.m * a.width;
+    float* sums = a.sums + (int64_t)share * a.m * a.n;
 #pragma unroll
     for (int j = 0; j < S::kN; ++j)
 #pragma unroll
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
         for (int t = 0; t < 4; ++t) {
           const int r = t * 8 + lane / 8, c = lane % 8, row = wave_row0 + 32 * j + r, column = wave_column0 + 32 * i + 4 * c;
           const f32x4 v = *(const f32x4*)(mine + r * 8 + (c ^ (r & 7)));
-          if (row < a.m && column < a.n) *(f32x4*)(sums + (int64_t)row * a.width + column) = v;
+          if (row < a.m && column < a.n) *(f32x4*)(sums + (int64_t)row * a.n + column) = v;
         }
         asm volatile("" ::: "memory");
       }
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   if constexpr (AFTER == After::kGated) {
     using Out = product::Region<2 * S::kM>;
     const Out gates{mine}, others{mine + Out::kSize}, next{mine + 2 * Out::kSize}, products{mine + 3 * Out::kSize};
-    static_assert(4 * Out::kSize <= kWaveChunks, "");
+    static_assert(4 * Out::kSize <= kRoom, "");
     Bias bias[S::kM];
     if (a.bias) {
 #pragma unroll
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
     // goes out from where z was.
     using Part = product::Region<8>;
     constexpr int kParts = S::kM / 2 * S::kN;
-    static_assert(S::kM % 2 == 0 && 5 * Part::kSize <= kWaveChunks, "");
+    static_assert(S::kM % 2 == 0 && 5 * Part::kSize <= kRoom, "");
     const bool slope = a.z, gated = a.gated;  // (without a z, dz is what the product gives)
     const bool whole = wave_row0 + 32 * S::kN <= a.m && wave_column0 + 32 * S::kM <= a.n;
     const int64_t z_bytes = gated ? 3 * n_bytes : n_bytes, out_bytes = gated ? 2 * n_bytes : n_bytes;
@@ -385,9 +385,9 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
         }
       }
     }
-  } else {
+  } else if constexpr (AFTER != After::kSums) {
     using Out = product::Region<4 * S::kM>;
-    constexpr int kRegions = kWaveChunks / Out::kSize;
+    constexpr int kRegions = kRoom / Out::kSize;
     static_assert(kRegions >= 2 && kRegions >= S::kN, "");
     const bool residual = AFTER == After::kForward && a.residual, keep = AFTER == After::kForward && a.z;
     // Regions of rows j: what is read, and goes out again in the same place; with z one region further.  All rows are asked for
@@ -441,8 +441,28 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   }
 }
 
-// The shares' sums added up, and what follows: eight columns of a row to LANES lanes, which share out the shares where there are
-// few rows and columns.
+struct Tiles {
+  int m, n;  // of one share
+};
+
+template <class T, class S, Layout LAYOUT, After AFTER>
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(LinearParams a, Tiles t) {
+  __shared__ u32x4 tiles[kWaveChunks<S, AFTER> * (S::kThreads / 64)];
+  make_tile<T, S, LAYOUT, AFTER>(a, block_by_die(), t.m, t.n, tiles);
+}
+
+// Two products in one launch, neither of which fills the GPU: dx (or dz) and a gradient of weights.  The first a_blocks workgroups
+// have the first.  1021 rows, 520 -> 1000: 10.6 us for 9.4 + 9.5 one after another.
+template <class T, class S, After FIRST>
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void pair_kernel(LinearParams a, Tiles a_tiles, uint32_t a_blocks, LinearParams b, Tiles b_tiles) {
+  __shared__ u32x4 tiles[std::max(kWaveChunks<S, FIRST>, kWaveChunks<S, After::kPlain>) * (S::kThreads / 64)];
+  const uint32_t block = block_by_die();
+  if (block < a_blocks) make_tile<T, S, Layout::kWeightColumns, FIRST>(a, block, a_tiles.m, a_tiles.n, tiles);
+  else make_tile<T, S, Layout::kColumns, After::kPlain>(b, block - a_blocks, b_tiles.m, b_tiles.n, tiles);
+}
+
+// The shares' sums of a forward pass added up, and what follows: eight columns of a row to LANES lanes, which share out the shares
+// where there are few rows and columns.
 template <class T, After AFTER, int LANES>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams a) {
   constexpr int kGroups = 256 / LANES, kSides = AFTER == After::kGated ? 2 : 1;
@@ -457,9 +477,10 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;
     if (there) {
-      const float* from = a.sums + ((int64_t)lane * a.m + row) * a.width + column;
+      const int64_t width = kSides * (int64_t)a.n;
+      const float* from = a.sums + ((int64_t)lane * a.m + row) * width + column;
 #pragma unroll 4
-      for (int s = lane; s < a.shares; s += LANES, from += (int64_t)LANES * a.m * a.width) {
+      for (int s = lane; s < a.shares; s += LANES, from += LANES * a.m * width) {
         const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -488,14 +509,75 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams a) {
   if (there) finish<T, AFTER>(a, row, c, v, u);
 }
 
+// Sums of shares added up: groups * 8 values in a row, out = (the sum of sums[share][value]) * *factor.  Several such jobs in one launch,
+// `lanes` lanes to eight values.
+struct Join {
+  const float* sums;
+  void* out;
+  const float* factor;  // null: 1
+  int64_t groups;
+  int32_t shares, lanes;
+  uint32_t first_block;
+};
+struct Joins {
+  static constexpr int kMost = 5;
+  Join job[kMost];
+  int n;
+};
+template <class T>
+__global__ __launch_bounds__(256) void joins_kernel(Joins joins) {
+  __shared__ float part[256][9];
+  int which = 0;
+  while (which + 1 < joins.n && blockIdx.x >= joins.job[which + 1].first_block) ++which;
+  const Join& a = joins.job[which];
+  const int here = 256 / a.lanes, own = threadIdx.x % here, lane = threadIdx.x / here;
+  const int64_t at = (int64_t)(blockIdx.x - a.first_block) * here + own;
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+  if (at < a.groups) {
+#pragma unroll 4
+    for (int s = lane; s < a.shares; s += a.lanes) {
+      const float* from = a.sums + (s * a.groups + at) * 8;
+      const f32x4 lo = *(const f32x4*)from, hi = *(const f32x4*)(from + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] += lo[i];
+        x[4 + i] += hi[i];
+      }
+    }
+  }
+  if (a.lanes > 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[threadIdx.x][i] = x[i];
+    __syncthreads();
+    if (lane > 0) return;
+    for (int l = 1; l < a.lanes; ++l)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += part[l * here + own][i];
+  }
+  if (at >= a.groups) return;
+  const float factor = a.factor ? *a.factor : 1.f;
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack_pair<T>(x[2 * i] * factor, x[2 * i + 1] * factor);
+  ((u32x4*)a.out)[at] = w;
+}
+
 // ---- launches (nd_linear_types.hpp, compiled for each type by itself) -----------------------------------------
 
 struct LinearPlan {
   int shape;  // 0 large, 1 medium, 2 small, 3 narrow
   int shares, share;
 };
+// kPlain with shares: leaves sums.
 template <class T>
 hipError_t launch_linear(const LinearParams& a, Layout layout, After after, const LinearPlan& plan, hipStream_t stream);
+// The first by columns of the weights, kPlain or kSlope, the second by columns, kPlain; of one shape, medium or small.
+template <class T>
+hipError_t launch_pair(const LinearParams& a, After after, const LinearPlan& a_plan, const LinearParams& b, const LinearPlan& b_plan, hipStream_t stream);
+template <class T>
+hipError_t launch_joins(const Joins& joins, uint32_t blocks, hipStream_t stream);
 template <class T>
 hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
 // dz = dout a'(z) times scale[0], if there is a z, and unless they are null sums of its rows (times 1), and the largest finite
@@ -503,9 +585,6 @@ hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t strea
 template <class T>
 hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts, hipStream_t stream);
 constexpr int kSlopeColumns = 64;  // of a workgroup there
-// scale: null, or as above: the sums are multiplied with scale[1].
-template <class T>
-hipError_t launch_column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out, hipStream_t stream);
 
 constexpr int kFewRows = 64;  // at most: a kernel of its own, which reads the weights once and keeps a sum in many waves
 

@@ -1,9 +1,6 @@
 // The kernels of nd_linear.hpp and the two that go with them, for one type of values.
 #pragma once
 
-#include <algorithm>
-
-#include "nd_column_sums.hpp"
 #include "nd_linear.hpp"
 
 namespace nd {
@@ -177,34 +174,38 @@ hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_by
   slope_kernel<T><<<dim3((a.n + kSlopeColumns - 1) / kSlopeColumns, (uint32_t)shares), 256, 0, stream>>>(a, dout, dout_bytes, sums, rows_per_share, parts);
   return hipGetLastError();
 }
-template <class T>
-hipError_t launch_column_join(const float* sums, int64_t shares, int64_t columns, const float* scale, void* out, hipStream_t stream) {
-  return column_join<T>(sums, shares, columns, scale ? scale + 1 : nullptr, out, columns, nullptr, stream);
-}
-
 // ---- tiles ----------------------------------------------------------------------------------------------------
 
+template <class S>
+Tiles tiles_of(const LinearParams& a, int columns = S::kTileM) {
+  return {(a.m + S::kTileN - 1) / S::kTileN, (a.n + columns - 1) / columns};
+}
+template <class S>
+bool too_many(int64_t blocks) {  // for one launch
+  return blocks * S::kThreads >> 32;
+}
+
 template <class T, class S, Layout LAYOUT, After AFTER>
-hipError_t launch_tiles(const LinearParams& a, int shares, hipStream_t stream) {
-  const int columns = AFTER == After::kGated ? S::kTileM / 2 : S::kTileM;
-  const int m_tiles = (a.m + S::kTileN - 1) / S::kTileN, n_tiles = (a.n + columns - 1) / columns;
-  if ((int64_t)m_tiles * n_tiles * shares * S::kThreads >> 32) return hipErrorInvalidConfiguration;  // (more than one launch holds)
-  linear_kernel<T, S, LAYOUT, AFTER><<<dim3((uint32_t)m_tiles * n_tiles * shares), S::kThreads, 0, stream>>>(a, m_tiles, n_tiles);
+hipError_t launch_tiles(const LinearParams& a, hipStream_t stream) {
+  const Tiles t = tiles_of<S>(a, AFTER == After::kGated ? S::kTileM / 2 : S::kTileM);
+  const int64_t blocks = (int64_t)t.m * t.n * a.shares;
+  if (too_many<S>(blocks)) return hipErrorInvalidConfiguration;
+  linear_kernel<T, S, LAYOUT, AFTER><<<(uint32_t)blocks, S::kThreads, 0, stream>>>(a, t);
   return hipGetLastError();
 }
 template <class T, Layout LAYOUT, After AFTER>
-hipError_t launch_shape(const LinearParams& a, int shape, int shares, hipStream_t stream) {
-  if (shape == 0) return launch_tiles<T, Large, LAYOUT, AFTER>(a, shares, stream);
-  if (shape == 1) return launch_tiles<T, Medium, LAYOUT, AFTER>(a, shares, stream);
+hipError_t launch_shape(const LinearParams& a, int shape, hipStream_t stream) {
+  if (shape == 0) return launch_tiles<T, Large, LAYOUT, AFTER>(a, stream);
+  if (shape == 1) return launch_tiles<T, Medium, LAYOUT, AFTER>(a, stream);
   if constexpr (AFTER != After::kGated && AFTER != After::kSlope) {  // (those have columns in pairs of 32)
-    if (shape == 3) return launch_tiles<T, Narrow, LAYOUT, AFTER>(a, shares, stream);
+    if (shape == 3) return launch_tiles<T, Narrow, LAYOUT, AFTER>(a, stream);
   }
-  return launch_tiles<T, Small, LAYOUT, AFTER>(a, shares, stream);
+  return launch_tiles<T, Small, LAYOUT, AFTER>(a, stream);
 }
 template <class T, After AFTER>
 hipError_t launch_join(const LinearParams& a, hipStream_t stream) {
   const int64_t groups = (int64_t)a.m * (a.n / 8);
-  // (64 x 256 values of 16 shares: 7.5 us with a lane to eight values, for the reads of one lane follow each other; 3.3 with eight)
+  // (64 x 256 values of 16 shares: 7.5 us with a lane to eight values, for the reads of one lane follow each other; 3.9 with eight)
   if (groups <= 1 << 14 && a.shares >= 4) linear_join_kernel<T, AFTER, 8><<<(uint32_t)((groups + 31) / 32), 256, 0, stream>>>(a);
   else linear_join_kernel<T, AFTER, 1><<<(uint32_t)((groups + 255) / 256), 256, 0, stream>>>(a);
   return hipGetLastError();
@@ -215,27 +216,44 @@ hipError_t launch_linear(const LinearParams& a, Layout layout, After after, cons
   LinearParams p = a;
   p.shares = plan.shares;
   p.share = plan.share;
-  if (plan.shares > 1) {  // (not kSlope)
-    p.n = p.width = after == After::kGated ? 2 * a.n : a.n;
-    hipError_t e = layout == Layout::kRows            ? launch_shape<T, Layout::kRows, After::kSums>(p, plan.shape, plan.shares, stream)
-                   : layout == Layout::kWeightColumns ? launch_shape<T, Layout::kWeightColumns, After::kSums>(p, plan.shape, plan.shares, stream)
-                                                      : launch_shape<T, Layout::kColumns, After::kSums>(p, plan.shape, plan.shares, stream);
-    if (e != hipSuccess) return e;
-    p.n = a.n;
-    switch (after) {
-      case After::kForward: return launch_join<T, After::kForward>(p, stream);
-      case After::kGated: return launch_join<T, After::kGated>(p, stream);
-      default: return launch_join<T, After::kPlain>(p, stream);
-    }
-  }
-  switch (after) {
-    case After::kForward: return launch_shape<T, Layout::kRows, After::kForward>(p, plan.shape, 1, stream);
-    case After::kGated: return launch_shape<T, Layout::kRows, After::kGated>(p, plan.shape, 1, stream);
-    case After::kSlope: return launch_shape<T, Layout::kWeightColumns, After::kSlope>(p, plan.shape, 1, stream);
-    default:
-      return layout == Layout::kWeightColumns ? launch_shape<T, Layout::kWeightColumns, After::kPlain>(p, plan.shape, 1, stream)
-                                              : launch_shape<T, Layout::kColumns, After::kPlain>(p, plan.shape, 1, stream);
-  }
+  if (after == After::kPlain)
+    return layout == Layout::kWeightColumns ? launch_shape<T, Layout::kWeightColumns, After::kPlain>(p, plan.shape, stream)
+                                            : launch_shape<T, Layout::kColumns, After::kPlain>(p, plan.shape, stream);
+  if (after == After::kSlope) return launch_shape<T, Layout::kWeightColumns, After::kSlope>(p, plan.shape, stream);
+  if (plan.shares == 1)
+    return after == After::kForward ? launch_shape<T, Layout::kRows, After::kForward>(p, plan.shape, stream)
+                                    : launch_shape<T, Layout::kRows, After::kGated>(p, plan.shape, stream);
+  p.n = after == After::kGated ? 2 * a.n : a.n;
+  const hipError_t e = launch_shape<T, Layout::kRows, After::kSums>(p, plan.shape, stream);
+  if (e != hipSuccess) return e;
+  p.n = a.n;
+  return after == After::kForward ? launch_join<T, After::kForward>(p, stream) : launch_join<T, After::kGated>(p, stream);
+}
+
+template <class T, class S, After FIRST>
+hipError_t launch_pair_of(const LinearParams& a, const LinearParams& b, hipStream_t stream) {
+  const Tiles at = tiles_of<S>(a), bt = tiles_of<S>(b);
+  const int64_t a_blocks = (int64_t)at.m * at.n * a.shares, blocks = a_blocks + (int64_t)bt.m * bt.n * b.shares;
+  if (too_many<S>(blocks)) return hipErrorInvalidConfiguration;
+  pair_kernel<T, S, FIRST><<<(uint32_t)blocks, S::kThreads, 0, stream>>>(a, at, (uint32_t)a_blocks, b, bt);
+  return hipGetLastError();
+}
+template <class T>
+hipError_t launch_pair(const LinearParams& a, After after, const LinearPlan& a_plan, const LinearParams& b, const LinearPlan& b_plan, hipStream_t stream) {
+  LinearParams p = a, q = b;
+  p.shares = a_plan.shares;
+  p.share = a_plan.share;
+  q.shares = b_plan.shares;
+  q.share = b_plan.share;
+  if (after == After::kSlope)
+    return a_plan.shape == 1 ? launch_pair_of<T, Medium, After::kSlope>(p, q, stream) : launch_pair_of<T, Small, After::kSlope>(p, q, stream);
+  return a_plan.shape == 1 ? launch_pair_of<T, Medium, After::kPlain>(p, q, stream) : launch_pair_of<T, Small, After::kPlain>(p, q, stream);
+}
+
+template <class T>
+hipError_t launch_joins(const Joins& joins, uint32_t blocks, hipStream_t stream) {
+  joins_kernel<T><<<blocks, 256, 0, stream>>>(joins);
+  return hipGetLastError();
 }
 
 }  // namespace nd
