@@ -60,34 +60,42 @@ struct Task {
   int64_t m, n, k;
   After after;
 };
-struct Estimate {
-  LinearPlan plan;
-  int64_t groups, rounds;    // workgroups; rounds of each
-  double time, joined;       // us in all, and how much of it is what adds the shares
+// Into how many shares its sums may be cut with tiles of one shape.
+struct Shares {
+  static constexpr int kMost = 12;
+  int n = 0;
+  int shares[kMost];
+  int64_t groups[kMost], rounds[kMost];  // workgroups; rounds of each
+  double joined[kMost];                  // us of adding the shares
 };
-// The best number of shares with tiles of one shape.
-Estimate estimate(const Task& t, int shape) {
-  const ShapeCost& c = kShapes[shape];
+void shares_of(const Task& t, const ShapeCost& c, Shares& s) {
   const int64_t rounds = std::max<int64_t>(1, (t.k + 63) / 64), columns = t.after == After::kGated ? 2 * t.n : t.n;
   const int64_t tiles = ((t.m + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n);
-  Estimate best = {};
-  best.time = INFINITY;
-  for (int64_t want = 1; want <= (t.after == After::kSlope ? 1 : kMostShares); want = want < 4 ? want + 1 : want * 3 / 2) {
-    if (shape == 3 && want == 1 && (t.after == After::kGated || t.after == After::kSlope)) continue;  // (columns in pairs of 32)
-    const int64_t each = (rounds + want - 1) / want, shares = (rounds + each - 1) / each;
-    if (shares != want && want > 1) continue;
+  const int most = t.after == After::kSlope ? 1 : kMostShares;
+  for (int want = 1; want <= most && s.n < Shares::kMost; want = want < 4 ? want + 1 : want * 3 / 2) {
     if (want > 1 && tiles * want > 4 * c.at_once) break;
-    const double joined = shares > 1 ? kJoin + (double)shares * t.m * columns * 8 / kJoinRate : 0;
-    const double time = time_of(c, tiles * shares, each) + joined;
-    if (time < best.time) best = {{shape, (int)shares, (int)(each * 64)}, tiles * shares, each, time, joined};
+    const int64_t each = (rounds + want - 1) / want;
+    if ((rounds + each - 1) / each != want) continue;
+    s.shares[s.n] = want;
+    s.groups[s.n] = tiles * want;
+    s.rounds[s.n] = each;
+    s.joined[s.n++] = want > 1 ? kJoin + (double)want * t.m * columns * 8 / kJoinRate : 0;
   }
-  return best;
 }
+struct Estimate {
+  LinearPlan plan;
+  double time;
+};
 Estimate estimate(const Task& t) {
-  Estimate best = estimate(t, 0);
-  for (int shape = 1; shape < 4; ++shape) {
-    const Estimate e = estimate(t, shape);
-    if (e.time < best.time) best = e;
+  Estimate best = {{}, INFINITY};
+  for (int shape = 0; shape < 4; ++shape) {
+    Shares s;
+    shares_of(t, kShapes[shape], s);
+    for (int i = 0; i < s.n; ++i) {
+      if (shape == 3 && s.shares[i] == 1 && (t.after == After::kGated || t.after == After::kSlope)) continue;  // (columns in pairs of 32)
+      const double time = time_of(kShapes[shape], s.groups[i], s.rounds[i]) + s.joined[i];
+      if (time < best.time) best = {{shape, s.shares[i], (int)s.rounds[i] * 64}, time};
+    }
   }
   return best;
 }
@@ -106,13 +114,22 @@ TwoPlans plan_two(const Task* a, const Task* b) {  // null: not wanted
   if (!a || !b) return best;
   double least = x.time + y.time + kLaunch;
   for (int shape = 1; shape < 3; ++shape) {
-    const Estimate p = estimate(*a, shape), q = estimate(*b, shape);
-    if (p.groups + q.groups > 2 * kShapes[shape].at_once) continue;
-    const double time = time_of(kShapes[shape], p.groups + q.groups, std::max(p.rounds, q.rounds)) + p.joined + q.joined;
-    if (time < least) {
-      least = time;
-      best = {p.plan, q.plan, true};
-    }
+    const ShapeCost& c = kShapes[shape];
+    Shares p, q;
+    shares_of(*a, c, p);
+    shares_of(*b, c, q);
+    for (int i = 0; i < p.n; ++i)
+      for (int j = 0; j < q.n; ++j) {
+        const int64_t groups = p.groups[i] + q.groups[j];
+        const int64_t most = std::max(p.rounds[i], q.rounds[j]);
+        // beyond one turn the compute units take one workgroup after another, the longer ones first
+        const double in_turns = (double)(p.groups[i] * p.rounds[i] + q.groups[j] * q.rounds[j]) / c.at_once * c.full + ceil((double)groups / c.at_once) * c.once;
+        const double time = p.joined[i] + q.joined[j] + (groups <= c.at_once ? time_of(c, groups, most) : std::max(most * c.full + c.once, 1.1 * in_turns));
+        if (time < least) {
+          least = time;
+          best = {{shape, p.shares[i], (int)p.rounds[i] * 64}, {shape, q.shares[j], (int)q.rounds[j] * 64}, true};
+        }
+      }
   }
   return best;
 }

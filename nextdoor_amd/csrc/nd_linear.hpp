@@ -451,14 +451,24 @@ __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(L
   make_tile<T, S, LAYOUT, AFTER>(a, block_by_die(), t.m, t.n, tiles);
 }
 
-// Two products in one launch, neither of which fills the GPU: dx (or dz) and a gradient of weights.  The first a_blocks workgroups
-// have the first.  1021 rows, 520 -> 1000: 10.6 us for 9.4 + 9.5 one after another.
+// Two products in one launch, neither of which fills the GPU: dx (or dz) and a gradient of weights; first the one whose workgroups take
+// longer.  Each die (consecutive workgroups go to the eight in turn) has an eighth of either.  1021 rows, 520 -> 1000: 13 us for 9.4
+// and 9.5 one after another, and a launch less.
+struct Pair {
+  Tiles a_tiles, b_tiles;
+  uint32_t a_blocks, b_blocks, a_turns, b_turns;  // turns: blocks of one die
+  bool b_first;
+};
 template <class T, class S, After FIRST>
-__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void pair_kernel(LinearParams a, Tiles a_tiles, uint32_t a_blocks, LinearParams b, Tiles b_tiles) {
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void pair_kernel(LinearParams a, LinearParams b, Pair p) {
   __shared__ u32x4 tiles[std::max(kWaveChunks<S, FIRST>, kWaveChunks<S, After::kPlain>) * (S::kThreads / 64)];
-  const uint32_t block = block_by_die();
-  if (block < a_blocks) make_tile<T, S, Layout::kWeightColumns, FIRST>(a, block, a_tiles.m, a_tiles.n, tiles);
-  else make_tile<T, S, Layout::kColumns, After::kPlain>(b, block - a_blocks, b_tiles.m, b_tiles.n, tiles);
+  const uint32_t die = blockIdx.x % 8, turn = blockIdx.x / 8;
+  const bool is_b = p.b_first ? turn < p.b_turns : turn >= p.a_turns;
+  const uint32_t before = is_b == p.b_first ? 0 : is_b ? p.a_turns : p.b_turns;
+  const uint32_t block = die * (is_b ? p.b_turns : p.a_turns) + turn - before;
+  if (block >= (is_b ? p.b_blocks : p.a_blocks)) return;
+  if (is_b) make_tile<T, S, Layout::kColumns, After::kPlain>(b, block, p.b_tiles.m, p.b_tiles.n, tiles);
+  else make_tile<T, S, Layout::kWeightColumns, FIRST>(a, block, p.a_tiles.m, p.a_tiles.n, tiles);
 }
 
 // The shares' sums of a forward pass added up, and what follows: eight columns of a row to LANES lanes, which share out the shares

@@ -19,7 +19,7 @@ __device__ __forceinline__ f32x4 product_16x16x32(u32x4 a, u32x4 b, f32x4 c, _Fl
 // whole lines of 128 bytes.  x is the same for all workgroups and comes from the caches.
 template <class T, int ROW_BLOCKS, After AFTER, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinearParams a) {
-  constexpr int kSides = AFTER == After::kGated ? 2 : 1, kAhead = 4;
+  constexpr int kSides = AFTER == After::kGated ? 2 : 1, kAhead = ROW_BLOCKS == 1 && kSides == 1 ? 8 : 4;  // slices asked for at once
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), column0 = blockIdx.x * 16;
   __shared__ float part[WAVES][kSides * ROW_BLOCKS][16][17];
   f32x4 sum[kSides][ROW_BLOCKS];
@@ -65,18 +65,22 @@ __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinearParams a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) part[wave][s * ROW_BLOCKS + b][lane & 15][4 * (lane >> 4) + e] = sum[s][b][e];
   __syncthreads();
+  // the waves' sums, one value to a lane; then eight columns of a row
+  for (int t = threadIdx.x; t < 256 * kSides * ROW_BLOCKS; t += 64 * WAVES) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v += part[w][t >> 8][(t >> 4) & 15][t & 15];
+    part[0][t >> 8][(t >> 4) & 15][t & 15] = v;  // (read by this lane only)
+  }
+  __syncthreads();
   for (int t = threadIdx.x; t < 32 * ROW_BLOCKS; t += 64 * WAVES) {
     const int r = t >> 1, c = (t & 1) * 8;
     if (r >= a.m || column0 + c >= a.n) continue;
     float v[8], u[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] = 0.f;
-      for (int w = 0; w < WAVES; ++w) v[e] += part[w][r >> 4][r & 15][c + e];
-      if (kSides == 2) {
-        u[e] = 0.f;
-        for (int w = 0; w < WAVES; ++w) u[e] += part[w][ROW_BLOCKS * (kSides - 1) + (r >> 4)][r & 15][c + e];
-      }
+      v[e] = part[0][r >> 4][r & 15][c + e];
+      if (kSides == 2) u[e] = part[0][ROW_BLOCKS * (kSides - 1) + (r >> 4)][r & 15][c + e];
     }
     finish<T, AFTER>(a, r, column0 + c, v, u);
   }
@@ -232,10 +236,15 @@ hipError_t launch_linear(const LinearParams& a, Layout layout, After after, cons
 
 template <class T, class S, After FIRST>
 hipError_t launch_pair_of(const LinearParams& a, const LinearParams& b, hipStream_t stream) {
-  const Tiles at = tiles_of<S>(a), bt = tiles_of<S>(b);
-  const int64_t a_blocks = (int64_t)at.m * at.n * a.shares, blocks = a_blocks + (int64_t)bt.m * bt.n * b.shares;
-  if (too_many<S>(blocks)) return hipErrorInvalidConfiguration;
-  pair_kernel<T, S, FIRST><<<(uint32_t)blocks, S::kThreads, 0, stream>>>(a, at, (uint32_t)a_blocks, b, bt);
+  Pair p = {tiles_of<S>(a), tiles_of<S>(b)};
+  const int64_t a_blocks = (int64_t)p.a_tiles.m * p.a_tiles.n * a.shares, b_blocks = (int64_t)p.b_tiles.m * p.b_tiles.n * b.shares;
+  if (too_many<S>(a_blocks + b_blocks + 16)) return hipErrorInvalidConfiguration;
+  p.a_blocks = (uint32_t)a_blocks;
+  p.b_blocks = (uint32_t)b_blocks;
+  p.a_turns = (p.a_blocks + 7) / 8;
+  p.b_turns = (p.b_blocks + 7) / 8;
+  p.b_first = (b.shares > 1 ? b.share : b.k) > (a.shares > 1 ? a.share : a.k);
+  pair_kernel<T, S, FIRST><<<8 * (p.a_turns + p.b_turns), S::kThreads, 0, stream>>>(a, b, p);
   return hipGetLastError();
 }
 template <class T>
