@@ -11,25 +11,6 @@
 
 namespace nd {
 
-// float16: what dz is held times.  scale[0] = the power of two that takes the largest of all parts to between 1/2 and 1 (1, if that is
-// 0), scale[1] = one over it.
-__global__ __launch_bounds__(256) void scale_kernel(const float* parts, int64_t n, float* scale) {
-  __shared__ float wave[4];
-  float most = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 256) most = fmaxf(most, parts[i]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  if ((threadIdx.x & 63) == 0) wave[threadIdx.x >> 6] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    most = fmaxf(fmaxf(wave[0], wave[1]), fmaxf(wave[2], wave[3]));
-    int power = 0;
-    if (most > 0.f) frexpf(most, &power);
-    scale[0] = ldexpf(1.f, -power);
-    scale[1] = ldexpf(1.f, power);
-  }
-}
-
 namespace {
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -142,8 +123,12 @@ int64_t row_shares(int64_t rows, int64_t columns) {
   return std::max<int64_t>(1, std::min<int64_t>({(rows + 63) / 64, std::max<int64_t>(1, 2048 / across), (int64_t)65535}));
 }
 
-// Workgroups of a survey of a matrix.
-int64_t survey_parts(int64_t rows, int64_t columns) { return row_shares(rows, columns) * ((columns + kSlopeColumns - 1) / kSlopeColumns); }
+// Those of a survey of dout, and its workgroups: some hundred, where each is to say what it found.
+int64_t survey_shares(int64_t rows, int64_t columns, bool parts) {
+  const int64_t across = (columns + kSlopeColumns - 1) / kSlopeColumns;
+  return parts ? std::min(row_shares(rows, columns), std::max<int64_t>(1, 512 / across)) : row_shares(rows, columns);
+}
+int64_t survey_parts(int64_t rows, int64_t columns) { return survey_shares(rows, columns, true) * ((columns + kSlopeColumns - 1) / kSlopeColumns); }
 
 // ---- calls --------------------------------------------------------------------------------------------------------
 
@@ -192,34 +177,30 @@ struct Call {
       if (a) one(*a, Layout::kWeightColumns, after, plans.first);
       if (b) one(*b, Layout::kColumns, After::kPlain, plans.second);
     }
-    if (a && plans.first.shares > 1) join(a->sums, plans.first.shares, (int64_t)a->m * a->n, a->scale ? a->scale + 1 : nullptr, a->out);
-    if (b && plans.second.shares > 1) join(b->sums, plans.second.shares, (int64_t)b->m * b->n, b->scale ? b->scale + 1 : nullptr, b->out);
+    if (a && plans.first.shares > 1) join(a->sums, plans.first.shares, (int64_t)a->m * a->n, a->unscale, a->out);
+    if (b && plans.second.shares > 1) join(b->sums, plans.second.shares, (int64_t)b->m * b->n, b->unscale, b->out);
   }
   void one(const LinearParams& a, Layout layout, After after, const LinearPlan& plan) {
     note(bf16 ? launch_linear<__bf16>(a, layout, after, plan, stream) : launch_linear<_Float16>(a, layout, after, plan, stream));
   }
-  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, float* parts) {
-    const int64_t shares = row_shares(a.m, a.n);
+  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts) {
     note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, parts, stream)
               : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, parts, stream));
   }
-  // Of dout [rows][columns]: the sums of its rows, unless out is null, and what dz is held times, unless scale is.
-  void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts, float* scale) {
+  // Of dout [rows][columns]: the sums of its rows, unless out is null, and the largest of its values, unless parts is.
+  void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts) {
     LinearParams p = {};
     p.m = (int32_t)rows;
     p.n = columns;
-    slope(p, dout, row_bytes, out ? sums : nullptr, scale ? parts : nullptr);
-    if (out) join(sums, row_shares(rows, columns), columns, nullptr, out);
-    if (scale) {
-      scale_kernel<<<1, 256, 0, stream>>>(parts, survey_parts(rows, columns), scale);
-      note(hipGetLastError());
-    }
+    const int64_t shares = survey_shares(rows, columns, parts);
+    slope(p, dout, row_bytes, out ? sums : nullptr, shares, parts);
+    if (out) join(sums, shares, columns, nullptr, out);
   }
   int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
 };
 
 // dx [rows][dim] = dz weight;  dweight [out][dim] = dz^T x
-LinearParams gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, const float* scale, void* dx, float* sums) {
+LinearParams gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight, int64_t rows, int32_t out, int32_t dim, float* unscale, void* dx, float* sums) {
   LinearParams p = {};
   p.p = weight;
   p.p_bytes = (int64_t)dim * 2;
@@ -228,12 +209,12 @@ LinearParams gradient_of_x(const void* dz, int64_t dz_bytes, const void* weight,
   p.m = (int32_t)rows;
   p.n = dim;
   p.k = out;
-  p.scale = scale;
+  p.unscale = unscale;
   p.out = dx;
   p.sums = sums;
   return p;
 }
-LinearParams gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, const float* scale,
+LinearParams gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x, int64_t x_bytes, int64_t rows, int32_t out, int32_t dim, float* unscale,
                                 void* dweight, float* sums) {
   LinearParams p = {};
   p.p = x;
@@ -243,7 +224,7 @@ LinearParams gradient_of_weight(const void* dz, int64_t dz_bytes, const void* x,
   p.m = out;
   p.n = dim;
   p.k = (int32_t)rows;
-  p.scale = scale;
+  p.unscale = unscale;
   p.out = dweight;
   p.sums = sums;
   return p;
@@ -295,7 +276,7 @@ int64_t forward_sums(int64_t m, int64_t n, int64_t k, bool gated) {
 
 struct LinearWork {
   TwoPlans plans;  // dx, dweight
-  int64_t dz, forward, dx, dweight, rows, parts, scale, bytes;
+  int64_t dz, forward, dx, dweight, rows, parts, unscale, bytes;
 };
 LinearWork work_of(const nd_linear* a, bool backward) {
   LinearWork w = {};
@@ -311,7 +292,7 @@ LinearWork work_of(const nd_linear* a, bool backward) {
     w.dweight = l.take(a->dweight ? sums_bytes(w.plans.second, dweight.m, dweight.n) : 0);
     w.rows = l.take(a->dbias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
     w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
-    w.scale = l.take(scaled ? 8 : 0);
+    w.unscale = l.take(scaled ? 4 : 0);
   }
   w.bytes = l.bytes;
   return w;
@@ -356,30 +337,30 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
   }
   const void* dz = a->dout;
   int64_t dz_bytes = a->dout_row * 2;
-  const float* scale = nullptr;
-  float* rows = (float*)(work + w.rows);
+  float *unscale = nullptr, *rows = (float*)(work + w.rows);
   if (active && (a->dx || a->dweight || a->dbias)) {
-    if (!call.bf16) {
-      scale = (const float*)(work + w.scale);
-      call.survey(a->dout, dz_bytes, a->rows, a->out_dim, nullptr, nullptr, (float*)(work + w.parts), (float*)(work + w.scale));
-    }
     LinearParams p = {};
+    if (!call.bf16) {
+      unscale = p.unscale = (float*)(work + w.unscale);
+      p.parts = (const float*)(work + w.parts);
+      p.n_parts = survey_parts(a->rows, a->out_dim);
+      call.survey(a->dout, dz_bytes, a->rows, a->out_dim, nullptr, nullptr, (float*)(work + w.parts));
+    }
     p.m = (int32_t)a->rows;
     p.n = a->out_dim;
     p.activation = a->activation;
     p.z = a->z;
-    p.scale = scale;
     p.out = work + w.dz;
-    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr, nullptr);
+    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr, row_shares(a->rows, a->out_dim), nullptr);
     if (a->dbias) call.join(rows, row_shares(a->rows, a->out_dim), a->out_dim, nullptr, a->dbias);
     dz = work + w.dz;
     dz_bytes = (int64_t)a->out_dim * 2;
   } else if (a->dbias) {
-    call.survey(a->dout, dz_bytes, a->rows, a->out_dim, rows, a->dbias, nullptr, nullptr);
+    call.survey(a->dout, dz_bytes, a->rows, a->out_dim, rows, a->dbias, nullptr);
   }
-  const LinearParams dx = gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, scale, a->dx, (float*)(work + w.dx));
+  const LinearParams dx = gradient_of_x(dz, dz_bytes, a->weight, a->rows, a->out_dim, a->dim, unscale, a->dx, (float*)(work + w.dx));
   const LinearParams dweight =
-      gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, scale, a->dweight, (float*)(work + w.dweight));
+      gradient_of_weight(dz, dz_bytes, a->x, a->x_row * 2, a->rows, a->out_dim, a->dim, unscale, a->dweight, (float*)(work + w.dweight));
   call.backward(a->dx ? &dx : nullptr, After::kPlain, a->dweight ? &dweight : nullptr, w.plans);
   call.add_up();
   return call.done();
@@ -390,7 +371,7 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
 struct MlpWork {
   TwoPlans first, second;  // dz and ddown; dx and dup
   int64_t shares;          // of the rows, whose sums the product that makes dz leaves
-  int64_t dz, forward, dx, dup, ddown, rows, columns, parts, scale, bytes;
+  int64_t dz, forward, dx, dup, ddown, rows, columns, parts, unscale, bytes;
 };
 MlpWork work_of(const nd_mlp* a, bool backward) {
   MlpWork w = {};
@@ -413,7 +394,7 @@ MlpWork work_of(const nd_mlp* a, bool backward) {
     w.rows = l.take(a->ddown_bias ? row_shares(a->rows, a->out_dim) * a->out_dim * 4 : 0);
     w.columns = l.take(a->dup_bias ? w.shares * wide * 4 : 0);
     w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
-    w.scale = l.take(scaled ? 8 : 0);
+    w.unscale = l.take(scaled ? 4 : 0);
   }
   w.bytes = l.bytes;
   return w;
@@ -473,9 +454,9 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     return call.done();
   }
   const int64_t dout_bytes = a->dout_row * 2;
-  float* scale = first && !call.bf16 ? (float*)(work + w.scale) : nullptr;
-  if (a->ddown_bias || scale)
-    call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, (float*)(work + w.parts), scale);
+  float* parts = first && !call.bf16 ? (float*)(work + w.parts) : nullptr;
+  float* unscale = parts ? (float*)(work + w.unscale) : nullptr;
+  if (a->ddown_bias || parts) call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, parts);
   float* columns = a->dup_bias ? (float*)(work + w.columns) : nullptr;
   LinearParams p = {};
   p.p = a->down;
@@ -489,15 +470,17 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   p.gated = a->gated;
   p.z = slope ? a->z : nullptr;
   p.out = work + w.dz;
-  p.scale = scale;
+  p.parts = parts;
+  p.n_parts = parts ? survey_parts(a->rows, a->out_dim) : 0;
+  p.unscale = unscale;
   p.column_sums = columns;
   const LinearParams ddown =
       gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, (float*)(work + w.ddown));
   call.backward(first ? &p : nullptr, After::kSlope, a->ddown ? &ddown : nullptr, w.first);
-  if (columns) call.join(columns, w.shares, wide, scale ? scale + 1 : nullptr, a->dup_bias);
+  if (columns) call.join(columns, w.shares, wide, unscale, a->dup_bias);
   const char* dz = work + w.dz;
-  const LinearParams dx = gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, scale, a->dx, (float*)(work + w.dx));
-  const LinearParams dup = gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, scale, a->dup, (float*)(work + w.dup));
+  const LinearParams dx = gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, unscale, a->dx, (float*)(work + w.dx));
+  const LinearParams dup = gradient_of_weight(dz, wide_bytes, a->x, a->x_row * 2, a->rows, wide, a->dim, unscale, a->dup, (float*)(work + w.dup));
   call.backward(a->dx ? &dx : nullptr, After::kPlain, a->dup ? &dup : nullptr, w.second);
   call.add_up();
   return call.done();

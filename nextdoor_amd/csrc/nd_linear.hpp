@@ -31,7 +31,11 @@ struct LinearParams {
   int64_t residual_bytes;  // of a row
   void* out;
   void* z;  // forward: written unless null; backward: read.  [m][n]; gated: rows of 6 n bytes, see Upper24
-  const float* scale;  // null: 1; kSlope: the sums are multiplied with scale[0]; kPlain: with scale[1], one over it
+  // float16: what dz is held times.  parts: the largest finite |dout| of workgroups, null: 1.  Who makes dz finds the scale in them and
+  // leaves one over it in *unscale, with which the sums of kPlain are multiplied (null: 1).
+  const float* parts;
+  int64_t n_parts;
+  float* unscale;
   // shares of the sum: share s has places s * share .. and leaves [m][n] values (gated: [m][2 n]) in 32 bits
   float* sums;
   int32_t shares, share;
@@ -59,6 +63,16 @@ struct Upper24 {
     v[3] = __uint_as_float(__builtin_amdgcn_perm(upper[1], next, 0x0706030c));
   }
 };
+
+// The power of two that takes the largest of all parts to between 1/2 and 1 (1, if that is 0); for all lanes of a wave.
+__device__ __forceinline__ float scale_of(const float* parts, int64_t n, int lane) {
+  float most = 0.f;
+#pragma unroll 4
+  for (int64_t i = lane; i < n; i += 64) most = fmaxf(most, parts[i]);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  return most > 0.f ? ldexpf(1.f, -(ilogbf(most) + 1)) : 1.f;
+}
 
 // The sums of 16 values over the 32 lanes of a half: lane l has that of value l & 15.  Each step sends half of the values on.
 __device__ __forceinline__ float sums_of_rows(const float (&v)[16], int lane) {
@@ -312,7 +326,8 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
     auto bring_next = [&](int part) {
       if (gated) next.bring((const char*)a.z + 2 * n_bytes, z_bytes, row_of(part), a.m, column_of(part), a.n, lane);
     };
-    const float factor = a.scale ? a.scale[0] : 1.f;
+    const float factor = a.parts ? scale_of(a.parts, a.n_parts, lane) : 1.f;
+    if (a.parts && block == 0 && share == 0 && threadIdx.x == 0) *a.unscale = 1.f / factor;
     bring(0);
     bring_next(0);
     float own_sums[2], other_sums[2];
@@ -397,7 +412,7 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
     auto bring = [&](int j) {
       if (residual) Out{mine + (ahead ? step * j : 0) * Out::kSize}.bring(a.residual, a.residual_bytes, wave_row0 + 32 * j, a.m, wave_column0, a.n, lane);
     };
-    const float factor = AFTER == After::kPlain && a.scale ? a.scale[1] : 1.f;
+    const float factor = AFTER == After::kPlain && a.unscale ? *a.unscale : 1.f;
     Bias bias[S::kM];
     if (AFTER == After::kForward && a.bias) {
 #pragma unroll
@@ -590,8 +605,8 @@ template <class T>
 hipError_t launch_joins(const Joins& joins, uint32_t blocks, hipStream_t stream);
 template <class T>
 hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
-// dz = dout a'(z) times scale[0], if there is a z, and unless they are null sums of its rows (times 1), and the largest finite
-// |dout| of each workgroup.
+// dz = dout a'(z), held times its scale, if there is a z, and unless they are null sums of its rows (times 1), and the largest
+// finite |dout| of each workgroup.
 template <class T>
 hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts, hipStream_t stream);
 constexpr int kSlopeColumns = 64;  // of a workgroup there

@@ -116,9 +116,11 @@ __global__ __launch_bounds__(256) void slope_kernel(LinearParams a, const void* 
   float total[8], most = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) total[i] = 0.f;
-  const float factor = a.scale ? a.scale[0] : 1.f;
+  const float factor = a.parts ? scale_of(a.parts, a.n_parts, threadIdx.x & 63) : 1.f;
+  if (a.parts && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.unscale = 1.f / factor;
   if (c < a.n) {
     const int64_t begin = blockIdx.y * rows_per_share, end = min(begin + rows_per_share, (int64_t)a.m);
+#pragma unroll 4
     for (int64_t row = begin + r0; row < end; row += 32) {
       u32x4 w = *(const u32x4*)((const char*)dout + row * dout_bytes + (int64_t)c * 2);
       float d[8];

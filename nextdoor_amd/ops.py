@@ -459,8 +459,9 @@ def layer_norm_backward(dout, x, weight, mean, rstd, needs=(True, True, True)):
             raise NextDoorError("layer norm: mean and rstd are not a forward pass's")
     dout, dout_row = _rows_in_place(dout, fields[1], 1)
     kind = x.dtype if weight is None else weight.dtype
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
-    dweight, dbias = (torch.empty(fields[1], dtype=kind, device=x.device) if need else None for need in needs[1:])
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if needs[0] else None
+    dweight = torch.empty(fields[1], dtype=kind, device=x.device) if needs[1] else None
+    dbias = torch.empty(fields[1], dtype=kind, device=x.device) if needs[2] else None
     a = LayerNorm(*fields, x_row, dout_row, rows.data_ptr(), _pointer(weight), None, None, mean.data_ptr(), rstd.data_ptr(),
                   dout.data_ptr(), _pointer(dx), _pointer(dweight), _pointer(dbias))
     workspace = _room(a, _library().nd_layer_norm_workspace(a), x.device)
@@ -545,7 +546,7 @@ def _check_rows(what, name, t, shape, dtype):
 
 def _result(x, wanted, *shape):
     """Room for a result that the kernels write as a matrix or vector of `shape`, in the shape that is wanted where both are the same."""
-    return torch.empty(wanted if wanted[-1] == shape[-1] else shape, dtype=x.dtype, device=x.device)
+    return x.new_empty(wanted if wanted[-1] == shape[-1] else shape)
 
 
 def _cut(t, *shape):
@@ -594,7 +595,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep=Fa
     weight, bias = _matrix(weight), _matrix(bias)
     n = rows.shape[0]
     out = _result(x, shape, n, wide)
-    z = torch.empty((n, wide), dtype=x.dtype, device=x.device) if keep and code else None
+    z = x.new_empty((n, wide)) if keep and code else None
     a = Linear(n, weight.shape[1], wide, _DTYPES[x.dtype], code, x_row, residual_row, 0, rows.data_ptr(), weight.data_ptr(), _pointer(bias),
                _pointer(residual), out.data_ptr(), _pointer(z))
     workspace = _room(a, _library().nd_linear_workspace(a, 0), x.device)
@@ -620,8 +621,8 @@ def linear_backward(dout, x, weight, z=None, activation=None, with_bias=True, ne
     if code and not (z is not None and z.shape == (n, wide) and z.is_contiguous()):
         raise NextDoorError("linear: z is not what a forward pass kept")
     dx = _result(x, x.shape, n, high) if needs[0] else None
-    dweight = torch.empty((wide, high), dtype=x.dtype, device=x.device) if needs[1] else None
-    dbias = torch.empty(wide, dtype=x.dtype, device=x.device) if with_bias else None
+    dweight = torch.empty_like(weight) if needs[1] else None
+    dbias = x.new_empty(wide) if with_bias else None
     a = Linear(n, high, wide, _DTYPES[x.dtype], code, x_row, 0, dout_row, rows.data_ptr(), weight.data_ptr(), None, None, None,
                _pointer(z) if code else None, dout.data_ptr(), _pointer(dx), _pointer(dweight), _pointer(dbias))
     workspace = _room(a, _library().nd_linear_workspace(a, 1), x.device)
@@ -709,15 +710,12 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
     up, up_bias, down, down_bias = _up(up, inner, gated), _up(up_bias, inner, gated), _matrix(down), _matrix(down_bias)
     n, wide = rows.shape[0], down.shape[0]
 
-    def empty(columns):
-        return torch.empty((n, columns), dtype=x.dtype, device=x.device)
-
-    out, h = _result(x, shape, n, wide), empty(down.shape[1])
+    out, h = _result(x, shape, n, wide), x.new_empty((n, down.shape[1]))
     z = None
     if keep and gated:
         z = torch.empty((n, 3 * up.shape[0]), dtype=torch.uint8, device=x.device)
     elif keep and code:
-        z = empty(up.shape[0])
+        z = x.new_empty((n, up.shape[0]))
     a = Mlp(n, up.shape[1], down.shape[1], wide, _DTYPES[x.dtype], code, gated, x_row, residual_row, 0, rows.data_ptr(), up.data_ptr(),
             _pointer(up_bias), down.data_ptr(), _pointer(down_bias), _pointer(residual), out.data_ptr(), _pointer(z), h.data_ptr())
     workspace = _room(a, _library().nd_mlp_workspace(a, 0), x.device)
@@ -748,12 +746,9 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
         if z is None or (z.shape, z.dtype) != kept or not z.is_contiguous():
             raise NextDoorError("mlp: z is not what a forward pass kept")
 
-    def empty(need, *size):
-        return torch.empty(size, dtype=x.dtype, device=x.device) if need else None
-
     dx = _result(x, x.shape, n, up.shape[1]) if needs[0] else None
-    dup, ddown = empty(needs[1], *up.shape), empty(needs[2], *down.shape)
-    dup_bias, ddown_bias = empty(with_up_bias, up.shape[0]), empty(with_down_bias, down.shape[0])
+    dup, ddown = torch.empty_like(up) if needs[1] else None, torch.empty_like(down) if needs[2] else None
+    dup_bias, ddown_bias = x.new_empty(up.shape[0]) if with_up_bias else None, x.new_empty(down.shape[0]) if with_down_bias else None
     a = Mlp(n, up.shape[1], down.shape[1], down.shape[0], _DTYPES[x.dtype], code, gated, x_row, 0, dout_row, rows.data_ptr(), up.data_ptr(),
             None, down.data_ptr(), None, None, None, _pointer(z), h.data_ptr(), dout.data_ptr(), _pointer(dx), _pointer(dup),
             _pointer(dup_bias), _pointer(ddown), _pointer(ddown_bias))
