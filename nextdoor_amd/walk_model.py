@@ -3,7 +3,8 @@
 Walks are its sentences, vertices its words.  The engine samples one walk from every vertex, once; a step takes some of them,
 packs them one after another (a walk ends where a vertex has no edges), and trains a small transformer to predict each next
 vertex: embeddings with dropout, causal attention within each walk, softmax cross entropy over all vertices
-(nextdoor_amd/ops.py).  It shows the operators as a training program uses them; nothing is tuned for accuracy.
+(nextdoor_amd/ops.py).  With ``--gated`` its blocks are a gated feed-forward part and projections and norms that are operators
+of the library too, so that all of a block is.  It shows the operators as a training program uses them; nothing is tuned for accuracy.
 """
 import argparse
 import time
@@ -50,17 +51,44 @@ class Block(nn.Module):
         return ops.dropout(self.down(F.gelu(self.up(self.norm2(x)))), self.p, seed, step + 1, residual=x)
 
 
+class GatedBlock(nn.Module):
+    """A block that is the library's operators from end to end, its feed-forward part gated."""
+
+    def __init__(self, width, heads, kv_heads, p):
+        super().__init__()
+        self.heads, self.kv_heads, self.dim, self.p = heads, kv_heads, width // heads, p
+        inner = 8 * -(-width // 3)  # two matrices into it: as many weights as with 4 width and one
+        self.norm1, self.norm2 = nn.LayerNorm(width), nn.LayerNorm(width)
+        self.qkv = nn.Linear(width, (heads + 2 * kv_heads) * self.dim, bias=False)
+        self.out = nn.Linear(width, width, bias=False)
+        self.up, self.down = nn.Linear(width, 2 * inner, bias=False), nn.Linear(inner, width, bias=False)
+
+    def forward(self, x, sequences, seed, step):
+        qkv = ops.linear(normed(x, self.norm1), self.qkv.weight).view(x.shape[0], -1, self.dim)
+        q, k, v = qkv.split([self.heads, self.kv_heads, self.kv_heads], dim=1)
+        attended = ops.packed_attention(q, k, v, sequences).reshape(x.shape)
+        if not self.p:  # what comes back is added to x in the products themselves
+            x = ops.linear(attended, self.out.weight, residual=x)
+            return ops.mlp(normed(x, self.norm2), self.up.weight, self.down.weight, residual=x)
+        x = ops.dropout(ops.linear(attended, self.out.weight), self.p, seed, step, residual=x)
+        return ops.dropout(ops.mlp(normed(x, self.norm2), self.up.weight, self.down.weight), self.p, seed, step + 1, residual=x)
+
+
+def normed(x, norm):
+    return ops.layer_norm(x, norm.weight, norm.bias, norm.eps)
+
+
 class WalkModel(nn.Module):
     """Next-vertex prediction; the embeddings of the vertices are the classes' vectors too."""
 
-    def __init__(self, n_vertices, width=64, heads=2, kv_heads=1, layers=2, longest=128, dropout=0.1):
+    def __init__(self, n_vertices, width=64, heads=2, kv_heads=1, layers=2, longest=128, dropout=0.1, gated=False):
         super().__init__()
-        self.p = dropout
+        self.p, self.gated = dropout, gated
         self.vertices = nn.Embedding(n_vertices, width)
         self.places = nn.Embedding(longest, width)
         nn.init.normal_(self.vertices.weight, std=width ** -0.5)
         nn.init.normal_(self.places.weight, std=width ** -0.5)
-        self.blocks = nn.ModuleList(Block(width, heads, kv_heads, dropout) for _ in range(layers))
+        self.blocks = nn.ModuleList((GatedBlock if gated else Block)(width, heads, kv_heads, dropout) for _ in range(layers))
         self.norm = nn.LayerNorm(width)
 
     def forward(self, tokens, places, targets, sequences, seed):
@@ -70,7 +98,8 @@ class WalkModel(nn.Module):
         x = ops.dropout(x, self.p, seed, 0)
         for i, block in enumerate(self.blocks):
             x = block(x, sequences, seed, 1 + 2 * i)
-        return ops.vocabulary_loss(self.norm(x), self.vertices.weight, targets)
+        x = normed(x, self.norm) if self.gated else self.norm(x)
+        return ops.vocabulary_loss(x, self.vertices.weight, targets)
 
 
 def batch_of(tokens, targets, starts, device="cuda"):
@@ -114,10 +143,11 @@ def main(argv=None):
     p.add_argument("--walks", type=int, default=1024, help="walks in a batch")
     p.add_argument("--width", type=int, default=64)
     p.add_argument("--layers", type=int, default=2)
+    p.add_argument("--gated", action="store_true", help="gated feed-forward parts; norms and projections are the library's too")
     p.add_argument("--seed", type=int, default=42)
     args = p.parse_args(argv)
     graph = Graph.load(args.graph_file) if args.graph_file else Graph.chung_lu(10000, 150000, 2.2, seed=args.seed)
-    train(graph, args.steps, args.walks, args.seed, width=args.width, layers=args.layers)
+    train(graph, args.steps, args.walks, args.seed, width=args.width, layers=args.layers, gated=args.gated)
 
 
 if __name__ == "__main__":

@@ -478,3 +478,76 @@ def test_an_autograd_step_is_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+
+
+# ---- together ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_a_gated_walk_model_has_the_gradients_of_plain_operations(p, monkeypatch):
+    """One step of the model in 16 bits against the same model with the definitions in 64 bits: every operator of the library."""
+    import numpy as np
+    from nextdoor_amd import walk_model
+    from tests import operators_reference
+    torch.manual_seed(1)
+    n = 97
+    rng = np.random.default_rng(2)
+    samples = rng.integers(0, n, (20, 30)).astype(np.int32)
+    for walk in samples[::2]:
+        walk[rng.integers(0, 30):] = n
+    tokens, targets, starts = walk_model.pack_walks(rng.integers(0, n, 20), samples, n)
+    how = dict(width=64, heads=2, kv_heads=1, layers=1, dropout=p, gated=True)
+    model = walk_model.WalkModel(n, **how).to("cuda", BF16)
+    batch = walk_model.batch_of(tokens, targets, starts)
+    each = model(*batch[:3], batch[3], 11)
+    each.sum().backward()
+    exact = walk_model.WalkModel(n, **how).double()
+    exact.load_state_dict({k: v.double().cpu() for k, v in model.state_dict().items()})
+
+    of = torch.from_numpy(np.repeat(np.arange(len(starts) - 1), np.diff(starts)))
+    at = torch.arange(len(of))
+    sees = (of[:, None] == of) & (at[:, None] >= at)
+    f = torch.nn.functional
+
+    def attention(q, k, v, sequences, scale=None):
+        out = []
+        for h in range(q.shape[1]):
+            i = h // (q.shape[1] // k.shape[1])
+            s = (q[:, h] @ k[:, i].T / math.sqrt(q.shape[2])).masked_fill(~sees, -math.inf)
+            out.append(torch.softmax(s, 1) @ v[:, i])
+        return torch.stack(out, 1)
+
+    def drop(x, p, seed, step, residual=None):
+        kept = torch.from_numpy(operators_reference.uniforms(x.numel(), seed, step) >= np.float32(p)).view(x.shape)
+        y = x * kept / (1 - p)
+        return y if residual is None else y + residual
+
+    def loss(h, w, t):
+        has = (t >= 0) & (t < n)
+        z = h @ w.T
+        return torch.where(has, torch.logsumexp(z, 1) - z.gather(1, torch.where(has, t, 0).long()[:, None])[:, 0], 0.0)
+
+    def plain_mlp(x, up, down, residual=None):
+        g, u = f.linear(x, up).chunk(2, -1)
+        y = f.linear(f.silu(g) * u, down)
+        return y if residual is None else y + residual
+
+    plain = {"packed_attention": attention, "dropout": drop, "vocabulary_loss": loss, "mlp": plain_mlp,
+             "linear": lambda x, w, residual=None: f.linear(x, w) if residual is None else f.linear(x, w) + residual,
+             "layer_norm": lambda x, w, b, eps: f.layer_norm(x, x.shape[-1:], w, b, eps)}
+    for name, function in plain.items():
+        monkeypatch.setattr(ops, name, function)
+    right = exact(*[torch.from_numpy(np.ascontiguousarray(a)) for a in
+                    (tokens, np.arange(len(tokens)) - np.repeat(starts[:-1], np.diff(starts)), targets)], None, 11)
+    right.sum().backward()
+    # some thirty roundings of 2^-8 on the way there and back, each of what is of the size of the result
+    assert float((each.detach().cpu().double() - right.detach()).norm() / right.detach().norm()) < 30 * 2.0 ** -8
+    for (name, a), b in zip(model.named_parameters(), exact.parameters()):
+        assert float((a.grad.cpu().double() - b.grad).norm() / b.grad.norm()) < 60 * 2.0 ** -8, name
+
+
+def test_the_gated_walk_model_trains():
+    from nextdoor_amd import Graph, walk_model
+    graph = Graph.chung_lu(500, 6000, 2.2, seed=3)
+    losses = [walk_model.train(graph, steps=3, walks=200, seed=5, log=None, gated=True)[1] for _ in range(2)]
+    assert len(losses[0]) == 3 and all(math.isfinite(v) for v in losses[0]) and losses[0][0] == losses[1][0]
