@@ -67,7 +67,8 @@ __device__ __forceinline__ void activate_with_slope(int activation, float (&x)[N
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float square = kTanhCube * x[i] * x[i], s = logistic(2.f * kTanhInside * x[i] * (1.f + square));
-      slope[i] = __builtin_fmaf(2.f * kTanhInside * x[i] * s * (1.f - s), __builtin_fmaf(3.f, square, 1.f), s);
+      const float flat = s * (1.f - s);  // (0 where the square may be infinite)
+      slope[i] = flat == 0.f ? s : __builtin_fmaf(2.f * kTanhInside * x[i] * flat, __builtin_fmaf(3.f, square, 1.f), s);
       x[i] *= s;
     }
   } else if (activation == ND_SILU) {

@@ -8,8 +8,9 @@
 // both by columns (gradient of the weights).  What follows a product is done to its results before they leave the registers.
 // Sums are held in 32 bits; z, h and dz, which the next product or the backward pass reads, are rounded to 16 bits once, as
 // the results are; but the z of a gated part, of which g and u are both factors of dz, keeps the upper 24 bits of 32: rounded to
-// bfloat16 they had brought the gradients' error from 2.4e-3 to 3.0e-3 (1.7e-3 is that of rounding them alone).  float16: dz is held times a power of two that takes max |dy| to between 1/2 and 1, so that the small
-// gradients of a mean over many rows are not lost below 2^-14; what is made of it is divided by that in 32 bits.
+// bfloat16 they had brought the gradients' error from 2.4e-3 to 3.0e-3 (1.7e-3 is that of rounding them alone).  float16: dz is held
+// times a power of two, so that the small gradients of a mean over many rows are not lost below 2^-14: see scale_of.  What is made of
+// it is divided by that in 32 bits.
 #pragma once
 
 #include <algorithm>
@@ -64,14 +65,18 @@ struct Upper24 {
   }
 };
 
-// The power of two that takes the largest of all parts to between 1/2 and 1 (1, if that is 0); for all lanes of a wave.
+// What dz is held times, for all lanes of a wave: a power of two that takes the largest |dout|, of all parts, to 16 or more where it is
+// less, and to below 256 where it is more.  Smaller rows next to larger ones lose nothing that dout itself has in 16 bits (but the
+// last bits of what is below 2^-14 next to more than 256), and dz may be 255 times the largest |dout|, 2000 times below 16.
 __device__ __forceinline__ float scale_of(const float* parts, int64_t n, int lane) {
   float most = 0.f;
 #pragma unroll 4
   for (int64_t i = lane; i < n; i += 64) most = fmaxf(most, parts[i]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  return most > 0.f ? ldexpf(1.f, -(ilogbf(most) + 1)) : 1.f;
+  if (most == 0.f) return 1.f;
+  const int power = ilogbf(most);
+  return ldexpf(1.f, power < 4 ? 4 - power : power > 7 ? 7 - power : 0);
 }
 
 // The sums of 16 values over the 32 lanes of a half: lane l has that of value l & 15.  Each step sends half of the values on.
@@ -174,7 +179,7 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
   if constexpr (LAYOUT == Layout::kRows) {
     using P = product::ByRows<S::kTileM, S::kDepth, S::kThreads, kGated>;
     using Q = product::ByRows<S::kTileN, S::kDepth, S::kThreads>;
-    product::multiply<T, S>(acc, P(a.p, a.p_bytes, column0, a.n, place_end, a.n), Q(a.q, a.q_bytes, row0, a.m, place_end), place0, place_end, tiles);
+    product::multiply<T, S>(acc, P(a.p, a.p_bytes, column0, a.n, place_end, a.n * a.p_bytes), Q(a.q, a.q_bytes, row0, a.m, place_end), place0, place_end, tiles);
   } else if constexpr (LAYOUT == Layout::kWeightColumns) {
     using P = product::ByColumns<S::kTileM, S::kDepth, S::kThreads>;
     using Q = product::ByRows<S::kTileN, S::kDepth, S::kThreads>;

@@ -37,29 +37,31 @@ struct Shape {
 // thread that asked for it, makes it 0; what lies past the last row is some row.  Offsets are 32 bits wide: ROWS (or DEPTH) rows of
 // a matrix lie within 4 GiB.
 
-// [row][place].  GATED: blocks of 32 rows come in turn from the first half of the matrix and, `other` rows further, from the
-// second; row0 and row_end count those of one half.
+// [row][place].  GATED: blocks of 32 rows come in turn from the first half of the matrix and, `other_bytes` further, from the second;
+// row0 and row_end count those of one half.
 template <int ROWS, int DEPTH, int THREADS, bool GATED = false>
 struct ByRows {
   static constexpr int kRowChunks = DEPTH / 8, kChunks = ROWS * kRowChunks, kTurns = kChunks / THREADS;
-  static_assert(kChunks % THREADS == 0 && THREADS / kRowChunks % 16 == 0, "");
+  static_assert(kChunks % THREADS == 0 && THREADS / kRowChunks % 16 == 0 && 64 / kRowChunks <= 32, "");
   const char* base;
+  int64_t other_bytes;
   uint32_t offset[kTurns];
   int places, chunk;
-  __device__ __forceinline__ ByRows(const void* matrix, int64_t row_bytes, int row0, int row_end, int places_, int other = 0)
-      : base((const char*)matrix + row0 * row_bytes), places(places_) {
+  __device__ __forceinline__ ByRows(const void* matrix, int64_t row_bytes, int row0, int row_end, int places_, int64_t other_bytes_ = 0)
+      : base((const char*)matrix + row0 * row_bytes), other_bytes(other_bytes_), places(places_) {
 #pragma unroll
     for (int i = 0; i < kTurns; ++i) {
       const int at = threadIdx.x + THREADS * i, r = at / kRowChunks, c = (at % kRowChunks) ^ tile_swizzle<kRowChunks>(r);
-      const int row = min(GATED ? (r >> 6) * 32 + (r & 31) : r, row_end - 1 - row0) + (GATED && (r & 32) ? other : 0);
-      offset[i] = (uint32_t)(row * row_bytes + c * 16);
+      offset[i] = (uint32_t)(min(GATED ? (r >> 6) * 32 + (r & 31) : r, row_end - 1 - row0) * row_bytes + c * 16);
       chunk = c;  // (the same in every turn)
     }
   }
   template <bool WHOLE>
   __device__ __forceinline__ void load(int i, uint32_t wave_lds, int place0) const {
     const uint32_t past = WHOLE || place0 + chunk * 8 < places ? 0 : chunk * 16;  // (the round's first place is there)
-    load_to_lds(base + (int64_t)place0 * 2, offset[i] - past, wave_lds + THREADS * 16 * i);
+    // (a wave's rows are of one half)
+    const bool second = GATED && ((uniform(threadIdx.x >> 6) * (64 / kRowChunks) + THREADS / kRowChunks * i) & 32);
+    load_to_lds(base + (int64_t)place0 * 2 + (second ? other_bytes : 0), offset[i] - past, wave_lds + THREADS * 16 * i);
   }
   __device__ __forceinline__ void clear(u32x4* tile, int place0) const {
     if (place0 + chunk * 8 < places) return;

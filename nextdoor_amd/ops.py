@@ -448,17 +448,22 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     return out, mean, rstd
 
 
-def layer_norm_backward(dout, x, weight, mean, rstd, needs=(True, True, True)):
+def layer_norm_backward(dout, x, weight, mean, rstd, needs=(True, True, True), dtype=None):
     """(dx, dweight, dbias) for the gradient ``dout`` of ``out``; mean and rstd are the forward pass's, ``weight`` None if there was
-    none (the gradients of weight and bias then have the type of x).  ``needs``: which to compute; the others are None."""
+    none.  dweight and dbias are of the type of weight; without one of ``dtype``, that of x or float32, by default that of x.
+    ``needs``: which to compute; the others are None."""
     index, rows, fields, x_row, weight, _ = _norm(x, weight, None, 0.0, (dout, mean, rstd))
+    if weight is None and dtype is not None:
+        if dtype is not x.dtype and dtype is not torch.float32:
+            raise NextDoorError("layer norm: gradients of the type of x or float32, not %s" % dtype)
+        fields = (*fields[:3], _DTYPES[dtype], fields[4])
     if dout.shape != x.shape or dout.dtype is not x.dtype:
         raise NextDoorError("layer norm: dout is of another shape or type than x")
     for t in (mean, rstd):
         if not (t.shape == (fields[0],) and t.dtype is torch.float32 and t.is_contiguous()):
             raise NextDoorError("layer norm: mean and rstd are not a forward pass's")
     dout, dout_row = _rows_in_place(dout, fields[1], 1)
-    kind = x.dtype if weight is None else weight.dtype
+    kind = weight.dtype if weight is not None else x.dtype if dtype is None else dtype
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if needs[0] else None
     dweight = torch.empty(fields[1], dtype=kind, device=x.device) if needs[1] else None
     dbias = torch.empty(fields[1], dtype=kind, device=x.device) if needs[2] else None
@@ -491,12 +496,13 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         x, weight, mean, rstd = ctx.saved_tensors
-        dx, dweight, dbias = layer_norm_backward(dout, x, weight, mean, rstd, ctx.needs_input_grad[:3])
-        return dx, dweight, dbias if dbias is None else dbias.to(ctx.bias_dtype), None
+        return (*layer_norm_backward(dout, x, weight, mean, rstd, ctx.needs_input_grad[:3], ctx.bias_dtype), None)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """The ``out`` of :func:`layer_norm_forward`, differentiable in x, weight and bias."""
+    if not torch.is_grad_enabled():
+        return layer_norm_forward(x, weight, bias, eps)[0]
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
@@ -608,7 +614,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep=Fa
 def linear_backward(dout, x, weight, z=None, activation=None, with_bias=True, needs=(True, True)):
     """(dx, dweight, dbias) for the gradient ``dout`` of ``out``; z is what the forward pass kept.  The residual's gradient is
     ``dout`` itself.  ``needs``: whether dx and dweight are wanted; what is not is None.  With an activation the gradient of z is
-    rounded to 16 bits before its products (float16: relative to max |dout|, so that small ones are not lost)."""
+    rounded to 16 bits before its products (float16: held times a power of two, so that small ones are not lost)."""
     index = _on_gpu("linear", x, dout, weight, *(() if z is None else (z,)))
     _types("linear", x, dout, weight, z)
     code = _activation("linear", activation)
@@ -654,6 +660,8 @@ class _Linear(torch.autograd.Function):
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """:func:`linear_forward`, differentiable in x, weight, bias and the residual."""
+    if not torch.is_grad_enabled():  # (nothing is kept)
+        return linear_forward(x, weight, bias, activation, residual)
     return _Linear.apply(x, weight, bias, residual, activation)
 
 
@@ -729,7 +737,8 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
                  needs=(True, True, True)):
     """(dx, dup, ddown, dup_bias, ddown_bias) for the gradient ``dout`` of ``out``; z and h are what the forward pass kept.  The
     residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None.  The gradient of z
-    is rounded to 16 bits before its products (float16: relative to max |dout|, and must stay below 65504 times that)."""
+    is rounded to 16 bits before its products (float16: held times a power of two, so that small ones are not lost; it may be 255
+    times max |dout|, and what is more may become infinite)."""
     index = _on_gpu("mlp", x, dout, up, down, h, *(() if z is None else (z,)))
     _types("mlp", x, dout, up, down, h)
     gated = bool(gated)
@@ -782,4 +791,6 @@ class _Mlp(torch.autograd.Function):
 
 def mlp(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None):
     """:func:`mlp_forward`, differentiable in x, the weights, the biases and the residual."""
+    if not torch.is_grad_enabled():
+        return mlp_forward(x, up, down, up_bias, down_bias, activation, gated, residual)
     return _Mlp.apply(x, up, down, up_bias, down_bias, activation, gated, residual)

@@ -86,10 +86,11 @@ def linear(x, weight, bias=None, name=None, residual=None, dout=None):
 
 
 def _held(d, least):
-    """What is lost of dz below the smallest number, dz being held relative to max |dout| (float16)."""
+    """What is lost of dz below the smallest number.  float16: dz is held times a power of two that takes max |dout| to 16 or more,
+    and to below 256."""
     finite = d[torch.isfinite(d)]
     most = float(finite.abs().max()) if finite.numel() else 0.0
-    return least * 2 * most if least > 2.0 ** -100 else least
+    return least * max(most / 16 if most < 16 else 1, most / 128) if least > 2.0 ** -100 else least
 
 
 def mlp(x, up, down, up_bias=None, down_bias=None, name="silu", gated=True, residual=None, dout=None):

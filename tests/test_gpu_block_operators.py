@@ -362,6 +362,104 @@ def test_mlp_reads_slices_in_place_and_gives_what_is_wanted():
                 assert (g is None) != need and (g is None or torch.equal(g, a))
 
 
+# ---- the ends of the ranges -----------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("big", [1.0, 3e2, 6e4])
+def test_small_rows_next_to_large_ones_keep_their_gradients(big):
+    """16-bit floats: what all rows of the gradient of z are held times does not lose the smaller ones."""
+    x, w, b, name, r, d = linear_case(200, 128, 256, F16, "gelu")
+    d = d.float().clamp(-1, 1)
+    d[::2] *= big
+    d[1::2] *= 1e-3
+    d = d.to(F16)
+    want, off = ref.linear(x, w, b, name, r, d)
+    got = run_linear(x, w, b, name, r, d)
+    check_all({n: got[n] for n in ("out", "dx", "dbias")}, want, off, big)
+    small = (got["dx"].cpu().double() - want["dx"])[1::2].norm() / want["dx"][1::2].norm()
+    # roundings of the gradient of z and of the result, 2^-11 each; z's own has a slope below 1; above 256 the last bits are cut
+    assert small < (2.0 ** -9 if big <= 256 else 2.0 ** -4)
+
+
+def test_slopes_of_pre_activations_of_any_size():
+    """z from 1e-30 to 1e30: slopes are 0 or 1 at the ends, and never NaN."""
+    sizes = torch.logspace(-30, 30, 61)
+    x = torch.zeros(122, 64)
+    x[:61, 0], x[61:, 0] = sizes, -sizes
+    x, w = x.to(BF16), torch.zeros(16, 64)
+    w[:, 0] = 1
+    w = w.to(BF16)
+    d = torch.ones(122, 16, dtype=BF16)
+    for name in ACTIVATIONS:
+        want, off = ref.linear(x, w, None, name, None, d)
+        got = run_linear(x, w, None, name, None, d)
+        assert torch.isfinite(got["dx"]).all()
+        slope = got["dx"][:, 0].cpu().double() / 16
+        exact = ref.activation(x[:, 0].double(), name)[1]
+        exact = torch.where(torch.isfinite(exact), exact, torch.where(x[:, 0] > 0, 1.0, 0.0).double())
+        assert (slope - exact).abs().max() < 2.0 ** -6, name
+        up = torch.cat([w, w])
+        out, z, h = ops.mlp_forward(x.cuda(), up.cuda(), torch.eye(16, dtype=BF16).cuda(), activation=name, keep=True)
+        a, u = ref.activation(x[:, 0].double(), name)[0], x[:, 0].double()
+        fits = (a * u).abs() < 1e38
+        assert ((h[:, 0].cpu().double() - a * u).abs() <= 2.0 ** -7 * (a * u).abs() + 2.0 ** -20 * (u * u).abs() + 1e-37)[fits].all(), name
+
+
+def test_biases_of_32_bits_without_a_weight():
+    x, b, d = normal(1, 600, 96), normal(2, 96, dtype=F32), normal(3, 600, 96)
+    gx, gb = x.cuda().requires_grad_(), b.cuda().requires_grad_()
+    ops.layer_norm(gx, None, gb).backward(d.cuda())
+    want, off = ref.layer_norm(x, None, b, 1e-5, d)
+    assert gb.grad.dtype is F32 and close(gx.grad, want["dx"], off["dx"])
+    assert (gb.grad.cpu().double() - d.double().sum(0)).abs().max() < 608 * 2.0 ** -24 * d.double().abs().sum(0).max()
+
+
+def test_nothing_is_kept_where_no_gradient_is_asked_for():
+    p = {n: t.cuda().requires_grad_() for n, t in block_parameters().items()}
+    x = normal(1, 130, 64).cuda()
+    with torch.no_grad():
+        out = block(x, p)
+    assert not out.requires_grad and same_bits(out, block(x, p).detach())
+
+
+def test_matrices_of_more_than_4_gib():
+    """Rows, columns and halves of matrices whose distances in bytes pass 32 bits."""
+    rows, dim = 70001, 32768
+    x = torch.empty(rows, dim, dtype=BF16, device="cuda").normal_()
+    w, d = normal(1, 16, dim, std=dim ** -0.5).cuda(), normal(2, rows, 16).cuda()
+    out = ops.linear_forward(x, w)
+    dx, dw, db = ops.linear_backward(d, x, w)
+    some = torch.tensor([0, 1, 65535, 65536, rows - 2, rows - 1], device="cuda")
+    want, off = ref.linear(x[some].cpu(), w.cpu(), None, None, None, d[some].cpu())
+    check_all({"out": out[some], "dx": dx[some]}, want, off, "rows")
+    columns = slice(dim - 24, dim)
+    exact = d.double().t() @ x[:, columns].double()
+    spread = d.double().abs().t() @ x[:, columns].double().abs()
+    assert ((dw[:, columns].double() - exact).abs() <= 2.0 ** -8 * exact.abs() + (rows + 8) * 2.0 ** -24 * spread).all()
+    del dx
+    x, d = x.view(2 * rows, dim // 2), torch.empty(2 * rows, dim // 2, dtype=BF16, device="cuda").normal_()
+    out, mean, rstd = ops.layer_norm_forward(x)
+    dx, dw, db = ops.layer_norm_backward(d, x, None, mean, rstd)
+    some = torch.tensor([0, 65536, 131072, 2 * rows - 1], device="cuda")
+    want, off = ref.layer_norm(x[some].cpu(), None, None, 1e-5, d[some].cpu())
+    check_all({"out": out[some], "dx": dx[some]}, want, off, "norm")
+    exact = d[:, -8:].double().sum(0)
+    assert ((db[-8:].double() - exact).abs() <= 2.0 ** -8 * exact.abs() + (2 * rows + 8) * 2.0 ** -24 * d[:, -8:].double().abs().sum(0)).all()
+    del x, d, out, dx
+    # the two projections of a gated part lie more than 4 GiB apart
+    inner = 65600
+    up = torch.empty(2 * inner, dim, dtype=BF16, device="cuda").normal_(std=dim ** -0.5)
+    down = torch.zeros(8, inner, dtype=BF16, device="cuda")
+    for n in (3, 300):
+        x = normal(3, n, dim).cuda()
+        _, _, h = ops.mlp_forward(x, up, down, keep=True)
+        some = torch.tensor([0, 31, 32, 63, 64, 40000, inner - 1], device="cuda")
+        want, off = ref.mlp(x.cpu(), torch.cat([up[some], up[some + inner]]).cpu(), torch.eye(7, dtype=BF16))
+        assert close(h[:, some], want["out"], off["out"])
+    del up, down
+    torch.cuda.empty_cache()
+
+
 # ---- autograd, streams, graphs ------------------------------------------------------------------------------
 
 
