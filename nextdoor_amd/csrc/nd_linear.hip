@@ -28,6 +28,7 @@ constexpr ShapeCost kShapes[4] = {{256, 256, 256, 1.05, 1.5, 1.5, 10.0},
                                   {64, 64, 768, 0.32, 0.4, 0.5, 3.0},
                                   {256, 192, 256, 0.9, 1.2, 1.2, 9.0}};
 constexpr int kMostShares = 128;
+constexpr int64_t kCaches = 32 << 20;  // bytes of the L2 caches of all dies
 constexpr double kJoin = 4.0, kJoinRate = 8e6, kLaunch = 3.0;  // us of adding sums; bytes a us of them, written and read again; us of a launch
 
 double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
@@ -153,6 +154,8 @@ struct Call {
     }
     LinearParams p = a;
     p.sums = sums;
+    // (what the caches do not hold until the backward pass: 8192 x 2 x 5632 at 3 bytes, 368 us and 346; 3001 x 2 x 1000, both passes, 87 and 89)
+    p.z_later = a.z && (int64_t)a.m * a.n * (after == After::kGated ? 6 : 2) > kCaches;
     const LinearPlan plan = plan_of({a.m, a.n, a.k, after});
     note(bf16 ? launch_linear<__bf16>(p, Layout::kRows, after, plan, stream) : launch_linear<_Float16>(p, Layout::kRows, after, plan, stream));
   }

@@ -32,6 +32,7 @@ struct LinearParams {
   int64_t residual_bytes;  // of a row
   void* out;
   void* z;  // forward: written unless null; backward: read.  [m][n]; gated: rows of 6 n bytes, see Upper24
+  bool z_later;  // forward: z is written past the caches
   // float16: what dz is held times.  parts: the largest finite |dout| of workgroups, null: 1.  Who makes dz finds the scale in them and
   // leaves one over it in *unscale, with which the sums of kPlain are multiplied (null: 1).
   const float* parts;
@@ -266,6 +267,10 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
       for (int e = 0; e < 4; ++e) v[4 * q + e] += x[e];
     }
   };
+  auto put_z = [&](const auto& region, void* to, auto... where) {
+    if (a.z_later) region.template put<true>(to, where...);
+    else region.put(to, where...);
+  };
   auto values = [](const f32x16& c, float(&v)[16]) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = c[e];
@@ -305,9 +310,9 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
         write(products, i, g);
       }
       if (a.z) {
-        gates.put(a.z, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
-        others.put((char*)a.z + n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
-        next.put((char*)a.z + 2 * n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        put_z(gates, a.z, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        put_z(others, (char*)a.z + n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
+        put_z(next, (char*)a.z + 2 * n_bytes, 3 * n_bytes, at, a.m, wave_column0, a.n, lane);
       }
       products.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
     }
@@ -455,7 +460,7 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
         }
         write(first, i, v);
       }
-      if (keep) second.put(a.z, n_bytes, at, a.m, wave_column0, a.n, lane);
+      if (keep) put_z(second, a.z, n_bytes, at, a.m, wave_column0, a.n, lane);
       first.put(a.out, n_bytes, at, a.m, wave_column0, a.n, lane);
     }
   }

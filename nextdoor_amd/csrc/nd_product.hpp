@@ -260,14 +260,20 @@ struct Region {
       load_to_lds(base, (uint32_t)(min(r, row_end - 1 - row0) * row_bytes) + (there ? c * 16 : 0), lds + t * 1024);
     }
   }
+  // LATER: written past the caches, for what is read by another kernel and after much else (z for the backward pass: kept in the
+  // caches it drives out the operands of the tiles that are being made).
+  template <bool LATER = false>
   __device__ __forceinline__ void put(void* matrix, int64_t row_bytes, int row0, int row_end, int column0, int column_end, int lane) const {
     asm volatile("" ::: "memory");  // (what other lanes wrote is read: LDS serves a wave in order)
 #pragma unroll
     for (int t = 0; t < kTurns; ++t) {
       const int p = t * 64 + lane, r = p / kRow, c = p % kRow;
       const u32x4 v = at[r * kRow + (c ^ (r & (kRow - 1)))];
-      if (row0 + r < row_end && c < CHUNKS && column0 + c * 8 < column_end)
-        *(u32x4*)((char*)matrix + (row0 + r) * row_bytes + (int64_t)(column0 + c * 8) * 2) = v;
+      if (row0 + r < row_end && c < CHUNKS && column0 + c * 8 < column_end) {
+        u32x4* to = (u32x4*)((char*)matrix + (row0 + r) * row_bytes + (int64_t)(column0 + c * 8) * 2);
+        if (LATER) __builtin_nontemporal_store(v, to);
+        else *to = v;
+      }
     }
     asm volatile("" ::: "memory");
   }
