@@ -29,6 +29,7 @@ struct NormParams {
   void* out;  // backward: dx, or null
   float *mean, *rstd;
   float* sums;  // [workgroup][2][dim], or null
+  void *dweight, *dbias;  // where there is one workgroup: written here, each unless it is null
   int64_t rows;
   int32_t dim;
   int32_t weight_32;
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
       }
     }
   }
-  if (!p.sums) return;
+  if (!p.sums && !p.dweight && !p.dbias) return;
   // The groups' sums: half of them leave theirs in LDS, the other half adds them, until one is left.
   __shared__ float part[kGroups > 1 ? kGroups / 2 : 1][2][kGroups > 1 ? LANES * VALUES : 1];
 #pragma unroll
@@ -250,13 +251,22 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
     }
   }
   if (group > 0) return;
-  float* sums = p.sums + (int64_t)blockIdx.x * 2 * p.dim;
+  auto put = [&](void* to, int c, float v) {
+    if (!to) return;
+    if (p.weight_32) ((float*)to)[c] = v;
+    else ((T*)to)[c] = (T)v;
+  };
 #pragma unroll
   for (int i = 0; i < VALUES; ++i) {
     const int c = Row::column(i, lane);
-    if (c < p.dim) {
+    if (c >= p.dim) continue;
+    if (p.sums) {
+      float* sums = p.sums + (int64_t)blockIdx.x * 2 * p.dim;
       sums[c] = dw[i];
       sums[p.dim + c] = db[i];
+    } else {
+      put(p.dweight, c, dw[i]);
+      put(p.dbias, c, db[i]);
     }
   }
 }
@@ -269,6 +279,7 @@ struct NormShape {
 };
 constexpr NormShape kNormShapes[] = {{128, 16, 64}, {512, 64, 16}, {1024, 128, 8}, {2048, 256, 4}, {4096, 512, 2}, {8192, 1024, 1}, {16384, 1024, 1}};
 constexpr int kForwardLanes = 1 << 19, kBackwardBlocks = 256;
+constexpr int kAlone = 6;  // times at most that one workgroup takes the next rows: less than another launch, which adds up sums, costs
 int shape_of(int32_t dim) {
   int i = 0;
   while (dim > kNormShapes[i].most) ++i;
@@ -276,6 +287,7 @@ int shape_of(int32_t dim) {
 }
 int64_t backward_blocks(int64_t rows, int32_t dim) {
   const int at_once = kNormShapes[shape_of(dim)].rows;
+  if (rows <= kAlone * at_once) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(kBackwardBlocks, (rows + at_once - 1) / at_once));
 }
 
@@ -309,7 +321,8 @@ void launch_norm(const NormParams& p, bool backward, hipStream_t stream) {
 }
 
 int64_t norm_workspace(const nd_layer_norm* a) {
-  return a->dweight || a->dbias ? backward_blocks(a->rows, a->dim) * 2 * a->dim * 4 : 0;
+  const int64_t blocks = backward_blocks(a->rows, a->dim);
+  return (a->dweight || a->dbias) && blocks > 1 ? blocks * 2 * a->dim * 4 : 0;
 }
 
 std::string refuse(const nd_layer_norm* a) {
@@ -346,12 +359,12 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
     if (x.needed && !x.at) return fail("layer norm: null array");
     if ((uintptr_t)x.at % x.size) return fail("layer norm: arrays are aligned as their elements are");
   }
-  const bool sums = backward && (a->dweight || a->dbias);
-  if (sums && (a->workspace_bytes < norm_workspace(a) || !a->workspace || ((uintptr_t)a->workspace & 15)))
-    return fail("layer norm: the workspace has " + std::to_string(a->workspace ? a->workspace_bytes : 0) + " bytes, " +
-                std::to_string(norm_workspace(a)) + " needed, aligned to 16");
-  if (backward ? !a->dx && !sums : !some) return 0;
-  if (!some && !sums) return 0;
+  const bool weights = backward && (a->dweight || a->dbias);
+  const int64_t room = backward ? norm_workspace(a) : 0;
+  if (room > 0 && (a->workspace_bytes < room || !a->workspace || ((uintptr_t)a->workspace & 15)))
+    return fail("layer norm: the workspace has " + std::to_string(a->workspace ? a->workspace_bytes : 0) + " bytes, " + std::to_string(room) +
+                " needed, aligned to 16");
+  if (!weights && (!some || (backward && !a->dx))) return 0;
   NormParams p = {};
   p.x = (const char*)a->x;
   p.x_bytes = a->x_row * size;
@@ -362,7 +375,9 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
   p.out = backward ? a->dx : a->out;
   p.mean = a->mean;
   p.rstd = a->rstd;
-  p.sums = sums ? (float*)a->workspace : nullptr;
+  p.sums = room > 0 ? (float*)a->workspace : nullptr;
+  p.dweight = backward ? a->dweight : nullptr;
+  p.dbias = backward ? a->dbias : nullptr;
   p.rows = a->rows;
   p.dim = a->dim;
   p.weight_32 = a->weight_dtype == ND_F32;
@@ -371,7 +386,7 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
   else if (a->dtype == ND_F16) launch_norm<_Float16>(p, backward, (hipStream_t)stream);
   else launch_norm<__bf16>(p, backward, (hipStream_t)stream);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && sums) {
+  if (e == hipSuccess && p.sums) {
     const int64_t blocks = backward_blocks(a->rows, a->dim), columns = 2 * a->dim;
     const hipStream_t s = (hipStream_t)stream;
     if (a->weight_dtype == ND_F32) e = column_join<float>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);

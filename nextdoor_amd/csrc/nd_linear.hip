@@ -28,6 +28,7 @@ constexpr ShapeCost kShapes[4] = {{256, 256, 256, 1.05, 1.5, 1.5, 10.0},
                                   {64, 64, 768, 0.32, 0.4, 0.5, 3.0},
                                   {256, 192, 256, 0.9, 1.2, 1.2, 9.0}};
 constexpr int kMostShares = 128;
+constexpr int64_t kRowsAlone = 256;     // whose sums one workgroup makes: less than another launch, which adds up shares, costs
 constexpr int64_t kCaches = 32 << 20;  // bytes of the L2 caches of all dies
 constexpr double kJoin = 4.0, kJoinRate = 8e6, kLaunch = 3.0;  // us of adding sums; bytes a us of them, written and read again; us of a launch
 
@@ -118,8 +119,10 @@ TwoPlans plan_two(const Task* a, const Task* b) {  // null: not wanted
 
 int64_t sums_bytes(const LinearPlan& p, int64_t m, int64_t columns) { return p.shares > 1 ? m * columns * 4 * p.shares : 0; }
 
-// Shares of the rows for the sums over them: workgroups of 64 columns, at least 64 rows to each, some thousand in all.
+// Shares of the rows for the sums over them: one where there are few, else workgroups of 64 columns, at least 64 rows to each, some
+// thousand in all.
 int64_t row_shares(int64_t rows, int64_t columns) {
+  if (rows <= kRowsAlone) return 1;
   const int64_t across = (columns + 63) / 64;
   return std::max<int64_t>(1, std::min<int64_t>({(rows + 63) / 64, std::max<int64_t>(1, 2048 / across), (int64_t)65535}));
 }
@@ -186,18 +189,20 @@ struct Call {
   void one(const LinearParams& a, Layout layout, After after, const LinearPlan& plan) {
     note(bf16 ? launch_linear<__bf16>(a, layout, after, plan, stream) : launch_linear<_Float16>(a, layout, after, plan, stream));
   }
-  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts) {
-    note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, sums, shares, parts, stream)
-              : launch_slope<_Float16>(a, dout, dout_bytes, sums, shares, parts, stream));
+  // dz and what is beside it; `total` gets the sums of the rows, unless it is null.
+  void slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, void* total, int64_t shares, float* parts) {
+    float* parted = total && shares > 1 ? sums : nullptr;
+    void* whole = shares > 1 ? nullptr : total;
+    note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, parted, whole, shares, parts, stream)
+              : launch_slope<_Float16>(a, dout, dout_bytes, parted, whole, shares, parts, stream));
+    if (parted) join(sums, shares, a.n, nullptr, total);
   }
   // Of dout [rows][columns]: the sums of its rows, unless out is null, and the largest of its values, unless parts is.
   void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts) {
     LinearParams p = {};
     p.m = (int32_t)rows;
     p.n = columns;
-    const int64_t shares = survey_shares(rows, columns, parts);
-    slope(p, dout, row_bytes, out ? sums : nullptr, shares, parts);
-    if (out) join(sums, shares, columns, nullptr, out);
+    slope(p, dout, row_bytes, sums, out, survey_shares(rows, columns, parts), parts);
   }
   int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
 };
@@ -354,8 +359,7 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
     p.activation = a->activation;
     p.z = a->z;
     p.out = work + w.dz;
-    call.slope(p, a->dout, dz_bytes, a->dbias ? rows : nullptr, row_shares(a->rows, a->out_dim), nullptr);
-    if (a->dbias) call.join(rows, row_shares(a->rows, a->out_dim), a->out_dim, nullptr, a->dbias);
+    call.slope(p, a->dout, dz_bytes, rows, a->dbias, row_shares(a->rows, a->out_dim), nullptr);
     dz = work + w.dz;
     dz_bytes = (int64_t)a->out_dim * 2;
   } else if (a->dbias) {

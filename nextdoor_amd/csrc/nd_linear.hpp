@@ -615,10 +615,10 @@ template <class T>
 hipError_t launch_joins(const Joins& joins, uint32_t blocks, hipStream_t stream);
 template <class T>
 hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
-// dz = dout a'(z), held times its scale, if there is a z, and unless they are null sums of its rows (times 1), and the largest
-// finite |dout| of each workgroup.
+// dz = dout a'(z), held times its scale, if there is a z, and unless they are null sums of its rows (times 1; with one share
+// to `total`, rounded), and the largest finite |dout| of each workgroup.
 template <class T>
-hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, int64_t shares, float* parts, hipStream_t stream);
+hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, void* total, int64_t shares, float* parts, hipStream_t stream);
 constexpr int kSlopeColumns = 64;  // of a workgroup there
 
 constexpr int kFewRows = 64;  // at most: a kernel of its own, which reads the weights once and keeps a sum in many waves

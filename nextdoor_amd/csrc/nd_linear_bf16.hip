@@ -6,5 +6,5 @@ template hipError_t launch_linear<__bf16>(const LinearParams&, Layout, After, co
 template hipError_t launch_pair<__bf16>(const LinearParams&, After, const LinearPlan&, const LinearParams&, const LinearPlan&, hipStream_t);
 template hipError_t launch_joins<__bf16>(const Joins&, uint32_t, hipStream_t);
 template hipError_t launch_few_rows<__bf16>(const LinearParams&, After, hipStream_t);
-template hipError_t launch_slope<__bf16>(const LinearParams&, const void*, int64_t, float*, int64_t, float*, hipStream_t);
+template hipError_t launch_slope<__bf16>(const LinearParams&, const void*, int64_t, float*, void*, int64_t, float*, hipStream_t);
 }  // namespace nd

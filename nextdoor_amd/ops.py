@@ -67,11 +67,12 @@ def _on_gpu(what, first, *others):
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream wraps in an object
+_current_device = torch._C._cuda_getDevice  # torch.cuda.current_device without the check for a first use: there is a tensor
 
 
 def _run(index, fn, *args):
     """Calls an entry point that takes a stream last, on torch's current one, with the device current."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -401,19 +402,23 @@ def _rows_in_place(x, dim, multiple):
     return x, step
 
 
-def _norm(x, weight, bias, eps, others=()):
+def _norm(x, weight, bias, eps, *others):
     """Checked arguments: (device index, x as rows, the struct's first fields, weight, bias)."""
-    index = _on_gpu("layer norm", x, *(t for t in (weight, bias, *others) if t is not None))
+    given = [x, *others]
+    if weight is not None:
+        given.append(weight)
+    if bias is not None:
+        given.append(bias)
+    index = _on_gpu("layer norm", *given)
     dtype = x.dtype
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise NextDoorError("layer norm: no kernel for %s" % dtype)
     if x.dim() == 0:
         raise NextDoorError("layer norm: x has no rows")
     dim = x.shape[-1]
     weight_dtype = dtype
-    for t in (weight, bias):
-        if t is None:
-            continue
+    for t in given[1 + len(others):]:
         if t.shape != (dim,):
             raise NextDoorError("layer norm: weight or bias is not [%d]" % dim)
         weight_dtype = t.dtype
@@ -427,7 +432,7 @@ def _norm(x, weight, bias, eps, others=()):
         raise NextDoorError("layer norm: rows of 1 to 16384 values, %d given" % dim)
     x, x_row = _rows_in_place(x, dim, 1)
     weight, bias = None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous()
-    return index, x, (x.shape[0], dim, _DTYPES[dtype], _DTYPES[weight_dtype], eps), x_row, weight, bias
+    return index, x, (x.shape[0], dim, code, _DTYPES[weight_dtype], eps), x_row, weight, bias
 
 
 def _pointer(t):
@@ -452,24 +457,24 @@ def layer_norm_backward(dout, x, weight, mean, rstd, needs=(True, True, True), d
     """(dx, dweight, dbias) for the gradient ``dout`` of ``out``; mean and rstd are the forward pass's, ``weight`` None if there was
     none.  dweight and dbias are of the type of weight; without one of ``dtype``, that of x or float32, by default that of x.
     ``needs``: which to compute; the others are None."""
-    index, rows, fields, x_row, weight, _ = _norm(x, weight, None, 0.0, (dout, mean, rstd))
+    index, rows, fields, x_row, weight, _ = _norm(x, weight, None, 0.0, dout, mean, rstd)
     if weight is None and dtype is not None:
         if dtype is not x.dtype and dtype is not torch.float32:
             raise NextDoorError("layer norm: gradients of the type of x or float32, not %s" % dtype)
         fields = (*fields[:3], _DTYPES[dtype], fields[4])
     if dout.shape != x.shape or dout.dtype is not x.dtype:
         raise NextDoorError("layer norm: dout is of another shape or type than x")
-    for t in (mean, rstd):
-        if not (t.shape == (fields[0],) and t.dtype is torch.float32 and t.is_contiguous()):
-            raise NextDoorError("layer norm: mean and rstd are not a forward pass's")
+    if not (mean.shape == rstd.shape == (fields[0],) and mean.dtype is rstd.dtype is torch.float32 and
+            mean.is_contiguous() and rstd.is_contiguous()):
+        raise NextDoorError("layer norm: mean and rstd are not a forward pass's")
     dout, dout_row = _rows_in_place(dout, fields[1], 1)
     kind = weight.dtype if weight is not None else x.dtype if dtype is None else dtype
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if needs[0] else None
-    dweight = torch.empty(fields[1], dtype=kind, device=x.device) if needs[1] else None
-    dbias = torch.empty(fields[1], dtype=kind, device=x.device) if needs[2] else None
+    dweight = mean.new_empty(fields[1], dtype=kind) if needs[1] else None
+    dbias = mean.new_empty(fields[1], dtype=kind) if needs[2] else None
     a = LayerNorm(*fields, x_row, dout_row, rows.data_ptr(), _pointer(weight), None, None, mean.data_ptr(), rstd.data_ptr(),
                   dout.data_ptr(), _pointer(dx), _pointer(dweight), _pointer(dbias))
-    workspace = _room(a, _library().nd_layer_norm_workspace(a), x.device)
+    workspace = _room(a, _library().nd_layer_norm_workspace(a), mean.device) if needs[1] or needs[2] else None
     _run(index, _library().nd_layer_norm_backward, a)
     del workspace
     return dx, dweight, dbias

@@ -55,15 +55,15 @@ def test_norm_calls_with_nothing_to_do_or_no_room():
     lib = _capi.lib()
     refused(lib.nd_layer_norm_forward, norm_call(out=None), "null")
     refused(lib.nd_layer_norm_backward, norm_call(dout=None), "null")
-    refused(lib.nd_layer_norm_backward, norm_call(workspace_bytes=16), "workspace")
-    refused(lib.nd_layer_norm_backward, norm_call(workspace=None), "workspace")
-    refused(lib.nd_layer_norm_backward, norm_call(workspace=BASE + 8), "workspace")
+    for changes in (dict(workspace_bytes=16), dict(workspace=None), dict(workspace=BASE + 8)):
+        refused(lib.nd_layer_norm_backward, norm_call(rows=1000, **changes), "workspace")
     refused(lib.nd_layer_norm_backward, norm_call(dx=BASE + 1), "aligned")
     assert lib.nd_layer_norm_forward(norm_call(rows=0, x=None, out=None), None) == 0
     assert lib.nd_layer_norm_backward(norm_call(dx=None, dweight=None, dbias=None), None) == 0
     assert lib.nd_layer_norm_backward(norm_call(rows=0, x=None, dout=None, dweight=None, dbias=None), None) == 0
     assert lib.nd_layer_norm_workspace(norm_call(dim=0)) == -1 and lib.nd_layer_norm_workspace(None) == -1
-    assert lib.nd_layer_norm_workspace(norm_call(dweight=None, dbias=None)) == 0 < lib.nd_layer_norm_workspace(norm_call(dbias=None))
+    room = [lib.nd_layer_norm_workspace(norm_call(rows=1000, **c)) for c in (dict(dweight=None, dbias=None), dict(dbias=None), {})]
+    assert room[0] == 0 < room[1] == room[2] and lib.nd_layer_norm_workspace(norm_call()) == 0  # (one workgroup needs none)
 
 
 COMMON = [(dict(dtype=0), "16-bit"), (dict(rows=-1), "rows"), (dict(rows=1 << 31), "rows"), (dict(dim=12), "multiples of 8"),
