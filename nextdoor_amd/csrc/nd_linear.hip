@@ -30,7 +30,8 @@ constexpr ShapeCost kShapes[4] = {{256, 256, 256, 1.05, 1.5, 1.5, 10.0},
 constexpr int kMostShares = 128;
 constexpr int64_t kRowsAlone = 256;     // whose sums one workgroup makes: less than another launch, which adds up shares, costs
 constexpr int64_t kCaches = 32 << 20;  // bytes of the L2 caches of all dies
-constexpr double kJoin = 4.0, kJoinRate = 8e6, kLaunch = 3.0;  // us of adding sums; bytes a us of them, written and read again; us of a launch
+// us of adding sums: a launch in a forward pass, a part of one in a backward pass; bytes a us of them, written and read again; us of a launch
+constexpr double kJoin = 4.0, kJoinPart = 2.0, kJoinRate = 8e6, kLaunch = 3.0;
 
 double time_of(const ShapeCost& c, int64_t groups, int64_t rounds) {
   const int64_t full = groups / c.at_once, rest = groups % c.at_once;
@@ -62,7 +63,7 @@ void shares_of(const Task& t, const ShapeCost& c, Shares& s) {
     s.shares[s.n] = want;
     s.groups[s.n] = tiles * want;
     s.rounds[s.n] = each;
-    s.joined[s.n++] = want > 1 ? kJoin + (double)want * t.m * columns * 8 / kJoinRate : 0;
+    s.joined[s.n++] = want > 1 ? (t.after == After::kPlain ? kJoinPart : kJoin) + (double)want * t.m * columns * 8 / kJoinRate : 0;
   }
 }
 struct Estimate {

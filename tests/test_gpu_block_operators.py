@@ -460,6 +460,66 @@ def test_matrices_of_more_than_4_gib():
     torch.cuda.empty_cache()
 
 
+# ---- every kind of tile ----------------------------------------------------------------------------------------
+# Sizes for which the rules take each of the four shapes of tiles, with whole sums and with shares of them, in the forward
+# pass, for dx and for dweight (alone: both together go into one launch).  References in 64 bits on the GPU.
+
+LINEAR_TILES = [(958, 528, 16008), (135, 13032, 15600), (2581, 3480, 8), (65, 976, 8), (13553, 136, 544), (5684, 11280, 136),
+                (958, 16008, 528), (5684, 136, 11280), (517, 1160, 12712), (12017, 15928, 136), (3479, 8, 2584), (129, 536, 13296),
+                (10768, 136, 5808)]
+
+
+@pytest.mark.parametrize("rows,dim,out", LINEAR_TILES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_with_every_shape_of_tile(rows, dim, out, dtype):
+    print("tiles", rows, dim, out, dtype, flush=True)
+    x, w, b, name, r, d = map_cuda(linear_case(rows, dim, out, dtype, "silu", residual=True))
+    want, off = ref.linear(x, w, b, name, r, d)
+    y, z = ops.linear_forward(x, w, b, name, r, keep=True)
+    dx, _, _ = ops.linear_backward(d, x, w, z, name, False, (True, False))
+    _, dw, db = ops.linear_backward(d, x, w, z, name, True, (False, True))
+    both = ops.linear_backward(d, x, w, z, name)
+    for i, got in enumerate(({"out": y, "dx": dx, "dweight": dw, "dbias": db}, dict(zip(("dx", "dweight", "dbias"), both)))):
+        for n, t in got.items():
+            assert within(t, want[n], off[n]), (i, n)
+
+
+MLP_TILES = [(391, 848, 8400, 64), (133, 7072, 9264, 64), (7122, 9576, 72, 8), (2581, 3480, 8, 8), (65, 976, 8, 8), (655, 136, 10992, 800),
+             (6400, 136, 448, 152), (20483, 64, 256, 64)]
+
+
+@pytest.mark.parametrize("rows,dim,inner,out", MLP_TILES)
+@pytest.mark.parametrize("gated,dtype", [(True, BF16), (True, F16), (False, BF16)])
+def test_mlp_with_every_shape_of_tile(rows, dim, inner, out, gated, dtype):
+    print("tiles", rows, dim, inner, out, gated, dtype, flush=True)
+    case = map_cuda(mlp_case(rows, dim, inner, out, dtype, "silu", gated))
+    x, up, down, up_bias, down_bias, name, _, r, d = case
+    want, off = ref.mlp(*case)
+    y, z, h = ops.mlp_forward(x, up, down, up_bias, down_bias, name, gated, r, keep=True)
+    names = ("dx", "dup", "ddown", "dup_bias", "ddown_bias")
+    everything = dict(zip(names, ops.mlp_backward(d, x, up, down, z, h, name, gated)))
+    alone = dict(zip(names, ops.mlp_backward(d, x, up, down, z, h, name, gated, True, False, (True, False, False))))
+    for i, got in enumerate(({"out": y, **everything}, {n: alone[n] for n in ("dx", "dup_bias")})):
+        for n, t in got.items():
+            assert within(t, want[n], off[n]), (i, n)
+
+
+def map_cuda(case):
+    return [t.cuda() if isinstance(t, torch.Tensor) else t for t in case]
+
+
+def within(got, right, off):
+    value = got.double()
+    if got.dtype is F16:
+        value = torch.where(torch.isinf(value) & (right.abs() + off >= 65520) & (value.sign() == right.sign()), right, value)
+    wrong = ((value - right).abs() > off) | torch.isnan(value)
+    if wrong.any():
+        at = tuple(int(i) for i in wrong.nonzero()[0])
+        print("%d of %d off; first at %s: %r, should be %r within %r" % (int(wrong.sum()), wrong.numel(), at, float(value[at]), float(right[at]),
+                                                                      float(off[at])))
+    return not wrong.any()
+
+
 # ---- autograd, streams, graphs ------------------------------------------------------------------------------
 
 
