@@ -47,7 +47,7 @@ __device__ __forceinline__ void activate(int activation, float (&x)[N]) {
   }
 }
 
-// x becomes a(x), slope a'(x).
+// x becomes a(x), slope a'(x), which is 0 or 1 where a is flat to 32 bits: x may be infinite there, as what a 16-bit float does not hold.
 template <int N>
 __device__ __forceinline__ void activate_with_slope(int activation, float (&x)[N], float (&slope)[N]) {
   if (activation == ND_RELU) {
@@ -59,23 +59,23 @@ __device__ __forceinline__ void activate_with_slope(int activation, float (&x)[N
   } else if (activation == ND_GELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float integral = normal_integral(x[i]);
-      slope[i] = __builtin_fmaf(x[i], normal_density(x[i]), integral);
+      const float integral = normal_integral(x[i]), density = normal_density(x[i]);
+      slope[i] = density == 0.f ? integral : __builtin_fmaf(x[i], density, integral);
       x[i] *= integral;
     }
   } else if (activation == ND_GELU_TANH) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float square = kTanhCube * x[i] * x[i], s = logistic(2.f * kTanhInside * x[i] * (1.f + square));
-      const float flat = s * (1.f - s);  // (0 where the square may be infinite)
+      const float flat = s * (1.f - s);
       slope[i] = flat == 0.f ? s : __builtin_fmaf(2.f * kTanhInside * x[i] * flat, __builtin_fmaf(3.f, square, 1.f), s);
       x[i] *= s;
     }
   } else if (activation == ND_SILU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float s = logistic(x[i]);
-      slope[i] = s * __builtin_fmaf(x[i], 1.f - s, 1.f);
+      const float s = logistic(x[i]), flat = s * (1.f - s);
+      slope[i] = flat == 0.f ? s : __builtin_fmaf(x[i], flat, s);
       x[i] *= s;
     }
   } else {

@@ -462,7 +462,7 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     return call.done();
   }
   const int64_t dout_bytes = a->dout_row * 2;
-  float* parts = first && !call.bf16 ? (float*)(work + w.parts) : nullptr;
+  float* parts = first && some && !call.bf16 ? (float*)(work + w.parts) : nullptr;  // (without rows nobody leaves an unscale)
   float* unscale = parts ? (float*)(work + w.unscale) : nullptr;
   if (a->ddown_bias || parts) call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, parts);
   float* columns = a->dup_bias ? (float*)(work + w.columns) : nullptr;

@@ -612,6 +612,8 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep=Fa
     workspace = _room(a, _library().nd_linear_workspace(a, 0), x.device)
     _run(index, _library().nd_linear_forward, a)
     del workspace
+    if z is not None and wide > out_dim:
+        z[:, out_dim:].zero_()  # (0 times a place of x that is not finite)
     out = _shaped(out, n, out_dim, shape)
     return (out, z) if keep else out
 
@@ -709,7 +711,8 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
 
     z = x up^T + up_bias; gated: ``h = activation(g) u`` with ``g, u = z.chunk(2, -1)``, else ``h = activation(z)``.  x: [..., dim];
     up: [2 inner or inner, dim]; down: [out_dim, inner]; activations, types and sizes as in :func:`linear_forward`.  Both
-    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second."""
+    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second.  Where inner is no
+multiple of 8, a row of x with infinities gives NaN."""
     index = _on_gpu("mlp", x, up, down, *(t for t in (up_bias, down_bias, residual) if t is not None))
     _types("mlp", x, up, down, up_bias, down_bias, residual)
     gated = bool(gated)
@@ -734,6 +737,8 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
     workspace = _room(a, _library().nd_mlp_workspace(a, 0), x.device)
     _run(index, _library().nd_mlp_forward, a)
     del workspace
+    if z is not None and inner % 8:  # (as in linear_forward; gated: the upper 16 bits of both halves)
+        (z.view(torch.int16).view(n, 3, up.shape[0] // 2)[:, :2, inner:] if gated else z[:, inner:]).zero_()
     out = _shaped(out, n, out_dim, shape)
     return (out, z, h) if keep else out
 

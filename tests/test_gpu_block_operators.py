@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from nextdoor_amd import ops
+from nextdoor_amd import _capi, ops
 from tests import block_operators_reference as ref
 from tests.operators_reference import close
 
@@ -403,6 +403,62 @@ def test_slopes_of_pre_activations_of_any_size():
         a, u = ref.activation(x[:, 0].double(), name)[0], x[:, 0].double()
         fits = (a * u).abs() < 1e38
         assert ((h[:, 0].cpu().double() - a * u).abs() <= 2.0 ** -7 * (a * u).abs() + 2.0 ** -20 * (u * u).abs() + 1e-37)[fits].all(), name
+
+
+@pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("out", [16, 13])
+def test_slopes_where_16_bit_floats_do_not_hold_z(name, out):
+    """z is 4 x 30000 and 4 x -30000, which float16 keeps as infinities: the slopes there are 1 and 0."""
+    x, w = torch.zeros(70, 64), torch.zeros(out, 64)
+    x[:35, 0], x[35:, 0], w[:, 0] = 30000, -30000, 4
+    x, w, d = x.to(F16).cuda(), w.to(F16).cuda(), torch.full((70, out), 0.5, dtype=F16).cuda()
+    z = ops.linear_forward(x, w, None, name, keep=True)[1]
+    dx, dw, db = ops.linear_backward(d, x, w, z, name)
+    # sums of `out` products 0.5 x 4 x slope, and of 35 of them; every one is a 16-bit float
+    assert dx[:35, 0].tolist() == [2.0 * out] * 35 and dx[35:].abs().max() == 0 and db.tolist() == [17.5] * out
+    # h = z of 0 or more than float16 holds; the second matrix is 0, so is what comes back to z
+    got = ops.mlp_forward(x, w, torch.zeros(8, out, dtype=F16).cuda(), activation=name, gated=False, keep=True)[1]
+    dx = ops.mlp_backward(torch.ones(70, 8, dtype=F16).cuda(), x, w, torch.zeros(8, out, dtype=F16).cuda(), got,
+                          torch.zeros(70, out + -out % 8, dtype=F16).cuda(), name, False)[0]
+    assert dx.abs().max() == 0
+
+
+def test_rows_with_infinities_where_sizes_are_no_multiples_of_8():
+    """Slopes of a relu are 0 or 1 whatever z is, so gradients of a row of x with an infinity are the formulas' and not NaN."""
+    x, w = normal(1, 100, 64), normal(2, 13, 64)
+    d = normal(3, 100, 13)
+    x[7, 3] = math.inf
+    z = ops.linear_forward(x.cuda(), w.cuda(), None, "relu", keep=True)[1]
+    dx = ops.linear_backward(d.cuda(), x.cuda(), w.cuda(), z, "relu")[0].cpu()
+    slope = (x.double() @ w.double().T > 0).double()
+    want = (d.double() * slope) @ w.double()
+    # 13 products, and the rounding of the result
+    assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -19 * ((d.double() * slope).abs() @ w.double().abs())).all()
+    down = normal(4, 24, 13)
+    e = normal(5, 100, 24)
+    z, h = ops.mlp_forward(x.cuda(), w.cuda(), down.cuda(), activation="relu", gated=False, keep=True)[1:]
+    dx = ops.mlp_backward(e.cuda(), x.cuda(), w.cuda(), down.cuda(), z, h, "relu", False)[0].cpu()
+    dz = (e.double() @ down.double()) * slope
+    want, spread = dz @ w.double(), dz.abs() @ w.double().abs()
+    # dz is rounded, 2^-8 (1 + 2^-8), and is a sum of 24 products, of which slopes leave all or nothing; then as above
+    off = 2.0 ** -7.9 * spread + 2.0 ** -18 * ((e.double().abs() @ down.double().abs()) * slope) @ w.double().abs()
+    assert ((dx.double() - want).abs() <= 2.0 ** -8 * want.abs() + off).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gradients_of_no_rows_are_0_whatever_the_workspace_held(dtype):
+    none, up, down = torch.empty(0, 64, dtype=dtype).cuda(), normal(1, 512, 64, dtype=dtype).cuda(), normal(2, 64, 256, dtype=dtype).cuda()
+    z, h = torch.empty(0, 3 * 512, dtype=torch.uint8).cuda(), torch.empty(0, 256, dtype=dtype).cuda()
+    got = [torch.full(shape, math.nan, dtype=dtype).cuda() for shape in ((512, 64), (512,), (64, 256), (64,))]
+    a = _capi.Mlp(0, 64, 256, 64, ops._DTYPES[dtype], 4, 1, 64, 0, 64, None, up.data_ptr(), None, down.data_ptr(), None, None, None, None, None, None, None,
+                  *(t.data_ptr() for t in got))
+    size = _capi.lib().nd_mlp_workspace(a, 1)
+    workspace = torch.full((max(size, 16),), 255, dtype=torch.uint8).cuda()
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    ops._run(torch.cuda.current_device(), ops._library().nd_mlp_backward, a)
+    torch.cuda.synchronize()
+    assert all((t == 0).all() for t in got)
+    assert all((t == 0).all() for t in ops.mlp_backward(none, none, up, down, z, h)[1:])
 
 
 def test_biases_of_32_bits_without_a_weight():
