@@ -70,15 +70,37 @@ struct Estimate {
   LinearPlan plan;
   double time;
 };
+// Columns of a pair's two halves alternate by 32, and a slope is read for 64 at a time: neither divides a wave's part of a narrow tile.
+bool makes(int shape, After after) { return shape != 3 || (after != After::kGated && after != After::kSlope); }
 Estimate estimate(const Task& t) {
   Estimate best = {{}, INFINITY};
   for (int shape = 0; shape < 4; ++shape) {
     Shares s;
     shares_of(t, kShapes[shape], s);
     for (int i = 0; i < s.n; ++i) {
-      if (shape == 3 && s.shares[i] == 1 && (t.after == After::kGated || t.after == After::kSlope)) continue;  // (columns in pairs of 32)
+      if (s.shares[i] == 1 && !makes(shape, t.after)) continue;
       const double time = time_of(kShapes[shape], s.groups[i], s.rounds[i]) + s.joined[i];
       if (time < best.time) best = {{shape, s.shares[i], (int)s.rounds[i] * 64}, time};
+    }
+  }
+  // Large tiles for as many rows as they fill whole turns of the compute units with, another shape for the rows behind those, where
+  // that is estimated to take a sixteenth less (what the estimate is off by; 9000 x 2000 -> 2048: 91 us for 112, its gradient of x 77 for
+  // 89; 20000 x 4096 -> 1024: 148 for 155; 8192 x 2048 x 11264 by columns, estimated at 303 for 321: no difference).
+  const ShapeCost& large = kShapes[0];
+  const int64_t rounds = std::max<int64_t>(1, (t.k + 63) / 64), columns = t.after == After::kGated ? 2 * t.n : t.n;
+  const int64_t across = (columns + large.n - 1) / large.n, down = (t.m + large.m - 1) / large.m, turns = across * down / large.at_once;
+  if (turns == 0 || turns * large.at_once == across * down || t.after == After::kSlope) return best;
+  const int64_t rows = turns * large.at_once / across * large.m;
+  if (rows == 0) return best;
+  const double first = time_of(large, rows / large.m * across, rounds) + kLaunch;
+  double least = best.time * 15 / 16;
+  for (int shape = 1; shape < 4; ++shape) {
+    if (!makes(shape, t.after)) continue;
+    const ShapeCost& c = kShapes[shape];
+    const double time = first + time_of(c, ((t.m - rows + c.m - 1) / c.m) * ((columns + c.n - 1) / c.n), rounds);
+    if (time < least) {
+      least = time;
+      best = {{0, 1, (int)rounds * 64, (int)rows, shape}, time};
     }
   }
   return best;

@@ -604,6 +604,7 @@ __global__ __launch_bounds__(256) void joins_kernel(Joins joins) {
 struct LinearPlan {
   int shape;  // 0 large, 1 medium, 2 small, 3 narrow
   int shares, share;
+  int rows, rest;  // with one share: if rows > 0, that many rows of C are made so, and those behind them with shape `rest`
 };
 // kPlain with shares: leaves sums.
 template <class T>

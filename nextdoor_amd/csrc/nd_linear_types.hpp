@@ -221,6 +221,21 @@ hipError_t launch_join(const LinearParams& a, hipStream_t stream) {
 template <class T>
 hipError_t launch_linear(const LinearParams& a, Layout layout, After after, const LinearPlan& plan, hipStream_t stream) {
   LinearParams p = a;
+  if (plan.rows > 0) {
+    p.m = plan.rows;
+    const hipError_t e = launch_linear<T>(p, layout, after, {plan.shape, 1, plan.share}, stream);
+    if (e != hipSuccess) return e;
+    auto behind = [&](auto*& at, int64_t row_bytes) {
+      if (at) at = (std::remove_reference_t<decltype(at)>)((uintptr_t)at + plan.rows * row_bytes);
+    };
+    const int64_t n_bytes = (int64_t)a.n * 2;
+    behind(p.q, layout == Layout::kColumns ? 2 : a.q_bytes);
+    behind(p.residual, a.residual_bytes);
+    behind(p.out, n_bytes);
+    behind(p.z, after == After::kGated ? 3 * n_bytes : n_bytes);
+    p.m = a.m - plan.rows;
+    return launch_linear<T>(p, layout, after, {plan.rest, 1, plan.share}, stream);
+  }
   p.shares = plan.shares;
   p.share = plan.share;
   if (after == After::kPlain)

@@ -518,11 +518,11 @@ def test_matrices_of_more_than_4_gib():
 
 # ---- every kind of tile ----------------------------------------------------------------------------------------
 # Sizes for which the rules take each of the four shapes of tiles, with whole sums and with shares of them, in the forward
-# pass, for dx and for dweight (alone: both together go into one launch).  References in 64 bits on the GPU.
+# pass, for dx and for dweight (alone: both together go into one launch), and two shapes for the rows of one product.  References in 64 bits on the GPU.
 
 LINEAR_TILES = [(958, 528, 16008), (135, 13032, 15600), (2581, 3480, 8), (65, 976, 8), (13553, 136, 544), (5684, 11280, 136),
                 (958, 16008, 528), (5684, 136, 11280), (517, 1160, 12712), (12017, 15928, 136), (3479, 8, 2584), (129, 536, 13296),
-                (10768, 136, 5808)]
+                (10768, 136, 5808), (4104, 1000, 4096), (4104, 4096, 1000), (1000, 4096, 4104)]
 
 
 @pytest.mark.parametrize("rows,dim,out", LINEAR_TILES)
@@ -541,7 +541,7 @@ def test_linear_with_every_shape_of_tile(rows, dim, out, dtype):
 
 
 MLP_TILES = [(391, 848, 8400, 64), (133, 7072, 9264, 64), (7122, 9576, 72, 8), (2581, 3480, 8, 8), (65, 976, 8, 8), (655, 136, 10992, 800),
-             (6400, 136, 448, 152), (20483, 64, 256, 64)]
+             (6400, 136, 448, 152), (20483, 64, 256, 64), (4104, 2000, 2048, 64), (4104, 1000, 4096, 64)]
 
 
 @pytest.mark.parametrize("rows,dim,inner,out", MLP_TILES)
