@@ -89,7 +89,7 @@ Estimate estimate(const Task& t) {
   const ShapeCost& large = kShapes[0];
   const int64_t rounds = std::max<int64_t>(1, (t.k + 63) / 64), columns = t.after == After::kGated ? 2 * t.n : t.n;
   const int64_t across = (columns + large.n - 1) / large.n, down = (t.m + large.m - 1) / large.m, turns = across * down / large.at_once;
-  if (turns == 0 || turns * large.at_once == across * down || t.after == After::kSlope) return best;
+  if (turns == 0 || turns * large.at_once == across * down || t.after == After::kSlope) return best;  // (kSlope: 278 us and 279, a part of 4104 x 1000, 4096 inner)
   const int64_t rows = turns * large.at_once / across * large.m;
   if (rows == 0) return best;
   const double first = time_of(large, rows / large.m * across, rounds) + kLaunch;

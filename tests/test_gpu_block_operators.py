@@ -541,7 +541,8 @@ def test_linear_with_every_shape_of_tile(rows, dim, out, dtype):
 
 
 MLP_TILES = [(391, 848, 8400, 64), (133, 7072, 9264, 64), (7122, 9576, 72, 8), (2581, 3480, 8, 8), (65, 976, 8, 8), (655, 136, 10992, 800),
-             (6400, 136, 448, 152), (20483, 64, 256, 64), (4104, 2000, 2048, 64), (4104, 1000, 4096, 64)]
+             (6400, 136, 448, 152), (20483, 64, 256, 64), (4104, 2000, 2048, 64), (4104, 1000, 4096, 64),
+             (4104, 64, 4096, 1000)]
 
 
 @pytest.mark.parametrize("rows,dim,inner,out", MLP_TILES)
