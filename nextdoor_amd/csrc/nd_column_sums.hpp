@@ -9,7 +9,8 @@
 namespace nd {
 
 // The sum of sums[s][c] over the shares, times *factor unless that is null, for column c: to first[c], or from column `split` on to
-// second[c - split]; either may be null.  32 columns to a workgroup, 32 lanes to a column.
+// second[c - split]; either may be null.  32 columns to a workgroup, 32 lanes to a column: bound by the latency of one lane's reads
+// (256 shares, 8 each: 4 to 5 us with the launch).
 template <class T>
 __global__ __launch_bounds__(1024) void column_join_kernel(const float* sums, int64_t shares, int64_t columns, const float* factor, T* first,
                                                            int64_t split, T* second) {
