@@ -279,7 +279,7 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
 struct NormShape {
   int most, lanes, rows;
 };
-constexpr NormShape kNormShapes[] = {{128, 16, 64}, {512, 64, 16}, {1024, 128, 8}, {2048, 256, 4}, {4096, 512, 2}, {8192, 1024, 1}, {16384, 1024, 1}};
+constexpr NormShape kNormShapes[] = {{64, 8, 128}, {128, 16, 64}, {256, 32, 32}, {512, 64, 16}, {1024, 128, 8}, {2048, 256, 4}, {4096, 512, 2}, {8192, 1024, 1}, {16384, 1024, 1}};
 constexpr int kForwardLanes = 1 << 19, kBackwardBlocks = 256;
 constexpr int kAlone = 6;  // times at most that one workgroup takes the next rows: less than another launch, which adds up sums, costs
 int shape_of(int32_t dim) {
@@ -312,12 +312,14 @@ void launch_norm(const NormParams& p, bool backward, hipStream_t stream) {
                        (backward ? (uintptr_t)p.dout | (uintptr_t)p.dout_bytes : 0);
   const bool vector = p.dim % 8 == 0 && (at & 15) == 0;
   switch (shape_of(p.dim)) {
-    case 0: return launch_norm_of<T, 16, 8>(p, backward, vector, stream);
-    case 1: return launch_norm_of<T, 64, 8>(p, backward, vector, stream);
-    case 2: return launch_norm_of<T, 128, 8>(p, backward, vector, stream);
-    case 3: return launch_norm_of<T, 256, 8>(p, backward, vector, stream);
-    case 4: return launch_norm_of<T, 512, 8>(p, backward, vector, stream);
-    case 5: return launch_norm_of<T, 1024, 8>(p, backward, vector, stream);
+    case 0: return launch_norm_of<T, 8, 8>(p, backward, vector, stream);
+    case 1: return launch_norm_of<T, 16, 8>(p, backward, vector, stream);
+    case 2: return launch_norm_of<T, 32, 8>(p, backward, vector, stream);
+    case 3: return launch_norm_of<T, 64, 8>(p, backward, vector, stream);
+    case 4: return launch_norm_of<T, 128, 8>(p, backward, vector, stream);
+    case 5: return launch_norm_of<T, 256, 8>(p, backward, vector, stream);
+    case 6: return launch_norm_of<T, 512, 8>(p, backward, vector, stream);
+    case 7: return launch_norm_of<T, 1024, 8>(p, backward, vector, stream);
     default: return launch_norm_of<T, 1024, 16>(p, backward, vector, stream);
   }
 }
