@@ -6,15 +6,16 @@
 // Bound by memory: a row is read once and stays in registers for its two sums, the deviations' squares being taken once the
 // mean is known.  LANES lanes have a row, each VALUES of its places; a workgroup has a number of rows at a time and asks for the next
 // ones before it sums those it has.  w and b, and in the backward pass the sums for dw and db, stay in registers over all rows of a
-// workgroup; another kernel adds the workgroups' sums.  Forward and backward, in 16 bits 8192 x 1024: 11 and 16 us (3.1 TB/s, of which
-// the start of workgroups and the last rows' sums are a third), 16384 x 4096: 59 and 88 (4.6 TB/s, as fast as a copy); in 32 bits
-// 20011 x 1021, places one by one: 34 and 42 (4.8 and 5.8, some of it from the last cache); the sums' kernel 4 to 5.
+// workgroup; another kernel adds the workgroups' sums.  Forward and backward, in 16 bits 8192 x 1024: 10 and 16 us (3.2 TB/s, of which
+// the start of workgroups and the last rows' sums are a third), 16384 x 4096: 50 and 93 (5.4 and 4.3 TB/s); in 32 bits 20011 x 1021: 32
+// and 42 (5.1 and 5.8, some of it from the last cache); the sums' kernel 4 to 5.
 #include "../../include/nextdoor_amd.h"
 
 #include <math.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "nd_column_sums.hpp"
 #include "nd_errors.hpp"
@@ -38,51 +39,46 @@ struct NormParams {
   float eps;
 };
 
-// VALUES places of a row: VECTOR: runs of eight, each 16 bytes aligned (32 bits: twice that), LANES runs apart; else single ones.
-template <class T, int LANES, int VALUES, bool VECTOR>
+// How a row's places are shared out among lanes.  kWhole: runs of 16 bytes, one after another, of which rows are multiples; kOver: the
+// same, but the last run ends where the row ends and begins among the places of the one before, which are not counted twice (and are
+// written twice, the same); kSingle: one by one, rows shorter than a run.  Loads need no alignment but the elements'.  (Place by place
+// 20011 x 1021 in 16 bits took 21.6 and 32.9 us for 16.5 and 30.9, 8000 x 4001 32.5 and 49 for 24 and 45.)
+enum class Runs { kWhole, kOver, kSingle };
+
+// VALUES places of a row with a lane, in runs that lie LANES runs apart.
+template <class T, int LANES, int VALUES, Runs RUNS, int RUN = RUNS == Runs::kSingle ? 1 : 16 / sizeof(T)>
 struct Places {
-  static constexpr int kRun = VECTOR ? 8 : 1;
+  static constexpr int kRun = RUN;
+  using Word = std::conditional_t<RUNS == Runs::kSingle, T, uint32_t>;  // (pairs of 16-bit values stay as they are until they are used)
+  struct __attribute__((packed, aligned(sizeof(T)))) Run {
+    Word w[kRun * sizeof(T) / sizeof(Word)];
+  };
   T v[VALUES];
-  __device__ __forceinline__ static int column(int i, int lane) { return (i / kRun * LANES + lane) * kRun + i % kRun; }
+  // The first place of the run that place i belongs to, and where that run is read.
+  __device__ __forceinline__ static int first(int i, int lane) { return (i / kRun * LANES + lane) * kRun; }
+  __device__ __forceinline__ static int at(int i, int lane, int dim) { return min(first(i, lane), dim - kRun); }
+  __device__ __forceinline__ static int column(int i, int lane, int dim) { return at(i, lane, dim) + i % kRun; }
+  __device__ __forceinline__ static bool there(int i, int lane, int dim) { return first(i, lane) < dim; }
+  // (past the row's end a run is at the end, and all of its places belong to others)
+  __device__ __forceinline__ static bool counts(int i, int lane, int dim) {
+    return RUNS == Runs::kOver ? column(i, lane, dim) >= first(i, lane) : there(i, lane, dim);
+  }
   __device__ __forceinline__ void load(const char* row, int dim, int lane) {
-    if constexpr (VECTOR) {
 #pragma unroll
-      for (int i = 0; i < VALUES; i += 8) {
-        const int c = column(i, lane);
-        u32x4 w[sizeof(T) / 2];
-#pragma unroll
-        for (unsigned j = 0; j < sizeof(T) / 2; ++j) w[j] = c < dim ? ((const u32x4*)(row + (int64_t)c * sizeof(T)))[j] : u32x4{0, 0, 0, 0};
-        __builtin_memcpy(&v[i], w, sizeof(w));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VALUES; ++i) {
-        const int c = column(i, lane);
-        v[i] = c < dim ? ((const T*)row)[c] : T(0.f);
-      }
+    for (int i = 0; i < VALUES; i += kRun) {
+      const Run r = *(const Run*)(row + (uint32_t)at(i, lane, dim) * sizeof(T));
+      __builtin_memcpy(&v[i], &r, sizeof(r));
     }
   }
   __device__ __forceinline__ static void store(char* row, int dim, int lane, const float (&x)[VALUES]) {
-    if constexpr (VECTOR) {
 #pragma unroll
-      for (int i = 0; i < VALUES; i += 8) {
-        const int c = column(i, lane);
-        T out[8];
+    for (int i = 0; i < VALUES; i += kRun) {
+      T out[kRun];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = (T)x[i + j];
-        u32x4 w[sizeof(T) / 2];
-        __builtin_memcpy(w, out, sizeof(w));
-        if (c < dim) {
-#pragma unroll
-          for (unsigned j = 0; j < sizeof(T) / 2; ++j) ((u32x4*)(row + (int64_t)c * sizeof(T)))[j] = w[j];
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VALUES; ++i) {
-        const int c = column(i, lane);
-        if (c < dim) ((T*)row)[c] = (T)x[i];
-      }
+      for (int j = 0; j < kRun; ++j) out[j] = (T)x[i + j];
+      Run r;
+      __builtin_memcpy(&r, out, sizeof(r));
+      if (there(i, lane, dim)) *(Run*)(row + (uint32_t)at(i, lane, dim) * sizeof(T)) = r;
     }
   }
   // Weights: of this type or in 32 bits; a null array is `otherwise` everywhere.
@@ -91,7 +87,7 @@ struct Places {
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) x[i] = otherwise;
     } else if (in_32) {
-      Places<float, LANES, VALUES, VECTOR> all;
+      Places<float, LANES, VALUES, RUNS, RUN> all;
       all.load((const char*)w, dim, lane);
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) x[i] = all.v[i];
@@ -127,15 +123,21 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 (*scratch)[THREADS /
   return v;
 }
 
-template <class T, int LANES, int VALUES, int THREADS, int AHEAD, bool VECTOR>
+// Which row of those that a workgroup has at a time; the same for a whole wave, and so are its addresses, where a row has 64 lanes.
+template <int LANES>
+__device__ __forceinline__ int group_of() {
+  return LANES < 64 ? threadIdx.x / LANES : uniform(threadIdx.x / LANES);
+}
+
+template <class T, int LANES, int VALUES, int THREADS, int AHEAD, Runs RUNS>
 __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormParams p) {
-  using Row = Places<T, LANES, VALUES, VECTOR>;
+  using Row = Places<T, LANES, VALUES, RUNS>;
   constexpr int kGroups = THREADS / LANES;
   __shared__ float2 scratch[2][THREADS / 64];
-  const int lane = threadIdx.x % LANES;
+  const int lane = threadIdx.x % LANES, group = group_of<LANES>();
   const int64_t stride = (int64_t)gridDim.x * kGroups;
   Row next[AHEAD];
-  int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / LANES;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
 #pragma unroll
   for (int a = 0; a < AHEAD; ++a)
     if (row + a * stride < p.rows) next[a].load(p.x + (row + a * stride) * p.x_bytes, p.dim, lane);
@@ -151,15 +153,15 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormParams p) {
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) {
         x[i] = there ? (float)next[a].v[i] : 0.f;
-        sum += x[i];
+        sum += Row::counts(i, lane, p.dim) ? x[i] : 0.f;
       }
       if (row + AHEAD * stride < p.rows) next[a].load(p.x + (row + AHEAD * stride) * p.x_bytes, p.dim, lane);
       const float mean = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
       sum = 0.f;
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) {
-        x[i] = Row::column(i, lane) < p.dim ? x[i] - mean : 0.f;
-        sum = __builtin_fmaf(x[i], x[i], sum);
+        x[i] -= mean;
+        sum = __builtin_fmaf(x[i], Row::counts(i, lane, p.dim) ? x[i] : 0.f, sum);
       }
       const float variance = row_sums<LANES, THREADS>(make_float2(sum, 0.f), scratch, turn++).x / p.dim;
       const float rstd = 1.f / sqrtf(variance + p.eps);
@@ -176,12 +178,12 @@ __global__ __launch_bounds__(THREADS) void norm_forward_kernel(NormParams p) {
   }
 }
 
-template <class T, int LANES, int VALUES, int THREADS, int AHEAD, bool VECTOR>
+template <class T, int LANES, int VALUES, int THREADS, int AHEAD, Runs RUNS>
 __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
-  using Row = Places<T, LANES, VALUES, VECTOR>;
+  using Row = Places<T, LANES, VALUES, RUNS>;
   constexpr int kGroups = THREADS / LANES;
   __shared__ float2 scratch[2][THREADS / 64];
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int lane = threadIdx.x % LANES, group = group_of<LANES>();
   const int64_t stride = (int64_t)gridDim.x * kGroups;
   Row next[AHEAD], next_dout[AHEAD];
   float next_mean[AHEAD], next_rstd[AHEAD];
@@ -211,14 +213,14 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < VALUES; ++i) {
-        const bool inside = there && Row::column(i, lane) < p.dim;
-        const float d = inside ? (float)next_dout[a].v[i] : 0.f;
-        n[i] = inside ? ((float)next[a].v[i] - mean) * rstd : 0.f;
+        const float d = there ? (float)next_dout[a].v[i] : 0.f;
+        n[i] = there ? ((float)next[a].v[i] - mean) * rstd : 0.f;
         dw[i] = __builtin_fmaf(d, n[i], dw[i]);
         db[i] += d;
         e[i] = d * w[i];
-        sum.x += e[i];
-        sum.y = __builtin_fmaf(e[i], n[i], sum.y);
+        const float counted = Row::counts(i, lane, p.dim) ? e[i] : 0.f;
+        sum.x += counted;
+        sum.y = __builtin_fmaf(counted, n[i], sum.y);
       }
       ask(a, row + AHEAD * stride);
       if (p.out) {
@@ -260,8 +262,8 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
   };
 #pragma unroll
   for (int i = 0; i < VALUES; ++i) {
-    const int c = Row::column(i, lane);
-    if (c >= p.dim) continue;
+    if (!Row::counts(i, lane, p.dim)) continue;
+    const int c = Row::column(i, lane, p.dim);
     if (p.sums) {
       float* sums = p.sums + (int64_t)blockIdx.x * 2 * p.dim;
       sums[c] = dw[i];
@@ -273,8 +275,9 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormParams p) {
   }
 }
 
-// Rows by size: eight places to a lane, sixteen for the longest, and as many lanes as that takes; `rows` of a workgroup at a time in
-// the backward pass, which has one workgroup of 1024 lanes to a compute unit, so that few sums are left to add.  The forward pass
+// Rows by size: eight places to a lane, sixteen for the longest, and as many lanes as that takes, 8 at least (with 16
+// lanes for up to 128 places and 64 for up to 512 alone, 92000 x 256 in 16 bits took 26.5 and 39 us for 17 and 31, 300000 x 64 24 and 34
+// for 14.6 and 29); `rows` of a workgroup at a time in the backward pass, which has one workgroup of 1024 lanes to a compute unit, so that few sums are left to add.  The forward pass
 // has workgroups of 256 or what a row takes.
 struct NormShape {
   int most, lanes, rows;
@@ -293,34 +296,48 @@ int64_t backward_blocks(int64_t rows, int32_t dim) {
   return std::max<int64_t>(1, std::min<int64_t>(kBackwardBlocks, (rows + at_once - 1) / at_once));
 }
 
-template <class T, int LANES, int VALUES>
-void launch_norm_of(const NormParams& p, bool backward, bool vector, hipStream_t stream) {
-  if (backward) {
-    const uint32_t blocks = (uint32_t)backward_blocks(p.rows, p.dim);
-    if (vector) norm_backward_kernel<T, LANES, VALUES, 1024, VALUES == 8 && sizeof(T) == 2 ? 2 : 1, true><<<blocks, 1024, 0, stream>>>(p);
-    else norm_backward_kernel<T, LANES, VALUES, 1024, 1, false><<<blocks, 1024, 0, stream>>>(p);
+template <class T, int LANES, int VALUES, Runs RUNS>
+void launch_backward(const NormParams& p, hipStream_t stream) {
+  const uint32_t blocks = (uint32_t)backward_blocks(p.rows, p.dim);
+  norm_backward_kernel<T, LANES, VALUES, 1024, VALUES == 8 && sizeof(T) == 2 ? 2 : 1, RUNS><<<blocks, 1024, 0, stream>>>(p);
+}
+template <class T, int LANES, int VALUES, Runs RUNS>
+void launch_forward(const NormParams& p, hipStream_t stream) {
+  constexpr int kThreads = LANES < 256 ? 256 : LANES, kGroups = kThreads / LANES;
+  const uint32_t blocks = (uint32_t)std::min<int64_t>((p.rows + kGroups - 1) / kGroups, kForwardLanes / kThreads);
+  norm_forward_kernel<T, LANES, VALUES, kThreads, 1, RUNS><<<blocks, kThreads, 0, stream>>>(p);
+}
+// FORWARD: lanes to a row in the forward pass: half as many for 513 to 8192 places of 16 bits, sixteen to each, as less waits for others
+// then (20011 x 1024: 15.6 us for 17.3, 5000 x 8000: 28 for 34; in 32 bits equal or slower).
+template <class T, int LANES, int VALUES, int FORWARD = LANES>
+void launch_norm_of(const NormParams& p, bool backward, hipStream_t stream) {
+  constexpr int kForwardValues = VALUES * LANES / FORWARD;
+  if (p.dim % (16 / sizeof(T)) == 0) {
+    if (backward) launch_backward<T, LANES, VALUES, Runs::kWhole>(p, stream);
+    else launch_forward<T, FORWARD, kForwardValues, Runs::kWhole>(p, stream);
   } else {
-    constexpr int kThreads = LANES < 256 ? 256 : LANES, kGroups = kThreads / LANES;
-    const uint32_t blocks = (uint32_t)std::min<int64_t>((p.rows + kGroups - 1) / kGroups, kForwardLanes / kThreads);
-    if (vector) norm_forward_kernel<T, LANES, VALUES, kThreads, 1, true><<<blocks, kThreads, 0, stream>>>(p);
-    else norm_forward_kernel<T, LANES, VALUES, kThreads, 1, false><<<blocks, kThreads, 0, stream>>>(p);
+    if (backward) launch_backward<T, LANES, VALUES, Runs::kOver>(p, stream);
+    else launch_forward<T, FORWARD, kForwardValues, Runs::kOver>(p, stream);
   }
 }
 template <class T>
 void launch_norm(const NormParams& p, bool backward, hipStream_t stream) {
-  const uintptr_t at = (uintptr_t)p.x | (uintptr_t)p.out | (uintptr_t)p.weight | (uintptr_t)p.bias | (uintptr_t)p.x_bytes |
-                       (backward ? (uintptr_t)p.dout | (uintptr_t)p.dout_bytes : 0);
-  const bool vector = p.dim % 8 == 0 && (at & 15) == 0;
+  if (p.dim < (int)(16 / sizeof(T))) {
+    if (backward) launch_backward<T, 8, 1, Runs::kSingle>(p, stream);
+    else launch_forward<T, 8, 1, Runs::kSingle>(p, stream);
+    return;
+  }
+  constexpr bool k16 = sizeof(T) == 2;
   switch (shape_of(p.dim)) {
-    case 0: return launch_norm_of<T, 8, 8>(p, backward, vector, stream);
-    case 1: return launch_norm_of<T, 16, 8>(p, backward, vector, stream);
-    case 2: return launch_norm_of<T, 32, 8>(p, backward, vector, stream);
-    case 3: return launch_norm_of<T, 64, 8>(p, backward, vector, stream);
-    case 4: return launch_norm_of<T, 128, 8>(p, backward, vector, stream);
-    case 5: return launch_norm_of<T, 256, 8>(p, backward, vector, stream);
-    case 6: return launch_norm_of<T, 512, 8>(p, backward, vector, stream);
-    case 7: return launch_norm_of<T, 1024, 8>(p, backward, vector, stream);
-    default: return launch_norm_of<T, 1024, 16>(p, backward, vector, stream);
+    case 0: return launch_norm_of<T, 8, 8>(p, backward, stream);
+    case 1: return launch_norm_of<T, 16, 8>(p, backward, stream);
+    case 2: return launch_norm_of<T, 32, 8>(p, backward, stream);
+    case 3: return launch_norm_of<T, 64, 8>(p, backward, stream);
+    case 4: return launch_norm_of<T, 128, 8, k16 ? 64 : 128>(p, backward, stream);
+    case 5: return launch_norm_of<T, 256, 8, k16 ? 128 : 256>(p, backward, stream);
+    case 6: return launch_norm_of<T, 512, 8, k16 ? 256 : 512>(p, backward, stream);
+    case 7: return launch_norm_of<T, 1024, 8, k16 ? 512 : 1024>(p, backward, stream);
+    default: return launch_norm_of<T, 1024, 16>(p, backward, stream);
   }
 }
 

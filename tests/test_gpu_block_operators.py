@@ -60,6 +60,25 @@ def test_norm_of_rows_of_every_size(dim, dtype):
     check_all(run_norm(x, w, b, d), want, off, (dim, dtype))
 
 
+@pytest.mark.parametrize("dim", [3, 4, 5, 9, 15, 16, 17, 63, 65, 66, 127, 130, 255, 256, 257, 264, 1023, 2047, 2049, 4095, 8191, 8193, 16381])
+@pytest.mark.parametrize("dtype,weights", [(BF16, BF16), (F16, F32), (F32, F32)])
+def test_norm_of_rows_between_others(dim, dtype, weights):
+    """Rows whose beginnings have the alignment of an element only, and NaN on both sides of them."""
+    rows = 70 if dim < 2049 else 5
+    def between(t, step):
+        room = torch.full((*t.shape[:-1], dim + step), math.nan, dtype=t.dtype)
+        room[..., 1:dim + 1] = t
+        return room.cuda()[..., 1:dim + 1]
+    x, d = normal(1, rows, dim, dtype=dtype, mean=0.5), normal(2, rows, dim, dtype=dtype)
+    w, b = normal(3, dim, dtype=weights, mean=1.0, std=0.3), normal(4, dim, dtype=weights)
+    want, off = ref.layer_norm(x, w, b, 1e-5, d)
+    gx, gd, gw, gb = between(x, 3), between(d, 2), between(w, 2), between(b, 2)
+    out, mean, rstd = ops.layer_norm_forward(gx, gw, gb, 1e-5)
+    got = ops.layer_norm_backward(gd, gx, gw, mean, rstd)
+    torch.cuda.synchronize()
+    check_all(dict(zip(("out", "dx", "dweight", "dbias"), (out, *got))), want, off, (dim, dtype))
+
+
 @pytest.mark.parametrize("rows,dim", [(0, 64), (1, 64), (1, 1024), (2049, 64), (40007, 24), (9001, 96), (3001, 1000), (1501, 1032)])
 def test_norm_of_any_number_of_rows(rows, dim):
     x, w, b, d = normal(1, rows, dim), normal(2, dim), normal(3, dim), normal(4, rows, dim)
