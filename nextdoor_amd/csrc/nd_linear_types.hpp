@@ -17,7 +17,7 @@ __device__ __forceinline__ f32x4 product_16x16x32(u32x4 a, u32x4 b, f32x4 c, _Fl
 // A workgroup makes 16 columns of C (gated: 16 pairs) for up to 16 ROW_BLOCKS rows.  Its waves share out the sum, 64 places at a
 // time, and read the weights straight to registers: lane l has row l & 15, places 8 (l >> 4) .. + 7 of 32, so two products use
 // whole lines of 128 bytes.  x is the same for all workgroups and comes from the caches.  Bound by the latency of one chain: launch,
-// weights, the waves' sums, what is added (1 x 1024 -> 4096: 8.4 MB in 4.2 us, 3.3 being what the smallest kernel takes; 16 x 1024 ->
+// weights, the waves' sums, what is added (1 x 1024 -> 4096: 8.4 MB in 4.2 us, 2.7 being what the smallest kernel takes; 16 x 1024 ->
 // 2 x 2816: 11.5 MB in 6.0).
 template <class T, int ROW_BLOCKS, After AFTER, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void few_rows_kernel(LinearParams a) {
