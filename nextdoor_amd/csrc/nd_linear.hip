@@ -181,8 +181,11 @@ struct Call {
     }
     LinearParams p = a;
     p.sums = sums;
-    // (what the caches do not hold until the backward pass: 8192 x 2 x 5632 at 3 bytes, 368 us and 346; 3001 x 2 x 1000, both passes, 87 and 89)
-    p.z_later = a.z && (int64_t)a.m * a.n * (after == After::kGated ? 6 : 2) > kCaches;
+    // What the caches do not hold until the backward pass is written past them (8192 x 2 x 5632 at 3 bytes, 368 us and 346; 3001 x 2 x
+    // 1000, both passes, 87 and 89), gated only where rows of its three parts begin with half lines: other pieces of 64 bytes are better put
+    // together in the caches (both passes, 26020 x 2 x 456 175 us and 157, 8192 x 2 x 2728 594 and 562; 18436 x 2 x 1056 272 and 274, and
+    // 30000 x 1000 without a gate 158 and 161).
+    p.z_later = a.z && (int64_t)a.m * a.n * (after == After::kGated ? 6 : 2) > kCaches && (after != After::kGated || a.n % 32 == 0);
     const LinearPlan plan = plan_of({a.m, a.n, a.k, after});
     note(bf16 ? launch_linear<__bf16>(p, Layout::kRows, after, plan, stream) : launch_linear<_Float16>(p, Layout::kRows, after, plan, stream));
   }
