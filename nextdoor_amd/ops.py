@@ -24,6 +24,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 from ._capi import LayerNorm, Linear, Mlp, NextDoorError, PackedAttention, VocabularyLoss, check
@@ -489,6 +490,12 @@ def _room(a, size, device):
     return workspace
 
 
+def _nothing_to_derive():
+    """Whether a call may pass autograd by, which costs some 5 us: gradients are off, and so is forward mode, which no_grad
+    leaves on and which has to see the call to refuse it."""
+    return not torch.is_grad_enabled() and forward_ad._current_level < 0
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -506,7 +513,7 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """The ``out`` of :func:`layer_norm_forward`, differentiable in x, weight and bias."""
-    if not torch.is_grad_enabled():
+    if _nothing_to_derive():
         return layer_norm_forward(x, weight, bias, eps)[0]
     return _LayerNorm.apply(x, weight, bias, eps)
 
@@ -667,7 +674,7 @@ class _Linear(torch.autograd.Function):
 
 def linear(x, weight, bias=None, activation=None, residual=None):
     """:func:`linear_forward`, differentiable in x, weight, bias and the residual."""
-    if not torch.is_grad_enabled():  # (nothing is kept)
+    if _nothing_to_derive():  # (nothing is kept)
         return linear_forward(x, weight, bias, activation, residual)
     return _Linear.apply(x, weight, bias, residual, activation)
 
@@ -801,6 +808,6 @@ class _Mlp(torch.autograd.Function):
 
 def mlp(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None):
     """:func:`mlp_forward`, differentiable in x, the weights, the biases and the residual."""
-    if not torch.is_grad_enabled():
+    if _nothing_to_derive():
         return mlp_forward(x, up, down, up_bias, down_bias, activation, gated, residual)
     return _Mlp.apply(x, up, down, up_bias, down_bias, activation, gated, residual)

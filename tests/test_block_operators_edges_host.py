@@ -1,0 +1,44 @@
+"""Layer norm, linear maps and feed-forward parts: what torch asks of them beside their values, without a GPU."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from nextdoor_amd import ops
+
+
+@pytest.fixture
+def without_kernels(monkeypatch):
+    """The forward functions give something of the right shape; what is kept for a backward pass is None."""
+    def norm(x, weight=None, bias=None, eps=1e-5):
+        return 2 * x.detach(), None, None
+
+    def linear(x, weight, bias=None, activation=None, residual=None, keep=False):
+        out = x.detach() @ weight.detach().T
+        return (out, None) if keep else out
+
+    def mlp(x, up, down, up_bias=None, down_bias=None, activation="silu", gated=True, residual=None, keep=False):
+        out = x.detach() @ down.detach().T
+        return (out, None, None) if keep else out
+    for name, function in (("layer_norm_forward", norm), ("linear_forward", linear), ("mlp_forward", mlp)):
+        monkeypatch.setattr(ops, name, function)
+
+
+CALLS = [("x", lambda x, w: ops.layer_norm(x)), ("x", lambda x, w: ops.linear(x, w)), ("weight", lambda x, w: ops.linear(x, w)),
+         ("x", lambda x, w: ops.mlp(x, w, w, gated=False)), ("weight", lambda x, w: ops.mlp(x, w, w, gated=False))]
+
+
+@pytest.mark.parametrize("which,call", CALLS)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_derivatives_are_refused_and_not_lost(without_kernels, which, call, grad):
+    """no_grad switches gradients off, and not forward mode: without a tangent the result would count as constant."""
+    x, w = torch.ones(4, 8), torch.ones(8, 8)
+    with torch.set_grad_enabled(grad):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x if which == "x" else w, torch.ones(4 if which == "x" else 8, 8))
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward mode|jvp"):
+                call(dual, w) if which == "x" else call(x, dual)
+        of = (lambda t: call(t, w)) if which == "x" else (lambda t: call(x, t))
+        at = x if which == "x" else w
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(of, (at,), (at,))
+        assert call(x, w).shape == (4, 8) and not call(x, w).requires_grad
