@@ -224,11 +224,14 @@ struct Call {
               : launch_slope<_Float16>(a, dout, dout_bytes, parted, whole, shares, parts, stream));
     if (parted) join(sums, shares, a.n, nullptr, total);
   }
+  // float16: dz made again where it leaves its range.
+  void again(const LinearParams& a, const LinearPlan& plan) { note(launch_again<_Float16>(a, plan, stream)); }
   // Of dout [rows][columns]: the sums of its rows, unless out is null, and the largest of its values, unless parts is.
-  void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts) {
+  void survey(const void* dout, int64_t row_bytes, int64_t rows, int32_t columns, float* sums, void* out, float* parts, uint32_t* found = nullptr) {
     LinearParams p = {};
     p.m = (int32_t)rows;
     p.n = columns;
+    p.found = found;
     slope(p, dout, row_bytes, sums, out, survey_shares(rows, columns, parts), parts);
   }
   int done() const { return error == hipSuccess ? 0 : fail(std::string(what) + ": " + hipGetErrorString(error)); }
@@ -405,7 +408,7 @@ int run_linear(const nd_linear* a, bool backward, void* stream) {
 struct MlpWork {
   TwoPlans first, second;  // dz and ddown; dx and dup
   int64_t shares;          // of the rows, whose sums the product that makes dz leaves
-  int64_t dz, forward, dx, dup, ddown, rows, columns, parts, unscale, bytes;
+  int64_t dz, forward, dx, dup, ddown, rows, columns, parts, unscale, found, bytes;
 };
 MlpWork work_of(const nd_mlp* a, bool backward) {
   MlpWork w = {};
@@ -429,6 +432,7 @@ MlpWork work_of(const nd_mlp* a, bool backward) {
     w.columns = l.take(a->dup_bias ? w.shares * wide * 4 : 0);
     w.parts = l.take(scaled ? survey_parts(a->rows, a->out_dim) * 4 : 0);
     w.unscale = l.take(scaled ? 4 : 0);
+    w.found = l.take(scaled ? kExponents * 4 : 0);
   }
   w.bytes = l.bytes;
   return w;
@@ -490,7 +494,8 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   const int64_t dout_bytes = a->dout_row * 2;
   float* parts = first && some && !call.bf16 ? (float*)(work + w.parts) : nullptr;  // (without rows nobody leaves an unscale)
   float* unscale = parts ? (float*)(work + w.unscale) : nullptr;
-  if (a->ddown_bias || parts) call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, parts);
+  uint32_t* found = parts ? (uint32_t*)(work + w.found) : nullptr;
+  if (a->ddown_bias || parts) call.survey(a->dout, dout_bytes, a->rows, a->out_dim, (float*)(work + w.rows), a->ddown_bias, parts, found);
   float* columns = a->dup_bias ? (float*)(work + w.columns) : nullptr;
   LinearParams p = {};
   p.p = a->down;
@@ -507,10 +512,12 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
   p.parts = parts;
   p.n_parts = parts ? survey_parts(a->rows, a->out_dim) : 0;
   p.unscale = unscale;
+  p.found = found;
   p.column_sums = columns;
   const LinearParams ddown =
       gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, (float*)(work + w.ddown));
   call.backward(first ? &p : nullptr, After::kSlope, a->ddown ? &ddown : nullptr, w.first);
+  if (parts) call.again(p, w.first.first);
   if (columns) call.join(columns, w.shares, wide, unscale, a->dup_bias);
   const char* dz = work + w.dz;
   const LinearParams dx = gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, unscale, a->dx, (float*)(work + w.dx));

@@ -9,8 +9,8 @@
 // Sums are held in 32 bits; z, h and dz, which the next product or the backward pass reads, are rounded to 16 bits once, as
 // the results are; but the z of a gated part, of which g and u are both factors of dz, keeps the upper 24 bits of 32: rounded to
 // bfloat16 they had brought the gradients' error from 2.4e-3 to 3.0e-3 (1.7e-3 is that of rounding them alone).  float16: dz is held
-// times a power of two, so that the small gradients of a mean over many rows are not lost below 2^-14: see scale_of.  What is made of
-// it is divided by that in 32 bits.
+// times a power of two, so that the small gradients of a mean over many rows are not lost below 2^-14, nor large ones above 65504: see
+// scale_of.  What is made of it is divided by that in 32 bits.
 #pragma once
 
 #include <algorithm>
@@ -21,6 +21,8 @@
 namespace nd {
 
 enum class After { kSums, kForward, kGated, kPlain, kSlope };  // (kPlain: sums too, where there are shares)
+
+constexpr int kExponents = 256;
 
 struct LinearParams {
   // C [m][n], sums over k; gated: n counts pairs, and P has 2 n rows
@@ -34,10 +36,13 @@ struct LinearParams {
   void* z;  // forward: written unless null; backward: read.  [m][n]; gated: rows of 6 n bytes, see Upper24
   bool z_later;  // forward: z is written past the caches
   // float16: what dz is held times.  parts: the largest finite |dout| of workgroups, null: 1.  Who makes dz finds the scale in them and
-  // leaves one over it in *unscale, with which the sums of kPlain are multiplied (null: 1).
+  // leaves one over it in *unscale, with which the sums of kPlain are multiplied (null: 1).  kSlope: found
+  // [kExponents], 0 before, see there; again: the scale comes from that.
   const float* parts;
   int64_t n_parts;
   float* unscale;
+  uint32_t* found;
+  bool again;
   // shares of the sum: share s has places s * share .. and leaves [m][n] values (gated: [m][2 n]) in 32 bits
   float* sums;
   int32_t shares, share;
@@ -66,18 +71,61 @@ struct Upper24 {
   }
 };
 
-// What dz is held times, for all lanes of a wave: a power of two that takes the largest |dout|, of all parts, to 16 or more where it is
-// less, and to below 256 where it is more.  Smaller rows next to larger ones lose nothing that dout itself has in 16 bits (but the
-// last bits of what is below 2^-14 next to more than 256), and dz may be 255 times the largest |dout|, 2000 times below 16.
-__device__ __forceinline__ float scale_of(const float* parts, int64_t n, int lane) {
+// What dz is held times, for all lanes of a wave: a power of two that takes the largest finite |dout|, of all parts, to 2^TO or more
+// and below twice that; but no less than LEAST.
+template <int TO>
+__device__ __forceinline__ float scale_of(const float* parts, int64_t n, int lane, float least) {
   float most = 0.f;
 #pragma unroll 4
   for (int64_t i = lane; i < n; i += 64) most = fmaxf(most, parts[i]);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   if (most == 0.f) return 1.f;
-  const int power = ilogbf(most);
-  return ldexpf(1.f, power < 4 ? 4 - power : power > 7 ? 7 - power : 0);
+  return fmaxf(least, ldexpf(1.f, TO - ilogbf(most)));
+}
+// dz = dout a'(z): no slope is above 1.13, so the largest dz is at most 1.13 2^15.
+__device__ __forceinline__ float scale_of_slopes(const float* parts, int64_t n, int lane) { return scale_of<14>(parts, n, lane, 0.f); }
+// dz of a feed-forward part is dh, a product with weights, times a slope and u: it may be any number of times dout.  The largest |dout|
+// is taken to 2^9 where it is less, so that 64 times that is still held, and 2^-23 of it with all its bits.  Where the largest dz turns out
+// to be above 65504, an infinity, or below 1, where smaller rows lose their last bits, dz is made again with the largest at 2^14: smaller
+// rows are then off by 2^-39 of it, less than the results' own rounding where its gradients are numbers of 16 bits.
+__device__ __forceinline__ float scale_of_products(const float* parts, int64_t n, int lane) { return scale_of<9>(parts, n, lane, 1.f); }
+// Each wave marks the exponent of the largest finite |dz| that it would hold: a store that no other wave's can spoil.  (With an atomic
+// maximum, of one word or of 64, the kernel took 2 to 12 us longer.)
+__device__ __forceinline__ void mark(uint32_t* found, float most) {
+  // (what is 65473 or more counts with what is 2^16 or more)
+  found[__float_as_uint(__builtin_fmaf(most, 0x1p-10f, most)) >> 23] = 1;
+}
+// The largest of the exponents that are marked, for all lanes of a wave; as they are in a float's bits, 0 if there is none.
+__device__ __forceinline__ int largest_of(const uint32_t* found, int lane) {
+  int largest = 0;
+#pragma unroll
+  for (int i = lane; i < kExponents; i += 64) largest = found[i] ? i : largest;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) largest = max(largest, __shfl_xor(largest, d));
+  return largest;
+}
+__device__ __forceinline__ bool leaves_range(int exponent) { return exponent > 0 && (exponent < 127 || exponent > 127 + 15); }
+// (2^48: dh, at most 2^52, stays a finite number of 32 bits before it is multiplied with a slope)
+__device__ __forceinline__ float scale_again(float scale, int exponent) { return fminf(ldexpf(scale, 127 + 14 - exponent), 0x1p48f); }
+
+// The largest |v| (NaN aside) of the first `quarters` quarters of a lane's values; what of v is finite, where there are others.
+__device__ __forceinline__ float most_of(const float (&v)[16], int quarters) {
+  float most = 0.f;
+  if (quarters >= 4) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(v[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 12; ++e) most = fmaxf(most, e / 4 < quarters ? fabsf(v[e]) : 0.f);
+  }
+  return most;
+}
+__device__ __forceinline__ float finite_most_of(const float (&v)[16], int quarters) {
+  float finite[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) finite[e] = fabsf(v[e]) < INFINITY ? v[e] : 0.f;
+  return most_of(finite, quarters);
 }
 
 // The sums of 16 values over the 32 lanes of a half: lane l has that of value l & 15.  Each step sends half of the values on.
@@ -325,6 +373,7 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
     // goes out from where z was.
     using Part = product::Region<8>;
     constexpr int kParts = S::kM / 2 * S::kN;
+    constexpr bool kHeld = std::is_same_v<T, _Float16>;
     static_assert(S::kM % 2 == 0 && 5 * Part::kSize <= kRoom, "");
     const bool slope = a.z, gated = a.gated;  // (without a z, dz is what the product gives)
     const bool whole = wave_row0 + 32 * S::kN <= a.m && wave_column0 + 32 * S::kM <= a.n;
@@ -340,7 +389,9 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
     auto bring_next = [&](int part) {
       if (gated) next.bring((const char*)a.z + 2 * n_bytes, z_bytes, row_of(part), a.m, column_of(part), a.n, lane);
     };
-    const float factor = a.parts ? scale_of(a.parts, a.n_parts, lane) : 1.f;
+    float factor = a.parts ? scale_of_products(a.parts, a.n_parts, lane) : 1.f, most = 0.f;
+    if (kHeld && a.again) factor = scale_again(factor, largest_of(a.found, lane));
+    const bool look = kHeld && a.parts && !a.again;
     if (a.parts && block == 0 && share == 0 && threadIdx.x == 0) *a.unscale = 1.f / factor;
     bring(0);
     bring_next(0);
@@ -384,6 +435,16 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] *= s[e];
         }
+        if (look) {  // (rows past the end are the last one again, with its z; of 8 columns all are there or none)
+          const int quarters = row_of(part) < a.m ? (a.n - column_of(part) - 32 * i) / 8 : 0;
+          float here = most_of(v, quarters);
+          if (gated) here = fmaxf(here, most_of(x, quarters));
+          if (here == INFINITY) {
+            here = finite_most_of(v, quarters);
+            if (gated) here = fmaxf(here, finite_most_of(x, quarters));
+          }
+          most = fmaxf(most, here);
+        }
         write(mine0, i, v);
         if (a.column_sums) {  // of dz before it is rounded, over the parts with these columns
 #pragma unroll
@@ -413,6 +474,11 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
           if (gated) sums[a.n + column] = other_sums[i];
         }
       }
+    }
+    if (look) {
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+      if (lane == 0) mark(a.found, most);
     }
   } else if constexpr (AFTER != After::kSums) {
     using Out = product::Region<4 * S::kM>;
@@ -478,6 +544,13 @@ template <class T, class S, Layout LAYOUT, After AFTER>
 __global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void linear_kernel(LinearParams a, Tiles t) {
   __shared__ u32x4 tiles[kWaveChunks<S, AFTER> * (S::kThreads / 64)];
   make_tile<T, S, LAYOUT, AFTER>(a, block_by_die(), t.m, t.n, tiles);
+}
+
+// float16: kSlope once more where dz leaves its range, with the scale that it takes; else nothing but the launch, 4 to 5 us.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads, S::kWavesPerSimd) void again_kernel(LinearParams a, Tiles t) {
+  __shared__ u32x4 tiles[kWaveChunks<S, After::kSlope> * (S::kThreads / 64)];
+  if (leaves_range(largest_of(a.found, threadIdx.x & 63))) make_tile<T, S, Layout::kWeightColumns, After::kSlope>(a, block_by_die(), t.m, t.n, tiles);
 }
 
 // Two products in one launch, neither of which fills the GPU: dx (or dz) and a gradient of weights; first the one whose workgroups take
@@ -616,12 +689,15 @@ hipError_t launch_linear(const LinearParams& a, Layout layout, After after, cons
 // The first by columns of the weights, kPlain or kSlope, the second by columns, kPlain; of one shape, medium or small.
 template <class T>
 hipError_t launch_pair(const LinearParams& a, After after, const LinearPlan& a_plan, const LinearParams& b, const LinearPlan& b_plan, hipStream_t stream);
+// Behind either of them, float16 only: a product of kSlope made again if it has to be.
+template <class T>
+hipError_t launch_again(const LinearParams& a, const LinearPlan& plan, hipStream_t stream);
 template <class T>
 hipError_t launch_joins(const Joins& joins, uint32_t blocks, hipStream_t stream);
 template <class T>
 hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t stream);
 // dz = dout a'(z), held times its scale, if there is a z, and unless they are null sums of its rows (times 1; with one share
-// to `total`, rounded), and the largest finite |dout| of each workgroup.
+// to `total`, rounded), and the largest finite |dout| of each workgroup, with zeros in `found` unless that is null.
 template <class T>
 hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_bytes, float* sums, void* total, int64_t shares, float* parts, hipStream_t stream);
 constexpr int kSlopeColumns = 64;  // of a workgroup there

@@ -118,8 +118,10 @@ __global__ __launch_bounds__(256) void slope_kernel(LinearParams a, const void* 
   float total[8], most = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) total[i] = 0.f;
-  const float factor = a.parts ? scale_of(a.parts, a.n_parts, threadIdx.x & 63) : 1.f;
+  const float factor = a.parts ? scale_of_slopes(a.parts, a.n_parts, threadIdx.x & 63) : 1.f;
   if (a.parts && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.unscale = 1.f / factor;
+  static_assert(kExponents == 256, "a word to a thread");
+  if (a.found && blockIdx.x == 0 && blockIdx.y == 0) a.found[threadIdx.x] = 0;
   if (c < a.n) {
     const int64_t begin = blockIdx.y * rows_per_share, end = min(begin + rows_per_share, (int64_t)a.m);
 #pragma unroll 4
@@ -183,6 +185,7 @@ hipError_t launch_slope(const LinearParams& a, const void* dout, int64_t dout_by
   slope_kernel<T><<<dim3((a.n + kSlopeColumns - 1) / kSlopeColumns, (uint32_t)shares), 256, 0, stream>>>(a, dout, dout_bytes, sums, (T*)total, rows_per_share, parts);
   return hipGetLastError();
 }
+
 // ---- tiles ----------------------------------------------------------------------------------------------------
 
 template <class S>
@@ -252,6 +255,24 @@ hipError_t launch_linear(const LinearParams& a, Layout layout, After after, cons
   if (e != hipSuccess) return e;
   p.n = a.n;
   return after == After::kForward ? launch_join<T, After::kForward>(p, stream) : launch_join<T, After::kGated>(p, stream);
+}
+
+template <class T, class S>
+hipError_t launch_again_of(const LinearParams& a, hipStream_t stream) {
+  const Tiles t = tiles_of<S>(a);
+  const int64_t blocks = (int64_t)t.m * t.n;
+  if (too_many<S>(blocks)) return hipErrorInvalidConfiguration;
+  again_kernel<T, S><<<(uint32_t)blocks, S::kThreads, 0, stream>>>(a, t);
+  return hipGetLastError();
+}
+template <class T>
+hipError_t launch_again(const LinearParams& a, const LinearPlan& plan, hipStream_t stream) {
+  LinearParams p = a;
+  p.shares = plan.shares;
+  p.share = plan.share;
+  p.again = true;
+  if (plan.shape == 0) return launch_again_of<T, Large>(p, stream);
+  return plan.shape == 1 ? launch_again_of<T, Medium>(p, stream) : launch_again_of<T, Small>(p, stream);
 }
 
 template <class T, class S, After FIRST>

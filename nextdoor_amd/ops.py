@@ -754,8 +754,8 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
                  needs=(True, True, True)):
     """(dx, dup, ddown, dup_bias, ddown_bias) for the gradient ``dout`` of ``out``; z and h are what the forward pass kept.  The
     residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None.  The gradient of z
-    is rounded to 16 bits before its products (float16: held times a power of two, so that small ones are not lost; it may be 255
-    times max |dout|, and what is more may become infinite)."""
+    is rounded to 16 bits before its products (float16: held times a power of two, so that small ones are not lost, and large ones do
+    not become infinite)."""
     index = _on_gpu("mlp", x, dout, up, down, h, *(() if z is None else (z,)))
     _types("mlp", x, dout, up, down, h)
     gated = bool(gated)

@@ -1,0 +1,173 @@
+"""Layer norm, linear maps and feed-forward parts on the GPU where their numbers go to the ends of the types, against their
+definitions in 64 bits (block_operators_reference.py)."""
+import math
+
+import pytest
+import torch
+
+from nextdoor_amd import ops
+from tests import block_operators_reference as ref
+from tests.test_gpu_block_operators import BF16, F16, F32, check_all, linear_case, map_cuda, mlp_case, normal, run_linear, run_mlp, run_norm, within
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("dx", "dup", "ddown", "dup_bias", "ddown_bias")
+
+
+# ---- float16: what the gradient of z is held times ------------------------------------------------------------
+
+
+def largest_dz(case):
+    """The largest finite gradient of z."""
+    x, up, down, up_bias, _, name, gated, _, d = [t.double() if isinstance(t, torch.Tensor) else t for t in case]
+    z = x @ up.T
+    if up_bias is not None:
+        z = z + up_bias
+    dh = d @ down
+    g = z[:, :down.shape[1]]
+    a, slope = ref.activation(g, name)
+    dz = torch.cat([dh * slope * z[:, down.shape[1]:], dh * a], 1) if gated else dh * slope
+    return float(dz.abs().max())
+
+
+def held_by(most):
+    """Half the smallest number, over what dz is held times: at least 1, and so much that max |dout| is 512 or more; where the largest
+    dz then is no number from 1 to 65504, so much that this is 2^14 or more."""
+    def held(d, least):
+        return least * max(float(d.abs().max()) / 512 if float(d.abs().max()) < 512 else 1.0, most / 2.0 ** 14)
+    return held
+
+
+def test_gradients_of_z_far_above_dout():
+    """One row whose dz is 4096 times dout, which float16 holds, as all the gradients made of it."""
+    x, up = torch.full((1, 8), 8.0).to(F16), torch.full((16, 8), 0.25).to(F16)
+    down, d = torch.full((512, 8), 0.5).to(F16), torch.ones(1, 512).to(F16)
+    got = run_mlp(x, up, down, None, None, "silu", True, None, d)
+    # g = u = 16, logistic(16) = 1 - 1.1e-7; dh = 256, dg = du = 4096 to 2e-6, which float16 rounds to 4096
+    assert got["dx"].tolist() == [[16 * 4096 * 0.25] * 8] and got["dup"].flatten().tolist() == [4096 * 8.0] * 128
+    assert got["dup_bias"].tolist() == [4096.0] * 16
+
+
+# both shapes of tile that a backward pass takes two products with in one launch, and all three that it takes alone
+HELD = [(5, 64, 256, 64), (300, 96, 136, 200), (2050, 64, 256, 64), (20483, 64, 256, 64), (4104, 64, 4096, 1000), (6400, 136, 448, 152)]
+
+
+@pytest.mark.parametrize("rows,dim,inner,out", HELD)
+@pytest.mark.parametrize("gated,name", [(True, "silu"), (False, "gelu"), (True, None), (False, None)])
+def test_rows_with_gradients_of_z_that_leave_the_range(rows, dim, inner, out, gated, name, monkeypatch):
+    """A few rows of large x, with large weights: dz is thousands of times the largest dout in them, and it fits, as dx does."""
+    print("held", rows, dim, inner, out, gated, name, flush=True)
+    case = mlp_case(rows, dim, inner, out, F16, name, gated)
+    x, d = case[0].float(), case[-1].float().clamp(-1, 1)
+    large = torch.arange(rows) % (rows // 4 + 1) == 0
+    x[large] *= 8 if gated else 1 / 16
+    d[~large] /= 16
+    # (without a gate dz is dh times a slope: that comes from larger weights alone)
+    down = (case[2].float() * (2048 if not gated else 256) * (inner / out) ** 0.5).to(F16)
+    case = map_cuda((x.to(F16), case[1], down, *case[3:-1], d.to(F16)))
+    most = largest_dz(case)
+    assert 2 ** 11 < most < 65504 and case[-1].abs().max() == 1
+    monkeypatch.setattr(ref, "_held", held_by(most))
+    want, off = ref.mlp(*case)
+    got = run_mlp(*case)
+    for n, t in got.items():
+        assert within(t, want[n], off[n]), n
+
+
+@pytest.mark.parametrize("rows", [40, 700, 5000])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("big", [1.0, 3e2, 6e4])
+def test_small_rows_of_a_feed_forward_part_next_to_large_ones(rows, gated, big):
+    """The gradients of rows 10^8 times smaller than the largest have the errors of a rounding or two."""
+    case = list(mlp_case(rows, 128, 256, 128, F16, "silu", gated, False, False))
+    d = case[-1].float().clamp(-1, 1)
+    d[::7] *= big
+    small = torch.arange(rows) % 7 != 0
+    d[small] *= 1e-3
+    case[-1] = d.to(F16)
+    want, got = ref.mlp(*case)[0], run_mlp(*case)
+    off = (got["dx"].cpu().double() - want["dx"])[small].norm() / want["dx"][small].norm()
+    # roundings of dz, of dx and of an ungated z (whose slopes change by less than it does), 2^-11 each at most; what of dz is below 2^-14
+    # times the scale (1/4 or more, with dz of 1e-3) is off by 2^-23 of 2^-10
+    assert off < 2.0 ** -9
+    assert big > 3e2 or torch.isfinite(got["dup"]).all()
+
+
+@pytest.mark.parametrize("rows", [40, 700, 5000])
+@pytest.mark.parametrize("gated", [True, False])
+def test_gradients_of_z_far_below_dout(rows, gated):
+    """Small weights behind z: the largest dz is below 1, where one row has a large dout."""
+    x, up, down, _, _, name, _, _, d = mlp_case(rows, 128, 256, 128, F16, "relu" if not gated else "silu", gated, False, False)
+    down = (down.float() * 2.0 ** -16).to(F16)
+    up = (up.float() * 16).to(F16)
+    d = d.float().clamp(-1, 1)
+    d[0] *= 1000 if gated else 20000
+    case = (x, up, down, None, None, name, gated, None, d.to(F16))
+    assert largest_dz(case) < 1
+    want, got = ref.mlp(*case)[0], run_mlp(*case)
+    for n, rest in (("dx", slice(1, None)), ("dup", slice(None))):
+        off = (got[n].cpu().double() - want[n])[rest].norm() / want[n][rest].norm()
+        assert off < 2.0 ** -9, n  # (as above)
+
+
+@pytest.mark.parametrize("big", [1.0, 3e2, 6e4])
+def test_small_rows_of_a_linear_map_next_to_large_ones(big):
+    x, w, b, name, r, d = linear_case(200, 128, 256, F16, "gelu")
+    d = d.float().clamp(-1, 1)
+    d[::2] *= big
+    d[1::2] *= 1e-3
+    d = d.to(F16)
+    want, got = ref.linear(x, w, b, name, r, d)[0], run_linear(x, w, b, name, r, d)
+    off = (got["dx"].cpu().double() - want["dx"])[1::2].norm() / want["dx"][1::2].norm()
+    assert off < 2.0 ** -9  # (roundings of dz, dx and z, as above)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_an_infinite_dout_leaves_the_others_their_gradients(rows, monkeypatch):
+    """Its row has infinities or NaN; the scale comes from the finite ones, also where they have to be scaled down."""
+    case = list(mlp_case(rows, 64, 128, 64, F16, "silu", True, False, False))
+    case[2] = (case[2].float() * 512).to(F16)
+    want, off = None, None
+    d = case[-1].float().clamp(-1, 1)
+    bad = d.clone()
+    bad[1, 5] = math.inf
+    d[1] = 0
+    case[-1] = d.to(F16)
+    monkeypatch.setattr(ref, "_held", held_by(largest_dz(case)))
+    want, off = ref.mlp(*case)
+    case[-1] = bad.to(F16)
+    got = run_mlp(*case)
+    rest = [i for i in range(rows) if i != 1]
+    assert not torch.isfinite(got["dx"][1]).any()
+    check_all({"dx": got["dx"][rest]}, {"dx": want["dx"][rest]}, {"dx": off["dx"][rest]}, "others")
+
+
+def test_a_step_that_is_held_anew_is_captured(monkeypatch):
+    """Two graphs, replayed in turn over inputs of which some need another scale than their dout's and some do not."""
+    case = map_cuda(mlp_case(300, 64, 256, 64, F16, "silu", True))
+    x, up, down, up_bias, down_bias, name, gated, r, d = case
+    down = down * 256
+    inputs = [(x * a, d * b) for a, b in ((1, 1), (0.125, 2.0 ** -8), (4, 1), (1, 2.0 ** -12))]
+
+    def step(x, d):
+        out, z, h = ops.mlp_forward(x, up, down, up_bias, down_bias, name, gated, r, keep=True)
+        return (out, *ops.mlp_backward(d, x, up, down, z, h, name, gated))
+    eager = [step(*i) for i in inputs]
+    again = [step(*i) for i in inputs]
+    bits = lambda t: t.view(torch.int16)
+    assert all(torch.equal(bits(s), bits(t)) for a, b in zip(eager, again) for s, t in zip(a, b))
+    gx, gd = torch.empty_like(x), torch.empty_like(d)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = step(gx, gd)
+        graphs.append((graph, results))
+    for turn in range(8):
+        gx.copy_(inputs[turn % 4][0])
+        gd.copy_(inputs[turn % 4][1])
+        graph, results = graphs[turn % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(bits(s), bits(t)) for s, t in zip(eager[turn % 4], results)), turn
+        step(*inputs[(turn + 1) % 4])
