@@ -428,7 +428,10 @@ int nd_linear_backward(const nd_linear* a, void* stream);
  * down^T + down_bias + residual.  up: [inner][dim], gated [2 inner][dim] (the rows of g, then those of u); down: [out_dim][inner].
  * h: [rows][inner], always written, and z unless it is NULL are what the backward call reads (z is not needed without an
  * activation and a gate).  z: [rows][inner] in 16 bits; gated: 6 inner bytes a row, 24 bits to each value of z.  Everything else
- * as for linear maps; dup_bias is of the gradient of z before it is rounded. */
+ * as for linear maps; dup_bias is of the gradient of z before it is rounded.  inner_filled, 0 to inner - 1: so many of the inner
+ * places, the last ones (gated: of either half), are there only because inner is a multiple of 8, and up, up_bias and down have zeros
+ * there.  h and the gradient of z are 0 in them whatever x and dout hold (0 times an infinity would be NaN), what z is there is not
+ * read. */
 typedef struct nd_mlp {
   int64_t rows;
   int32_t dim, inner, out_dim, dtype, activation, gated;
@@ -439,6 +442,7 @@ typedef struct nd_mlp {
   void *dx, *dup, *dup_bias, *ddown, *ddown_bias;
   void* workspace;
   int64_t workspace_bytes;
+  int32_t inner_filled;
 } nd_mlp;
 int64_t nd_mlp_workspace(const nd_mlp* a, int backward);
 int nd_mlp_forward(const nd_mlp* a, void* stream);

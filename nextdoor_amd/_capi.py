@@ -51,7 +51,7 @@ class Mlp(C.Structure):
                 [(n, C.c_int64) for n in ("x_row", "residual_row", "dout_row")] +
                 [(n, C.c_void_p) for n in ("x", "up", "up_bias", "down", "down_bias", "residual", "out", "z", "h", "dout", "dx",
                                            "dup", "dup_bias", "ddown", "ddown_bias", "workspace")] +
-                [("workspace_bytes", C.c_int64)])
+                [("workspace_bytes", C.c_int64), ("inner_filled", C.c_int32)])
 
 
 # name -> (restype, argtypes); every symbol include/nextdoor_amd.h declares

@@ -158,6 +158,14 @@ int64_t survey_shares(int64_t rows, int64_t columns, bool parts) {
 }
 int64_t survey_parts(int64_t rows, int64_t columns) { return survey_shares(rows, columns, true) * ((columns + kSlopeColumns - 1) / kSlopeColumns); }
 
+// Places `first` .. `end` - 1 of rows of 16-bit values become 0, in blockIdx.y = 1 those `other` places behind them: a launch that only
+// sizes which are no multiples of 8 cost, instead of comparisons in every tile (of which the largest spilled registers).
+__global__ __launch_bounds__(256) void clear_places_kernel(uint16_t* matrix, int64_t rows, int64_t row, int32_t first, int32_t end, int32_t other) {
+  const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (r >= rows) return;
+  for (int32_t i = first; i < end; ++i) matrix[r * row + blockIdx.y * (int64_t)other + i] = 0;
+}
+
 // ---- calls --------------------------------------------------------------------------------------------------------
 
 struct Call {
@@ -223,6 +231,13 @@ struct Call {
     note(bf16 ? launch_slope<__bf16>(a, dout, dout_bytes, parted, whole, shares, parts, stream)
               : launch_slope<_Float16>(a, dout, dout_bytes, parted, whole, shares, parts, stream));
     if (parted) join(sums, shares, a.n, nullptr, total);
+  }
+  // The places of h or dz (gated: of both halves) that are filled up.
+  void clear_filled(void* matrix, const nd_mlp* a, int halves) {
+    if (a->inner_filled == 0 || a->rows == 0) return;
+    clear_places_kernel<<<dim3((uint32_t)((a->rows + 255) / 256), halves), 256, 0, stream>>>((uint16_t*)matrix, a->rows, (int64_t)a->inner * halves,
+                                                                                          a->inner - a->inner_filled, a->inner, a->inner);
+    note(hipGetLastError());
   }
   // float16: dz made again where it leaves its range.
   void again(const LinearParams& a, const LinearPlan& plan) { note(launch_again<_Float16>(a, plan, stream)); }
@@ -442,6 +457,8 @@ std::string refuse(const nd_mlp* a) {
   if (!a) return "null argument";
   std::string why = refuse(a->rows, {a->dim, a->inner, a->out_dim}, a->dtype, a->activation, {a->x_row, a->residual_row, a->dout_row});
   if (why.empty() && a->gated && a->inner > ND_LINEAR_MAX_DIM / 2) why = "gated: at most " + number(ND_LINEAR_MAX_DIM / 2) + " inner places";
+  if (why.empty() && (a->inner_filled < 0 || a->inner_filled >= a->inner))
+    why = "between 0 and inner - 1 places are filled up, " + number(a->inner_filled) + " given";
   return why;
 }
 
@@ -476,6 +493,7 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
     p.out = a->h;
     p.z = a->z;
     call.forward(p, a->gated ? After::kGated : After::kForward, (float*)(work + w.forward));
+    call.clear_filled(a->h, a, 1);
     LinearParams r = {};
     r.p = a->down;
     r.p_bytes = inner_bytes;
@@ -518,6 +536,7 @@ int run_mlp(const nd_mlp* a, bool backward, void* stream) {
       gradient_of_weight(a->dout, dout_bytes, a->h, inner_bytes, a->rows, a->out_dim, a->inner, nullptr, a->ddown, (float*)(work + w.ddown));
   call.backward(first ? &p : nullptr, After::kSlope, a->ddown ? &ddown : nullptr, w.first);
   if (parts) call.again(p, w.first.first);
+  if (first) call.clear_filled(work + w.dz, a, a->gated ? 2 : 1);
   if (columns) call.join(columns, w.shares, wide, unscale, a->dup_bias);
   const char* dz = work + w.dz;
   const LinearParams dx = gradient_of_x(dz, wide_bytes, a->up, a->rows, wide, a->dim, unscale, a->dx, (float*)(work + w.dx));

@@ -718,8 +718,7 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
 
     z = x up^T + up_bias; gated: ``h = activation(g) u`` with ``g, u = z.chunk(2, -1)``, else ``h = activation(z)``.  x: [..., dim];
     up: [2 inner or inner, dim]; down: [out_dim, inner]; activations, types and sizes as in :func:`linear_forward`.  Both
-    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second.  Where inner is no
-multiple of 8, a row of x with infinities gives NaN."""
+    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second."""
     index = _on_gpu("mlp", x, up, down, *(t for t in (up_bias, down_bias, residual) if t is not None))
     _types("mlp", x, up, down, up_bias, down_bias, residual)
     gated = bool(gated)
@@ -741,11 +740,10 @@ multiple of 8, a row of x with infinities gives NaN."""
         z = x.new_empty((n, up.shape[0]))
     a = Mlp(n, up.shape[1], down.shape[1], wide, _DTYPES[x.dtype], code, gated, x_row, residual_row, 0, rows.data_ptr(), up.data_ptr(),
             _pointer(up_bias), down.data_ptr(), _pointer(down_bias), _pointer(residual), out.data_ptr(), _pointer(z), h.data_ptr())
+    a.inner_filled = down.shape[1] - inner
     workspace = _room(a, _library().nd_mlp_workspace(a, 0), x.device)
     _run(index, _library().nd_mlp_forward, a)
     del workspace
-    if z is not None and inner % 8:  # (as in linear_forward; gated: the upper 16 bits of both halves)
-        (z.view(torch.int16).view(n, 3, up.shape[0] // 2)[:, :2, inner:] if gated else z[:, inner:]).zero_()
     out = _shaped(out, n, out_dim, shape)
     return (out, z, h) if keep else out
 
@@ -778,6 +776,7 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
     a = Mlp(n, up.shape[1], down.shape[1], down.shape[0], _DTYPES[x.dtype], code, gated, x_row, 0, dout_row, rows.data_ptr(), up.data_ptr(),
             None, down.data_ptr(), None, None, None, _pointer(z), h.data_ptr(), dout.data_ptr(), _pointer(dx), _pointer(dup),
             _pointer(dup_bias), _pointer(ddown), _pointer(ddown_bias))
+    a.inner_filled = down.shape[1] - inner
     workspace = _room(a, _library().nd_mlp_workspace(a, 1), x.device)
     _run(index, _library().nd_mlp_backward, a)
     del workspace

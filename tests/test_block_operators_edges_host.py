@@ -3,7 +3,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from nextdoor_amd import ops
+from nextdoor_amd import _capi, ops
+from tests.test_block_operators_host import mlp_call, refused
 
 
 @pytest.fixture
@@ -42,3 +43,12 @@ def test_forward_mode_derivatives_are_refused_and_not_lost(without_kernels, whic
         with pytest.raises(RuntimeError):
             torch.func.jvp(of, (at,), (at,))
         assert call(x, w).shape == (4, 8) and not call(x, w).requires_grad
+
+
+@pytest.mark.parametrize("filled", [-1, 128, 1 << 20])
+def test_more_filled_up_places_than_there_are_is_refused(filled):
+    lib = _capi.lib()
+    for fn in (lib.nd_mlp_forward, lib.nd_mlp_backward):
+        refused(fn, mlp_call(inner_filled=filled), "filled up")
+    assert lib.nd_mlp_workspace(mlp_call(inner_filled=filled), 0) == -1
+    assert lib.nd_mlp_workspace(mlp_call(inner_filled=7), 1) == lib.nd_mlp_workspace(mlp_call(), 1) > 0

@@ -171,3 +171,30 @@ def test_a_step_that_is_held_anew_is_captured(monkeypatch):
         torch.cuda.synchronize()
         assert all(torch.equal(bits(s), bits(t)) for s, t in zip(eager[turn % 4], results)), turn
         step(*inputs[(turn + 1) % 4])
+
+
+# ---- sizes that are filled up -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows,dim", [(3, 64), (100, 64), (700, 136), (70, 4096)])
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_infinite_rows_of_a_part_whose_inner_size_is_filled_up(rows, dim, gated, dtype):
+    """Of positive numbers all that a row with an infinity makes is infinite, and NaN nowhere: places that are filled up add 0."""
+    inner, out = 13, 24
+    x, d = normal(1, rows, dim).abs(), normal(2, rows, out).abs()
+    up, down = normal(3, inner * (1 + gated), dim, std=dim ** -0.5).abs() + 0.01, normal(4, out, inner, std=0.25).abs() + 0.01
+    x, d, up, down = (t.to(dtype) for t in (x, d, up, down))
+    case = [x, up, down, None, None, "relu", gated, None, d]
+    want, off = ref.mlp(*case)
+    case[0] = x.clone()
+    case[0][1, 5] = math.inf
+    rest = [i for i in range(rows) if i != 1]
+    out_ = run_mlp(*case)["out"]
+    assert (out_[1] == math.inf).all()
+    check_all({"out": out_[rest]}, {"out": want["out"][rest]}, {"out": off["out"][rest]}, "out")
+    case[0], case[-1] = x, d.clone()
+    case[-1][1, 7] = math.inf
+    dx = run_mlp(*case)["dx"]
+    assert (dx[1] == math.inf).all()
+    check_all({"dx": dx[rest]}, {"dx": want["dx"][rest]}, {"dx": off["dx"][rest]}, "dx")
