@@ -113,11 +113,24 @@ __device__ __forceinline__ float2 row_sums(float2 v, float2 (*scratch)[THREADS /
     const int wave = threadIdx.x >> 6, first = wave / kWaves * kWaves;
     if ((threadIdx.x & 63) == 0) scratch[turn & 1][wave] = v;
     __syncthreads();  // (two arrays in turn: this one is written again only after the barrier of the next call)
+    // (four at a time, those in pairs, so that the chain of roundings is not as long as the waves are many; in pairs of all sixteen the longest
+    // rows' gradients spilled registers)
+    constexpr int kAtOnce = kWaves < 4 ? kWaves : 4;
     v = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int w = 0; w < kWaves; ++w) {
-      v.x += scratch[turn & 1][first + w].x;
-      v.y += scratch[turn & 1][first + w].y;
+#pragma unroll 1
+    for (int w = 0; w < kWaves; w += kAtOnce) {
+      float2 s[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) s[i] = scratch[turn & 1][first + w + i];
+#pragma unroll
+      for (int d = kAtOnce / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < d; ++i) {
+          s[i].x += s[i + d].x;
+          s[i].y += s[i + d].y;
+        }
+      v.x += s[0].x;
+      v.y += s[0].y;
     }
   }
   return v;

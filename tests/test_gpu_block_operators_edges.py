@@ -198,3 +198,21 @@ def test_infinite_rows_of_a_part_whose_inner_size_is_filled_up(rows, dim, gated,
     dx = run_mlp(*case)["dx"]
     assert (dx[1] == math.inf).all()
     check_all({"dx": dx[rest]}, {"dx": want["dx"][rest]}, {"dx": off["dx"][rest]}, "dx")
+
+
+# ---- rows of layer norm -----------------------------------------------------------------------------------------
+
+
+def test_the_mean_of_a_row_whose_sum_loses_a_half_step_at_every_addition():
+    """1 and, for every addition on its way, what one alone leaves no trace of: 15 places of a lane, 6 pairings of a wave's
+    lanes, and the other 15 waves.  A row of 16384 numbers: lanes have runs of four, 4096 places apart."""
+    x = torch.zeros(1, 16384)
+    x[0, [4096 * turn + i for turn in range(4) for i in range(4)]] = 2.0 ** -24
+    x[0, [4 * lane for lane in (1, 2, 4, 8, 16, 32)]] = 2.0 ** -24
+    x[0, [4 * 64 * wave for wave in range(1, 16)]] = 2.0 ** -24
+    x[0, 0] = 1
+    want, off = ref.layer_norm(x)
+    mean = ops.layer_norm_forward(x.cuda())[1]
+    check_all({"mean": mean}, want, off, "mean")
+    # the waves' sums are added four at a time, those in pairs: 15 + 6 + 2 + 3 half steps at most
+    assert abs(float(mean) * 16384 - float(x.double().sum())) <= 26 * 2.0 ** -24
