@@ -297,21 +297,23 @@ struct NormShape {
 };
 constexpr NormShape kNormShapes[] = {{64, 8, 128}, {128, 16, 64}, {256, 32, 32}, {512, 64, 16}, {1024, 128, 8}, {2048, 256, 4}, {4096, 512, 2}, {8192, 1024, 1}, {16384, 1024, 1}};
 constexpr int kForwardLanes = 1 << 19, kBackwardBlocks = 256;
-constexpr int kAlone = 6;  // times at most that one workgroup takes the next rows: less than another launch, which adds up sums, costs
+// Times at most that one workgroup takes the next rows: less than another launch, which adds up sums, costs where a program makes each call
+// (48 x 1024 13.1 us for 15.7, 4 x 16384 18 for 21.5; in a graph 12.9 for 8.7 and 18 for 21.3).
+constexpr int kAlone = 6;
 int shape_of(int32_t dim) {
   int i = 0;
   while (dim > kNormShapes[i].most) ++i;
   return i;
 }
-int64_t backward_blocks(int64_t rows, int32_t dim) {
+int64_t backward_blocks(int64_t rows, int32_t dim, bool weights) {  // (for dx alone there is no such launch: 48 x 1024 5.0 us for 11.2, 6 x 16384 4.4 for 16)
   const int at_once = kNormShapes[shape_of(dim)].rows;
-  if (rows <= kAlone * at_once) return 1;
+  if (weights && rows <= kAlone * at_once) return 1;
   return std::max<int64_t>(1, std::min<int64_t>(kBackwardBlocks, (rows + at_once - 1) / at_once));
 }
 
 template <class T, int LANES, int VALUES, Runs RUNS>
 void launch_backward(const NormParams& p, hipStream_t stream) {
-  const uint32_t blocks = (uint32_t)backward_blocks(p.rows, p.dim);
+  const uint32_t blocks = (uint32_t)backward_blocks(p.rows, p.dim, p.sums || p.dweight || p.dbias);
   norm_backward_kernel<T, LANES, VALUES, 1024, VALUES == 8 && sizeof(T) == 2 ? 2 : 1, RUNS><<<blocks, 1024, 0, stream>>>(p);
 }
 template <class T, int LANES, int VALUES, Runs RUNS>
@@ -355,8 +357,9 @@ void launch_norm(const NormParams& p, bool backward, hipStream_t stream) {
 }
 
 int64_t norm_workspace(const nd_layer_norm* a) {
-  const int64_t blocks = backward_blocks(a->rows, a->dim);
-  return (a->dweight || a->dbias) && blocks > 1 ? blocks * 2 * a->dim * 4 : 0;
+  if (!a->dweight && !a->dbias) return 0;
+  const int64_t blocks = backward_blocks(a->rows, a->dim, true);
+  return blocks > 1 ? blocks * 2 * a->dim * 4 : 0;
 }
 
 std::string refuse(const nd_layer_norm* a) {
@@ -421,7 +424,7 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
   else launch_norm<__bf16>(p, backward, (hipStream_t)stream);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.sums) {
-    const int64_t blocks = backward_blocks(a->rows, a->dim), columns = 2 * a->dim;
+    const int64_t blocks = backward_blocks(a->rows, a->dim, true), columns = 2 * a->dim;
     const hipStream_t s = (hipStream_t)stream;
     if (a->weight_dtype == ND_F32) e = column_join<float>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);
     else if (a->weight_dtype == ND_F16) e = column_join<_Float16>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);

@@ -216,3 +216,12 @@ def test_the_mean_of_a_row_whose_sum_loses_a_half_step_at_every_addition():
     check_all({"mean": mean}, want, off, "mean")
     # the waves' sums are added four at a time, those in pairs: 15 + 6 + 2 + 3 half steps at most
     assert abs(float(mean) * 16384 - float(x.double().sum())) <= 26 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 64), (100, 64), (768, 64), (769, 64), (48, 1024), (49, 1024), (6, 8192), (5000, 4096), (40007, 24), (3001, 1000)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_gradient_of_rows_alone_is_that_of_all_three_together(rows, dim, dtype):
+    x, w, d = normal(1, rows, dim, dtype=dtype).cuda(), normal(2, dim, dtype=dtype).cuda(), normal(3, rows, dim, dtype=dtype).cuda()
+    _, mean, rstd = ops.layer_norm_forward(x, w)
+    alone = ops.layer_norm_backward(d, x, w, mean, rstd, (True, False, False))[0]
+    assert torch.equal(alone, ops.layer_norm_backward(d, x, w, mean, rstd)[0])
