@@ -751,10 +751,11 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
 def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up_bias=True, with_down_bias=True,
                  needs=(True, True, True)):
     """(dx, dup, ddown, dup_bias, ddown_bias) for the gradient ``dout`` of ``out``; z and h are what the forward pass kept.  The
-    residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None.  The gradient of z
+    residual's gradient is ``dout`` itself.  ``needs``: whether dx, dup and ddown are wanted; what is not is None (ddown alone reads h, dx,
+    dup and dup_bias read z: what nothing reads may be None).  The gradient of z
     is rounded to 16 bits before its products (float16: held times a power of two, so that small ones are not lost, and large ones do
     not become infinite)."""
-    index = _on_gpu("mlp", x, dout, up, down, h, *(() if z is None else (z,)))
+    index = _on_gpu("mlp", x, dout, up, down, *(t for t in (z, h) if t is not None))
     _types("mlp", x, dout, up, down, h)
     gated = bool(gated)
     dim, inner, out_dim, code = _mlp_arguments(x, up, down, None, None, activation, gated)
@@ -763,18 +764,18 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
     dout, dout_row = _vectors_in_place(dout, out_dim)
     up, down = _up(up, inner, gated), _matrix(down)
     n = rows.shape[0]
-    if not (h.shape == (n, down.shape[1]) and h.is_contiguous()):
+    if needs[2] if h is None else not (h.shape == (n, down.shape[1]) and h.is_contiguous()):
         raise NextDoorError("mlp: h is not what a forward pass kept")
     if gated or code:
         kept = ((n, 3 * up.shape[0]), torch.uint8) if gated else ((n, up.shape[0]), x.dtype)
-        if z is None or (z.shape, z.dtype) != kept or not z.is_contiguous():
+        if needs[0] or needs[1] or with_up_bias if z is None else (z.shape, z.dtype) != kept or not z.is_contiguous():
             raise NextDoorError("mlp: z is not what a forward pass kept")
 
     dx = _result(x, x.shape, n, up.shape[1]) if needs[0] else None
     dup, ddown = torch.empty_like(up) if needs[1] else None, torch.empty_like(down) if needs[2] else None
     dup_bias, ddown_bias = x.new_empty(up.shape[0]) if with_up_bias else None, x.new_empty(down.shape[0]) if with_down_bias else None
     a = Mlp(n, up.shape[1], down.shape[1], down.shape[0], _DTYPES[x.dtype], code, gated, x_row, 0, dout_row, rows.data_ptr(), up.data_ptr(),
-            None, down.data_ptr(), None, None, None, _pointer(z), h.data_ptr(), dout.data_ptr(), _pointer(dx), _pointer(dup),
+            None, down.data_ptr(), None, None, None, _pointer(z), _pointer(h), dout.data_ptr(), _pointer(dx), _pointer(dup),
             _pointer(dup_bias), _pointer(ddown), _pointer(ddown_bias))
     a.inner_filled = down.shape[1] - inner
     workspace = _room(a, _library().nd_mlp_workspace(a, 1), x.device)
@@ -787,10 +788,12 @@ def mlp_backward(dout, x, up, down, z, h, activation="silu", gated=True, with_up
 class _Mlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, up, down, up_bias, down_bias, activation, gated, residual):
-        keep = any(ctx.needs_input_grad[:5])
+        needs = ctx.needs_input_grad
+        first = needs[0] or needs[1] or needs[3]  # (what of z and h no gradient reads is not kept)
+        keep = first or needs[2]
         got = mlp_forward(x, up, down, up_bias, down_bias, activation, gated, residual, keep)
         out, z, h = got if keep else (got, None, None)
-        ctx.save_for_backward(x, up, down, z, h)
+        ctx.save_for_backward(x, up, down, z if first else None, h if needs[2] else None)
         ctx.how = activation, gated
         return out
 

@@ -225,3 +225,40 @@ def test_the_gradient_of_rows_alone_is_that_of_all_three_together(rows, dim, dty
     _, mean, rstd = ops.layer_norm_forward(x, w)
     alone = ops.layer_norm_backward(d, x, w, mean, rstd, (True, False, False))[0]
     assert torch.equal(alone, ops.layer_norm_backward(d, x, w, mean, rstd)[0])
+
+
+# ---- autograd and the model ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("gated", [True, False])
+def test_nothing_of_the_inner_size_is_kept_for_what_dout_alone_gives(rows, gated):
+    x, up, down, up_bias, down_bias, name, _, r, d = map_cuda(mlp_case(rows, 64, 128, 64, BF16, "silu", gated))
+    for wanted in ((down_bias,), (r,), (down_bias, r)):
+        for t in (down_bias, r):
+            t.grad = None
+            t.requires_grad_(any(t is w for w in wanted))
+        y = ops.mlp(x, up, down, up_bias, down_bias, name, gated, r)
+        assert all(t is None or t.shape != (rows, 128) and t.dtype is BF16 for t in y.grad_fn.saved_tensors)
+        y.backward(d)
+        for t, right in ((down_bias, d.double().sum(0)), (r, d.double())):
+            assert (t.grad is not None) == any(t is w for w in wanted)
+            if t.grad is not None:
+                assert ((t.grad.double() - right).abs() <= 2.0 ** -8 * right.abs() + (rows + 8) * 2.0 ** -24 * d.double().abs().sum(0)).all()
+        down_bias.requires_grad_(False)
+        r.requires_grad_(False)
+
+
+def test_z_and_h_are_asked_for_where_a_gradient_reads_them():
+    x, up, down, _, _, name, _, _, d = map_cuda(mlp_case(70, 64, 128, 64))
+    _, z, h = ops.mlp_forward(x, up, down, keep=True)
+    every = ops.mlp_backward(d, x, up, down, z, h)
+    assert torch.equal(ops.mlp_backward(d, x, up, down, None, h, "silu", True, False, True, (False, False, True))[2], every[2])
+    got = ops.mlp_backward(d, x, up, down, z, None, "silu", True, True, False, (True, True, False))
+    assert all(torch.equal(got[i], every[i]) for i in (0, 1, 3))
+    assert torch.equal(ops.mlp_backward(d, x, up, down, None, None, "silu", True, False, True, (False, False, False))[4], every[4])
+    for a, b, up_bias, needs, which in ((None, h, False, (True, False, False), "z"), (None, h, False, (False, True, False), "z"),
+                                        (None, h, True, (False, False, False), "z"), (z, None, False, (False, False, True), "h"),
+                                        (z[1:], h, False, (False, False, False), "z"), (z, h[1:], False, (False, False, False), "h")):
+        with pytest.raises(ops.NextDoorError, match="%s is not what" % which):
+            ops.mlp_backward(d, x, up, down, a, b, "silu", True, up_bias, True, needs)
