@@ -173,6 +173,40 @@ def test_a_step_that_is_held_anew_is_captured(monkeypatch):
         step(*inputs[(turn + 1) % 4])
 
 
+# ---- every row of a sum counts ----------------------------------------------------------------------------------
+# Bounds element by element allow what all roundings could add up to, which for a gradient of weights grows with the rows, its
+# values with their root: of these norms a round of 64 rows that is left out is 6 % or more.
+
+
+def far(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("rows,dim,out", [(13553, 136, 544), (10768, 136, 584), (12017, 2048, 136), (5684, 136, 11280), (4104, 1000, 4096), (958, 528, 16008)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_linear_gradients_leave_no_rows_out(rows, dim, out, dtype):
+    print("norms", rows, dim, out, dtype, flush=True)
+    x, w, b, name, r, d = map_cuda(linear_case(rows, dim, out, dtype, "silu"))
+    want = ref.linear(x, w, b, name, r, d)[0]
+    y, z = ops.linear_forward(x, w, b, name, r, keep=True)
+    # roundings of z, dz and the result, of a step's half each; they are as random as the values, and add up like them
+    unit = 2.0 ** -8 if dtype is BF16 else 2.0 ** -11
+    for got in (ops.linear_backward(d, x, w, z, name), ops.linear_backward(d, x, w, z, name, True, (False, True))):
+        for n, t in zip(("dx", "dweight", "dbias"), got):
+            assert t is None or far(t, want[n]) < 3 * unit, n
+    assert far(y, want["out"]) < 2 * unit
+
+
+@pytest.mark.parametrize("rows,dim,inner,out", [(20483, 64, 256, 64), (6400, 136, 448, 152), (4104, 64, 4096, 1000), (4104, 1000, 4096, 64), (2581, 3480, 8, 8)])
+@pytest.mark.parametrize("gated", [True, False])
+def test_feed_forward_gradients_leave_no_rows_out(rows, dim, inner, out, gated):
+    print("norms", rows, dim, inner, out, gated, flush=True)
+    case = map_cuda(mlp_case(rows, dim, inner, out, BF16, "silu", gated, residual=False))
+    want, got = ref.mlp(*case)[0], run_mlp(*case)
+    for n, t in got.items():
+        assert far(t, want[n]) < 3 * 2.0 ** -8, n  # (as above; of out and ddown: h and the result)
+
+
 # ---- sizes that are filled up -------------------------------------------------------------------------------------
 
 
