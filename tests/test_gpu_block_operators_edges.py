@@ -296,3 +296,37 @@ def test_z_and_h_are_asked_for_where_a_gradient_reads_them():
                                         (z[1:], h, False, (False, False, False), "z"), (z, h[1:], False, (False, False, False), "h")):
         with pytest.raises(ops.NextDoorError, match="%s is not what" % which):
             ops.mlp_backward(d, x, up, down, a, b, "silu", True, up_bias, True, needs)
+
+
+def test_every_step_of_the_gated_walk_model_has_the_gradients_of_a_model_that_never_ran():
+    """Nothing of the steps before is left in what a step computes; the first step's gradients are tested against the definitions."""
+    import copy
+    import numpy as np
+    from nextdoor_amd import walk_model
+    torch.manual_seed(3)
+    n = 211
+    rng = np.random.default_rng(4)
+    model = walk_model.WalkModel(n, width=64, heads=2, kv_heads=1, layers=2, dropout=0.1, gated=True).to("cuda", BF16)
+    optimizer = torch.optim.SGD(model.parameters(), lr=0.05)
+    for turn in range(4):
+        samples = rng.integers(0, n, (40 + 30 * turn, 25)).astype(np.int32)
+        for walk in samples[::3]:
+            walk[rng.integers(0, 25):] = n
+        tokens, targets, starts = walk_model.pack_walks(rng.integers(0, n, len(samples)), samples, n)
+        batch = walk_model.batch_of(tokens, targets, starts)
+        fresh = walk_model.WalkModel(n, width=64, heads=2, kv_heads=1, layers=2, dropout=0.1, gated=True).to("cuda", BF16)
+        fresh.load_state_dict(copy.deepcopy(model.state_dict()))
+        losses = []
+        for m in (fresh, model):
+            m.zero_grad()
+            each = m(*batch[:3], batch[3], 17 + turn)
+            each.mean().backward()
+            losses.append(each.detach())
+        assert torch.equal(*losses)
+        for (name, a), b in zip(model.named_parameters(), fresh.parameters()):
+            assert a.grad.abs().max() > 0, name
+            if name.startswith("blocks") or name.startswith("norm"):
+                assert torch.equal(a.grad, b.grad), (turn, name)
+            else:  # (torch adds up the embeddings' gradients, in an order that it does not promise)
+                assert far(a.grad, b.grad) < 2.0 ** -8, (turn, name)
+        optimizer.step()
