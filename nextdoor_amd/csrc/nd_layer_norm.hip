@@ -426,9 +426,9 @@ int run_norm(const nd_layer_norm* a, bool backward, void* stream) {
   if (e == hipSuccess && p.sums) {
     const int64_t blocks = backward_blocks(a->rows, a->dim, true), columns = 2 * a->dim;
     const hipStream_t s = (hipStream_t)stream;
-    if (a->weight_dtype == ND_F32) e = column_join<float>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);
-    else if (a->weight_dtype == ND_F16) e = column_join<_Float16>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);
-    else e = column_join<__bf16>(p.sums, blocks, columns, nullptr, a->dweight, a->dim, a->dbias, s);
+    if (a->weight_dtype == ND_F32) e = column_join<float>(p.sums, blocks, columns, a->dweight, a->dim, a->dbias, s);
+    else if (a->weight_dtype == ND_F16) e = column_join<_Float16>(p.sums, blocks, columns, a->dweight, a->dim, a->dbias, s);
+    else e = column_join<__bf16>(p.sums, blocks, columns, a->dweight, a->dim, a->dbias, s);
   }
   if (e != hipSuccess) return fail(std::string("layer norm: ") + hipGetErrorString(e));
   return 0;

@@ -113,14 +113,14 @@ __device__ __forceinline__ void wait_for_loads() {
   static_assert(N < 64, "");
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
-// The same for `tiles` (at most MOST) times EACH loads and MORE besides.
-template <int EACH, int MOST, int MORE = 0>
+// The same for `tiles` (at most MOST) times EACH loads.
+template <int EACH, int MOST>
 __device__ __forceinline__ void wait_for_tiles(int tiles) {
   if constexpr (MOST <= 0) {
-    wait_for_loads<MORE>();
+    wait_for_loads<0>();
   } else {
-    if (tiles >= MOST) wait_for_loads<EACH * MOST + MORE>();
-    else wait_for_tiles<EACH, MOST - 1, MORE>(tiles);
+    if (tiles >= MOST) wait_for_loads<EACH * MOST>();
+    else wait_for_tiles<EACH, MOST - 1>(tiles);
   }
 }
 // All waves are here.
