@@ -128,6 +128,17 @@ __device__ __forceinline__ float finite_most_of(const float (&v)[16], int quarte
   return most_of(finite, quarters);
 }
 
+// z as it is kept.  float16: what is positive stays so, for that is what a relu's slope is read from (below 2^-25 it was rounded to 0: one
+// in 10^8 of normal values, and with it a slope of 0 for 1).
+template <class T, int N>
+__device__ __forceinline__ void keep_sign(int activation, const float (&v)[N], float (&z)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i] = v[i];
+  if (!std::is_same_v<T, _Float16> || activation != ND_RELU) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i] = v[i] > 0.f ? fmaxf(v[i], 0x1p-24f) : v[i];
+}
+
 // The sums of 16 values over the 32 lanes of a half: lane l has that of value l & 15.  Each step sends half of the values on.
 __device__ __forceinline__ float sums_of_rows(const float (&v)[16], int lane) {
   auto other = [](float x, auto how) { return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), decltype(how)::value, 0xf, 0xf, true)); };
@@ -174,7 +185,10 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
     }
   }
   if (AFTER == After::kForward) {
-    if (a.z) *at(a.z, n_bytes, c) = pack(v);
+    if (a.z) {
+      keep_sign<T>(a.activation, v, x);
+      *at(a.z, n_bytes, c) = pack(x);
+    }
     activate(a.activation, v);
     if (a.residual) {
       unpack(*at(a.residual, a.residual_bytes, c), x);
@@ -517,7 +531,10 @@ __device__ __forceinline__ void make_tile(const LinearParams& a, uint32_t block,
         values(acc[i][j], v);
         if (AFTER == After::kForward) {
           if (a.bias) add_bias(bias[i], v);
-          if (keep) write(second, i, v);
+          if (keep) {
+            keep_sign<T>(a.activation, v, x);
+            write(second, i, x);
+          }
           activate(a.activation, v);
           if (residual) {
             read(first, i, x);

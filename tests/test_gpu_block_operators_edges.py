@@ -330,3 +330,24 @@ def test_every_step_of_the_gated_walk_model_has_the_gradients_of_a_model_that_ne
             else:  # (torch adds up the embeddings' gradients, in an order that it does not promise)
                 assert far(a.grad, b.grad) < 2.0 ** -8, (turn, name)
         optimizer.step()
+
+
+@pytest.mark.parametrize("rows,dim", [(3, 64), (50, 64), (100, 64), (70, 4096), (2500, 520)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_slopes_of_positive_numbers_that_16_bits_do_not_hold(rows, dim, dtype):
+    """z of 2^-28 and -2^-28: the slopes of a relu are 1 and 0."""
+    x, w = torch.zeros(rows, dim), torch.zeros(40, dim)
+    x[:, 3], w[:, 3] = 2.0 ** -14, 2.0 ** -14
+    x[::2] *= -1
+    x, w, d = x.to(dtype).cuda(), w.to(dtype).cuda(), torch.full((rows, 40), 0.5, dtype=dtype).cuda()
+    slope = (torch.arange(rows) % 2).double()
+    out, z = ops.linear_forward(x, w, None, "relu", keep=True)
+    dx, dw, db = ops.linear_backward(d, x, w, z, "relu")
+    # 40 products 0.5 x 2^-14; 0.5 x 2^-14 of every second row; 0.5 of those: sums that 32 bits hold
+    assert torch.equal(dx[:, 3].cpu().double(), 40 * 0.5 * 2.0 ** -14 * slope)
+    assert dw[:, 3].tolist() == [float(torch.tensor(0.5 * 2.0 ** -14 * int(slope.sum())).to(dtype))] * 40
+    assert db.tolist() == [float(torch.tensor(0.5 * int(slope.sum())).to(dtype))] * 40
+    assert out.abs().max() <= 2.0 ** -28  # (float16: 0)
+    out, z, h = ops.mlp_forward(x, w, torch.ones(8, 40, dtype=dtype).cuda(), activation="relu", gated=False, keep=True)
+    dx = ops.mlp_backward(torch.full((rows, 8), 0.25, dtype=dtype).cuda(), x, w, torch.ones(8, 40, dtype=dtype).cuda(), z, h, "relu", False)[0]
+    assert torch.equal(dx[:, 3].cpu().double(), 40 * 2 * 2.0 ** -14 * slope)
