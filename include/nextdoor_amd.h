@@ -426,7 +426,7 @@ int nd_linear_backward(const nd_linear* a, void* stream);
 
 /* A feed-forward part: z = x up^T + up_bias, h = activation(z) (gated == 0) or, of z = [g, u], activation(g) u (gated != 0), out = h
  * down^T + down_bias + residual.  up: [inner][dim], gated [2 inner][dim] (the rows of g, then those of u); down: [out_dim][inner].
- * h: [rows][inner], always written, and z unless it is NULL are what the backward call reads (z is not needed without an
+ * h: [rows][inner], rounded to 16 bits (ND_F16: an infinity from 65520 on), always written, and z unless it is NULL are what the backward call reads (z is not needed without an
  * activation and a gate).  z: [rows][inner] in 16 bits; gated: 6 inner bytes a row, 24 bits to each value of z.  Everything else
  * as for linear maps; dup_bias is of the gradient of z before it is rounded.  inner_filled, 0 to inner - 1: so many of the inner
  * places, the last ones (gated: of either half), are there only because inner is a multiple of 8, and up, up_bias and down have zeros

@@ -7,8 +7,9 @@
 // mean is known.  LANES lanes have a row, each VALUES of its places; a workgroup has a number of rows at a time and asks for the next
 // ones before it sums those it has.  w and b, and in the backward pass the sums for dw and db, stay in registers over all rows of a
 // workgroup; another kernel adds the workgroups' sums.  Forward and backward, in 16 bits 8192 x 1024: 10 and 16 us (3.2 TB/s, of which
-// the start of workgroups and the last rows' sums are a third), 16384 x 4096: 50 and 93 (5.4 and 4.3 TB/s); in 32 bits 20011 x 1021: 32
-// and 42 (5.1 and 5.8, some of it from the last cache); the sums' kernel 4 to 5.
+// the start of workgroups and the last rows' sums are a third), 16384 x 4096: 48 and 87 (5.6 and 4.6 TB/s); in 32 bits 20011 x 1021: 32
+// and 42 (5.1 and 5.8, some of it from the last cache); the sums' kernel 4 to 5.  Rows of fewer than 64 values leave lanes without places:
+// 128 MiB of rows of 32, 16 and 8 16-bit values 4.1, 2.5 and 1.4 TB/s forward, 4.4, 2.8 and 1.6 backward.
 #include "../../include/nextdoor_amd.h"
 
 #include <math.h>

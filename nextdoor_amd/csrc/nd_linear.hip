@@ -189,8 +189,8 @@ struct Call {
     }
     LinearParams p = a;
     p.sums = sums;
-    // What the caches do not hold until the backward pass is written past them (8192 x 2 x 5632 at 3 bytes, 368 us and 346; 3001 x 2 x
-    // 1000, both passes, 87 and 89), gated only where rows of its three parts begin with half lines: other pieces of 64 bytes are better put
+    // What the caches do not hold until the backward pass is written past them (8192 x 2 x 5632 at 3 bytes, 354 us and 351, and the product
+    // behind it, which finds its operands there, 155 and 143; 3001 x 2 x 1000, both passes, 87 and 89), gated only where rows of its three parts begin with half lines: other pieces of 64 bytes are better put
     // together in the caches (both passes, 26020 x 2 x 456 175 us and 157, 8192 x 2 x 2728 594 and 562; 18436 x 2 x 1056 272 and 274, and
     // 30000 x 1000 without a gate 158 and 161).
     p.z_later = a.z && (int64_t)a.m * a.n * (after == After::kGated ? 6 : 2) > kCaches && (after != After::kGated || a.n % 32 == 0);

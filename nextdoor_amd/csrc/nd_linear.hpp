@@ -213,9 +213,11 @@ __device__ __forceinline__ void finish(const LinearParams& a, int row, int c, fl
 
 // 256 x 256, eight waves with 4 x 2 results each, alone on a compute unit; 256 rows of C x 192 columns, which leaves fewer compute
 // units without work at the end of some sizes; 128 x 128 and 64 x 64, two and three of which share a compute unit.  Turns of large
-// tiles run at 1.3 to 1.36 PFLOP/s (8192 x 8192 x 8192: 810 us; the library's large product: 1.55 to 1.6 by rows), with the matrix cores
-// busy 75 % of the time at the 1.7 GHz that the power allows.  What follows a tile is not hidden: all workgroups store at once (8192 x
-// 1024 -> 4096: 66 us, 74 with a gelu, 86 with z too).  Within 2 % either way: four waves with 4 x 4 results, a third stage for P, two
+// tiles run at 1.25 to 1.37 PFLOP/s (8192 x 8192 x 8192: 785 to 807 us; the library's large product: 1.55 to 1.6 by rows), with the matrix
+// cores busy 66 to 80 % of the time, LDS a third of it, at 1.5 to 1.7 GHz (the library's: 86 to 90 %, half of it, 1.66 GHz): neither power
+// nor LDS is short, what the loop waits for has not been found.  What follows a tile is not hidden: all workgroups store at once (8192 x
+// 1024 -> 4096: 66 us, 78 with a gelu, 85 with z too, on the same operands again and again; 76, 82 and 92 on others; 104 for the last
+// between the backward passes of a training step).  Within 2 % either way: four waves with 4 x 4 results, a third stage for P, two
 // stages of small tiles, other spans of the reads and loads; workgroups set apart in time: 3 to 10 % slower.
 using Large = product::Shape<2, 4, 4, 2, 64, 2, 1, 4, 16, 2>;
 using Narrow = product::Shape<2, 4, 3, 2, 64, 2, 1, 4, 12, 2>;

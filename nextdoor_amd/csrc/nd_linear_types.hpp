@@ -110,7 +110,8 @@ hipError_t launch_few_rows(const LinearParams& a, After after, hipStream_t strea
 
 // ---- dz = dy a'(z) of a linear map, and the sums of the rows of dz ------------------------------------------------
 
-// Workgroups of 64 columns, 8 lanes of 8 values, 32 rows at a time.  Bound by memory: 8192 x 4096, 200 MB: 42 us, 4.8 TB/s.
+// Workgroups of 64 columns, 8 lanes of 8 values, 32 rows at a time.  Bound by memory: 8192 x 4096, 200 MB: 43 us, 4.7 TB/s, and
+// 47 behind a forward pass.
 template <class T>
 __global__ __launch_bounds__(256) void slope_kernel(LinearParams a, const void* dout, int64_t dout_bytes, float* sums, T* total_out, int64_t rows_per_share, float* parts) {
   __shared__ float part[32][kSlopeColumns + 4];

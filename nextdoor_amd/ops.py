@@ -718,7 +718,8 @@ def mlp_forward(x, up, down, up_bias=None, down_bias=None, activation="silu", ga
 
     z = x up^T + up_bias; gated: ``h = activation(g) u`` with ``g, u = z.chunk(2, -1)``, else ``h = activation(z)``.  x: [..., dim];
     up: [2 inner or inner, dim]; down: [out_dim, inner]; activations, types and sizes as in :func:`linear_forward`.  Both
-    projections, the activation and the product are one kernel; h is rounded to 16 bits before the second."""
+    projections, the activation and the product are one kernel (and one more where few rows share out the sums); h is rounded to 16 bits
+    before the second, which makes an infinity of what is 65520 or more in float16."""
     index = _on_gpu("mlp", x, up, down, *(t for t in (up_bias, down_bias, residual) if t is not None))
     _types("mlp", x, up, down, up_bias, down_bias, residual)
     gated = bool(gated)
