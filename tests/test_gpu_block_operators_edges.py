@@ -48,8 +48,10 @@ def test_gradients_of_z_far_above_dout():
     assert got["dup_bias"].tolist() == [4096.0] * 16
 
 
-# both shapes of tile that a backward pass takes two products with in one launch, and all three that it takes alone
-HELD = [(5, 64, 256, 64), (300, 96, 136, 200), (2050, 64, 256, 64), (20483, 64, 256, 64), (4104, 64, 4096, 1000), (6400, 136, 448, 152)]
+# Both shapes of tile that a backward pass takes two products with in one launch, and the third, that it takes alone; the first two are
+# alone where ddown is not wanted.
+HELD = [(5, 64, 256, 64), (300, 96, 136, 200), (2050, 64, 256, 64), (20483, 64, 256, 64), (4104, 64, 4096, 1000), (6400, 136, 448, 152),
+        (8000, 64, 2048, 1000)]
 
 
 @pytest.mark.parametrize("rows,dim,inner,out", HELD)
@@ -72,6 +74,11 @@ def test_rows_with_gradients_of_z_that_leave_the_range(rows, dim, inner, out, ga
     got = run_mlp(*case)
     for n, t in got.items():
         assert within(t, want[n], off[n]), n
+    x, up, down, up_bias, down_bias, _, _, r, d = case
+    _, z, h = ops.mlp_forward(x, up, down, up_bias, down_bias, name, gated, r, keep=True)
+    alone = dict(zip(NAMES, ops.mlp_backward(d, x, up, down, z, None, name, gated, True, False, (True, True, False))))
+    for n in ("dx", "dup", "dup_bias"):
+        assert within(alone[n], want[n], off[n]), ("alone", n)
 
 
 @pytest.mark.parametrize("rows", [40, 700, 5000])
